@@ -76,6 +76,17 @@ SIGNATURES = {
     "actkv_decode_workspace_bytes": (SZ, [I32, I32, I32, I32, I64]),
     "actkv_decode_attention": (I32, [P, I32, I64, I64, P, I64, I64, I64, I64, P, I64, P, P, I64, I64, P, I64,
                                      I32, I32, I32, I32, I32, I32, I32, F, P, SZ, P, P]),
+    "actkv_chunk_workspace_bytes": (SZ, []),
+    "actkv_chunk_attention": (I32, [P, I32, I64, I64, P, I32, P, I64, I64, I64, I64, P, I64, P, P, I64, I64, P, I64,
+                                    I32, I32, I32, I32, I32, I32, I32, F, I32, P, SZ, P, P]),
+    "actkv_chunk_attention_quant": (I32, [P, I32, I64, I64, P, I32, P, I64, I64, I64, P, I64, P, P, I64, I64, P, I64,
+                                          I32, I32, I32, I32, I32, I32, I32, F, I32, P, SZ, P, P]),
+    "actkv_quantize_write": (I32, [P, P, I32, I64, I64, I64, I64, I64, I64, P, I32, P, I64, I64, I64, I64, P, I64, P,
+                                   I32, I32, I32, I32, I32, I32, I32, P, P]),
+    "actkv_dequantize_read": (I32, [P, P, I32, I64, I64, I64, I64, I64, I64, P, I32, P, I64, I64, I64, I64, P, I64, P,
+                                    I32, I32, I32, I32, I32, I32, I32, P, P]),
+    "actkv_quant_append": (I32, [P, P, I32, I64, I64, I64, I64, I64, I64, P, I32, P, I64, I64, I64, I64, P, I64, P, P,
+                                 P, I64, I32, I32, I32, I32, I32, I32, I32, P, SZ, P, P]),
 }
 
 _lib = None

@@ -212,6 +212,8 @@ __global__ void release_push_kernel(int32_t* seq_used, int32_t* block_table, int
 
 }  // namespace
 
+const int32_t* append_ok_flags(void* workspace, int R) { return carve_blocks(workspace, R).ok; }
+
 size_t blocks_workspace_bytes(int R) { return align256(size_t(R > 0 ? R : 1) * 4 * 4 + 16); }
 
 cudaError_t launch_append(char* kv, int L, int64_t plane_stride, int64_t slot_stride, int64_t row_bytes,

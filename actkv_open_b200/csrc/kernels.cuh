@@ -301,6 +301,56 @@ bool decode_tc_supported(const DecodeArgs& a, int dtype);
 int decode_tc_splits(int R, int Hkv, int64_t max_seq, int n_sm);
 cudaError_t launch_decode_tc(const DecodeArgs& a, int dtype, cudaStream_t st, const char** why);
 
+// ---------------------------------------------------------------- chunk attention (chunk_umma.cu, chunk_simt.cu)
+struct ChunkArgs {
+  const void* q;             // [T][Hq][D], D contiguous
+  int64_t q_stride_t, q_stride_h;
+  const int32_t* q_off;      // [R + 1] packed offsets of the sessions' queries
+  const void* kv;            // one layer: [2][NB][BS][Hkv][D], or the 8-bit rows [2][NB][BS][row]
+  int64_t kv_stride_kv, kv_stride_b, kv_stride_s, kv_stride_h;   // 8-bit rows: in bytes, no stride_h
+  const int32_t* block_table;
+  int64_t bt_stride_r;
+  const int32_t* seq_used;
+  void* out;                 // [T][Hq][D] of q's dtype
+  int64_t out_stride_t, out_stride_h;
+  float* lse;                // [T][Hq]
+  int64_t lse_stride_t;
+  int T, R, MB, NB, BS, Hq, Hkv, G, D;
+  bool quant;
+  float scale;
+  void* workspace;           // chunk_workspace_bytes()
+  int32_t* status;
+};
+
+size_t chunk_workspace_bytes(int n_sm);
+bool chunk_umma_supported(const ChunkArgs& a, int dtype, const char** why);
+cudaError_t launch_chunk_umma(const ChunkArgs& a, int dtype, cudaStream_t st, const char** why);
+cudaError_t launch_chunk_simt(const ChunkArgs& a, int dtype, cudaStream_t st);
+
+// ---------------------------------------------------------------- 8-bit cache rows (quant_cache.cu)
+struct QuantMoveArgs {
+  void *k, *v;               // the 16- / 32-bit rows [L][T][Hkv][D], D contiguous (read or written)
+  int64_t ext_stride_l[2], ext_stride_t[2], ext_stride_h[2];     // of k and of v
+  uint8_t* rows;             // [L][2][NB][BS][row]
+  int64_t rows_stride_l, rows_stride_kv, rows_stride_b, rows_stride_s;
+  const int32_t* tok_off;    // [R + 1]; session r's last tok_off[r + 1] - tok_off[r] tokens
+  const int32_t* block_table;
+  int64_t bt_stride_r;
+  const int32_t* seq_used;
+  const int32_t* ok;         // nullable: sessions with ok[r] == 0 are left alone
+  int T, R, MB, NB, BS, Hkv, D;
+  int planes;                // planes moved per token: 2 L, or L when one of k, v is left out
+  int both, only;            // both planes, or plane `only` (0: K, 1: V)
+  bool vec, vec_rows;        // 16-byte accesses allowed on k / v, on the payload
+  int32_t* status;
+};
+
+cudaError_t launch_quant_write(const QuantMoveArgs& a, int dtype, cudaStream_t st);
+cudaError_t launch_quant_read(const QuantMoveArgs& a, int dtype, cudaStream_t st);
+
+// Which sessions the last launch_append over this workspace appended ([R] flags).
+const int32_t* append_ok_flags(void* workspace, int R);
+
 // ---------------------------------------------------------------- failure-path self-test (selftest.cu)
 cudaError_t launch_bounded_wait_probe(int32_t* status, long long* waited, cudaStream_t st);
 cudaError_t launch_kv_gather(const void* kv, int64_t n_blocks, int BS, int row_bytes, int head_bytes, int mode,

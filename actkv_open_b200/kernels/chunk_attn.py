@@ -1,0 +1,78 @@
+"""Attention of each session's newest tokens over a paged KV cache, with its log-sum-exp: the step
+before scoring in an agent loop (the reference leaves it to its attention backend and takes the lse,
+actkv/kernels/lse_attn.py:42-60).
+
+A session's chunk (an observation, a drafted run, a prompt piece, or a single token) is appended to
+the cache first; its queries then attend over everything the session holds, causally within the
+chunk.  bf16 / fp16 caches with head_dim 64 or 128 run on the tensor cores, the rest on CUDA cores.
+"""
+from __future__ import annotations
+
+import torch
+
+from .. import _native as N
+
+_PATHS = {"auto": N.PATH_AUTO, "simt": N.PATH_SIMT, "tcgen05": N.PATH_TCGEN05}
+_ws_bytes = {}
+
+
+def chunk_workspace(device) -> torch.Tensor:
+    """The workspace of the chunk attention calls on ``device``: any sizes, kept from call to call;
+    calls that may overlap on the GPU (other streams) need one each."""
+    dev = torch.device(device)
+    idx = dev.index if dev.index is not None else torch.cuda.current_device()
+    if idx not in _ws_bytes:
+        with torch.cuda.device(idx):
+            _ws_bytes[idx] = int(N.load().actkv_chunk_workspace_bytes())
+    return N.workspace(_ws_bytes[idx], torch.device("cuda", idx))
+
+
+def _check(q, q_off, cache, block_table, seq_used, out, lse, workspace):
+    """Checks shared by the two caches; returns (device, out, lse, workspace)."""
+    dev = N.require_cuda(q, q_off, cache, block_table, seq_used, out, lse, workspace)
+    assert q.dim() == 3, "q is [T, Hq, D]"
+    assert q.stride(2) == 1 and block_table.stride(1) == 1
+    assert q_off.dtype == torch.int32 and seq_used.dtype == torch.int32 and block_table.dtype == torch.int32
+    assert q_off.is_contiguous() and seq_used.is_contiguous()
+    r_n = seq_used.shape[0]
+    assert q_off.shape[0] == r_n + 1 and block_table.shape[0] == r_n, "q_off [R + 1], block_table [R, MB], seq_used [R]"
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    if lse is None:
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev)
+    assert out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1
+    assert lse.shape == q.shape[:2] and lse.dtype == torch.float32 and lse.stride(1) == 1
+    if workspace is None:
+        workspace = chunk_workspace(dev)
+    return dev, out, lse, workspace
+
+
+def paged_chunk_attention(q, q_off, kv, block_table, seq_used, scale=None, out=None, lse=None, workspace=None,
+                          path: str = "auto"):
+    """Attention of every session's newest tokens over its paged cache: (out [T, Hq, D] of q's dtype,
+    lse [T, Hq] fp32).
+
+    q [T, Hq, D] holds the sessions' queries packed, session r owning rows q_off[r]:q_off[r+1]
+    (int32 [R+1], T = q_off[R]); kv [2, NB, BS, Hkv, D] is one layer's cache, of q's dtype;
+    block_table [R, MB] and seq_used [R] int32.  The queries belong to the newest
+    A = q_off[r+1] - q_off[r] of the seq_used[r] tokens, already in the cache: query j sees the
+    first seq_used[r] - A + j + 1 of them.  A query that sees none gets out 0, lse -inf; a session
+    may have no queries.  ``scale`` defaults to D ** -0.5; ``workspace`` to a new
+    ``chunk_workspace`` (a loop keeps one).  ``path``: "auto", or "tcgen05" / "simt" to force the
+    tensor cores (NotImplementedError where they do not apply) or the CUDA cores.
+    """
+    dev, out, lse, workspace = _check(q, q_off, kv, block_table, seq_used, out, lse, workspace)
+    t_n, hq, d = q.shape
+    assert kv.dim() == 5 and kv.shape[0] == 2 and kv.shape[4] == d, "kv is [2, NB, BS, Hkv, D]"
+    assert kv.dtype == q.dtype, "q and the cache must share a dtype"
+    _, nb, bs, hkv, _ = kv.shape
+    assert hq % hkv == 0
+    s_kv, s_b, s_s, s_h, s_d = kv.stride()
+    assert s_d == 1
+    N.check(N.load().actkv_chunk_attention(
+        q.data_ptr(), N.dtype_code(q), q.stride(0), q.stride(1), q_off.data_ptr(), t_n, kv.data_ptr(), s_kv, s_b, s_s,
+        s_h, block_table.data_ptr(), block_table.stride(0), seq_used.data_ptr(), out.data_ptr(), out.stride(0),
+        out.stride(1), lse.data_ptr(), lse.stride(0), seq_used.shape[0], block_table.shape[1], nb, bs, hq, hkv, d,
+        d ** -0.5 if scale is None else float(scale), _PATHS[path], workspace.data_ptr(), workspace.numel(),
+        N.status_word(dev).data_ptr(), N.stream_ptr(dev)), "paged_chunk_attention")
+    return out, lse

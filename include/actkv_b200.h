@@ -448,6 +448,88 @@ ACTKV_API int actkv_decode_attention(const void* q, int dtype, int64_t q_stride_
                                      int32_t* status, void* stream);
 
 /*
+ * Attention of a chunk of new tokens over the paged cache, with its lse, one layer (no counterpart
+ * in the reference, whose attention backend is outside it; a chunk of one token is decode
+ * attention, actkv/kernels/lse_attn.py:42-60).  Session r owns the queries q_off[r]..q_off[r+1]
+ * of q [T][Hq][D] (T = q_off[R]); they belong to the newest A = q_off[r+1] - q_off[r] of its
+ * seq_used[r] tokens, which the cache already holds, so query j sees the first
+ * seq_used[r] - A + j + 1 tokens:
+ *   out[t, hq, :] = softmax(scale * q . k) @ v,  lse[t, hq] = log sum exp(scale * q . k)
+ * (out 0 and lse -inf for a query that sees no token).  Sessions may have no queries.  Tokens a
+ * query does not see do not reach its results, whatever they hold.
+ * q, out and the cache kv [2][NB][BS][Hkv][D] have one dtype (element strides, D contiguous), out
+ * [T][Hq][D], lse fp32 [T][Hq]; scale > 0.
+ * path: ACTKV_PATH_AUTO takes the tensor cores (bf16 / fp16, head_dim 64 or 128, G = Hq / Hkv <= 128,
+ * a block size of 8, 16, 32, 64 or a multiple of 128, heads and slots packed, 16-byte aligned bases
+ * and strides) and CUDA cores otherwise (head_dim <= 256); ACTKV_PATH_TCGEN05 / ACTKV_PATH_SIMT
+ * force one (ACTKV_ERR_UNSUPPORTED where it does not apply).
+ * workspace: actkv_chunk_workspace_bytes() bytes, 16-byte aligned, of any contents; calls that may
+ * overlap on the GPU need one each.
+ *
+ * actkv_chunk_attention_quant: the same over the 8-bit cache rows [2][NB][BS][row_bytes] (strides in
+ * bytes), see actkv_quantize_write; the values are those the bytes stand for, rounded to q's dtype.
+ */
+ACTKV_API size_t actkv_chunk_workspace_bytes(void);
+ACTKV_API int actkv_chunk_attention(const void* q, int dtype, int64_t q_stride_t, int64_t q_stride_h,
+                                    const int32_t* q_off, int T, const void* kv, int64_t kv_stride_kv,
+                                    int64_t kv_stride_b, int64_t kv_stride_s, int64_t kv_stride_h,
+                                    const int32_t* block_table, int64_t bt_stride_r, const int32_t* seq_used,
+                                    void* out, int64_t out_stride_t, int64_t out_stride_h, float* lse,
+                                    int64_t lse_stride_t, int R, int MB, int NB, int BS, int Hq, int Hkv, int D,
+                                    float scale, int path, void* workspace, size_t workspace_bytes,
+                                    int32_t* status, void* stream);
+ACTKV_API int actkv_chunk_attention_quant(const void* q, int dtype, int64_t q_stride_t, int64_t q_stride_h,
+                                          const int32_t* q_off, int T, const uint8_t* rows,
+                                          int64_t rows_stride_kv_bytes, int64_t rows_stride_b_bytes,
+                                          int64_t rows_stride_s_bytes, const int32_t* block_table,
+                                          int64_t bt_stride_r, const int32_t* seq_used, void* out,
+                                          int64_t out_stride_t, int64_t out_stride_h, float* lse,
+                                          int64_t lse_stride_t, int R, int MB, int NB, int BS, int Hq, int Hkv,
+                                          int D, float scale, int path, void* workspace, size_t workspace_bytes,
+                                          int32_t* status, void* stream);
+
+/*
+ * The 8-bit paged cache (no counterpart in the reference).  rows [L][2][NB][BS][row_bytes]: a
+ * token's row of one plane is Hkv * D e4m3 values, then Hkv * D / 32 scale bytes (one per 32
+ * values: value = e4m3 * 2^(byte - 127); 255: NaN), then padding; head_dim a multiple of 32,
+ * row_bytes >= Hkv * (D + D / 32).  A row moves as bytes, so actkv_append / actkv_compact /
+ * actkv_release work on such a cache as on any other.
+ *
+ * actkv_quantize_write: the newest tok_off[r+1] - tok_off[r] of session r's seq_used[r] tokens get
+ *   the rows tok_off[r]..tok_off[r+1] of k_new / v_new [L][T][Hkv][D] (element strides, D
+ *   contiguous; T = tok_off[R]), quantised: per group of 32 the smallest scale with
+ *   max|x| <= 448 * scale, values rounded to nearest even; a group with a non-finite value
+ *   becomes NaN.  The tables already hold the tokens' blocks.
+ * actkv_dequantize_read: the same tokens read back into k_out / v_out (either may be NULL), rounded to dtype.
+ * actkv_quant_append: actkv_append (tables, lengths, free stack) followed by actkv_quantize_write of
+ *   the new rows, for the sessions that fit; new_off as there.
+ * Tokens that the tables do not hold set ACTKV_DEV_BAD_INDEX and are skipped.
+ */
+ACTKV_API int actkv_quantize_write(const void* k_new, const void* v_new, int dtype, int64_t k_stride_l,
+                                   int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_l, int64_t v_stride_t,
+                                   int64_t v_stride_h, const int32_t* tok_off, int T, uint8_t* rows,
+                                   int64_t rows_stride_l_bytes, int64_t rows_stride_kv_bytes,
+                                   int64_t rows_stride_b_bytes, int64_t rows_stride_s_bytes,
+                                   const int32_t* block_table, int64_t bt_stride_r, const int32_t* seq_used, int R,
+                                   int L, int MB, int NB, int BS, int Hkv, int D, int32_t* status, void* stream);
+ACTKV_API int actkv_dequantize_read(void* k_out, void* v_out, int dtype, int64_t k_stride_l, int64_t k_stride_t,
+                                    int64_t k_stride_h, int64_t v_stride_l, int64_t v_stride_t, int64_t v_stride_h,
+                                    const int32_t* tok_off, int T, const uint8_t* rows,
+                                    int64_t rows_stride_l_bytes, int64_t rows_stride_kv_bytes,
+                                    int64_t rows_stride_b_bytes, int64_t rows_stride_s_bytes,
+                                    const int32_t* block_table, int64_t bt_stride_r, const int32_t* seq_used, int R,
+                                    int L, int MB, int NB, int BS, int Hkv, int D, int32_t* status, void* stream);
+ACTKV_API int actkv_quant_append(const void* k_new, const void* v_new, int dtype, int64_t k_stride_l,
+                                 int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_l, int64_t v_stride_t,
+                                 int64_t v_stride_h, const int32_t* new_off, int T, uint8_t* rows,
+                                 int64_t rows_stride_l_bytes, int64_t rows_stride_kv_bytes,
+                                 int64_t rows_stride_b_bytes, int64_t rows_stride_s_bytes, int32_t* block_table,
+                                 int64_t bt_stride_r, int32_t* seq_used, const int32_t* free_list,
+                                 int32_t* free_top, int64_t free_capacity, int R, int L, int MB, int NB, int BS,
+                                 int Hkv, int D, void* workspace, size_t workspace_bytes, int32_t* status,
+                                 void* stream);
+
+/*
  * Self-test of the kernels' failure path (no counterpart in the reference): one block waits, with
  * the bounded mbarrier wait that every pipelined kernel here uses, on a barrier that nothing
  * completes.  The wait gives up after ~2^31 cycles (about a second), sets ACTKV_DEV_TIMEOUT in
