@@ -1,15 +1,972 @@
-// Chunk attention on the sm_100a tensor cores: not there yet, every call takes chunk_simt.cu.
+// Chunk attention over the paged cache on the sm_100a tensor cores (tcgen05 + TMA + TMEM): the newest
+// A of a session's S tokens are the queries, query j sees tokens t <= S - A + j, and the call gives
+// out = softmax(scale q.k) v and lse = log sum exp(scale q.k) of every (query, head) row.
+//
+// With c = scale * log2 e and a reference exponent m per row, p_t = 2^(c q.k_t - m), l = sum p_t,
+// O = sum p_t v_t, out = O / l, lse = (m + log2 l) ln 2.  m need not be the running maximum, only
+// near it: it is raised (and O and l rescaled) when the maximum has grown by more than 2^8, so p
+// stays below 2^8 and the rescaling, a pass over O, is rare.  S = Q K^T and O are accumulated in 32
+// bits in TMEM, m and l are 32-bit registers; p is rounded to the cache's 16-bit type for the second
+// product only (l sums the unrounded values), the same half unit that the output is rounded by.
+//
+// Work.  A unit is (session, KV head, group of up to 256 query rows): rows are (token, head of the
+// GQA group), two tiles of 128.  The units' key tiles of 128 tokens, laid end to end with a fixed
+// cost per unit, are cut into one equal share per CTA (one CTA per SM), so ragged batches, one long
+// session and many short ones balance alike; a unit that a cut divides leaves 32-bit partial
+// results (m, l, O) in the workspace, at most two per CTA, which chunk_combine_kernel joins in a
+// fixed order.
+//
+// Two streams of (S, p, O) run in a CTA, each with its own softmax warpgroup and 256 TMEM columns:
+//   two row tiles   both streams take every key tile (one copy of K and V serves 256 rows)
+//   one row tile    (few new tokens) stream w takes every second key tile with the same queries,
+//                   and the first warpgroup joins the two at the end
+// While one stream's softmax runs, the tensor core works on the other's products.
+//
+// Warp roles (384 threads): warp 0 TMA (a paged block per lane and tile: one 5-D box of 8-token
+// groups x both D-halves; 4 KB boxes, since the copy engine spends ~60 cycles per box whatever its
+// size), warp 1 MMA issue (p from TMEM as the A operand, V as an MN-major B operand straight from
+// the tile), warps 4-7 and 8-11 softmax (a thread per row).  Every wait is bounded
+// (umma_common.cuh).
+#include <cuda.h>
+
+#include "common.cuh"
 #include "kernels.cuh"
+#include "umma_common.cuh"
 
 namespace actkv {
+namespace chunk {
 
-size_t chunk_workspace_bytes(int) { return 256; }
+using namespace umma;
 
-bool chunk_umma_supported(const ChunkArgs&, int, const char** why) {
-  *why = "not built";
-  return false;
+constexpr int kThreads = 384;
+constexpr int kRows = 128;                  // query rows per tile (MMA M)
+constexpr int kTile = 128;                  // tokens per key tile
+constexpr int kUnitCost = 2;                // a unit's fixed cost (queries in, results out) in key tiles
+constexpr float kSlack = 8.0f;              // log2 units the maximum may outgrow m by
+constexpr int kMaxD = 128;
+
+template <int D>
+struct Layout {
+  static constexpr int kHalves = D / 64;
+  static constexpr uint32_t kTileBytes = kTile * D * 2;      // a K, V or Q tile
+  static constexpr int kSlots = D == 128 ? 5 : 10;
+  static constexpr uint32_t kGroupBytes = kHalves * 1024;    // 8 tokens of a K / V tile
+  static constexpr uint32_t kKvOff = 2 * kTileBytes;
+  static constexpr uint32_t kMlOff = kKvOff + kSlots * kTileBytes;       // stream 1's (m, l) per row
+  static constexpr uint32_t kBarOff = kMlOff + kRows * 8;
+  // kv_full[slots] kv_empty[slots] q_full q_empty s_full[2] p_full[2] o_full[2] o_empty[2] x_full
+  static constexpr int kNumBars = 2 * kSlots + 11;
+  static constexpr uint32_t kSchedOff = kBarOff + kNumBars * 8;
+  static constexpr uint32_t kSmemBytes = kSchedOff + 512;
+  static_assert(kSmemBytes <= 232448, "exceeds the 227 KB of shared memory a CTA can have");
+};
+
+// TMEM columns: S (and p over it) of stream w at 128 w, O of stream w at 256 + 128 w.
+constexpr uint32_t kSCol = 0, kOCol = 256;
+
+// ------------------------------------------------------------------------------------ the schedule
+struct Unit {
+  int r, h, j0, ntok;        // session, KV head, first query token of the group, tokens in it
+  int S, A, a0;
+  int nt, t0, t1;            // key tiles of the unit, and this CTA's part of them
+  int64_t end;               // the unit's end in the schedule
+  bool two;                  // two row tiles
+};
+
+struct Desc {                // the unit that a CTA began and left to the next ones
+  int32_t valid, r, h, j0, ntok, S, A, a0;
+  int64_t end, total;
+  int32_t two, pad[3];
+};
+static_assert(sizeof(Desc) == 64, "the partial results after the descriptors are 16-byte aligned");
+
+struct Sched {               // in shared memory
+  int64_t total, pre;        // all weight, weight before session r0
+  int r0;
+  uint32_t tmem;
+  int abort_flag;
+  int bad_v;                 // a value that some row of the unit does not see is not finite
+  int64_t scan[12];
+};
+
+struct Geometry {
+  int tpb;                   // tokens per row tile
+  __device__ explicit Geometry(const ChunkArgs& a) : tpb(kRows / a.G) {}
+  __device__ int groups(int A) const { return (A + 2 * tpb - 1) / (2 * tpb); }
+  // key tiles that some query of tokens [j0, j0 + n) sees
+  __device__ int tiles(int S, int A, int j_end) const {
+    const int last = S - A + j_end - 1;
+    return last >= 0 ? last / kTile + 1 : 0;
+  }
+  __device__ int64_t head_weight(int S, int A) const {
+    int64_t w = 0;
+    for (int j = 0; j < A; j += 2 * tpb) w += kUnitCost + tiles(S, A, min(A, j + 2 * tpb));
+    return w;
+  }
+};
+
+// Walks the units that overlap this CTA's share [lo, hi) of the schedule: sessions in order, KV heads,
+// then row groups.  Every thread walks the same sequence.
+struct Walker {
+  const ChunkArgs* a;
+  Geometry geo;
+  int64_t lo, hi, at;
+  int r, h, j, S, A, a0;
+
+  __device__ void load() {
+    while (r < a->R) {
+      a0 = a->q_off[r];
+      A = a->q_off[r + 1] - a0;
+      S = a->seq_used[r];
+      if (A > 0) return;
+      ++r;
+    }
+  }
+  __device__ Walker(const ChunkArgs* args, const Sched& s, int cta, int n) : a(args), geo(*args) {
+    lo = s.total * cta / n;
+    hi = s.total * (cta + 1) / n;
+    r = s.r0;
+    h = j = S = A = a0 = 0;
+    at = s.pre;
+    if (lo >= hi) {
+      at = hi;
+      return;
+    }
+    load();
+    const int64_t w = geo.head_weight(S, A);
+    h = int((lo - at) / w);
+    at += h * w;
+    while (true) {                            // the group that holds lo
+      const int64_t x = kUnitCost + geo.tiles(S, A, min(A, j + 2 * geo.tpb));
+      if (lo < at + x) break;
+      at += x;
+      j += 2 * geo.tpb;
+    }
+  }
+  __device__ bool next(Unit& x) {
+    while (at < hi && r < a->R) {
+      x.r = r;
+      x.h = h;
+      x.j0 = j;
+      x.ntok = min(2 * geo.tpb, A - j);
+      x.S = S;
+      x.A = A;
+      x.a0 = a0;
+      x.nt = geo.tiles(S, A, j + x.ntok);
+      x.two = x.ntok > geo.tpb;
+      const int64_t start = at, first = at + kUnitCost;
+      at = x.end = first + x.nt;
+      j += 2 * geo.tpb;
+      if (j >= A) {
+        j = 0;
+        if (++h == a->Hkv) {
+          h = 0;
+          ++r;
+          load();
+        }
+      }
+      x.t0 = int(lo > first ? lo - first : 0);
+      x.t1 = x.nt == 0 ? 0 : int(min(int64_t(x.nt), hi - first));
+      if (x.nt == 0 ? start >= lo : x.t0 < x.t1) return true;
+    }
+    return false;
+  }
+};
+
+// Total weight, and the session that holds this CTA's first unit of weight.
+__device__ void make_schedule(const ChunkArgs& a, Sched& s, int cta, int n) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Geometry geo(a);
+  // pass 0 adds the weights up, pass 1 finds the session (only when a pass over all does not fit)
+  int64_t lo = 0;
+  for (int pass = 0; pass < 2; ++pass) {
+    int64_t carry = 0;
+    for (int base = 0; base < a.R; base += kThreads) {
+      const int r = base + int(threadIdx.x);
+      int64_t w = 0;
+      if (r < a.R) {
+        const int A = a.q_off[r + 1] - a.q_off[r];
+        if (A > 0) w = a.Hkv * geo.head_weight(a.seq_used[r], A);
+      }
+      int64_t incl = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+      }
+      if (lane == 31) s.scan[warp] = incl;
+      __syncthreads();
+      int64_t before = carry, all = carry;
+      for (int i = 0; i < kThreads / 32; ++i) {
+        if (i < warp) before += s.scan[i];
+        all += s.scan[i];
+      }
+      __syncthreads();
+      if (pass == 0 && base + kThreads >= a.R) {            // the last step: the total is known
+        if (threadIdx.x == 0) s.total = all;
+        lo = all * cta / n;
+      }
+      const int64_t excl = before + incl - w;
+      if ((pass == 1 || a.R <= kThreads) && w > 0 && lo >= excl && lo < excl + w) {
+        s.r0 = r;
+        s.pre = excl;
+      }
+      carry = all;
+    }
+    if (a.R <= kThreads) break;
+  }
+  __syncthreads();
 }
 
-cudaError_t launch_chunk_umma(const ChunkArgs&, int, cudaStream_t, const char**) { return cudaErrorNotSupported; }
+// ------------------------------------------------------------------------------------ operands
+__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+  uint64_t d = uint64_t((addr >> 4) & 0x3FFFu);
+  d |= uint64_t(lbo >> 4) << 16;
+  d |= uint64_t(sbo >> 4) << 32;
+  d |= uint64_t(1) << 46;
+  d |= uint64_t(2) << 61;                     // 128-byte swizzle
+  return d;
+}
+
+__device__ __forceinline__ void mma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2,
+                                            int c3, int c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* u) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(u[0]), "r"(u[1]), "r"(u[2]),
+      "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]), "r"(u[10]), "r"(u[11]), "r"(u[12]),
+      "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]), "r"(u[19]), "r"(u[20]), "r"(u[21]),
+      "r"(u[22]), "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]), "r"(u[28]), "r"(u[29]), "r"(u[30]),
+      "r"(u[31]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if constexpr (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Ring position, within a unit of nt key tiles of which `lead` keys go ahead of the values, of the
+// values of tile t: keys 0 .. lead - 1, then values t and keys t + lead in turn.
+__device__ __forceinline__ int v_position(int t, int nt, int lead) {
+  return min(lead, nt) + t + min(t, max(0, nt - lead));
+}
+__device__ __forceinline__ int k_position(int t, int lead) { return t < lead ? t : 2 * t - lead + 1; }
+
+// Part `slot` (0: a unit begun by an earlier CTA, 1: one left to the next) of CTA `cta`'s partial
+// results: rows of D values, then (m, l) per row.
+constexpr int64_t kPartFloats = int64_t(2 * kRows) * (kMaxD + 2);
+__device__ __forceinline__ float* part_of(void* ws, int n_cta, int cta, int slot) {
+  return reinterpret_cast<float*>(static_cast<char*>(ws) + int64_t(n_cta) * sizeof(Desc)) +
+         (int64_t(cta) * 2 + slot) * kPartFloats;
+}
+
+template <int D, bool BF16>
+__device__ __forceinline__ void store_row(uint16_t* dst, const float (&o)[32], float inv, bool vec) {
+  uint32_t u[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) u[i] = pack2<BF16>(o[2 * i] * inv, o[2 * i + 1] * inv);
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      reinterpret_cast<uint4*>(dst)[i] = make_uint4(u[4 * i], u[4 * i + 1], u[4 * i + 2], u[4 * i + 3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      dst[2 * i] = uint16_t(u[i]);
+      dst[2 * i + 1] = uint16_t(u[i] >> 16);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------ the kernel
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1)
+    chunk_umma_kernel(const __grid_constant__ CUtensorMap tmap_kv, const __grid_constant__ CUtensorMap tmap_q,
+                      const __grid_constant__ ChunkArgs a, bool vec_out) {
+  using Ly = Layout<D>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t base = smem_u32(smem);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Ly::kBarOff);
+  Sched& sched = *reinterpret_cast<Sched*>(smem + Ly::kSchedOff);
+  volatile int* abort_flag = &sched.abort_flag;
+  volatile int* bad_v = &sched.bad_v;
+  auto bar = [&](int i) { return smem_u32(&bars[i]); };
+  constexpr int kSlots = Ly::kSlots;
+  constexpr int B_KVF = 0, B_KVE = kSlots, B_QF = 2 * kSlots, B_QE = B_QF + 1, B_SF = B_QE + 1, B_PF = B_SF + 2,
+                B_OF = B_PF + 2, B_OE = B_OF + 2, B_XF = B_OE + 2;
+  const unsigned full = 0xffffffffu;
+  const int cta = blockIdx.x, n_cta = gridDim.x;
+
+  if ((base & 1023u) != 0) {
+    if (threadIdx.x == 0) flag(a.status, ACTKV_DEV_MISALIGNED);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(bar(B_KVF + i), 1);
+      mbar_init(bar(B_KVE + i), 1);
+    }
+    mbar_init(bar(B_QF), 1);
+    mbar_init(bar(B_QE), 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(B_SF + i), 1);
+      mbar_init(bar(B_PF + i), 4);
+      mbar_init(bar(B_OF + i), 1);
+      mbar_init(bar(B_OE + i), 4);
+    }
+    mbar_init(bar(B_XF), 4);
+    sched.total = sched.pre = 0;
+    sched.r0 = a.R;
+    sched.abort_flag = 0;
+    sched.bad_v = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    Desc* dsc = static_cast<Desc*>(a.workspace) + cta;
+    dsc->valid = 0;
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sched.tmem))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_trigger();
+  __syncthreads();
+  make_schedule(a, sched, cta, n_cta);
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = sched.tmem;
+  Walker wk(&a, sched, cta, n_cta);
+  const int tpb = wk.geo.tpb;
+  Unit x;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer (whole warp)
+    if (lane == 0) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_kv)) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_q)) : "memory");
+    }
+    const int bs_box = min(a.BS, kTile);         // token rows of a box
+    const int bpt = kTile / bs_box;              // boxes per tile (<= 16: one per lane)
+    const uint32_t box_bytes = uint32_t(bs_box) * D * 2;
+    uint32_t ring = 0, q_uses = 0;
+    bool ok = true;
+    while (ok && wk.next(x)) {
+      if (x.t0 >= x.t1) continue;
+      const int lead = x.two ? 1 : 2, nt = x.t1 - x.t0;
+      // first token slot, in units of 8, of lane b's box of key tile t; -2 past the session's end
+      auto read_id = [&](int t) -> int {
+        const int tok = t * kTile + lane * bs_box;
+        if (lane >= bpt || t >= x.t1 || tok >= x.S) return -2;
+        const int lb = tok / a.BS;
+        const int phys = lb < a.MB ? a.block_table[x.r * a.bt_stride_r + lb] : -1;
+        if (phys < 0 || phys >= a.NB) {
+          flag(a.status, ACTKV_DEV_BAD_INDEX);
+          return 0;
+        }
+        return int((int64_t(phys) * a.BS + (tok - lb * a.BS)) >> 3);
+      };
+      int id0 = read_id(x.t0), id1 = read_id(x.t0 + 1), id2 = read_id(x.t0 + 2);
+      bool w = mbar_wait(bar(B_QE), (q_uses & 1u) ^ 1u, abort_flag, a.status);
+      if (!__all_sync(full, w)) break;
+      if (lane == 0) {
+        const int blocks = x.two ? 2 : 1;
+        mbar_expect_tx(bar(B_QF), uint32_t(blocks) * tpb * a.G * D * 2);
+        for (int b = 0; b < blocks; ++b)
+          for (int hf = 0; hf < Ly::kHalves; ++hf)
+            tma_load_3d(base + b * Ly::kTileBytes + hf * (kRows * 128), &tmap_q, bar(B_QF), hf * 64, x.h * a.G,
+                        x.a0 + x.j0 + b * tpb);
+      }
+      ++q_uses;
+      auto load = [&](int t, int id, int plane) -> bool {
+        const int slot = ring % kSlots;
+        const bool w2 = mbar_wait(bar(B_KVE + slot), ((ring / kSlots) & 1u) ^ 1u, abort_flag, a.status);
+        if (!__all_sync(full, w2)) return false;
+        const int n = __popc(__ballot_sync(full, id >= 0));
+        if (lane == 0) mbar_expect_tx(bar(B_KVF + slot), uint32_t(n) * box_bytes);
+        __syncwarp();
+        if (id >= 0)
+          tma_load_5d(base + Ly::kKvOff + slot * Ly::kTileBytes + lane * box_bytes, &tmap_kv, bar(B_KVF + slot), 0, 0,
+                      x.h * Ly::kHalves, id, plane);
+        ++ring;
+        return true;
+      };
+      ok = load(x.t0, id0, 0);
+      if (ok && lead == 2 && nt > 1) ok = load(x.t0 + 1, id1, 0);
+      for (int t = 0; ok && t < nt; ++t) {
+        const int id3 = read_id(x.t0 + t + 3);
+        ok = load(x.t0 + t, id0, 1);
+        if (ok && t + lead < nt) ok = load(x.t0 + t + lead, lead == 1 ? id1 : id2, 0);
+        id0 = id1;
+        id1 = id2;
+        id2 = id3;
+      }
+    }
+    if (*abort_flag && lane == 0) {
+      for (uint32_t s = 0; s < kSlots; ++s) {
+        const uint32_t uses = ring / kSlots + (s < ring % kSlots ? 1u : 0u);
+        if (uses) mbar_drain(bar(B_KVF + s), (uses - 1) & 1u);
+      }
+      if (q_uses) mbar_drain(bar(B_QF), (q_uses - 1) & 1u);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer (one thread)
+    if (lane == 0) {
+      const uint32_t idesc_s = instr_desc_mn(kRows, kTile, BF16);
+      const uint32_t idesc_o = instr_desc_mn(kRows, D, BF16) | (1u << 16);       // B (V) MN-major
+      uint32_t ring = 0, q_uses = 0;
+      uint32_t p_uses[2] = {0, 0}, o_uses[2] = {0, 0};
+      int last_bar = -1;
+      uint32_t last_par = 0;
+      bool ok = true;
+      auto kv_wait = [&](uint32_t pos) -> bool {
+        return mbar_wait(bar(B_KVF + pos % kSlots), (pos / kSlots) & 1u, abort_flag, a.status);
+      };
+      auto issue_s = [&](int w, int q_tile, uint32_t pos) {
+        fence_after();
+        const uint32_t kaddr = base + Ly::kKvOff + (pos % kSlots) * Ly::kTileBytes;
+        const uint32_t qaddr = base + q_tile * Ly::kTileBytes;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          mma_f16(tmem + kSCol + w * 128, desc(qaddr + (k >> 2) * (kRows * 128) + (k & 3) * 32, 16, 1024),
+                  desc(kaddr + (k >> 2) * 1024 + (k & 3) * 32, 16, Ly::kGroupBytes), idesc_s, k > 0);
+        mma_commit(bar(B_SF + w));
+        last_bar = B_SF + w;
+        last_par = p_uses[w] & 1u;
+      };
+      auto issue_o = [&](int w, uint32_t pos, bool first) -> bool {
+        if (!mbar_wait(bar(B_PF + w), p_uses[w] & 1u, abort_flag, a.status)) return false;
+        ++p_uses[w];
+        if (first) {
+          if (!mbar_wait(bar(B_OE + w), (o_uses[w] & 1u) ^ 1u, abort_flag, a.status)) return false;
+          ++o_uses[w];
+        }
+        fence_after();
+        const uint32_t vaddr = base + Ly::kKvOff + (pos % kSlots) * Ly::kTileBytes;
+#pragma unroll
+        for (int k = 0; k < kTile / 16; ++k)
+          mma_f16_ta(tmem + kOCol + w * 128, tmem + kSCol + w * 128 + k * 8,
+                     desc(vaddr + k * 2 * Ly::kGroupBytes, 1024, Ly::kGroupBytes), idesc_o, !first || k > 0);
+        return true;
+      };
+      auto finish_o = [&](int w) {
+        mma_commit(bar(B_OF + w));
+        last_bar = B_OF + w;
+        last_par = (o_uses[w] - 1) & 1u;
+      };
+      while (ok && wk.next(x)) {
+        if (x.t0 >= x.t1) continue;
+        const int nt = x.t1 - x.t0;
+        ok = mbar_wait(bar(B_QF), q_uses & 1u, abort_flag, a.status);
+        if (!ok) break;
+        ++q_uses;
+        if (x.two) {
+          ok = kv_wait(ring);
+          if (!ok) break;
+          issue_s(0, 0, ring);
+          issue_s(1, 1, ring);
+          mma_commit(bar(B_KVE + ring % kSlots));
+          if (nt == 1) mma_commit(bar(B_QE));
+          for (int i = 0; ok && i < nt; ++i) {
+            const uint32_t v = ring + 1 + 2 * i, k = v + 1;
+            const bool more = i + 1 < nt;
+            ok = kv_wait(v) && issue_o(0, v, i == 0);
+            if (!ok) break;
+            if (more) {
+              ok = kv_wait(k);
+              if (!ok) break;
+              issue_s(0, 0, k);
+            } else {
+              finish_o(0);
+            }
+            ok = issue_o(1, v, i == 0);
+            if (!ok) break;
+            mma_commit(bar(B_KVE + v % kSlots));
+            if (more) {
+              issue_s(1, 1, k);
+              mma_commit(bar(B_KVE + k % kSlots));
+              if (i + 2 == nt) mma_commit(bar(B_QE));
+            } else {
+              finish_o(1);
+            }
+          }
+        } else {
+          for (int t = 0; ok && t < min(2, nt); ++t) {
+            ok = kv_wait(ring + t);
+            if (!ok) break;
+            issue_s(t, 0, ring + t);
+            mma_commit(bar(B_KVE + (ring + t) % kSlots));
+            if (t + 1 == nt) mma_commit(bar(B_QE));
+          }
+          for (int t = 0; ok && t < nt; ++t) {
+            const int w = t & 1;
+            const uint32_t v = ring + v_position(t, nt, 2);
+            ok = kv_wait(v) && issue_o(w, v, t < 2);
+            if (!ok) break;
+            mma_commit(bar(B_KVE + v % kSlots));
+            if (t + 2 < nt) {
+              const uint32_t k = ring + k_position(t + 2, 2);
+              ok = kv_wait(k);
+              if (!ok) break;
+              issue_s(w, 0, k);
+              mma_commit(bar(B_KVE + k % kSlots));
+              if (t + 3 == nt) mma_commit(bar(B_QE));
+            } else {
+              finish_o(w);
+            }
+          }
+        }
+        ring += 2 * nt;
+      }
+      if (*abort_flag && last_bar >= 0) mbar_drain(bar(last_bar), last_par);
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------------ softmax and output
+    const int w = (warp - 4) >> 2;               // stream
+    const int quad = warp & 3;                   // TMEM lanes 32 quad .. + 31
+    const int row = quad * 32 + lane;
+    const uint32_t lane_addr = tmem + (uint32_t(quad * 32) << 16);
+    const uint32_t s_addr = lane_addr + kSCol + w * 128;
+    const float c2 = a.scale * kLog2e;
+    const float ninf = -__int_as_float(0x7f800000);
+    float2* ml = reinterpret_cast<float2*>(smem + Ly::kMlOff);
+    const int jr = row / a.G, g = row - jr * a.G;             // token of the tile, head of the group
+    uint32_t it = 0, ring = 0, o_uses[2] = {0, 0}, x_uses = 0;
+    bool ok = true;
+    while (ok && wk.next(x)) {
+      const int nt = max(0, x.t1 - x.t0);
+      const int lead = x.two ? 1 : 2;
+      const int n_w = x.two ? nt : (nt + 1 - w) / 2;
+      const int j = x.j0 + (x.two ? w * tpb : 0) + jr;        // query token of the chunk
+      const int live = min(tpb, x.ntok - (x.two ? w * tpb : 0)) * a.G;   // rows of this tile
+      const bool mine = row < live;
+      const int lim = x.S - x.A + j;                          // last token this row sees
+      const int lim_min = x.S - x.A + x.j0;                   // last token every row of the unit sees
+      const bool busy = quad * 32 < live;                     // some row of this warp is live
+      float m = ninf, l = 0.0f;
+      for (int i = 0; i < n_w; ++i, ++it) {
+        const int t = x.two ? i : 2 * i + w;                  // tile of this CTA's part
+        const int tok0 = (x.t0 + t) * kTile;
+        const bool wt = mbar_wait(bar(B_SF + w), it & 1u, abort_flag, a.status);
+        if (!__all_sync(full, wt)) {
+          ok = false;
+          break;
+        }
+        fence_after();
+        // The value rows of tokens past the session's end hold anything (slots never written, another
+        // session's rows): zeroed, since 0 * NaN is NaN.  Values that some row of the unit does not
+        // see must not reach it either: if one is not finite it is zeroed too, and the rows that do
+        // see it get it back at the end.
+        if (tok0 + kTile - 1 > lim_min && (!x.two || w == 0)) {
+          const uint32_t pos = ring + v_position(t, nt, lead);
+          const bool wv = mbar_wait(bar(B_KVF + pos % kSlots), (pos / kSlots) & 1u, abort_flag, a.status);
+          if (!__all_sync(full, wv)) {
+            ok = false;
+            break;
+          }
+          uint8_t* tile = smem + Ly::kKvOff + (pos % kSlots) * Ly::kTileBytes + (row >> 3) * Ly::kGroupBytes + (row & 7) * 128;
+          const bool past = tok0 + row >= x.S;
+#pragma unroll
+          for (int hf = 0; hf < Ly::kHalves; ++hf)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              uint4* p = reinterpret_cast<uint4*>(tile + hf * 1024 + c * 16);
+              if (past) {
+                *p = make_uint4(0u, 0u, 0u, 0u);
+              } else if (tok0 + row > lim_min) {
+                uint32_t u[4] = {p->x, p->y, p->z, p->w};
+                constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
+                bool bad = false;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  if ((u[e] & kExp) == kExp) {
+                    u[e] &= 0xffff0000u;
+                    bad = true;
+                  }
+                  if (((u[e] >> 16) & kExp) == kExp) {
+                    u[e] &= 0xffffu;
+                    bad = true;
+                  }
+                }
+                if (bad) {
+                  *p = make_uint4(u[0], u[1], u[2], u[3]);
+                  *bad_v = 1;
+                }
+              }
+            }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        if (busy) {
+          float v[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, v[c]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_wait(v[c]);
+          if (!__all_sync(full, tok0 + kTile - 1 <= lim)) {
+            const int n = lim - tok0;                         // columns 0 .. n are seen
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int k = 0; k < 32; ++k) v[c][k] = c * 32 + k <= n ? v[c][k] : ninf;
+          }
+          float mx[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            mx[c] = v[c][0];
+#pragma unroll
+            for (int k = 1; k < 31; k += 2) mx[c] = fmax3(mx[c], v[c][k], v[c][k + 1]);
+            mx[c] = fmaxf(mx[c], v[c][31]);
+          }
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c2;
+          const bool raise = top > m + kSlack;                // also when m is still -inf
+          if (__any_sync(full, raise)) {
+            const float mn = raise ? top : m;
+            const float al = raise ? ex2(m - mn) : 1.0f;      // 0 from m = -inf
+            m = mn;
+            l *= al;
+            if (i > 0) {
+#pragma unroll 1
+              for (int c = 0; c < D / 32; ++c) {
+                float o[32];
+                tmem_ld32(lane_addr + kOCol + w * 128 + c * 32, o);
+                tmem_wait(o);
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] *= al;
+                tmem_st32(lane_addr + kOCol + w * 128 + c * 32, reinterpret_cast<uint32_t*>(o));
+              }
+            }
+          }
+          const float off = m == ninf ? 0.0f : m;
+          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int c = 0; c < 4; c += 2) {
+            uint32_t u[32];
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              const float p0 = ex2(fmaf(v[c + (k >> 4)][2 * (k & 15)], c2, -off));
+              const float p1 = ex2(fmaf(v[c + (k >> 4)][2 * (k & 15) + 1], c2, -off));
+              sum[k & 1] += p0;
+              sum[2 + (k & 1)] += p1;
+              u[k] = pack2<BF16>(p0, p1);
+            }
+            tmem_st32(s_addr + c * 16, u);
+          }
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_wait_st();
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_PF + w));
+      }
+      if (!ok) break;
+      ring += 2 * nt;
+      // ---- the unit's results
+      const int n_o = nt == 0 ? 0 : (x.two || nt == 1 ? 1 : 2);   // accumulators this warpgroup reads
+      const bool store = x.two || w == 0;
+      const bool joined = !x.two && nt > 1;                   // stream 1 hands its half over
+      if (joined && w == 1) {
+        // its last product is done, so the first warpgroup has read the previous unit's (m, l)
+        const bool wt = mbar_wait(bar(B_OF + 1), o_uses[1] & 1u, abort_flag, a.status);
+        if (!__all_sync(full, wt)) {
+          ok = false;
+          break;
+        }
+        ml[row] = make_float2(m, l);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_XF));
+      }
+      const int w0 = x.two ? w : 0;
+      if (store) {
+        bool wt = true;
+        for (int s = 0; s < n_o; ++s)
+          wt = wt && mbar_wait(bar(B_OF + w0 + s), o_uses[w0 + s] & 1u, abort_flag, a.status);
+        if (joined) wt = wt && mbar_wait(bar(B_XF), x_uses & 1u, abort_flag, a.status);
+        if (!__all_sync(full, wt)) {
+          ok = false;
+          break;
+        }
+        fence_after();
+        float al0 = 1.0f, al1 = 0.0f;
+        if (joined) {
+          const float2 y = ml[row];
+          const float M = fmaxf(m, y.x);
+          al0 = m == ninf ? 0.0f : ex2(m - M);
+          al1 = y.x == ninf ? 0.0f : ex2(y.x - M);
+          // a row whose keys gave NaN keeps it: l is NaN then, whatever m says
+          l = (l == 0.0f ? 0.0f : l * (m == ninf ? 1.0f : al0)) + (y.y == 0.0f ? 0.0f : y.y * (y.x == ninf ? 1.0f : al1));
+          m = M;
+        }
+        const bool whole = x.t0 == 0 && x.t1 == x.nt;
+        const bool fix = *bad_v != 0;
+        const bool put = mine && j < x.A;
+        const int hq = x.h * a.G + g;
+        const int64_t qt = int64_t(x.a0) + j;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const int pr = (x.two ? w * kRows : 0) + row;
+        float* part = whole ? nullptr : part_of(a.workspace, n_cta, cta, x.t0 > 0 ? 0 : 1);
+        if (busy) {
+#pragma unroll 1
+          for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            if (n_o == 0) {
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o[k] = 0.0f;
+            } else {
+              tmem_ld32(lane_addr + kOCol + w0 * 128 + c * 32, o);
+              tmem_wait(o);
+              if (joined) {
+                float o1[32];
+                tmem_ld32(lane_addr + kOCol + 128 + c * 32, o1);
+                tmem_wait(o1);
+                // a stream that saw nothing of this row left zeros
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] = fmaf(o[k], al0, o1[k] * al1);
+              }
+            }
+            if (fix && put) {
+              const int first = max(lim_min + 1, x.t0 * kTile), last = min(lim, x.t1 * kTile - 1);
+              for (int t = first; t <= last; ++t) {
+                const int lb = t / a.BS;
+                const int phys = lb < a.MB ? a.block_table[x.r * a.bt_stride_r + lb] : -1;
+                if (phys < 0 || phys >= a.NB) continue;
+                const uint16_t* vr = static_cast<const uint16_t*>(a.kv) + a.kv_stride_kv + int64_t(phys) * a.kv_stride_b +
+                                     int64_t(t - lb * a.BS) * a.kv_stride_s + int64_t(x.h) * a.kv_stride_h + c * 32;
+#pragma unroll
+                for (int k = 0; k < 32; ++k) {
+                  const float f = BF16 ? __uint_as_float(uint32_t(vr[k]) << 16) : __half2float(__ushort_as_half(vr[k]));
+                  if (!isfinite(f)) o[k] += f;
+                }
+              }
+            }
+            if (put) {
+              if (whole) {
+                store_row<D, BF16>(static_cast<uint16_t*>(a.out) + qt * a.out_stride_t + int64_t(hq) * a.out_stride_h + c * 32,
+                                   o, inv, vec_out);
+              } else {
+#pragma unroll
+                for (int k = 0; k < 32; k += 4)
+                  *reinterpret_cast<float4*>(part + int64_t(pr) * D + c * 32 + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+              }
+            }
+          }
+        }
+        if (put) {
+          if (whole)
+            a.lse[qt * a.lse_stride_t + hq] = l == 0.0f ? ninf : (m == ninf ? l : (m + log2f(l)) * 0.69314718055994531f);
+          else
+            *reinterpret_cast<float2*>(part + int64_t(2 * kRows) * D + 2 * pr) = make_float2(m, l);
+        }
+        if (!whole && x.t0 == 0 && row == 0 && w == 0) {
+          Desc d = {};
+          d.valid = 1;
+          d.r = x.r;
+          d.h = x.h;
+          d.j0 = x.j0;
+          d.ntok = x.ntok;
+          d.S = x.S;
+          d.A = x.A;
+          d.a0 = x.a0;
+          d.end = x.end;
+          d.total = sched.total;
+          d.two = x.two;
+          static_cast<Desc*>(a.workspace)[cta] = d;
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0)
+          for (int s = 0; s < n_o; ++s) mbar_arrive(bar(B_OE + w0 + s));
+      }
+      if (x.two) {
+        ++o_uses[0];
+        ++o_uses[1];
+      } else {
+        if (nt > 0) ++o_uses[0];
+        if (nt > 1) ++o_uses[1];
+      }
+      if (joined) ++x_uses;
+    }
+    fence_before();
+  }
+  __syncthreads();
+  if (warp == 1) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+// ------------------------------------------------------------------------------------ joining split units
+constexpr int kJoinThreads = 256;
+constexpr int kJoinSlices = 8;               // CTAs per split unit, rows dealt in turn
+
+// One CTA per (CTA that began a unit and left it, slice of its rows); a warp per row.
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kJoinThreads) chunk_combine_kernel(const __grid_constant__ ChunkArgs a, int n_cta) {
+  pdl_wait();
+  const int cta = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Desc d = static_cast<const Desc*>(a.workspace)[cta];
+  if (!d.valid) return;
+  const float ninf = -__int_as_float(0x7f800000);
+  int last = cta;                            // parts: slot 1 of cta, slot 0 of cta + 1 .. last
+  while (last + 1 < n_cta && d.total * (last + 1) / n_cta < d.end) ++last;
+  const int tpb = kRows / a.G;
+  const int live0 = min(tpb, d.ntok) * a.G, live1 = d.two ? (d.ntok - tpb) * a.G : 0;
+  for (int i = blockIdx.y * (kJoinThreads / 32) + warp; i < live0 + live1; i += kJoinSlices * (kJoinThreads / 32)) {
+    const int b = i < live0 ? 0 : 1;
+    const int row = i - b * live0;
+    const int pr = b * kRows + row;
+    const int jr = row / a.G, hq = d.h * a.G + row - jr * a.G;
+    const int64_t qt = int64_t(d.a0) + d.j0 + b * tpb + jr;
+    auto ml_of = [&](int c) {
+      return *reinterpret_cast<const float2*>(part_of(a.workspace, n_cta, c, c == cta ? 1 : 0) + int64_t(2 * kRows) * D + 2 * pr);
+    };
+    float M = ninf;
+    for (int c = cta + lane; c <= last; c += 32)
+      if (d.total * c / n_cta < d.total * (c + 1) / n_cta) M = fmaxf(M, ml_of(c).x);
+    M = warp_max(M);
+    float L = 0.0f;
+    float o[D / 32];
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) o[k] = 0.0f;
+    for (int c = cta; c <= last; ++c) {
+      if (d.total * c / n_cta >= d.total * (c + 1) / n_cta) continue;      // a CTA without a share
+      const float2 y = ml_of(c);
+      if (y.y == 0.0f) continue;             // saw none of the row's tokens
+      const float al = y.x == ninf ? 1.0f : ex2(y.x - M);
+      L += y.y * al;
+      const float* p = part_of(a.workspace, n_cta, c, c == cta ? 1 : 0) + int64_t(pr) * D;
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) o[k] = fmaf(p[k * 32 + lane], al, o[k]);
+    }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    uint16_t* dst = static_cast<uint16_t*>(a.out) + qt * a.out_stride_t + int64_t(hq) * a.out_stride_h;
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) dst[k * 32 + lane] = uint16_t(pack2<BF16>(o[k] * inv, 0.0f));
+    if (lane == 0)
+      a.lse[qt * a.lse_stride_t + hq] = L == 0.0f ? ninf : (M == ninf ? L : (M + log2f(L)) * 0.69314718055994531f);
+  }
+}
+
+}  // namespace chunk
+
+// ------------------------------------------------------------------------------------ host side
+size_t chunk_workspace_bytes(int n_sm) {
+  return align256(size_t(n_sm) * (sizeof(chunk::Desc) + 2 * chunk::kPartFloats * sizeof(float)));
+}
+
+bool chunk_umma_supported(const ChunkArgs& a, int dtype, const char** why) {
+  auto no = [&](const char* w) {
+    *why = w;
+    return false;
+  };
+  if (a.quant) return no("the 8-bit cache runs on CUDA cores");
+  if (dtype != ACTKV_BF16 && dtype != ACTKV_F16) return no("needs bf16 or fp16");
+  if (a.D != 64 && a.D != 128) return no("needs head_dim 64 or 128");
+  if (a.G > chunk::kRows) return no("needs a GQA group of at most 128");
+  if (!((a.BS % 8 == 0 && chunk::kTile % a.BS == 0) || a.BS % chunk::kTile == 0))
+    return no("needs a block size of 8, 16, 32, 64 or a multiple of 128");
+  if (a.kv_stride_h != a.D || a.kv_stride_b != int64_t(a.BS) * a.kv_stride_s)
+    return no("needs heads next to one another and blocks of consecutive slots");
+  if ((reinterpret_cast<uintptr_t>(a.kv) | reinterpret_cast<uintptr_t>(a.q)) % 16) return no("q and kv must be 16-byte aligned");
+  if (a.kv_stride_s % 8 || a.kv_stride_kv % 8 || a.q_stride_h % 8 || a.q_stride_t % 8 || a.kv_stride_s < 0 ||
+      a.kv_stride_kv < 0 || a.q_stride_h < 0 || a.q_stride_t < 0)
+    return no("q and kv strides must be multiples of 16 bytes");
+  if (int64_t(a.NB) * a.BS / 8 > 0x7fffffffll) return no("too many slots");
+  return true;
+}
+
+namespace {
+
+template <int D, bool BF16>
+cudaError_t launch_chunk_t(const CUtensorMap& mkv, const CUtensorMap& mq, const ChunkArgs& a, int grid, cudaStream_t st) {
+  auto k = chunk::chunk_umma_kernel<D, BF16>;
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(chunk::Layout<D>::kSmemBytes));
+  if (e != cudaSuccess) return e;
+  const bool vec_out = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_stride_t % 8 == 0 && a.out_stride_h % 8 == 0;
+  k<<<grid, chunk::kThreads, chunk::Layout<D>::kSmemBytes, st>>>(mkv, mq, a, vec_out);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, chunk::kJoinSlices);
+  cfg.blockDim = dim3(chunk::kJoinThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, chunk::chunk_combine_kernel<D, BF16>, a, grid);
+}
+
+}  // namespace
+
+cudaError_t launch_chunk_umma(const ChunkArgs& a, int dtype, cudaStream_t st, const char** why) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (!enc) {
+    *why = "cuTensorMapEncodeTiled unavailable";
+    return cudaErrorNotSupported;
+  }
+  const CUtensorMapDataType dt = dtype == ACTKV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const cuuint32_t es[5] = {1, 1, 1, 1, 1};
+  CUtensorMap mkv, mq;
+  {
+    // (64 dims, slot within 8, D-half of a head, group of 8 slots, plane): a box leaves every 8-token
+    // group's D-halves next to one another, so the groups of a tile are evenly spaced
+    const cuuint32_t halves = cuuint32_t(a.D / 64), rows = cuuint32_t(a.BS < chunk::kTile ? a.BS : chunk::kTile);
+    const cuuint64_t row = cuuint64_t(a.kv_stride_s) * 2;
+    const cuuint64_t dims[5] = {64, 8, cuuint64_t(a.Hkv) * halves, cuuint64_t(a.NB) * a.BS / 8, 2};
+    const cuuint64_t strides[4] = {row, 128, row * 8, cuuint64_t(a.kv_stride_kv) * 2};
+    const cuuint32_t box[5] = {64, 8, halves, rows / 8, 1};
+    if (enc(&mkv, dt, 5, const_cast<void*>(a.kv), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+      *why = "cuTensorMapEncodeTiled rejected the cache layout";
+      return cudaErrorInvalidValue;
+    }
+  }
+  {
+    const cuuint64_t dims[3] = {cuuint64_t(a.D), cuuint64_t(a.Hq), cuuint64_t(a.T)};
+    const cuuint64_t strides[2] = {cuuint64_t(a.q_stride_h) * 2, cuuint64_t(a.q_stride_t) * 2};
+    const cuuint32_t box[3] = {64, cuuint32_t(a.G), cuuint32_t(chunk::kRows / a.G)};
+    if (enc(&mq, dt, 3, const_cast<void*>(a.q), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+      *why = "cuTensorMapEncodeTiled rejected the query layout";
+      return cudaErrorInvalidValue;
+    }
+  }
+  *why = "chunk attention";
+  const int grid = device_sm_count();
+  if (a.D == 128)
+    return dtype == ACTKV_BF16 ? launch_chunk_t<128, true>(mkv, mq, a, grid, st) : launch_chunk_t<128, false>(mkv, mq, a, grid, st);
+  return dtype == ACTKV_BF16 ? launch_chunk_t<64, true>(mkv, mq, a, grid, st) : launch_chunk_t<64, false>(mkv, mq, a, grid, st);
+}
 
 }  // namespace actkv

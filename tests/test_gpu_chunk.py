@@ -1,8 +1,8 @@
 """Chunk attention over a paged cache (paged_chunk_attention, paged_chunk_attention_quant) against a
 64-bit statement of the formula, on the tensor cores and on CUDA cores.
 
-The bounds.  Let u be half a unit in the last place of the output type (2^-9 bf16, 2^-12 fp16) and
-A = sum p |v| / l of an output, |out| <= A.  p is rounded to that type before it multiplies v (u A at
+The bounds.  Let u be the output type's unit roundoff (half a unit in the last place of 1.0: 2^-8 for
+bf16's 8-bit significand, 2^-11 for fp16's 11 bits) and A = sum p |v| / l of an output, |out| <= A.  p is rounded to that type before it multiplies v (u A at
 most over the sum) and the result once more (u A); products and sums are 32-bit, logits err by at most
 ~D 2^-24 sum |q k| scale and ex2 by 2^-22, well under 1e-4 relative of p for these inputs:
 |out - ref| <= (2 u + 1e-4) A.  fp16 p below 2^-14 err by 2^-25 absolutely: + S 2^-25 max|v|.  fp32
@@ -17,7 +17,7 @@ from gpu_util import assert_device_clean, need_gpu
 
 pytestmark = pytest.mark.gpu
 
-U = {torch.bfloat16: 2.0 ** -9, torch.float16: 2.0 ** -12}
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 
 
 class Case:
