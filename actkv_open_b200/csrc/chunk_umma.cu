@@ -54,8 +54,8 @@ struct Layout {
   static constexpr uint32_t kKvOff = 2 * kTileBytes;
   static constexpr uint32_t kMlOff = kKvOff + kSlots * kTileBytes;       // stream 1's (m, l) per row
   static constexpr uint32_t kBarOff = kMlOff + kRows * 8;
-  // kv_full[slots] kv_empty[slots] q_full q_empty s_full[2] p_full[2] o_full[2] o_empty[2] x_full
-  static constexpr int kNumBars = 2 * kSlots + 11;
+  // kv_full[slots] kv_empty[slots] q_full q_empty s_full[2] p_full[2][2] o_full[2] o_empty[2] x_full
+  static constexpr int kNumBars = 2 * kSlots + 13;
   static constexpr uint32_t kSchedOff = kBarOff + kNumBars * 8;
   static constexpr uint32_t kSmemBytes = kSchedOff + 512;
   static_assert(kSmemBytes <= 232448, "exceeds the 227 KB of shared memory a CTA can have");
@@ -265,6 +265,42 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* u) {
       "r"(u[31]), "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]),
+        "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* u) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(u[0]), "r"(u[1]), "r"(u[2]),
+      "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]), "r"(u[10]), "r"(u[11]), "r"(u[12]),
+      "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(taddr)
+      : "memory");
+}
+// Two 32-bit operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 template <bool BF16>
@@ -275,12 +311,31 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return r;
 }
 
+// A slot of the K / V ring and the parity of its current use.
+struct Ring {
+  uint32_t slot = 0, par = 0;
+  __device__ __forceinline__ void next(uint32_t n) {
+    const bool wrap = slot + 1 == n;
+    slot = wrap ? 0 : slot + 1;
+    par ^= uint32_t(wrap);
+  }
+};
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
 // Ring position, within a unit of nt key tiles of which `lead` keys go ahead of the values, of the
 // values of tile t: keys 0 .. lead - 1, then values t and keys t + lead in turn.
 __device__ __forceinline__ int v_position(int t, int nt, int lead) {
   return min(lead, nt) + t + min(t, max(0, nt - lead));
 }
-__device__ __forceinline__ int k_position(int t, int lead) { return t < lead ? t : 2 * t - lead + 1; }
 
 // Part `slot` (0: a unit begun by an earlier CTA, 1: one left to the next) of CTA `cta`'s partial
 // results: rows of D values, then (m, l) per row.
@@ -324,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
   constexpr int kSlots = Ly::kSlots;
   constexpr int B_KVF = 0, B_KVE = kSlots, B_QF = 2 * kSlots, B_QE = B_QF + 1, B_SF = B_QE + 1, B_PF = B_SF + 2,
-                B_OF = B_PF + 2, B_OE = B_OF + 2, B_XF = B_OE + 2;
+                B_OF = B_PF + 4, B_OE = B_OF + 2, B_XF = B_OE + 2;
   const unsigned full = 0xffffffffu;
   const int cta = blockIdx.x, n_cta = gridDim.x;
 
@@ -341,7 +396,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(bar(B_QE), 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(B_SF + i), 1);
-      mbar_init(bar(B_PF + i), 4);
+      mbar_init(bar(B_PF + 2 * i), 4);
+      mbar_init(bar(B_PF + 2 * i + 1), 4);
       mbar_init(bar(B_OF + i), 1);
       mbar_init(bar(B_OE + i), 4);
     }
@@ -371,6 +427,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tpb = wk.geo.tpb;
   Unit x;
 
+  // 384 threads of 168 registers: the softmax warps take 208 each, the others keep 88
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (whole warp)
     if (lane == 0) {
@@ -441,117 +500,131 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (q_uses) mbar_drain(bar(B_QF), (q_uses - 1) & 1u);
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA issuer (one thread)
-    if (lane == 0) {
-      const uint32_t idesc_s = instr_desc_mn(kRows, kTile, BF16);
-      const uint32_t idesc_o = instr_desc_mn(kRows, D, BF16) | (1u << 16);       // B (V) MN-major
-      uint32_t ring = 0, q_uses = 0;
-      uint32_t p_uses[2] = {0, 0}, o_uses[2] = {0, 0};
-      int last_bar = -1;
-      uint32_t last_par = 0;
-      bool ok = true;
-      auto kv_wait = [&](uint32_t pos) -> bool {
-        return mbar_wait(bar(B_KVF + pos % kSlots), (pos / kSlots) & 1u, abort_flag, a.status);
-      };
-      auto issue_s = [&](int w, int q_tile, uint32_t pos) {
-        fence_after();
-        const uint32_t kaddr = base + Ly::kKvOff + (pos % kSlots) * Ly::kTileBytes;
-        const uint32_t qaddr = base + q_tile * Ly::kTileBytes;
+    // ------------------------------------------------------------------ MMA issuer
+    // The whole warp walks the loop, so that the operand descriptors are warp-uniform values, and one
+    // elected lane issues: with a lone thread the descriptors went through vector registers and an MMA
+    // took ~90 cycles to issue, more than the 64 it runs.
+    const uint32_t idesc_s = instr_desc_mn(kRows, kTile, BF16);
+    const uint32_t idesc_o = instr_desc_mn(kRows, D, BF16) | (1u << 16);       // B (V) MN-major
+    const uint64_t q_desc = desc(base, 16, 1024), k_desc = desc(base + Ly::kKvOff, 16, Ly::kGroupBytes),
+                   v_desc = desc(base + Ly::kKvOff, 1024, Ly::kGroupBytes);
+    const uint32_t tm = __shfl_sync(full, tmem, 0);
+    const bool leader = elect_one();
+    Ring ring;
+    uint32_t q_uses = 0, p_uses[2] = {0, 0}, o_uses[2] = {0, 0};
+    int last_bar = -1;
+    uint32_t last_par = 0;
+    bool ok = true;
+    auto wait = [&](int b, uint32_t par) -> bool {
+      return __all_sync(full, mbar_wait(bar(b), par, abort_flag, a.status));
+    };
+    auto commit = [&](int b) {
+      if (leader) mma_commit(bar(b));
+    };
+    auto issue_s = [&](int w, int q_tile, uint32_t slot) {
+      fence_after();
+      if (leader) {
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
-          mma_f16(tmem + kSCol + w * 128, desc(qaddr + (k >> 2) * (kRows * 128) + (k & 3) * 32, 16, 1024),
-                  desc(kaddr + (k >> 2) * 1024 + (k & 3) * 32, 16, Ly::kGroupBytes), idesc_s, k > 0);
+          mma_f16(tm + kSCol + w * 128, q_desc + (q_tile * Ly::kTileBytes + (k >> 2) * (kRows * 128) + (k & 3) * 32) / 16,
+                  k_desc + (slot * Ly::kTileBytes + (k >> 2) * 1024 + (k & 3) * 32) / 16, idesc_s, k > 0);
         mma_commit(bar(B_SF + w));
-        last_bar = B_SF + w;
-        last_par = p_uses[w] & 1u;
-      };
-      auto issue_o = [&](int w, uint32_t pos, bool first) -> bool {
-        if (!mbar_wait(bar(B_PF + w), p_uses[w] & 1u, abort_flag, a.status)) return false;
-        ++p_uses[w];
-        if (first) {
-          if (!mbar_wait(bar(B_OE + w), (o_uses[w] & 1u) ^ 1u, abort_flag, a.status)) return false;
-          ++o_uses[w];
-        }
-        fence_after();
-        const uint32_t vaddr = base + Ly::kKvOff + (pos % kSlots) * Ly::kTileBytes;
-#pragma unroll
-        for (int k = 0; k < kTile / 16; ++k)
-          mma_f16_ta(tmem + kOCol + w * 128, tmem + kSCol + w * 128 + k * 8,
-                     desc(vaddr + k * 2 * Ly::kGroupBytes, 1024, Ly::kGroupBytes), idesc_o, !first || k > 0);
-        return true;
-      };
-      auto finish_o = [&](int w) {
-        mma_commit(bar(B_OF + w));
-        last_bar = B_OF + w;
-        last_par = (o_uses[w] - 1) & 1u;
-      };
-      while (ok && wk.next(x)) {
-        if (x.t0 >= x.t1) continue;
-        const int nt = x.t1 - x.t0;
-        ok = mbar_wait(bar(B_QF), q_uses & 1u, abort_flag, a.status);
-        if (!ok) break;
-        ++q_uses;
-        if (x.two) {
-          ok = kv_wait(ring);
-          if (!ok) break;
-          issue_s(0, 0, ring);
-          issue_s(1, 1, ring);
-          mma_commit(bar(B_KVE + ring % kSlots));
-          if (nt == 1) mma_commit(bar(B_QE));
-          for (int i = 0; ok && i < nt; ++i) {
-            const uint32_t v = ring + 1 + 2 * i, k = v + 1;
-            const bool more = i + 1 < nt;
-            ok = kv_wait(v) && issue_o(0, v, i == 0);
-            if (!ok) break;
-            if (more) {
-              ok = kv_wait(k);
-              if (!ok) break;
-              issue_s(0, 0, k);
-            } else {
-              finish_o(0);
-            }
-            ok = issue_o(1, v, i == 0);
-            if (!ok) break;
-            mma_commit(bar(B_KVE + v % kSlots));
-            if (more) {
-              issue_s(1, 1, k);
-              mma_commit(bar(B_KVE + k % kSlots));
-              if (i + 2 == nt) mma_commit(bar(B_QE));
-            } else {
-              finish_o(1);
-            }
-          }
-        } else {
-          for (int t = 0; ok && t < min(2, nt); ++t) {
-            ok = kv_wait(ring + t);
-            if (!ok) break;
-            issue_s(t, 0, ring + t);
-            mma_commit(bar(B_KVE + (ring + t) % kSlots));
-            if (t + 1 == nt) mma_commit(bar(B_QE));
-          }
-          for (int t = 0; ok && t < nt; ++t) {
-            const int w = t & 1;
-            const uint32_t v = ring + v_position(t, nt, 2);
-            ok = kv_wait(v) && issue_o(w, v, t < 2);
-            if (!ok) break;
-            mma_commit(bar(B_KVE + v % kSlots));
-            if (t + 2 < nt) {
-              const uint32_t k = ring + k_position(t + 2, 2);
-              ok = kv_wait(k);
-              if (!ok) break;
-              issue_s(w, 0, k);
-              mma_commit(bar(B_KVE + k % kSlots));
-              if (t + 3 == nt) mma_commit(bar(B_QE));
-            } else {
-              finish_o(w);
-            }
-          }
-        }
-        ring += 2 * nt;
       }
-      if (*abort_flag && last_bar >= 0) mbar_drain(bar(last_bar), last_par);
+      last_bar = B_SF + w;
+      last_par = p_uses[w] & 1u;
+    };
+    auto issue_o = [&](int w, uint32_t slot, bool first) -> bool {
+      const uint32_t par = p_uses[w] & 1u;
+      ++p_uses[w];
+      if (first) {
+        if (!wait(B_OE + w, (o_uses[w] & 1u) ^ 1u)) return false;
+        ++o_uses[w];
+      }
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        if (!wait(B_PF + 2 * w + hf, par)) return false;
+        fence_after();
+        if (leader) {
+#pragma unroll
+          for (int k = hf * (kTile / 32); k < (hf + 1) * (kTile / 32); ++k)
+            mma_f16_ta(tm + kOCol + w * 128, tm + kSCol + w * 128 + k * 8,
+                       v_desc + (slot * Ly::kTileBytes + k * 2 * Ly::kGroupBytes) / 16, idesc_o, !first || k > 0);
+        }
+      }
+      return true;
+    };
+    auto finish_o = [&](int w) {
+      commit(B_OF + w);
+      last_bar = B_OF + w;
+      last_par = (o_uses[w] - 1) & 1u;
+    };
+    auto kv_wait = [&](const Ring& r) { return wait(B_KVF + r.slot, r.par); };
+    while (ok && wk.next(x)) {
+      const int nt = __shfl_sync(full, x.t1 - x.t0, 0);
+      const bool two = __shfl_sync(full, int(x.two), 0) != 0;
+      if (nt <= 0) continue;
+      ok = wait(B_QF, q_uses & 1u);
+      if (!ok) break;
+      ++q_uses;
+      if (two) {
+        ok = kv_wait(ring);
+        if (!ok) break;
+        issue_s(0, 0, ring.slot);
+        issue_s(1, 1, ring.slot);
+        commit(B_KVE + ring.slot);
+        ring.next(kSlots);
+        if (nt == 1) commit(B_QE);
+        for (int i = 0; ok && i < nt; ++i) {
+          const Ring v = ring;
+          ring.next(kSlots);
+          const Ring k = ring;
+          const bool more = i + 1 < nt;
+          if (more) ring.next(kSlots);
+          ok = kv_wait(v) && issue_o(0, v.slot, i == 0);
+          if (!ok) break;
+          if (more) {
+            ok = kv_wait(k);
+            if (!ok) break;
+            issue_s(0, 0, k.slot);
+          } else {
+            finish_o(0);
+          }
+          ok = issue_o(1, v.slot, i == 0);
+          if (!ok) break;
+          commit(B_KVE + v.slot);
+          if (more) {
+            issue_s(1, 1, k.slot);
+            commit(B_KVE + k.slot);
+            if (i + 2 == nt) commit(B_QE);
+          } else {
+            finish_o(1);
+          }
+        }
+      } else {
+        // ring order: keys 0, 1, then values t and keys t + 2 in turn
+        auto key = [&](int t) -> bool {
+          if (!kv_wait(ring)) return false;
+          issue_s(t & 1, 0, ring.slot);
+          commit(B_KVE + ring.slot);
+          ring.next(kSlots);
+          if (t + 1 == nt) commit(B_QE);
+          return true;
+        };
+        ok = key(0) && (nt == 1 || key(1));
+        for (int t = 0; ok && t < nt; ++t) {
+          ok = kv_wait(ring) && issue_o(t & 1, ring.slot, t < 2);
+          if (!ok) break;
+          commit(B_KVE + ring.slot);
+          ring.next(kSlots);
+          if (t + 2 < nt) ok = key(t + 2);
+          else finish_o(t & 1);
+        }
+      }
     }
-  } else if (warp >= 4) {
+    if (*abort_flag && last_bar >= 0 && lane == 0) mbar_drain(bar(last_bar), last_par);
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ------------------------------------------------------------------ softmax and output
     const int w = (warp - 4) >> 2;               // stream
     const int quad = warp & 3;                   // TMEM lanes 32 quad .. + 31
@@ -628,27 +701,28 @@ __global__ void __launch_bounds__(kThreads, 1)
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         if (busy) {
-          float v[4][32];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, v[c]);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_wait(v[c]);
-          if (!__all_sync(full, tok0 + kTile - 1 <= lim)) {
-            const int n = lim - tok0;                         // columns 0 .. n are seen
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-              for (int k = 0; k < 32; ++k) v[c][k] = c * 32 + k <= n ? v[c][k] : ninf;
-          }
+          float v[2][64];
+          tmem_ld64(s_addr, v[0]);
+          tmem_ld64(s_addr + 64, v[1]);
+          tmem_wait(v[0]);
+          tmem_wait(v[1]);
+          const bool masked = !__all_sync(full, tok0 + kTile - 1 <= lim);
+          const int n_seen = lim - tok0;                      // columns 0 .. n_seen are seen
           float mx[4];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            mx[c] = v[c][0];
+          for (int hf = 0; hf < 2; ++hf) {
+            if (masked) {
 #pragma unroll
-            for (int k = 1; k < 31; k += 2) mx[c] = fmax3(mx[c], v[c][k], v[c][k + 1]);
-            mx[c] = fmaxf(mx[c], v[c][31]);
+              for (int k = 0; k < 64; ++k) v[hf][k] = hf * 64 + k <= n_seen ? v[hf][k] : ninf;
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) mx[c] = hf ? fmax3(mx[c], v[hf][c], v[hf][c + 4]) : fmaxf(v[hf][c], v[hf][c + 4]);
+#pragma unroll
+            for (int k = 8; k < 64; k += 8)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) mx[c] = fmax3(mx[c], v[hf][k + c], v[hf][k + c + 4]);
           }
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c2;
+          const float top = fmax3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * c2;
           const bool raise = top > m + kSlack;                // also when m is still -inf
           if (__any_sync(full, raise)) {
             const float mn = raise ? top : m;
@@ -657,37 +731,53 @@ __global__ void __launch_bounds__(kThreads, 1)
             l *= al;
             if (i > 0) {
 #pragma unroll 1
-              for (int c = 0; c < D / 32; ++c) {
-                float o[32];
-                tmem_ld32(lane_addr + kOCol + w * 128 + c * 32, o);
-                tmem_wait(o);
+              for (int c = 0; c < D / 16; ++c) {
+                float o[16];
+                tmem_ld16(lane_addr + kOCol + w * 128 + c * 16, o);
 #pragma unroll
-                for (int k = 0; k < 32; ++k) o[k] *= al;
-                tmem_st32(lane_addr + kOCol + w * 128 + c * 32, reinterpret_cast<uint32_t*>(o));
+                for (int k = 0; k < 16; ++k) o[k] *= al;
+                tmem_st16(lane_addr + kOCol + w * 128 + c * 16, reinterpret_cast<uint32_t*>(o));
               }
             }
           }
           const float off = m == ninf ? 0.0f : m;
-          float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          const float2 c2v = make_float2(c2, c2), offv = make_float2(-off, -off);
+          float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+          // p of 32 tokens at a time; a store is waited for after the next 32 are computed, and the
+          // second product starts on the first 64
 #pragma unroll
-          for (int c = 0; c < 4; c += 2) {
-            uint32_t u[32];
+          for (int q = 0; q < 4; ++q) {
+            uint32_t u[16];
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const float p0 = ex2(fmaf(v[c + (k >> 4)][2 * (k & 15)], c2, -off));
-              const float p1 = ex2(fmaf(v[c + (k >> 4)][2 * (k & 15) + 1], c2, -off));
-              sum[k & 1] += p0;
-              sum[2 + (k & 1)] += p1;
-              u[k] = pack2<BF16>(p0, p1);
+            for (int k = 0; k < 16; ++k) {
+              const float* vp = &v[q >> 1][(q & 1) * 32 + 2 * k];
+              const float2 e = fma2(make_float2(vp[0], vp[1]), c2v, offv);
+              const float2 p = make_float2(ex2(e.x), ex2(e.y));
+              sum[k & 1] = add2(sum[k & 1], p);
+              u[k] = pack2<BF16>(p.x, p.y);
             }
-            tmem_st32(s_addr + c * 16, u);
+            if (q == 2) {
+              tmem_wait_st();
+              fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bar(B_PF + 2 * w));
+            }
+            tmem_st16(s_addr + q * 16, u);
           }
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
           tmem_wait_st();
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(B_PF + 2 * w + 1));
+          const float2 s2 = add2(sum[0], sum[1]);
+          l += s2.x + s2.y;
+        } else {
+          fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(bar(B_PF + 2 * w));
+            mbar_arrive(bar(B_PF + 2 * w + 1));
+          }
         }
-        fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(B_PF + w));
       }
       if (!ok) break;
       ring += 2 * nt;
