@@ -39,11 +39,14 @@ namespace chunk {
 using namespace umma;
 
 constexpr int kThreads = 384;
+constexpr int kUnitSlots = 4;               // units announced ahead of their results
 constexpr int kRows = 128;                  // query rows per tile (MMA M)
 constexpr int kTile = 128;                  // tokens per key tile
 constexpr int kUnitCost = 2;                // a unit's fixed cost (queries in, results out) in key tiles
 constexpr float kSlack = 8.0f;              // log2 units the maximum may outgrow m by
 constexpr int kMaxD = 128;
+
+constexpr uint32_t kSchedBytes = 512;
 
 template <int D>
 struct Layout {
@@ -54,10 +57,11 @@ struct Layout {
   static constexpr uint32_t kKvOff = 2 * kTileBytes;
   static constexpr uint32_t kMlOff = kKvOff + kSlots * kTileBytes;       // stream 1's (m, l) per row
   static constexpr uint32_t kBarOff = kMlOff + kRows * 8;
-  // kv_full[slots] kv_empty[slots] q_full q_empty s_full[2] p_full[2][2] o_full[2] o_empty[2] x_full
-  static constexpr int kNumBars = 2 * kSlots + 13;
+  // kv_full[slots] kv_empty[slots] q_full q_empty s_full[2] p_full[2][2] o_full[2] o_empty[2]
+  // x_full unit_full[4] unit_empty[4]
+  static constexpr int kNumBars = 2 * kSlots + 13 + 2 * kUnitSlots;
   static constexpr uint32_t kSchedOff = kBarOff + kNumBars * 8;
-  static constexpr uint32_t kSmemBytes = kSchedOff + 512;
+  static constexpr uint32_t kSmemBytes = kSchedOff + kSchedBytes;
   static_assert(kSmemBytes <= 232448, "exceeds the 227 KB of shared memory a CTA can have");
 };
 
@@ -69,8 +73,8 @@ struct Unit {
   int r, h, j0, ntok;        // session, KV head, first query token of the group, tokens in it
   int S, A, a0;
   int nt, t0, t1;            // key tiles of the unit, and this CTA's part of them
+  int two;                   // two row tiles
   int64_t end;               // the unit's end in the schedule
-  bool two;                  // two row tiles
 };
 
 struct Desc {                // the unit that a CTA began and left to the next ones
@@ -86,8 +90,10 @@ struct Sched {               // in shared memory
   uint32_t tmem;
   int abort_flag;
   int bad_v;                 // a value that some row of the unit does not see is not finite
-  int64_t scan[12];
+  int64_t scan[kThreads / 32];
+  Unit units[kUnitSlots];    // from the TMA warp, which alone walks the schedule; r < 0 ends it
 };
+static_assert(sizeof(Sched) <= kSchedBytes, "the schedule's place in shared memory");
 
 struct Geometry {
   int tpb;                   // tokens per row tile
@@ -363,6 +369,39 @@ __device__ __forceinline__ void store_row(uint16_t* dst, const float (&o)[32], f
   }
 }
 
+// One token's values of a tile in shared memory: zeroed when the token is past the session's end; when
+// `hidden` (some row does not see it), what is not finite is zeroed and *bad_v set.
+template <int D, bool BF16>
+__device__ __forceinline__ void clean_values(uint8_t* tile, bool past, bool hidden, volatile int* bad_v) {
+  constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
+  if (!past && !hidden) return;
+#pragma unroll
+  for (int k = 0; k < D / 8; ++k) {
+    uint4* p = reinterpret_cast<uint4*>(tile + (k >> 3) * 1024) + (k & 7);
+    if (past) {
+      *p = make_uint4(0u, 0u, 0u, 0u);
+      continue;
+    }
+    uint32_t u[4] = {p->x, p->y, p->z, p->w};
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if ((u[e] & kExp) == kExp) {
+        u[e] &= 0xffff0000u;
+        bad = true;
+      }
+      if (((u[e] >> 16) & kExp) == kExp) {
+        u[e] &= 0xffffu;
+        bad = true;
+      }
+    }
+    if (bad) {
+      *p = make_uint4(u[0], u[1], u[2], u[3]);
+      *bad_v = 1;
+    }
+  }
+}
+
 // ------------------------------------------------------------------------------------ the kernel
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -379,7 +418,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
   constexpr int kSlots = Ly::kSlots;
   constexpr int B_KVF = 0, B_KVE = kSlots, B_QF = 2 * kSlots, B_QE = B_QF + 1, B_SF = B_QE + 1, B_PF = B_SF + 2,
-                B_OF = B_PF + 4, B_OE = B_OF + 2, B_XF = B_OE + 2;
+                B_OF = B_PF + 4, B_OE = B_OF + 2, B_XF = B_OE + 2, B_UF = B_XF + 1,
+                B_UE = B_UF + kUnitSlots;
   const unsigned full = 0xffffffffu;
   const int cta = blockIdx.x, n_cta = gridDim.x;
 
@@ -402,6 +442,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar(B_OE + i), 4);
     }
     mbar_init(bar(B_XF), 4);
+    for (int i = 0; i < kUnitSlots; ++i) {
+      mbar_init(bar(B_UF + i), 1);
+      mbar_init(bar(B_UE + i), 9);           // the MMA warp and the softmax warps
+    }
     sched.total = sched.pre = 0;
     sched.r0 = a.R;
     sched.abort_flag = 0;
@@ -423,9 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   fence_after();
   const uint32_t tmem = sched.tmem;
-  Walker wk(&a, sched, cta, n_cta);
-  const int tpb = wk.geo.tpb;
-  Unit x;
+  const int tpb = kRows / a.G;
 
   // 384 threads of 168 registers: the softmax warps take 208 each, the others keep 88
   if (warp < 4) {
@@ -439,9 +481,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int bs_box = min(a.BS, kTile);         // token rows of a box
     const int bpt = kTile / bs_box;              // boxes per tile (<= 16: one per lane)
     const uint32_t box_bytes = uint32_t(bs_box) * D * 2;
+    Walker wk(&a, sched, cta, n_cta);
+    Unit x;
     uint32_t ring = 0, q_uses = 0;
     bool ok = true;
-    while (ok && wk.next(x)) {
+    for (uint32_t n = 0;; ++n) {
+      const bool any = wk.next(x);
+      ok = __all_sync(full, mbar_wait(bar(B_UE + n % kUnitSlots), ((n / kUnitSlots) & 1u) ^ 1u, abort_flag, a.status));
+      if (!ok) break;
+      if (lane == 0) {
+        if (!any) x.r = -1;
+        sched.units[n % kUnitSlots] = x;
+        mbar_arrive(bar(B_UF + n % kUnitSlots));
+      }
+      if (!any) break;
       if (x.t0 >= x.t1) continue;
       const int lead = x.two ? 1 : 2, nt = x.t1 - x.t0;
       // first token slot, in units of 8, of lane b's box of key tile t; -2 past the session's end
@@ -457,8 +510,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         return int((int64_t(phys) * a.BS + (tok - lb * a.BS)) >> 3);
       };
       int id0 = read_id(x.t0), id1 = read_id(x.t0 + 1), id2 = read_id(x.t0 + 2);
-      bool w = mbar_wait(bar(B_QE), (q_uses & 1u) ^ 1u, abort_flag, a.status);
-      if (!__all_sync(full, w)) break;
+      ok = __all_sync(full, mbar_wait(bar(B_QE), (q_uses & 1u) ^ 1u, abort_flag, a.status));
+      if (!ok) break;
       if (lane == 0) {
         const int blocks = x.two ? 2 : 1;
         mbar_expect_tx(bar(B_QF), uint32_t(blocks) * tpb * a.G * D * 2);
@@ -491,6 +544,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         id1 = id2;
         id2 = id3;
       }
+      if (!ok) break;
     }
     if (*abort_flag && lane == 0) {
       for (uint32_t s = 0; s < kSlots; ++s) {
@@ -511,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tm = __shfl_sync(full, tmem, 0);
     const bool leader = elect_one();
     Ring ring;
-    uint32_t q_uses = 0, p_uses[2] = {0, 0}, o_uses[2] = {0, 0};
+    uint32_t q_uses = 0, p_uses[2] = {0, 0}, o_uses[2] = {0, 0};   // p_uses: tiles
     int last_bar = -1;
     uint32_t last_par = 0;
     bool ok = true;
@@ -522,7 +576,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (leader) mma_commit(bar(b));
     };
     auto issue_s = [&](int w, int q_tile, uint32_t slot) {
-      fence_after();
       if (leader) {
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
@@ -533,6 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       last_bar = B_SF + w;
       last_par = p_uses[w] & 1u;
     };
+    // p arrives in halves of 64 tokens
     auto issue_o = [&](int w, uint32_t slot, bool first) -> bool {
       const uint32_t par = p_uses[w] & 1u;
       ++p_uses[w];
@@ -541,12 +595,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++o_uses[w];
       }
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        if (!wait(B_PF + 2 * w + hf, par)) return false;
+      for (int b = 0; b < 2; ++b) {
+        if (!wait(B_PF + 2 * w + b, par)) return false;
         fence_after();
         if (leader) {
 #pragma unroll
-          for (int k = hf * (kTile / 32); k < (hf + 1) * (kTile / 32); ++k)
+          for (int k = b * (kTile / 32); k < (b + 1) * (kTile / 32); ++k)
             mma_f16_ta(tm + kOCol + w * 128, tm + kSCol + w * 128 + k * 8,
                        v_desc + (slot * Ly::kTileBytes + k * 2 * Ly::kGroupBytes) / 16, idesc_o, !first || k > 0);
         }
@@ -558,11 +612,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       last_bar = B_OF + w;
       last_par = (o_uses[w] - 1) & 1u;
     };
-    auto kv_wait = [&](const Ring& r) { return wait(B_KVF + r.slot, r.par); };
-    while (ok && wk.next(x)) {
-      const int nt = __shfl_sync(full, x.t1 - x.t0, 0);
-      const bool two = __shfl_sync(full, int(x.two), 0) != 0;
-      if (nt <= 0) continue;
+    auto kv_wait = [&](const Ring& r) {
+      const bool r_ok = wait(B_KVF + r.slot, r.par);
+      fence_after();
+      return r_ok;
+    };
+    for (uint32_t n = 0; ok; ++n) {
+      const uint32_t slot = n % kUnitSlots;
+      if (!wait(B_UF + slot, (n / kUnitSlots) & 1u)) break;
+      const volatile Unit& x = sched.units[slot];
+      const int nt = __shfl_sync(full, x.r < 0 ? -1 : x.t1 - x.t0, 0);
+      const bool two = __shfl_sync(full, x.two, 0) != 0;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(B_UE + slot));
+      if (nt < 0) break;
+      if (nt == 0) continue;
       ok = wait(B_QF, q_uses & 1u);
       if (!ok) break;
       ++q_uses;
@@ -626,80 +690,56 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ------------------------------------------------------------------ softmax and output
+    // A thread per row; p goes to the second product in two halves of 64 tokens.
     const int w = (warp - 4) >> 2;               // stream
     const int quad = warp & 3;                   // TMEM lanes 32 quad .. + 31
     const int row = quad * 32 + lane;
     const uint32_t lane_addr = tmem + (uint32_t(quad * 32) << 16);
-    const uint32_t s_addr = lane_addr + kSCol + w * 128;
+    const uint32_t s_addr = lane_addr + kSCol + w * 128, o_addr = lane_addr + kOCol + w * 128;
     const float c2 = a.scale * kLog2e;
     const float ninf = -__int_as_float(0x7f800000);
     float2* ml = reinterpret_cast<float2*>(smem + Ly::kMlOff);
     const int jr = row / a.G, g = row - jr * a.G;             // token of the tile, head of the group
     uint32_t it = 0, ring = 0, o_uses[2] = {0, 0}, x_uses = 0;
+    auto wait = [&](int b, uint32_t par) -> bool {
+      return __all_sync(full, mbar_wait(bar(b), par, abort_flag, a.status));
+    };
     bool ok = true;
-    while (ok && wk.next(x)) {
+    for (uint32_t n = 0; ok; ++n) {
+      const uint32_t slot = n % kUnitSlots;
+      if (!wait(B_UF + slot, (n / kUnitSlots) & 1u)) break;
+      const volatile Unit& x = sched.units[slot];
+      if (x.r < 0) break;
       const int nt = max(0, x.t1 - x.t0);
-      const int lead = x.two ? 1 : 2;
-      const int n_w = x.two ? nt : (nt + 1 - w) / 2;
-      const int j = x.j0 + (x.two ? w * tpb : 0) + jr;        // query token of the chunk
-      const int live = min(tpb, x.ntok - (x.two ? w * tpb : 0)) * a.G;   // rows of this tile
+      const bool two = x.two;
+      const int lead = two ? 1 : 2;
+      const int n_w = two ? nt : (nt + 1 - w) / 2;
+      const int j = x.j0 + (two ? w * tpb : 0) + jr;          // query token of the chunk
+      const int live = min(tpb, x.ntok - (two ? w * tpb : 0)) * a.G;   // rows of this tile
       const bool mine = row < live;
       const int lim = x.S - x.A + j;                          // last token this row sees
       const int lim_min = x.S - x.A + x.j0;                   // last token every row of the unit sees
       const bool busy = quad * 32 < live;                     // some row of this warp is live
+      const int t_first = x.t0;
       float m = ninf, l = 0.0f;
-      for (int i = 0; i < n_w; ++i, ++it) {
-        const int t = x.two ? i : 2 * i + w;                  // tile of this CTA's part
-        const int tok0 = (x.t0 + t) * kTile;
-        const bool wt = mbar_wait(bar(B_SF + w), it & 1u, abort_flag, a.status);
-        if (!__all_sync(full, wt)) {
-          ok = false;
-          break;
-        }
-        fence_after();
+      for (int i = 0; ok && i < n_w; ++i, ++it) {
+        const int t = two ? i : 2 * i + w;                    // tile of this CTA's part
+        const int tok0 = (t_first + t) * kTile;
+        ok = wait(B_SF + w, it & 1u);
+        if (!ok) break;
         // The value rows of tokens past the session's end hold anything (slots never written, another
         // session's rows): zeroed, since 0 * NaN is NaN.  Values that some row of the unit does not
         // see must not reach it either: if one is not finite it is zeroed too, and the rows that do
         // see it get it back at the end.
-        if (tok0 + kTile - 1 > lim_min && (!x.two || w == 0)) {
+        if (tok0 + kTile - 1 > lim_min && (!two || w == 0)) {
           const uint32_t pos = ring + v_position(t, nt, lead);
-          const bool wv = mbar_wait(bar(B_KVF + pos % kSlots), (pos / kSlots) & 1u, abort_flag, a.status);
-          if (!__all_sync(full, wv)) {
-            ok = false;
-            break;
-          }
-          uint8_t* tile = smem + Ly::kKvOff + (pos % kSlots) * Ly::kTileBytes + (row >> 3) * Ly::kGroupBytes + (row & 7) * 128;
-          const bool past = tok0 + row >= x.S;
-#pragma unroll
-          for (int hf = 0; hf < Ly::kHalves; ++hf)
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              uint4* p = reinterpret_cast<uint4*>(tile + hf * 1024 + c * 16);
-              if (past) {
-                *p = make_uint4(0u, 0u, 0u, 0u);
-              } else if (tok0 + row > lim_min) {
-                uint32_t u[4] = {p->x, p->y, p->z, p->w};
-                constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
-                bool bad = false;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  if ((u[e] & kExp) == kExp) {
-                    u[e] &= 0xffff0000u;
-                    bad = true;
-                  }
-                  if (((u[e] >> 16) & kExp) == kExp) {
-                    u[e] &= 0xffffu;
-                    bad = true;
-                  }
-                }
-                if (bad) {
-                  *p = make_uint4(u[0], u[1], u[2], u[3]);
-                  *bad_v = 1;
-                }
-              }
-            }
+          ok = wait(B_KVF + pos % kSlots, (pos / kSlots) & 1u);
+          if (!ok) break;
+          clean_values<D, BF16>(smem + Ly::kKvOff + (pos % kSlots) * Ly::kTileBytes + (row >> 3) * Ly::kGroupBytes +
+                                (row & 7) * 128, tok0 + row >= x.S, tok0 + row > lim_min, bad_v);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
+        fence_after();
         if (busy) {
           float v[2][64];
           tmem_ld64(s_addr, v[0]);
@@ -707,20 +747,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_wait(v[0]);
           tmem_wait(v[1]);
           const bool masked = !__all_sync(full, tok0 + kTile - 1 <= lim);
-          const int n_seen = lim - tok0;                      // columns 0 .. n_seen are seen
+          const int last = lim - tok0;                        // columns 0 .. last are seen
           float mx[4];
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
             if (masked) {
 #pragma unroll
-              for (int k = 0; k < 64; ++k) v[hf][k] = hf * 64 + k <= n_seen ? v[hf][k] : ninf;
+              for (int k = 0; k < 64; ++k) v[hf][k] = hf * 64 + k <= last ? v[hf][k] : ninf;
             }
 #pragma unroll
-            for (int c = 0; c < 4; ++c) mx[c] = hf ? fmax3(mx[c], v[hf][c], v[hf][c + 4]) : fmaxf(v[hf][c], v[hf][c + 4]);
+            for (int e = 0; e < 4; ++e) mx[e] = hf ? fmax3(mx[e], v[hf][e], v[hf][e + 4]) : fmaxf(v[hf][e], v[hf][e + 4]);
 #pragma unroll
             for (int k = 8; k < 64; k += 8)
 #pragma unroll
-              for (int c = 0; c < 4; ++c) mx[c] = fmax3(mx[c], v[hf][k + c], v[hf][k + c + 4]);
+              for (int e = 0; e < 4; ++e) mx[e] = fmax3(mx[e], v[hf][k + e], v[hf][k + e + 4]);
           }
           const float top = fmax3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * c2;
           const bool raise = top > m + kSlack;                // also when m is still -inf
@@ -729,14 +769,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float al = raise ? ex2(m - mn) : 1.0f;      // 0 from m = -inf
             m = mn;
             l *= al;
-            if (i > 0) {
+            if (i > 0) {                                      // O is at rest: its last product came before this S
 #pragma unroll 1
-              for (int c = 0; c < D / 16; ++c) {
+              for (int q = 0; q < D / 16; ++q) {
                 float o[16];
-                tmem_ld16(lane_addr + kOCol + w * 128 + c * 16, o);
+                tmem_ld16(o_addr + q * 16, o);
 #pragma unroll
                 for (int k = 0; k < 16; ++k) o[k] *= al;
-                tmem_st16(lane_addr + kOCol + w * 128 + c * 16, reinterpret_cast<uint32_t*>(o));
+                tmem_st16(o_addr + q * 16, reinterpret_cast<uint32_t*>(o));
               }
             }
           }
@@ -764,48 +804,35 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tmem_st16(s_addr + q * 16, u);
           }
-          tmem_wait_st();
-          fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(B_PF + 2 * w + 1));
           const float2 s2 = add2(sum[0], sum[1]);
           l += s2.x + s2.y;
-        } else {
-          fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(bar(B_PF + 2 * w));
-            mbar_arrive(bar(B_PF + 2 * w + 1));
-          }
+          tmem_wait_st();
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (!busy) mbar_arrive(bar(B_PF + 2 * w));
+          mbar_arrive(bar(B_PF + 2 * w + 1));
         }
       }
       if (!ok) break;
       ring += 2 * nt;
       // ---- the unit's results
-      const int n_o = nt == 0 ? 0 : (x.two || nt == 1 ? 1 : 2);   // accumulators this warpgroup reads
-      const bool store = x.two || w == 0;
-      const bool joined = !x.two && nt > 1;                   // stream 1 hands its half over
+      const int n_o = nt == 0 ? 0 : (two || nt == 1 ? 1 : 2);   // accumulators this warpgroup reads
+      const bool joined = !two && nt > 1;                     // stream 1 hands its half over
       if (joined && w == 1) {
         // its last product is done, so the first warpgroup has read the previous unit's (m, l)
-        const bool wt = mbar_wait(bar(B_OF + 1), o_uses[1] & 1u, abort_flag, a.status);
-        if (!__all_sync(full, wt)) {
-          ok = false;
-          break;
-        }
+        ok = wait(B_OF + 1, o_uses[1] & 1u);
+        if (!ok) break;
         ml[row] = make_float2(m, l);
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(B_XF));
       }
-      const int w0 = x.two ? w : 0;
-      if (store) {
-        bool wt = true;
-        for (int s = 0; s < n_o; ++s)
-          wt = wt && mbar_wait(bar(B_OF + w0 + s), o_uses[w0 + s] & 1u, abort_flag, a.status);
-        if (joined) wt = wt && mbar_wait(bar(B_XF), x_uses & 1u, abort_flag, a.status);
-        if (!__all_sync(full, wt)) {
-          ok = false;
-          break;
-        }
+      const int w0 = two ? w : 0;
+      if (two || w == 0) {
+        for (int s = 0; ok && s < n_o; ++s) ok = wait(B_OF + w0 + s, o_uses[w0 + s] & 1u);
+        if (joined) ok = ok && wait(B_XF, x_uses & 1u);
+        if (!ok) break;
         fence_after();
         float al0 = 1.0f, al1 = 0.0f;
         if (joined) {
@@ -823,21 +850,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int hq = x.h * a.G + g;
         const int64_t qt = int64_t(x.a0) + j;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        const int pr = (x.two ? w * kRows : 0) + row;
+        const int pr = (two ? w * kRows : 0) + row;
         float* part = whole ? nullptr : part_of(a.workspace, n_cta, cta, x.t0 > 0 ? 0 : 1);
         if (busy) {
 #pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
+          for (int q = 0; q < D / 32; ++q) {
             float o[32];
             if (n_o == 0) {
 #pragma unroll
               for (int k = 0; k < 32; ++k) o[k] = 0.0f;
             } else {
-              tmem_ld32(lane_addr + kOCol + w0 * 128 + c * 32, o);
+              tmem_ld32(lane_addr + kOCol + w0 * 128 + q * 32, o);
               tmem_wait(o);
               if (joined) {
                 float o1[32];
-                tmem_ld32(lane_addr + kOCol + 128 + c * 32, o1);
+                tmem_ld32(lane_addr + kOCol + 128 + q * 32, o1);
                 tmem_wait(o1);
                 // a stream that saw nothing of this row left zeros
 #pragma unroll
@@ -851,7 +878,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int phys = lb < a.MB ? a.block_table[x.r * a.bt_stride_r + lb] : -1;
                 if (phys < 0 || phys >= a.NB) continue;
                 const uint16_t* vr = static_cast<const uint16_t*>(a.kv) + a.kv_stride_kv + int64_t(phys) * a.kv_stride_b +
-                                     int64_t(t - lb * a.BS) * a.kv_stride_s + int64_t(x.h) * a.kv_stride_h + c * 32;
+                                     int64_t(t - lb * a.BS) * a.kv_stride_s + int64_t(x.h) * a.kv_stride_h + q * 32;
 #pragma unroll
                 for (int k = 0; k < 32; ++k) {
                   const float f = BF16 ? __uint_as_float(uint32_t(vr[k]) << 16) : __half2float(__ushort_as_half(vr[k]));
@@ -861,12 +888,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             if (put) {
               if (whole) {
-                store_row<D, BF16>(static_cast<uint16_t*>(a.out) + qt * a.out_stride_t + int64_t(hq) * a.out_stride_h + c * 32,
+                store_row<D, BF16>(static_cast<uint16_t*>(a.out) + qt * a.out_stride_t + int64_t(hq) * a.out_stride_h + q * 32,
                                    o, inv, vec_out);
               } else {
 #pragma unroll
                 for (int k = 0; k < 32; k += 4)
-                  *reinterpret_cast<float4*>(part + int64_t(pr) * D + c * 32 + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                  *reinterpret_cast<float4*>(part + int64_t(pr) * D + q * 32 + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
               }
             }
           }
@@ -889,7 +916,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           d.a0 = x.a0;
           d.end = x.end;
           d.total = sched.total;
-          d.two = x.two;
+          d.two = two;
           static_cast<Desc*>(a.workspace)[cta] = d;
         }
         fence_before();
@@ -897,7 +924,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0)
           for (int s = 0; s < n_o; ++s) mbar_arrive(bar(B_OE + w0 + s));
       }
-      if (x.two) {
+      if (two) {
         ++o_uses[0];
         ++o_uses[1];
       } else {
@@ -905,6 +932,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (nt > 1) ++o_uses[1];
       }
       if (joined) ++x_uses;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(B_UE + slot));
     }
     fence_before();
   }
