@@ -38,7 +38,8 @@ namespace chunk {
 
 using namespace umma;
 
-constexpr int kThreads = 384;
+constexpr int kMaxThreads = 512;
+constexpr int threads(bool quant) { return quant ? 512 : 384; }
 constexpr int kUnitSlots = 4;               // units announced ahead of their results
 constexpr int kRows = 128;                  // query rows per tile (MMA M)
 constexpr int kTile = 128;                  // tokens per key tile
@@ -90,7 +91,7 @@ struct Sched {               // in shared memory
   uint32_t tmem;
   int abort_flag;
   int bad_v;                 // a value that some row of the unit does not see is not finite
-  int64_t scan[kThreads / 32];
+  int64_t scan[kMaxThreads / 32];
   Unit units[kUnitSlots];    // from the TMA warp, which alone walks the schedule; r < 0 ends it
 };
 static_assert(sizeof(Sched) <= kSchedBytes, "the schedule's place in shared memory");
@@ -180,6 +181,7 @@ struct Walker {
 };
 
 // Total weight, and the session that holds this CTA's first unit of weight.
+template <int kThreads>
 __device__ void make_schedule(const ChunkArgs& a, Sched& s, int cta, int n) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Geometry geo(a);
@@ -369,6 +371,53 @@ __device__ __forceinline__ void store_row(uint16_t* dst, const float (&o)[32], f
   }
 }
 
+// 16 e4m3 values with scale byte b as 16-bit values.  The four exponent and three mantissa bits of a
+// byte, moved under the wider type's exponent, read as the value times 2^-120 (bf16) or 2^-8 (fp16),
+// subnormals included, so one multiplication by a power of two, 2^(b - 127) with that put right, gives
+// the value exactly; a power of two outside the type takes a second one.  fp16 values past its range
+// become its largest.
+template <bool BF16>
+__device__ __forceinline__ void widen16(const uint4& raw, uint32_t b, uint4 (&out)[2]) {
+  const uint32_t in[4] = {raw.x, raw.y, raw.z, raw.w};
+  uint32_t r[8];
+  // bits of the multiplier in both halves
+  const int e = BF16 ? int(b) + 120 : int(b) - 104;
+  const int top = BF16 ? 254 : 30;
+  const int e1 = min(max(e, 1), top);
+  uint32_t f1 = uint32_t(e1) << (BF16 ? 7 : 10);
+  if (b == 255u) f1 = 0x7fffu;               // NaN
+  f1 |= f1 << 16;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t x = __byte_perm(in[i >> 1], 0u, (i & 1) ? 0x3424 : 0x1404);   // two bytes, each atop a half
+    const uint32_t y = ((x >> (BF16 ? 4 : 1)) & (BF16 ? 0x07f007f0u : 0x3f803f80u)) | (x & 0x80008000u);
+    if constexpr (BF16) asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r[i]) : "r"(y), "r"(f1));
+    else asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r[i]) : "r"(y), "r"(f1));
+  }
+  if (e != e1 && b != 255u) {
+    const int e2 = min(max(e - e1 + (BF16 ? 127 : 15), 1), top);
+    uint32_t f2 = uint32_t(e2) << (BF16 ? 7 : 10);
+    f2 |= f2 << 16;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (BF16) {
+        asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(f2));
+      } else {
+        asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(f2));
+      }
+    }
+  }
+  if (!BF16 && b >= 134u && b != 255u) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      asm("min.f16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(0x7bff7bffu));
+      asm("max.f16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(0xfbfffbffu));
+    }
+  }
+  out[0] = make_uint4(r[0], r[1], r[2], r[3]);
+  out[1] = make_uint4(r[4], r[5], r[6], r[7]);
+}
+
 // One token's values of a tile in shared memory: zeroed when the token is past the session's end; when
 // `hidden` (some row does not see it), what is not finite is zeroed and *bad_v set.
 template <int D, bool BF16>
@@ -403,8 +452,8 @@ __device__ __forceinline__ void clean_values(uint8_t* tile, bool past, bool hidd
 }
 
 // ------------------------------------------------------------------------------------ the kernel
-template <int D, bool BF16>
-__global__ void __launch_bounds__(kThreads, 1)
+template <int D, bool BF16, bool QUANT>
+__global__ void __launch_bounds__(threads(QUANT), 1)
     chunk_umma_kernel(const __grid_constant__ CUtensorMap tmap_kv, const __grid_constant__ CUtensorMap tmap_q,
                       const __grid_constant__ ChunkArgs a, bool vec_out) {
   using Ly = Layout<D>;
@@ -429,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSlots; ++i) {
-      mbar_init(bar(B_KVF + i), 1);
+      mbar_init(bar(B_KVF + i), QUANT ? 4 : 1);
       mbar_init(bar(B_KVE + i), 1);
     }
     mbar_init(bar(B_QF), 1);
@@ -444,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(bar(B_XF), 4);
     for (int i = 0; i < kUnitSlots; ++i) {
       mbar_init(bar(B_UF + i), 1);
-      mbar_init(bar(B_UE + i), 9);           // the MMA warp and the softmax warps
+      mbar_init(bar(B_UE + i), QUANT ? 13 : 9);   // the MMA warp, the softmax warps, the converting warps
     }
     sched.total = sched.pre = 0;
     sched.r0 = a.R;
@@ -462,20 +511,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   pdl_trigger();
   __syncthreads();
-  make_schedule(a, sched, cta, n_cta);
+  make_schedule<threads(QUANT)>(a, sched, cta, n_cta);
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = sched.tmem;
   const int tpb = kRows / a.G;
 
-  // 384 threads of 168 registers: the softmax warps take 208 each, the others keep 88
+  // 384 threads of 168 registers: the softmax warps take 208 each, the others keep 88.  With the
+  // converting warps 512 threads of 128: 160, 64, and 128 for those.
   if (warp < 4) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  if constexpr (QUANT) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (whole warp)
     if (lane == 0) {
-      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_kv)) : "memory");
+      if constexpr (!QUANT) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_kv)) : "memory");
       asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_q)) : "memory");
     }
     const int bs_box = min(a.BS, kTile);         // token rows of a box
@@ -509,7 +560,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         return int((int64_t(phys) * a.BS + (tok - lb * a.BS)) >> 3);
       };
-      int id0 = read_id(x.t0), id1 = read_id(x.t0 + 1), id2 = read_id(x.t0 + 2);
+      int id0 = -2, id1 = -2, id2 = -2;
+      if constexpr (!QUANT) {
+        id0 = read_id(x.t0);
+        id1 = read_id(x.t0 + 1);
+        id2 = read_id(x.t0 + 2);
+      }
       ok = __all_sync(full, mbar_wait(bar(B_QE), (q_uses & 1u) ^ 1u, abort_flag, a.status));
       if (!ok) break;
       if (lane == 0) {
@@ -521,6 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         x.a0 + x.j0 + b * tpb);
       }
       ++q_uses;
+      if constexpr (QUANT) continue;             // keys and values come through the converting warps
       auto load = [&](int t, int id, int plane) -> bool {
         const int slot = ring % kSlots;
         const bool w2 = mbar_wait(bar(B_KVE + slot), ((ring / kSlots) & 1u) ^ 1u, abort_flag, a.status);
@@ -687,8 +744,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (*abort_flag && last_bar >= 0 && lane == 0) mbar_drain(bar(last_bar), last_par);
   }
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+  } else if (warp < 12) {
+    if constexpr (QUANT) asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ------------------------------------------------------------------ softmax and output
     // A thread per row; p goes to the second product in two halves of 64 tokens.
     const int w = (warp - 4) >> 2;               // stream
@@ -731,7 +789,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // session's rows): zeroed, since 0 * NaN is NaN.  Values that some row of the unit does not
         // see must not reach it either: if one is not finite it is zeroed too, and the rows that do
         // see it get it back at the end.
-        if (tok0 + kTile - 1 > lim_min && (!two || w == 0)) {
+        if (!QUANT && tok0 + kTile - 1 > lim_min && (!two || w == 0)) {
           const uint32_t pos = ring + v_position(t, nt, lead);
           ok = wait(B_KVF + pos % kSlots, (pos / kSlots) & 1u);
           if (!ok) break;
@@ -877,12 +935,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int lb = t / a.BS;
                 const int phys = lb < a.MB ? a.block_table[x.r * a.bt_stride_r + lb] : -1;
                 if (phys < 0 || phys >= a.NB) continue;
-                const uint16_t* vr = static_cast<const uint16_t*>(a.kv) + a.kv_stride_kv + int64_t(phys) * a.kv_stride_b +
-                                     int64_t(t - lb * a.BS) * a.kv_stride_s + int64_t(x.h) * a.kv_stride_h + q * 32;
+                const int64_t at = a.kv_stride_kv + int64_t(phys) * a.kv_stride_b + int64_t(t - lb * a.BS) * a.kv_stride_s;
+                if constexpr (QUANT) {           // 32 values share a scale byte; 255 makes them NaN
+                  if (static_cast<const uint8_t*>(a.kv)[at + a.Hkv * D + x.h * (D / 32) + q] == 255)
 #pragma unroll
-                for (int k = 0; k < 32; ++k) {
-                  const float f = BF16 ? __uint_as_float(uint32_t(vr[k]) << 16) : __half2float(__ushort_as_half(vr[k]));
-                  if (!isfinite(f)) o[k] += f;
+                    for (int k = 0; k < 32; ++k) o[k] = __int_as_float(0x7fffffff);
+                } else {
+                  const uint16_t* vr = static_cast<const uint16_t*>(a.kv) + at + int64_t(x.h) * a.kv_stride_h + q * 32;
+#pragma unroll
+                  for (int k = 0; k < 32; ++k) {
+                    const float f = BF16 ? __uint_as_float(uint32_t(vr[k]) << 16) : __half2float(__ushort_as_half(vr[k]));
+                    if (!isfinite(f)) o[k] += f;
+                  }
                 }
               }
             }
@@ -936,6 +1000,145 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(bar(B_UE + slot));
     }
     fence_before();
+  } else if constexpr (QUANT) {
+    // ------------------------------------------------------------------ e4m3 -> 16 bits (four warps)
+    // A warp takes 32 of a tile's tokens: D / 16 lanes per token read 16 values each (one tile ahead, in
+    // registers; the tile three further on is asked of L2), and write them converted into the ring in the
+    // layout the TMA would have left.
+    constexpr int kLpr = D / 16, kRpi = 32 / kLpr, kLoads = 32 / kRpi;
+    const int row0 = (warp - 12) * 32, lr = lane / kLpr, lc = lane % kLpr;
+    const uint8_t* rows = static_cast<const uint8_t*>(a.kv);
+    struct Item {                                // a K or V tile on its way
+      int t, plane, S, h, r, lim_min, t1;
+    };
+    struct Cursor {                              // the unit being loaded
+      int t0, t1, lead, p, S, h, r, lim_min;
+    } cu;
+    uint32_t n = 0;
+    bool ok = true;
+    auto wait = [&](int b, uint32_t par) -> bool {
+      return __all_sync(full, mbar_wait(bar(b), par, abort_flag, a.status));
+    };
+    cu.t0 = cu.t1 = cu.p = 0;
+    auto next_item = [&](Item& y) -> bool {
+      while (cu.p >= 2 * (cu.t1 - cu.t0)) {
+        const uint32_t slot = n % kUnitSlots;
+        if (!wait(B_UF + slot, (n / kUnitSlots) & 1u)) {
+          ok = false;
+          return false;
+        }
+        const volatile Unit& x = sched.units[slot];
+        const int r = x.r;
+        cu.t0 = x.t0;
+        cu.t1 = x.t1;
+        cu.lead = x.two ? 1 : 2;
+        cu.S = x.S;
+        cu.h = x.h;
+        cu.r = r;
+        cu.lim_min = x.S - x.A + x.j0;
+        cu.p = 0;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_UE + slot));
+        ++n;
+        if (r < 0) return false;
+      }
+      // ring order: keys 0 .. lead - 1, values t and keys t + lead in turn, the last values
+      const int nt = cu.t1 - cu.t0, l0 = min(cu.lead, nt), q = cu.p - l0, both = 2 * (nt - l0);
+      if (q < 0) {
+        y.t = cu.p;
+        y.plane = 0;
+      } else if (q < both) {
+        y.plane = 1 - (q & 1);
+        y.t = (q >> 1) + (y.plane ? 0 : l0);
+      } else {
+        y.plane = 1;
+        y.t = nt - l0 + q - both;
+      }
+      y.t += cu.t0;
+      y.S = cu.S;
+      y.h = cu.h;
+      y.r = cu.r;
+      y.lim_min = cu.lim_min;
+      y.t1 = cu.t1;
+      ++cu.p;
+      return true;
+    };
+    // slot of this lane's token (row0 + lane) of tile t; -1 past the session's end
+    auto row_slot = [&](const Item& y, int t) -> int {
+      const int tok = t * kTile + row0 + lane;
+      if (tok >= y.S || t >= y.t1) return -1;
+      const int lb = tok / a.BS;
+      int phys = lb < a.MB ? a.block_table[y.r * a.bt_stride_r + lb] : -1;
+      if (phys < 0 || phys >= a.NB) {
+        flag(a.status, ACTKV_DEV_BAD_INDEX);
+        phys = 0;
+      }
+      return phys * a.BS + (tok - lb * a.BS);
+    };
+    auto load = [&](const Item& y, int rs, uint4 (&raw)[kLoads], uint32_t (&sc)[kLoads]) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int s = __shfl_sync(full, rs, i * kRpi + lr);
+        raw[i] = make_uint4(0u, 0u, 0u, 0u);
+        sc[i] = 127u;
+        if (s >= 0) {
+          const uint8_t* row = rows + y.plane * a.kv_stride_kv + int64_t(s) * a.kv_stride_s;
+          raw[i] = __ldg(reinterpret_cast<const uint4*>(row + y.h * D + lc * 16));
+          sc[i] = __ldg(row + a.Hkv * D + y.h * (D / 32) + (lc >> 1));
+        }
+      }
+    };
+    Item cur, nxt;
+    uint4 raw[2][kLoads];
+    uint32_t sc[2][kLoads];
+    Ring ring;
+    bool have = next_item(cur);
+    if (have) load(cur, row_slot(cur, cur.t), raw[0], sc[0]);
+    bool more = have && next_item(nxt);
+    int rs = more ? row_slot(nxt, nxt.t) : -1;
+    while (have && ok) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {              // two steps, so that the buffers are registers
+        if (!have || !ok) break;
+        Item nn = nxt;
+        if (more) load(nxt, rs, raw[k ^ 1], sc[k ^ 1]);
+        const bool more2 = more && next_item(nn);
+        if (!ok) break;
+        const int rs2 = more2 ? row_slot(nn, nn.t) : -1;
+        const int ahead = row_slot(cur, cur.t + 3);
+        ok = wait(B_KVE + ring.slot, ring.par ^ 1u);
+        if (!ok) break;
+        uint8_t* tile = smem + Ly::kKvOff + ring.slot * Ly::kTileBytes;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+          const int row = row0 + i * kRpi + lr;
+          uint4 o[2];
+          uint32_t b = sc[k][i];
+          if (cur.plane == 1 && b == 255u && cur.t * kTile + row > cur.lim_min) {
+            b = 127u;                            // its values are 0; the rows that see it get NaN at the end
+            *bad_v = 1;
+          }
+          widen16<BF16>(raw[k][i], b, o);
+          uint8_t* dst = tile + (row >> 3) * Ly::kGroupBytes + (lc >> 2) * 1024 + (row & 7) * 128;
+          // the lanes of a token's two halves write even and odd chunks first: eight banks' worth each time
+          const int c0 = (lc & 3) * 2, sw = D == 128 ? lc >> 2 : 0;
+          *reinterpret_cast<uint4*>(dst + (((c0 + sw) ^ (row & 7)) << 4)) = sw ? o[1] : o[0];
+          *reinterpret_cast<uint4*>(dst + (((c0 + 1 - sw) ^ (row & 7)) << 4)) = sw ? o[0] : o[1];
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_KVF + ring.slot));
+        ring.next(kSlots);
+        if (ahead >= 0)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(rows + cur.plane * a.kv_stride_kv + int64_t(ahead) * a.kv_stride_s +
+                                                        cur.h * D));
+        cur = nxt;
+        nxt = nn;
+        rs = rs2;
+        have = more;
+        more = more2;
+      }
+    }
   }
   __syncthreads();
   if (warp == 1) {
@@ -1008,31 +1211,31 @@ bool chunk_umma_supported(const ChunkArgs& a, int dtype, const char** why) {
     *why = w;
     return false;
   };
-  if (a.quant) return no("the 8-bit cache runs on CUDA cores");
   if (dtype != ACTKV_BF16 && dtype != ACTKV_F16) return no("needs bf16 or fp16");
   if (a.D != 64 && a.D != 128) return no("needs head_dim 64 or 128");
   if (a.G > chunk::kRows) return no("needs a GQA group of at most 128");
   if (!((a.BS % 8 == 0 && chunk::kTile % a.BS == 0) || a.BS % chunk::kTile == 0))
     return no("needs a block size of 8, 16, 32, 64 or a multiple of 128");
-  if (a.kv_stride_h != a.D || a.kv_stride_b != int64_t(a.BS) * a.kv_stride_s)
+  if (a.kv_stride_b != int64_t(a.BS) * a.kv_stride_s || (!a.quant && a.kv_stride_h != a.D))
     return no("needs heads next to one another and blocks of consecutive slots");
-  if ((reinterpret_cast<uintptr_t>(a.kv) | reinterpret_cast<uintptr_t>(a.q)) % 16) return no("q and kv must be 16-byte aligned");
-  if (a.kv_stride_s % 8 || a.kv_stride_kv % 8 || a.q_stride_h % 8 || a.q_stride_t % 8 || a.kv_stride_s < 0 ||
+  if ((reinterpret_cast<uintptr_t>(a.kv) | reinterpret_cast<uintptr_t>(a.q)) % 16) return no("q and the cache must be 16-byte aligned");
+  const int64_t es = a.quant ? 1 : 2;
+  if (a.kv_stride_s * es % 16 || a.kv_stride_kv * es % 16 || a.q_stride_h % 8 || a.q_stride_t % 8 || a.kv_stride_s < 0 ||
       a.kv_stride_kv < 0 || a.q_stride_h < 0 || a.q_stride_t < 0)
-    return no("q and kv strides must be multiples of 16 bytes");
-  if (int64_t(a.NB) * a.BS / 8 > 0x7fffffffll) return no("too many slots");
+    return no("strides of q and the cache must be multiples of 16 bytes");
+  if (int64_t(a.NB) * a.BS > 0x7fffffffll) return no("too many slots");
   return true;
 }
 
 namespace {
 
-template <int D, bool BF16>
+template <int D, bool BF16, bool QUANT>
 cudaError_t launch_chunk_t(const CUtensorMap& mkv, const CUtensorMap& mq, const ChunkArgs& a, int grid, cudaStream_t st) {
-  auto k = chunk::chunk_umma_kernel<D, BF16>;
+  auto k = chunk::chunk_umma_kernel<D, BF16, QUANT>;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(chunk::Layout<D>::kSmemBytes));
   if (e != cudaSuccess) return e;
   const bool vec_out = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_stride_t % 8 == 0 && a.out_stride_h % 8 == 0;
-  k<<<grid, chunk::kThreads, chunk::Layout<D>::kSmemBytes, st>>>(mkv, mq, a, vec_out);
+  k<<<grid, chunk::threads(QUANT), chunk::Layout<D>::kSmemBytes, st>>>(mkv, mq, a, vec_out);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid, chunk::kJoinSlices);
@@ -1056,8 +1259,8 @@ cudaError_t launch_chunk_umma(const ChunkArgs& a, int dtype, cudaStream_t st, co
   }
   const CUtensorMapDataType dt = dtype == ACTKV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const cuuint32_t es[5] = {1, 1, 1, 1, 1};
-  CUtensorMap mkv, mq;
-  {
+  CUtensorMap mkv = {}, mq;
+  if (!a.quant) {
     // (64 dims, slot within 8, D-half of a head, group of 8 slots, plane): a box leaves every 8-token
     // group's D-halves next to one another, so the groups of a tile are evenly spaced
     const cuuint32_t halves = cuuint32_t(a.D / 64), rows = cuuint32_t(a.BS < chunk::kTile ? a.BS : chunk::kTile);
@@ -1083,9 +1286,13 @@ cudaError_t launch_chunk_umma(const ChunkArgs& a, int dtype, cudaStream_t st, co
   }
   *why = "chunk attention";
   const int grid = device_sm_count();
-  if (a.D == 128)
-    return dtype == ACTKV_BF16 ? launch_chunk_t<128, true>(mkv, mq, a, grid, st) : launch_chunk_t<128, false>(mkv, mq, a, grid, st);
-  return dtype == ACTKV_BF16 ? launch_chunk_t<64, true>(mkv, mq, a, grid, st) : launch_chunk_t<64, false>(mkv, mq, a, grid, st);
+  const bool bf = dtype == ACTKV_BF16;
+  if (a.quant) {
+    if (a.D == 128) return bf ? launch_chunk_t<128, true, true>(mkv, mq, a, grid, st) : launch_chunk_t<128, false, true>(mkv, mq, a, grid, st);
+    return bf ? launch_chunk_t<64, true, true>(mkv, mq, a, grid, st) : launch_chunk_t<64, false, true>(mkv, mq, a, grid, st);
+  }
+  if (a.D == 128) return bf ? launch_chunk_t<128, true, false>(mkv, mq, a, grid, st) : launch_chunk_t<128, false, false>(mkv, mq, a, grid, st);
+  return bf ? launch_chunk_t<64, true, false>(mkv, mq, a, grid, st) : launch_chunk_t<64, false, false>(mkv, mq, a, grid, st);
 }
 
 }  // namespace actkv

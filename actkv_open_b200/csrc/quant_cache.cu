@@ -34,7 +34,9 @@ __device__ __forceinline__ void load16(const T* p, bool vec, float (&x)[16]) {
 
 template <typename T> __device__ __forceinline__ T from_f32(float x);
 template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
-template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __half from_f32<__half>(float x) {   // past the range: its largest
+  return __float2half_rn(x == x ? fminf(fmaxf(x, -65504.0f), 65504.0f) : x);
+}
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
 template <typename T>

@@ -64,7 +64,8 @@ def quantize_write(k_new, v_new, tok_off, rows, block_table, seq_used):
 def dequantize_read(rows, n_kv_heads, head_dim, tok_off, block_table, seq_used, n_tokens, dtype=torch.bfloat16,
                     k_out=None, v_out=None, planes: str = "kv"):
     """Read each session's newest tok_off[r+1] - tok_off[r] tokens back: (k, v) [L, n_tokens, Hkv, D],
-    packed as ``quantize_write`` takes them (n_tokens = tok_off[R]), rounded to ``dtype``.
+    packed as ``quantize_write`` takes them (n_tokens = tok_off[R]), rounded to ``dtype`` (fp16:
+    values past its range become its largest).
 
     ``planes`` "k" or "v" reads one of the two (the other comes back as None).
     """

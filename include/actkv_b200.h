@@ -500,7 +500,8 @@ ACTKV_API int actkv_chunk_attention_quant(const void* q, int dtype, int64_t q_st
  *   contiguous; T = tok_off[R]), quantised: per group of 32 the smallest scale with
  *   max|x| <= 448 * scale, values rounded to nearest even; a group with a non-finite value
  *   becomes NaN.  The tables already hold the tokens' blocks.
- * actkv_dequantize_read: the same tokens read back into k_out / v_out (either may be NULL), rounded to dtype.
+ * actkv_dequantize_read: the same tokens read back into k_out / v_out (either may be NULL), rounded to
+ *   dtype (fp16: values past its range become its largest).
  * actkv_quant_append: actkv_append (tables, lengths, free stack) followed by actkv_quantize_write of
  *   the new rows, for the sessions that fit; new_off as there.
  * Tokens that the tables do not hold set ACTKV_DEV_BAD_INDEX and are skipped.
