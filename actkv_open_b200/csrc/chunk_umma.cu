@@ -38,8 +38,8 @@ namespace chunk {
 
 using namespace umma;
 
-constexpr int kMaxThreads = 512;
-constexpr int threads(bool quant) { return quant ? 512 : 384; }
+constexpr int kMaxThreads = 640;
+constexpr int threads(bool quant) { return quant ? 640 : 384; }
 constexpr int kUnitSlots = 4;               // units announced ahead of their results
 constexpr int kRows = 128;                  // query rows per tile (MMA M)
 constexpr int kTile = 128;                  // tokens per key tile
@@ -49,18 +49,23 @@ constexpr int kMaxD = 128;
 
 constexpr uint32_t kSchedBytes = 512;
 
-template <int D>
+template <int D, bool QUANT>
 struct Layout {
   static constexpr int kHalves = D / 64;
   static constexpr uint32_t kTileBytes = kTile * D * 2;      // a K, V or Q tile
-  static constexpr int kSlots = D == 128 ? 5 : 10;
+  static constexpr int kSlots = QUANT ? (D == 128 ? 3 : 6) : (D == 128 ? 5 : 10);
   static constexpr uint32_t kGroupBytes = kHalves * 1024;    // 8 tokens of a K / V tile
   static constexpr uint32_t kKvOff = 2 * kTileBytes;
-  static constexpr uint32_t kMlOff = kKvOff + kSlots * kTileBytes;       // stream 1's (m, l) per row
+  // the 8-bit cache's tiles before they are widened, and their scale words per token
+  static constexpr int kRaw = QUANT ? (D == 128 ? 3 : 6) : 0;
+  static constexpr uint32_t kRawBytes = kTile * D;
+  static constexpr uint32_t kRawOff = kKvOff + kSlots * kTileBytes;
+  static constexpr uint32_t kScaleOff = kRawOff + kRaw * kRawBytes;
+  static constexpr uint32_t kMlOff = kScaleOff + kRaw * kTile * 4;       // stream 1's (m, l) per row
   static constexpr uint32_t kBarOff = kMlOff + kRows * 8;
   // kv_full[slots] kv_empty[slots] q_full q_empty s_full[2] p_full[2][2] o_full[2] o_empty[2]
-  // x_full unit_full[4] unit_empty[4]
-  static constexpr int kNumBars = 2 * kSlots + 13 + 2 * kUnitSlots;
+  // x_full unit_full[4] unit_empty[4] raw_full[raw] raw_empty[raw] scale_full[raw]
+  static constexpr int kNumBars = 2 * kSlots + 13 + 2 * kUnitSlots + 3 * kRaw;
   static constexpr uint32_t kSchedOff = kBarOff + kNumBars * 8;
   static constexpr uint32_t kSmemBytes = kSchedOff + kSchedBytes;
   static_assert(kSmemBytes <= 232448, "exceeds the 227 KB of shared memory a CTA can have");
@@ -345,6 +350,29 @@ __device__ __forceinline__ int v_position(int t, int nt, int lead) {
   return min(lead, nt) + t + min(t, max(0, nt - lead));
 }
 
+// The K and V tiles of a unit's part in ring order: keys 0 .. lead - 1, then values t and keys t + lead
+// in turn, then the last values.
+struct UnitItems {
+  int t0 = 0, nt = 0, lead = 0, p = 0, S = 0, h = 0, r = 0, hidden = 0;
+  __device__ bool done() const { return p >= 2 * nt; }
+  __device__ void start(const volatile Unit& x) {
+    r = x.r;
+    t0 = x.t0;
+    nt = r < 0 ? 0 : max(0, x.t1 - x.t0);
+    lead = min(x.two ? 1 : 2, nt);
+    S = x.S;
+    h = x.h;
+    hidden = x.S - x.A + x.j0 + 1;           // the first token that some row does not see
+    p = 0;
+  }
+  __device__ void next(int& t, int& plane) {
+    const int q = p - lead, both = 2 * (nt - lead);
+    plane = q < 0 ? 0 : (q < both ? 1 - (q & 1) : 1);
+    t = t0 + (q < 0 ? p : (q < both ? (q >> 1) + (plane ? 0 : lead) : nt - lead + q - both));
+    ++p;
+  }
+};
+
 // Part `slot` (0: a unit begun by an earlier CTA, 1: one left to the next) of CTA `cta`'s partial
 // results: rows of D values, then (m, l) per row.
 constexpr int64_t kPartFloats = int64_t(2 * kRows) * (kMaxD + 2);
@@ -377,45 +405,48 @@ __device__ __forceinline__ void store_row(uint16_t* dst, const float (&o)[32], f
 // the value exactly; a power of two outside the type takes a second one.  fp16 values past its range
 // become its largest.
 template <bool BF16>
-__device__ __forceinline__ void widen16(const uint4& raw, uint32_t b, uint4 (&out)[2]) {
+__device__ __forceinline__ uint32_t mul16x2(uint32_t x, uint32_t f) {
+  uint32_t r;
+  if constexpr (BF16) asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(f));
+  else asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(f));
+  return r;
+}
+// Whether one multiplication does for every byte of a word of scale bytes.
+template <bool BF16>
+__device__ __forceinline__ bool plain_scales(uint32_t w) {
+  return __vcmpgtu4(w, 0x86868686u) == 0 && (BF16 || __vcmpgtu4(0x69696969u, w) == 0);   // <= 134 (fp16: >= 105)
+}
+template <bool BF16>
+__device__ __forceinline__ void widen16(const uint4& raw, uint32_t f, uint32_t (&r)[8]) {
   const uint32_t in[4] = {raw.x, raw.y, raw.z, raw.w};
-  uint32_t r[8];
-  // bits of the multiplier in both halves
-  const int e = BF16 ? int(b) + 120 : int(b) - 104;
-  const int top = BF16 ? 254 : 30;
-  const int e1 = min(max(e, 1), top);
-  uint32_t f1 = uint32_t(e1) << (BF16 ? 7 : 10);
-  if (b == 255u) f1 = 0x7fffu;               // NaN
-  f1 |= f1 << 16;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const uint32_t x = __byte_perm(in[i >> 1], 0u, (i & 1) ? 0x3424 : 0x1404);   // two bytes, each atop a half
     const uint32_t y = ((x >> (BF16 ? 4 : 1)) & (BF16 ? 0x07f007f0u : 0x3f803f80u)) | (x & 0x80008000u);
-    if constexpr (BF16) asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r[i]) : "r"(y), "r"(f1));
-    else asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r[i]) : "r"(y), "r"(f1));
+    r[i] = mul16x2<BF16>(y, f);
   }
-  if (e != e1 && b != 255u) {
-    const int e2 = min(max(e - e1 + (BF16 ? 127 : 15), 1), top);
-    uint32_t f2 = uint32_t(e2) << (BF16 ? 7 : 10);
-    f2 |= f2 << 16;
+}
+// The multiplier of scale byte b, in both halves, where plain_scales holds.
+template <bool BF16>
+__device__ __forceinline__ uint32_t plain_factor(uint32_t b) {
+  return BF16 ? b * 0x00800080u + 0x3c003c00u : (b - 104u) * 0x04000400u;
+}
+// Any scale byte.
+template <bool BF16>
+__device__ __noinline__ void widen16_any(const uint4 raw, uint32_t b, uint32_t (&r)[8]) {
+  const int e = BF16 ? int(b) + 120 : int(b) - 104, top = BF16 ? 254 : 30;
+  const int e1 = min(max(e, 1), top), e2 = min(max(e - e1 + (BF16 ? 127 : 15), 1), top);
+  const uint32_t one = BF16 ? 0x00800080u : 0x04000400u;
+  widen16<BF16>(raw, b == 255u ? 0x7fff7fffu : e1 * one, r);                     // 255: NaN
+  if (b == 255u) return;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if constexpr (BF16) {
-        asm("mul.rn.bf16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(f2));
-      } else {
-        asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(f2));
-      }
-    }
-  }
-  if (!BF16 && b >= 134u && b != 255u) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 8; ++i) {
+    r[i] = mul16x2<BF16>(r[i], e2 * one);
+    if constexpr (!BF16) {
       asm("min.f16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(0x7bff7bffu));
       asm("max.f16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(0xfbfffbffu));
     }
   }
-  out[0] = make_uint4(r[0], r[1], r[2], r[3]);
-  out[1] = make_uint4(r[4], r[5], r[6], r[7]);
 }
 
 // One token's values of a tile in shared memory: zeroed when the token is past the session's end; when
@@ -456,7 +487,7 @@ template <int D, bool BF16, bool QUANT>
 __global__ void __launch_bounds__(threads(QUANT), 1)
     chunk_umma_kernel(const __grid_constant__ CUtensorMap tmap_kv, const __grid_constant__ CUtensorMap tmap_q,
                       const __grid_constant__ ChunkArgs a, bool vec_out) {
-  using Ly = Layout<D>;
+  using Ly = Layout<D, QUANT>;
   extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = smem_u32(smem);
@@ -468,7 +499,7 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
   constexpr int kSlots = Ly::kSlots;
   constexpr int B_KVF = 0, B_KVE = kSlots, B_QF = 2 * kSlots, B_QE = B_QF + 1, B_SF = B_QE + 1, B_PF = B_SF + 2,
                 B_OF = B_PF + 4, B_OE = B_OF + 2, B_XF = B_OE + 2, B_UF = B_XF + 1,
-                B_UE = B_UF + kUnitSlots;
+                B_UE = B_UF + kUnitSlots, B_RF = B_UE + kUnitSlots, B_RE = B_RF + Ly::kRaw, B_CF = B_RE + Ly::kRaw;
   const unsigned full = 0xffffffffu;
   const int cta = blockIdx.x, n_cta = gridDim.x;
 
@@ -478,7 +509,7 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSlots; ++i) {
-      mbar_init(bar(B_KVF + i), QUANT ? 4 : 1);
+      mbar_init(bar(B_KVF + i), QUANT ? 8 : 1);
       mbar_init(bar(B_KVE + i), 1);
     }
     mbar_init(bar(B_QF), 1);
@@ -493,7 +524,12 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
     mbar_init(bar(B_XF), 4);
     for (int i = 0; i < kUnitSlots; ++i) {
       mbar_init(bar(B_UF + i), 1);
-      mbar_init(bar(B_UE + i), QUANT ? 13 : 9);   // the MMA warp, the softmax warps, the converting warps
+      mbar_init(bar(B_UE + i), QUANT ? 18 : 9);   // MMA, softmax, scale and widening warps
+    }
+    for (int i = 0; i < Ly::kRaw; ++i) {
+      mbar_init(bar(B_RF + i), 1);
+      mbar_init(bar(B_RE + i), 8);
+      mbar_init(bar(B_CF + i), 1);
     }
     sched.total = sched.pre = 0;
     sched.r0 = a.R;
@@ -519,19 +555,21 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
   const int tpb = kRows / a.G;
 
   // 384 threads of 168 registers: the softmax warps take 208 each, the others keep 88.  With the
-  // converting warps 512 threads of 128: 160, 64, and 128 for those.
+  // widening warps 640 threads of 96: 152 and 56, and 56 for those.
   if (warp < 4) {
-  if constexpr (QUANT) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+  if constexpr (QUANT) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
   else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (whole warp)
     if (lane == 0) {
-      if constexpr (!QUANT) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_kv)) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_kv)) : "memory");
       asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmap_q)) : "memory");
     }
     const int bs_box = min(a.BS, kTile);         // token rows of a box
     const int bpt = kTile / bs_box;              // boxes per tile (<= 16: one per lane)
-    const uint32_t box_bytes = uint32_t(bs_box) * D * 2;
+    const uint32_t box_bytes = uint32_t(bs_box) * D * (QUANT ? 1 : 2);
+    // where the copies go: the ring itself, or the tiles to be widened into it
+    constexpr int kIn = QUANT ? Ly::kRaw : kSlots, B_FULL = QUANT ? B_RF : B_KVF, B_EMPTY = QUANT ? B_RE : B_KVE;
     Walker wk(&a, sched, cta, n_cta);
     Unit x;
     uint32_t ring = 0, q_uses = 0;
@@ -548,7 +586,7 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
       if (!any) break;
       if (x.t0 >= x.t1) continue;
       const int lead = x.two ? 1 : 2, nt = x.t1 - x.t0;
-      // first token slot, in units of 8, of lane b's box of key tile t; -2 past the session's end
+      // first token slot (16-bit rows: in units of 8) of lane b's box of key tile t; -2 past the session's end
       auto read_id = [&](int t) -> int {
         const int tok = t * kTile + lane * bs_box;
         if (lane >= bpt || t >= x.t1 || tok >= x.S) return -2;
@@ -558,14 +596,9 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
           flag(a.status, ACTKV_DEV_BAD_INDEX);
           return 0;
         }
-        return int((int64_t(phys) * a.BS + (tok - lb * a.BS)) >> 3);
+        return int((int64_t(phys) * a.BS + (tok - lb * a.BS)) >> (QUANT ? 0 : 3));
       };
-      int id0 = -2, id1 = -2, id2 = -2;
-      if constexpr (!QUANT) {
-        id0 = read_id(x.t0);
-        id1 = read_id(x.t0 + 1);
-        id2 = read_id(x.t0 + 2);
-      }
+      int id0 = read_id(x.t0), id1 = read_id(x.t0 + 1), id2 = read_id(x.t0 + 2);
       ok = __all_sync(full, mbar_wait(bar(B_QE), (q_uses & 1u) ^ 1u, abort_flag, a.status));
       if (!ok) break;
       if (lane == 0) {
@@ -577,17 +610,21 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
                         x.a0 + x.j0 + b * tpb);
       }
       ++q_uses;
-      if constexpr (QUANT) continue;             // keys and values come through the converting warps
       auto load = [&](int t, int id, int plane) -> bool {
-        const int slot = ring % kSlots;
-        const bool w2 = mbar_wait(bar(B_KVE + slot), ((ring / kSlots) & 1u) ^ 1u, abort_flag, a.status);
+        const int slot = ring % kIn;
+        const bool w2 = mbar_wait(bar(B_EMPTY + slot), ((ring / kIn) & 1u) ^ 1u, abort_flag, a.status);
         if (!__all_sync(full, w2)) return false;
         const int n = __popc(__ballot_sync(full, id >= 0));
-        if (lane == 0) mbar_expect_tx(bar(B_KVF + slot), uint32_t(n) * box_bytes);
+        if (lane == 0) mbar_expect_tx(bar(B_FULL + slot), uint32_t(n) * box_bytes);
         __syncwarp();
-        if (id >= 0)
-          tma_load_5d(base + Ly::kKvOff + slot * Ly::kTileBytes + lane * box_bytes, &tmap_kv, bar(B_KVF + slot), 0, 0,
-                      x.h * Ly::kHalves, id, plane);
+        if (id >= 0) {
+          if constexpr (QUANT)
+            tma_load_3d(base + Ly::kRawOff + slot * Ly::kRawBytes + lane * box_bytes, &tmap_kv, bar(B_FULL + slot), x.h * D,
+                        id, plane);
+          else
+            tma_load_5d(base + Ly::kKvOff + slot * Ly::kTileBytes + lane * box_bytes, &tmap_kv, bar(B_FULL + slot), 0, 0,
+                        x.h * Ly::kHalves, id, plane);
+        }
         ++ring;
         return true;
       };
@@ -604,9 +641,9 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
       if (!ok) break;
     }
     if (*abort_flag && lane == 0) {
-      for (uint32_t s = 0; s < kSlots; ++s) {
-        const uint32_t uses = ring / kSlots + (s < ring % kSlots ? 1u : 0u);
-        if (uses) mbar_drain(bar(B_KVF + s), (uses - 1) & 1u);
+      for (uint32_t s = 0; s < kIn; ++s) {
+        const uint32_t uses = ring / kIn + (s < ring % kIn ? 1u : 0u);
+        if (uses) mbar_drain(bar(B_FULL + s), (uses - 1) & 1u);
       }
       if (q_uses) mbar_drain(bar(B_QF), (q_uses - 1) & 1u);
     }
@@ -743,9 +780,74 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
       }
     }
     if (*abort_flag && last_bar >= 0 && lane == 0) mbar_drain(bar(last_bar), last_par);
+  } else if (QUANT && warp == 2) {
+    // ------------------------------------------------------------------ scale words of the 8-bit rows
+    // Four tokens per lane, from the cache through registers (one tile ahead) into the tile's words.
+    const int bpt = a.BS < kTile ? kTile / a.BS : 0, mpb = a.BS < kTile ? 1 : a.BS / kTile;
+    int sub[4], in_block[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      sub[i] = bpt ? (lane + 32 * i) / a.BS : 0;
+      in_block[i] = lane + 32 * i - sub[i] * a.BS;
+    }
+    UnitItems u;
+    uint32_t n = 0;
+    bool ok = true, have = true;
+    auto wait = [&](int b, uint32_t par) -> bool {
+      return __all_sync(full, mbar_wait(bar(b), par, abort_flag, a.status));
+    };
+    auto read_words = [&](uint32_t (&word)[4]) -> bool {      // of the next tile; false at the end
+      while (u.done()) {
+        const uint32_t slot = n % kUnitSlots;
+        if (!wait(B_UF + slot, (n / kUnitSlots) & 1u)) {
+          ok = false;
+          return false;
+        }
+        u.start(sched.units[slot]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_UE + slot));
+        ++n;
+        if (u.r < 0) return false;
+      }
+      int t, plane;
+      u.next(t, plane);
+      const int32_t* table = a.block_table + u.r * a.bt_stride_r;
+      int phys[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int lb = bpt ? t * bpt + sub[i] : t / mpb;
+        phys[i] = t * kTile + lane + 32 * i < u.S && lb < a.MB ? table[lb] : 0;
+      }
+      const uint8_t* p0 = static_cast<const uint8_t*>(a.kv) + plane * a.kv_stride_kv + a.Hkv * D + u.h * (D / 32);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int ph = phys[i] < 0 || phys[i] >= a.NB ? 0 : phys[i];          // flagged by the TMA warp
+        const uint8_t* p = p0 + (int64_t(ph) * a.BS + in_block[i] + (bpt ? 0 : t % mpb * kTile)) * a.kv_stride_s;
+        if constexpr (D == 128) word[i] = *reinterpret_cast<const uint32_t*>(p);
+        else word[i] = *reinterpret_cast<const uint16_t*>(p) | 0x7f7f0000u;
+      }
+      return true;
+    };
+    uint32_t w0[4], w1[4];
+    Ring ring;
+    have = read_words(w0);
+    while (have && ok) {
+      const bool more = read_words(w1);
+      if (!ok || !wait(B_RE + ring.slot, ring.par ^ 1u)) break;
+      uint32_t* dst = reinterpret_cast<uint32_t*>(smem + Ly::kScaleOff) + ring.slot * kTile;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        dst[lane + 32 * i] = w0[i];
+        w0[i] = w1[i];
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(B_CF + ring.slot));
+      ring.next(Ly::kRaw);
+      have = more;
+    }
   }
   } else if (warp < 12) {
-    if constexpr (QUANT) asm volatile("setmaxnreg.inc.sync.aligned.u32 160;");
+    if constexpr (QUANT) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ------------------------------------------------------------------ softmax and output
     // A thread per row; p goes to the second product in two halves of 64 tokens.
@@ -799,26 +901,36 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
         }
         fence_after();
         if (busy) {
-          float v[2][64];
-          tmem_ld64(s_addr, v[0]);
-          tmem_ld64(s_addr + 64, v[1]);
-          tmem_wait(v[0]);
-          tmem_wait(v[1]);
+          // With the widening warps a thread has registers for half a row only: the second half is read for
+          // the maximum, and again for p.
+          float v[QUANT ? 1 : 2][64];
           const bool masked = !__all_sync(full, tok0 + kTile - 1 <= lim);
           const int last = lim - tok0;                        // columns 0 .. last are seen
-          float mx[4];
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
+          float mx[4] = {ninf, ninf, ninf, ninf};
+          auto half_max = [&](float (&x)[64], int hf) {
             if (masked) {
 #pragma unroll
-              for (int k = 0; k < 64; ++k) v[hf][k] = hf * 64 + k <= last ? v[hf][k] : ninf;
+              for (int k = 0; k < 64; ++k) x[k] = hf * 64 + k <= last ? x[k] : ninf;
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mx[e] = hf ? fmax3(mx[e], v[hf][e], v[hf][e + 4]) : fmaxf(v[hf][e], v[hf][e + 4]);
+            for (int k = 0; k < 64; k += 8)
 #pragma unroll
-            for (int k = 8; k < 64; k += 8)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) mx[e] = fmax3(mx[e], v[hf][k + e], v[hf][k + e + 4]);
+              for (int e = 0; e < 4; ++e) mx[e] = fmax3(mx[e], x[k + e], x[k + e + 4]);
+          };
+          if constexpr (QUANT) {
+            tmem_ld64(s_addr + 64, v[0]);
+            tmem_wait(v[0]);
+            half_max(v[0], 1);
+            tmem_ld64(s_addr, v[0]);
+            tmem_wait(v[0]);
+            half_max(v[0], 0);
+          } else {
+            tmem_ld64(s_addr, v[0]);
+            tmem_ld64(s_addr + 64, v[QUANT ? 0 : 1]);
+            tmem_wait(v[0]);
+            tmem_wait(v[QUANT ? 0 : 1]);
+            half_max(v[0], 0);
+            half_max(v[QUANT ? 0 : 1], 1);
           }
           const float top = fmax3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * c2;
           const bool raise = top > m + kSlack;                // also when m is still -inf
@@ -845,10 +957,18 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
           // second product starts on the first 64
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
+            if (QUANT && q == 2) {
+              tmem_ld64(s_addr + 64, v[0]);
+              tmem_wait(v[0]);
+              if (masked) {
+#pragma unroll
+                for (int k = 0; k < 64; ++k) v[0][k] = 64 + k <= last ? v[0][k] : ninf;
+              }
+            }
             uint32_t u[16];
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
-              const float* vp = &v[q >> 1][(q & 1) * 32 + 2 * k];
+              const float* vp = &v[QUANT ? 0 : q >> 1][(q & 1) * 32 + 2 * k];
               const float2 e = fma2(make_float2(vp[0], vp[1]), c2v, offv);
               const float2 p = make_float2(ex2(e.x), ex2(e.y));
               sum[k & 1] = add2(sum[k & 1], p);
@@ -1001,143 +1121,84 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
     }
     fence_before();
   } else if constexpr (QUANT) {
-    // ------------------------------------------------------------------ e4m3 -> 16 bits (four warps)
-    // A warp takes 32 of a tile's tokens: D / 16 lanes per token read 16 values each (one tile ahead, in
-    // registers; the tile three further on is asked of L2), and write them converted into the ring in the
-    // layout the TMA would have left.
-    constexpr int kLpr = D / 16, kRpi = 32 / kLpr, kLoads = 32 / kRpi;
-    const int row0 = (warp - 12) * 32, lr = lane / kLpr, lc = lane % kLpr;
-    const uint8_t* rows = static_cast<const uint8_t*>(a.kv);
-    struct Item {                                // a K or V tile on its way
-      int t, plane, S, h, r, lim_min, t1;
-    };
-    struct Cursor {                              // the unit being loaded
-      int t0, t1, lead, p, S, h, r, lim_min;
-    } cu;
+    // ------------------------------------------------------------------ e4m3 -> 16 bits (eight warps)
+    // A warp takes 16 of a tile's tokens, D / 16 lanes per token, and leaves them in the ring in the layout
+    // the TMA leaves 16-bit rows in.
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    constexpr int kLpr = D / 16, kRpi = 32 / kLpr, kLoads = 16 / kRpi;
+    const int row0 = (warp - 12) * 16, lr = lane / kLpr, lc = lane % kLpr;
+    // Where a lane's piece comes from and its two 16-byte pieces go within 8 tokens.  The lanes of a token's two
+    // halves write even and odd chunks first: eight banks' worth each time.
+    const bool sw = D == 128 && lc >= 4;
+    uint32_t get[8 / kRpi], put0[8 / kRpi], put1[8 / kRpi];
+#pragma unroll
+    for (int i = 0; i < 8 / kRpi; ++i) {
+      const int r8 = i * kRpi + lr, c0 = (lc & 3) * 2;
+      get[i] = r8 * D + ((lc ^ (D == 128 ? r8 : (r8 >> 1) & 3)) << 4);
+      put0[i] = (lc >> 2) * 1024 + r8 * 128 + (((c0 + sw) ^ r8) << 4);
+      put1[i] = (lc >> 2) * 1024 + r8 * 128 + (((c0 + 1 - sw) ^ r8) << 4);
+    }
+    UnitItems u;
+    Ring ring, in;
     uint32_t n = 0;
     bool ok = true;
     auto wait = [&](int b, uint32_t par) -> bool {
       return __all_sync(full, mbar_wait(bar(b), par, abort_flag, a.status));
     };
-    cu.t0 = cu.t1 = cu.p = 0;
-    auto next_item = [&](Item& y) -> bool {
-      while (cu.p >= 2 * (cu.t1 - cu.t0)) {
+    while (true) {
+      while (ok && u.done()) {
         const uint32_t slot = n % kUnitSlots;
-        if (!wait(B_UF + slot, (n / kUnitSlots) & 1u)) {
-          ok = false;
-          return false;
-        }
-        const volatile Unit& x = sched.units[slot];
-        const int r = x.r;
-        cu.t0 = x.t0;
-        cu.t1 = x.t1;
-        cu.lead = x.two ? 1 : 2;
-        cu.S = x.S;
-        cu.h = x.h;
-        cu.r = r;
-        cu.lim_min = x.S - x.A + x.j0;
-        cu.p = 0;
+        ok = wait(B_UF + slot, (n / kUnitSlots) & 1u);
+        if (!ok) break;
+        u.start(sched.units[slot]);
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(B_UE + slot));
         ++n;
-        if (r < 0) return false;
+        if (u.r < 0) break;
       }
-      // ring order: keys 0 .. lead - 1, values t and keys t + lead in turn, the last values
-      const int nt = cu.t1 - cu.t0, l0 = min(cu.lead, nt), q = cu.p - l0, both = 2 * (nt - l0);
-      if (q < 0) {
-        y.t = cu.p;
-        y.plane = 0;
-      } else if (q < both) {
-        y.plane = 1 - (q & 1);
-        y.t = (q >> 1) + (y.plane ? 0 : l0);
-      } else {
-        y.plane = 1;
-        y.t = nt - l0 + q - both;
+      if (!ok || u.r < 0) break;
+      int t, plane;
+      u.next(t, plane);
+      ok = wait(B_CF + in.slot, in.par) && wait(B_RF + in.slot, in.par) && wait(B_KVE + ring.slot, ring.par ^ 1u);
+      if (!ok) break;
+      uint32_t sc = reinterpret_cast<const uint32_t*>(smem + Ly::kScaleOff)[in.slot * kTile + row0 + (lane & 15)];
+      const int first = t * kTile + row0;                     // the warp's first token
+      const bool edge = first + 16 > min(u.S, plane ? u.hidden : u.S);
+      if (edge) {
+        const int tok = first + (lane & 15);
+        if (tok >= u.S) {
+          sc = 0x7f7f7f7fu;
+        } else if (plane && tok >= u.hidden) {   // a NaN group's values are 0; the rows that see it get NaN at the end
+          const uint32_t bad = __vcmpeq4(sc, 0xffffffffu);
+          if (bad) *bad_v = 1;
+          sc = (sc & ~bad) | (0x7f7f7f7fu & bad);
+        }
       }
-      y.t += cu.t0;
-      y.S = cu.S;
-      y.h = cu.h;
-      y.r = cu.r;
-      y.lim_min = cu.lim_min;
-      y.t1 = cu.t1;
-      ++cu.p;
-      return true;
-    };
-    // slot of this lane's token (row0 + lane) of tile t; -1 past the session's end
-    auto row_slot = [&](const Item& y, int t) -> int {
-      const int tok = t * kTile + row0 + lane;
-      if (tok >= y.S || t >= y.t1) return -1;
-      const int lb = tok / a.BS;
-      int phys = lb < a.MB ? a.block_table[y.r * a.bt_stride_r + lb] : -1;
-      if (phys < 0 || phys >= a.NB) {
-        flag(a.status, ACTKV_DEV_BAD_INDEX);
-        phys = 0;
-      }
-      return phys * a.BS + (tok - lb * a.BS);
-    };
-    auto load = [&](const Item& y, int rs, uint4 (&raw)[kLoads], uint32_t (&sc)[kLoads]) {
+      const uint8_t* src = smem + Ly::kRawOff + in.slot * Ly::kRawBytes + row0 * D;
+      uint8_t* dst = smem + Ly::kKvOff + ring.slot * Ly::kTileBytes + (row0 >> 3) * Ly::kGroupBytes;
+      const bool plain = __all_sync(full, plain_scales<BF16>(sc));
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const int s = __shfl_sync(full, rs, i * kRpi + lr);
-        raw[i] = make_uint4(0u, 0u, 0u, 0u);
-        sc[i] = 127u;
-        if (s >= 0) {
-          const uint8_t* row = rows + y.plane * a.kv_stride_kv + int64_t(s) * a.kv_stride_s;
-          raw[i] = __ldg(reinterpret_cast<const uint4*>(row + y.h * D + lc * 16));
-          sc[i] = __ldg(row + a.Hkv * D + y.h * (D / 32) + (lc >> 1));
-        }
+        const int g8 = i * kRpi / 8, i8 = i * kRpi % 8 / kRpi;
+        uint4 x = *reinterpret_cast<const uint4*>(src + g8 * 8 * D + get[i8]);
+        if (edge && first + i * kRpi + lr >= u.S) x = make_uint4(0u, 0u, 0u, 0u);
+        const uint32_t b = __byte_perm(__shfl_sync(full, sc, i * kRpi + lr), 0u, 0x4440 | (lc >> 1));
+        uint32_t r[8];
+        if (plain) widen16<BF16>(x, plain_factor<BF16>(b), r);
+        else widen16_any<BF16>(x, b, r);
+        *reinterpret_cast<uint4*>(dst + g8 * Ly::kGroupBytes + put0[i8]) =
+            sw ? make_uint4(r[4], r[5], r[6], r[7]) : make_uint4(r[0], r[1], r[2], r[3]);
+        *reinterpret_cast<uint4*>(dst + g8 * Ly::kGroupBytes + put1[i8]) =
+            sw ? make_uint4(r[0], r[1], r[2], r[3]) : make_uint4(r[4], r[5], r[6], r[7]);
       }
-    };
-    Item cur, nxt;
-    uint4 raw[2][kLoads];
-    uint32_t sc[2][kLoads];
-    Ring ring;
-    bool have = next_item(cur);
-    if (have) load(cur, row_slot(cur, cur.t), raw[0], sc[0]);
-    bool more = have && next_item(nxt);
-    int rs = more ? row_slot(nxt, nxt.t) : -1;
-    while (have && ok) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {              // two steps, so that the buffers are registers
-        if (!have || !ok) break;
-        Item nn = nxt;
-        if (more) load(nxt, rs, raw[k ^ 1], sc[k ^ 1]);
-        const bool more2 = more && next_item(nn);
-        if (!ok) break;
-        const int rs2 = more2 ? row_slot(nn, nn.t) : -1;
-        const int ahead = row_slot(cur, cur.t + 3);
-        ok = wait(B_KVE + ring.slot, ring.par ^ 1u);
-        if (!ok) break;
-        uint8_t* tile = smem + Ly::kKvOff + ring.slot * Ly::kTileBytes;
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-          const int row = row0 + i * kRpi + lr;
-          uint4 o[2];
-          uint32_t b = sc[k][i];
-          if (cur.plane == 1 && b == 255u && cur.t * kTile + row > cur.lim_min) {
-            b = 127u;                            // its values are 0; the rows that see it get NaN at the end
-            *bad_v = 1;
-          }
-          widen16<BF16>(raw[k][i], b, o);
-          uint8_t* dst = tile + (row >> 3) * Ly::kGroupBytes + (lc >> 2) * 1024 + (row & 7) * 128;
-          // the lanes of a token's two halves write even and odd chunks first: eight banks' worth each time
-          const int c0 = (lc & 3) * 2, sw = D == 128 ? lc >> 2 : 0;
-          *reinterpret_cast<uint4*>(dst + (((c0 + sw) ^ (row & 7)) << 4)) = sw ? o[1] : o[0];
-          *reinterpret_cast<uint4*>(dst + (((c0 + 1 - sw) ^ (row & 7)) << 4)) = sw ? o[0] : o[1];
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(B_KVF + ring.slot));
-        ring.next(kSlots);
-        if (ahead >= 0)
-          asm volatile("prefetch.global.L2 [%0];" ::"l"(rows + cur.plane * a.kv_stride_kv + int64_t(ahead) * a.kv_stride_s +
-                                                        cur.h * D));
-        cur = nxt;
-        nxt = nn;
-        rs = rs2;
-        have = more;
-        more = more2;
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(bar(B_RE + in.slot));
+        mbar_arrive(bar(B_KVF + ring.slot));
       }
+      ring.next(kSlots);
+      in.next(Ly::kRaw);
     }
   }
   __syncthreads();
@@ -1223,7 +1284,7 @@ bool chunk_umma_supported(const ChunkArgs& a, int dtype, const char** why) {
   if (a.kv_stride_s * es % 16 || a.kv_stride_kv * es % 16 || a.q_stride_h % 8 || a.q_stride_t % 8 || a.kv_stride_s < 0 ||
       a.kv_stride_kv < 0 || a.q_stride_h < 0 || a.q_stride_t < 0)
     return no("strides of q and the cache must be multiples of 16 bytes");
-  if (int64_t(a.NB) * a.BS > 0x7fffffffll) return no("too many slots");
+  if (int64_t(a.NB) * a.BS > 0x7fffffffll || a.kv_stride_s > 0x7fffffffll) return no("too many slots, or too far apart");
   return true;
 }
 
@@ -1232,10 +1293,10 @@ namespace {
 template <int D, bool BF16, bool QUANT>
 cudaError_t launch_chunk_t(const CUtensorMap& mkv, const CUtensorMap& mq, const ChunkArgs& a, int grid, cudaStream_t st) {
   auto k = chunk::chunk_umma_kernel<D, BF16, QUANT>;
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(chunk::Layout<D>::kSmemBytes));
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(chunk::Layout<D, QUANT>::kSmemBytes));
   if (e != cudaSuccess) return e;
   const bool vec_out = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_stride_t % 8 == 0 && a.out_stride_h % 8 == 0;
-  k<<<grid, chunk::threads(QUANT), chunk::Layout<D>::kSmemBytes, st>>>(mkv, mq, a, vec_out);
+  k<<<grid, chunk::threads(QUANT), chunk::Layout<D, QUANT>::kSmemBytes, st>>>(mkv, mq, a, vec_out);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid, chunk::kJoinSlices);
@@ -1259,8 +1320,20 @@ cudaError_t launch_chunk_umma(const ChunkArgs& a, int dtype, cudaStream_t st, co
   }
   const CUtensorMapDataType dt = dtype == ACTKV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const cuuint32_t es[5] = {1, 1, 1, 1, 1};
-  CUtensorMap mkv = {}, mq;
-  if (!a.quant) {
+  CUtensorMap mkv, mq;
+  if (a.quant) {
+    // (the heads' values of a row, slot, plane): one head's values of a paged block per box
+    const cuuint32_t rows = cuuint32_t(a.BS < chunk::kTile ? a.BS : chunk::kTile);
+    const cuuint64_t dims[3] = {cuuint64_t(a.Hkv) * a.D, cuuint64_t(a.NB) * a.BS, 2};
+    const cuuint64_t strides[2] = {cuuint64_t(a.kv_stride_s), cuuint64_t(a.kv_stride_kv)};
+    const cuuint32_t box[3] = {cuuint32_t(a.D), rows, 1};
+    if (enc(&mkv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(a.kv), dims, strides, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, a.D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+      *why = "cuTensorMapEncodeTiled rejected the layout of the 8-bit rows";
+      return cudaErrorInvalidValue;
+    }
+  } else {
     // (64 dims, slot within 8, D-half of a head, group of 8 slots, plane): a box leaves every 8-token
     // group's D-halves next to one another, so the groups of a tile are evenly spaced
     const cuuint32_t halves = cuuint32_t(a.D / 64), rows = cuuint32_t(a.BS < chunk::kTile ? a.BS : chunk::kTile);
