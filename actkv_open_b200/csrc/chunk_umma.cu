@@ -29,6 +29,8 @@
 // (umma_common.cuh).
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "kernels.cuh"
 #include "umma_common.cuh"
@@ -431,17 +433,21 @@ template <bool BF16>
 __device__ __forceinline__ uint32_t plain_factor(uint32_t b) {
   return BF16 ? b * 0x00800080u + 0x3c003c00u : (b - 104u) * 0x04000400u;
 }
-// Any scale byte.
+// For any scale byte: the multiplier within the type, and a second one.
 template <bool BF16>
-__device__ __noinline__ void widen16_any(const uint4 raw, uint32_t b, uint32_t (&r)[8]) {
+__device__ __forceinline__ void any_factors(uint32_t b, uint32_t& f1, uint32_t& f2) {
   const int e = BF16 ? int(b) + 120 : int(b) - 104, top = BF16 ? 254 : 30;
   const int e1 = min(max(e, 1), top), e2 = min(max(e - e1 + (BF16 ? 127 : 15), 1), top);
   const uint32_t one = BF16 ? 0x00800080u : 0x04000400u;
-  widen16<BF16>(raw, b == 255u ? 0x7fff7fffu : e1 * one, r);                     // 255: NaN
+  f1 = b == 255u ? 0x7fff7fffu : e1 * one;   // 255: NaN
+  f2 = e2 * one;
+}
+template <bool BF16>
+__device__ __forceinline__ void widen16_rest(uint32_t b, uint32_t f2, uint32_t (&r)[8]) {
   if (b == 255u) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    r[i] = mul16x2<BF16>(r[i], e2 * one);
+    r[i] = mul16x2<BF16>(r[i], f2);
     if constexpr (!BF16) {
       asm("min.f16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(0x7bff7bffu));
       asm("max.f16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(0xfbfffbffu));
@@ -1177,20 +1183,32 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
       const uint8_t* src = smem + Ly::kRawOff + in.slot * Ly::kRawBytes + row0 * D;
       uint8_t* dst = smem + Ly::kKvOff + ring.slot * Ly::kTileBytes + (row0 >> 3) * Ly::kGroupBytes;
       const bool plain = __all_sync(full, plain_scales<BF16>(sc));
+      // Rolled, 8 tokens at a time: the warps of a scheduler are at five places of the kernel, and straight code
+      // for all 16 tokens starved it of instructions.
+      auto widen_all = [&](auto simple) {
+#pragma unroll 1
+        for (int g8 = 0; g8 < 2; ++g8) {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int g8 = i * kRpi / 8, i8 = i * kRpi % 8 / kRpi;
-        uint4 x = *reinterpret_cast<const uint4*>(src + g8 * 8 * D + get[i8]);
-        if (edge && first + i * kRpi + lr >= u.S) x = make_uint4(0u, 0u, 0u, 0u);
-        const uint32_t b = __byte_perm(__shfl_sync(full, sc, i * kRpi + lr), 0u, 0x4440 | (lc >> 1));
-        uint32_t r[8];
-        if (plain) widen16<BF16>(x, plain_factor<BF16>(b), r);
-        else widen16_any<BF16>(x, b, r);
-        *reinterpret_cast<uint4*>(dst + g8 * Ly::kGroupBytes + put0[i8]) =
-            sw ? make_uint4(r[4], r[5], r[6], r[7]) : make_uint4(r[0], r[1], r[2], r[3]);
-        *reinterpret_cast<uint4*>(dst + g8 * Ly::kGroupBytes + put1[i8]) =
-            sw ? make_uint4(r[0], r[1], r[2], r[3]) : make_uint4(r[4], r[5], r[6], r[7]);
-      }
+          for (int i = 0; i < 8 / kRpi; ++i) {
+            const int row = g8 * 8 + i * kRpi + lr;           // of the warp's 16
+            uint4 x = *reinterpret_cast<const uint4*>(src + get[i]);
+            if (!decltype(simple)::value && first + row >= u.S) x = make_uint4(0u, 0u, 0u, 0u);
+            const uint32_t b = __byte_perm(__shfl_sync(full, sc, row), 0u, 0x4440 | (lc >> 1));
+            uint32_t r[8], f1 = plain_factor<BF16>(b), f2 = 0;
+            if (!decltype(simple)::value) any_factors<BF16>(b, f1, f2);
+            widen16<BF16>(x, f1, r);
+            if (!decltype(simple)::value) widen16_rest<BF16>(b, f2, r);
+            *reinterpret_cast<uint4*>(dst + put0[i]) =
+                sw ? make_uint4(r[4], r[5], r[6], r[7]) : make_uint4(r[0], r[1], r[2], r[3]);
+            *reinterpret_cast<uint4*>(dst + put1[i]) =
+                sw ? make_uint4(r[0], r[1], r[2], r[3]) : make_uint4(r[4], r[5], r[6], r[7]);
+          }
+          src += 8 * D;
+          dst += Ly::kGroupBytes;
+        }
+      };
+      if (plain && !edge) widen_all(std::true_type());
+      else widen_all(std::false_type());
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) {
