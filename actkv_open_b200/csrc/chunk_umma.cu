@@ -29,8 +29,6 @@
 // (umma_common.cuh).
 #include <cuda.h>
 
-#include <type_traits>
-
 #include "common.cuh"
 #include "kernels.cuh"
 #include "umma_common.cuh"
@@ -326,6 +324,35 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return r;
 }
 
+// The waits of this kernel, bounded like mbar_wait's but shorter: the kernel's roles share an instruction
+// cache, which the waits' slow paths filled.  false when the wait gave up (about 2^31 cycles; *abort is
+// then 1, and the kernel reports it at its end) or another role did.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, uint32_t abort) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 t0, t1;\n\t.reg .b32 a;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra done;\n\t"
+      "mov.u64 t0, %%clock64;\n"
+      "again:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %4;\n\t"
+      "@p bra done;\n\t"
+      "ld.volatile.shared.b32 a, [%3];\n\t"
+      "setp.ne.b32 q, a, 0;\n\t"
+      "@q bra done;\n\t"
+      "mov.u64 t1, %%clock64;\n\t"
+      "sub.s64 t1, t1, t0;\n\t"
+      "setp.lt.s64 q, t1, %5;\n\t"
+      "@q bra again;\n\t"
+      "st.volatile.shared.b32 [%3], 1;\n"
+      "done:\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "r"(abort), "r"(kSleepNs), "l"(kTimeoutCycles)
+      : "memory");
+  return ok != 0;
+}
+
 // A slot of the K / V ring and the parity of its current use.
 struct Ring {
   uint32_t slot = 0, par = 0;
@@ -461,7 +488,7 @@ template <int D, bool BF16>
 __device__ __forceinline__ void clean_values(uint8_t* tile, bool past, bool hidden, volatile int* bad_v) {
   constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
   if (!past && !hidden) return;
-#pragma unroll
+#pragma unroll 1
   for (int k = 0; k < D / 8; ++k) {
     uint4* p = reinterpret_cast<uint4*>(tile + (k >> 3) * 1024) + (k & 7);
     if (past) {
@@ -500,6 +527,7 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Ly::kBarOff);
   Sched& sched = *reinterpret_cast<Sched*>(smem + Ly::kSchedOff);
   volatile int* abort_flag = &sched.abort_flag;
+  const uint32_t abort_addr = smem_u32(&sched.abort_flag);
   volatile int* bad_v = &sched.bad_v;
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
   constexpr int kSlots = Ly::kSlots;
@@ -573,6 +601,7 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
     }
     const int bs_box = min(a.BS, kTile);         // token rows of a box
     const int bpt = kTile / bs_box;              // boxes per tile (<= 16: one per lane)
+    const int mpb = a.BS / bs_box;               // tiles per block, of blocks longer than a tile
     const uint32_t box_bytes = uint32_t(bs_box) * D * (QUANT ? 1 : 2);
     // where the copies go: the ring itself, or the tiles to be widened into it
     constexpr int kIn = QUANT ? Ly::kRaw : kSlots, B_FULL = QUANT ? B_RF : B_KVF, B_EMPTY = QUANT ? B_RE : B_KVE;
@@ -582,7 +611,7 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
     bool ok = true;
     for (uint32_t n = 0;; ++n) {
       const bool any = wk.next(x);
-      ok = __all_sync(full, mbar_wait(bar(B_UE + n % kUnitSlots), ((n / kUnitSlots) & 1u) ^ 1u, abort_flag, a.status));
+      ok = __all_sync(full, bar_wait(bar(B_UE + n % kUnitSlots), ((n / kUnitSlots) & 1u) ^ 1u, abort_addr));
       if (!ok) break;
       if (lane == 0) {
         if (!any) x.r = -1;
@@ -594,18 +623,17 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
       const int lead = x.two ? 1 : 2, nt = x.t1 - x.t0;
       // first token slot (16-bit rows: in units of 8) of lane b's box of key tile t; -2 past the session's end
       auto read_id = [&](int t) -> int {
-        const int tok = t * kTile + lane * bs_box;
-        if (lane >= bpt || t >= x.t1 || tok >= x.S) return -2;
-        const int lb = tok / a.BS;
+        if (lane >= bpt || t < x.t0 || t >= x.t1 || t * kTile + lane * bs_box >= x.S) return -2;
+        const int lb = mpb == 1 ? t * bpt + lane : t / mpb;
         const int phys = lb < a.MB ? a.block_table[x.r * a.bt_stride_r + lb] : -1;
         if (phys < 0 || phys >= a.NB) {
           flag(a.status, ACTKV_DEV_BAD_INDEX);
           return 0;
         }
-        return int((int64_t(phys) * a.BS + (tok - lb * a.BS)) >> (QUANT ? 0 : 3));
+        const int64_t first = int64_t(phys) * a.BS + (mpb == 1 ? 0 : (t - lb * mpb) * kTile);
+        return int(first >> (QUANT ? 0 : 3));
       };
-      int id0 = read_id(x.t0), id1 = read_id(x.t0 + 1), id2 = read_id(x.t0 + 2);
-      ok = __all_sync(full, mbar_wait(bar(B_QE), (q_uses & 1u) ^ 1u, abort_flag, a.status));
+      ok = __all_sync(full, bar_wait(bar(B_QE), (q_uses & 1u) ^ 1u, abort_addr));
       if (!ok) break;
       if (lane == 0) {
         const int blocks = x.two ? 2 : 1;
@@ -616,9 +644,9 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
                         x.a0 + x.j0 + b * tpb);
       }
       ++q_uses;
-      auto load = [&](int t, int id, int plane) -> bool {
+      auto load = [&](int id, int plane) -> bool {
         const int slot = ring % kIn;
-        const bool w2 = mbar_wait(bar(B_EMPTY + slot), ((ring / kIn) & 1u) ^ 1u, abort_flag, a.status);
+        const bool w2 = bar_wait(bar(B_EMPTY + slot), ((ring / kIn) & 1u) ^ 1u, abort_addr);
         if (!__all_sync(full, w2)) return false;
         const int n = __popc(__ballot_sync(full, id >= 0));
         if (lane == 0) mbar_expect_tx(bar(B_FULL + slot), uint32_t(n) * box_bytes);
@@ -634,15 +662,15 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
         ++ring;
         return true;
       };
-      ok = load(x.t0, id0, 0);
-      if (ok && lead == 2 && nt > 1) ok = load(x.t0 + 1, id1, 0);
-      for (int t = 0; ok && t < nt; ++t) {
-        const int id3 = read_id(x.t0 + t + 3);
-        ok = load(x.t0 + t, id0, 1);
-        if (ok && t + lead < nt) ok = load(x.t0 + t + lead, lead == 1 ? id1 : id2, 0);
+      // keys `lead` tiles ahead of the values; block ids three tiles ahead of the values
+      int id0 = -2, id1 = -2, id2 = -2;
+#pragma unroll 1
+      for (int t = -lead - 3; ok && t < nt; ++t) {
+        if (t >= 0) ok = load(id0, 1);
+        if (ok && t >= -lead && t + lead < nt) ok = load(lead == 1 ? id1 : id2, 0);
         id0 = id1;
         id1 = id2;
-        id2 = id3;
+        id2 = read_id(x.t0 + t + 3);
       }
       if (!ok) break;
     }
@@ -670,7 +698,7 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
     uint32_t last_par = 0;
     bool ok = true;
     auto wait = [&](int b, uint32_t par) -> bool {
-      return __all_sync(full, mbar_wait(bar(b), par, abort_flag, a.status));
+      return __all_sync(full, bar_wait(bar(b), par, abort_addr));
     };
     auto commit = [&](int b) {
       if (leader) mma_commit(bar(b));
@@ -730,58 +758,36 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
       ok = wait(B_QF, q_uses & 1u);
       if (!ok) break;
       ++q_uses;
-      if (two) {
-        ok = kv_wait(ring);
-        if (!ok) break;
-        issue_s(0, 0, ring.slot);
-        issue_s(1, 1, ring.slot);
-        commit(B_KVE + ring.slot);
-        ring.next(kSlots);
-        if (nt == 1) commit(B_QE);
-        for (int i = 0; ok && i < nt; ++i) {
-          const Ring v = ring;
-          ring.next(kSlots);
-          const Ring k = ring;
-          const bool more = i + 1 < nt;
-          if (more) ring.next(kSlots);
-          ok = kv_wait(v) && issue_o(0, v.slot, i == 0);
+      // Step by step: the second product of step s, then the logits of step s + 2 of the same stream.  Two row
+      // tiles take every key tile in a step each; one row tile takes a key tile per step.
+      const int steps = two ? 2 * nt : nt;
+      Ring v, k;
+#pragma unroll 1
+      for (int s = -2; s < steps; ++s) {
+        const int w = s & 1;
+        const bool opens = !two || w == 0, closes = !two || w == 1, more = s + 2 < steps;
+        if (s >= 0) {
+          if (opens) {
+            v = ring;
+            ring.next(kSlots);
+            ok = kv_wait(v);
+          }
+          ok = ok && issue_o(w, v.slot, s < 2);
           if (!ok) break;
-          if (more) {
+          if (closes) commit(B_KVE + v.slot);
+        }
+        if (more) {
+          if (opens) {
+            k = ring;
+            ring.next(kSlots);
             ok = kv_wait(k);
             if (!ok) break;
-            issue_s(0, 0, k.slot);
-          } else {
-            finish_o(0);
           }
-          ok = issue_o(1, v.slot, i == 0);
-          if (!ok) break;
-          commit(B_KVE + v.slot);
-          if (more) {
-            issue_s(1, 1, k.slot);
-            commit(B_KVE + k.slot);
-            if (i + 2 == nt) commit(B_QE);
-          } else {
-            finish_o(1);
-          }
-        }
-      } else {
-        // ring order: keys 0, 1, then values t and keys t + 2 in turn
-        auto key = [&](int t) -> bool {
-          if (!kv_wait(ring)) return false;
-          issue_s(t & 1, 0, ring.slot);
-          commit(B_KVE + ring.slot);
-          ring.next(kSlots);
-          if (t + 1 == nt) commit(B_QE);
-          return true;
-        };
-        ok = key(0) && (nt == 1 || key(1));
-        for (int t = 0; ok && t < nt; ++t) {
-          ok = kv_wait(ring) && issue_o(t & 1, ring.slot, t < 2);
-          if (!ok) break;
-          commit(B_KVE + ring.slot);
-          ring.next(kSlots);
-          if (t + 2 < nt) ok = key(t + 2);
-          else finish_o(t & 1);
+          issue_s(w, two ? w : 0, k.slot);
+          if (closes) commit(B_KVE + k.slot);
+          if (s + 3 == steps) commit(B_QE);
+        } else if (s >= 0) {
+          finish_o(w);
         }
       }
     }
@@ -789,66 +795,62 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
   } else if (QUANT && warp == 2) {
     // ------------------------------------------------------------------ scale words of the 8-bit rows
     // Four tokens per lane, from the cache through registers (one tile ahead) into the tile's words.
-    const int bpt = a.BS < kTile ? kTile / a.BS : 0, mpb = a.BS < kTile ? 1 : a.BS / kTile;
+    const int bpt = a.BS < kTile ? kTile / a.BS : 1, mpb = a.BS < kTile ? 1 : a.BS / kTile;
     int sub[4], in_block[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      sub[i] = bpt ? (lane + 32 * i) / a.BS : 0;
+      sub[i] = mpb == 1 ? (lane + 32 * i) / a.BS : 0;
       in_block[i] = lane + 32 * i - sub[i] * a.BS;
     }
     UnitItems u;
-    uint32_t n = 0;
-    bool ok = true, have = true;
+    uint32_t n = 0, w0[4] = {}, w1[4] = {};
+    Ring ring;
+    bool have = false, more = true;
     auto wait = [&](int b, uint32_t par) -> bool {
-      return __all_sync(full, mbar_wait(bar(b), par, abort_flag, a.status));
+      return __all_sync(full, bar_wait(bar(b), par, abort_addr));
     };
-    auto read_words = [&](uint32_t (&word)[4]) -> bool {      // of the next tile; false at the end
-      while (u.done()) {
+    while (have || more) {
+      while (more && u.done()) {
         const uint32_t slot = n % kUnitSlots;
-        if (!wait(B_UF + slot, (n / kUnitSlots) & 1u)) {
-          ok = false;
-          return false;
-        }
+        more = wait(B_UF + slot, (n / kUnitSlots) & 1u);
+        if (!more) break;
         u.start(sched.units[slot]);
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(B_UE + slot));
         ++n;
-        if (u.r < 0) return false;
+        more = u.r >= 0;
       }
-      int t, plane;
-      u.next(t, plane);
-      const int32_t* table = a.block_table + u.r * a.bt_stride_r;
-      int phys[4];
+      if (more) {
+        int t, plane;
+        u.next(t, plane);
+        const int block0 = mpb == 1 ? t * bpt : t / mpb, off = mpb == 1 ? 0 : (t - block0 * mpb) * kTile;
+        const int32_t* table = a.block_table + u.r * a.bt_stride_r;
+        const uint8_t* p0 = static_cast<const uint8_t*>(a.kv) + plane * a.kv_stride_kv + a.Hkv * D + u.h * (D / 32);
+        int phys[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int lb = bpt ? t * bpt + sub[i] : t / mpb;
-        phys[i] = t * kTile + lane + 32 * i < u.S && lb < a.MB ? table[lb] : 0;
-      }
-      const uint8_t* p0 = static_cast<const uint8_t*>(a.kv) + plane * a.kv_stride_kv + a.Hkv * D + u.h * (D / 32);
+        for (int i = 0; i < 4; ++i) {
+          const int lb = block0 + sub[i];
+          phys[i] = t * kTile + lane + 32 * i < u.S && lb < a.MB ? table[lb] : 0;
+        }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int ph = phys[i] < 0 || phys[i] >= a.NB ? 0 : phys[i];          // flagged by the TMA warp
-        const uint8_t* p = p0 + (int64_t(ph) * a.BS + in_block[i] + (bpt ? 0 : t % mpb * kTile)) * a.kv_stride_s;
-        if constexpr (D == 128) word[i] = *reinterpret_cast<const uint32_t*>(p);
-        else word[i] = *reinterpret_cast<const uint16_t*>(p) | 0x7f7f0000u;
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t ph = phys[i] < 0 || phys[i] >= a.NB ? 0 : phys[i];   // flagged by the TMA warp
+          const uint8_t* p = p0 + uint64_t(ph * uint32_t(a.BS) + uint32_t(in_block[i] + off)) * uint32_t(a.kv_stride_s);
+          if constexpr (D == 128) w1[i] = *reinterpret_cast<const uint32_t*>(p);
+          else w1[i] = *reinterpret_cast<const uint16_t*>(p) | 0x7f7f0000u;
+        }
       }
-      return true;
-    };
-    uint32_t w0[4], w1[4];
-    Ring ring;
-    have = read_words(w0);
-    while (have && ok) {
-      const bool more = read_words(w1);
-      if (!ok || !wait(B_RE + ring.slot, ring.par ^ 1u)) break;
-      uint32_t* dst = reinterpret_cast<uint32_t*>(smem + Ly::kScaleOff) + ring.slot * kTile;
+      if (have) {
+        if (!wait(B_RE + ring.slot, ring.par ^ 1u)) break;
+        uint32_t* dst = reinterpret_cast<uint32_t*>(smem + Ly::kScaleOff) + ring.slot * kTile;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        dst[lane + 32 * i] = w0[i];
-        w0[i] = w1[i];
+        for (int i = 0; i < 4; ++i) dst[lane + 32 * i] = w0[i];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_CF + ring.slot));
+        ring.next(Ly::kRaw);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(B_CF + ring.slot));
-      ring.next(Ly::kRaw);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w0[i] = w1[i];
       have = more;
     }
   }
@@ -868,7 +870,7 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
     const int jr = row / a.G, g = row - jr * a.G;             // token of the tile, head of the group
     uint32_t it = 0, ring = 0, o_uses[2] = {0, 0}, x_uses = 0;
     auto wait = [&](int b, uint32_t par) -> bool {
-      return __all_sync(full, mbar_wait(bar(b), par, abort_flag, a.status));
+      return __all_sync(full, bar_wait(bar(b), par, abort_addr));
     };
     bool ok = true;
     for (uint32_t n = 0; ok; ++n) {
@@ -913,11 +915,19 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
           const bool masked = !__all_sync(full, tok0 + kTile - 1 <= lim);
           const int last = lim - tok0;                        // columns 0 .. last are seen
           float mx[4] = {ninf, ninf, ninf, ninf};
-          auto half_max = [&](float (&x)[64], int hf) {
-            if (masked) {
+          if (masked) {                                       // hidden columns become -inf where they are
+#pragma unroll 1
+            for (int q = 0; q < 8; ++q) {
+              if (__all_sync(full, q * 16 + 15 <= last)) continue;
+              float x[16];
+              tmem_ld16(s_addr + q * 16, x);
 #pragma unroll
-              for (int k = 0; k < 64; ++k) x[k] = hf * 64 + k <= last ? x[k] : ninf;
+              for (int k = 0; k < 16; ++k) x[k] = q * 16 + k <= last ? x[k] : ninf;
+              tmem_st16(s_addr + q * 16, reinterpret_cast<uint32_t*>(x));
             }
+            tmem_wait_st();
+          }
+          auto half_max = [&](float (&x)[64]) {
 #pragma unroll
             for (int k = 0; k < 64; k += 8)
 #pragma unroll
@@ -926,17 +936,17 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
           if constexpr (QUANT) {
             tmem_ld64(s_addr + 64, v[0]);
             tmem_wait(v[0]);
-            half_max(v[0], 1);
+            half_max(v[0]);
             tmem_ld64(s_addr, v[0]);
             tmem_wait(v[0]);
-            half_max(v[0], 0);
+            half_max(v[0]);
           } else {
             tmem_ld64(s_addr, v[0]);
             tmem_ld64(s_addr + 64, v[QUANT ? 0 : 1]);
             tmem_wait(v[0]);
             tmem_wait(v[QUANT ? 0 : 1]);
-            half_max(v[0], 0);
-            half_max(v[QUANT ? 0 : 1], 1);
+            half_max(v[0]);
+            half_max(v[QUANT ? 0 : 1]);
           }
           const float top = fmax3(fmaxf(mx[0], mx[1]), mx[2], mx[3]) * c2;
           const bool raise = top > m + kSlack;                // also when m is still -inf
@@ -966,10 +976,6 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
             if (QUANT && q == 2) {
               tmem_ld64(s_addr + 64, v[0]);
               tmem_wait(v[0]);
-              if (masked) {
-#pragma unroll
-                for (int k = 0; k < 64; ++k) v[0][k] = 64 + k <= last ? v[0][k] : ninf;
-              }
             }
             uint32_t u[16];
 #pragma unroll
@@ -1055,27 +1061,6 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
                 for (int k = 0; k < 32; ++k) o[k] = fmaf(o[k], al0, o1[k] * al1);
               }
             }
-            if (fix && put) {
-              const int first = max(lim_min + 1, x.t0 * kTile), last = min(lim, x.t1 * kTile - 1);
-              for (int t = first; t <= last; ++t) {
-                const int lb = t / a.BS;
-                const int phys = lb < a.MB ? a.block_table[x.r * a.bt_stride_r + lb] : -1;
-                if (phys < 0 || phys >= a.NB) continue;
-                const int64_t at = a.kv_stride_kv + int64_t(phys) * a.kv_stride_b + int64_t(t - lb * a.BS) * a.kv_stride_s;
-                if constexpr (QUANT) {           // 32 values share a scale byte; 255 makes them NaN
-                  if (static_cast<const uint8_t*>(a.kv)[at + a.Hkv * D + x.h * (D / 32) + q] == 255)
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) o[k] = __int_as_float(0x7fffffff);
-                } else {
-                  const uint16_t* vr = static_cast<const uint16_t*>(a.kv) + at + int64_t(x.h) * a.kv_stride_h + q * 32;
-#pragma unroll
-                  for (int k = 0; k < 32; ++k) {
-                    const float f = BF16 ? __uint_as_float(uint32_t(vr[k]) << 16) : __half2float(__ushort_as_half(vr[k]));
-                    if (!isfinite(f)) o[k] += f;
-                  }
-                }
-              }
-            }
             if (put) {
               if (whole) {
                 store_row<D, BF16>(static_cast<uint16_t*>(a.out) + qt * a.out_stride_t + int64_t(hq) * a.out_stride_h + q * 32,
@@ -1084,6 +1069,36 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
 #pragma unroll
                 for (int k = 0; k < 32; k += 4)
                   *reinterpret_cast<float4*>(part + int64_t(pr) * D + q * 32 + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+              }
+            }
+          }
+        }
+        // values that some row does not see and that are not finite went in as zeros: the rows that do see them
+        if (fix && put) {
+          uint16_t* dst = static_cast<uint16_t*>(a.out) + qt * a.out_stride_t + int64_t(hq) * a.out_stride_h;
+          const int first = max(lim_min + 1, x.t0 * kTile), end = min(lim, x.t1 * kTile - 1);
+#pragma unroll 1
+          for (int t = first; t <= end; ++t) {
+            const int lb = t / a.BS;
+            const int phys = lb < a.MB ? a.block_table[x.r * a.bt_stride_r + lb] : -1;
+            if (phys < 0 || phys >= a.NB) continue;
+            const int64_t at = a.kv_stride_kv + int64_t(phys) * a.kv_stride_b + int64_t(t - lb * a.BS) * a.kv_stride_s;
+#pragma unroll 1
+            for (int d = 0; d < D; ++d) {
+              float f;
+              if constexpr (QUANT) {             // 32 values share a scale byte; 255 makes them NaN
+                f = static_cast<const uint8_t*>(a.kv)[at + a.Hkv * D + x.h * (D / 32) + d / 32] == 255
+                        ? __int_as_float(0x7fffffff) : 0.0f;
+              } else {
+                const uint16_t u = static_cast<const uint16_t*>(a.kv)[at + int64_t(x.h) * a.kv_stride_h + d];
+                f = BF16 ? __uint_as_float(uint32_t(u) << 16) : __half2float(__ushort_as_half(u));
+              }
+              if (isfinite(f)) continue;
+              if (whole) {
+                const float y = BF16 ? __uint_as_float(uint32_t(dst[d]) << 16) : __half2float(__ushort_as_half(dst[d]));
+                dst[d] = uint16_t(pack2<BF16>(y + f, 0.0f));
+              } else {
+                part[int64_t(pr) * D + d] += f;
               }
             }
           }
@@ -1131,7 +1146,7 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
     // A warp takes 16 of a tile's tokens, D / 16 lanes per token, and leaves them in the ring in the layout
     // the TMA leaves 16-bit rows in.
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    constexpr int kLpr = D / 16, kRpi = 32 / kLpr, kLoads = 16 / kRpi;
+    constexpr int kLpr = D / 16, kRpi = 32 / kLpr;
     const int row0 = (warp - 12) * 16, lr = lane / kLpr, lc = lane % kLpr;
     // Where a lane's piece comes from and its two 16-byte pieces go within 8 tokens.  The lanes of a token's two
     // halves write even and odd chunks first: eight banks' worth each time.
@@ -1144,12 +1159,16 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
       put0[i] = (lc >> 2) * 1024 + r8 * 128 + (((c0 + sw) ^ r8) << 4);
       put1[i] = (lc >> 2) * 1024 + r8 * 128 + (((c0 + 1 - sw) ^ r8) << 4);
     }
+    auto put = [&](uint8_t* p0, uint8_t* p1, const uint32_t (&r)[8]) {
+      *reinterpret_cast<uint4*>(p0) = sw ? make_uint4(r[4], r[5], r[6], r[7]) : make_uint4(r[0], r[1], r[2], r[3]);
+      *reinterpret_cast<uint4*>(p1) = sw ? make_uint4(r[0], r[1], r[2], r[3]) : make_uint4(r[4], r[5], r[6], r[7]);
+    };
     UnitItems u;
     Ring ring, in;
     uint32_t n = 0;
     bool ok = true;
     auto wait = [&](int b, uint32_t par) -> bool {
-      return __all_sync(full, mbar_wait(bar(b), par, abort_flag, a.status));
+      return __all_sync(full, bar_wait(bar(b), par, abort_addr));
     };
     while (true) {
       while (ok && u.done()) {
@@ -1185,30 +1204,36 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
       const bool plain = __all_sync(full, plain_scales<BF16>(sc));
       // Rolled, 8 tokens at a time: the warps of a scheduler are at five places of the kernel, and straight code
       // for all 16 tokens starved it of instructions.
-      auto widen_all = [&](auto simple) {
+      if (plain && !edge) {
 #pragma unroll 1
         for (int g8 = 0; g8 < 2; ++g8) {
 #pragma unroll
           for (int i = 0; i < 8 / kRpi; ++i) {
-            const int row = g8 * 8 + i * kRpi + lr;           // of the warp's 16
-            uint4 x = *reinterpret_cast<const uint4*>(src + get[i]);
-            if (!decltype(simple)::value && first + row >= u.S) x = make_uint4(0u, 0u, 0u, 0u);
-            const uint32_t b = __byte_perm(__shfl_sync(full, sc, row), 0u, 0x4440 | (lc >> 1));
-            uint32_t r[8], f1 = plain_factor<BF16>(b), f2 = 0;
-            if (!decltype(simple)::value) any_factors<BF16>(b, f1, f2);
-            widen16<BF16>(x, f1, r);
-            if (!decltype(simple)::value) widen16_rest<BF16>(b, f2, r);
-            *reinterpret_cast<uint4*>(dst + put0[i]) =
-                sw ? make_uint4(r[4], r[5], r[6], r[7]) : make_uint4(r[0], r[1], r[2], r[3]);
-            *reinterpret_cast<uint4*>(dst + put1[i]) =
-                sw ? make_uint4(r[0], r[1], r[2], r[3]) : make_uint4(r[4], r[5], r[6], r[7]);
+            const uint4 x = *reinterpret_cast<const uint4*>(src + get[i]);
+            const uint32_t b = __byte_perm(__shfl_sync(full, sc, g8 * 8 + i * kRpi + lr), 0u, 0x4440 | (lc >> 1));
+            uint32_t r[8];
+            widen16<BF16>(x, plain_factor<BF16>(b), r);
+            put(dst + put0[i], dst + put1[i], r);
           }
           src += 8 * D;
           dst += Ly::kGroupBytes;
         }
-      };
-      if (plain && !edge) widen_all(std::true_type());
-      else widen_all(std::false_type());
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < 16 / kRpi; ++i) {
+          const int row = i * kRpi + lr, g8 = i * kRpi / 8;     // of the warp's 16
+          const bool odd = i * kRpi % 8 != 0;
+          uint4 x = *reinterpret_cast<const uint4*>(src + g8 * 8 * D + (odd ? get[8 / kRpi - 1] : get[0]));
+          if (first + row >= u.S) x = make_uint4(0u, 0u, 0u, 0u);
+          const uint32_t b = __byte_perm(__shfl_sync(full, sc, row), 0u, 0x4440 | (lc >> 1));
+          uint32_t r[8], f1, f2;
+          any_factors<BF16>(b, f1, f2);
+          widen16<BF16>(x, f1, r);
+          widen16_rest<BF16>(b, f2, r);
+          uint8_t* d8 = dst + g8 * Ly::kGroupBytes;
+          put(d8 + (odd ? put0[8 / kRpi - 1] : put0[0]), d8 + (odd ? put1[8 / kRpi - 1] : put1[0]), r);
+        }
+      }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) {
@@ -1220,6 +1245,7 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
     }
   }
   __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag) flag(a.status, ACTKV_DEV_TIMEOUT);
   if (warp == 1) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
