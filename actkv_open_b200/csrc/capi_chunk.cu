@@ -105,7 +105,7 @@ int actkv_chunk_attention(const void* q, int dtype, int64_t q_stride_t, int64_t 
                           int path, void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
   ChunkArgs a{q,   q_stride_t,   q_stride_h,   q_off, kv,           kv_stride_kv, kv_stride_b, kv_stride_s,
               kv_stride_h, block_table, bt_stride_r, seq_used, out, out_stride_t, out_stride_h, lse,
-              lse_stride_t, T, R, MB, NB, BS, Hq, Hkv, 0, D, false, scale, workspace, status};
+              lse_stride_t, T, R, MB, NB, BS, Hq, Hkv, 0, D, false, scale, workspace, status, 0};
   return chunk_attention(a, dtype, path, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
@@ -118,7 +118,7 @@ int actkv_chunk_attention_quant(const void* q, int dtype, int64_t q_stride_t, in
                                 int32_t* status, void* stream) {
   ChunkArgs a{q,   q_stride_t,   q_stride_h,   q_off, rows, rows_stride_kv_bytes, rows_stride_b_bytes, rows_stride_s_bytes,
               0, block_table, bt_stride_r, seq_used, out, out_stride_t, out_stride_h, lse,
-              lse_stride_t, T, R, MB, NB, BS, Hq, Hkv, 0, D, true, scale, workspace, status};
+              lse_stride_t, T, R, MB, NB, BS, Hq, Hkv, 0, D, true, scale, workspace, status, 0};
   return chunk_attention(a, dtype, path, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 

@@ -1,0 +1,167 @@
+// What the two tensor-core kernels of chunk attention share (chunk_umma.cu, chunk_few.cu): the shares of
+// work, the partial results that a cut unit leaves, and 16-bit values from 8-bit rows.
+#pragma once
+
+#include "common.cuh"
+#include "kernels.cuh"
+#include "umma_common.cuh"
+
+namespace actkv {
+namespace chunk {
+
+using namespace umma;
+
+constexpr int kRows = 128;                  // query rows per row tile (MMA M)
+constexpr int kTile = 128;                  // tokens per key tile, the grain of the schedule
+constexpr int kFewRows = 16;                // query rows of a session and KV head that chunk_few_kernel takes
+constexpr int kUnitCost = 2;                // a unit's fixed cost (queries in, results out) in key tiles
+constexpr float kSlack = 8.0f;              // log2 units the maximum may outgrow m by
+constexpr int kMaxD = 128;
+
+// ------------------------------------------------------------------------------------ shares of work
+struct Share {
+  int64_t total, pre;        // all weight, weight before session r0
+  int r0;                    // the session that holds the CTA's first unit of weight
+};
+
+// CTA `cta` of n takes the weight [total * cta / n, total * (cta + 1) / n), sessions in order.  Every thread
+// of the block calls it; `s` starts as {0, 0, R}.
+template <int kThreads, typename Weight>
+__device__ __forceinline__ void share_out(int R, Weight weight, Share& s, int64_t* scan, int cta, int n) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // pass 0 adds the weights up, pass 1 finds the session (only when a pass over all does not fit)
+  int64_t lo = 0;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    int64_t carry = 0;
+#pragma unroll 1
+    for (int base = 0; base < R; base += kThreads) {
+      const int r = base + int(threadIdx.x);
+      const int64_t w = r < R ? weight(r) : 0;
+      int64_t incl = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+      }
+      if (lane == 31) scan[warp] = incl;
+      __syncthreads();
+      int64_t before = carry, all = carry;
+      for (int i = 0; i < kThreads / 32; ++i) {
+        if (i < warp) before += scan[i];
+        all += scan[i];
+      }
+      __syncthreads();
+      if (pass == 0 && base + kThreads >= R) {              // the last step: the total is known
+        if (threadIdx.x == 0) s.total = all;
+        lo = all * cta / n;
+      }
+      const int64_t excl = before + incl - w;
+      if ((pass == 1 || R <= kThreads) && w > 0 && lo >= excl && lo < excl + w) {
+        s.r0 = r;
+        s.pre = excl;
+      }
+      carry = all;
+    }
+    if (R <= kThreads) break;
+  }
+  __syncthreads();
+}
+
+// ------------------------------------------------------------------------------------ partial results
+struct Desc {                // the unit that a CTA began and left to the next ones
+  int32_t valid, r, h, j0, ntok, S, A, a0;
+  int64_t end, total;
+  int32_t two, pad[3];
+};
+static_assert(sizeof(Desc) == 64, "the partial results after the descriptors are 16-byte aligned");
+
+
+// The workspace of one kernel: a descriptor per CTA, then two partial results per CTA (slot 0: of a unit begun
+// by an earlier CTA, 1: of one left to the next), each `rows` rows of D values and (m, l) per row.
+struct Parts {
+  Desc* desc;
+  float* base;
+  int rows;
+  __device__ __forceinline__ float* out(int cta, int slot) const {
+    return base + (int64_t(cta) * 2 + slot) * rows * (kMaxD + 2);
+  }
+  __device__ __forceinline__ float* ml(int cta, int slot, int D) const { return out(cta, slot) + int64_t(rows) * D; }
+};
+__host__ __device__ inline size_t parts_bytes(int n_cta, int rows) {
+  return size_t(n_cta) * (sizeof(Desc) + size_t(2) * rows * (kMaxD + 2) * sizeof(float));
+}
+__host__ __device__ inline size_t few_offset(int n_cta) { return (parts_bytes(n_cta, 2 * kRows) + 255) & ~size_t(255); }
+__device__ __forceinline__ Parts parts_at(void* ws, size_t off, int n_cta, int rows) {
+  char* p = static_cast<char*>(ws) + off;
+  return Parts{reinterpret_cast<Desc*>(p), reinterpret_cast<float*>(p + int64_t(n_cta) * sizeof(Desc)), rows};
+}
+__device__ __forceinline__ Parts wide_parts(void* ws, int n_cta) { return parts_at(ws, 0, n_cta, 2 * kRows); }
+__device__ __forceinline__ Parts few_parts(void* ws, int n_cta) { return parts_at(ws, few_offset(n_cta), n_cta, kFewRows); }
+
+// ------------------------------------------------------------------------------------ 16-bit values
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  uint32_t r;
+  if constexpr (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// 16 e4m3 values with scale byte b as 16-bit values.  The four exponent and three mantissa bits of a
+// byte, moved under the wider type's exponent, read as the value times 2^-120 (bf16) or 2^-8 (fp16),
+// subnormals included, so one multiplication by a power of two, 2^(b - 127) with that put right, gives
+// the value exactly; a power of two outside the type takes a second one.  fp16 values past its range
+// become its largest.
+template <bool BF16>
+__device__ __forceinline__ uint32_t mul16x2(uint32_t x, uint32_t f) {
+  uint32_t r;
+  if constexpr (BF16) asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(f));
+  else asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(f));
+  return r;
+}
+// Whether one multiplication does for every byte of a word of scale bytes.
+template <bool BF16>
+__device__ __forceinline__ bool plain_scales(uint32_t w) {
+  return __vcmpgtu4(w, 0x86868686u) == 0 && (BF16 || __vcmpgtu4(0x69696969u, w) == 0);   // <= 134 (fp16: >= 105)
+}
+template <bool BF16>
+__device__ __forceinline__ void widen16(const uint4& raw, uint32_t f, uint32_t (&r)[8]) {
+  const uint32_t in[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t x = __byte_perm(in[i >> 1], 0u, (i & 1) ? 0x3424 : 0x1404);   // two bytes, each atop a half
+    const uint32_t y = ((x >> (BF16 ? 4 : 1)) & (BF16 ? 0x07f007f0u : 0x3f803f80u)) | (x & 0x80008000u);
+    r[i] = mul16x2<BF16>(y, f);
+  }
+}
+// The multiplier of scale byte b, in both halves, where plain_scales holds.
+template <bool BF16>
+__device__ __forceinline__ uint32_t plain_factor(uint32_t b) {
+  return BF16 ? b * 0x00800080u + 0x3c003c00u : (b - 104u) * 0x04000400u;
+}
+// For any scale byte: the multiplier within the type, and a second one.
+template <bool BF16>
+__device__ __forceinline__ void any_factors(uint32_t b, uint32_t& f1, uint32_t& f2) {
+  const int e = BF16 ? int(b) + 120 : int(b) - 104, top = BF16 ? 254 : 30;
+  const int e1 = min(max(e, 1), top), e2 = min(max(e - e1 + (BF16 ? 127 : 15), 1), top);
+  const uint32_t one = BF16 ? 0x00800080u : 0x04000400u;
+  f1 = b == 255u ? 0x7fff7fffu : e1 * one;   // 255: NaN
+  f2 = e2 * one;
+}
+template <bool BF16>
+__device__ __forceinline__ void widen16_rest(uint32_t b, uint32_t f2, uint32_t (&r)[8]) {
+  if (b == 255u) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    r[i] = mul16x2<BF16>(r[i], f2);
+    if constexpr (!BF16) {
+      asm("min.f16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(0x7bff7bffu));
+      asm("max.f16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(0xfbfffbffu));
+    }
+  }
+}
+
+
+}  // namespace chunk
+}  // namespace actkv

@@ -29,9 +29,7 @@
 // (umma_common.cuh).
 #include <cuda.h>
 
-#include "common.cuh"
-#include "kernels.cuh"
-#include "umma_common.cuh"
+#include "chunk_common.cuh"
 
 namespace actkv {
 namespace chunk {
@@ -41,11 +39,6 @@ using namespace umma;
 constexpr int kMaxThreads = 640;
 constexpr int threads(bool quant) { return quant ? 640 : 384; }
 constexpr int kUnitSlots = 4;               // units announced ahead of their results
-constexpr int kRows = 128;                  // query rows per tile (MMA M)
-constexpr int kTile = 128;                  // tokens per key tile
-constexpr int kUnitCost = 2;                // a unit's fixed cost (queries in, results out) in key tiles
-constexpr float kSlack = 8.0f;              // log2 units the maximum may outgrow m by
-constexpr int kMaxD = 128;
 
 constexpr uint32_t kSchedBytes = 512;
 
@@ -83,16 +76,8 @@ struct Unit {
   int64_t end;               // the unit's end in the schedule
 };
 
-struct Desc {                // the unit that a CTA began and left to the next ones
-  int32_t valid, r, h, j0, ntok, S, A, a0;
-  int64_t end, total;
-  int32_t two, pad[3];
-};
-static_assert(sizeof(Desc) == 64, "the partial results after the descriptors are 16-byte aligned");
-
 struct Sched {               // in shared memory
-  int64_t total, pre;        // all weight, weight before session r0
-  int r0;
+  Share share;
   uint32_t tmem;
   int abort_flag;
   int bad_v;                 // a value that some row of the unit does not see is not finite
@@ -130,16 +115,16 @@ struct Walker {
       a0 = a->q_off[r];
       A = a->q_off[r + 1] - a0;
       S = a->seq_used[r];
-      if (A > 0) return;
+      if (A > 0 && A * a->G > a->few_rows) return;
       ++r;
     }
   }
   __device__ Walker(const ChunkArgs* args, const Sched& s, int cta, int n) : a(args), geo(*args) {
-    lo = s.total * cta / n;
-    hi = s.total * (cta + 1) / n;
-    r = s.r0;
+    lo = s.share.total * cta / n;
+    hi = s.share.total * (cta + 1) / n;
+    r = s.share.r0;
     h = j = S = A = a0 = 0;
-    at = s.pre;
+    at = s.share.pre;
     if (lo >= hi) {
       at = hi;
       return;
@@ -188,47 +173,11 @@ struct Walker {
 // Total weight, and the session that holds this CTA's first unit of weight.
 template <int kThreads>
 __device__ void make_schedule(const ChunkArgs& a, Sched& s, int cta, int n) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Geometry geo(a);
-  // pass 0 adds the weights up, pass 1 finds the session (only when a pass over all does not fit)
-  int64_t lo = 0;
-  for (int pass = 0; pass < 2; ++pass) {
-    int64_t carry = 0;
-    for (int base = 0; base < a.R; base += kThreads) {
-      const int r = base + int(threadIdx.x);
-      int64_t w = 0;
-      if (r < a.R) {
-        const int A = a.q_off[r + 1] - a.q_off[r];
-        if (A > 0) w = a.Hkv * geo.head_weight(a.seq_used[r], A);
-      }
-      int64_t incl = w;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
-      }
-      if (lane == 31) s.scan[warp] = incl;
-      __syncthreads();
-      int64_t before = carry, all = carry;
-      for (int i = 0; i < kThreads / 32; ++i) {
-        if (i < warp) before += s.scan[i];
-        all += s.scan[i];
-      }
-      __syncthreads();
-      if (pass == 0 && base + kThreads >= a.R) {            // the last step: the total is known
-        if (threadIdx.x == 0) s.total = all;
-        lo = all * cta / n;
-      }
-      const int64_t excl = before + incl - w;
-      if ((pass == 1 || a.R <= kThreads) && w > 0 && lo >= excl && lo < excl + w) {
-        s.r0 = r;
-        s.pre = excl;
-      }
-      carry = all;
-    }
-    if (a.R <= kThreads) break;
-  }
-  __syncthreads();
+  share_out<kThreads>(a.R, [&](int r) -> int64_t {
+    const int A = a.q_off[r + 1] - a.q_off[r];
+    return A * a.G > a.few_rows ? a.Hkv * geo.head_weight(a.seq_used[r], A) : 0;
+  }, s.share, s.scan, cta, n);
 }
 
 // ------------------------------------------------------------------------------------ operands
@@ -316,14 +265,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  uint32_t r;
-  if constexpr (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-
 // The waits of this kernel, bounded like mbar_wait's but shorter: the kernel's roles share an instruction
 // cache, which the waits' slow paths filled.  false when the wait gave up (about 2^31 cycles; *abort is
 // then 1, and the kernel reports it at its end) or another role did.
@@ -402,14 +343,6 @@ struct UnitItems {
   }
 };
 
-// Part `slot` (0: a unit begun by an earlier CTA, 1: one left to the next) of CTA `cta`'s partial
-// results: rows of D values, then (m, l) per row.
-constexpr int64_t kPartFloats = int64_t(2 * kRows) * (kMaxD + 2);
-__device__ __forceinline__ float* part_of(void* ws, int n_cta, int cta, int slot) {
-  return reinterpret_cast<float*>(static_cast<char*>(ws) + int64_t(n_cta) * sizeof(Desc)) +
-         (int64_t(cta) * 2 + slot) * kPartFloats;
-}
-
 template <int D, bool BF16>
 __device__ __forceinline__ void store_row(uint16_t* dst, const float (&o)[32], float inv, bool vec) {
   uint32_t u[16];
@@ -424,60 +357,6 @@ __device__ __forceinline__ void store_row(uint16_t* dst, const float (&o)[32], f
     for (int i = 0; i < 16; ++i) {
       dst[2 * i] = uint16_t(u[i]);
       dst[2 * i + 1] = uint16_t(u[i] >> 16);
-    }
-  }
-}
-
-// 16 e4m3 values with scale byte b as 16-bit values.  The four exponent and three mantissa bits of a
-// byte, moved under the wider type's exponent, read as the value times 2^-120 (bf16) or 2^-8 (fp16),
-// subnormals included, so one multiplication by a power of two, 2^(b - 127) with that put right, gives
-// the value exactly; a power of two outside the type takes a second one.  fp16 values past its range
-// become its largest.
-template <bool BF16>
-__device__ __forceinline__ uint32_t mul16x2(uint32_t x, uint32_t f) {
-  uint32_t r;
-  if constexpr (BF16) asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(f));
-  else asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(f));
-  return r;
-}
-// Whether one multiplication does for every byte of a word of scale bytes.
-template <bool BF16>
-__device__ __forceinline__ bool plain_scales(uint32_t w) {
-  return __vcmpgtu4(w, 0x86868686u) == 0 && (BF16 || __vcmpgtu4(0x69696969u, w) == 0);   // <= 134 (fp16: >= 105)
-}
-template <bool BF16>
-__device__ __forceinline__ void widen16(const uint4& raw, uint32_t f, uint32_t (&r)[8]) {
-  const uint32_t in[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t x = __byte_perm(in[i >> 1], 0u, (i & 1) ? 0x3424 : 0x1404);   // two bytes, each atop a half
-    const uint32_t y = ((x >> (BF16 ? 4 : 1)) & (BF16 ? 0x07f007f0u : 0x3f803f80u)) | (x & 0x80008000u);
-    r[i] = mul16x2<BF16>(y, f);
-  }
-}
-// The multiplier of scale byte b, in both halves, where plain_scales holds.
-template <bool BF16>
-__device__ __forceinline__ uint32_t plain_factor(uint32_t b) {
-  return BF16 ? b * 0x00800080u + 0x3c003c00u : (b - 104u) * 0x04000400u;
-}
-// For any scale byte: the multiplier within the type, and a second one.
-template <bool BF16>
-__device__ __forceinline__ void any_factors(uint32_t b, uint32_t& f1, uint32_t& f2) {
-  const int e = BF16 ? int(b) + 120 : int(b) - 104, top = BF16 ? 254 : 30;
-  const int e1 = min(max(e, 1), top), e2 = min(max(e - e1 + (BF16 ? 127 : 15), 1), top);
-  const uint32_t one = BF16 ? 0x00800080u : 0x04000400u;
-  f1 = b == 255u ? 0x7fff7fffu : e1 * one;   // 255: NaN
-  f2 = e2 * one;
-}
-template <bool BF16>
-__device__ __forceinline__ void widen16_rest(uint32_t b, uint32_t f2, uint32_t (&r)[8]) {
-  if (b == 255u) return;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    r[i] = mul16x2<BF16>(r[i], f2);
-    if constexpr (!BF16) {
-      asm("min.f16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(0x7bff7bffu));
-      asm("max.f16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(0xfbfffbffu));
     }
   }
 }
@@ -565,14 +444,12 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
       mbar_init(bar(B_RE + i), 8);
       mbar_init(bar(B_CF + i), 1);
     }
-    sched.total = sched.pre = 0;
-    sched.r0 = a.R;
+    sched.share = Share{0, 0, a.R};
     sched.abort_flag = 0;
     sched.bad_v = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    Desc* dsc = static_cast<Desc*>(a.workspace) + cta;
-    dsc->valid = 0;
+    wide_parts(a.workspace, n_cta).desc[cta].valid = 0;
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sched.tmem))
@@ -1041,7 +918,9 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
         const int64_t qt = int64_t(x.a0) + j;
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         const int pr = (two ? w * kRows : 0) + row;
-        float* part = whole ? nullptr : part_of(a.workspace, n_cta, cta, x.t0 > 0 ? 0 : 1);
+        const Parts ps = wide_parts(a.workspace, n_cta);
+        const int ps_slot = x.t0 > 0 ? 0 : 1;
+        float* part = ps.out(cta, ps_slot);
         if (busy) {
 #pragma unroll 1
           for (int q = 0; q < D / 32; ++q) {
@@ -1107,7 +986,7 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
           if (whole)
             a.lse[qt * a.lse_stride_t + hq] = l == 0.0f ? ninf : (m == ninf ? l : (m + log2f(l)) * 0.69314718055994531f);
           else
-            *reinterpret_cast<float2*>(part + int64_t(2 * kRows) * D + 2 * pr) = make_float2(m, l);
+            *reinterpret_cast<float2*>(ps.ml(cta, ps_slot, D) + 2 * pr) = make_float2(m, l);
         }
         if (!whole && x.t0 == 0 && row == 0 && w == 0) {
           Desc d = {};
@@ -1120,9 +999,9 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
           d.A = x.A;
           d.a0 = x.a0;
           d.end = x.end;
-          d.total = sched.total;
+          d.total = sched.share.total;
           d.two = two;
-          static_cast<Desc*>(a.workspace)[cta] = d;
+          ps.desc[cta] = d;
         }
         fence_before();
         __syncwarp();
@@ -1245,6 +1124,7 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
     }
   }
   __syncthreads();
+  pdl_wait();                                // chunk_few_kernel is done too when this one is
   if (threadIdx.x == 0 && *abort_flag) flag(a.status, ACTKV_DEV_TIMEOUT);
   if (warp == 1) {
     fence_after();
@@ -1256,27 +1136,31 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
 constexpr int kJoinThreads = 256;
 constexpr int kJoinSlices = 8;               // CTAs per split unit, rows dealt in turn
 
-// One CTA per (CTA that began a unit and left it, slice of its rows); a warp per row.
+// One CTA per (CTA that began a unit and left it, slice of its rows); a warp per row.  The last slice is
+// for the units of chunk_few_kernel.
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kJoinThreads) chunk_combine_kernel(const __grid_constant__ ChunkArgs a, int n_cta) {
+__global__ void __launch_bounds__(kJoinThreads) chunk_combine_kernel(const __grid_constant__ ChunkArgs a, int n_cta,
+                                                                             int first_slice) {
   pdl_wait();
+  const int y = first_slice + blockIdx.y;
+  const bool few = y == kJoinSlices;
+  const Parts ps = few ? few_parts(a.workspace, n_cta) : wide_parts(a.workspace, n_cta);
   const int cta = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Desc d = static_cast<const Desc*>(a.workspace)[cta];
+  const int slice = few ? 0 : y, slices = few ? 1 : kJoinSlices;
+  const Desc d = ps.desc[cta];
   if (!d.valid) return;
   const float ninf = -__int_as_float(0x7f800000);
   int last = cta;                            // parts: slot 1 of cta, slot 0 of cta + 1 .. last
   while (last + 1 < n_cta && d.total * (last + 1) / n_cta < d.end) ++last;
   const int tpb = kRows / a.G;
-  const int live0 = min(tpb, d.ntok) * a.G, live1 = d.two ? (d.ntok - tpb) * a.G : 0;
-  for (int i = blockIdx.y * (kJoinThreads / 32) + warp; i < live0 + live1; i += kJoinSlices * (kJoinThreads / 32)) {
+  const int live0 = (d.two ? tpb : d.ntok) * a.G, live1 = d.two ? (d.ntok - tpb) * a.G : 0;
+  for (int i = slice * (kJoinThreads / 32) + warp; i < live0 + live1; i += slices * (kJoinThreads / 32)) {
     const int b = i < live0 ? 0 : 1;
     const int row = i - b * live0;
     const int pr = b * kRows + row;
     const int jr = row / a.G, hq = d.h * a.G + row - jr * a.G;
     const int64_t qt = int64_t(d.a0) + d.j0 + b * tpb + jr;
-    auto ml_of = [&](int c) {
-      return *reinterpret_cast<const float2*>(part_of(a.workspace, n_cta, c, c == cta ? 1 : 0) + int64_t(2 * kRows) * D + 2 * pr);
-    };
+    auto ml_of = [&](int c) { return *reinterpret_cast<const float2*>(ps.ml(c, c == cta ? 1 : 0, D) + 2 * pr); };
     float M = ninf;
     for (int c = cta + lane; c <= last; c += 32)
       if (d.total * c / n_cta < d.total * (c + 1) / n_cta) M = fmaxf(M, ml_of(c).x);
@@ -1291,7 +1175,7 @@ __global__ void __launch_bounds__(kJoinThreads) chunk_combine_kernel(const __gri
       if (y.y == 0.0f) continue;             // saw none of the row's tokens
       const float al = y.x == ninf ? 1.0f : ex2(y.x - M);
       L += y.y * al;
-      const float* p = part_of(a.workspace, n_cta, c, c == cta ? 1 : 0) + int64_t(pr) * D;
+      const float* p = ps.out(c, c == cta ? 1 : 0) + int64_t(pr) * D;
 #pragma unroll
       for (int k = 0; k < D / 32; ++k) o[k] = fmaf(p[k * 32 + lane], al, o[k]);
     }
@@ -1308,7 +1192,7 @@ __global__ void __launch_bounds__(kJoinThreads) chunk_combine_kernel(const __gri
 
 // ------------------------------------------------------------------------------------ host side
 size_t chunk_workspace_bytes(int n_sm) {
-  return align256(size_t(n_sm) * (sizeof(chunk::Desc) + 2 * chunk::kPartFloats * sizeof(float)));
+  return align256(chunk::few_offset(n_sm) + chunk::parts_bytes(n_sm, chunk::kFewRows));
 }
 
 bool chunk_umma_supported(const ChunkArgs& a, int dtype, const char** why) {
@@ -1340,23 +1224,31 @@ cudaError_t launch_chunk_t(const CUtensorMap& mkv, const CUtensorMap& mq, const 
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(chunk::Layout<D, QUANT>::kSmemBytes));
   if (e != cudaSuccess) return e;
   const bool vec_out = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_stride_t % 8 == 0 && a.out_stride_h % 8 == 0;
-  k<<<grid, chunk::threads(QUANT), chunk::Layout<D, QUANT>::kSmemBytes, st>>>(mkv, mq, a, vec_out);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid, chunk::kJoinSlices);
-  cfg.blockDim = dim3(chunk::kJoinThreads);
   cfg.stream = st;
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
+  const bool wide = a.T * int64_t(a.G) > a.few_rows;         // else every session is chunk_few_kernel's
+  if (wide) {
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(chunk::threads(QUANT));
+    cfg.dynamicSmemBytes = chunk::Layout<D, QUANT>::kSmemBytes;
+    cfg.numAttrs = a.few_rows > 0 ? 1 : 0;   // beside chunk_few_kernel's last CTAs
+    if ((e = cudaLaunchKernelEx(&cfg, k, mkv, mq, a, vec_out)) != cudaSuccess) return e;
+  }
+  cfg.gridDim = dim3(grid, (wide ? chunk::kJoinSlices : 0) + (a.few_rows > 0 ? 1 : 0));
+  cfg.blockDim = dim3(chunk::kJoinThreads);
+  cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, chunk::chunk_combine_kernel<D, BF16>, a, grid);
+  return cudaLaunchKernelEx(&cfg, chunk::chunk_combine_kernel<D, BF16>, a, grid, wide ? 0 : chunk::kJoinSlices);
 }
 
 }  // namespace
 
-cudaError_t launch_chunk_umma(const ChunkArgs& a, int dtype, cudaStream_t st, const char** why) {
+cudaError_t launch_chunk_umma(const ChunkArgs& args, int dtype, cudaStream_t st, const char** why) {
+  ChunkArgs a = args;
   EncodeTiledFn enc = get_encode_fn();
   if (!enc) {
     *why = "cuTensorMapEncodeTiled unavailable";
@@ -1403,6 +1295,12 @@ cudaError_t launch_chunk_umma(const ChunkArgs& a, int dtype, cudaStream_t st, co
   }
   *why = "chunk attention";
   const int grid = device_sm_count();
+  // sessions of few query rows go to a kernel of their own, where a GQA group fits it
+  a.few_rows = a.G <= chunk::kFewRows ? chunk::kFewRows : 0;
+  if (a.few_rows > 0) {
+    const cudaError_t e = launch_chunk_few(a, dtype, grid, st);
+    if (e != cudaSuccess) return e;
+  }
   const bool bf = dtype == ACTKV_BF16;
   if (a.quant) {
     if (a.D == 128) return bf ? launch_chunk_t<128, true, true>(mkv, mq, a, grid, st) : launch_chunk_t<128, false, true>(mkv, mq, a, grid, st);
