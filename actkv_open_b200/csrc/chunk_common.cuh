@@ -14,6 +14,7 @@ using namespace umma;
 constexpr int kRows = 128;                  // query rows per row tile (MMA M)
 constexpr int kTile = 128;                  // tokens per key tile, the grain of the schedule
 constexpr int kFewRows = 16;                // query rows of a session and KV head that chunk_few_kernel takes
+constexpr int kFewParts = 8 * kFewRows;     // rows of its units: up to 8 heads
 constexpr int kUnitCost = 2;                // a unit's fixed cost (queries in, results out) in key tiles
 constexpr float kSlack = 8.0f;              // log2 units the maximum may outgrow m by
 constexpr int kMaxD = 128;
@@ -24,10 +25,16 @@ struct Share {
   int r0;                    // the session that holds the CTA's first unit of weight
 };
 
-// CTA `cta` of n takes the weight [total * cta / n, total * (cta + 1) / n), sessions in order.  Every thread
-// of the block calls it; `s` starts as {0, 0, R}.
+// CTAs that get work when a share is at least `least`.
+__device__ __forceinline__ int used_ctas(int64_t total, int n, int least) {
+  return int(max(int64_t(1), min(int64_t(n), total / least)));
+}
+
+// CTA `cta` of the n used takes the weight [total * cta / n, total * (cta + 1) / n), sessions in order.
+// Every thread of the block calls it; `s` starts as {0, 0, R}.
 template <int kThreads, typename Weight>
-__device__ __forceinline__ void share_out(int R, Weight weight, Share& s, int64_t* scan, int cta, int n) {
+__device__ __forceinline__ void share_out(int R, Weight weight, Share& s, int64_t* scan, int cta, int n,
+                                          int least) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // pass 0 adds the weights up, pass 1 finds the session (only when a pass over all does not fit)
   int64_t lo = 0;
@@ -54,7 +61,7 @@ __device__ __forceinline__ void share_out(int R, Weight weight, Share& s, int64_
       __syncthreads();
       if (pass == 0 && base + kThreads >= R) {              // the last step: the total is known
         if (threadIdx.x == 0) s.total = all;
-        lo = all * cta / n;
+        lo = all * cta / used_ctas(all, n, least);
       }
       const int64_t excl = before + incl - w;
       if ((pass == 1 || R <= kThreads) && w > 0 && lo >= excl && lo < excl + w) {
@@ -72,7 +79,8 @@ __device__ __forceinline__ void share_out(int R, Weight weight, Share& s, int64_
 struct Desc {                // the unit that a CTA began and left to the next ones
   int32_t valid, r, h, j0, ntok, S, A, a0;
   int64_t end, total;
-  int32_t two, pad[3];
+  int32_t two, heads;        // two row tiles; KV heads from h on
+  int32_t n_used, pad;       // CTAs that the work was shared out to
 };
 static_assert(sizeof(Desc) == 64, "the partial results after the descriptors are 16-byte aligned");
 
@@ -97,7 +105,7 @@ __device__ __forceinline__ Parts parts_at(void* ws, size_t off, int n_cta, int r
   return Parts{reinterpret_cast<Desc*>(p), reinterpret_cast<float*>(p + int64_t(n_cta) * sizeof(Desc)), rows};
 }
 __device__ __forceinline__ Parts wide_parts(void* ws, int n_cta) { return parts_at(ws, 0, n_cta, 2 * kRows); }
-__device__ __forceinline__ Parts few_parts(void* ws, int n_cta) { return parts_at(ws, few_offset(n_cta), n_cta, kFewRows); }
+__device__ __forceinline__ Parts few_parts(void* ws, int n_cta) { return parts_at(ws, few_offset(n_cta), n_cta, kFewParts); }
 
 // ------------------------------------------------------------------------------------ 16-bit values
 template <bool BF16>

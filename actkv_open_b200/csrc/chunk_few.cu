@@ -16,8 +16,10 @@
 // consecutive bytes of a row; the pairs of tokens that an operand register holds are put together
 // by byte permutes.  p goes from the layout of S to that of the second product without a move.
 //
-// Work is shared out as in chunk_umma.cu: equal shares of key tiles per CTA, a unit being (session, KV head);
-// the eight warps of a CTA take every eighth step of 16 tokens of its part.
+// Work is shared out as in chunk_umma.cu, in equal shares per CTA.  A unit is a session and a group of 8 (4, 2, 1:
+// what divides them) KV heads, a warp per head: a token's row is read whole by one CTA at one time.  With a
+// head per CTA the 8-bit rows' scale bytes, 4 per head and row, were fetched from memory once per head, 64 bytes
+// each time (1.7 times the bytes of the rows).  With fewer heads the warps of one take its tokens in turn.
 #include <type_traits>
 
 #include "chunk_common.cuh"
@@ -28,7 +30,10 @@ namespace few {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
+constexpr int kRoundCost = 6;               // a unit's fixed cost in rounds of its warps
+constexpr int kMinRounds = 6;               // a CTA's share is at least so many: fewer partial results to join
 constexpr int kStep = 16;                   // tokens per step
+constexpr int kJoinRow = kMaxD + 8;         // a warp's O, m and l in shared memory: 16 of these floats
 
 template <int D, bool QUANT>
 struct Ring {
@@ -38,7 +43,7 @@ struct Ring {
   static constexpr uint32_t kStage = 2 * kPlane + (QUANT ? 128 : 0);     // and their scale words
   static constexpr int kStages = QUANT ? 6 : (D == 128 ? 3 : 6);
   static constexpr uint32_t kBytes = kWarps * kStages * kStage;
-  static constexpr uint32_t kJoinBytes = kWarps * kFewRows * (D + 4) * 4;
+  static constexpr uint32_t kJoinBytes = kWarps * kFewRows * kJoinRow * 4;
   static constexpr uint32_t kSmemBytes = (kBytes > kJoinBytes ? kBytes : kJoinBytes) + 512;
   static_assert(kSmemBytes <= 232448, "exceeds the 227 KB of shared memory a CTA can have");
 };
@@ -125,7 +130,7 @@ struct Sched {
 static_assert(sizeof(Sched) <= 512, "the schedule's place in shared memory");
 
 template <int D, bool BF16, bool QUANT>
-__global__ void __launch_bounds__(kThreads, 1) chunk_few_kernel(const __grid_constant__ ChunkArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) chunk_few_kernel(const __grid_constant__ ChunkArgs a, bool vec_out) {
   using Rg = Ring<D, QUANT>;
   constexpr int CH = Rg::kChunks, kRowsPerCopy = 32 / CH, kCopies = kStep / kRowsPerCopy;
   constexpr int kKSteps = D / 16, kTiles = D / 8;           // products per S, per O
@@ -146,39 +151,48 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few_kernel(const __grid_con
     ps.desc[cta].valid = 0;
   }
   __syncthreads();
+  const int HG = a.Hkv % 8 == 0 ? 8 : (a.Hkv % 4 == 0 ? 4 : (a.Hkv % 2 == 0 ? 2 : 1));   // heads per unit
+  const int wph = kWarps / HG, round = kStep * wph;         // warps per head, tokens of a round of theirs
+  const int my_head = warp % HG, my_part = warp / HG;
   share_out<kThreads>(a.R, [&](int r) -> int64_t {
     const int A = a.q_off[r + 1] - a.q_off[r];
-    return A > 0 && A * a.G <= a.few_rows ? int64_t(a.Hkv) * (kUnitCost + (a.seq_used[r] + kTile - 1) / kTile) : 0;
-  }, sched.share, sched.scan, cta, n_cta);
-  const int64_t lo = sched.share.total * cta / n_cta, hi = sched.share.total * (cta + 1) / n_cta;
-  if (lo >= hi) return;
+    return A > 0 && A * a.G <= a.few_rows ? int64_t(a.Hkv / HG) * (kRoundCost + (a.seq_used[r] + round - 1) / round) : 0;
+  }, sched.share, sched.scan, cta, n_cta, kMinRounds);
+  const int64_t total = sched.share.total;
+  const int n_used = used_ctas(total, n_cta, kMinRounds);
+  const int64_t lo = total * cta / n_used, hi = total * (cta + 1) / n_used;
+  if (cta >= n_used || lo >= hi) return;
   int r = sched.share.r0;
-  int64_t at = sched.share.pre;              // start of (session r, head h) in the schedule
-  int h = 0;
+  int64_t at = sched.share.pre;              // start of (session r, head group hg) in the schedule
+  int hg = 0;
   bool seek = true;
   const float c2 = a.scale * kLog2e;
   const char* kv = static_cast<const char*>(a.kv);
   const int64_t es = QUANT ? 1 : 2, stride_s = a.kv_stride_s * es, stride_b = a.kv_stride_b * es;
+  const int64_t to_values = a.kv_stride_kv * es;
+  const int shift = (a.BS & (a.BS - 1)) == 0 ? __ffs(a.BS) - 1 : -1;
+  auto block_of = [&](int tok) { return shift >= 0 ? tok >> shift : tok / a.BS; };
 
-  for (; r < a.R && at < hi; ++r, h = 0) {
+  for (; r < a.R && at < hi; ++r, hg = 0) {
     const int a0 = a.q_off[r], A = a.q_off[r + 1] - a0, S = a.seq_used[r];
     if (A <= 0 || A * a.G > a.few_rows) continue;
     const int rows = A * a.G;
-    const int nt = S > 0 ? (S + kTile - 1) / kTile : 0;
-    const int64_t weight = kUnitCost + nt;
-    if (seek) {                               // the head that holds lo
-      h = int((lo - at) / weight);
-      at += h * weight;
+    const int nt = S > 0 ? (S + round - 1) / round : 0;
+    const int64_t weight = kRoundCost + nt;
+    if (seek) {                               // the group that holds lo
+      hg = int((lo - at) / weight);
+      at += hg * weight;
       seek = false;
     }
     const int32_t* table = a.block_table + r * a.bt_stride_r;
-    for (; h < a.Hkv && at < hi; ++h, at += weight) {
-      const int64_t first = at + kUnitCost;
+    for (; hg < a.Hkv / HG && at < hi; ++hg, at += weight) {
+      const int64_t first = at + kRoundCost;
       const int t0 = int(lo > first ? lo - first : 0), t1 = nt == 0 ? 0 : int(min(int64_t(nt), hi - first));
       if (nt == 0 ? at < lo : t0 >= t1) continue;
-      const int begin = t0 * kTile, end = min(t1 * kTile, S);
-      const int steps = (end - begin + kStep - 1) / kStep;
-      const int mine = warp < steps ? (steps - warp + kWarps - 1) / kWarps : 0;    // steps of this warp
+      const int h = hg * HG + my_head;
+      const int begin = t0 * round, end = min(t1 * round, S);
+      const int start = begin + my_part * kStep;              // this warp's steps: start, start + round, ...
+      const int mine = start < end ? (end - start + round - 1) / round : 0;
       const int lim0 = S - A + r8 / a.G, lim1 = S - A + (r8 + 8) / a.G;           // last tokens the lane's rows see
       const bool wide = rows > 8;
       // ---- queries as the first operand: for each k-step rows r8 and r8 + 8, dims as the keys come
@@ -207,39 +221,37 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few_kernel(const __grid_con
         for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
       float m0 = ninf, m1 = ninf, l0 = 0.0f, l1 = 0.0f;
 
-      // ---- copies of step i of this warp: lane l < 16 looks up token l's slot a step ahead
+      // ---- copies of step i of this warp: lane l (and l - 16) looks up token l's block a step ahead
       auto look_up = [&](int i) -> int {
-        const int tok = begin + (warp + i * kWarps) * kStep + (lane & 15);
+        const int tok = start + i * round + (lane & 15);
         if (i >= mine || tok >= end) return -2;
-        const int lb = tok / a.BS;
+        const int lb = block_of(tok);
         return lb < a.MB ? table[lb] : -1;
       };
       int phys = look_up(0);
+      const char* head = kv + (QUANT ? int64_t(h) * D : int64_t(h) * a.kv_stride_h * 2);
+      const int at_word = a.Hkv * D + (D == 128 ? h * 4 : (h * 2) & ~3);
       auto issue = [&](int i, int slot) {
-        const int t = begin + (warp + i * kWarps) * kStep;
         if (i < mine) {
           int ph = phys;
           if (ph != -2 && (ph < 0 || ph >= a.NB)) {
             flag(a.status, ACTKV_DEV_BAD_INDEX);
             ph = 0;
           }
-          const int tok = t + (lane & 15);
-          const int64_t off = ph < 0 ? -1 : int64_t(ph) * stride_b + int64_t(tok % a.BS) * stride_s;
+          const int tok = start + i * round + (lane & 15);
+          const int in_block = shift >= 0 ? tok & (a.BS - 1) : tok % a.BS;
+          const int64_t off = ph < 0 ? -1 : int64_t(ph) * stride_b + int64_t(in_block) * stride_s;
           const uint32_t dst = ring + slot * Rg::kStage;
-          const int64_t head = QUANT ? int64_t(h) * D : int64_t(h) * a.kv_stride_h * 2;
 #pragma unroll
           for (int e = 0; e < kCopies; ++e) {
             const int row = e * kRowsPerCopy + lane / CH, c = lane % CH;
             const int64_t from = __shfl_sync(full, off, row);
-            const char* p = kv + (from < 0 ? 0 : from + head + c * 16);
+            const char* p = (from < 0 ? kv : head + from) + c * 16;
             copy16(dst + row * (CH * 16) + key_piece<CH>(row, c) * 16, p, from >= 0);
-            copy16(dst + Rg::kPlane + row * (CH * 16) + value_piece<CH>(row, c) * 16,
-                   from < 0 ? p : p + a.kv_stride_kv * es, from >= 0);
+            copy16(dst + Rg::kPlane + row * (CH * 16) + value_piece<CH>(row, c) * 16, p + to_values, from >= 0);
           }
-          if constexpr (QUANT) {              // words: lanes 0-15 the keys', 16-31 the values'
-            const int at_word = a.Hkv * D + (D == 128 ? h * 4 : (h * 2) & ~3);
-            copy4(dst + 2 * Rg::kPlane + lane * 4, kv + (off < 0 ? 0 : off + at_word + (lane >> 4) * a.kv_stride_kv), off >= 0);
-          }
+          if constexpr (QUANT)                // words: lanes 0-15 the keys', 16-31 the values'
+            copy4(dst + 2 * Rg::kPlane + lane * 4, kv + (off < 0 ? 0 : off + at_word) + (lane >> 4) * to_values, off >= 0);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
         phys = look_up(i + 1);
@@ -247,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few_kernel(const __grid_con
 
       auto step = [&](int i, int slot, auto edge_) {
         constexpr bool EDGE = decltype(edge_)::value;        // hidden tokens, or scale bytes out of the ordinary
-        const int t = begin + (warp + i * kWarps) * kStep;
+        const int t = start + i * round;
         const uint32_t kb = ring + slot * Rg::kStage, vb = kb + Rg::kPlane, sb = kb + 2 * Rg::kPlane;
         const int sh = QUANT && D == 64 && (h & 1) ? 16 : 0; // the head's bytes within the word
         float s[2][4];
@@ -406,7 +418,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few_kernel(const __grid_con
         issue(i + kAhead, fill);
         asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
         __syncwarp();
-        const int t = begin + (warp + i * kWarps) * kStep;
+        const int t = start + i * round;
         bool edge = t + kStep - 1 > S - A || t + kStep > end;
         if constexpr (QUANT) {
           const uint32_t word = lds4(ring + slot * Rg::kStage + 2 * Rg::kPlane + lane * 4);
@@ -419,86 +431,131 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few_kernel(const __grid_con
         fill = fill + 1 == Rg::kStages ? 0 : fill + 1;
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
-      // ---- the warps meet: (m, l) and O of each through shared memory
+      // ---- results: l of a row over its four lanes, then rows r8 and r8 + 8 of the warp's head
       l0 += __shfl_xor_sync(full, l0, 1);
       l0 += __shfl_xor_sync(full, l0, 2);
       l1 += __shfl_xor_sync(full, l1, 1);
       l1 += __shfl_xor_sync(full, l1, 2);
-      __syncthreads();                        // the rings are free
-      float* jo = reinterpret_cast<float*>(smem) + warp * kFewRows * D;
-      float2* jml = reinterpret_cast<float2*>(smem + kWarps * kFewRows * D * 4) + warp * kFewRows;
-      if (c4 == 0) {
-        jml[r8] = make_float2(m0, l0);
-        jml[r8 + 8] = make_float2(m1, l1);
-      }
-#pragma unroll
-      for (int j = 0; j < kTiles; ++j) {      // columns 2 c4, 2 c4 + 1 of product j: dims kTiles n + j
-        if (r8 < rows) {
-          jo[r8 * D + kTiles * (2 * c4) + j] = o[j][0];
-          jo[r8 * D + kTiles * (2 * c4 + 1) + j] = o[j][1];
-        }
-        if (r8 + 8 < rows) {
-          jo[(r8 + 8) * D + kTiles * (2 * c4) + j] = o[j][2];
-          jo[(r8 + 8) * D + kTiles * (2 * c4 + 1) + j] = o[j][3];
-        }
-      }
-      __syncthreads();
-      const bool whole = t0 == 0 && t1 == nt, fix = sched.bad_v != 0;
+      const bool whole = t0 == 0 && t1 == nt;
       const int ps_slot = t0 > 0 ? 0 : 1;
-      const float2* all_ml = reinterpret_cast<const float2*>(smem + kWarps * kFewRows * D * 4);
-      for (int x = threadIdx.x; x < rows * D; x += kThreads) {
-        const int row = x / D, d = x - row * D;
-        float M = ninf;
-        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, all_ml[w * kFewRows + row].x);
-        float L = 0.0f, y = 0.0f;
-        for (int w = 0; w < kWarps; ++w) {
-          const float2 ml = all_ml[w * kFewRows + row];
-          if (ml.y == 0.0f) continue;         // saw none of the row's tokens
-          const float al = ml.x == ninf ? 1.0f : ex2(ml.x - M);
-          L = fmaf(ml.y, al, L);
-          y = fmaf(reinterpret_cast<const float*>(smem)[(w * kFewRows + row) * D + d], al, y);
+      if (wph > 1) {                          // the warps of a head meet through shared memory, the first goes on
+        __syncthreads();                      // the rings are free
+        float* jo = reinterpret_cast<float*>(smem) + warp * (kFewRows * kJoinRow);
+        if (my_part > 0) {
+#pragma unroll
+          for (int j = 0; j < kTiles; ++j)
+            *reinterpret_cast<float4*>(jo + (j * 32 + lane) * 4) = make_float4(o[j][0], o[j][1], o[j][2], o[j][3]);
+          *reinterpret_cast<float4*>(jo + (kTiles * 32 + lane) * 4) = make_float4(m0, l0, m1, l1);
         }
-        const int jq = row / a.G, hq = h * a.G + row - jq * a.G;
-        if (fix) {                            // values that were not finite and that this row does see
-          for (int t = max(S - A + 1, begin); t <= min(S - A + jq, end - 1); ++t) {
-            const int lb = t / a.BS, ph = lb < a.MB ? table[lb] : -1;
-            if (ph < 0 || ph >= a.NB) continue;
-            const char* p = kv + a.kv_stride_kv * es + int64_t(ph) * stride_b + int64_t(t - lb * a.BS) * stride_s;
-            float f;
-            if constexpr (QUANT) {
-              f = static_cast<uint8_t>(p[a.Hkv * D + (h * D + d) / 32]) == 255 ? __int_as_float(0x7fffffff) : 0.0f;
-            } else {
-              const uint16_t u = reinterpret_cast<const uint16_t*>(p)[int64_t(h) * a.kv_stride_h + d];
-              f = BF16 ? __uint_as_float(uint32_t(u) << 16) : __half2float(__ushort_as_half(u));
+        __syncthreads();
+        if (my_part == 0)
+#pragma unroll 1
+          for (int w = warp + HG; w < kWarps; w += HG) {
+            const float4* po = reinterpret_cast<const float4*>(smem) + w * (kFewRows * kJoinRow / 4);
+            const float4 y = po[kTiles * 32 + lane];
+            const float M0 = fmaxf(m0, y.x), M1 = fmaxf(m1, y.z);
+            // an empty side (sum 0) counts for nothing; a NaN sum stays
+            const float p0 = l0 == 0.0f ? 0.0f : (m0 == M0 ? 1.0f : ex2(m0 - M0)), q0 = y.y == 0.0f ? 0.0f : (y.x == M0 ? 1.0f : ex2(y.x - M0));
+            const float p1 = l1 == 0.0f ? 0.0f : (m1 == M1 ? 1.0f : ex2(m1 - M1)), q1 = y.w == 0.0f ? 0.0f : (y.z == M1 ? 1.0f : ex2(y.z - M1));
+            m0 = M0;
+            m1 = M1;
+            l0 = fmaf(l0, p0, y.y * q0);
+            l1 = fmaf(l1, p1, y.w * q1);
+#pragma unroll
+            for (int j = 0; j < kTiles; ++j) {
+              const float4 x = po[j * 32 + lane];
+              o[j][0] = fmaf(o[j][0], p0, x.x * q0);
+              o[j][1] = fmaf(o[j][1], p0, x.y * q0);
+              o[j][2] = fmaf(o[j][2], p1, x.z * q1);
+              o[j][3] = fmaf(o[j][3], p1, x.w * q1);
             }
-            if (!isfinite(f)) y += f;
           }
-        }
-        if (whole) {
+      }
+      // columns 2 c4 and 2 c4 + 1 of the products: dims kTiles * column + j, kTiles in a row
+      if (my_part == 0) {
+        const bool fix = *reinterpret_cast<volatile int*>(&sched.bad_v) != 0;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const int row = r8 + hf * 8;
+          if (row >= rows) continue;
+          const float L = hf ? l1 : l0, M = hf ? m1 : m0, inv = L == 0.0f ? 0.0f : 1.0f / L;
+          const int jq = row / a.G, hq = h * a.G + row - jq * a.G, hr = my_head * rows + row;
           const int64_t qt = int64_t(a0) + jq;
-          static_cast<uint16_t*>(a.out)[qt * a.out_stride_t + int64_t(hq) * a.out_stride_h + d] =
-              uint16_t(pack2<BF16>(L == 0.0f ? 0.0f : y / L, 0.0f));
-          if (d == 0)
-            a.lse[qt * a.lse_stride_t + hq] = L == 0.0f ? ninf : (M == ninf ? L : (M + log2f(L)) * 0.69314718055994531f);
-        } else {
-          ps.out(cta, ps_slot)[int64_t(row) * D + d] = y;
-          if (d == 0) reinterpret_cast<float2*>(ps.ml(cta, ps_slot, D))[row] = make_float2(M, L);
+          uint16_t* dst = static_cast<uint16_t*>(a.out) + qt * a.out_stride_t + int64_t(hq) * a.out_stride_h;
+          float* part = ps.out(cta, ps_slot) + int64_t(hr) * D;
+#pragma unroll
+          for (int cc = 0; cc < 2; ++cc) {
+            const int d0 = kTiles * (2 * c4 + cc);
+            if (whole) {
+#pragma unroll
+              for (int j = 0; j < kTiles; j += 8) {
+                uint32_t u[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  u[k] = pack2<BF16>(o[j + 2 * k][2 * hf + cc] * inv, o[j + 2 * k + 1][2 * hf + cc] * inv);
+                if (vec_out) {
+                  *reinterpret_cast<uint4*>(dst + d0 + j) = make_uint4(u[0], u[1], u[2], u[3]);
+                } else {
+#pragma unroll
+                  for (int k = 0; k < 8; ++k) dst[d0 + j + k] = uint16_t(u[k >> 1] >> (k & 1) * 16);
+                }
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < kTiles; j += 4)
+                *reinterpret_cast<float4*>(part + d0 + j) = make_float4(o[j][2 * hf + cc], o[j + 1][2 * hf + cc],
+                                                                        o[j + 2][2 * hf + cc], o[j + 3][2 * hf + cc]);
+            }
+            if (fix) {                        // values that were not finite and that this row does see
+#pragma unroll 1
+              for (int t = max(S - A + 1, begin); t <= min(S - A + jq, end - 1); ++t) {
+                const int lb = block_of(t), ph = lb < a.MB ? table[lb] : -1;
+                if (ph < 0 || ph >= a.NB) continue;
+                const char* p = kv + to_values + int64_t(ph) * stride_b + int64_t(t - lb * a.BS) * stride_s;
+#pragma unroll 1
+                for (int d = d0; d < d0 + kTiles; ++d) {
+                  float f;
+                  if constexpr (QUANT) {
+                    f = static_cast<uint8_t>(p[a.Hkv * D + (h * D + d) / 32]) == 255 ? __int_as_float(0x7fffffff) : 0.0f;
+                  } else {
+                    const uint16_t u = reinterpret_cast<const uint16_t*>(p)[int64_t(h) * a.kv_stride_h + d];
+                    f = BF16 ? __uint_as_float(uint32_t(u) << 16) : __half2float(__ushort_as_half(u));
+                  }
+                  if (isfinite(f)) continue;
+                  if (whole) {
+                    const float y = BF16 ? __uint_as_float(uint32_t(dst[d]) << 16) : __half2float(__ushort_as_half(dst[d]));
+                    dst[d] = uint16_t(pack2<BF16>(y + f, 0.0f));
+                  } else {
+                    part[d] += f;
+                  }
+                }
+              }
+            }
+          }
+          if (c4 == 0) {
+            if (whole)
+              a.lse[qt * a.lse_stride_t + hq] = L == 0.0f ? ninf : (M == ninf ? L : (M + log2f(L)) * 0.69314718055994531f);
+            else
+              *reinterpret_cast<float2*>(ps.ml(cta, ps_slot, D) + 2 * hr) = make_float2(M, L);
+          }
         }
       }
       if (!whole && t0 == 0 && threadIdx.x == 0) {
         Desc ds = {};
         ds.valid = 1;
         ds.r = r;
-        ds.h = h;
+        ds.h = hg * HG;
+        ds.heads = HG;
+        ds.n_used = n_used;
         ds.ntok = A;
         ds.S = S;
         ds.A = A;
         ds.a0 = a0;
         ds.end = first + nt;
-        ds.total = sched.share.total;
+        ds.total = total;
         ps.desc[cta] = ds;
       }
-      __syncthreads();                        // the rings are written again
+      if (wph > 1) __syncthreads();           // the rings are written again
     }
   }
 }
@@ -514,7 +571,8 @@ cudaError_t launch_few_t(const ChunkArgs& a, int grid, cudaStream_t st) {
   constexpr int bytes = int(chunk::few::Ring<D, QUANT>::kSmemBytes);
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return e;
-  k<<<grid, chunk::few::kThreads, bytes, st>>>(a);
+  const bool vec_out = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_stride_t % 8 == 0 && a.out_stride_h % 8 == 0;
+  k<<<grid, chunk::few::kThreads, bytes, st>>>(a, vec_out);
   return cudaGetLastError();
 }
 

@@ -120,8 +120,9 @@ struct Walker {
     }
   }
   __device__ Walker(const ChunkArgs* args, const Sched& s, int cta, int n) : a(args), geo(*args) {
+    n = used_ctas(s.share.total, n, 1);
     lo = s.share.total * cta / n;
-    hi = s.share.total * (cta + 1) / n;
+    hi = cta < n ? s.share.total * (cta + 1) / n : lo;
     r = s.share.r0;
     h = j = S = A = a0 = 0;
     at = s.share.pre;
@@ -177,7 +178,7 @@ __device__ void make_schedule(const ChunkArgs& a, Sched& s, int cta, int n) {
   share_out<kThreads>(a.R, [&](int r) -> int64_t {
     const int A = a.q_off[r + 1] - a.q_off[r];
     return A * a.G > a.few_rows ? a.Hkv * geo.head_weight(a.seq_used[r], A) : 0;
-  }, s.share, s.scan, cta, n);
+  }, s.share, s.scan, cta, n, 1);
 }
 
 // ------------------------------------------------------------------------------------ operands
@@ -1000,6 +1001,8 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
           d.a0 = x.a0;
           d.end = x.end;
           d.total = sched.share.total;
+          d.heads = 1;
+          d.n_used = used_ctas(d.total, n_cta, 1);
           d.two = two;
           ps.desc[cta] = d;
         }
@@ -1136,49 +1139,60 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
 constexpr int kJoinThreads = 256;
 constexpr int kJoinSlices = 8;               // CTAs per split unit, rows dealt in turn
 
-// One CTA per (CTA that began a unit and left it, slice of its rows); a warp per row.  The last slice is
-// for the units of chunk_few_kernel.
+// One CTA per (CTA that began a unit and left it, slice of its rows); a warp per row.  The slices from
+// kJoinSlices on are for the units of chunk_few_kernel.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kJoinThreads) chunk_combine_kernel(const __grid_constant__ ChunkArgs a, int n_cta,
-                                                                             int first_slice) {
+                                                                     int first_slice) {
   pdl_wait();
-  const int y = first_slice + blockIdx.y;
-  const bool few = y == kJoinSlices;
+  const bool few = first_slice + int(blockIdx.y) >= kJoinSlices;
   const Parts ps = few ? few_parts(a.workspace, n_cta) : wide_parts(a.workspace, n_cta);
   const int cta = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int slice = few ? 0 : y, slices = few ? 1 : kJoinSlices;
+  const int slice = (first_slice + blockIdx.y) % kJoinSlices;
   const Desc d = ps.desc[cta];
   if (!d.valid) return;
   const float ninf = -__int_as_float(0x7f800000);
+  const int n = d.n_used;
   int last = cta;                            // parts: slot 1 of cta, slot 0 of cta + 1 .. last
-  while (last + 1 < n_cta && d.total * (last + 1) / n_cta < d.end) ++last;
+  while (last + 1 < n && d.total * (last + 1) / n < d.end) ++last;
+  // (every CTA that is used has a share)
   const int tpb = kRows / a.G;
-  const int live0 = (d.two ? tpb : d.ntok) * a.G, live1 = d.two ? (d.ntok - tpb) * a.G : 0;
-  for (int i = slice * (kJoinThreads / 32) + warp; i < live0 + live1; i += slices * (kJoinThreads / 32)) {
-    const int b = i < live0 ? 0 : 1;
-    const int row = i - b * live0;
-    const int pr = b * kRows + row;
-    const int jr = row / a.G, hq = d.h * a.G + row - jr * a.G;
+  const int live0 = (d.two ? tpb : d.ntok) * a.G, live1 = d.two ? (d.ntok - tpb) * a.G : 0, live = live0 + live1;
+  for (int i = slice * (kJoinThreads / 32) + warp; i < live * d.heads; i += kJoinSlices * (kJoinThreads / 32)) {
+    const int hh = i / live, ii = i - hh * live;
+    const int b = ii < live0 ? 0 : 1, row = ii - b * live0;
+    const int pr = few ? i : b * kRows + row;
+    const int jr = row / a.G, hq = (d.h + hh) * a.G + row - jr * a.G;
     const int64_t qt = int64_t(d.a0) + d.j0 + b * tpb + jr;
-    auto ml_of = [&](int c) { return *reinterpret_cast<const float2*>(ps.ml(c, c == cta ? 1 : 0, D) + 2 * pr); };
-    float M = ninf;
-    for (int c = cta + lane; c <= last; c += 32)
-      if (d.total * c / n_cta < d.total * (c + 1) / n_cta) M = fmaxf(M, ml_of(c).x);
-    M = warp_max(M);
-    float L = 0.0f;
+    float M = ninf, L = 0.0f;
     float o[D / 32];
 #pragma unroll
     for (int k = 0; k < D / 32; ++k) o[k] = 0.0f;
-    for (int c = cta; c <= last; ++c) {
-      if (d.total * c / n_cta >= d.total * (c + 1) / n_cta) continue;      // a CTA without a share
-      const float2 y = ml_of(c);
-      if (y.y == 0.0f) continue;             // saw none of the row's tokens
-      const float al = y.x == ninf ? 1.0f : ex2(y.x - M);
-      L += y.y * al;
-      const float* p = ps.out(c, c == cta ? 1 : 0) + int64_t(pr) * D;
+    for (int c = cta + lane; c <= last; c += 32)
+      M = fmaxf(M, *(ps.ml(c, c == cta ? 1 : 0, D) + 2 * pr));
+    M = warp_max(M);
+    // 32 parts at a time: a lane has one's weight
+    for (int c0 = cta; c0 <= last; c0 += 32) {
+      const int c = c0 + lane;
+      float w = 0.0f;
+      if (c <= last) {
+        const float2 y = *reinterpret_cast<const float2*>(ps.ml(c, c == cta ? 1 : 0, D) + 2 * pr);
+        w = y.y == 0.0f ? 0.0f : (y.x == ninf ? 1.0f : ex2(y.x - M));      // 0: saw none of the row's tokens
+        L += y.y == 0.0f ? 0.0f : y.y * w;
+      }
+      const int m = min(32, last + 1 - c0);
+#pragma unroll 4
+      for (int e = 0; e < m; ++e) {
+        const float al = __shfl_sync(0xffffffffu, w, e);
+        const float* p = ps.out(c0 + e, c0 + e == cta ? 1 : 0) + int64_t(pr) * D;
 #pragma unroll
-      for (int k = 0; k < D / 32; ++k) o[k] = fmaf(p[k * 32 + lane], al, o[k]);
+        for (int k = 0; k < D / 32; ++k) {
+          const float x = p[k * 32 + lane];
+          o[k] = al == 0.0f ? o[k] : fmaf(x, al, o[k]);
+        }
+      }
     }
+    L = warp_sum(L);
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     uint16_t* dst = static_cast<uint16_t*>(a.out) + qt * a.out_stride_t + int64_t(hq) * a.out_stride_h;
 #pragma unroll
@@ -1192,7 +1206,7 @@ __global__ void __launch_bounds__(kJoinThreads) chunk_combine_kernel(const __gri
 
 // ------------------------------------------------------------------------------------ host side
 size_t chunk_workspace_bytes(int n_sm) {
-  return align256(chunk::few_offset(n_sm) + chunk::parts_bytes(n_sm, chunk::kFewRows));
+  return align256(chunk::few_offset(n_sm) + chunk::parts_bytes(n_sm, chunk::kFewParts));
 }
 
 bool chunk_umma_supported(const ChunkArgs& a, int dtype, const char** why) {
@@ -1238,7 +1252,7 @@ cudaError_t launch_chunk_t(const CUtensorMap& mkv, const CUtensorMap& mq, const 
     cfg.numAttrs = a.few_rows > 0 ? 1 : 0;   // beside chunk_few_kernel's last CTAs
     if ((e = cudaLaunchKernelEx(&cfg, k, mkv, mq, a, vec_out)) != cudaSuccess) return e;
   }
-  cfg.gridDim = dim3(grid, (wide ? chunk::kJoinSlices : 0) + (a.few_rows > 0 ? 1 : 0));
+  cfg.gridDim = dim3(grid, ((wide ? 1 : 0) + (a.few_rows > 0 ? 1 : 0)) * chunk::kJoinSlices);
   cfg.blockDim = dim3(chunk::kJoinThreads);
   cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
