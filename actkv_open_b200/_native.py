@@ -160,7 +160,13 @@ def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_ptr(device) -> int:
+    """The current stream's handle on ``device`` (without building a Stream object where torch can)."""
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -169,7 +175,9 @@ _status = {}
 
 def status_word(device) -> torch.Tensor:
     """A per-device int32 that kernels OR ACTKV_DEV_* bits into (never reset implicitly)."""
-    key = torch.device(device).index if torch.device(device).index is not None else torch.cuda.current_device()
+    key = device.index if isinstance(device, torch.device) else torch.device(device).index
+    if key is None:
+        key = torch.cuda.current_device()
     t = _status.get(key)
     if t is None:
         t = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", key))

@@ -5,6 +5,7 @@
 #include <stdio.h>
 
 #include <algorithm>
+#include <atomic>
 #include <string>
 
 #include "kernels.cuh"
@@ -109,10 +110,13 @@ namespace actkv {
 void set_last_error(const char* msg) { g_err = msg; }
 
 int device_sm_count() {
+  static std::atomic<int> known[64] = {};     // asked of the driver once per device
   int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    n = 0;
-  return n > 0 ? n : 148;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+  return n;
 }
 }  // namespace actkv
 

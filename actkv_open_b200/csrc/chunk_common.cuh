@@ -25,6 +25,37 @@ struct Share {
   int r0;                    // the session that holds the CTA's first unit of weight
 };
 
+// Query rows per KV head up to which chunk_few_kernel takes a session in this call, 0 when chunk_umma_kernel takes
+// all.  The two kernels run one after the other, so short work is not split between them: where the other kernel
+// has sessions too, those of few rows go to their own only when they hold bytes enough to win back a
+// kernel's start and end (about 15 us) by its higher rate: 512 MB of 16-bit rows (6.3 against 5.3 TB/s), 64 MB
+// of 8-bit ones (3.3 against 1.6 TB/s).  (16 sessions of 1000 to 9000 tokens with 3 to 7 new ones each, 4 query
+// heads per KV head, 330 MB: 120 us split, 77 us together.)
+// Every thread of the block calls it; `sums` is shared.
+template <int kThreads>
+__device__ __forceinline__ int few_rows_now(const ChunkArgs& a, int64_t (&sums)[2]) {
+  if (a.few_rows == 0 || int64_t(a.T) * a.G <= a.few_rows) return a.few_rows;      // none, or all of them
+  if (threadIdx.x < 2) sums[threadIdx.x] = 0;
+  __syncthreads();
+  int64_t few = 0, all = 0;
+  for (int r = threadIdx.x; r < a.R; r += kThreads) {
+    const int A = a.q_off[r + 1] - a.q_off[r];
+    if (A <= 0) continue;
+    const int s = max(a.seq_used[r], 1);
+    all += s;
+    if (A * a.G <= a.few_rows) few += s;
+  }
+  few = warp_sum(few);
+  all = warp_sum(all);
+  if ((threadIdx.x & 31) == 0 && all > 0) {
+    atomicAdd(reinterpret_cast<unsigned long long*>(&sums[0]), static_cast<unsigned long long>(few));
+    atomicAdd(reinterpret_cast<unsigned long long*>(&sums[1]), static_cast<unsigned long long>(all));
+  }
+  __syncthreads();
+  const int64_t bytes = sums[0] * a.Hkv * a.D * 2 * (a.quant ? 1 : 2);
+  return sums[0] == sums[1] || bytes >= (int64_t(a.quant ? 64 : 512) << 20) ? a.few_rows : 0;
+}
+
 // CTAs that get work when a share is at least `least`.
 __device__ __forceinline__ int used_ctas(int64_t total, int n, int least) {
   return int(max(int64_t(1), min(int64_t(n), total / least)));

@@ -124,7 +124,7 @@ __device__ __forceinline__ uint32_t drop_bad(uint32_t u, uint32_t hide, bool& fo
 
 struct Sched {
   Share share;
-  int64_t scan[kWarps];
+  int64_t scan[kWarps], sums[2];
   int bad_v;
 };
 static_assert(sizeof(Sched) <= 512, "the schedule's place in shared memory");
@@ -154,9 +154,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few_kernel(const __grid_con
   const int HG = a.Hkv % 8 == 0 ? 8 : (a.Hkv % 4 == 0 ? 4 : (a.Hkv % 2 == 0 ? 2 : 1));   // heads per unit
   const int wph = kWarps / HG, round = kStep * wph;         // warps per head, tokens of a round of theirs
   const int my_head = warp % HG, my_part = warp / HG;
+  const int few_rows = few_rows_now<kThreads>(a, sched.sums);
+  if (few_rows == 0) return;
   share_out<kThreads>(a.R, [&](int r) -> int64_t {
     const int A = a.q_off[r + 1] - a.q_off[r];
-    return A > 0 && A * a.G <= a.few_rows ? int64_t(a.Hkv / HG) * (kRoundCost + (a.seq_used[r] + round - 1) / round) : 0;
+    return A > 0 && A * a.G <= few_rows ? int64_t(a.Hkv / HG) * (kRoundCost + (a.seq_used[r] + round - 1) / round) : 0;
   }, sched.share, sched.scan, cta, n_cta, kMinRounds);
   const int64_t total = sched.share.total;
   const int n_used = used_ctas(total, n_cta, kMinRounds);
@@ -175,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few_kernel(const __grid_con
 
   for (; r < a.R && at < hi; ++r, hg = 0) {
     const int a0 = a.q_off[r], A = a.q_off[r + 1] - a0, S = a.seq_used[r];
-    if (A <= 0 || A * a.G > a.few_rows) continue;
+    if (A <= 0 || A * a.G > few_rows) continue;
     const int rows = A * a.G;
     const int nt = S > 0 ? (S + round - 1) / round : 0;
     const int64_t weight = kRoundCost + nt;
@@ -569,7 +571,8 @@ template <int D, bool BF16, bool QUANT>
 cudaError_t launch_few_t(const ChunkArgs& a, int grid, cudaStream_t st) {
   auto k = chunk::few::chunk_few_kernel<D, BF16, QUANT>;
   constexpr int bytes = int(chunk::few::Ring<D, QUANT>::kSmemBytes);
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  static SmemLimit limit;
+  const cudaError_t e = limit.set(reinterpret_cast<const void*>(k), bytes);
   if (e != cudaSuccess) return e;
   const bool vec_out = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_stride_t % 8 == 0 && a.out_stride_h % 8 == 0;
   k<<<grid, chunk::few::kThreads, bytes, st>>>(a, vec_out);

@@ -81,7 +81,8 @@ struct Sched {               // in shared memory
   uint32_t tmem;
   int abort_flag;
   int bad_v;                 // a value that some row of the unit does not see is not finite
-  int64_t scan[kMaxThreads / 32];
+  int few_rows;              // sessions of at most so many rows are chunk_few_kernel's in this call
+  int64_t scan[kMaxThreads / 32], sums[2];
   Unit units[kUnitSlots];    // from the TMA warp, which alone walks the schedule; r < 0 ends it
 };
 static_assert(sizeof(Sched) <= kSchedBytes, "the schedule's place in shared memory");
@@ -108,14 +109,14 @@ struct Walker {
   const ChunkArgs* a;
   Geometry geo;
   int64_t lo, hi, at;
-  int r, h, j, S, A, a0;
+  int r, h, j, S, A, a0, few_rows;
 
   __device__ void load() {
     while (r < a->R) {
       a0 = a->q_off[r];
       A = a->q_off[r + 1] - a0;
       S = a->seq_used[r];
-      if (A > 0 && A * a->G > a->few_rows) return;
+      if (A > 0 && A * a->G > few_rows) return;
       ++r;
     }
   }
@@ -124,6 +125,7 @@ struct Walker {
     lo = s.share.total * cta / n;
     hi = cta < n ? s.share.total * (cta + 1) / n : lo;
     r = s.share.r0;
+    few_rows = s.few_rows;
     h = j = S = A = a0 = 0;
     at = s.share.pre;
     if (lo >= hi) {
@@ -175,9 +177,11 @@ struct Walker {
 template <int kThreads>
 __device__ void make_schedule(const ChunkArgs& a, Sched& s, int cta, int n) {
   const Geometry geo(a);
+  const int few_rows = few_rows_now<kThreads>(a, s.sums);
+  if (threadIdx.x == 0) s.few_rows = few_rows;
   share_out<kThreads>(a.R, [&](int r) -> int64_t {
     const int A = a.q_off[r + 1] - a.q_off[r];
-    return A * a.G > a.few_rows ? a.Hkv * geo.head_weight(a.seq_used[r], A) : 0;
+    return A > 0 && A * a.G > few_rows ? a.Hkv * geo.head_weight(a.seq_used[r], A) : 0;
   }, s.share, s.scan, cta, n, 1);
 }
 
@@ -452,14 +456,18 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     wide_parts(a.workspace, n_cta).desc[cta].valid = 0;
   }
+  pdl_trigger();
+  __syncthreads();
+  make_schedule<threads(QUANT)>(a, sched, cta, n_cta);
+  if (sched.share.total == 0) {              // everything is chunk_few_kernel's
+    pdl_wait();
+    return;
+  }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&sched.tmem))
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  pdl_trigger();
-  __syncthreads();
-  make_schedule<threads(QUANT)>(a, sched, cta, n_cta);
   fence_before();
   __syncthreads();
   fence_after();
@@ -1137,14 +1145,19 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
 
 // ------------------------------------------------------------------------------------ joining split units
 constexpr int kJoinThreads = 256;
-constexpr int kJoinSlices = 8;               // CTAs per split unit, rows dealt in turn
+constexpr int kJoinWarps = kJoinThreads / 32;
+constexpr int kJoinSlices = 16;              // CTAs per split unit, rows dealt in turn
 
-// One CTA per (CTA that began a unit and left it, slice of its rows); a warp per row.  The slices from
-// kJoinSlices on are for the units of chunk_few_kernel.
+// One CTA per (CTA that began a unit and left it, slice of its rows): a warp per row where a row has up to 8
+// parts, else its warps take them in turn and the warps' sums are added in order (one token over 2000: 21
+// parts, 28.7 -> 22.4 us for the call).  The slices from kJoinSlices on are for the units of
+// chunk_few_kernel.  Bound by latency: two dependent reads per eight parts, a row after the other.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kJoinThreads) chunk_combine_kernel(const __grid_constant__ ChunkArgs a, int n_cta,
                                                                      int first_slice) {
+  __shared__ float sh_m[kJoinWarps], sh_l[kJoinWarps], sh_o[kJoinWarps][D];
   pdl_wait();
+  constexpr int kPer = D / 32;                              // values per lane
   const bool few = first_slice + int(blockIdx.y) >= kJoinSlices;
   const Parts ps = few ? few_parts(a.workspace, n_cta) : wide_parts(a.workspace, n_cta);
   const int cta = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1152,53 +1165,82 @@ __global__ void __launch_bounds__(kJoinThreads) chunk_combine_kernel(const __gri
   const Desc d = ps.desc[cta];
   if (!d.valid) return;
   const float ninf = -__int_as_float(0x7f800000);
-  const int n = d.n_used;
-  int last = cta;                            // parts: slot 1 of cta, slot 0 of cta + 1 .. last
-  while (last + 1 < n && d.total * (last + 1) / n < d.end) ++last;
-  // (every CTA that is used has a share)
+  // parts: slot 1 of cta, slot 0 of cta + 1 .. last, the last CTA whose share total * c / n_used starts before end
+  const int last = int((d.end * d.n_used - 1) / d.total);
   const int tpb = kRows / a.G;
   const int live0 = (d.two ? tpb : d.ntok) * a.G, live1 = d.two ? (d.ntok - tpb) * a.G : 0, live = live0 + live1;
-  for (int i = slice * (kJoinThreads / 32) + warp; i < live * d.heads; i += kJoinSlices * (kJoinThreads / 32)) {
+  // where row i of the unit is: in the parts, and in the results
+  auto place = [&](int i, int& pr, int64_t& qt, int& hq) {
     const int hh = i / live, ii = i - hh * live;
     const int b = ii < live0 ? 0 : 1, row = ii - b * live0;
-    const int pr = few ? i : b * kRows + row;
-    const int jr = row / a.G, hq = (d.h + hh) * a.G + row - jr * a.G;
-    const int64_t qt = int64_t(d.a0) + d.j0 + b * tpb + jr;
-    float M = ninf, L = 0.0f;
-    float o[D / 32];
+    const int jr = row / a.G;
+    pr = few ? i : b * kRows + row;
+    hq = (d.h + hh) * a.G + row - jr * a.G;
+    qt = int64_t(d.a0) + d.j0 + b * tpb + jr;
+  };
+  // a warp's sum over the parts c, c + step, ..
+  float M, L, o[kPer];
+  auto add_parts = [&](int pr, int c, int step) {
+    M = ninf;
+    L = 0.0f;
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) o[k] = 0.0f;
-    for (int c = cta + lane; c <= last; c += 32)
-      M = fmaxf(M, *(ps.ml(c, c == cta ? 1 : 0, D) + 2 * pr));
-    M = warp_max(M);
-    // 32 parts at a time: a lane has one's weight
-    for (int c0 = cta; c0 <= last; c0 += 32) {
-      const int c = c0 + lane;
-      float w = 0.0f;
-      if (c <= last) {
-        const float2 y = *reinterpret_cast<const float2*>(ps.ml(c, c == cta ? 1 : 0, D) + 2 * pr);
-        w = y.y == 0.0f ? 0.0f : (y.x == ninf ? 1.0f : ex2(y.x - M));      // 0: saw none of the row's tokens
-        L += y.y == 0.0f ? 0.0f : y.y * w;
-      }
-      const int m = min(32, last + 1 - c0);
+    for (int k = 0; k < kPer; ++k) o[k] = 0.0f;
 #pragma unroll 4
-      for (int e = 0; e < m; ++e) {
-        const float al = __shfl_sync(0xffffffffu, w, e);
-        const float* p = ps.out(c0 + e, c0 + e == cta ? 1 : 0) + int64_t(pr) * D;
+    for (; c <= last; c += step) {
+      const float* p = ps.out(c, c == cta ? 1 : 0);
+      const float2 y = *reinterpret_cast<const float2*>(p + int64_t(ps.rows) * D + 2 * pr);
+      float x[kPer];
 #pragma unroll
-        for (int k = 0; k < D / 32; ++k) {
-          const float x = p[k * 32 + lane];
-          o[k] = al == 0.0f ? o[k] : fmaf(x, al, o[k]);
-        }
-      }
+      for (int k = 0; k < kPer; ++k) x[k] = p[int64_t(pr) * D + k * 32 + lane];
+      if (y.y == 0.0f) continue;             // saw none of the row's tokens
+      const float Mn = fmaxf(M, y.x), al = M == Mn ? 1.0f : ex2(M - Mn), be = y.x == Mn ? 1.0f : ex2(y.x - Mn);
+      M = Mn;
+      L = fmaf(L, al, y.y * be);
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) o[k] = fmaf(o[k], al, x[k] * be);
     }
-    L = warp_sum(L);
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    uint16_t* dst = static_cast<uint16_t*>(a.out) + qt * a.out_stride_t + int64_t(hq) * a.out_stride_h;
+  };
+  auto lse_of = [&](float m, float l) { return l == 0.0f ? ninf : (m == ninf ? l : (m + log2f(l)) * 0.69314718055994531f); };
+  int pr, hq;
+  int64_t qt;
+  if (last - cta < kJoinWarps) {              // few parts: a warp per row
+    for (int i = slice * kJoinWarps + warp; i < live * d.heads; i += kJoinSlices * kJoinWarps) {
+      place(i, pr, qt, hq);
+      add_parts(pr, cta, 1);
+      uint16_t* dst = static_cast<uint16_t*>(a.out) + qt * a.out_stride_t + int64_t(hq) * a.out_stride_h;
+      const float inv = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
-    for (int k = 0; k < D / 32; ++k) dst[k * 32 + lane] = uint16_t(pack2<BF16>(o[k] * inv, 0.0f));
-    if (lane == 0)
-      a.lse[qt * a.lse_stride_t + hq] = L == 0.0f ? ninf : (M == ninf ? L : (M + log2f(L)) * 0.69314718055994531f);
+      for (int k = 0; k < kPer; ++k) dst[k * 32 + lane] = uint16_t(pack2<BF16>(o[k] * inv, 0.0f));
+      if (lane == 0) a.lse[qt * a.lse_stride_t + hq] = lse_of(M, L);
+    }
+    return;
+  }
+  for (int i = slice; i < live * d.heads; i += kJoinSlices) {   // many: the warps share a row's
+    place(i, pr, qt, hq);
+    add_parts(pr, cta + warp, kJoinWarps);
+    if (lane == 0) {
+      sh_m[warp] = M;
+      sh_l[warp] = L;
+    }
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) sh_o[warp][k * 32 + lane] = o[k];
+    __syncthreads();
+    if (threadIdx.x < D) {
+      float m = ninf, l = 0.0f, y = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) m = fmaxf(m, sh_m[w]);
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) {
+        if (sh_l[w] == 0.0f) continue;
+        const float al = sh_m[w] == m ? 1.0f : ex2(sh_m[w] - m);
+        l = fmaf(sh_l[w], al, l);
+        y = fmaf(sh_o[w][threadIdx.x], al, y);
+      }
+      static_cast<uint16_t*>(a.out)[qt * a.out_stride_t + int64_t(hq) * a.out_stride_h + threadIdx.x] =
+          uint16_t(pack2<BF16>(l == 0.0f ? 0.0f : y / l, 0.0f));
+      if (threadIdx.x == 0) a.lse[qt * a.lse_stride_t + hq] = lse_of(m, l);
+    }
+    __syncthreads();
   }
 }
 
@@ -1235,8 +1277,7 @@ namespace {
 template <int D, bool BF16, bool QUANT>
 cudaError_t launch_chunk_t(const CUtensorMap& mkv, const CUtensorMap& mq, const ChunkArgs& a, int grid, cudaStream_t st) {
   auto k = chunk::chunk_umma_kernel<D, BF16, QUANT>;
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(chunk::Layout<D, QUANT>::kSmemBytes));
-  if (e != cudaSuccess) return e;
+  cudaError_t e = cudaSuccess;
   const bool vec_out = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_stride_t % 8 == 0 && a.out_stride_h % 8 == 0;
   cudaLaunchConfig_t cfg = {};
   cfg.stream = st;
@@ -1249,6 +1290,8 @@ cudaError_t launch_chunk_t(const CUtensorMap& mkv, const CUtensorMap& mq, const 
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(chunk::threads(QUANT));
     cfg.dynamicSmemBytes = chunk::Layout<D, QUANT>::kSmemBytes;
+    static SmemLimit limit;
+    if ((e = limit.set(reinterpret_cast<const void*>(k), int(cfg.dynamicSmemBytes))) != cudaSuccess) return e;
     cfg.numAttrs = a.few_rows > 0 ? 1 : 0;   // beside chunk_few_kernel's last CTAs
     if ((e = cudaLaunchKernelEx(&cfg, k, mkv, mq, a, vec_out)) != cudaSuccess) return e;
   }
@@ -1263,50 +1306,6 @@ cudaError_t launch_chunk_t(const CUtensorMap& mkv, const CUtensorMap& mq, const 
 
 cudaError_t launch_chunk_umma(const ChunkArgs& args, int dtype, cudaStream_t st, const char** why) {
   ChunkArgs a = args;
-  EncodeTiledFn enc = get_encode_fn();
-  if (!enc) {
-    *why = "cuTensorMapEncodeTiled unavailable";
-    return cudaErrorNotSupported;
-  }
-  const CUtensorMapDataType dt = dtype == ACTKV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  const cuuint32_t es[5] = {1, 1, 1, 1, 1};
-  CUtensorMap mkv, mq;
-  if (a.quant) {
-    // (the heads' values of a row, slot, plane): one head's values of a paged block per box
-    const cuuint32_t rows = cuuint32_t(a.BS < chunk::kTile ? a.BS : chunk::kTile);
-    const cuuint64_t dims[3] = {cuuint64_t(a.Hkv) * a.D, cuuint64_t(a.NB) * a.BS, 2};
-    const cuuint64_t strides[2] = {cuuint64_t(a.kv_stride_s), cuuint64_t(a.kv_stride_kv)};
-    const cuuint32_t box[3] = {cuuint32_t(a.D), rows, 1};
-    if (enc(&mkv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(a.kv), dims, strides, box, es,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, a.D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
-      *why = "cuTensorMapEncodeTiled rejected the layout of the 8-bit rows";
-      return cudaErrorInvalidValue;
-    }
-  } else {
-    // (64 dims, slot within 8, D-half of a head, group of 8 slots, plane): a box leaves every 8-token
-    // group's D-halves next to one another, so the groups of a tile are evenly spaced
-    const cuuint32_t halves = cuuint32_t(a.D / 64), rows = cuuint32_t(a.BS < chunk::kTile ? a.BS : chunk::kTile);
-    const cuuint64_t row = cuuint64_t(a.kv_stride_s) * 2;
-    const cuuint64_t dims[5] = {64, 8, cuuint64_t(a.Hkv) * halves, cuuint64_t(a.NB) * a.BS / 8, 2};
-    const cuuint64_t strides[4] = {row, 128, row * 8, cuuint64_t(a.kv_stride_kv) * 2};
-    const cuuint32_t box[5] = {64, 8, halves, rows / 8, 1};
-    if (enc(&mkv, dt, 5, const_cast<void*>(a.kv), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
-      *why = "cuTensorMapEncodeTiled rejected the cache layout";
-      return cudaErrorInvalidValue;
-    }
-  }
-  {
-    const cuuint64_t dims[3] = {cuuint64_t(a.D), cuuint64_t(a.Hq), cuuint64_t(a.T)};
-    const cuuint64_t strides[2] = {cuuint64_t(a.q_stride_h) * 2, cuuint64_t(a.q_stride_t) * 2};
-    const cuuint32_t box[3] = {64, cuuint32_t(a.G), cuuint32_t(chunk::kRows / a.G)};
-    if (enc(&mq, dt, 3, const_cast<void*>(a.q), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
-      *why = "cuTensorMapEncodeTiled rejected the query layout";
-      return cudaErrorInvalidValue;
-    }
-  }
   *why = "chunk attention";
   const int grid = device_sm_count();
   // sessions of few query rows go to a kernel of their own, where a GQA group fits it
@@ -1315,6 +1314,53 @@ cudaError_t launch_chunk_umma(const ChunkArgs& args, int dtype, cudaStream_t st,
     const cudaError_t e = launch_chunk_few(a, dtype, grid, st);
     if (e != cudaSuccess) return e;
   }
+  CUtensorMap mkv, mq;
+  if (a.T * int64_t(a.G) > a.few_rows) {     // chunk_umma_kernel is launched
+    EncodeTiledFn enc = get_encode_fn();
+    if (!enc) {
+      *why = "cuTensorMapEncodeTiled unavailable";
+      return cudaErrorNotSupported;
+    }
+    const CUtensorMapDataType dt = dtype == ACTKV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const cuuint32_t es[5] = {1, 1, 1, 1, 1};
+    if (a.quant) {
+      // (the heads' values of a row, slot, plane): one head's values of a paged block per box
+      const cuuint32_t rows = cuuint32_t(a.BS < chunk::kTile ? a.BS : chunk::kTile);
+      const cuuint64_t dims[3] = {cuuint64_t(a.Hkv) * a.D, cuuint64_t(a.NB) * a.BS, 2};
+      const cuuint64_t strides[2] = {cuuint64_t(a.kv_stride_s), cuuint64_t(a.kv_stride_kv)};
+      const cuuint32_t box[3] = {cuuint32_t(a.D), rows, 1};
+      if (enc(&mkv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(a.kv), dims, strides, box, es,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, a.D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+        *why = "cuTensorMapEncodeTiled rejected the layout of the 8-bit rows";
+        return cudaErrorInvalidValue;
+      }
+    } else {
+      // (64 dims, slot within 8, D-half of a head, group of 8 slots, plane): a box leaves every 8-token
+      // group's D-halves next to one another, so the groups of a tile are evenly spaced
+      const cuuint32_t halves = cuuint32_t(a.D / 64), rows = cuuint32_t(a.BS < chunk::kTile ? a.BS : chunk::kTile);
+      const cuuint64_t row = cuuint64_t(a.kv_stride_s) * 2;
+      const cuuint64_t dims[5] = {64, 8, cuuint64_t(a.Hkv) * halves, cuuint64_t(a.NB) * a.BS / 8, 2};
+      const cuuint64_t strides[4] = {row, 128, row * 8, cuuint64_t(a.kv_stride_kv) * 2};
+      const cuuint32_t box[5] = {64, 8, halves, rows / 8, 1};
+      if (enc(&mkv, dt, 5, const_cast<void*>(a.kv), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+        *why = "cuTensorMapEncodeTiled rejected the cache layout";
+        return cudaErrorInvalidValue;
+      }
+    }
+    {
+      const cuuint64_t dims[3] = {cuuint64_t(a.D), cuuint64_t(a.Hq), cuuint64_t(a.T)};
+      const cuuint64_t strides[2] = {cuuint64_t(a.q_stride_h) * 2, cuuint64_t(a.q_stride_t) * 2};
+      const cuuint32_t box[3] = {64, cuuint32_t(a.G), cuuint32_t(chunk::kRows / a.G)};
+      if (enc(&mq, dt, 3, const_cast<void*>(a.q), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+        *why = "cuTensorMapEncodeTiled rejected the query layout";
+        return cudaErrorInvalidValue;
+      }
+    }
+  }
+  *why = "chunk attention";
   const bool bf = dtype == ACTKV_BF16;
   if (a.quant) {
     if (a.D == 128) return bf ? launch_chunk_t<128, true, true>(mkv, mq, a, grid, st) : launch_chunk_t<128, false, true>(mkv, mq, a, grid, st);

@@ -1,5 +1,7 @@
 // Declarations shared by the kernel translation units and the C-ABI layer.
 #pragma once
+
+#include <atomic>
 #include "common.cuh"
 #include "score_common.cuh"
 
@@ -321,6 +323,21 @@ struct ChunkArgs {
   void* workspace;           // chunk_workspace_bytes()
   int32_t* status;
   int few_rows;              // sessions of at most so many rows per KV head are chunk_few_kernel's
+};
+
+// A kernel's shared memory limit, raised once per device (the call costs more than the launch's other work).
+struct SmemLimit {
+  std::atomic<uint64_t> done{0};             // a bit per device
+  cudaError_t set(const void* kernel, int bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = uint64_t(1) << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
+  }
 };
 
 size_t chunk_workspace_bytes(int n_sm);

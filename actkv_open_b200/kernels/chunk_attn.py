@@ -29,21 +29,27 @@ def chunk_workspace(device) -> torch.Tensor:
 
 def _check(q, q_off, cache, block_table, seq_used, out, lse, workspace):
     """Checks shared by the two caches; returns (device, out, lse, workspace)."""
-    dev = N.require_cuda(q, q_off, cache, block_table, seq_used, out, lse, workspace)
+    dev = q.device
+    if dev.type != "cuda" or not (q_off.device == cache.device == block_table.device == seq_used.device == dev):
+        N.require_cuda(q, q_off, cache, block_table, seq_used)
     assert q.dim() == 3, "q is [T, Hq, D]"
-    assert q.stride(2) == 1 and block_table.stride(1) == 1
-    assert q_off.dtype == torch.int32 and seq_used.dtype == torch.int32 and block_table.dtype == torch.int32
-    assert q_off.is_contiguous() and seq_used.is_contiguous()
+    i32 = torch.int32
+    assert q_off.dtype is i32 and seq_used.dtype is i32 and block_table.dtype is i32
+    assert q.stride(2) == 1 and block_table.stride(1) == 1 and q_off.is_contiguous() and seq_used.is_contiguous()
     r_n = seq_used.shape[0]
     assert q_off.shape[0] == r_n + 1 and block_table.shape[0] == r_n, "q_off [R + 1], block_table [R, MB], seq_used [R]"
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    else:
+        assert out.device == dev and out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1
     if lse is None:
         lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev)
-    assert out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1
-    assert lse.shape == q.shape[:2] and lse.dtype == torch.float32 and lse.stride(1) == 1
+    else:
+        assert lse.device == dev and lse.shape == q.shape[:2] and lse.dtype == torch.float32 and lse.stride(1) == 1
     if workspace is None:
         workspace = chunk_workspace(dev)
+    else:
+        assert workspace.device == dev and workspace.is_contiguous()
     return dev, out, lse, workspace
 
 
