@@ -15,20 +15,21 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kItems = 4;                   // items in flight per lane
 
+// 16 values as they are in memory.
 template <typename T>
-__device__ __forceinline__ void load16(const T* p, bool vec, float (&x)[16]) {
+struct Raw16 {
+  uint4 u[sizeof(T)];
+};
+
+template <typename T>
+__device__ __forceinline__ void load16(const T* p, bool vec, Raw16<T>& r) {
   if (vec) {
-    constexpr int kPer = 16 / sizeof(T);
 #pragma unroll
-    for (int i = 0; i < 16 / kPer; ++i) {
-      const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p) + i);
-      const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) x[i * kPer + k] = to_f32(e[k]);
-    }
+    for (int i = 0; i < int(sizeof(T)); ++i) r.u[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
   } else {
+    T* e = reinterpret_cast<T*>(r.u);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = to_f32(p[i]);
+    for (int k = 0; k < 16; ++k) e[k] = p[k];
   }
 }
 
@@ -49,7 +50,7 @@ __device__ __forceinline__ void store16(T* p, bool vec, const float (&x)[16]) {
       T* e = reinterpret_cast<T*>(&u);
 #pragma unroll
       for (int k = 0; k < kPer; ++k) e[k] = from_f32<T>(x[i * kPer + k]);
-      reinterpret_cast<uint4*>(p)[i] = u;
+      __stcs(reinterpret_cast<uint4*>(p) + i, u);
     }
   } else {
 #pragma unroll
@@ -75,6 +76,8 @@ template <typename T, bool WRITE>
 __global__ void __launch_bounds__(kThreads) quant_move_kernel(QuantMoveArgs a) {
   const int lane = threadIdx.x & 31;
   const int per_row = a.Hkv * a.D / 16;                     // items of one plane
+  const int shift = (per_row & (per_row - 1)) == 0 ? __ffs(per_row) - 1 : -1;
+  const bool packed = a.ext_stride_h[0] == a.D && a.ext_stride_h[1] == a.D;     // heads next to one another
   const int items = a.planes * per_row;                     // items of one token
   const int runs = (items + 32 * kItems - 1) / (32 * kItems);
   const int64_t warp = (int64_t(blockIdx.x) * kThreads + threadIdx.x) >> 5;
@@ -89,7 +92,7 @@ __global__ void __launch_bounds__(kThreads) quant_move_kernel(QuantMoveArgs a) {
     T* ext[kItems];
     uint8_t* pay[kItems];
     uint8_t* sc[kItems];
-    float x[kItems][16];
+    Raw16<T> in[WRITE ? kItems : 1];
     uint4 raw[kItems];
     uint32_t byte[kItems];
     // whether a lane has item i is the same for both lanes of a pair: per_row is even
@@ -98,19 +101,23 @@ __global__ void __launch_bounds__(kThreads) quant_move_kernel(QuantMoveArgs a) {
       const int f = (run * kItems + i) * 32 + lane;
       ext[i] = nullptr;
       if (f >= items) continue;
-      const int lp = f / per_row, c = f - lp * per_row;
+      const int lp = shift >= 0 ? f >> shift : f / per_row, c = f - lp * per_row;
       const int l = a.both ? lp >> 1 : lp, p = a.both ? lp & 1 : a.only;
-      const int h = c * 16 / a.D, d = c * 16 - h * a.D;
+      int64_t at = c * 16;
+      if (!packed) {
+        const int h = c * 16 / a.D;
+        at = int64_t(h) * a.ext_stride_h[p] + (c * 16 - h * a.D);
+      }
       T* base = static_cast<T*>(p ? a.v : a.k);
-      ext[i] = base + int64_t(l) * a.ext_stride_l[p] + int64_t(t) * a.ext_stride_t[p] + int64_t(h) * a.ext_stride_h[p] + d;
+      ext[i] = base + (int64_t(l) * a.ext_stride_l[p] + int64_t(t) * a.ext_stride_t[p] + at);
       uint8_t* row = a.rows + int64_t(l) * a.rows_stride_l + int64_t(p) * a.rows_stride_kv + slot;
       pay[i] = row + c * 16;
       sc[i] = row + a.Hkv * a.D + c / 2;
       if constexpr (WRITE) {
-        load16(ext[i], a.vec, x[i]);
+        load16(ext[i], a.vec, in[i]);
       } else {
         if (a.vec_rows) {
-          raw[i] = *reinterpret_cast<const uint4*>(pay[i]);
+          raw[i] = __ldcs(reinterpret_cast<const uint4*>(pay[i]));
         } else {
           uint8_t* b = reinterpret_cast<uint8_t*>(&raw[i]);
           for (int k = 0; k < 16; ++k) b[k] = pay[i][k];
@@ -121,10 +128,15 @@ __global__ void __launch_bounds__(kThreads) quant_move_kernel(QuantMoveArgs a) {
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
       if constexpr (WRITE) {
+        float x[16];
         uint32_t top = 0;
-        if (ext[i])
+        const T* e = reinterpret_cast<const T*>(in[i].u);
 #pragma unroll
-          for (int k = 0; k < 16; ++k) top = max(top, __float_as_uint(x[i][k]) & 0x7fffffffu);
+        for (int k = 0; k < 16; ++k) {
+          x[k] = to_f32(e[k]);
+          top = max(top, __float_as_uint(x[k]) & 0x7fffffffu);
+        }
+        if (!ext[i]) top = 0;
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));      // the group's other 16 values
         if (!ext[i]) continue;
         const uint32_t b = scale_byte(top);
@@ -132,8 +144,8 @@ __global__ void __launch_bounds__(kThreads) quant_move_kernel(QuantMoveArgs a) {
         uint32_t u[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const uint32_t lo = f32_e4m3x2(x[i][4 * k] * inv, x[i][4 * k + 1] * inv);
-          const uint32_t hi = f32_e4m3x2(x[i][4 * k + 2] * inv, x[i][4 * k + 3] * inv);
+          const uint32_t lo = f32_e4m3x2(x[4 * k] * inv, x[4 * k + 1] * inv);
+          const uint32_t hi = f32_e4m3x2(x[4 * k + 2] * inv, x[4 * k + 3] * inv);
           u[k] = b == 255u ? 0u : (lo & 0xffffu) | (hi << 16);
         }
         if (a.vec_rows) {
@@ -144,15 +156,16 @@ __global__ void __launch_bounds__(kThreads) quant_move_kernel(QuantMoveArgs a) {
         if ((lane & 1) == 0) *sc[i] = uint8_t(b);
       } else {
         if (!ext[i]) continue;
+        float x[16];
         const float s = scale_of(byte[i]);
         const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const float2 v = e4m3x2_f32((u[k >> 1] >> (16 * (k & 1))) & 0xffffu);
-          x[i][2 * k] = v.x * s;
-          x[i][2 * k + 1] = v.y * s;
+          x[2 * k] = v.x * s;
+          x[2 * k + 1] = v.y * s;
         }
-        store16(ext[i], a.vec, x[i]);
+        store16(ext[i], a.vec, x);
       }
     }
   }
