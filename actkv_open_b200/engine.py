@@ -31,8 +31,10 @@ from . import _native as N
 from . import sharding
 from ._native import OutOfBlocks
 from .config import EvictionConfig
+from .kernels.chunk_attn import chunk_workspace, paged_chunk_attention
 from .kernels.lse_attn import (action_region_lse, action_scores_region, region_lse_workspace_bytes,
                                 score_region_workspace_bytes, stream_signal)
+from .kernels.quant_cache import (dequantize_read, paged_chunk_attention_quant, quant_row_bytes)
 
 
 class DevicePagedCache:
@@ -54,6 +56,7 @@ class DevicePagedCache:
         self.pinned = torch.zeros(max_sessions, max_tokens, dtype=torch.uint8, device=self.device)
         self.n_sessions = 0
         self._blocks_ws = None
+        self._chunk_ws = None
         # pinned staging for the small per-call inputs of append / release (offsets, masks): reused,
         # guarded by the event of the last copy out of it
         self._stage = torch.empty(max_sessions + 1, dtype=torch.int32).pin_memory()
@@ -179,11 +182,117 @@ class DevicePagedCache:
             self.pinned.data_ptr(), self.pinned.stride(0), self.max_tokens, R, ws.data_ptr(), ws.numel(),
             N.status_word(dev).data_ptr(), N.stream_ptr(dev)), "release")
 
+    def chunk_attention(self, layer: int, q: torch.Tensor, q_off: torch.Tensor, scale: float | None = None,
+                        out: torch.Tensor | None = None, lse: torch.Tensor | None = None):
+        """Attention of each session's newest tokens (appended before) over its cache, one layer:
+        (out [T, Hq, D], lse [T, Hq]) for queries q [T, Hq, D] packed by q_off [R+1] (device int32),
+        see ``paged_chunk_attention``.  The lse of the action tokens is what ``EvictionPipeline.step``
+        takes.  Calls on one cache share a workspace: keep them on one stream."""
+        R = q_off.shape[0] - 1
+        if self._chunk_ws is None:
+            self._chunk_ws = chunk_workspace(self.device)
+        return paged_chunk_attention(q, q_off, self.kv[layer], self.block_table[:R], self.seq_used[:R], scale=scale,
+                                     out=out, lse=lse, workspace=self._chunk_ws)
+
+    def keys16(self, l0: int, l1: int) -> torch.Tensor:
+        """Layers [l0, l1) as the scoring kernels read them: [l1 - l0, 2, NB, BS, Hkv, D]."""
+        return self.kv[l0:l1]
+
+    def layer_groups(self, l0: int, l1: int):
+        """The runs of layers that ``keys16`` gives at a time."""
+        return [(l0, l1)]
+
     def flat_planes(self):
         """(plane_stride_bytes, slot_stride_bytes, row_bytes, n_slots) of the [2L, NB*BS, Hkv*D] view."""
         es = self.kv.element_size()
         row = self.n_kv_heads * self.head_dim * es
         return self.kv.stride(1) * es, row, row, self.num_blocks * self.block_size
+
+
+class QuantPagedCache(DevicePagedCache):
+    """A ``DevicePagedCache`` whose rows are held in 8 bits (``kernels.quant_cache``): half the memory
+    per token, and half the bytes per attention call.  append quantises; release, eviction and
+    compaction move rows as bytes; ``EvictionPipeline`` scores it from keys read back into 16 bits,
+    a few layers at a time.  ``dtype`` (bf16 or fp16) is the type of its queries and outputs.
+    ``rows`` is the cache as the functions of ``kernels.quant_cache`` take it."""
+
+    def __init__(self, num_blocks: int, block_size: int, n_kv_heads: int, head_dim: int, n_layers: int,
+                 max_sessions: int, max_tokens: int, dtype=torch.bfloat16, device="cuda"):
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ValueError(f"dtype {dtype}: the 8-bit cache works in bf16 or fp16")
+        row = quant_row_bytes(n_kv_heads, head_dim)
+        super().__init__(num_blocks, block_size, 1, row, n_layers, max_sessions, max_tokens, dtype=torch.uint8,
+                         device=device)
+        self.n_kv_heads, self.head_dim, self.row_bytes, self.dtype = n_kv_heads, head_dim, row, dtype
+        self.rows = self.kv.view(n_layers, 2, num_blocks, block_size, row)
+        self._keys = None
+
+    def append(self, k_new: torch.Tensor, v_new: torch.Tensor, n_new, max_new: int | None = None,
+               check: bool = True) -> None:
+        """``DevicePagedCache.append`` with the new rows quantised; ``max_new`` is not needed."""
+        L, H, D = self.n_layers, self.n_kv_heads, self.head_dim
+        assert k_new.shape == v_new.shape and k_new.dim() == 4 and tuple(k_new.shape[::2]) == (L, H) and \
+            k_new.shape[3] == D, "k_new / v_new must be [L, sum(n_new), Hkv, D]"
+        assert k_new.dtype == v_new.dtype and k_new.stride(3) == 1 and v_new.stride(3) == 1
+        N.require_cuda(k_new, v_new, self.kv)
+        if isinstance(n_new, torch.Tensor):
+            off, R = n_new, n_new.numel() - 1
+        else:
+            offs = [0]
+            for x in n_new:
+                offs.append(offs[-1] + int(x))
+            R = len(offs) - 1
+            if R <= self.max_sessions:
+                off = self._upload(offs)
+        if R > self.max_sessions:
+            raise ValueError(f"{R} sessions, room for {self.max_sessions}")
+        dev, ws, rows = self.device, self._blocks_workspace(), self.rows
+        N.check(N.load().actkv_quant_append(
+            k_new.data_ptr(), v_new.data_ptr(), N.dtype_code(k_new), *k_new.stride()[:3], *v_new.stride()[:3],
+            off.data_ptr(), k_new.shape[1], rows.data_ptr(), *rows.stride()[:4], self.block_table.data_ptr(),
+            self.block_table.stride(0), self.seq_used.data_ptr(), self.free_list.data_ptr(), self.free_top.data_ptr(),
+            self.num_blocks, R, L, self.max_blocks, self.num_blocks, self.block_size, H, D, ws.data_ptr(), ws.numel(),
+            N.status_word(dev).data_ptr(), N.stream_ptr(dev)), "append")
+        self.n_sessions = max(self.n_sessions, R)
+        if check:
+            bits = N.read_device_status(dev)
+            if bits & N.DEV_OUT_OF_BLOCKS:
+                raise OutOfBlocks("append: the free stack (or a table row) ran out of blocks")
+            if bits:
+                raise RuntimeError(f"append: device status {bits:#x}")
+
+    def chunk_attention(self, layer: int, q: torch.Tensor, q_off: torch.Tensor, scale: float | None = None,
+                        out: torch.Tensor | None = None, lse: torch.Tensor | None = None):
+        """As ``DevicePagedCache.chunk_attention``, over the 8-bit rows."""
+        R = q_off.shape[0] - 1
+        if self._chunk_ws is None:
+            self._chunk_ws = chunk_workspace(self.device)
+        return paged_chunk_attention_quant(q, q_off, self.rows[layer], self.n_kv_heads, self.block_table[:R],
+                                           self.seq_used[:R], scale=scale, out=out, lse=lse, workspace=self._chunk_ws)
+
+    # The keys read back for scoring: every block of the pool in its place, so that the tables serve
+    # unchanged (one "session" with the identity table), in layer groups of about a gigabyte.
+    def layer_groups(self, l0: int, l1: int):
+        per = self.num_blocks * self.block_size * self.n_kv_heads * self.head_dim * 2
+        step = max(1, min(self.n_layers, (1 << 30) // per))
+        return [(l, min(l + step, l1)) for l in range(l0, l1, step)]
+
+    def keys16(self, l0: int, l1: int) -> torch.Tensor:
+        n, slots = l1 - l0, self.num_blocks * self.block_size
+        if self._keys is None:
+            most = max(b - a for a, b in self.layer_groups(0, self.n_layers))
+            self._keys = torch.empty(most, slots, self.n_kv_heads, self.head_dim, dtype=self.dtype, device=self.device)
+            self._all_blocks = torch.arange(self.num_blocks, dtype=torch.int32, device=self.device).view(1, -1)
+            self._all_slots = torch.tensor([0, slots], dtype=torch.int32, device=self.device)
+        assert n <= self._keys.shape[0]
+        keys = self._keys[:n]
+        dequantize_read(self.rows[l0:l1], self.n_kv_heads, self.head_dim, self._all_slots, self._all_blocks,
+                        self._all_slots[1:], slots, k_out=keys, planes="k")
+        keys = keys.view(n, 1, self.num_blocks, self.block_size, self.n_kv_heads, self.head_dim)
+        return keys.expand(-1, 2, -1, -1, -1, -1)          # scoring reads the key plane only
+
+    def flat_planes(self):
+        return self.kv.stride(1), self.row_bytes, self.row_bytes, self.num_blocks * self.block_size
 
 
 def _no_mark(name) -> None:
@@ -255,7 +364,8 @@ class EvictionPipeline:
         self.host_inputs_read = None              # event: step_host's last copy out of host memory done
         self._ready = None                        # step_host's streamed mode: copied-groups counter
         self._ready_base = 0
-        self._streamed = None                     # None: not tried yet; False: the grouped launches
+        # None: not tried yet; False: the grouped launches (an 8-bit cache is scored in layer groups)
+        self._streamed = False if isinstance(cache, QuantPagedCache) else None
         self._lse_own = None                      # lse computed here when a step gets none
         self._lse_ws = None
         self._score_ws = None                     # the CTA-pair scoring kernel's lse operand rows
@@ -389,8 +499,11 @@ class EvictionPipeline:
             self._lse_own = torch.empty(shape, dtype=torch.float32, device=c.device)
             need = region_lse_workspace_bytes(L, q.shape[1], q.shape[2], c.max_tokens)
             self._lse_ws = N.workspace(need, c.device)
-        return action_region_lse(q, self.act_off[:R + 1], c.kv, c.block_table[:R], c.seq_used[:R],
-                                 scale=self.scale, max_seq=c.max_tokens, out=self._lse_own, workspace=self._lse_ws)
+        for l0, l1 in c.layer_groups(0, L):
+            action_region_lse(q[l0:l1], self.act_off[:R + 1], c.keys16(l0, l1), c.block_table[:R], c.seq_used[:R],
+                              scale=self.scale, max_seq=c.max_tokens, out=self._lse_own[l0:l1],
+                              workspace=self._lse_ws)
+        return self._lse_own
 
     def step_host(self, q_host: torch.Tensor, lse_host: torch.Tensor, layer_groups: int = 4) -> None:
         """``step`` with the action queries and their lse in pinned host memory.
@@ -510,9 +623,10 @@ class EvictionPipeline:
         need = score_region_workspace_bytes(c.n_layers, q.shape[1], q.shape[2])
         if self._score_ws is None or self._score_ws.numel() < need:
             self._score_ws = N.workspace(need, c.device)
-        action_scores_region(q[l0:l1], lse[l0:l1], self.act_off[:R + 1], c.kv[l0:l1], c.block_table[:R],
-                             c.seq_used[:R], self.heads[:R, l0:l1], scale=self.scale, path=self.path,
-                             max_actions=self.max_actions, workspace=self._score_ws, streamed=streamed)
+        for a, b in c.layer_groups(l0, l1):
+            action_scores_region(q[a:b], lse[a:b], self.act_off[:R + 1], c.keys16(a, b), c.block_table[:R],
+                                 c.seq_used[:R], self.heads[:R, a:b], scale=self.scale, path=self.path,
+                                 max_actions=self.max_actions, workspace=self._score_ws, streamed=streamed)
 
     def _finish_step(self, mark=None) -> None:
         """Steps 2-5 of ``step`` (everything after the scores)."""

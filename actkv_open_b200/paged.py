@@ -18,6 +18,7 @@ import torch
 from . import _native as N
 from ._native import OutOfBlocks
 from .kernels.compaction import _keep_u8, apply_copies
+from .kernels.chunk_attn import paged_chunk_attention
 from .kernels.lse_attn import action_scores, paged_decode_attention
 
 __all__ = ["OutOfBlocks", "PagedKVCache", "keep_mask_from_scores"]
@@ -151,6 +152,15 @@ class PagedKVCache:
         ``paged_decode_attention``), the role the reference's torch stand-in plays for the paged
         FA backend."""
         return paged_decode_attention(q, self.kv[layer], self.block_table(reqs), self.seq_tensor(reqs), scale)
+
+    def chunk_attention(self, reqs, q, n_new, layer=0, scale=None):
+        """Attention of each request's newest n_new[i] tokens (already appended) over its cache ->
+        (out [sum(n_new), Hq, D] of the cache's dtype, lse [sum(n_new), Hq]); q packed likewise."""
+        off = [0]
+        for n in n_new:
+            off.append(off[-1] + int(n))
+        return paged_chunk_attention(q, self._to_device(torch.tensor(off, dtype=torch.int32)), self.kv[layer],
+                                     self.block_table(reqs), self.seq_tensor(reqs), scale)
 
     def cal_attn(self, reqs, q, lse, out, n_seen, layer=0, scale=None):
         """Primitive 1: AttnScore <- CalAttn(target_q, KCache) via LSE recovery (Algorithm 3)."""
