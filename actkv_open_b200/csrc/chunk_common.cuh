@@ -14,6 +14,7 @@ using namespace umma;
 constexpr int kRows = 128;                  // query rows per row tile (MMA M)
 constexpr int kTile = 128;                  // tokens per key tile, the grain of the schedule
 constexpr int kFewRows = 16;                // query rows of a session and KV head that chunk_few_kernel takes
+constexpr int few_limit(bool quant) { return quant ? 8 : kFewRows; }      // ... of which over the 8-bit cache
 constexpr int kFewParts = 8 * kFewRows;     // rows of its units: up to 8 heads
 constexpr int kUnitCost = 2;                // a unit's fixed cost (queries in, results out) in key tiles
 constexpr float kSlack = 8.0f;              // log2 units the maximum may outgrow m by
@@ -29,8 +30,8 @@ struct Share {
 // all.  The two kernels run one after the other, so short work is not split between them: where the other kernel
 // has sessions too, those of few rows go to their own only when they hold bytes enough to win back a
 // kernel's start and end (about 15 us) by its higher rate: 512 MB of 16-bit rows (6.3 against 5.3 TB/s), 64 MB
-// of 8-bit ones (3.3 against 1.6 TB/s).  (16 sessions of 1000 to 9000 tokens with 3 to 7 new ones each, 4 query
-// heads per KV head, 330 MB: 120 us split, 77 us together.)
+// of 8-bit ones (4.1 against 1.6 TB/s).  (16 sessions of 1000 to 9000 tokens with 3 to 7 new ones each, 4 query
+// heads per KV head, 330 MB: 120 us split, 80 us together.)
 // Every thread of the block calls it; `sums` is shared.
 template <int kThreads>
 __device__ __forceinline__ int few_rows_now(const ChunkArgs& a, int64_t (&sums)[2]) {

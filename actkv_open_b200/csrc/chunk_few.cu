@@ -1,25 +1,38 @@
 // Chunk attention of sessions with few new tokens (a single token, a drafted run: at most 16 query rows,
-// token x head of the GQA group, per KV head) over the paged cache: the formulas of chunk_umma.cu.
+// token x head of the GQA group, per KV head; 8 over the 8-bit cache) over the paged cache: the formulas of
+// chunk_umma.cu.
 //
 // Such a call reads each key and value once for a handful of products, so memory bounds it: 4 (2 over
-// the 8-bit cache) bytes per value pair against 2 * rows operations.  What matters is bytes in flight
-// and no hand-overs between them and the sums.  So there are none: a warp copies 16 tokens of keys
-// and values (cp.async, a private ring of several steps), reads them as operands of the warp-wide
-// m16n8k16 product straight from there, keeps its own running maximum, sum and output in registers,
-// and the warps meet once per unit.  The 128-row tensor-core tile of chunk_umma.cu would be at most
-// an eighth full here, and over the 8-bit cache would need the widened values in shared memory;
-// here they are widened in registers on their way into the product.
+// the 8-bit cache) bytes per key-value pair of values against 4 operations per query row.  What matters is
+// bytes in flight and no hand-overs between them and the sums.  So there are none: a warp copies 16 tokens
+// of keys and values (cp.async, a private ring of three steps), reads them as operands of the warp-wide
+// m16n8k16 product straight from there, keeps its own running maximum, sum and output in registers, and the
+// results leave from registers.  The 128-row tensor-core tile of chunk_umma.cu would be at most an eighth
+// full here, and over the 8-bit cache would need the widened values in shared memory; here they are
+// widened in registers on their way into the product.
 //
-// Operands.  S = Q K^T: the product sums over dims in any order, as long as both operands agree, so a
-// lane's four dims of a k-step are consecutive ones of a 16-byte piece of its token's row.  O = P V:
-// columns come in any order, so lane group n takes dims (D / 8) n + j in its j-th product, again
-// consecutive bytes of a row; the pairs of tokens that an operand register holds are put together
-// by byte permutes.  p goes from the layout of S to that of the second product without a move.
+// Operands.  The first product sums over dims in any order, as long as both operands agree, so a lane's four
+// dims of a k-step are consecutive ones of a 16-byte piece of its token's row.  The outputs' dims come in any
+// order, so lane group n takes dims (D / 8) n .. of the values, again consecutive bytes of a row; the
+// pairs of tokens that an operand register holds are put together by byte permutes.
+//   16-bit rows: S = Q K^T and O = P V, 16 query rows as the products' rows; p goes from the layout of S to
+//     that of the second product without a move.  8 warps of 244 registers.
+//   8-bit rows: S^T = K Q^T and O^T = V^T P^T, tokens and dims as the products' rows and 8 query rows as
+//     their columns: half the products, and O^T takes half the registers, so that 16 warps of 127 hide
+//     the widening's latencies (8 warps 344 us, 16 warps 304 us; the other way round 379 us); p^T is an
+//     8 x 8 transpose per 8 tokens.
 //
 // Work is shared out as in chunk_umma.cu, in equal shares per CTA.  A unit is a session and a group of 8 (4, 2, 1:
 // what divides them) KV heads, a warp per head: a token's row is read whole by one CTA at one time.  With a
 // head per CTA the 8-bit rows' scale bytes, 4 per head and row, were fetched from memory once per head, 64 bytes
-// each time (1.7 times the bytes of the rows).  With fewer heads the warps of one take its tokens in turn.
+// each time: 1.7 times the bytes of the rows, against 1.03 times now.  Further warps of a head take its tokens in
+// turn and join through shared memory.
+//
+// Measured: 32 single-token sessions of 4096 to 32768 tokens, 32 query heads over 8 KV heads of 128: 16-bit
+// rows (2.4 GB) 379 us, 6.4 TB/s, 0.97 of the measured copy rate, memory bound; 8-bit rows (1.25 GB) 304 us,
+// 4.1 TB/s, 0.63 of it, bound by issue (five integer operations per pair of values to widen them to bf16, of
+// about 650 instructions per step; conversion to fp16 by one instruction per pair instead, with the ranges kept by
+// powers of two, measured no faster).
 #include <type_traits>
 
 #include "chunk_common.cuh"
@@ -28,8 +41,6 @@ namespace actkv {
 namespace chunk {
 namespace few {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
 constexpr int kRoundCost = 6;               // a unit's fixed cost in rounds of its warps
 constexpr int kMinRounds = 6;               // a CTA's share is at least so many: fewer partial results to join
 constexpr int kStep = 16;                   // tokens per step
@@ -37,11 +48,12 @@ constexpr int kJoinRow = kMaxD + 8;         // a warp's O, m and l in shared mem
 
 template <int D, bool QUANT>
 struct Ring {
+  static constexpr int kWarps = QUANT ? 16 : 8, kThreads = kWarps * 32;
   static constexpr int kEs = QUANT ? 1 : 2;
   static constexpr int kChunks = D * kEs / 16;              // 16-byte pieces of a row
   static constexpr uint32_t kPlane = kStep * D * kEs;       // keys, then values
   static constexpr uint32_t kStage = 2 * kPlane + (QUANT ? 128 : 0);     // and their scale words
-  static constexpr int kStages = QUANT ? 6 : (D == 128 ? 3 : 6);
+  static constexpr int kStages = QUANT ? 3 : (D == 128 ? 3 : 6);
   static constexpr uint32_t kBytes = kWarps * kStages * kStage;
   static constexpr uint32_t kJoinBytes = kWarps * kFewRows * kJoinRow * 4;
   static constexpr uint32_t kSmemBytes = (kBytes > kJoinBytes ? kBytes : kJoinBytes) + 512;
@@ -91,6 +103,13 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Lane (r, c) has elements (r, 2 c) and (r, 2 c + 1) of an 8 x 8 matrix; of its transpose after.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
 // Two e4m3 bytes, one atop each half of x (anything below them), times f.
 template <bool BF16>
 __device__ __forceinline__ uint32_t widen2(uint32_t x, uint32_t f) {
@@ -124,16 +143,18 @@ __device__ __forceinline__ uint32_t drop_bad(uint32_t u, uint32_t hide, bool& fo
 
 struct Sched {
   Share share;
-  int64_t scan[kWarps], sums[2];
+  int64_t scan[32], sums[2];
   int bad_v;
 };
 static_assert(sizeof(Sched) <= 512, "the schedule's place in shared memory");
 
 template <int D, bool BF16, bool QUANT>
-__global__ void __launch_bounds__(kThreads, 1) chunk_few_kernel(const __grid_constant__ ChunkArgs a, bool vec_out) {
+__global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(const __grid_constant__ ChunkArgs a, bool vec_out) {
   using Rg = Ring<D, QUANT>;
+  constexpr int kWarps = Rg::kWarps, kThreads = Rg::kThreads;
   constexpr int CH = Rg::kChunks, kRowsPerCopy = 32 / CH, kCopies = kStep / kRowsPerCopy;
-  constexpr int kKSteps = D / 16, kTiles = D / 8;           // products per S, per O
+  constexpr int kKSteps = D / 16, kTiles = D / 8;           // k-steps of S, dims of O per lane (group)
+  constexpr int kOut = QUANT ? kTiles / 2 : kTiles;         // products of O
   extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r8 = lane >> 2, c4 = lane & 3;
@@ -195,14 +216,18 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few_kernel(const __grid_con
       const int begin = t0 * round, end = min(t1 * round, S);
       const int start = begin + my_part * kStep;              // this warp's steps: start, start + round, ...
       const int mine = start < end ? (end - start + round - 1) / round : 0;
-      const int lim0 = S - A + r8 / a.G, lim1 = S - A + (r8 + 8) / a.G;           // last tokens the lane's rows see
+      // the lane's two query rows, and the last tokens they see
+      const int row0 = QUANT ? 2 * c4 : r8, row1 = QUANT ? row0 + 1 : r8 + 8;
+      const int lim0 = S - A + row0 / a.G, lim1 = S - A + row1 / a.G;
       const bool wide = rows > 8;
-      // ---- queries as the first operand: for each k-step rows r8 and r8 + 8, dims as the keys come
-      uint32_t q[kKSteps][4];
+      // ---- queries, dims as the keys come: 16-bit rows as the first operand, rows r8 and r8 + 8 for each k-step;
+      // 8-bit rows as the second, row r8
+      constexpr int kQ = QUANT ? 1 : 2;
+      uint32_t q[kKSteps][2 * kQ];
       {
         const uint16_t* qp = static_cast<const uint16_t*>(a.q);
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
+        for (int hf = 0; hf < kQ; ++hf) {
           const int row = r8 + hf * 8, jq = row / a.G;
           const uint16_t* p = qp + (int64_t(a0) + jq) * a.q_stride_t + int64_t(h * a.G + row - jq * a.G) * a.q_stride_h;
 #pragma unroll
@@ -212,13 +237,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few_kernel(const __grid_con
             const int d = (c4 + 4 * (k / per)) * (per * 4) + (k % per) * 4;
             const uint2 u = row < rows ? *reinterpret_cast<const uint2*>(p + d) : make_uint2(0u, 0u);
             q[k][hf] = u.x;
-            q[k][2 + hf] = u.y;
+            q[k][kQ + hf] = u.y;
           }
         }
       }
-      float o[kTiles][4];
+      float o[kOut][4];
 #pragma unroll
-      for (int j = 0; j < kTiles; ++j)
+      for (int j = 0; j < kOut; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
       float m0 = ninf, m1 = ninf, l0 = 0.0f, l1 = 0.0f;
@@ -259,112 +284,97 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few_kernel(const __grid_con
         phys = look_up(i + 1);
       };
 
+      // the rows' references go up to the maxima given (the same in all lanes of a row)
+      auto raise = [&](float top0, float top1) {
+        const float n0 = fmaxf(m0, top0), n1 = fmaxf(m1, top1);
+        const float e0 = m0 == n0 ? 1.0f : ex2(m0 - n0), e1 = m1 == n1 ? 1.0f : ex2(m1 - n1);
+        m0 = n0;
+        m1 = n1;
+        l0 *= e0;
+        l1 *= e1;
+#pragma unroll
+        for (int j = 0; j < kOut; ++j) {
+          o[j][0] *= e0;
+          o[j][1] *= QUANT ? e1 : e0;
+          o[j][2] *= QUANT ? e0 : e1;
+          o[j][3] *= e1;
+        }
+      };
       auto step = [&](int i, int slot, auto edge_) {
         constexpr bool EDGE = decltype(edge_)::value;        // hidden tokens, or scale bytes out of the ordinary
         const int t = start + i * round;
-        const uint32_t kb = ring + slot * Rg::kStage, vb = kb + Rg::kPlane, sb = kb + 2 * Rg::kPlane;
-        const int sh = QUANT && D == 64 && (h & 1) ? 16 : 0; // the head's bytes within the word
-        float s[2][4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const int row = n * 8 + r8;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
-          [[maybe_unused]] const uint32_t word = QUANT ? lds4(sb + row * 4) >> sh : 0u;
-#pragma unroll
-          for (int p = 0; p < (CH + 3) / 4; ++p) {
-            const uint4 u = lds16(kb + row * (CH * 16) + key_piece<CH>(row, c4 + 4 * p) * 16);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-            if constexpr (QUANT) {            // 16 dims: four k-steps of one scale group
-              const uint32_t b = (word >> ((c4 + 4 * p) / 2 * 8)) & 255u, f = plain_factor<BF16>(b);
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const uint32_t x0 = __byte_perm(w[k], 0u, 0x1404), x1 = __byte_perm(w[k], 0u, 0x3424);
-                mma16816<BF16>(s[n], q[p * 4 + k], EDGE ? widen2_any<BF16>(x0, b, b) : widen2<BF16>(x0, f),
-                               EDGE ? widen2_any<BF16>(x1, b, b) : widen2<BF16>(x1, f));
-              }
-            } else {                          // 8 dims: two k-steps
-              mma16816<BF16>(s[n], q[p * 2], w[0], w[1]);
-              mma16816<BF16>(s[n], q[p * 2 + 1], w[2], w[3]);
-            }
-          }
-        }
-        // s[n][0..1]: row r8, tokens t + 8 n + 2 c4, + 1; s[n][2..3]: row r8 + 8
-        float top0 = ninf, top1 = ninf;
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            if constexpr (EDGE) {
-              const int tok = t + 8 * n + 2 * c4 + e;
-              s[n][e] = tok <= lim0 && tok < end ? s[n][e] : ninf;
-              s[n][2 + e] = tok <= lim1 && tok < end ? s[n][2 + e] : ninf;
-            }
-            top0 = fmaxf(top0, s[n][e]);
-            top1 = fmaxf(top1, s[n][2 + e]);
-          }
-        top0 *= c2;
-        top1 *= c2;
-        if (__any_sync(full, top0 > m0 + kSlack || top1 > m1 + kSlack)) {
-          top0 = fmaxf(top0, __shfl_xor_sync(full, top0, 1));
-          top0 = fmaxf(top0, __shfl_xor_sync(full, top0, 2));
-          top1 = fmaxf(top1, __shfl_xor_sync(full, top1, 1));
-          top1 = fmaxf(top1, __shfl_xor_sync(full, top1, 2));
-          const float n0 = fmaxf(m0, top0), n1 = fmaxf(m1, top1);
-          const float e0 = m0 == n0 ? 1.0f : ex2(m0 - n0), e1 = m1 == n1 ? 1.0f : ex2(m1 - n1);
-          m0 = n0;
-          m1 = n1;
-          l0 *= e0;
-          l1 *= e1;
-#pragma unroll
-          for (int j = 0; j < kTiles; ++j) {
-            o[j][0] *= e0;
-            o[j][1] *= e0;
-            o[j][2] *= e1;
-            o[j][3] *= e1;
-          }
-        }
-        const float b0 = m0 == ninf ? 0.0f : m0, b1 = m1 == ninf ? 0.0f : m1;
-        uint32_t p[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const float x = ex2(fmaf(s[n][0], c2, -b0)), y = ex2(fmaf(s[n][1], c2, -b0));
-          l0 += x + y;
-          p[2 * n] = pack2<BF16>(x, y);
-          if (wide) {
-            const float z = ex2(fmaf(s[n][2], c2, -b1)), w = ex2(fmaf(s[n][3], c2, -b1));
-            l1 += z + w;
-            p[2 * n + 1] = pack2<BF16>(z, w);
-          }
-        }
-        // ---- values: tokens 2 c4, 2 c4 + 1 and those + 8, dims kTiles r8 ..
-        const int row[4] = {2 * c4, 2 * c4 + 1, 2 * c4 + 8, 2 * c4 + 9};
-        uint32_t hide[2] = {0u, 0u};
-        if constexpr (EDGE) {
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-            hide[n] = (t + row[2 * n] > S - A ? 0xffffu : 0u) | (t + row[2 * n + 1] > S - A ? 0xffff0000u : 0u);
-        }
+        const uint32_t kb = ring + slot * Rg::kStage, vb = kb + Rg::kPlane;
+        [[maybe_unused]] const uint32_t sb = kb + 2 * Rg::kPlane;
+        [[maybe_unused]] const int sh = QUANT && D == 64 && (h & 1) ? 16 : 0; // the head's bytes within the word
         bool found = false;
         if constexpr (QUANT) {
-          uint32_t w[4][kTiles / 4], b[4];
+          // ---- S^T = K Q^T, tokens as the product's rows: s[0..1] token t + r8, s[2..3] token t + r8 + 8, query
+          // rows 2 c4 and 2 c4 + 1.  Eight query rows fill the product's columns, O^T takes half the registers
+          // that O would, and twice the warps fit.
+          float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          const uint32_t word0 = lds4(sb + r8 * 4) >> sh, word1 = lds4(sb + 32 + r8 * 4) >> sh;
+#pragma unroll
+          for (int p = 0; p < CH / 4; ++p) {
+            const uint4 u = lds16(kb + r8 * (CH * 16) + key_piece<CH>(r8, c4 + 4 * p) * 16);
+            const uint4 v = lds16(kb + (r8 + 8) * (CH * 16) + key_piece<CH>(r8 + 8, c4 + 4 * p) * 16);
+            const uint32_t w0[4] = {u.x, u.y, u.z, u.w}, w1[4] = {v.x, v.y, v.z, v.w};
+            const int g8 = (c4 + 4 * p) / 2 * 8;             // 16 dims: four k-steps of one scale group
+            const uint32_t b0 = word0 >> g8 & 255u, b1 = word1 >> g8 & 255u;
+            const uint32_t f0 = plain_factor<BF16>(b0), f1 = plain_factor<BF16>(b1);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t x[4] = {__byte_perm(w0[k], 0u, 0x1404), __byte_perm(w1[k], 0u, 0x1404),
+                                     __byte_perm(w0[k], 0u, 0x3424), __byte_perm(w1[k], 0u, 0x3424)};
+              uint32_t m[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                m[e] = EDGE ? widen2_any<BF16>(x[e], e & 1 ? b1 : b0, e & 1 ? b1 : b0) : widen2<BF16>(x[e], e & 1 ? f1 : f0);
+              mma16816<BF16>(s, m, q[p * 4 + k][0], q[p * 4 + k][1]);
+            }
+          }
+          if constexpr (EDGE) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int tok = t + r8 + (e >> 1) * 8;
+              s[e] = tok <= (e & 1 ? lim1 : lim0) && tok < end ? s[e] : ninf;
+            }
+          }
+          float top0 = fmaxf(s[0], s[2]) * c2, top1 = fmaxf(s[1], s[3]) * c2;
+          if (__any_sync(full, top0 > m0 + kSlack || top1 > m1 + kSlack)) {
+#pragma unroll
+            for (int x = 4; x < 32; x *= 2) {
+              top0 = fmaxf(top0, __shfl_xor_sync(full, top0, x));
+              top1 = fmaxf(top1, __shfl_xor_sync(full, top1, x));
+            }
+            raise(top0, top1);
+          }
+          const float o0 = m0 == ninf ? 0.0f : m0, o1 = m1 == ninf ? 0.0f : m1;
+          const float x = ex2(fmaf(s[0], c2, -o0)), y = ex2(fmaf(s[1], c2, -o1)), z = ex2(fmaf(s[2], c2, -o0)),
+                      w = ex2(fmaf(s[3], c2, -o1));
+          l0 += x + z;
+          l1 += y + w;
+          // p^T as the second operand: row r8, tokens 2 c4, 2 c4 + 1 and those + 8
+          const uint32_t p0 = transpose8x8(pack2<BF16>(x, y)), p1 = transpose8x8(pack2<BF16>(z, w));
+          // ---- O^T += V^T p^T: values of tokens 2 c4, 2 c4 + 1 and those + 8, dims kTiles r8 ..
+          const int row[4] = {2 * c4, 2 * c4 + 1, 2 * c4 + 8, 2 * c4 + 9};
+          uint32_t vw[4][kTiles / 4], b[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const uint32_t base = vb + row[e] * (CH * 16);
             if constexpr (D == 128) {
               const uint4 u = lds16(base + value_piece<CH>(row[e], r8) * 16);
-              w[e][0] = u.x;
-              w[e][1] = u.y;
-              w[e][kTiles / 4 - 2] = u.z;
-              w[e][kTiles / 4 - 1] = u.w;
+              vw[e][0] = u.x;
+              vw[e][1] = u.y;
+              vw[e][kTiles / 4 - 2] = u.z;
+              vw[e][kTiles / 4 - 1] = u.w;
             } else {
               const uint2 u = lds8(base + value_piece<CH>(row[e], r8 >> 1) * 16 + (r8 & 1) * 8);
-              w[e][0] = u.x;
-              w[e][1] = u.y;
+              vw[e][0] = u.x;
+              vw[e][1] = u.y;
             }
             b[e] = (lds4(sb + 64 + row[e] * 4) >> (sh + kTiles * r8 / 32 * 8)) & 255u;
             if constexpr (EDGE) {
-              if (b[e] == 255u && t + row[e] > S - A) {     // its values are 0; the rows that see it get NaN later
+              if (b[e] == 255u && t + row[e] > S - A) {       // its values are 0; the rows that see it get NaN later
                 b[e] = 127u;
                 found = true;
               }
@@ -375,37 +385,99 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few_kernel(const __grid_con
 #pragma unroll
           for (int k = 0; k < kTiles / 4; ++k)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {     // dim 4 k + e: its byte of two tokens atop the halves
-              const uint32_t sel = 0x0000u | (e << 4) | ((4 + e) << 12);
-              const uint32_t x0 = __byte_perm(w[0][k], w[1][k], sel), x1 = __byte_perm(w[2][k], w[3][k], sel);
-              mma16816<BF16>(o[k * 4 + e], p, EDGE ? widen2_any<BF16>(x0, b[0], b[1]) : widen2<BF16>(x0, f0),
-                             EDGE ? widen2_any<BF16>(x1, b[2], b[3]) : widen2<BF16>(x1, f1));
+            for (int e = 0; e < 4; e += 2) {  // dims 4 k + e and + 1: rows r8 and r8 + 8 of the product
+              uint32_t m[4];
+#pragma unroll
+              for (int n = 0; n < 4; ++n) {
+                const uint32_t sel = uint32_t(e + (n & 1)) << 4 | uint32_t(4 + e + (n & 1)) << 12;
+                const uint32_t v2 = __byte_perm(vw[n >> 1 << 1][k], vw[(n >> 1 << 1) + 1][k], sel);
+                m[n] = EDGE ? widen2_any<BF16>(v2, b[n >> 1 << 1], b[(n >> 1 << 1) + 1]) : widen2<BF16>(v2, n >> 1 ? f1 : f0);
+              }
+              mma16816<BF16>(o[k * 2 + e / 2], m, p0, p1);
             }
         } else {
+          float s[2][4];
 #pragma unroll
-          for (int c = 0; c < kTiles / 8; ++c) {
-            uint32_t w[4][4];
+          for (int n = 0; n < 2; ++n) {
+            const int row = n * 8 + r8;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint4 u = lds16(vb + row[e] * (CH * 16) + value_piece<CH>(row[e], r8 * (kTiles / 8) + c) * 16);
-              w[e][0] = u.x;
-              w[e][1] = u.y;
-              w[e][2] = u.z;
-              w[e][3] = u.w;
+            for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
+#pragma unroll
+            for (int p = 0; p < (CH + 3) / 4; ++p) {
+              const uint4 u = lds16(kb + row * (CH * 16) + key_piece<CH>(row, c4 + 4 * p) * 16);
+              const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+              mma16816<BF16>(s[n], q[p * 2], w[0], w[1]);           // 8 dims: two k-steps
+              mma16816<BF16>(s[n], q[p * 2 + 1], w[2], w[3]);
             }
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                uint32_t x0 = __byte_perm(w[0][k], w[1][k], e ? 0x7632 : 0x5410);
-                uint32_t x1 = __byte_perm(w[2][k], w[3][k], e ? 0x7632 : 0x5410);
-                if constexpr (EDGE) {
-                  x0 = drop_bad<BF16>(x0, hide[0], found);
-                  x1 = drop_bad<BF16>(x1, hide[1], found);
-                }
-                mma16816<BF16>(o[c * 8 + k * 2 + e], p, x0, x1);
-              }
           }
+          // s[n][0..1]: row r8, tokens t + 8 n + 2 c4, + 1; s[n][2..3]: row r8 + 8
+          float top0 = ninf, top1 = ninf;
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              if constexpr (EDGE) {
+                const int tok = t + 8 * n + 2 * c4 + e;
+                s[n][e] = tok <= lim0 && tok < end ? s[n][e] : ninf;
+                s[n][2 + e] = tok <= lim1 && tok < end ? s[n][2 + e] : ninf;
+              }
+              top0 = fmaxf(top0, s[n][e]);
+              top1 = fmaxf(top1, s[n][2 + e]);
+            }
+          top0 *= c2;
+          top1 *= c2;
+          if (__any_sync(full, top0 > m0 + kSlack || top1 > m1 + kSlack)) {
+            top0 = fmaxf(top0, __shfl_xor_sync(full, top0, 1));
+            top0 = fmaxf(top0, __shfl_xor_sync(full, top0, 2));
+            top1 = fmaxf(top1, __shfl_xor_sync(full, top1, 1));
+            top1 = fmaxf(top1, __shfl_xor_sync(full, top1, 2));
+            raise(top0, top1);
+          }
+          const float b0 = m0 == ninf ? 0.0f : m0, b1 = m1 == ninf ? 0.0f : m1;
+          uint32_t p[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const float x = ex2(fmaf(s[n][0], c2, -b0)), y = ex2(fmaf(s[n][1], c2, -b0));
+            l0 += x + y;
+            p[2 * n] = pack2<BF16>(x, y);
+            if (wide) {
+              const float z = ex2(fmaf(s[n][2], c2, -b1)), w = ex2(fmaf(s[n][3], c2, -b1));
+              l1 += z + w;
+              p[2 * n + 1] = pack2<BF16>(z, w);
+            }
+          }
+          // ---- values: tokens 2 c4, 2 c4 + 1 and those + 8, dims kTiles r8 ..
+          const int row[4] = {2 * c4, 2 * c4 + 1, 2 * c4 + 8, 2 * c4 + 9};
+          uint32_t hide[2] = {0u, 0u};
+          if constexpr (EDGE) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+              hide[n] = (t + row[2 * n] > S - A ? 0xffffu : 0u) | (t + row[2 * n + 1] > S - A ? 0xffff0000u : 0u);
+          }
+#pragma unroll
+            for (int c = 0; c < kTiles / 8; ++c) {
+              uint32_t w[4][4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint4 u = lds16(vb + row[e] * (CH * 16) + value_piece<CH>(row[e], r8 * (kTiles / 8) + c) * 16);
+                w[e][0] = u.x;
+                w[e][1] = u.y;
+                w[e][2] = u.z;
+                w[e][3] = u.w;
+              }
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  uint32_t x0 = __byte_perm(w[0][k], w[1][k], e ? 0x7632 : 0x5410);
+                  uint32_t x1 = __byte_perm(w[2][k], w[3][k], e ? 0x7632 : 0x5410);
+                  if constexpr (EDGE) {
+                    x0 = drop_bad<BF16>(x0, hide[0], found);
+                    x1 = drop_bad<BF16>(x1, hide[1], found);
+                  }
+                  mma16816<BF16>(o[c * 8 + k * 2 + e], p, x0, x1);
+                }
+            }
         }
         if (EDGE && found) sched.bad_v = 1;
       };
@@ -433,11 +505,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few_kernel(const __grid_con
         fill = fill + 1 == Rg::kStages ? 0 : fill + 1;
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
-      // ---- results: l of a row over its four lanes, then rows r8 and r8 + 8 of the warp's head
-      l0 += __shfl_xor_sync(full, l0, 1);
-      l0 += __shfl_xor_sync(full, l0, 2);
-      l1 += __shfl_xor_sync(full, l1, 1);
-      l1 += __shfl_xor_sync(full, l1, 2);
+      // ---- results: l of a row over the lanes that share it
+#pragma unroll
+      for (int x = QUANT ? 4 : 1; x < (QUANT ? 32 : 4); x *= 2) {
+        l0 += __shfl_xor_sync(full, l0, x);
+        l1 += __shfl_xor_sync(full, l1, x);
+      }
       const bool whole = t0 == 0 && t1 == nt;
       const int ps_slot = t0 > 0 ? 0 : 1;
       if (wph > 1) {                          // the warps of a head meet through shared memory, the first goes on
@@ -445,16 +518,16 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few_kernel(const __grid_con
         float* jo = reinterpret_cast<float*>(smem) + warp * (kFewRows * kJoinRow);
         if (my_part > 0) {
 #pragma unroll
-          for (int j = 0; j < kTiles; ++j)
+          for (int j = 0; j < kOut; ++j)
             *reinterpret_cast<float4*>(jo + (j * 32 + lane) * 4) = make_float4(o[j][0], o[j][1], o[j][2], o[j][3]);
-          *reinterpret_cast<float4*>(jo + (kTiles * 32 + lane) * 4) = make_float4(m0, l0, m1, l1);
+          *reinterpret_cast<float4*>(jo + (kOut * 32 + lane) * 4) = make_float4(m0, l0, m1, l1);
         }
         __syncthreads();
         if (my_part == 0)
 #pragma unroll 1
           for (int w = warp + HG; w < kWarps; w += HG) {
             const float4* po = reinterpret_cast<const float4*>(smem) + w * (kFewRows * kJoinRow / 4);
-            const float4 y = po[kTiles * 32 + lane];
+            const float4 y = po[kOut * 32 + lane];
             const float M0 = fmaxf(m0, y.x), M1 = fmaxf(m1, y.z);
             // an empty side (sum 0) counts for nothing; a NaN sum stays
             const float p0 = l0 == 0.0f ? 0.0f : (m0 == M0 ? 1.0f : ex2(m0 - M0)), q0 = y.y == 0.0f ? 0.0f : (y.x == M0 ? 1.0f : ex2(y.x - M0));
@@ -464,21 +537,22 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few_kernel(const __grid_con
             l0 = fmaf(l0, p0, y.y * q0);
             l1 = fmaf(l1, p1, y.w * q1);
 #pragma unroll
-            for (int j = 0; j < kTiles; ++j) {
+            for (int j = 0; j < kOut; ++j) {
               const float4 x = po[j * 32 + lane];
               o[j][0] = fmaf(o[j][0], p0, x.x * q0);
-              o[j][1] = fmaf(o[j][1], p0, x.y * q0);
-              o[j][2] = fmaf(o[j][2], p1, x.z * q1);
+              o[j][1] = QUANT ? fmaf(o[j][1], p1, x.y * q1) : fmaf(o[j][1], p0, x.y * q0);
+              o[j][2] = QUANT ? fmaf(o[j][2], p0, x.z * q0) : fmaf(o[j][2], p1, x.z * q1);
               o[j][3] = fmaf(o[j][3], p1, x.w * q1);
             }
           }
       }
-      // columns 2 c4 and 2 c4 + 1 of the products: dims kTiles * column + j, kTiles in a row
+      // The lane's dims come in runs of kTiles: over the 8-bit cache one run, kTiles r8 on, of both its rows; else
+      // two, of columns 2 c4 and 2 c4 + 1 of the products.
       if (my_part == 0) {
         const bool fix = *reinterpret_cast<volatile int*>(&sched.bad_v) != 0;
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
-          const int row = r8 + hf * 8;
+          const int row = hf ? row1 : row0;
           if (row >= rows) continue;
           const float L = hf ? l1 : l0, M = hf ? m1 : m0, inv = L == 0.0f ? 0.0f : 1.0f / L;
           const int jq = row / a.G, hq = h * a.G + row - jq * a.G, hr = my_head * rows + row;
@@ -486,15 +560,16 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few_kernel(const __grid_con
           uint16_t* dst = static_cast<uint16_t*>(a.out) + qt * a.out_stride_t + int64_t(hq) * a.out_stride_h;
           float* part = ps.out(cta, ps_slot) + int64_t(hr) * D;
 #pragma unroll
-          for (int cc = 0; cc < 2; ++cc) {
-            const int d0 = kTiles * (2 * c4 + cc);
+          for (int cc = 0; cc < (QUANT ? 1 : 2); ++cc) {
+            const int d0 = kTiles * (QUANT ? r8 : 2 * c4 + cc);
+            auto val = [&](int j) { return QUANT ? o[j >> 1][(j & 1) * 2 + hf] : o[QUANT ? 0 : j][2 * hf + cc]; };
             if (whole) {
 #pragma unroll
               for (int j = 0; j < kTiles; j += 8) {
                 uint32_t u[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                  u[k] = pack2<BF16>(o[j + 2 * k][2 * hf + cc] * inv, o[j + 2 * k + 1][2 * hf + cc] * inv);
+                  u[k] = pack2<BF16>(val(j + 2 * k) * inv, val(j + 2 * k + 1) * inv);
                 if (vec_out) {
                   *reinterpret_cast<uint4*>(dst + d0 + j) = make_uint4(u[0], u[1], u[2], u[3]);
                 } else {
@@ -505,8 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few_kernel(const __grid_con
             } else {
 #pragma unroll
               for (int j = 0; j < kTiles; j += 4)
-                *reinterpret_cast<float4*>(part + d0 + j) = make_float4(o[j][2 * hf + cc], o[j + 1][2 * hf + cc],
-                                                                        o[j + 2][2 * hf + cc], o[j + 3][2 * hf + cc]);
+                *reinterpret_cast<float4*>(part + d0 + j) = make_float4(val(j), val(j + 1), val(j + 2), val(j + 3));
             }
             if (fix) {                        // values that were not finite and that this row does see
 #pragma unroll 1
@@ -534,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few_kernel(const __grid_con
               }
             }
           }
-          if (c4 == 0) {
+          if ((QUANT ? r8 : c4) == 0) {
             if (whole)
               a.lse[qt * a.lse_stride_t + hq] = L == 0.0f ? ninf : (M == ninf ? L : (M + log2f(L)) * 0.69314718055994531f);
             else
@@ -575,7 +649,7 @@ cudaError_t launch_few_t(const ChunkArgs& a, int grid, cudaStream_t st) {
   const cudaError_t e = limit.set(reinterpret_cast<const void*>(k), bytes);
   if (e != cudaSuccess) return e;
   const bool vec_out = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_stride_t % 8 == 0 && a.out_stride_h % 8 == 0;
-  k<<<grid, chunk::few::kThreads, bytes, st>>>(a, vec_out);
+  k<<<grid, chunk::few::Ring<D, QUANT>::kThreads, bytes, st>>>(a, vec_out);
   return cudaGetLastError();
 }
 

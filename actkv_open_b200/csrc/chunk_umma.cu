@@ -14,7 +14,7 @@
 // cost per unit, are cut into one equal share per CTA (one CTA per SM), so ragged batches, one long
 // session and many short ones balance alike; a unit that a cut divides leaves 32-bit partial
 // results (m, l, O) in the workspace, at most two per CTA, which chunk_combine_kernel joins in a
-// fixed order.
+// fixed order.  Sessions of few query rows are chunk_few.cu's.
 //
 // Two streams of (S, p, O) run in a CTA, each with its own softmax warpgroup and 256 TMEM columns:
 //   two row tiles   both streams take every key tile (one copy of K and V serves 256 rows)
@@ -22,11 +22,27 @@
 //                   and the first warpgroup joins the two at the end
 // While one stream's softmax runs, the tensor core works on the other's products.
 //
-// Warp roles (384 threads): warp 0 TMA (a paged block per lane and tile: one 5-D box of 8-token
-// groups x both D-halves; 4 KB boxes, since the copy engine spends ~60 cycles per box whatever its
-// size), warp 1 MMA issue (p from TMEM as the A operand, V as an MN-major B operand straight from
-// the tile), warps 4-7 and 8-11 softmax (a thread per row).  Every wait is bounded
-// (umma_common.cuh).
+// Warp roles: warp 0 walks the schedule, announces units to the others (so that only it spends registers
+// on it) and issues the TMA copies (a paged block per lane and tile: one 5-D box of 8-token groups x
+// both D-halves, 4 KB for blocks of 16: the copy engine spends ~60 cycles per box whatever its size, and 2 KB
+// boxes, one per D-half, gave 7.1 TB/s from L2 against 10.6); warp 1 issues the MMAs (p from TMEM as
+// the A operand, V as an MN-major B operand straight from the tile); warps 4-7 and 8-11 are the
+// softmax warpgroups (a thread per row, p handed over in halves of 64 tokens).  Over the 8-bit cache the
+// TMA brings the e4m3 tiles, warp 2 their scale bytes, and warps 12-19 widen them into the ring.  Every
+// wait is bounded.
+//
+// What bounds it.  128 x 128 logits take the tensor core 1024 cycles (two products of head size 128) and the
+// special-function unit as many (16 exponentials per cycle), so both would have to be full all the time.
+// Measured for a 2048-token chunk over 32K tokens (32 heads over 8, 1.07 TFLOP): 1.05 to 1.13 ms, 950 to 1020
+// TFLOP/s, with the board at its power limit and the SM clock at 1450 to 1600 MHz (cuBLAS at that limit:
+// 1385): about 0.57 of the tensor rate at that clock, the rest going into the chain from S through
+// softmax (~1900 cycles: 350 to read S, 350 for the maximum, 1100 for the exponentials, which two warps per
+// scheduler share) to the products.  Tried and not kept: 1 in 2, 4 or 8 exponentials on the FMA pipe
+// (polynomial of degree 4: 941, 1050, 1097 TFLOP/s against 1098), two threads per row (640 threads of 104
+// registers, spills: 858 against 960), S in halves of 64 tokens with twice the buffers (M128 N64 products
+// run at 0.6 of their rate from shared memory: 864).  What helped: descriptors in uniform registers (issue by an
+// elected lane of a converged warp, 880 to 963), p in halves, packed 32-bit math, and code that fits the
+// instruction cache (the 8-bit variant 650 to 480 us for 4 chunks of 512 over 4K to 16K tokens).
 #include <cuda.h>
 
 #include "chunk_common.cuh"
@@ -1309,7 +1325,7 @@ cudaError_t launch_chunk_umma(const ChunkArgs& args, int dtype, cudaStream_t st,
   *why = "chunk attention";
   const int grid = device_sm_count();
   // sessions of few query rows go to a kernel of their own, where a GQA group fits it
-  a.few_rows = a.G <= chunk::kFewRows ? chunk::kFewRows : 0;
+  a.few_rows = a.G <= chunk::few_limit(a.quant) ? chunk::few_limit(a.quant) : 0;
   if (a.few_rows > 0) {
     const cudaError_t e = launch_chunk_few(a, dtype, grid, st);
     if (e != cudaSuccess) return e;

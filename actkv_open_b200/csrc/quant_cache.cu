@@ -5,6 +5,10 @@
 // item (two 16-byte loads, one 16-byte store when writing; the reverse when reading), kItems items
 // in flight, so a group of 32 is two neighbouring lanes and its maximum one shuffle.  The token's
 // session and slot are found once per warp.
+//
+// Measured: writing 8 x 1088 tokens of 8 layers (8 heads of 128, bf16; 432 MB) 91 us, 4.7 TB/s, 0.73 of the
+// measured copy rate, bound by issue (two conversions, a maximum and a multiplication per value); reading 46 K
+// tokens of 4 layers (1.14 GB) 204 us, 5.6 TB/s, 0.86 of it.  kItems 2 and 8 were slower (100 and 96 us written).
 #include "kernels.cuh"
 #include "quant_row.cuh"
 
