@@ -39,11 +39,11 @@ def _check(q, q_off, cache, block_table, seq_used, out, lse, workspace):
     r_n = seq_used.shape[0]
     assert q_off.shape[0] == r_n + 1 and block_table.shape[0] == r_n, "q_off [R + 1], block_table [R, MB], seq_used [R]"
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out = q.new_empty(q.shape)
     else:
         assert out.device == dev and out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1
     if lse is None:
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev)
+        lse = q.new_empty(q.shape[:2], dtype=torch.float32)
     else:
         assert lse.device == dev and lse.shape == q.shape[:2] and lse.dtype == torch.float32 and lse.stride(1) == 1
     if workspace is None:

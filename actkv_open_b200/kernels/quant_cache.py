@@ -49,7 +49,10 @@ def quantize_write(k_new, v_new, tok_off, rows, block_table, seq_used):
     owning tok_off[r]:tok_off[r+1] (int32 [R+1], T = tok_off[R]); they become the newest
     tok_off[r+1] - tok_off[r] of its seq_used[r] tokens, whose blocks block_table [R, MB] holds.
     """
-    dev = N.require_cuda(k_new, v_new, tok_off, rows, block_table, seq_used)
+    dev = k_new.device
+    if dev.type != "cuda" or not (v_new.device == tok_off.device == rows.device == block_table.device ==
+                                  seq_used.device == dev):
+        N.require_cuda(k_new, v_new, tok_off, rows, block_table, seq_used)
     assert k_new.dim() == 4 and k_new.shape == v_new.shape and k_new.dtype == v_new.dtype, \
         "k_new / v_new are [L, T, Hkv, D] of one dtype"
     ks, vs = k_new.stride(), v_new.stride()
@@ -71,16 +74,19 @@ def dequantize_read(rows, n_kv_heads, head_dim, tok_off, block_table, seq_used, 
     """
     if planes not in ("kv", "k", "v"):
         raise ValueError(planes)
-    dev = N.require_cuda(rows, tok_off, block_table, seq_used, k_out, v_out)
+    dev = rows.device
+    if dev.type != "cuda" or not (tok_off.device == block_table.device == seq_used.device == dev) or \
+            k_out is not None or v_out is not None:
+        N.require_cuda(rows, tok_off, block_table, seq_used, k_out, v_out)
     shape = (rows.shape[0], n_tokens, n_kv_heads, head_dim)
     if "k" not in planes:
         k_out = None
     elif k_out is None:
-        k_out = torch.empty(shape, dtype=dtype, device=dev)
+        k_out = rows.new_empty(shape, dtype=dtype)
     if "v" not in planes:
         v_out = None
     elif v_out is None:
-        v_out = torch.empty(shape, dtype=dtype, device=dev)
+        v_out = rows.new_empty(shape, dtype=dtype)
     some = k_out if k_out is not None else v_out
     strides = []
     for x in (k_out, v_out):
