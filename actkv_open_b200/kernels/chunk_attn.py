@@ -27,30 +27,33 @@ def chunk_workspace(device) -> torch.Tensor:
     return N.workspace(_ws_bytes[idx], torch.device("cuda", idx))
 
 
+_I32, _F32 = torch.int32, torch.float32
+
+
 def _check(q, q_off, cache, block_table, seq_used, out, lse, workspace):
-    """Checks shared by the two caches; returns (device, out, lse, workspace)."""
+    """Checks shared by the two caches; returns (device, sessions, out, lse, workspace)."""
     dev = q.device
-    if dev.type != "cuda" or not (q_off.device == cache.device == block_table.device == seq_used.device == dev):
+    if not q.is_cuda or q_off.device != dev or cache.device != dev or block_table.device != dev or \
+            seq_used.device != dev:
         N.require_cuda(q, q_off, cache, block_table, seq_used)
-    assert q.dim() == 3, "q is [T, Hq, D]"
-    i32 = torch.int32
-    assert q_off.dtype is i32 and seq_used.dtype is i32 and block_table.dtype is i32
-    assert q.stride(2) == 1 and block_table.stride(1) == 1 and q_off.is_contiguous() and seq_used.is_contiguous()
-    r_n = seq_used.shape[0]
-    assert q_off.shape[0] == r_n + 1 and block_table.shape[0] == r_n, "q_off [R + 1], block_table [R, MB], seq_used [R]"
+    assert q.dim() == 3 and q.stride(2) == 1, "q is [T, Hq, D] with contiguous rows"
+    assert q_off.dtype is _I32 and seq_used.dtype is _I32 and block_table.dtype is _I32
+    assert block_table.stride(1) == 1 and q_off.is_contiguous() and seq_used.is_contiguous()
+    r_n = len(seq_used)
+    assert len(q_off) == r_n + 1 and len(block_table) == r_n, "q_off [R + 1], block_table [R, MB], seq_used [R]"
     if out is None:
         out = q.new_empty(q.shape)
     else:
-        assert out.device == dev and out.shape == q.shape and out.dtype == q.dtype and out.stride(2) == 1
+        assert out.device == dev and out.shape == q.shape and out.dtype is q.dtype and out.stride(2) == 1
     if lse is None:
-        lse = q.new_empty(q.shape[:2], dtype=torch.float32)
+        lse = q.new_empty(q.shape[:2], dtype=_F32)
     else:
-        assert lse.device == dev and lse.shape == q.shape[:2] and lse.dtype == torch.float32 and lse.stride(1) == 1
+        assert lse.device == dev and lse.shape == q.shape[:2] and lse.dtype is _F32 and lse.stride(1) == 1
     if workspace is None:
         workspace = chunk_workspace(dev)
     else:
         assert workspace.device == dev and workspace.is_contiguous()
-    return dev, out, lse, workspace
+    return dev, r_n, out, lse, workspace
 
 
 def paged_chunk_attention(q, q_off, kv, block_table, seq_used, scale=None, out=None, lse=None, workspace=None,
@@ -67,18 +70,21 @@ def paged_chunk_attention(q, q_off, kv, block_table, seq_used, scale=None, out=N
     ``chunk_workspace`` (a loop keeps one).  ``path``: "auto", or "tcgen05" / "simt" to force the
     tensor cores (NotImplementedError where they do not apply) or the CUDA cores.
     """
-    dev, out, lse, workspace = _check(q, q_off, kv, block_table, seq_used, out, lse, workspace)
+    dev, r_n, out, lse, workspace = _check(q, q_off, kv, block_table, seq_used, out, lse, workspace)
     t_n, hq, d = q.shape
-    assert kv.dim() == 5 and kv.shape[0] == 2 and kv.shape[4] == d, "kv is [2, NB, BS, Hkv, D]"
-    assert kv.dtype == q.dtype, "q and the cache must share a dtype"
-    _, nb, bs, hkv, _ = kv.shape
+    _2, nb, bs, hkv, kd = kv.shape
+    assert _2 == 2 and kd == d, "kv is [2, NB, BS, Hkv, D]"
+    assert kv.dtype is q.dtype, "q and the cache must share a dtype"
     assert hq % hkv == 0
     s_kv, s_b, s_s, s_h, s_d = kv.stride()
     assert s_d == 1
-    N.check(N.load().actkv_chunk_attention(
-        q.data_ptr(), N.dtype_code(q), q.stride(0), q.stride(1), q_off.data_ptr(), t_n, kv.data_ptr(), s_kv, s_b, s_s,
-        s_h, block_table.data_ptr(), block_table.stride(0), seq_used.data_ptr(), out.data_ptr(), out.stride(0),
-        out.stride(1), lse.data_ptr(), lse.stride(0), seq_used.shape[0], block_table.shape[1], nb, bs, hq, hkv, d,
-        d ** -0.5 if scale is None else float(scale), _PATHS[path], workspace.data_ptr(), workspace.numel(),
-        N.status_word(dev).data_ptr(), N.stream_ptr(dev)), "paged_chunk_attention")
+    q_t, q_h, _1 = q.stride()
+    o_t, o_h, _1 = out.stride()
+    code = N.load().actkv_chunk_attention(
+        q.data_ptr(), N.dtype_code(q), q_t, q_h, q_off.data_ptr(), t_n, kv.data_ptr(), s_kv, s_b, s_s, s_h,
+        block_table.data_ptr(), block_table.stride(0), seq_used.data_ptr(), out.data_ptr(), o_t, o_h, lse.data_ptr(),
+        lse.stride(0), r_n, block_table.size(1), nb, bs, hq, hkv, d, d ** -0.5 if scale is None else float(scale),
+        _PATHS[path], workspace.data_ptr(), workspace.nbytes, N.status_word(dev).data_ptr(), N.stream_ptr(dev))
+    if code:
+        N.check(code, "paged_chunk_attention")
     return out, lse

@@ -25,21 +25,24 @@ def quant_row_bytes(n_kv_heads: int, head_dim: int) -> int:
     return -(-n_kv_heads * (head_dim + head_dim // QUANT_GROUP) // 64) * 64
 
 
-def _move_args(x, rows, tok_off, block_table, seq_used):
-    assert rows.dim() == 5 and rows.shape[1] == 2 and rows.dtype == torch.uint8, "rows is [L, 2, NB, BS, row_bytes] uint8"
-    assert rows.stride(4) == 1 and block_table.stride(1) == 1
-    assert tok_off.dtype == torch.int32 and seq_used.dtype == torch.int32 and block_table.dtype == torch.int32
+_I32, _U8 = torch.int32, torch.uint8
+
+
+def _tables(dev, L, t_n, hkv, d, rows, tok_off, block_table, seq_used):
+    """The checks and the arguments that writing and reading share."""
+    assert rows.dim() == 5 and rows.dtype is _U8, "rows is [L, 2, NB, BS, row_bytes] uint8"
+    rl, _2, nb, bs, row = rows.shape
+    assert _2 == 2 and rl == L, "rows and the tokens must have the same layers"
+    assert row >= hkv * (d + d // QUANT_GROUP), "rows are too short for these heads"
+    s_l, s_kv, s_b, s_s, s_1 = rows.stride()
+    assert s_1 == 1 and block_table.stride(1) == 1
+    assert tok_off.dtype is _I32 and seq_used.dtype is _I32 and block_table.dtype is _I32
     assert tok_off.is_contiguous() and seq_used.is_contiguous()
-    r_n = seq_used.shape[0]
-    assert tok_off.shape[0] == r_n + 1 and block_table.shape[0] == r_n, \
-        "tok_off [R + 1], block_table [R, MB], seq_used [R]"
-    L, t_n, hkv, d = x.shape
-    assert rows.shape[0] == L, "rows and the tokens must have the same layers"
-    assert rows.shape[4] >= hkv * (d + d // QUANT_GROUP), "rows are too short for these heads"
-    s_l, s_kv, s_b, s_s, _ = rows.stride()
-    return ((tok_off.data_ptr(), t_n, rows.data_ptr(), s_l, s_kv, s_b, s_s, block_table.data_ptr(),
-             block_table.stride(0), seq_used.data_ptr(), r_n, L, block_table.shape[1], rows.shape[2], rows.shape[3],
-             hkv, d))
+    r_n = len(seq_used)
+    assert len(tok_off) == r_n + 1 and len(block_table) == r_n, "tok_off [R + 1], block_table [R, MB], seq_used [R]"
+    return (tok_off.data_ptr(), t_n, rows.data_ptr(), s_l, s_kv, s_b, s_s, block_table.data_ptr(),
+            block_table.stride(0), seq_used.data_ptr(), r_n, L, block_table.size(1), nb, bs, hkv, d,
+            N.status_word(dev).data_ptr(), N.stream_ptr(dev))
 
 
 def quantize_write(k_new, v_new, tok_off, rows, block_table, seq_used):
@@ -50,17 +53,20 @@ def quantize_write(k_new, v_new, tok_off, rows, block_table, seq_used):
     tok_off[r+1] - tok_off[r] of its seq_used[r] tokens, whose blocks block_table [R, MB] holds.
     """
     dev = k_new.device
-    if dev.type != "cuda" or not (v_new.device == tok_off.device == rows.device == block_table.device ==
-                                  seq_used.device == dev):
+    if not k_new.is_cuda or v_new.device != dev or tok_off.device != dev or rows.device != dev or \
+            block_table.device != dev or seq_used.device != dev:
         N.require_cuda(k_new, v_new, tok_off, rows, block_table, seq_used)
-    assert k_new.dim() == 4 and k_new.shape == v_new.shape and k_new.dtype == v_new.dtype, \
+    shape = k_new.shape
+    assert len(shape) == 4 and shape == v_new.shape and k_new.dtype is v_new.dtype, \
         "k_new / v_new are [L, T, Hkv, D] of one dtype"
-    ks, vs = k_new.stride(), v_new.stride()
-    assert ks[3] == 1 and vs[3] == 1
-    N.check(N.load().actkv_quantize_write(
-        k_new.data_ptr(), v_new.data_ptr(), N.dtype_code(k_new), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-        *_move_args(k_new, rows, tok_off, block_table, seq_used), N.status_word(dev).data_ptr(), N.stream_ptr(dev)),
-        "quantize_write")
+    k_l, k_t, k_h, k_1 = k_new.stride()
+    v_l, v_t, v_h, v_1 = v_new.stride()
+    assert k_1 == 1 and v_1 == 1
+    code = N.load().actkv_quantize_write(
+        k_new.data_ptr(), v_new.data_ptr(), N.dtype_code(k_new), k_l, k_t, k_h, v_l, v_t, v_h,
+        *_tables(dev, *shape, rows, tok_off, block_table, seq_used))
+    if code:
+        N.check(code, "quantize_write")
     return rows
 
 
@@ -75,7 +81,7 @@ def dequantize_read(rows, n_kv_heads, head_dim, tok_off, block_table, seq_used, 
     if planes not in ("kv", "k", "v"):
         raise ValueError(planes)
     dev = rows.device
-    if dev.type != "cuda" or not (tok_off.device == block_table.device == seq_used.device == dev) or \
+    if not rows.is_cuda or tok_off.device != dev or block_table.device != dev or seq_used.device != dev or \
             k_out is not None or v_out is not None:
         N.require_cuda(rows, tok_off, block_table, seq_used, k_out, v_out)
     shape = (rows.shape[0], n_tokens, n_kv_heads, head_dim)
@@ -90,13 +96,17 @@ def dequantize_read(rows, n_kv_heads, head_dim, tok_off, block_table, seq_used, 
     some = k_out if k_out is not None else v_out
     strides = []
     for x in (k_out, v_out):
-        if x is not None:
-            assert tuple(x.shape) == shape and x.dtype == some.dtype and x.stride(3) == 1
-        strides += [0, 0, 0] if x is None else x.stride()[:3]
-    N.check(N.load().actkv_dequantize_read(
+        if x is None:
+            strides += (0, 0, 0)
+            continue
+        *three, one = x.stride()
+        assert x.shape == shape and x.dtype is some.dtype and one == 1
+        strides += three
+    code = N.load().actkv_dequantize_read(
         N.ptr(k_out), N.ptr(v_out), N.dtype_code(some), *strides,
-        *_move_args(some, rows, tok_off, block_table, seq_used), N.status_word(dev).data_ptr(), N.stream_ptr(dev)),
-        "dequantize_read")
+        *_tables(dev, *shape, rows, tok_off, block_table, seq_used))
+    if code:
+        N.check(code, "dequantize_read")
     return k_out, v_out
 
 
@@ -104,18 +114,22 @@ def paged_chunk_attention_quant(q, q_off, rows, n_kv_heads, block_table, seq_use
                                 workspace=None, path: str = "auto"):
     """``paged_chunk_attention`` over one layer of the 8-bit cache, rows [2, NB, BS, row_bytes]: the
     keys and values are what ``dequantize_read`` gives in q's dtype."""
-    dev, out, lse, workspace = _check(q, q_off, rows, block_table, seq_used, out, lse, workspace)
+    dev, r_n, out, lse, workspace = _check(q, q_off, rows, block_table, seq_used, out, lse, workspace)
     t_n, hq, d = q.shape
-    assert rows.dim() == 4 and rows.shape[0] == 2 and rows.dtype == torch.uint8, "rows is [2, NB, BS, row_bytes] uint8"
+    _2, nb, bs, row = rows.shape
+    assert _2 == 2 and rows.dtype is _U8, "rows is [2, NB, BS, row_bytes] uint8"
     assert hq % n_kv_heads == 0
-    assert rows.shape[3] >= n_kv_heads * (d + d // QUANT_GROUP), "rows are too short for these heads"
+    assert row >= n_kv_heads * (d + d // QUANT_GROUP), "rows are too short for these heads"
     s_kv, s_b, s_s, s_1 = rows.stride()
     assert s_1 == 1
-    N.check(N.load().actkv_chunk_attention_quant(
-        q.data_ptr(), N.dtype_code(q), q.stride(0), q.stride(1), q_off.data_ptr(), t_n, rows.data_ptr(), s_kv, s_b, s_s,
-        block_table.data_ptr(), block_table.stride(0), seq_used.data_ptr(), out.data_ptr(), out.stride(0),
-        out.stride(1), lse.data_ptr(), lse.stride(0), seq_used.shape[0], block_table.shape[1], rows.shape[1],
-        rows.shape[2], hq, n_kv_heads, d, d ** -0.5 if scale is None else float(scale), _PATHS[path],
-        workspace.data_ptr(), workspace.numel(), N.status_word(dev).data_ptr(), N.stream_ptr(dev)),
-        "paged_chunk_attention_quant")
+    q_t, q_h, _1 = q.stride()
+    o_t, o_h, _1 = out.stride()
+    code = N.load().actkv_chunk_attention_quant(
+        q.data_ptr(), N.dtype_code(q), q_t, q_h, q_off.data_ptr(), t_n, rows.data_ptr(), s_kv, s_b, s_s,
+        block_table.data_ptr(), block_table.stride(0), seq_used.data_ptr(), out.data_ptr(), o_t, o_h, lse.data_ptr(),
+        lse.stride(0), r_n, block_table.size(1), nb, bs, hq, n_kv_heads, d,
+        d ** -0.5 if scale is None else float(scale), _PATHS[path], workspace.data_ptr(), workspace.nbytes,
+        N.status_word(dev).data_ptr(), N.stream_ptr(dev))
+    if code:
+        N.check(code, "paged_chunk_attention_quant")
     return out, lse
