@@ -325,10 +325,14 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
             for (int k = 0; k < 4; ++k) {
               const uint32_t x[4] = {__byte_perm(w0[k], 0u, 0x1404), __byte_perm(w1[k], 0u, 0x1404),
                                      __byte_perm(w0[k], 0u, 0x3424), __byte_perm(w1[k], 0u, 0x3424)};
+              const uint32_t n0 = w0[k] & 0x7f7f7f7fu, n1 = w1[k] & 0x7f7f7f7fu;
+              const uint32_t v[4] = {__byte_perm(n0, 0u, 0x4140), __byte_perm(n1, 0u, 0x4140),
+                                     __byte_perm(n0, 0u, 0x4342), __byte_perm(n1, 0u, 0x4342)};
               uint32_t m[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                m[e] = EDGE ? widen2_any<BF16>(x[e], e & 1 ? b1 : b0, e & 1 ? b1 : b0) : widen2<BF16>(x[e], e & 1 ? f1 : f0);
+                m[e] = EDGE ? widen2_any<BF16>(x[e], e & 1 ? b1 : b0, e & 1 ? b1 : b0)
+                            : mul16x2<BF16>(under_exponent<BF16>(x[e], v[e]), e & 1 ? f1 : f0);
               mma16816<BF16>(s, m, q[p * 4 + k][0], q[p * 4 + k][1]);
             }
           }

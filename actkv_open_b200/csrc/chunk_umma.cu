@@ -836,12 +836,12 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
               for (int e = 0; e < 4; ++e) mx[e] = fmax3(mx[e], x[k + e], x[k + e + 4]);
           };
           if constexpr (QUANT) {
-            tmem_ld64(s_addr + 64, v[0]);
-            tmem_wait(v[0]);
-            half_max(v[0]);
-            tmem_ld64(s_addr, v[0]);
-            tmem_wait(v[0]);
-            half_max(v[0]);
+#pragma unroll 1
+            for (int h = 1; h >= 0; --h) {
+              tmem_ld64(s_addr + h * 64, v[0]);
+              tmem_wait(v[0]);
+              half_max(v[0]);
+            }
           } else {
             tmem_ld64(s_addr, v[0]);
             tmem_ld64(s_addr + 64, v[QUANT ? 0 : 1]);
@@ -871,30 +871,48 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
           const float off = m == ninf ? 0.0f : m;
           const float2 c2v = make_float2(c2, c2), offv = make_float2(-off, -off);
           float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-          // p of 32 tokens at a time; a store is waited for after the next 32 are computed, and the
-          // second product starts on the first 64
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if (QUANT && q == 2) {
-              tmem_ld64(s_addr + 64, v[0]);
-              tmem_wait(v[0]);
-            }
-            uint32_t u[16];
+          auto quarter = [&](const float (&x)[64], int at, uint32_t (&u)[16]) {
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
-              const float* vp = &v[QUANT ? 0 : q >> 1][(q & 1) * 32 + 2 * k];
-              const float2 e = fma2(make_float2(vp[0], vp[1]), c2v, offv);
+              const float2 e = fma2(make_float2(x[at + 2 * k], x[at + 2 * k + 1]), c2v, offv);
               const float2 p = make_float2(ex2(e.x), ex2(e.y));
               sum[k & 1] = add2(sum[k & 1], p);
               u[k] = pack2<BF16>(p.x, p.y);
             }
-            if (q == 2) {
-              tmem_wait_st();
-              fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(bar(B_PF + 2 * w));
+          };
+          // p of 32 tokens at a time; the second product starts on the first 64
+          if constexpr (QUANT) {
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+              if (h) {
+                tmem_ld64(s_addr + 64, v[0]);
+                tmem_wait(v[0]);
+                tmem_wait_st();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(B_PF + 2 * w));
+              }
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                uint32_t u[16];
+                quarter(v[0], q * 32, u);
+                tmem_st16(s_addr + h * 32 + q * 16, u);
+              }
             }
-            tmem_st16(s_addr + q * 16, u);
+          } else {
+            // a store is waited for after the next 32 are computed
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint32_t u[16];
+              quarter(v[QUANT ? 0 : q >> 1], (q & 1) * 32, u);
+              if (q == 2) {
+                tmem_wait_st();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(B_PF + 2 * w));
+              }
+              tmem_st16(s_addr + q * 16, u);
+            }
           }
           const float2 s2 = add2(sum[0], sum[1]);
           l += s2.x + s2.y;
