@@ -19,7 +19,8 @@
 //     that of the second product without a move.  8 warps of 244 registers.
 //   8-bit rows: S^T = K Q^T and O^T = V^T P^T, tokens and dims as the products' rows and 8 query rows as
 //     their columns: half the products, and O^T takes half the registers, so that 16 warps of 127 hide
-//     the widening's latencies (8 warps 344 us, 16 warps 304 us; the other way round 379 us); p^T is an
+//     the widening's latencies (8 warps 344 us, 16 warps 304 us, both before the
+//     widening was made shorter; the other way round 379 us); p^T is an
 //     8 x 8 transpose per 8 tokens.
 //
 // Work is shared out as in chunk_umma.cu, in equal shares per CTA.  A unit is a session and a group of 8 (4, 2, 1:
@@ -29,10 +30,10 @@
 // turn and join through shared memory.
 //
 // Measured: 32 single-token sessions of 4096 to 32768 tokens, 32 query heads over 8 KV heads of 128: 16-bit
-// rows (2.4 GB) 379 us, 6.4 TB/s, 0.97 of the measured copy rate, memory bound; 8-bit rows (1.25 GB) 304 us,
-// 4.1 TB/s, 0.63 of it, bound by issue (five integer operations per pair of values to widen them to bf16, of
-// about 650 instructions per step; conversion to fp16 by one instruction per pair instead, with the ranges kept by
-// powers of two, measured no faster).
+// rows (2.4 GB) 379 us, 6.4 TB/s, 0.97 of the measured copy rate, memory bound; 8-bit rows (1.25 GB) 268 to 298 us
+// (the board's power limit), 4.2 to 4.6 TB/s, 0.64 to 0.71 of it, bound by issue and the logic pipe (five
+// operations per pair of values to widen them to bf16, of about 650 instructions per step; conversion to fp16 by one
+// instruction per pair instead, with the ranges kept by powers of two, measured no faster).
 #include <type_traits>
 
 #include "chunk_common.cuh"
@@ -110,10 +111,11 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
-// Two e4m3 bytes, one atop each half of x (anything below them), times f.
+// Two e4m3 bytes, at the bottom of x's halves, times f.  (Two of four operations on the logic pipe: 260 us for 32
+// single tokens of 18432; with the bytes' order and mask of widen16 269, with a shift, two masks and an or 278.)
 template <bool BF16>
 __device__ __forceinline__ uint32_t widen2(uint32_t x, uint32_t f) {
-  return mul16x2<BF16>(((x >> (BF16 ? 4 : 1)) & (BF16 ? 0x07f007f0u : 0x3f803f80u)) | (x & 0x80008000u), f);
+  return mul16x2<BF16>(under_exponent<BF16>(x * 256u, x & 0x007f007fu), f);
 }
 // ... for any scale bytes of the two halves.
 template <bool BF16>
@@ -323,16 +325,13 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
             const uint32_t f0 = plain_factor<BF16>(b0), f1 = plain_factor<BF16>(b1);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const uint32_t x[4] = {__byte_perm(w0[k], 0u, 0x1404), __byte_perm(w1[k], 0u, 0x1404),
-                                     __byte_perm(w0[k], 0u, 0x3424), __byte_perm(w1[k], 0u, 0x3424)};
-              const uint32_t n0 = w0[k] & 0x7f7f7f7fu, n1 = w1[k] & 0x7f7f7f7fu;
-              const uint32_t v[4] = {__byte_perm(n0, 0u, 0x4140), __byte_perm(n1, 0u, 0x4140),
-                                     __byte_perm(n0, 0u, 0x4342), __byte_perm(n1, 0u, 0x4342)};
+              const uint32_t x[4] = {__byte_perm(w0[k], 0u, 0x4140), __byte_perm(w1[k], 0u, 0x4140),
+                                     __byte_perm(w0[k], 0u, 0x4342), __byte_perm(w1[k], 0u, 0x4342)};
               uint32_t m[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e)
                 m[e] = EDGE ? widen2_any<BF16>(x[e], e & 1 ? b1 : b0, e & 1 ? b1 : b0)
-                            : mul16x2<BF16>(under_exponent<BF16>(x[e], v[e]), e & 1 ? f1 : f0);
+                            : widen2<BF16>(x[e], e & 1 ? f1 : f0);
               mma16816<BF16>(s, m, q[p * 4 + k][0], q[p * 4 + k][1]);
             }
           }
@@ -387,18 +386,21 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
           const uint32_t f0 = __byte_perm(plain_factor<BF16>(b[0]), plain_factor<BF16>(b[1]), 0x5410);
           const uint32_t f1 = __byte_perm(plain_factor<BF16>(b[2]), plain_factor<BF16>(b[3]), 0x5410);
 #pragma unroll
-          for (int k = 0; k < kTiles / 4; ++k)
+          for (int k = 0; k < kTiles / 4; ++k) {
+            // dims 4 k .. 4 k + 3 of two tokens each, a dim's two bytes next to one another
+            const uint32_t pair[2][2] = {{__byte_perm(vw[0][k], vw[1][k], 0x5140), __byte_perm(vw[2][k], vw[3][k], 0x5140)},
+                                         {__byte_perm(vw[0][k], vw[1][k], 0x7362), __byte_perm(vw[2][k], vw[3][k], 0x7362)}};
 #pragma unroll
-            for (int e = 0; e < 4; e += 2) {  // dims 4 k + e and + 1: rows r8 and r8 + 8 of the product
+            for (int e = 0; e < 2; ++e) {     // dims 4 k + 2 e and + 1: rows r8 and r8 + 8 of the product
               uint32_t m[4];
 #pragma unroll
               for (int n = 0; n < 4; ++n) {
-                const uint32_t sel = uint32_t(e + (n & 1)) << 4 | uint32_t(4 + e + (n & 1)) << 12;
-                const uint32_t v2 = __byte_perm(vw[n >> 1 << 1][k], vw[(n >> 1 << 1) + 1][k], sel);
-                m[n] = EDGE ? widen2_any<BF16>(v2, b[n >> 1 << 1], b[(n >> 1 << 1) + 1]) : widen2<BF16>(v2, n >> 1 ? f1 : f0);
+                const uint32_t x = __byte_perm(pair[e][n >> 1], 0u, n & 1 ? 0x4342 : 0x4140);
+                m[n] = EDGE ? widen2_any<BF16>(x, b[n >> 1 << 1], b[(n >> 1 << 1) + 1]) : widen2<BF16>(x, n >> 1 ? f1 : f0);
               }
-              mma16816<BF16>(o[k * 2 + e / 2], m, p0, p1);
+              mma16816<BF16>(o[k * 2 + e], m, p0, p1);
             }
+          }
         } else {
           float s[2][4];
 #pragma unroll
