@@ -6,9 +6,10 @@
 // in flight, so a group of 32 is two neighbouring lanes and its maximum one shuffle.  The token's
 // session and slot are found once per warp.
 //
-// Measured: writing 8 x 1088 tokens of 8 layers (8 heads of 128, bf16; 432 MB) 91 us, 4.7 TB/s, 0.73 of the
-// measured copy rate, bound by issue (two conversions, a maximum and a multiplication per value); reading 46 K
-// tokens of 4 layers (1.14 GB) 204 us, 5.6 TB/s, 0.86 of it.  kItems 2 and 8 were slower (100 and 96 us written).
+// Measured: writing 8 x 1088 tokens of 8 layers (8 heads of 128, bf16; 432 MB) 88 us, 4.9 TB/s, 0.75 of the
+// measured copy rate, bound by issue (conversions and a multiplication per value; with a maximum per value instead
+// of per pair 92 us); reading 46 K tokens of 4 layers (1.14 GB) 204 to 212 us, 5.4 to 5.6 TB/s, 0.82 to 0.86 of it.
+// kItems 2 and 8 were slower (100 and 96 us written, where 4 took 91).
 #include "kernels.cuh"
 #include "quant_row.cuh"
 
@@ -35,6 +36,12 @@ __device__ __forceinline__ void load16(const T* p, bool vec, Raw16<T>& r) {
 #pragma unroll
     for (int k = 0; k < 16; ++k) e[k] = p[k];
   }
+}
+
+__device__ __forceinline__ uint32_t max16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 
 template <typename T> __device__ __forceinline__ T from_f32(float x);
@@ -135,10 +142,18 @@ __global__ void __launch_bounds__(kThreads) quant_move_kernel(QuantMoveArgs a) {
         float x[16];
         uint32_t top = 0;
         const T* e = reinterpret_cast<const T*>(in[i].u);
+        // without the sign, floats order as their bits do, NaN above all: 16-bit types in pairs
+        if constexpr (sizeof(T) == 2) {
+          const uint32_t* w = reinterpret_cast<const uint32_t*>(in[i].u);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) top = max16x2(top, w[k] & 0x7fff7fffu);
+          const uint16_t t16 = uint16_t(max(top & 0xffffu, top >> 16));
+          top = __float_as_uint(to_f32(reinterpret_cast<const T&>(t16)));
+        }
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
           x[k] = to_f32(e[k]);
-          top = max(top, __float_as_uint(x[k]) & 0x7fffffffu);
+          if constexpr (sizeof(T) == 4) top = max(top, __float_as_uint(x[k]) & 0x7fffffffu);
         }
         if (!ext[i]) top = 0;
         top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));      // the group's other 16 values
