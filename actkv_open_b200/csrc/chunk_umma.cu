@@ -1054,13 +1054,9 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
         if (lane == 0)
           for (int s = 0; s < n_o; ++s) mbar_arrive(bar(B_OE + w0 + s));
       }
-      if (two) {
-        ++o_uses[0];
-        ++o_uses[1];
-      } else {
-        if (nt > 0) ++o_uses[0];
-        if (nt > 1) ++o_uses[1];
-      }
+      // the accumulators that the unit produced: none where its rows see no token
+      if (nt > 0) ++o_uses[0];
+      if (nt > (two ? 0 : 1)) ++o_uses[1];
       if (joined) ++x_uses;
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(B_UE + slot));
