@@ -712,6 +712,18 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
     auto wait = [&](int b, uint32_t par) -> bool {
       return __all_sync(full, bar_wait(bar(b), par, abort_addr));
     };
+    auto put_words = [&]() -> bool {             // the words in hand, when their tile's place is free
+      if (!have) return true;
+      if (!wait(B_RE + ring.slot, ring.par ^ 1u)) return false;
+      uint32_t* dst = reinterpret_cast<uint32_t*>(smem + Ly::kScaleOff) + ring.slot * kTile;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dst[lane + 32 * i] = w0[i];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(B_CF + ring.slot));
+      ring.next(Ly::kRaw);
+      have = false;
+      return true;
+    };
     while (have || more) {
       while (more && u.done()) {
         const uint32_t slot = n % kUnitSlots;
@@ -721,7 +733,9 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(B_UE + slot));
         ++n;
-        more = u.r >= 0;
+        // A unit without tiles: the one after it is announced, kUnitSlots on, only when the unit whose words are
+        // in hand is finished, so they go out first.
+        more = u.r >= 0 && (!u.done() || put_words());
       }
       if (more) {
         int t, plane;
@@ -743,15 +757,7 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
           else w1[i] = *reinterpret_cast<const uint16_t*>(p) | 0x7f7f0000u;
         }
       }
-      if (have) {
-        if (!wait(B_RE + ring.slot, ring.par ^ 1u)) break;
-        uint32_t* dst = reinterpret_cast<uint32_t*>(smem + Ly::kScaleOff) + ring.slot * kTile;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) dst[lane + 32 * i] = w0[i];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(B_CF + ring.slot));
-        ring.next(Ly::kRaw);
-      }
+      if (!put_words()) break;
 #pragma unroll
       for (int i = 0; i < 4; ++i) w0[i] = w1[i];
       have = more;

@@ -28,3 +28,10 @@ def _empty_units(d, quant):
 @pytest.mark.parametrize("d", [64, 128])
 def test_units_that_see_nothing_among_units_that_do(d):
     _empty_units(d, quant=False)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_units_that_see_nothing_among_units_that_do_over_the_8_bit_cache(d):
+    """Three and more such units in a row: the warp that brings scale bytes reads a tile ahead, and must
+    not hold the last tile's while it looks for the next unit that has any."""
+    _empty_units(d, quant=True)
