@@ -28,6 +28,16 @@ struct Share {
   int r0;                    // the session that holds the CTA's first unit of weight
 };
 
+// New tokens of session r; 0, and flagged, when its offsets leave the call's T rows (negative, or past the end), so
+// that no row outside q, out and lse is touched.
+__device__ __forceinline__ int new_tokens(const ChunkArgs& a, int r) {
+  const int a0 = a.q_off[r], a1 = a.q_off[r + 1];
+  if (a1 <= a0) return 0;
+  if (a0 >= 0 && a1 <= a.T) return a1 - a0;
+  flag(a.status, ACTKV_DEV_BAD_INDEX);
+  return 0;
+}
+
 // Query rows per KV head up to which chunk_few_kernel takes a session in this call, 0 when chunk_umma_kernel takes
 // all.  The two kernels run one after the other, so short work is not split between them: where the other kernel
 // has sessions too, those of few rows go to their own only when they hold bytes enough to win back a
@@ -42,8 +52,8 @@ __device__ __forceinline__ int few_rows_now(const ChunkArgs& a, int64_t (&sums)[
   __syncthreads();
   int64_t few = 0, all = 0;
   for (int r = threadIdx.x; r < a.R; r += kThreads) {
-    const int A = a.q_off[r + 1] - a.q_off[r];
-    if (A <= 0) continue;
+    const int A = new_tokens(a, r);
+    if (A == 0) continue;
     const int s = max(a.seq_used[r], 1);
     all += s;
     if (A * a.G <= a.few_rows) few += s;

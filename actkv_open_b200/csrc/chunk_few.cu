@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
   const int few_rows = few_rows_now<kThreads>(a, sched.sums);
   if (few_rows == 0) return;
   share_out<kThreads>(a.R, [&](int r) -> int64_t {
-    const int A = a.q_off[r + 1] - a.q_off[r];
+    const int A = new_tokens(a, r);
     return A > 0 && A * a.G <= few_rows ? int64_t(a.Hkv / HG) * (kRoundCost + (a.seq_used[r] + round - 1) / round) : 0;
   }, sched.share, sched.scan, cta, n_cta, kMinRounds);
   const int64_t total = sched.share.total;
@@ -199,8 +199,8 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
   auto block_of = [&](int tok) { return shift >= 0 ? tok >> shift : tok / a.BS; };
 
   for (; r < a.R && at < hi; ++r, hg = 0) {
-    const int a0 = a.q_off[r], A = a.q_off[r + 1] - a0, S = a.seq_used[r];
-    if (A <= 0 || A * a.G > few_rows) continue;
+    const int a0 = a.q_off[r], A = new_tokens(a, r), S = a.seq_used[r];
+    if (A == 0 || A * a.G > few_rows) continue;
     const int rows = A * a.G;
     const int nt = S > 0 ? (S + round - 1) / round : 0;
     const int64_t weight = kRoundCost + nt;

@@ -131,7 +131,7 @@ struct Walker {
   __device__ void load() {
     while (r < a->R) {
       a0 = a->q_off[r];
-      A = a->q_off[r + 1] - a0;
+      A = new_tokens(*a, r);
       S = a->seq_used[r];
       if (A > 0 && A * a->G > few_rows) return;
       ++r;
@@ -197,7 +197,7 @@ __device__ void make_schedule(const ChunkArgs& a, Sched& s, int cta, int n) {
   const int few_rows = few_rows_now<kThreads>(a, s.sums);
   if (threadIdx.x == 0) s.few_rows = few_rows;
   share_out<kThreads>(a.R, [&](int r) -> int64_t {
-    const int A = a.q_off[r + 1] - a.q_off[r];
+    const int A = new_tokens(a, r);
     return A > 0 && A * a.G > few_rows ? a.Hkv * geo.head_weight(a.seq_used[r], A) : 0;
   }, s.share, s.scan, cta, n, 1);
 }

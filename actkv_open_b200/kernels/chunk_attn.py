@@ -66,7 +66,8 @@ def paged_chunk_attention(q, q_off, kv, block_table, seq_used, scale=None, out=N
     block_table [R, MB] and seq_used [R] int32.  The queries belong to the newest
     A = q_off[r+1] - q_off[r] of the seq_used[r] tokens, already in the cache: query j sees the
     first seq_used[r] - A + j + 1 of them.  A query that sees none gets out 0, lse -inf; a session
-    may have no queries.  ``scale`` defaults to D ** -0.5; ``workspace`` to a new
+    may have no queries; one whose offsets leave the T rows is left alone (device status BAD_INDEX).
+    ``scale`` defaults to D ** -0.5; ``workspace`` to a new
     ``chunk_workspace`` (a loop keeps one).  ``path``: "auto", or "tcgen05" / "simt" to force the
     tensor cores (NotImplementedError where they do not apply) or the CUDA cores.
     """

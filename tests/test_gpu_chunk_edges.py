@@ -3,6 +3,7 @@ nothing among units that do, both tensor-core kernels in one call, sessions of a
 and head size, table entries and offsets out of range, values that are not finite.  Bounds as derived in
 test_gpu_chunk.py."""
 import pytest
+import torch
 
 from gpu_util import assert_device_clean, need_gpu
 from test_gpu_chunk import BF, Case, _equal
@@ -35,3 +36,30 @@ def test_units_that_see_nothing_among_units_that_do_over_the_8_bit_cache(d):
     """Three and more such units in a row: the warp that brings scale bytes reads a tile ahead, and must
     not hold the last tile's while it looks for the next unit that has any."""
     _empty_units(d, quant=True)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("path", ["auto", "simt"])
+@pytest.mark.parametrize("new, bad", [((2, 3, 2), (0, 2, 9, 9)), ((2, 90, 5), (0, 2, 92, 300)),
+                                      ((4, 80, 5), (-3, 4, 84, 89)), ((2, 3, 2), (0, 2, 5, 1 << 30))])
+def test_sessions_whose_offsets_leave_the_rows_are_left_alone(new, bad, path, quant):
+    """Offsets past the last row of q, and below the first: flagged; the other sessions have their results, and
+    nothing is written for the one that is out of range, inside the call's rows or past them."""
+    dev = need_gpu()
+    from actkv_open_b200 import _native as N
+    case = Case([500, 300, 40], list(new), 8, 2, 128, 16, BF, seed=22, quant=quant)
+    t = sum(new)
+    want = case.run(dev, path=path)
+    room = torch.full((t + 400, 8, 128), 3.0, dtype=BF, device=dev), torch.full((t + 400, 8), 3.0, device=dev)
+    off = torch.tensor(bad, dtype=torch.int32, device=dev)
+    case.run(dev, given=dict(q_off=off), path=path, out=room[0][200:200 + t], lse=room[1][200:200 + t])
+    torch.cuda.synchronize()
+    assert N.read_device_status(dev) == N.DEV_BAD_INDEX
+    written = torch.zeros(t + 400, dtype=torch.bool, device=dev)
+    for a, b in zip(bad, bad[1:]):
+        if 0 <= a < b <= t:
+            rows = slice(200 + a, 200 + b)
+            written[rows] = True
+            if (a, b) in list(zip(case.off.tolist(), case.off.tolist()[1:])):
+                assert all((x[rows] - y[a:b]).abs().max() <= 0.02 for x, y in zip(room, want))
+    assert (room[0][~written] == 3).all() and (room[1][~written] == 3).all()
