@@ -45,7 +45,7 @@ __global__ void __launch_bounds__(kWarps * 32) chunk_simt_kernel(ChunkArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int t = int(blockIdx.x / a.Hq), hq = int(blockIdx.x % a.Hq);
   const int r = session_of(a.q_off, a.R, t, lane);
-  if (r >= a.R) return;                      // past the last offset: not a query of any session
+  if (r >= a.R) return;                      // not a query of any session
   if (a.q_off[r] < 0 || a.q_off[r + 1] > a.T) {             // a session that leaves the call's rows: left alone
     if (threadIdx.x == 0) flag(a.status, ACTKV_DEV_BAD_INDEX);
     return;

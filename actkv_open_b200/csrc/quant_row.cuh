@@ -43,8 +43,8 @@ __device__ __forceinline__ uint32_t f32_e4m3x2(float lo, float hi) {
   return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
 
-// Session of packed token t: the number of sessions whose last token comes at or before t.  Called
-// by a whole warp with one t; 32 offsets per step.
+// Session of packed token t, R when it is none's (before the first offset or past the last): the number of
+// sessions whose last token comes at or before t.  Called by a whole warp with one t; 32 offsets per step.
 __device__ __forceinline__ int session_of(const int32_t* off, int R, int t, int lane) {
   int n = 0;
   for (int base = 0; base < R; base += 32) {
@@ -53,7 +53,7 @@ __device__ __forceinline__ int session_of(const int32_t* off, int R, int t, int 
     n += c;
     if (c < 32) break;
   }
-  return n;
+  return n < R && t >= off[n] ? n : R;
 }
 
 }  // namespace actkv

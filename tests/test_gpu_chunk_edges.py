@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from gpu_util import assert_device_clean, need_gpu
-from test_gpu_chunk import BF, Case, _equal
+from test_gpu_chunk import BF, Case, U, _equal
 
 pytestmark = pytest.mark.gpu
 
@@ -63,3 +63,21 @@ def test_sessions_whose_offsets_leave_the_rows_are_left_alone(new, bad, path, qu
             if (a, b) in list(zip(case.off.tolist(), case.off.tolist()[1:])):
                 assert all((x[rows] - y[a:b]).abs().max() <= 0.02 for x, y in zip(room, want))
     assert (room[0][~written] == 3).all() and (room[1][~written] == 3).all()
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("path", ["auto", "simt"])
+def test_rows_before_the_first_offset_are_no_sessions(path, quant):
+    """The last sessions of a batch by a slice of its offsets, q being the whole batch's: the rows of the sessions
+    that were left out are not written."""
+    dev = need_gpu()
+    case = Case([500, 300, 40], [6, 70, 3], 8, 2, 128, 16, BF, seed=23, quant=quant)
+    x = case.device(dev)
+    want = case.run(dev, given=x, path=path)
+    out, lse = torch.full_like(want[0], 3.0), torch.full_like(want[1], 3.0)
+    case.run(dev, given=dict(q_off=x["q_off"][2:], table=x["table"][2:], seq=x["seq"][2:]), path=path, out=out, lse=lse)
+    assert (out[:76] == 3).all() and (lse[:76] == 3).all()
+    # the same session may run on another kernel in the smaller batch: equal within twice the bound of one
+    assert ((out[76:].double() - want[0][76:].double()).abs() <= 2 * (2 * U[BF] + 1e-4) * case.ref()[2].to(dev)[76:]).all()
+    assert (lse[76:] - want[1][76:]).abs().max() <= 1e-3
+    assert_device_clean(dev)
