@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
         const int tok = start + i * round + (lane & 15);
         if (i >= mine || tok >= end) return -2;
         const int lb = block_of(tok);
-        return lb < a.MB ? table[lb] : -1;
+        return lb < a.MB ? max(table[lb], -1) : -1;           // -2 is this kernel's own, for the places past the end
       };
       int phys = look_up(0);
       const char* head = kv + (QUANT ? int64_t(h) * D : int64_t(h) * a.kv_stride_h * 2);

@@ -81,3 +81,19 @@ def test_rows_before_the_first_offset_are_no_sessions(path, quant):
     assert ((out[76:].double() - want[0][76:].double()).abs() <= 2 * (2 * U[BF] + 1e-4) * case.ref()[2].to(dev)[76:]).all()
     assert (lse[76:] - want[1][76:]).abs().max() <= 1e-3
     assert_device_clean(dev)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("new", [1, 3, 90])
+@pytest.mark.parametrize("bad", [-2, -3, -(1 << 31), (1 << 31) - 1])
+def test_every_block_id_outside_the_cache_is_flagged(bad, new, quant):
+    """One bad entry in the middle of a session's table, on the kernel for few rows, the wide one and the CUDA cores."""
+    dev = need_gpu()
+    from actkv_open_b200 import _native as N
+    case = Case([500], [new], 8, 4, 128, 16, BF, seed=24, quant=quant)
+    x = case.device(dev)
+    x["table"][0, 7] = bad
+    for path in ("auto", "simt"):
+        case.run(dev, given=x, path=path)
+        torch.cuda.synchronize()
+        assert N.read_device_status(dev) == N.DEV_BAD_INDEX
