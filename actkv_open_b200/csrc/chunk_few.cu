@@ -250,24 +250,25 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
         for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
       float m0 = ninf, m1 = ninf, l0 = 0.0f, l1 = 0.0f;
 
-      // ---- copies of step i of this warp: lane l (and l - 16) looks up token l's block a step ahead
+      // ---- copies of step i of this warp: lane l (and l - 16) looks up token l's block a step ahead (and looks at
+      // what it got only then: 32 single tokens over 18432 in 8 bits 314 us where the id was used at once, 271 here)
       auto look_up = [&](int i) -> int {
         const int tok = start + i * round + (lane & 15);
-        if (i >= mine || tok >= end) return -2;
+        if (i >= mine || tok >= end) return -1;
         const int lb = block_of(tok);
-        return lb < a.MB ? max(table[lb], -1) : -1;           // -2 is this kernel's own, for the places past the end
+        return lb < a.MB ? table[lb] : -1;
       };
       int phys = look_up(0);
       const char* head = kv + (QUANT ? int64_t(h) * D : int64_t(h) * a.kv_stride_h * 2);
       const int at_word = a.Hkv * D + (D == 128 ? h * 4 : (h * 2) & ~3);
       auto issue = [&](int i, int slot) {
         if (i < mine) {
-          int ph = phys;
-          if (ph != -2 && (ph < 0 || ph >= a.NB)) {
-            flag(a.status, ACTKV_DEV_BAD_INDEX);
-            ph = 0;
-          }
           const int tok = start + i * round + (lane & 15);
+          int ph = phys;
+          if (uint32_t(ph) >= uint32_t(a.NB)) {               // past the end, or an id outside the cache
+            if (tok < end) flag(a.status, ACTKV_DEV_BAD_INDEX);
+            ph = tok < end ? 0 : -1;
+          }
           const int in_block = shift >= 0 ? tok & (a.BS - 1) : tok % a.BS;
           const int64_t off = ph < 0 ? -1 : int64_t(ph) * stride_b + int64_t(in_block) * stride_s;
           const uint32_t dst = ring + slot * Rg::kStage;
