@@ -261,16 +261,17 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
       int phys = look_up(0);
       const char* head = kv + (QUANT ? int64_t(h) * D : int64_t(h) * a.kv_stride_h * 2);
       const int at_word = a.Hkv * D + (D == 128 ? h * 4 : (h * 2) & ~3);
+      bool gaps = false;                      // this lane met a block outside the cache: from there on every step looks
       auto issue = [&](int i, int slot) {
         if (i < mine) {
           const int tok = start + i * round + (lane & 15);
-          int ph = phys;
-          if (uint32_t(ph) >= uint32_t(a.NB)) {               // past the end, or an id outside the cache
-            if (tok < end) flag(a.status, ACTKV_DEV_BAD_INDEX);
-            ph = tok < end ? 0 : -1;
+          const bool none = uint32_t(phys) >= uint32_t(a.NB); // past the end, or an id outside the cache: zeros
+          if (none && tok < end) {
+            flag(a.status, ACTKV_DEV_BAD_INDEX);
+            gaps = true;
           }
           const int in_block = shift >= 0 ? tok & (a.BS - 1) : tok % a.BS;
-          const int64_t off = ph < 0 ? -1 : int64_t(ph) * stride_b + int64_t(in_block) * stride_s;
+          const int64_t off = none ? -1 : int64_t(phys) * stride_b + int64_t(in_block) * stride_s;
           const uint32_t dst = ring + slot * Rg::kStage;
 #pragma unroll
           for (int e = 0; e < kCopies; ++e) {
@@ -310,6 +311,16 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
         [[maybe_unused]] const uint32_t sb = kb + 2 * Rg::kPlane;
         [[maybe_unused]] const int sh = QUANT && D == 64 && (h & 1) ? 16 : 0; // the head's bytes within the word
         bool found = false;
+        // the step's tokens that are there: neither past the end nor in a block outside the cache
+        [[maybe_unused]] uint32_t there = 0xffffu;
+        if constexpr (EDGE) {
+          bool here = lane < kStep && t + lane < end;
+          if (__any_sync(full, gaps) && here) {
+            const int lb = block_of(t + lane);
+            here = lb < a.MB && uint32_t(table[lb]) < uint32_t(a.NB);
+          }
+          there = __ballot_sync(full, here);
+        }
         if constexpr (QUANT) {
           // ---- S^T = K Q^T, tokens as the product's rows: s[0..1] token t + r8, s[2..3] token t + r8 + 8, query
           // rows 2 c4 and 2 c4 + 1.  Eight query rows fill the product's columns, O^T takes half the registers
@@ -339,8 +350,8 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
           if constexpr (EDGE) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int tok = t + r8 + (e >> 1) * 8;
-              s[e] = tok <= (e & 1 ? lim1 : lim0) && tok < end ? s[e] : ninf;
+              const int at = r8 + (e >> 1) * 8;
+              s[e] = t + at <= (e & 1 ? lim1 : lim0) && (there >> at & 1u) ? s[e] : ninf;
             }
           }
           float top0 = fmaxf(s[0], s[2]) * c2, top1 = fmaxf(s[1], s[3]) * c2;
@@ -424,9 +435,10 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               if constexpr (EDGE) {
-                const int tok = t + 8 * n + 2 * c4 + e;
-                s[n][e] = tok <= lim0 && tok < end ? s[n][e] : ninf;
-                s[n][2 + e] = tok <= lim1 && tok < end ? s[n][2 + e] : ninf;
+                const int at = 8 * n + 2 * c4 + e;
+                const bool is = there >> at & 1u;
+                s[n][e] = t + at <= lim0 && is ? s[n][e] : ninf;
+                s[n][2 + e] = t + at <= lim1 && is ? s[n][2 + e] : ninf;
               }
               top0 = fmaxf(top0, s[n][e]);
               top1 = fmaxf(top1, s[n][2 + e]);
@@ -503,7 +515,9 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
         bool edge = t + kStep - 1 > S - A || t + kStep > end;
         if constexpr (QUANT) {
           const uint32_t word = lds4(ring + slot * Rg::kStage + 2 * Rg::kPlane + lane * 4);
-          edge = edge || !__all_sync(full, plain_scales<BF16>(word));
+          edge = edge || !__all_sync(full, plain_scales<BF16>(word) && !gaps);
+        } else {
+          edge = edge || __any_sync(full, gaps);
         }
         if (edge) step(i, slot, std::true_type());
         else step(i, slot, std::false_type());

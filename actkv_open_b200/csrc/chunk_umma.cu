@@ -98,6 +98,7 @@ struct Sched {               // in shared memory
   uint32_t tmem;
   int abort_flag;
   int bad_v;                 // a value that some row of the unit does not see is not finite
+  int gaps;                  // some block was outside the cache: from there on every tile looks for them
   int few_rows;              // sessions of at most so many rows are chunk_few_kernel's in this call
   int64_t scan[kMaxThreads / 32], sums[2];
   Unit units[kUnitSlots];    // from the TMA warp, which alone walks the schedule; r < 0 ends it
@@ -268,6 +269,9 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* u) {
       "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_fill8(uint32_t taddr, uint32_t x) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%1], {%0,%0,%0,%0,%0,%0,%0,%0};" ::"r"(x), "r"(taddr) : "memory");
+}
 // Two 32-bit operations in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 r;
@@ -430,6 +434,12 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
   volatile int* abort_flag = &sched.abort_flag;
   const uint32_t abort_addr = smem_u32(&sched.abort_flag);
   volatile int* bad_v = &sched.bad_v;
+  volatile int* gaps = &sched.gaps;
+  // token tok of session r is in a block outside the cache
+  auto missing = [&](int r, int tok) {
+    const int lb = tok / a.BS;
+    return lb >= a.MB || uint32_t(a.block_table[r * a.bt_stride_r + lb]) >= uint32_t(a.NB);
+  };
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
   constexpr int kSlots = Ly::kSlots;
   constexpr int B_KVF = 0, B_KVE = kSlots, B_QF = 2 * kSlots, B_QE = B_QF + 1, B_SF = B_QE + 1, B_PF = B_SF + 2,
@@ -469,6 +479,7 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
     sched.share = Share{0, 0, a.R};
     sched.abort_flag = 0;
     sched.bad_v = 0;
+    sched.gaps = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     wide_parts(a.workspace, n_cta).desc[cta].valid = 0;
@@ -524,14 +535,16 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
       if (!any) break;
       if (x.t0 >= x.t1) continue;
       const int lead = x.two ? 1 : 2, nt = x.t1 - x.t0;
-      // first token slot (16-bit rows: in units of 8) of lane b's box of key tile t; -2 past the session's end
+      // first token slot (16-bit rows: in units of 8) of lane b's box of key tile t; -2 past the session's end or when
+      // the block is outside the cache (its tokens are hidden; the copies' barrier orders `gaps` before the tile)
       auto read_id = [&](int t) -> int {
         if (lane >= bpt || t < x.t0 || t >= x.t1 || t * kTile + lane * bs_box >= x.S) return -2;
         const int lb = mpb == 1 ? t * bpt + lane : t / mpb;
         const int phys = lb < a.MB ? a.block_table[x.r * a.bt_stride_r + lb] : -1;
         if (phys < 0 || phys >= a.NB) {
           flag(a.status, ACTKV_DEV_BAD_INDEX);
-          return 0;
+          *gaps = 1;
+          return -2;
         }
         const int64_t first = int64_t(phys) * a.BS + (mpb == 1 ? 0 : (t - lb * mpb) * kTile);
         return int(first >> (QUANT ? 0 : 3));
@@ -751,7 +764,7 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t ph = phys[i] < 0 || phys[i] >= a.NB ? 0 : phys[i];   // flagged by the TMA warp
+          const uint32_t ph = uint32_t(phys[i]) < uint32_t(a.NB) ? phys[i] : 0;   // else hidden, whatever the bytes say
           const uint8_t* p = p0 + uint64_t(ph * uint32_t(a.BS) + uint32_t(in_block[i] + off)) * uint32_t(a.kv_stride_s);
           if constexpr (D == 128) w1[i] = *reinterpret_cast<const uint32_t*>(p);
           else w1[i] = *reinterpret_cast<const uint16_t*>(p) | 0x7f7f0000u;
@@ -807,13 +820,16 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
         // The value rows of tokens past the session's end hold anything (slots never written, another
         // session's rows): zeroed, since 0 * NaN is NaN.  Values that some row of the unit does not
         // see must not reach it either: if one is not finite it is zeroed too, and the rows that do
-        // see it get it back at the end.
-        if (!QUANT && tok0 + kTile - 1 > lim_min && (!two || w == 0)) {
+        // see it get it back at the end.  Tokens of blocks outside the cache were not copied: hidden from all.
+        const bool gap = *gaps;
+        const bool masked = !__all_sync(full, tok0 + kTile - 1 <= lim && !gap);
+        if (!QUANT && (masked || tok0 + kTile - 1 > lim_min) && (!two || w == 0)) {
           const uint32_t pos = ring + v_position(t, nt, lead);
           ok = wait(B_KVF + pos % kSlots, (pos / kSlots) & 1u);
           if (!ok) break;
           clean_values<D, BF16>(smem + Ly::kKvOff + (pos % kSlots) * Ly::kTileBytes + (row >> 3) * Ly::kGroupBytes +
-                                (row & 7) * 128, tok0 + row >= x.S, tok0 + row > lim_min, bad_v);
+                                (row & 7) * 128, tok0 + row >= x.S || (gap && missing(x.r, tok0 + row)),
+                                tok0 + row > lim_min, bad_v);
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         fence_after();
@@ -821,10 +837,15 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
           // With the widening warps a thread has registers for half a row only: the second half is read for
           // the maximum, and again for p.
           float v[QUANT ? 1 : 2][64];
-          const bool masked = !__all_sync(full, tok0 + kTile - 1 <= lim);
           const int last = lim - tok0;                        // columns 0 .. last are seen
           float mx[4] = {ninf, ninf, ninf, ninf};
           if (masked) {                                       // hidden columns become -inf where they are
+            if (__any_sync(full, gap)) {                      // 8 tokens are in one block
+#pragma unroll 1
+              for (int q = 0; q < kTile / 8; ++q)
+                if (missing(x.r, tok0 + q * 8)) tmem_fill8(s_addr + q * 8, __float_as_uint(ninf));
+              tmem_wait_st();
+            }
 #pragma unroll 1
             for (int q = 0; q < 8; ++q) {
               if (__all_sync(full, q * 16 + 15 <= last)) continue;
@@ -1115,10 +1136,14 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
       if (!ok) break;
       uint32_t sc = reinterpret_cast<const uint32_t*>(smem + Ly::kScaleOff)[in.slot * kTile + row0 + (lane & 15)];
       const int first = t * kTile + row0;                     // the warp's first token
-      const bool edge = first + 16 > min(u.S, plane ? u.hidden : u.S);
-      if (edge) {
+      const bool gap = *gaps, edge = first + 16 > min(u.S, plane ? u.hidden : u.S);
+      const bool plain = __all_sync(full, plain_scales<BF16>(sc) && !gap);
+      uint32_t gone = 0;                                      // the warp's tokens that are not there: zeros
+      if (edge || !plain) {
         const int tok = first + (lane & 15);
-        if (tok >= u.S) {
+        const bool out = tok >= u.S || (gap && missing(u.r, tok));
+        gone = __ballot_sync(full, out);
+        if (out) {
           sc = 0x7f7f7f7fu;
         } else if (plane && tok >= u.hidden) {   // a NaN group's values are 0; the rows that see it get NaN at the end
           const uint32_t bad = __vcmpeq4(sc, 0xffffffffu);
@@ -1128,7 +1153,6 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
       }
       const uint8_t* src = smem + Ly::kRawOff + in.slot * Ly::kRawBytes + row0 * D;
       uint8_t* dst = smem + Ly::kKvOff + ring.slot * Ly::kTileBytes + (row0 >> 3) * Ly::kGroupBytes;
-      const bool plain = __all_sync(full, plain_scales<BF16>(sc));
       // Rolled, 8 tokens at a time: the warps of a scheduler are at five places of the kernel, and straight code
       // for all 16 tokens starved it of instructions.
       if (plain && !edge) {
@@ -1151,7 +1175,7 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
           const int row = i * kRpi + lr, g8 = i * kRpi / 8;     // of the warp's 16
           const bool odd = i * kRpi % 8 != 0;
           uint4 x = *reinterpret_cast<const uint4*>(src + g8 * 8 * D + (odd ? get[8 / kRpi - 1] : get[0]));
-          if (first + row >= u.S) x = make_uint4(0u, 0u, 0u, 0u);
+          if (gone >> row & 1u) x = make_uint4(0u, 0u, 0u, 0u);
           const uint32_t b = __byte_perm(__shfl_sync(full, sc, row), 0u, 0x4440 | (lc >> 1));
           uint32_t r[8], f1, f2;
           any_factors<BF16>(b, f1, f2);

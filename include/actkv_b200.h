@@ -457,6 +457,8 @@ ACTKV_API int actkv_decode_attention(const void* q, int dtype, int64_t q_stride_
  *   out[t, hq, :] = softmax(scale * q . k) @ v,  lse[t, hq] = log sum exp(scale * q . k)
  * (out 0 and lse -inf for a query that sees no token).  Sessions may have no queries.  Tokens a
  * query does not see do not reach its results, whatever they hold.
+ * Tokens of a block id outside the cache, or past the table's width, set ACTKV_DEV_BAD_INDEX and are hidden from
+ * every query: nothing is read in their place.
  * A session whose offsets leave the T rows sets ACTKV_DEV_BAD_INDEX and gets no results; rows of out
  * and lse that are no session's are not written.
  * q, out and the cache kv [2][NB][BS][Hkv][D] have one dtype (element strides, D contiguous), out

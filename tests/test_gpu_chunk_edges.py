@@ -97,3 +97,68 @@ def test_every_block_id_outside_the_cache_is_flagged(bad, new, quant):
         case.run(dev, given=x, path=path)
         torch.cuda.synchronize()
         assert N.read_device_status(dev) == N.DEV_BAD_INDEX
+
+
+def _holes_ref(case, gone):
+    """64-bit attention of a one- or many-session case in which the tokens gone[r] (a bool per token) are hidden."""
+    t, hq, d = case.q.shape
+    out, mag = torch.zeros(t, hq, d, dtype=torch.float64), torch.zeros(t, hq, d, dtype=torch.float64)
+    lse, size = torch.full((t, hq), -torch.inf, dtype=torch.float64), torch.zeros(t, hq, dtype=torch.float64)
+    for r, s in enumerate(case.lens):
+        o0, o1 = int(case.off[r]), int(case.off[r + 1])
+        k, v = (case.tokens(p, r).double().repeat_interleave(hq // case.hkv, 1) for p in range(2))
+        q = case.q[o0:o1].double()
+        x = torch.einsum("ahd,shd->ahs", q, k) * d ** -0.5
+        hide = (torch.arange(s)[None] > torch.arange(s - (o1 - o0), s)[:, None]) | gone[r][None]
+        x = x.masked_fill(hide[:, None], -torch.inf)
+        one = torch.logsumexp(x, -1)
+        p = torch.where(torch.isfinite(one)[..., None], torch.exp(x - one[..., None]), torch.zeros_like(x))
+        out[o0:o1], mag[o0:o1] = (torch.einsum("ahs,shd->ahd", p, y) for y in (v, v.abs()))
+        lse[o0:o1], size[o0:o1] = one, torch.einsum("ahd,shd->ahs", q.abs(), k.abs()).amax(-1) * d ** -0.5
+    return out, lse, mag, size
+
+
+def _within(got, ref):
+    out, lse = (x.cpu().double() for x in got)
+    want, want_l, mag, size = ref
+    assert ((out - want).abs() <= (2 * U[BF] + 1e-4) * mag).all()
+    empty = want_l == -torch.inf
+    assert torch.equal(lse == -torch.inf, empty) and (out[empty] == 0).all()
+    assert ((lse - want_l).abs()[~empty] <= 2e-5 + 8e-6 * size[~empty]).all()
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("lens, new, bs, d", [([500], [1], 16, 128), ([500], [3], 16, 64), ([500, 300], [90, 2], 16, 128),
+                                              ([700, 129], [300, 33], 64, 64), ([9000], [2], 16, 128),
+                                              ([9000, 60], [70, 4], 16, 128), ([900], [140], 256, 128)])
+def test_tokens_of_blocks_outside_the_cache_are_hidden(lens, new, bs, d, quant):
+    """A bad entry at a table's start, middle and end, a whole bad row, and a table narrower than its session, on the
+    tensor cores and the CUDA cores: those tokens count for nothing, and what block 0 holds (NaN here) is not read in
+    their place."""
+    dev = need_gpu()
+    from actkv_open_b200 import _native as N
+    case = Case(lens, new, 8, 4, d, bs, BF, seed=25, quant=quant)
+    x = case.device(dev)
+    nan = 255 if quant else float("nan")
+    x["cache"] = torch.cat([torch.full_like(x["cache"][:, :1], nan), x["cache"]], 1)
+    whole = x["table"] + 1
+    n = [-(-s // bs) for s in lens]
+    for bad in ([0], [n[0] // 2], [n[0] - 1], [0, n[0] // 3, n[0] - 2], list(range(n[0])), "narrow"):
+        gone = [torch.zeros(s, dtype=torch.bool) for s in lens]
+        if bad == "narrow":
+            keep = n[0] - 1 - n[0] // 4
+            table = whole[:, :keep]
+            for g in gone:
+                g[keep * bs:] = True
+            if keep == 0:
+                continue
+        else:
+            table = whole.clone()
+            for b in bad:
+                table[0, b] = -1 if b % 2 else case.nb + 1 + b
+                gone[0][b * bs:(b + 1) * bs] = True
+        ref = _holes_ref(case, gone)
+        for path in ("auto", "simt"):
+            _within(case.run(dev, given={**x, "table": table}, path=path), ref)
+            torch.cuda.synchronize()
+            assert N.read_device_status(dev) == N.DEV_BAD_INDEX
