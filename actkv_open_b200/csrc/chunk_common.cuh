@@ -199,26 +199,40 @@ template <bool BF16>
 __device__ __forceinline__ uint32_t plain_factor(uint32_t b) {
   return BF16 ? b * 0x00800080u + 0x3c003c00u : (b - 104u) * 0x04000400u;
 }
-// For any scale byte: the multiplier within the type, and a second one.
+// For any scale byte: multipliers whose product is the power of two, each a value of the type, in an order in which
+// only the last one that is not 1 rounds.  fp16: 2^(b - 119) is 2^-7, exact for what comes first, and the rest, down to
+// its subnormals (0 below: such values round to 0); or up to three factors of at most 2^15, past which everything but 0
+// is past the range.
 template <bool BF16>
-__device__ __forceinline__ void any_factors(uint32_t b, uint32_t& f1, uint32_t& f2) {
-  const int e = BF16 ? int(b) + 120 : int(b) - 104, top = BF16 ? 254 : 30;
-  const int e1 = min(max(e, 1), top), e2 = min(max(e - e1 + (BF16 ? 127 : 15), 1), top);
-  const uint32_t one = BF16 ? 0x00800080u : 0x04000400u;
-  f1 = b == 255u ? 0x7fff7fffu : e1 * one;   // 255: NaN
-  f2 = e2 * one;
-}
-template <bool BF16>
-__device__ __forceinline__ void widen16_rest(uint32_t b, uint32_t f2, uint32_t (&r)[8]) {
-  if (b == 255u) return;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    r[i] = mul16x2<BF16>(r[i], f2);
-    if constexpr (!BF16) {
-      asm("min.f16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(0x7bff7bffu));
-      asm("max.f16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(0xfbfffbffu));
-    }
+__device__ __forceinline__ void any_factors(uint32_t b, uint32_t (&f)[3]) {
+  const uint32_t one = BF16 ? 0x3f803f80u : 0x3c003c00u;
+  f[1] = f[2] = one;
+  if constexpr (BF16) {
+    const int e = int(b) + 120, e1 = min(e, 254);
+    f[0] = e1 * 0x00800080u;
+    f[1] = (e - e1 + 127) * 0x00800080u;
+  } else if (b < 105u) {
+    f[0] = 0x20002000u;                        // 2^-7
+    f[1] = (b >= 98u ? b - 97u << 10 : (b >= 88u ? 1u << b - 88u : 0u)) * 0x00010001u;
+  } else {
+    const uint32_t e = min(b, 164u) - 104u;    // the exponent field of one factor, 30 of which it can hold
+    const uint32_t e1 = min(e, 30u), e2 = min(e - e1, 15u), e3 = e - e1 - e2;
+    f[0] = e1 * 0x04000400u;
+    f[1] = (e2 + 15u) * 0x04000400u;
+    f[2] = (e3 + 15u) * 0x04000400u;
   }
+  if (b == 255u) f[0] = 0x7fff7fffu;           // NaN
+}
+// x, already under the exponent and times the first factor, times the others; past fp16's range: its largest.
+template <bool BF16>
+__device__ __forceinline__ uint32_t mul_rest(uint32_t x, uint32_t f1, uint32_t f2) {
+  x = mul16x2<BF16>(x, f1);
+  if constexpr (!BF16) {
+    x = mul16x2<BF16>(x, f2);
+    asm("min.NaN.f16x2 %0, %0, %1;" : "+r"(x) : "r"(0x7bff7bffu));
+    asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(x) : "r"(0xfbfffbffu));
+  }
+  return x;
 }
 
 

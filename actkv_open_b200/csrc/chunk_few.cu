@@ -120,18 +120,11 @@ __device__ __forceinline__ uint32_t widen2(uint32_t x, uint32_t f) {
 // ... for any scale bytes of the two halves.
 template <bool BF16>
 __device__ __forceinline__ uint32_t widen2_any(uint32_t x, uint32_t b_lo, uint32_t b_hi) {
-  uint32_t l1, l2, h1, h2;
-  any_factors<BF16>(b_lo, l1, l2);
-  any_factors<BF16>(b_hi, h1, h2);
-  uint32_t r = widen2<BF16>(x, __byte_perm(l1, h1, 0x5410));
-  if (b_lo == 255u) l2 = BF16 ? 0x3f803f80u : 0x3c003c00u;             // 1: NaN stays
-  if (b_hi == 255u) h2 = BF16 ? 0x3f803f80u : 0x3c003c00u;
-  r = mul16x2<BF16>(r, __byte_perm(l2, h2, 0x5410));
-  if constexpr (!BF16) {                      // past fp16's range: its largest
-    asm("min.NaN.f16x2 %0, %0, %1;" : "+r"(r) : "r"(0x7bff7bffu));
-    asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(r) : "r"(0xfbfffbffu));
-  }
-  return r;
+  uint32_t lo[3], hi[3];
+  any_factors<BF16>(b_lo, lo);
+  any_factors<BF16>(b_hi, hi);
+  return mul_rest<BF16>(widen2<BF16>(x, __byte_perm(lo[0], hi[0], 0x5410)), __byte_perm(lo[1], hi[1], 0x5410),
+                        __byte_perm(lo[2], hi[2], 0x5410));
 }
 // What is not finite among two 16-bit values, in the halves `hide` (0xffff per half), becomes 0.
 template <bool BF16>

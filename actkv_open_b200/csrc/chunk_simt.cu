@@ -32,7 +32,7 @@ __device__ __forceinline__ void load_row(const ChunkArgs& a, const void* base, i
     if constexpr (QUANT) {
       const uint8_t* row = static_cast<const uint8_t*>(base) + off;
       const int e = h * a.D + d;
-      x[i] = e4m3x2_f32(row[e]).x * scale_of(row[a.Hkv * a.D + e / kQuantGroup]);
+      x[i] = to_f32(from_f32<T>(e4m3x2_f32(row[e]).x * scale_of(row[a.Hkv * a.D + e / kQuantGroup])));
     } else {
       x[i] = to_f32(static_cast<const T*>(base)[off + int64_t(h) * a.kv_stride_h + d]);
     }

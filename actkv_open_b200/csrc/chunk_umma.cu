@@ -1177,10 +1177,11 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
           uint4 x = *reinterpret_cast<const uint4*>(src + g8 * 8 * D + (odd ? get[8 / kRpi - 1] : get[0]));
           if (gone >> row & 1u) x = make_uint4(0u, 0u, 0u, 0u);
           const uint32_t b = __byte_perm(__shfl_sync(full, sc, row), 0u, 0x4440 | (lc >> 1));
-          uint32_t r[8], f1, f2;
-          any_factors<BF16>(b, f1, f2);
-          widen16<BF16>(x, f1, r);
-          widen16_rest<BF16>(b, f2, r);
+          uint32_t r[8], f[3];
+          any_factors<BF16>(b, f);
+          widen16<BF16>(x, f[0], r);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) r[k] = mul_rest<BF16>(r[k], f[1], f[2]);
           uint8_t* d8 = dst + g8 * Ly::kGroupBytes;
           put(d8 + (odd ? put0[8 / kRpi - 1] : put0[0]), d8 + (odd ? put1[8 / kRpi - 1] : put1[0]), r);
         }

@@ -44,13 +44,6 @@ __device__ __forceinline__ uint32_t max16x2(uint32_t a, uint32_t b) {
   return r;
 }
 
-template <typename T> __device__ __forceinline__ T from_f32(float x);
-template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
-template <> __device__ __forceinline__ __half from_f32<__half>(float x) {   // past the range: its largest
-  return __float2half_rn(x == x ? fminf(fmaxf(x, -65504.0f), 65504.0f) : x);
-}
-template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-
 template <typename T>
 __device__ __forceinline__ void store16(T* p, bool vec, const float (&x)[16]) {
   if (vec) {

@@ -43,6 +43,14 @@ __device__ __forceinline__ uint32_t f32_e4m3x2(float lo, float hi) {
   return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
 
+// A value of the cache in the type it is read in.
+template <typename T> __device__ __forceinline__ T from_f32(float x);
+template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float x) {   // past the range: its largest
+  return __float2half_rn(x == x ? fminf(fmaxf(x, -65504.0f), 65504.0f) : x);
+}
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
 // Session of packed token t, R when it is none's (before the first offset or past the last): the number of
 // sessions whose last token comes at or before t.  Called by a whole warp with one t; 32 offsets per step.
 __device__ __forceinline__ int session_of(const int32_t* off, int R, int t, int lane) {

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from gpu_util import assert_device_clean, need_gpu
-from test_gpu_chunk import BF, Case, U, _equal
+from test_gpu_chunk import BF, HF, Case, U, _equal
 
 pytestmark = pytest.mark.gpu
 
@@ -162,3 +162,60 @@ def test_tokens_of_blocks_outside_the_cache_are_hidden(lens, new, bs, d, quant):
             _within(case.run(dev, given={**x, "table": table}, path=path), ref)
             torch.cuda.synchronize()
             assert N.read_device_status(dev) == N.DEV_BAD_INDEX
+
+
+def _one_token_sessions(byte, scale, plane, hkv, d, dtype, new):
+    """R sessions of one token; its row of ``plane`` (0: keys, 1: values) has the given e4m3 bytes [R, Hkv, D] and scale
+    bytes [R, Hkv, D / 32], the other plane's row is zero.  ``new`` query tokens each, the last of which sees the token;
+    q is one-hot, of 1.  Returns the case and the dim [R * new, Hq] in which q is 1."""
+    from actkv_open_b200.kernels.quant_cache import quant_row_bytes
+    r = byte.shape[0]
+    case = Case.__new__(Case)
+    case.lens, case.new, case.hq, case.hkv, case.d, case.bs, case.dtype, case.quant = [1] * r, [new] * r, 2 * hkv, hkv, d, 16, dtype, True
+    case.table, case.nb = torch.arange(r, dtype=torch.int32)[:, None], r
+    case.off = torch.arange(r + 1, dtype=torch.int32) * new
+    case.row = quant_row_bytes(hkv, d)
+    case.cache = torch.full((2, r, 16, case.row), 255, dtype=torch.uint8)
+    case.cache[:, :, 0] = 0
+    case.cache[plane, :, 0, :hkv * d] = byte.reshape(r, -1)
+    case.cache[plane, :, 0, hkv * d:hkv * (d + d // 32)] = scale.reshape(r, -1)
+    hot = (torch.arange(r * new)[:, None] * 7 + torch.arange(2 * hkv)[None] * 3) % d
+    case.q = torch.nn.functional.one_hot(hot, d).to(dtype)
+    return case, hot
+
+
+def _read_back(case, dev):
+    from actkv_open_b200.kernels.quant_cache import dequantize_read
+    x = case.device(dev)
+    r = len(case.lens)
+    off = torch.arange(r + 1, dtype=torch.int32, device=dev)
+    k, v = dequantize_read(x["cache"][None], case.hkv, case.d, off, x["table"], x["seq"], r, dtype=case.dtype)
+    return k[0], v[0]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new, path", [(1, "auto"), (20, "auto"), (1, "simt")])
+def test_every_scale_byte_is_attended_as_it_is_read_back(new, path, d, dtype):
+    """One token per session: with a zero key the output is its value row bit for bit, and with one-hot queries the lse
+    is a dim of its key, which shows what the attention kernels make of e4m3 bytes and scale bytes.  Scale bytes
+    0 to 254 for the values (fp16: results that round to subnormals, to zero and past the range, which
+    saturate; bf16 short of inf), and for keys those of logits up to 2^24."""
+    dev = need_gpu()
+    hkv, r = 2, 256
+    gen = torch.Generator().manual_seed(26)
+    byte = torch.randint(0, 256, (r, hkv, d), generator=gen)
+    byte = torch.where((byte & 127) == 127, byte - 1, byte).to(torch.uint8)      # e4m3's own NaN is not of this test
+    scale = torch.randint(0, 255, (r, hkv, d // 32), generator=gen)
+    scale[:255, 0, 0] = torch.arange(255)
+    scale[:60, 1, 0] = torch.arange(90, 150)
+    last = torch.arange(r, device=dev) * new + new - 1
+    most = (245, 142) if dtype == BF else (254, 254)
+    case, _ = _one_token_sessions(byte, scale.clamp(max=most[0]), 1, hkv, d, dtype, new)
+    out, lse = case.run(dev, path=path)
+    assert torch.equal(out[last], _read_back(case, dev)[1].repeat_interleave(2, 1)) and (lse[last] == 0).all()
+    case, hot = _one_token_sessions(byte, scale.clamp(max=most[1]), 0, hkv, d, dtype, new)
+    out, lse = case.run(dev, path=path, scale=1.0)
+    want = _read_back(case, dev)[0].repeat_interleave(2, 1).gather(2, hot.to(dev)[last][..., None])[..., 0].double()
+    assert ((lse[last].double() - want).abs() <= 1e-6 * want.abs()).all() and (out[last] == 0).all()
+    assert_device_clean(dev)
