@@ -4,6 +4,7 @@
 
 #include "common.cuh"
 #include "kernels.cuh"
+#include "quant_row.cuh"
 #include "umma_common.cuh"
 
 namespace actkv {
@@ -234,7 +235,21 @@ __device__ __forceinline__ uint32_t mul_rest(uint32_t x, uint32_t f1, uint32_t f
   }
   return x;
 }
-
+// What is not finite among two 16-bit values, in the halves `hide` (0xffff per half), becomes 0.
+template <bool BF16>
+__device__ __forceinline__ uint32_t drop_bad(uint32_t u, uint32_t hide, bool& found) {
+  constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
+  uint32_t bad = ((u & kExp) == kExp ? 0xffffu : 0u) | (((u >> 16) & kExp) == kExp ? 0xffff0000u : 0u);
+  bad &= hide;
+  found |= bad != 0;
+  return u & ~bad;
+}
+// Value e of an 8-bit row, inf and NaN as in the 16-bit type (whose finite values it may exceed in digits).
+template <bool BF16>
+__device__ __forceinline__ float quant_value(const uint8_t* row, int Hkv, int D, int e) {
+  const float x = e4m3x2_f32(row[e]).x * scale_of(row[Hkv * D + e / kQuantGroup]);
+  return BF16 || x != x ? x : fminf(fmaxf(x, -65504.0f), 65504.0f);
+}
 
 }  // namespace chunk
 }  // namespace actkv

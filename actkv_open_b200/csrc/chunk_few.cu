@@ -126,16 +126,6 @@ __device__ __forceinline__ uint32_t widen2_any(uint32_t x, uint32_t b_lo, uint32
   return mul_rest<BF16>(widen2<BF16>(x, __byte_perm(lo[0], hi[0], 0x5410)), __byte_perm(lo[1], hi[1], 0x5410),
                         __byte_perm(lo[2], hi[2], 0x5410));
 }
-// What is not finite among two 16-bit values, in the halves `hide` (0xffff per half), becomes 0.
-template <bool BF16>
-__device__ __forceinline__ uint32_t drop_bad(uint32_t u, uint32_t hide, bool& found) {
-  constexpr uint32_t kExp = BF16 ? 0x7f80u : 0x7c00u;
-  uint32_t bad = ((u & kExp) == kExp ? 0xffffu : 0u) | (((u >> 16) & kExp) == kExp ? 0xffff0000u : 0u);
-  bad &= hide;
-  found |= bad != 0;
-  return u & ~bad;
-}
-
 struct Sched {
   Share share;
   int64_t scan[32], sums[2];
@@ -314,6 +304,14 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
           }
           there = __ballot_sync(full, here);
         }
+        // the lane's tokens of the values, and those that some row does not see: what is not finite goes in as 0
+        const int row[4] = {2 * c4, 2 * c4 + 1, 2 * c4 + 8, 2 * c4 + 9};
+        [[maybe_unused]] uint32_t hide[2] = {0u, 0u};
+        if constexpr (EDGE) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+            hide[n] = (t + row[2 * n] > S - A ? 0xffffu : 0u) | (t + row[2 * n + 1] > S - A ? 0xffff0000u : 0u);
+        }
         if constexpr (QUANT) {
           // ---- S^T = K Q^T, tokens as the product's rows: s[0..1] token t + r8, s[2..3] token t + r8 + 8, query
           // rows 2 c4 and 2 c4 + 1.  Eight query rows fill the product's columns, O^T takes half the registers
@@ -364,7 +362,6 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
           // p^T as the second operand: row r8, tokens 2 c4, 2 c4 + 1 and those + 8
           const uint32_t p0 = transpose8x8(pack2<BF16>(x, y)), p1 = transpose8x8(pack2<BF16>(z, w));
           // ---- O^T += V^T p^T: values of tokens 2 c4, 2 c4 + 1 and those + 8, dims kTiles r8 ..
-          const int row[4] = {2 * c4, 2 * c4 + 1, 2 * c4 + 8, 2 * c4 + 9};
           uint32_t vw[4][kTiles / 4], b[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -381,12 +378,6 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
               vw[e][1] = u.y;
             }
             b[e] = (lds4(sb + 64 + row[e] * 4) >> (sh + kTiles * r8 / 32 * 8)) & 255u;
-            if constexpr (EDGE) {
-              if (b[e] == 255u && t + row[e] > S - A) {       // its values are 0; the rows that see it get NaN later
-                b[e] = 127u;
-                found = true;
-              }
-            }
           }
           const uint32_t f0 = __byte_perm(plain_factor<BF16>(b[0]), plain_factor<BF16>(b[1]), 0x5410);
           const uint32_t f1 = __byte_perm(plain_factor<BF16>(b[2]), plain_factor<BF16>(b[3]), 0x5410);
@@ -401,7 +392,8 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
 #pragma unroll
               for (int n = 0; n < 4; ++n) {
                 const uint32_t x = __byte_perm(pair[e][n >> 1], 0u, n & 1 ? 0x4342 : 0x4140);
-                m[n] = EDGE ? widen2_any<BF16>(x, b[n >> 1 << 1], b[(n >> 1 << 1) + 1]) : widen2<BF16>(x, n >> 1 ? f1 : f0);
+                if constexpr (EDGE) m[n] = drop_bad<BF16>(widen2_any<BF16>(x, b[n >> 1 << 1], b[(n >> 1 << 1) + 1]), hide[n >> 1], found);
+                else m[n] = widen2<BF16>(x, n >> 1 ? f1 : f0);
               }
               mma16816<BF16>(o[k * 2 + e], m, p0, p1);
             }
@@ -410,12 +402,12 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
           float s[2][4];
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
-            const int row = n * 8 + r8;
+            const int tok = n * 8 + r8;
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
 #pragma unroll
             for (int p = 0; p < (CH + 3) / 4; ++p) {
-              const uint4 u = lds16(kb + row * (CH * 16) + key_piece<CH>(row, c4 + 4 * p) * 16);
+              const uint4 u = lds16(kb + tok * (CH * 16) + key_piece<CH>(tok, c4 + 4 * p) * 16);
               const uint32_t w[4] = {u.x, u.y, u.z, u.w};
               mma16816<BF16>(s[n], q[p * 2], w[0], w[1]);           // 8 dims: two k-steps
               mma16816<BF16>(s[n], q[p * 2 + 1], w[2], w[3]);
@@ -459,13 +451,6 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
             }
           }
           // ---- values: tokens 2 c4, 2 c4 + 1 and those + 8, dims kTiles r8 ..
-          const int row[4] = {2 * c4, 2 * c4 + 1, 2 * c4 + 8, 2 * c4 + 9};
-          uint32_t hide[2] = {0u, 0u};
-          if constexpr (EDGE) {
-#pragma unroll
-            for (int n = 0; n < 2; ++n)
-              hide[n] = (t + row[2 * n] > S - A ? 0xffffu : 0u) | (t + row[2 * n + 1] > S - A ? 0xffff0000u : 0u);
-          }
 #pragma unroll
             for (int c = 0; c < kTiles / 8; ++c) {
               uint32_t w[4][4];
@@ -606,7 +591,7 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
                 for (int d = d0; d < d0 + kTiles; ++d) {
                   float f;
                   if constexpr (QUANT) {
-                    f = static_cast<uint8_t>(p[a.Hkv * D + (h * D + d) / 32]) == 255 ? __int_as_float(0x7fffffff) : 0.0f;
+                    f = quant_value<BF16>(reinterpret_cast<const uint8_t*>(p), a.Hkv, D, h * D + d);
                   } else {
                     const uint16_t u = reinterpret_cast<const uint16_t*>(p)[int64_t(h) * a.kv_stride_h + d];
                     f = BF16 ? __uint_as_float(uint32_t(u) << 16) : __half2float(__ushort_as_half(u));

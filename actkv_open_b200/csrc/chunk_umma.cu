@@ -1036,9 +1036,8 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
 #pragma unroll 1
             for (int d = 0; d < D; ++d) {
               float f;
-              if constexpr (QUANT) {             // 32 values share a scale byte; 255 makes them NaN
-                f = static_cast<const uint8_t*>(a.kv)[at + a.Hkv * D + x.h * (D / 32) + d / 32] == 255
-                        ? __int_as_float(0x7fffffff) : 0.0f;
+              if constexpr (QUANT) {
+                f = quant_value<BF16>(static_cast<const uint8_t*>(a.kv) + at, a.Hkv, D, x.h * D + d);
               } else {
                 const uint16_t u = static_cast<const uint16_t*>(a.kv)[at + int64_t(x.h) * a.kv_stride_h + d];
                 f = BF16 ? __uint_as_float(uint32_t(u) << 16) : __half2float(__ushort_as_half(u));
@@ -1143,13 +1142,7 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
         const int tok = first + (lane & 15);
         const bool out = tok >= u.S || (gap && missing(u.r, tok));
         gone = __ballot_sync(full, out);
-        if (out) {
-          sc = 0x7f7f7f7fu;
-        } else if (plane && tok >= u.hidden) {   // a NaN group's values are 0; the rows that see it get NaN at the end
-          const uint32_t bad = __vcmpeq4(sc, 0xffffffffu);
-          if (bad) *bad_v = 1;
-          sc = (sc & ~bad) | (0x7f7f7f7fu & bad);
-        }
+        if (out) sc = 0x7f7f7f7fu;
       }
       const uint8_t* src = smem + Ly::kRawOff + in.slot * Ly::kRawBytes + row0 * D;
       uint8_t* dst = smem + Ly::kKvOff + ring.slot * Ly::kTileBytes + (row0 >> 3) * Ly::kGroupBytes;
@@ -1182,6 +1175,12 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
           widen16<BF16>(x, f[0], r);
 #pragma unroll
           for (int k = 0; k < 8; ++k) r[k] = mul_rest<BF16>(r[k], f[1], f[2]);
+          if (plane && first + row >= u.hidden) {   // some row does not see it: what is not finite goes in as 0
+            bool found = false;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) r[k] = drop_bad<BF16>(r[k], 0xffffffffu, found);
+            if (found) *bad_v = 1;
+          }
           uint8_t* d8 = dst + g8 * Ly::kGroupBytes;
           put(d8 + (odd ? put0[8 / kRpi - 1] : put0[0]), d8 + (odd ? put1[8 / kRpi - 1] : put1[0]), r);
         }

@@ -5,6 +5,7 @@ test_gpu_chunk.py."""
 import pytest
 import torch
 
+import chunk_cases as C
 from gpu_util import assert_device_clean, need_gpu
 from test_gpu_chunk import BF, HF, Case, U, _equal
 
@@ -218,4 +219,33 @@ def test_every_scale_byte_is_attended_as_it_is_read_back(new, path, d, dtype):
     out, lse = case.run(dev, path=path, scale=1.0)
     want = _read_back(case, dev)[0].repeat_interleave(2, 1).gather(2, hot.to(dev)[last][..., None])[..., 0].double()
     assert ((lse[last].double() - want).abs() <= 1e-6 * want.abs()).all() and (out[last] == 0).all()
+    assert_device_clean(dev)
+
+
+@pytest.mark.parametrize("new, path", [(3, "auto"), (90, "auto"), (200, "auto"), (3, "simt"), (90, "simt")])
+@pytest.mark.parametrize("lens", [500, 5000])
+@pytest.mark.parametrize("d", [64, 128])
+def test_hidden_values_past_the_range_of_an_8_bit_cache(d, lens, new, path):
+    """A value e4m3 * 2^(byte - 127) past bf16's range is inf, of either sign: rows that see its token have it in that
+    dim, rows that do not (their p is 0) are as without it."""
+    dev = need_gpu()
+    case = Case([lens], [new], 8, 4, d, 16, BF, seed=27, quant=True)
+    clean = case.run(dev, path=path)
+    tok = lens - new + new // 2                          # the second half of the new tokens sees it
+    at = int(C.slots(case.table, 0, tok, tok + 1, 16))
+    head, dim = 2, 37
+    group = slice(4 * d + (head * d + 32) // 32, 4 * d + (head * d + 32) // 32 + 1)
+    lo = head * d + 32
+    case.cache[1, at, lo:lo + 32] = 0
+    case.cache[1, at, group] = 127
+    zero = case.run(dev, path=path)                      # the same without those 32 values
+    case.cache[1, at, head * d + dim], case.cache[1, at, head * d + dim + 1] = 0x7e, 0xfe
+    case.cache[1, at, group] = 254
+    got = case.run(dev, path=path)
+    see, q = new // 2, slice(2 * head, 2 * head + 2)
+    assert _equal([x[:see] for x in got], [x[:see] for x in clean]) and torch.equal(got[1], clean[1])
+    assert (got[0][see:, q, dim] == torch.inf).all() and (got[0][see:, q, dim + 1] == -torch.inf).all()
+    want = zero[0].clone()
+    want[see:, q, dim], want[see:, q, dim + 1] = torch.inf, -torch.inf
+    assert torch.equal(got[0], want)
     assert_device_clean(dev)
