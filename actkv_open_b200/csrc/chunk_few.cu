@@ -123,13 +123,13 @@ __device__ __forceinline__ uint32_t widen2_any(uint32_t x, uint32_t b_lo, uint32
   uint32_t lo[3], hi[3];
   any_factors<BF16>(b_lo, lo);
   any_factors<BF16>(b_hi, hi);
-  return mul_rest<BF16>(widen2<BF16>(x, __byte_perm(lo[0], hi[0], 0x5410)), __byte_perm(lo[1], hi[1], 0x5410),
-                        __byte_perm(lo[2], hi[2], 0x5410));
+  return put_nan(mul_rest<BF16>(widen2<BF16>(x, __byte_perm(lo[0], hi[0], 0x5410)), __byte_perm(lo[1], hi[1], 0x5410),
+                                __byte_perm(lo[2], hi[2], 0x5410)), x & 0x007f007fu);
 }
 struct Sched {
   Share share;
   int64_t scan[32], sums[2];
-  int bad_v;
+  int bad_v;                 // values that are not finite went in as 0: 1 among those some row does not see, 2 anywhere
 };
 static_assert(sizeof(Sched) <= 512, "the schedule's place in shared memory");
 
@@ -287,6 +287,8 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
           o[j][3] *= e1;
         }
       };
+      // 8-bit rows: e4m3 NaN among the keys and among the values of the steps whose every token every row sees
+      [[maybe_unused]] uint32_t odd_k = 0, odd_v = 0;
       auto step = [&](int i, int slot, auto edge_) {
         constexpr bool EDGE = decltype(edge_)::value;        // hidden tokens, or scale bytes out of the ordinary
         const int t = start + i * round;
@@ -323,6 +325,10 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
             const uint4 u = lds16(kb + r8 * (CH * 16) + key_piece<CH>(r8, c4 + 4 * p) * 16);
             const uint4 v = lds16(kb + (r8 + 8) * (CH * 16) + key_piece<CH>(r8 + 8, c4 + 4 * p) * 16);
             const uint32_t w0[4] = {u.x, u.y, u.z, u.w}, w1[4] = {v.x, v.y, v.z, v.w};
+            if constexpr (!EDGE) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) odd_k = nan_bytes(nan_bytes(odd_k, w0[k]), w1[k]);
+            }
             const int g8 = (c4 + 4 * p) / 2 * 8;             // 16 dims: four k-steps of one scale group
             const uint32_t b0 = word0 >> g8 & 255u, b1 = word1 >> g8 & 255u;
             const uint32_t f0 = plain_factor<BF16>(b0), f1 = plain_factor<BF16>(b1);
@@ -376,6 +382,10 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
               const uint2 u = lds8(base + value_piece<CH>(row[e], r8 >> 1) * 16 + (r8 & 1) * 8);
               vw[e][0] = u.x;
               vw[e][1] = u.y;
+            }
+            if constexpr (!EDGE) {
+#pragma unroll
+              for (int k = 0; k < kTiles / 4; ++k) odd_v = nan_bytes(odd_v, vw[e][k]);
             }
             b[e] = (lds4(sb + 64 + row[e] * 4) >> (sh + kTiles * r8 / 32 * 8)) & 255u;
           }
@@ -476,7 +486,7 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
                 }
             }
         }
-        if (EDGE && found) sched.bad_v = 1;
+        if (EDGE && found) atomicOr(&sched.bad_v, 1);
       };
 
       // ---- the steps
@@ -504,6 +514,11 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
         fill = fill + 1 == Rg::kStages ? 0 : fill + 1;
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
+      if constexpr (QUANT) {                  // such a key makes every row NaN, such a value a dim of every row
+        if (__any_sync(full, any_nan_byte(odd_k))) l0 = l1 = __int_as_float(0x7fffffff);
+        if (any_nan_byte(odd_v)) atomicOr(&sched.bad_v, 2);
+        __syncwarp();
+      }
       // ---- results: l of a row over the lanes that share it
 #pragma unroll
       for (int x = QUANT ? 4 : 1; x < (QUANT ? 32 : 4); x *= 2) {
@@ -548,7 +563,7 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
       // The lane's dims come in runs of kTiles: over the 8-bit cache one run, kTiles r8 on, of both its rows; else
       // two, of columns 2 c4 and 2 c4 + 1 of the products.
       if (my_part == 0) {
-        const bool fix = *reinterpret_cast<volatile int*>(&sched.bad_v) != 0;
+        const int fix = *reinterpret_cast<volatile int*>(&sched.bad_v);
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           const int row = hf ? row1 : row0;
@@ -581,9 +596,9 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
               for (int j = 0; j < kTiles; j += 4)
                 *reinterpret_cast<float4*>(part + d0 + j) = make_float4(val(j), val(j + 1), val(j + 2), val(j + 3));
             }
-            if (fix) {                        // values that were not finite and that this row does see
+            if (fix) {                        // values that are not finite and that this row does see
 #pragma unroll 1
-              for (int t = max(S - A + 1, begin); t <= min(S - A + jq, end - 1); ++t) {
+              for (int t = (fix & 2) ? begin : max(S - A + 1, begin); t <= min(S - A + jq, end - 1); ++t) {
                 const int lb = block_of(t), ph = lb < a.MB ? table[lb] : -1;
                 if (ph < 0 || ph >= a.NB) continue;
                 const char* p = kv + to_values + int64_t(ph) * stride_b + int64_t(t - lb * a.BS) * stride_s;

@@ -1148,21 +1148,23 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
       uint8_t* dst = smem + Ly::kKvOff + ring.slot * Ly::kTileBytes + (row0 >> 3) * Ly::kGroupBytes;
       // Rolled, 8 tokens at a time: the warps of a scheduler are at five places of the kernel, and straight code
       // for all 16 tokens starved it of instructions.
-      if (plain && !edge) {
+      bool slow = edge || !plain;
+      if (!slow) {
+        uint32_t seen = 0;
 #pragma unroll 1
         for (int g8 = 0; g8 < 2; ++g8) {
 #pragma unroll
           for (int i = 0; i < 8 / kRpi; ++i) {
-            const uint4 x = *reinterpret_cast<const uint4*>(src + get[i]);
+            const uint4 x = *reinterpret_cast<const uint4*>(src + g8 * 8 * D + get[i]);
             const uint32_t b = __byte_perm(__shfl_sync(full, sc, g8 * 8 + i * kRpi + lr), 0u, 0x4440 | (lc >> 1));
             uint32_t r[8];
-            widen16<BF16>(x, plain_factor<BF16>(b), r);
-            put(dst + put0[i], dst + put1[i], r);
+            widen16<BF16>(x, plain_factor<BF16>(b), r, seen);
+            put(dst + g8 * Ly::kGroupBytes + put0[i], dst + g8 * Ly::kGroupBytes + put1[i], r);
           }
-          src += 8 * D;
-          dst += Ly::kGroupBytes;
         }
-      } else {
+        slow = __any_sync(full, any_nan_byte(seen));
+      }
+      if (slow) {
 #pragma unroll 1
         for (int i = 0; i < 16 / kRpi; ++i) {
           const int row = i * kRpi + lr, g8 = i * kRpi / 8;     // of the warp's 16
@@ -1170,11 +1172,15 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
           uint4 x = *reinterpret_cast<const uint4*>(src + g8 * 8 * D + (odd ? get[8 / kRpi - 1] : get[0]));
           if (gone >> row & 1u) x = make_uint4(0u, 0u, 0u, 0u);
           const uint32_t b = __byte_perm(__shfl_sync(full, sc, row), 0u, 0x4440 | (lc >> 1));
-          uint32_t r[8], f[3];
+          uint32_t r[8], f[3], seen = 0;
           any_factors<BF16>(b, f);
-          widen16<BF16>(x, f[0], r);
+          widen16<BF16>(x, f[0], r, seen);
+          const uint32_t in4[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-          for (int k = 0; k < 8; ++k) r[k] = mul_rest<BF16>(r[k], f[1], f[2]);
+          for (int k = 0; k < 8; ++k) {
+            const uint32_t m = __byte_perm(in4[k >> 1] & 0x7f7f7f7fu, 0u, (k & 1) ? 0x4342 : 0x4140);
+            r[k] = put_nan(mul_rest<BF16>(r[k], f[1], f[2]), m);
+          }
           if (plane && first + row >= u.hidden) {   // some row does not see it: what is not finite goes in as 0
             bool found = false;
 #pragma unroll

@@ -249,3 +249,35 @@ def test_hidden_values_past_the_range_of_an_8_bit_cache(d, lens, new, path):
     want[see:, q, dim], want[see:, q, dim + 1] = torch.inf, -torch.inf
     assert torch.equal(got[0], want)
     assert_device_clean(dev)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("new, path", [(1, "auto"), (3, "auto"), (90, "auto"), (200, "auto"), (3, "simt")])
+@pytest.mark.parametrize("lens", [500, 6000])
+@pytest.mark.parametrize("d", [64, 128])
+def test_nan_among_e4m3_bytes_is_attended_as_it_is_read_back(d, lens, new, path, dtype):
+    """Bytes 0x7f and 0xff read back as NaN: a value makes its dim of every row that sees it NaN, a key every dim
+    and the lse, of its head's queries and of no others, wherever the token lies: among the first tokens, in the
+    middle (all rows see it) and among the new ones (some do)."""
+    dev = need_gpu()
+    case = Case([lens, 40], [new, 1], 8, 4, d, 16, dtype, seed=28, quant=True)
+    clean = case.run(dev, path=path)
+    head, dim = 2, 37
+    q, others = slice(2 * head, 2 * head + 2), [0, 1, 2, 3, 6, 7]
+    rows = case.cache.clone()
+    for tok in sorted({0, lens // 2 + 3, lens - new + new // 2}):
+        at = int(C.slots(case.table, 0, tok, tok + 1, 16))
+        see = max(0, tok - (lens - new))
+        for plane, byte in ((1, 0x7f), (1, 0xff), (0, 0x7f), (0, 0xff)):
+            case.cache = rows.clone()
+            case.cache[plane, at, head * d + dim] = byte
+            out, lse = case.run(dev, path=path)
+            assert torch.equal(out[:, others], clean[0][:, others]) and torch.equal(lse[:, others], clean[1][:, others])
+            assert _equal((out[:see], lse[:see]), [x[:see] for x in clean]) and _equal((out[new:], lse[new:]), [x[new:] for x in clean])
+            if plane == 0:
+                assert torch.isnan(out[see:new, q]).all() and torch.isnan(lse[see:new, q]).all()
+            else:
+                assert torch.isnan(out[see:new, q, dim]).all() and torch.equal(lse, clean[1])
+                rest = [x for x in range(d) if x != dim]
+                assert torch.equal(out[:, q][..., rest], clean[0][:, q][..., rest])
+    assert_device_clean(dev)
