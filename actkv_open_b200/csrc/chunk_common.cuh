@@ -21,6 +21,10 @@ constexpr int kFewParts = 8 * kFewRows;     // rows of its units: up to 8 heads
 // single tokens of head size 64: 157, 153, 157)
 constexpr int kUnitCost = 4;                // a unit's fixed cost (queries in, results out) in key tiles
 constexpr float kSlack = 8.0f;              // log2 units the maximum may outgrow m by
+// p is multiplied by this, exactly, before it is rounded to 16 bits, and O / l divided by it: p is at most 2^8, and fp16
+// then holds what is 2^-32 of the maximum's (of 2^-24 at least, it lost the tail of a dominant token: thousands of
+// others of 2^-25 each).  bf16 has the range of 32 bits.
+template <bool BF16> constexpr float kPScale = BF16 ? 1.0f : 128.0f;
 constexpr int kMaxD = 128;
 
 // ------------------------------------------------------------------------------------ shares of work
@@ -160,6 +164,20 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+
+// Two probabilities.
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack_p(float lo, float hi) {
+  if constexpr (BF16) return pack2<true>(lo, hi);
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %2};\n\t"
+      "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(lo), "+f"(hi)
+      : "f"(kPScale<BF16>));
+  return pack2<BF16>(lo, hi);
+}
+// What O is multiplied by for the output, from l.
+template <bool BF16>
+__device__ __forceinline__ float over(float l) { return l == 0.0f ? 0.0f : 1.0f / (l * kPScale<BF16>); }
 
 // 16 e4m3 values with scale byte b as 16-bit values.  The four exponent and three mantissa bits of a
 // byte, moved under the wider type's exponent, read as the value times 2^-120 (bf16) or 2^-8 (fp16),

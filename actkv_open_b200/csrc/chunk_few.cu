@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
           l0 += x + z;
           l1 += y + w;
           // p^T as the second operand: row r8, tokens 2 c4, 2 c4 + 1 and those + 8
-          const uint32_t p0 = transpose8x8(pack2<BF16>(x, y)), p1 = transpose8x8(pack2<BF16>(z, w));
+          const uint32_t p0 = transpose8x8(pack_p<BF16>(x, y)), p1 = transpose8x8(pack_p<BF16>(z, w));
           // ---- O^T += V^T p^T: values of tokens 2 c4, 2 c4 + 1 and those + 8, dims kTiles r8 ..
           uint32_t vw[4][kTiles / 4], b[4];
 #pragma unroll
@@ -453,11 +453,11 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
           for (int n = 0; n < 2; ++n) {
             const float x = ex2(fmaf(s[n][0], c2, -b0)), y = ex2(fmaf(s[n][1], c2, -b0));
             l0 += x + y;
-            p[2 * n] = pack2<BF16>(x, y);
+            p[2 * n] = pack_p<BF16>(x, y);
             if (wide) {
               const float z = ex2(fmaf(s[n][2], c2, -b1)), w = ex2(fmaf(s[n][3], c2, -b1));
               l1 += z + w;
-              p[2 * n + 1] = pack2<BF16>(z, w);
+              p[2 * n + 1] = pack_p<BF16>(z, w);
             }
           }
           // ---- values: tokens 2 c4, 2 c4 + 1 and those + 8, dims kTiles r8 ..
@@ -568,7 +568,7 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
         for (int hf = 0; hf < 2; ++hf) {
           const int row = hf ? row1 : row0;
           if (row >= rows) continue;
-          const float L = hf ? l1 : l0, M = hf ? m1 : m0, inv = L == 0.0f ? 0.0f : 1.0f / L;
+          const float L = hf ? l1 : l0, M = hf ? m1 : m0, inv = over<BF16>(L);
           const int jq = row / a.G, hq = h * a.G + row - jq * a.G, hr = my_head * rows + row;
           const int64_t qt = int64_t(a0) + jq;
           uint16_t* dst = static_cast<uint16_t*>(a.out) + qt * a.out_stride_t + int64_t(hq) * a.out_stride_h;

@@ -7,7 +7,8 @@
 // near it: it is raised (and O and l rescaled) when the maximum has grown by more than 2^8, so p
 // stays below 2^8 and the rescaling, a pass over O, is rare.  S = Q K^T and O are accumulated in 32
 // bits in TMEM, m and l are 32-bit registers; p is rounded to the cache's 16-bit type for the second
-// product only (l sums the unrounded values), the same half unit that the output is rounded by.
+// product only (l sums the unrounded values), the same half unit that the output is rounded by (fp16 p, held times
+// 2^7: or 2^-32 of the largest, when that is more).  32 bits tell logits apart up to about 2^24.
 //
 // Work.  A unit is (session, KV head, group of up to 256 query rows): rows are (token, head of the
 // GQA group), two tiles of 128.  The units' key tiles of 128 tokens, laid end to end with a fixed
@@ -905,7 +906,7 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
               const float2 e = fma2(make_float2(x[at + 2 * k], x[at + 2 * k + 1]), c2v, offv);
               const float2 p = make_float2(ex2(e.x), ex2(e.y));
               sum[k & 1] = add2(sum[k & 1], p);
-              u[k] = pack2<BF16>(p.x, p.y);
+              u[k] = pack_p<BF16>(p.x, p.y);
             }
           };
           // p of 32 tokens at a time; the second product starts on the first 64
@@ -987,7 +988,7 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
         const bool put = mine && j < x.A;
         const int hq = x.h * a.G + g;
         const int64_t qt = int64_t(x.a0) + j;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = over<BF16>(l);
         const int pr = (two ? w * kRows : 0) + row;
         const Parts ps = wide_parts(a.workspace, n_cta);
         const int ps_slot = x.t0 > 0 ? 0 : 1;
@@ -1275,7 +1276,7 @@ __global__ void __launch_bounds__(kJoinThreads) chunk_combine_kernel(const __gri
       place(i, pr, qt, hq);
       add_parts(pr, cta, 1);
       uint16_t* dst = static_cast<uint16_t*>(a.out) + qt * a.out_stride_t + int64_t(hq) * a.out_stride_h;
-      const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+      const float inv = over<BF16>(L);
 #pragma unroll
       for (int k = 0; k < kPer; ++k) dst[k * 32 + lane] = uint16_t(pack2<BF16>(o[k] * inv, 0.0f));
       if (lane == 0) a.lse[qt * a.lse_stride_t + hq] = lse_of(M, L);
@@ -1304,7 +1305,7 @@ __global__ void __launch_bounds__(kJoinThreads) chunk_combine_kernel(const __gri
         y = fmaf(sh_o[w][threadIdx.x], al, y);
       }
       static_cast<uint16_t*>(a.out)[qt * a.out_stride_t + int64_t(hq) * a.out_stride_h + threadIdx.x] =
-          uint16_t(pack2<BF16>(l == 0.0f ? 0.0f : y / l, 0.0f));
+          uint16_t(pack2<BF16>(l == 0.0f ? 0.0f : y / (l * kPScale<BF16>), 0.0f));
       if (threadIdx.x == 0) a.lse[qt * a.lse_stride_t + hq] = lse_of(m, l);
     }
     __syncthreads();

@@ -281,3 +281,28 @@ def test_nan_among_e4m3_bytes_is_attended_as_it_is_read_back(d, lens, new, path,
                 rest = [x for x in range(d) if x != dim]
                 assert torch.equal(out[:, q][..., rest], clean[0][:, q][..., rest])
     assert_device_clean(dev)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("new", [1, 3, 90, 200])
+def test_fp16_keeps_what_a_dominant_token_leaves(new, quant):
+    """One token 17.4 above all others (an attention sink), with a zero value: the output is what 2000 others of
+    p = e^-17.4 = 2^-25.1 add up to, half of fp16's smallest number each.  p is held in fp16 times 2^7 at least, so it
+    errs by u of itself or 2^-25 / 2^7 = 2^-32 absolutely: |out - ref| <= (2 u + 1e-4) A + S 2^-32 max|v|, and the output's own
+    subnormals err by 2^-25."""
+    dev = need_gpu()
+    s = 2000
+    case = Case([s], [new], 4, 2, 128, 16, HF, seed=29, quant=quant)
+    case.q.zero_()
+    case.q[..., 0] = 17.4 / 18
+    k, v = torch.zeros(s, 2, 128, dtype=HF), torch.ones(s, 2, 128, dtype=HF)
+    k[0, :, 0], v[0] = 18, 0                             # 18 is exact in e4m3 too
+    at = C.slots(case.table, 0, 0, s, 16)
+    for p, x in enumerate((k, v)):
+        case.cache[p, at] = C.pack_rows(x, case.row) if quant else x
+    out, lse = (x.cpu().double() for x in case.run(dev, scale=1.0))
+    want, want_l, mag, size = case.ref(1.0)
+    assert (want < 1e-4).all() and (want > 2e-5).all()
+    assert ((out - want).abs() <= (2 * U[HF] + 1e-4) * mag + s * 2.0 ** -32 + 2.0 ** -25).all()
+    assert ((lse - want_l).abs() <= 2e-5 + 8e-6 * size).all()
+    assert_device_clean(dev)
