@@ -164,8 +164,9 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def stream_ptr(device) -> int:
-    """The current stream's handle on ``device`` (without building a Stream object where torch can)."""
-    if _raw_stream is not None and device.index is not None:
+    """The current stream's handle on ``device``, a torch.device, string or index (without building a Stream object
+    where torch can)."""
+    if _raw_stream is not None and isinstance(device, torch.device) and device.index is not None:
         return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
