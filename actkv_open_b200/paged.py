@@ -159,6 +159,8 @@ class PagedKVCache:
         off = [0]
         for n in n_new:
             off.append(off[-1] + int(n))
+        assert len(n_new) == len(reqs) and min(n_new, default=0) >= 0 and off[-1] == q.shape[0], \
+            "n_new counts each request's rows of q"
         return paged_chunk_attention(q, self._to_device(torch.tensor(off, dtype=torch.int32)), self.kv[layer],
                                      self.block_table(reqs), self.seq_tensor(reqs), scale)
 
