@@ -242,6 +242,7 @@ class QuantPagedCache(DevicePagedCache):
             for x in n_new:
                 offs.append(offs[-1] + int(x))
             R = len(offs) - 1
+            assert k_new.shape[1] >= offs[-1], f"{offs[-1]} new tokens, {k_new.shape[1]} rows of k_new"
             if R <= self.max_sessions:
                 off = self._upload(offs)
         if R > self.max_sessions:

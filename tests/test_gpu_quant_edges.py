@@ -29,3 +29,20 @@ def test_rows_before_the_first_offset_are_no_sessions():
     dequantize_read(full, 2, 64, off[1:].to(dev), table[1:].to(dev), seqs[1:], 53, k_out=out, planes="k")
     assert (out[:, :33] == 3).all() and torch.equal(out[:, 33:].cpu(), C.quantise_ref(k)[0].to(BF)[:, 33:])
     assert_device_clean(dev)
+
+
+def test_append_refuses_fewer_rows_than_new_tokens():
+    """The counts are on the host: nothing is appended, where lengths would grow over rows that were never written."""
+    dev = need_gpu()
+    from actkv_open_b200.engine import QuantPagedCache
+    c = QuantPagedCache(16, 16, 2, 64, 2, 2, 64, device=dev)
+    c.set_state([[], []], [0, 0], list(range(16)))
+    k = torch.ones(2, 20, 2, 64, dtype=BF, device=dev)
+    c.append(k, k, [12, 8])
+    state = c.state()
+    with pytest.raises(AssertionError, match="rows"):
+        c.append(k, k, [12, 9])
+    assert c.state() == state
+    c.append(k, k, [2, 3])                                # rows past the last count are no session's
+    assert c.state()[1] == [14, 11]
+    assert_device_clean(dev)
