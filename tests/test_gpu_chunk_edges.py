@@ -306,3 +306,130 @@ def test_fp16_keeps_what_a_dominant_token_leaves(new, quant):
     assert ((out - want).abs() <= (2 * U[HF] + 1e-4) * mag + s * 2.0 ** -32 + 2.0 ** -25).all()
     assert ((lse - want_l).abs() <= 2e-5 + 8e-6 * size).all()
     assert_device_clean(dev)
+
+
+# ---------------------------------------------------------------- the kernel for few rows, and both kernels in one call
+
+FEW = {   # lens, new, hq, hkv, block size: at most 16 rows (token x head of the group) per KV head; 8 over the 8-bit cache
+    "one row": ([700, 129, 128, 127, 1, 2000, 40], [1] * 7, 8, 8, 16),
+    "four of two": ([700, 129, 128, 127, 1, 2000, 0], [4, 1, 3, 2, 4, 4, 1], 8, 4, 16),
+    "two of four": ([700, 17, 16, 15, 3000, 2], [2, 1, 2, 0, 2, 2], 32, 8, 32),
+    "two of three": ([333, 64, 1000], [2, 1, 2], 6, 2, 8),
+    "eight of one": ([500, 8, 3, 1200], [8, 8, 8, 5], 3, 3, 64),
+    "one of five, one KV head": ([900, 33], [1, 1], 5, 1, 16),
+    "one of eight": ([900, 33, 2500], [1, 1, 1], 32, 4, 128),
+}
+FEW16 = {
+    "four of four": ([700, 129, 128, 4, 3000, 2], [4, 3, 4, 4, 4, 4], 32, 8, 16),
+    "sixteen of one": ([500, 16, 3, 1200], [16, 9, 16, 13], 2, 2, 16),
+    "five of three": ([333, 64, 1000], [5, 4, 3], 12, 4, 32),
+    "one of sixteen": ([900, 33, 2500], [1, 1, 1], 32, 2, 16),
+    "two of eight": ([900, 33, 1], [2, 1, 2], 16, 2, 8),
+}
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("name, quant", [(n, q) for n in FEW for q in (False, True)] + [(n, False) for n in FEW16])
+def test_sessions_of_a_few_rows_match_64_bits(name, quant, d, dtype):
+    dev = need_gpu()
+    lens, new, hq, hkv, bs = {**FEW, **FEW16}[name]
+    case = Case(lens, new, hq, hkv, d, bs, dtype, seed=30 + len(name), quant=quant)
+    case.check(case.run(dev))
+    assert_device_clean(dev)
+
+
+@pytest.mark.parametrize("quant, d, dtype, n_short, s_short", [(True, 128, BF, 17, 3200), (True, 64, HF, 9, 11000),
+                                                              (False, 128, HF, 8, 27001), (False, 64, BF, 70, 5600)])
+def test_both_kernels_in_one_call(quant, d, dtype, n_short, s_short):
+    """Short sessions of 64 MB of 8-bit rows (512 MB of 16-bit ones) and more beside longer ones: the two tensor-core
+    kernels share the call, each skips the other's sessions, and both leave units cut between CTAs to the join."""
+    dev = need_gpu()
+    from actkv_open_b200.kernels.chunk_attn import paged_chunk_attention
+    from actkv_open_b200.kernels.quant_cache import (dequantize_read, paged_chunk_attention_quant, quant_row_bytes,
+                                                     quantize_write)
+    hq, hkv, bs = 32, 8, 16
+    lens = [s_short + 7 * i for i in range(n_short)]
+    new = [i % 3 for i in range(n_short)]
+    for at, s, a in ((0, 1500, 300), (3, 6000, 70), (len(lens), 40, 40), (len(lens) - 1, 5, 130)):
+        lens.insert(at, s)
+        new.insert(at, a)
+    short = sum(s for s, a in zip(lens, new) if 0 < a <= 2)
+    assert short * hkv * d * 2 * (1 if quant else 2) >= (64 if quant else 512) << 20
+    gen = torch.Generator(device=dev).manual_seed(31)
+    table, nb = C.pages(lens, bs, torch.Generator().manual_seed(31))
+    off = C.offsets(new)
+    table, seq, q_off = table.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev), off.to(dev)
+    q = torch.randn(int(off[-1]), hq, d, generator=gen, device=dev).to(dtype)
+    n = sum(lens)
+    k, v = (torch.randn(1, n, hkv, d, generator=gen, device=dev).to(dtype) for _ in range(2))
+    tok_off = C.offsets(lens).to(dev)
+    if quant:
+        rows = torch.full((1, 2, nb, bs, quant_row_bytes(hkv, d)), 255, dtype=torch.uint8, device=dev)
+        quantize_write(k, v, tok_off, rows, table, seq)
+        k, v = dequantize_read(rows, hkv, d, tok_off, table, seq, n, dtype=dtype)
+        call = lambda: paged_chunk_attention_quant(q, q_off, rows[0], hkv, table, seq)                 # noqa: E731
+    else:
+        kv = torch.full((2, nb, bs, hkv, d), float("nan"), dtype=dtype, device=dev)
+        for r, s in enumerate(lens):
+            pos = torch.arange(s, device=dev)
+            slot = table[r].long()[pos // bs] * bs + pos % bs
+            for p, x in enumerate((k, v)):
+                kv[p].view(nb * bs, hkv, d)[slot] = x[0, int(tok_off[r]):int(tok_off[r]) + s]
+        call = lambda: paged_chunk_attention(q, q_off, kv, table, seq)                                 # noqa: E731
+    out, lse = call()
+    g = hq // hkv
+    for r, (s, a) in enumerate(zip(lens, new)):
+        if a == 0:
+            continue
+        o0, o1, t0 = int(off[r]), int(off[r + 1]), int(tok_off[r])
+        kk, vv = (x[0, t0:t0 + s].double() for x in (k, v))
+        qq = q[o0:o1].double().view(a, hkv, g, d)
+        hide = torch.arange(s, device=dev)[None] > torch.arange(s - a, s, device=dev)[:, None]
+        x = (torch.einsum("ahgd,shd->ahgs", qq, kk) * d ** -0.5).masked_fill(hide[:, None, None], -torch.inf)
+        one = torch.logsumexp(x, -1)
+        p = torch.where(torch.isfinite(one)[..., None], torch.exp(x - one[..., None]), torch.zeros_like(x))
+        want, mag = (torch.einsum("ahgs,shd->ahgd", p, y).reshape(a, hq, d) for y in (vv, vv.abs()))
+        size = (torch.einsum("ahgd,shd->ahgs", qq.abs(), kk.abs()).amax(-1) * d ** -0.5).view(a, hq)
+        one = one.view(a, hq)
+        tol = (2 * U[dtype] + 1e-4) * mag + (s * 2.0 ** -25 * vv.abs().amax() if dtype == HF else 0.0)
+        assert ((out[o0:o1].double() - want).abs() <= tol).all(), r
+        none = one == -torch.inf
+        assert torch.equal(lse[o0:o1] == -torch.inf, none) and (out[o0:o1][none] == 0).all()
+        assert ((lse[o0:o1].double() - one).abs()[~none] <= (2e-5 + 8e-6 * size)[~none]).all(), r
+    for _ in range(3):
+        assert _equal((out, lse), call())
+    assert_device_clean(dev)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("lens", [500, 6000])
+@pytest.mark.parametrize("new, hq, d", [(1, 8, 128), (2, 16, 64), (4, 16, 128), (4, 8, 64), (90, 8, 128), (200, 8, 64)])
+def test_values_that_are_not_finite(new, hq, d, lens, dtype):
+    """inf, -inf and NaN in a value of 16-bit rows, and a NaN group (scale byte 255) of 8-bit ones, at a session's start,
+    in its middle and among its new tokens, in the kernels for few rows (up to 16, whole and cut between CTAs) and many:
+    in that dim of the rows that see the token, and nowhere else."""
+    dev = need_gpu()
+    for quant in (False, True):
+        case = Case([lens, 40], [new, 1], hq, 4, d, 16, dtype, seed=32, quant=quant)
+        clean = case.run(dev)
+        rows, head, dim, g = case.cache.clone(), 2, 37, hq // 4
+        q = torch.arange(head * g, head * g + g)
+        for tok in sorted({0, lens // 2 + 3, lens - new + new // 2, lens - 1}):
+            at, see = int(C.slots(case.table, 0, tok, tok + 1, 16)), max(0, tok - (lens - new))
+            for bad in ((float("inf"), -float("inf"), float("nan")) if not quant else (255,)):
+                case.cache = rows.clone()
+                dims = [dim] if not quant else list(range(32, 64))
+                if quant:
+                    case.cache[1, at, 4 * d + (head * d + 32) // 32] = 255
+                else:
+                    case.cache[1, at, head, dim] = bad
+                out, lse = case.run(dev)
+                assert torch.equal(lse, clean[1])
+                hit = out[see:new][:, q][..., dims]
+                assert torch.isnan(hit).all() if bad != bad or quant else (hit == bad).all()
+                want = clean[0].clone()
+                want[see:new, q[:, None], torch.tensor(dims)[None]] = hit
+                assert torch.equal(torch.nan_to_num(out, nan=77.0), torch.nan_to_num(want, nan=77.0))
+                assert torch.equal(torch.isnan(out), torch.isnan(want))
+    assert_device_clean(dev)
