@@ -675,36 +675,96 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
       ok = wait(B_QF, q_uses & 1u);
       if (!ok) break;
       ++q_uses;
-      // Step by step: the second product of step s, then the logits of step s + 2 of the same stream.  Two row
-      // tiles take every key tile in a step each; one row tile takes a key tile per step.
-      const int steps = two ? 2 * nt : nt;
-      Ring v, k;
+      // Either in steps: the second product of step s, then the logits of step s + 2 of the same stream, two row tiles
+      // taking every key tile in a step each and one row tile a key tile per step.  Or the same order written out, with
+      // streams and tiles known to the compiler, which issues sooner but is longer code.  2048 tokens over 32768: 1120
+      // us in steps, 1063 written out; 1088 over 2000 to 10000 623 and 601; head size 64, fp16, 171 and 174; 8-bit
+      // rows, whose five roles crowd the instruction cache, only lose by longer code.
+      if constexpr (QUANT || D == 64) {
+        const int steps = two ? 2 * nt : nt;
+        Ring v, k;
 #pragma unroll 1
-      for (int s = -2; s < steps; ++s) {
-        const int w = s & 1;
-        const bool opens = !two || w == 0, closes = !two || w == 1, more = s + 2 < steps;
-        if (s >= 0) {
-          if (opens) {
-            v = ring;
-            ring.next(kSlots);
-            ok = kv_wait(v);
+        for (int s = -2; s < steps; ++s) {
+          const int w = s & 1;
+          const bool opens = !two || w == 0, closes = !two || w == 1, more = s + 2 < steps;
+          if (s >= 0) {
+            if (opens) {
+              v = ring;
+              ring.next(kSlots);
+              ok = kv_wait(v);
+            }
+            ok = ok && issue_o(w, v.slot, s < 2);
+            if (!ok) break;
+            if (closes) commit(B_KVE + v.slot);
           }
-          ok = ok && issue_o(w, v.slot, s < 2);
-          if (!ok) break;
-          if (closes) commit(B_KVE + v.slot);
+          if (more) {
+            if (opens) {
+              k = ring;
+              ring.next(kSlots);
+              ok = kv_wait(k);
+              if (!ok) break;
+            }
+            issue_s(w, two ? w : 0, k.slot);
+            if (closes) commit(B_KVE + k.slot);
+            if (s + 3 == steps) commit(B_QE);
+          } else if (s >= 0) {
+            finish_o(w);
+          }
         }
-        if (more) {
-          if (opens) {
-            k = ring;
-            ring.next(kSlots);
+      } else if (two) {
+        ok = kv_wait(ring);
+        if (!ok) break;
+        issue_s(0, 0, ring.slot);
+        issue_s(1, 1, ring.slot);
+        commit(B_KVE + ring.slot);
+        ring.next(kSlots);
+        if (nt == 1) commit(B_QE);
+#pragma unroll 1
+        for (int i = 0; i < nt; ++i) {
+          const Ring v = ring;
+          ring.next(kSlots);
+          const Ring k = ring;
+          const bool more = i + 1 < nt;
+          if (more) ring.next(kSlots);
+          ok = kv_wait(v) && issue_o(0, v.slot, i == 0);
+          if (!ok) break;
+          if (more) {
             ok = kv_wait(k);
             if (!ok) break;
+            issue_s(0, 0, k.slot);
+          } else {
+            finish_o(0);
           }
-          issue_s(w, two ? w : 0, k.slot);
-          if (closes) commit(B_KVE + k.slot);
-          if (s + 3 == steps) commit(B_QE);
-        } else if (s >= 0) {
-          finish_o(w);
+          ok = issue_o(1, v.slot, i == 0);
+          if (!ok) break;
+          commit(B_KVE + v.slot);
+          if (more) {
+            issue_s(1, 1, k.slot);
+            commit(B_KVE + k.slot);
+            if (i + 2 == nt) commit(B_QE);
+          } else {
+            finish_o(1);
+          }
+        }
+      } else {
+        // ring order: keys 0, 1, then values t and keys t + 2 in turn
+        auto key = [&](int t) -> bool {
+          if (!kv_wait(ring)) return false;
+          issue_s(t & 1, 0, ring.slot);
+          commit(B_KVE + ring.slot);
+          ring.next(kSlots);
+          if (t + 1 == nt) commit(B_QE);
+          return true;
+        };
+        ok = key(0) && (nt == 1 || key(1));
+#pragma unroll 1
+        for (int t = 0; ok && t < nt; ++t) {
+          ok = kv_wait(ring) && issue_o(t & 1, ring.slot, t < 2);
+          if (!ok) break;
+          commit(B_KVE + ring.slot);
+          ring.next(kSlots);
+          if (t + 2 < nt) ok = key(t + 2);
+          else finish_o(t & 1);
         }
       }
     }
