@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
   if (few_rows == 0) return;
   share_out<kThreads>(a.R, [&](int r) -> int64_t {
     const int A = new_tokens(a, r);
-    return A > 0 && A * a.G <= few_rows ? int64_t(a.Hkv / HG) * (kRoundCost + (a.seq_used[r] + round - 1) / round) : 0;
+    return A > 0 && A * a.G <= few_rows ? int64_t(a.Hkv / HG) * (kRoundCost + (max(a.seq_used[r], 0) + round - 1) / round) : 0;
   }, sched.share, sched.scan, cta, n_cta, kMinRounds);
   const int64_t total = sched.share.total;
   const int n_used = used_ctas(total, n_cta, kMinRounds);

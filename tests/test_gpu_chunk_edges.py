@@ -433,3 +433,20 @@ def test_values_that_are_not_finite(new, hq, d, lens, dtype):
                 assert torch.equal(torch.nan_to_num(out, nan=77.0), torch.nan_to_num(want, nan=77.0))
                 assert torch.equal(torch.isnan(out), torch.isnan(want))
     assert_device_clean(dev)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("new", [1, 90])
+def test_a_negative_length_is_an_empty_session(new, quant):
+    """Its queries see nothing; the sessions beside it are as without it."""
+    dev = need_gpu()
+    case = Case([300, 40, 700], [new, 2, new], 8, 4, 128, 16, BF, seed=33, quant=quant)
+    x = case.device(dev)
+    want = case.run(dev, given={**x, "seq": torch.tensor([300, 0, 700], dtype=torch.int32, device=dev)})
+    for path in ("auto", "simt"):
+        base = want if path == "auto" else case.run(dev, given={**x, "seq": torch.tensor([300, 0, 700], dtype=torch.int32, device=dev)}, path=path)
+        for bad in (-1, -100000, -(1 << 31) + 1000):
+            got = case.run(dev, given={**x, "seq": torch.tensor([300, bad, 700], dtype=torch.int32, device=dev)}, path=path)
+            assert _equal(base, got)
+            assert (got[0][new:new + 2] == 0).all() and (got[1][new:new + 2] == -torch.inf).all()
+    assert_device_clean(dev)
