@@ -43,6 +43,14 @@ __device__ __forceinline__ int new_tokens(const ChunkArgs& a, int r) {
   return 0;
 }
 
+// Tokens that a table has a place for (short of where 32-bit token arithmetic would end): what the kernels walk of a
+// session.  A longer one is flagged, and the rest of it hidden like any token of a block outside the cache.
+__device__ __forceinline__ int table_room(const ChunkArgs& a) { return int(min(int64_t(a.MB) * a.BS, int64_t(0x7fffff00))); }
+__device__ __forceinline__ int held_tokens(const ChunkArgs& a, int S) { return min(max(S, 0), table_room(a)); }
+__device__ __forceinline__ void flag_long(const ChunkArgs& a, int S) {
+  if (S > table_room(a)) flag(a.status, ACTKV_DEV_BAD_INDEX);
+}
+
 // Query rows per KV head up to which chunk_few_kernel takes a session in this call, 0 when chunk_umma_kernel takes
 // all.  The two kernels run one after the other, so short work is not split between them: where the other kernel
 // has sessions too, those of few rows go to their own only when they hold bytes enough to win back a

@@ -163,8 +163,10 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
   const int few_rows = few_rows_now<kThreads>(a, sched.sums);
   if (few_rows == 0) return;
   share_out<kThreads>(a.R, [&](int r) -> int64_t {
-    const int A = new_tokens(a, r);
-    return A > 0 && A * a.G <= few_rows ? int64_t(a.Hkv / HG) * (kRoundCost + (max(a.seq_used[r], 0) + round - 1) / round) : 0;
+    const int A = new_tokens(a, r), S = a.seq_used[r];
+    if (A == 0 || A * a.G > few_rows) return 0;
+    flag_long(a, S);
+    return int64_t(a.Hkv / HG) * (kRoundCost + (held_tokens(a, S) + round - 1) / round);
   }, sched.share, sched.scan, cta, n_cta, kMinRounds);
   const int64_t total = sched.share.total;
   const int n_used = used_ctas(total, n_cta, kMinRounds);
@@ -185,7 +187,7 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
     const int a0 = a.q_off[r], A = new_tokens(a, r), S = a.seq_used[r];
     if (A == 0 || A * a.G > few_rows) continue;
     const int rows = A * a.G;
-    const int nt = S > 0 ? (S + round - 1) / round : 0;
+    const int nt = (held_tokens(a, S) + round - 1) / round;
     const int64_t weight = kRoundCost + nt;
     if (seek) {                               // the group that holds lo
       hg = int((lo - at) / weight);
@@ -198,7 +200,7 @@ __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(
       const int t0 = int(lo > first ? lo - first : 0), t1 = nt == 0 ? 0 : int(min(int64_t(nt), hi - first));
       if (nt == 0 ? at < lo : t0 >= t1) continue;
       const int h = hg * HG + my_head;
-      const int begin = t0 * round, end = min(t1 * round, S);
+      const int begin = t0 * round, end = min(t1 * round, held_tokens(a, S));
       const int start = begin + my_part * kStep;              // this warp's steps: start, start + round, ...
       const int mine = start < end ? (end - start + round - 1) / round : 0;
       // the lane's two query rows, and the last tokens they see

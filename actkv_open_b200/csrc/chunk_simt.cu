@@ -51,7 +51,10 @@ __global__ void __launch_bounds__(kWarps * 32) chunk_simt_kernel(ChunkArgs a) {
     return;
   }
   const int S = a.seq_used[r];
-  const int seen = S - (a.q_off[r + 1] - t) + 1;            // tokens this query sees
+  const int64_t room = int64_t(a.MB) * a.BS;                // of the table: what is past it is hidden
+  const int64_t sees = int64_t(S) - (a.q_off[r + 1] - t) + 1;
+  if (S > room && threadIdx.x == 0) flag(a.status, ACTKV_DEV_BAD_INDEX);
+  const int seen = int(min(max(sees, int64_t(0)), room));   // tokens this query sees
   const int h = hq / a.G;
   float q[kMaxPer], o[kMaxPer];
   const T* qp = static_cast<const T*>(a.q) + int64_t(t) * a.q_stride_t + int64_t(hq) * a.q_stride_h;
@@ -65,7 +68,7 @@ __global__ void __launch_bounds__(kWarps * 32) chunk_simt_kernel(ChunkArgs a) {
   const float c2 = a.scale * kLog2e;
   for (int p = warp; p < seen; p += kWarps) {
     const int lb = p / a.BS;
-    const int phys = lb < a.MB ? a.block_table[r * a.bt_stride_r + lb] : -1;
+    const int phys = a.block_table[r * a.bt_stride_r + lb];
     if (phys < 0 || phys >= a.NB) {
       if (lane == 0) flag(a.status, ACTKV_DEV_BAD_INDEX);
       continue;

@@ -107,12 +107,13 @@ struct Sched {               // in shared memory
 static_assert(sizeof(Sched) <= kSchedBytes, "the schedule's place in shared memory");
 
 struct Geometry {
+  const ChunkArgs* a;
   int tpb;                   // tokens per row tile
-  __device__ explicit Geometry(const ChunkArgs& a) : tpb(kRows / a.G) {}
+  __device__ explicit Geometry(const ChunkArgs& args) : a(&args), tpb(kRows / args.G) {}
   __device__ int groups(int A) const { return (A + 2 * tpb - 1) / (2 * tpb); }
   // key tiles that some query of tokens [j0, j0 + n) sees
   __device__ int tiles(int S, int A, int j_end) const {
-    const int last = S - A + j_end - 1;
+    const int last = min(S - A + j_end, table_room(*a)) - 1;
     return last >= 0 ? last / kTile + 1 : 0;
   }
   __device__ int64_t head_weight(int S, int A) const {
@@ -200,7 +201,9 @@ __device__ void make_schedule(const ChunkArgs& a, Sched& s, int cta, int n) {
   if (threadIdx.x == 0) s.few_rows = few_rows;
   share_out<kThreads>(a.R, [&](int r) -> int64_t {
     const int A = new_tokens(a, r);
-    return A > 0 && A * a.G > few_rows ? a.Hkv * geo.head_weight(a.seq_used[r], A) : 0;
+    if (A == 0 || A * a.G <= few_rows) return 0;
+    flag_long(a, a.seq_used[r]);
+    return a.Hkv * geo.head_weight(a.seq_used[r], A);
   }, s.share, s.scan, cta, n, 1);
 }
 

@@ -450,3 +450,38 @@ def test_a_negative_length_is_an_empty_session(new, quant):
             assert _equal(base, got)
             assert (got[0][new:new + 2] == 0).all() and (got[1][new:new + 2] == -torch.inf).all()
     assert_device_clean(dev)
+
+
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("new", [1, 3, 90])
+@pytest.mark.parametrize("width", [3, 8])
+def test_lengths_past_the_table(width, new, quant):
+    """A length that its table has no place for, up to the largest there is: flagged, the tokens past the table are
+    hidden (and not walked, whatever the length), and the session beside it is as it should be."""
+    dev = need_gpu()
+    from actkv_open_b200 import _native as N
+    room = width * 16
+    case = Case([room, 120], [new, 2], 8, 4, 128, 16, BF, seed=34, quant=quant)
+    x = case.device(dev)
+    x["table"] = x["table"][:, :width].contiguous()
+    if width == 3:
+        case.lens[1] = 40
+        x["seq"][1] = 40
+    for length in (room + 1, 5000, 1 << 30, (1 << 31) - 1):
+        seq = x["seq"].clone()
+        seq[0] = length
+        first = [max(0, min(room, length - new + j + 1)) for j in range(new)]
+        refs = [t.double().repeat_interleave(2, 1) for t in (case.tokens(0, 0), case.tokens(1, 0))]
+        logit = torch.einsum("ahd,shd->ahs", case.q[:new].double(), refs[0]) * 128 ** -0.5
+        hide = torch.arange(room)[None] >= torch.tensor(first)[:, None]
+        logit = logit.masked_fill(hide[:, None], -torch.inf)
+        one = torch.logsumexp(logit, -1)
+        p = torch.where(torch.isfinite(one)[..., None], torch.exp(logit - one[..., None]), torch.zeros_like(logit))
+        out, lse, mag, size = case.ref()
+        out[:new], mag[:new] = (torch.einsum("ahs,shd->ahd", p, v) for v in (refs[1], refs[1].abs()))
+        lse[:new] = one
+        size[:new] = torch.einsum("ahd,shd->ahs", case.q[:new].double().abs(), refs[0].abs()).amax(-1) * 128 ** -0.5
+        for path in ("auto", "simt"):
+            _within(case.run(dev, given={**x, "seq": seq}, path=path), (out, lse, mag, size))
+            torch.cuda.synchronize()
+            assert N.read_device_status(dev) == N.DEV_BAD_INDEX
