@@ -54,9 +54,13 @@ __device__ __forceinline__ void flag_long(const ChunkArgs& a, int S) {
 // Query rows per KV head up to which chunk_few_kernel takes a session in this call, 0 when chunk_umma_kernel takes
 // all.  The two kernels run one after the other, so short work is not split between them: where the other kernel
 // has sessions too, those of few rows go to their own only when they hold bytes enough to win back a
-// kernel's start and end (about 15 us) by its higher rate: 512 MB of 16-bit rows (6.3 against 5.3 TB/s), 64 MB
-// of 8-bit ones (4.1 against 1.6 TB/s).  (16 sessions of 1000 to 9000 tokens with 3 to 7 new ones each, 4 query
-// heads per KV head, 330 MB: 120 us split, 80 us together.)
+// kernel's start and end (about 15 us) by its higher rate: 512 MB of 16-bit rows, 64 MB of 8-bit ones.  Single tokens
+// over 8192 (32 query heads over 8 of 128) beside one chunk, together and split, us:
+//                                   16-bit rows: 128 MB   256 MB    512 MB    1 GB      8-bit rows: 32 MB    64 MB     128 MB
+//   beside 512 new over 8192               139, 142  171, 160  226, 203  347, 283              142, 141  162, 149  198, 161
+//   beside 64 new over 2048                 79, 101  110, 122  158, 169  272, 246               61, 89    83, 94   123, 110
+// The more the chunk has to do the sooner splitting pays; the limits lie between the two.  (16 sessions of 1000 to 9000
+// tokens with 3 to 7 new ones each, 4 query heads per KV head, 330 MB: 120 us split, 82 us together.)
 // Every thread of the block calls it; `sums` is shared.
 template <int kThreads>
 __device__ __forceinline__ int few_rows_now(const ChunkArgs& a, int64_t (&sums)[2]) {

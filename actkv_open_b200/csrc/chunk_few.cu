@@ -19,8 +19,8 @@
 //     that of the second product without a move.  8 warps of 244 registers.
 //   8-bit rows: S^T = K Q^T and O^T = V^T P^T, tokens and dims as the products' rows and 8 query rows as
 //     their columns: half the products, and O^T takes half the registers, so that 16 warps of 127 hide
-//     the widening's latencies (8 warps 344 us, 16 warps 304 us, both before the
-//     widening was made shorter; the other way round 379 us); p^T is an
+//     the widening's latencies (the batch below: 8 warps 344 us, 16 warps 304 us, the other way round 379 us, all before
+//     the widening was made shorter); p^T is an
 //     8 x 8 transpose per 8 tokens.
 //
 // Work is shared out as in chunk_umma.cu, in equal shares per CTA.  A unit is a session and a group of 8 (4, 2, 1:
@@ -30,9 +30,9 @@
 // turn and join through shared memory.
 //
 // Measured: 32 single-token sessions of 4096 to 32768 tokens, 32 query heads over 8 KV heads of 128: 16-bit
-// rows (2.4 GB) 379 us, 6.4 TB/s, 0.97 of the measured copy rate, memory bound; 8-bit rows (1.25 GB) 268 to 298 us
-// (the board's power limit), 4.2 to 4.6 TB/s, 0.64 to 0.71 of it, bound by issue and the logic pipe (five
-// operations per pair of values to widen them to bf16, of about 650 instructions per step; conversion to fp16 by one
+// rows (2.4 GB) 380 us, 6.3 TB/s, 0.97 of the measured copy rate, memory bound; 8-bit rows (1.25 GB) 292 to 300 us
+// (the board's power limit), 4.2 TB/s, 0.64 of it, bound by issue and the logic pipe (five operations per pair of values to
+// widen them to bf16 and one to find e4m3's NaN, of about 730 instructions per step; conversion to fp16 by one
 // instruction per pair instead, with the ranges kept by powers of two, measured no faster).
 #include <type_traits>
 
@@ -112,7 +112,8 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
 }
 
 // Two e4m3 bytes, at the bottom of x's halves, times f.  (Two of four operations on the logic pipe: 260 us for 32
-// single tokens of 18432; with the bytes' order and mask of widen16 269, with a shift, two masks and an or 278.)
+// single tokens of 18432; with the bytes' order and mask of widen16 269, with a shift, two masks and an or 278, all
+// before NaN bytes were looked for.)
 template <bool BF16>
 __device__ __forceinline__ uint32_t widen2(uint32_t x, uint32_t f) {
   return mul16x2<BF16>(under_exponent<BF16>(x * 256u, x & 0x007f007fu), f);

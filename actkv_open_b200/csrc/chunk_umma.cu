@@ -34,17 +34,21 @@
 //
 // What bounds it.  128 x 128 logits take the tensor core 1024 cycles (two products of head size 128) and the
 // special-function unit as many (16 exponentials per cycle), so both would have to be full all the time.
-// Measured for a 2048-token chunk over 32K tokens (32 heads over 8, 1.07 TFLOP): 1.05 to 1.13 ms, 950 to 1020
+// Measured for a 2048-token chunk over 32K tokens (32 heads over 8, 1.07 TFLOP): 1.02 to 1.11 ms by board, 960 to 1040
 // TFLOP/s, with the board at its power limit and the SM clock at 1450 to 1600 MHz (cuBLAS at that limit:
-// 1385): about 0.57 of the tensor rate at that clock, the rest going into the chain from S through
+// 1385): about 0.6 of the tensor rate at that clock, the rest going into the chain from S through
 // softmax (~1900 cycles: 350 to read S, 350 for the maximum, 1100 for the exponentials, which two warps per
-// scheduler share) to the products.  Tried and not kept: 1 in 2, 4 or 8 exponentials on the FMA pipe
-// (polynomial of degree 4: 941, 1050, 1097 TFLOP/s against 1098), two threads per row (640 threads of 104
-// registers, spills: 858 against 960), S in halves of 64 tokens with twice the buffers (M128 N64 products
-// run at 0.6 of their rate from shared memory: 864).  What helped: descriptors in uniform registers (issue by an
+// scheduler share) to the products.  The row groups of a head run at the same time at unrelated key tiles, so
+// tiles come from DRAM several times over: 1.17 GB for 4 chunks of 512 over 10240, where keys, values and queries are
+// 185 MB; at 3.5 TB/s that is no bound by itself, what it takes from the power limit is not known.  Tried on that chunk (head
+// size 128, where the tensor core takes as long as the exponentials; not at 64) and not kept: 1 in 2, 4 or 8
+// exponentials on the FMA pipe (polynomial of degree 4: 941, 1050, 1097 TFLOP/s against 1098), two threads per row
+// (640 threads of 104 registers, spills: 858 against 960), S in halves of 64 tokens with twice the buffers (M128 N64
+// products run at 0.6 of their rate from shared memory: 864).  What helped: descriptors in uniform registers (issue by an
 // elected lane of a converged warp, 880 to 963), p in halves, packed 32-bit math, and code that fits the
 // instruction cache (the 8-bit variant 650 to 480 us for 4 chunks of 512 over 4K to 16K tokens, and to 430 with the
-// softmax in a loop over halves of a row and a shorter widening; its cache's hit rate 0.88 to 0.96).
+// softmax in a loop over halves of a row and a shorter widening, its cache's hit rate 0.88 to 0.96; 447 and 0.945 since
+// it looks for e4m3's NaN).
 #include <cuda.h>
 
 #include "chunk_common.cuh"

@@ -272,7 +272,8 @@ class QuantPagedCache(DevicePagedCache):
                                            self.seq_used[:R], scale=scale, out=out, lse=lse, workspace=self._chunk_ws)
 
     # The keys read back for scoring: every block of the pool in its place, so that the tables serve
-    # unchanged (one "session" with the identity table), in layer groups of about a gigabyte.
+    # unchanged (one "session" with the identity table), in layer groups of about a gigabyte.  ``keys16`` gives views of
+    # one buffer, which its next call overwrites.
     def layer_groups(self, l0: int, l1: int):
         per = self.num_blocks * self.block_size * self.n_kv_heads * self.head_dim * 2
         step = max(1, min(self.n_layers, (1 << 30) // per))

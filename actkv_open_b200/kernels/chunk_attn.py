@@ -70,6 +70,10 @@ def paged_chunk_attention(q, q_off, kv, block_table, seq_used, scale=None, out=N
     ``scale`` defaults to D ** -0.5; ``workspace`` to a new
     ``chunk_workspace`` (a loop keeps one).  ``path``: "auto", or "tcgen05" / "simt" to force the
     tensor cores (NotImplementedError where they do not apply) or the CUDA cores.
+
+    16-bit calls round the softmax's p and the result to the cache's type each.  For single tokens
+    ``lse_attn.paged_decode_attention`` is the more exact (p in two 16-bit terms, out in fp32) where it applies (1, 2,
+    4 or 8 query heads per KV head); this call takes any number of tokens, gives q's dtype and shares a batch with chunks.
     """
     dev, r_n, out, lse, workspace = _check(q, q_off, kv, block_table, seq_used, out, lse, workspace)
     t_n, hq, d = q.shape
