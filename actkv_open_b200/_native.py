@@ -87,7 +87,15 @@ SIGNATURES = {
                                     I32, I32, I32, I32, I32, I32, I32, P, P]),
     "actkv_quant_append": (I32, [P, P, I32, I64, I64, I64, I64, I64, I64, P, I32, P, I64, I64, I64, I64, P, I64, P, P,
                                  P, I64, I32, I32, I32, I32, I32, I32, I32, P, SZ, P, P]),
+    "actkv_rotate_write": (I32, [P, I64, I64, I64, P, I64, I64, I64, P, I64, I64, I64, P, I64, I64, I64, I32, P, P, I64,
+                                 I32, I32, I32, P, I32, P, I32, I64, I64, I64, I64, I64, P, I64, P, I32, I32, I32, I32,
+                                 I32, I32, I32, I32, P, P]),
 }
+# the 4-bit cache's entries take what the 8-bit cache's do
+for _eight, _four in (("actkv_chunk_attention_quant", "actkv_chunk_attention_quant4"),
+                      ("actkv_quantize_write", "actkv_quantize_write4"),
+                      ("actkv_dequantize_read", "actkv_dequantize_read4"), ("actkv_quant_append", "actkv_quant4_append")):
+    SIGNATURES[_four] = SIGNATURES[_eight]
 
 _lib = None
 _lock = threading.Lock()

@@ -1,6 +1,6 @@
 // Attention of each session's newest tokens (a chunk of queries) over its paged cache, with the
-// log-sum-exp, on CUDA cores: any dtype, head size (a multiple of 32 up to 256 over the 8-bit
-// cache, any up to 256 else), block size, GQA group and stride.  The tensor-core kernel
+// log-sum-exp, on CUDA cores: any dtype, head size (a multiple of 32 up to 256 over the 8- and 4-bit
+// caches, any up to 256 else), block size, GQA group and stride.  The tensor-core kernel
 // (chunk_umma.cu) takes the layouts it can; this one takes the rest (fp32 caches above all).
 //
 // Query j of a session with S tokens and A new ones sees tokens t <= S - A + j.  With
@@ -21,7 +21,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kMaxPer = 8;                  // dims per lane: head_dim <= 256
 
-template <typename T, bool QUANT>
+template <typename T, int BITS>
 __device__ __forceinline__ void load_row(const ChunkArgs& a, const void* base, int64_t off, int h, int lane,
                                          float (&x)[kMaxPer]) {
 #pragma unroll
@@ -29,7 +29,9 @@ __device__ __forceinline__ void load_row(const ChunkArgs& a, const void* base, i
     const int d = lane + 32 * i;
     x[i] = 0.0f;
     if (d >= a.D) continue;
-    if constexpr (QUANT) {
+    if constexpr (BITS == 4) {
+      x[i] = to_f32(from_f32<T>(value4(static_cast<const uint8_t*>(base) + off, a.Hkv, a.D, h, d)));
+    } else if constexpr (BITS == 8) {
       const uint8_t* row = static_cast<const uint8_t*>(base) + off;
       const int e = h * a.D + d;
       x[i] = to_f32(from_f32<T>(e4m3x2_f32(row[e]).x * scale_of(row[a.Hkv * a.D + e / kQuantGroup])));
@@ -39,7 +41,7 @@ __device__ __forceinline__ void load_row(const ChunkArgs& a, const void* base, i
   }
 }
 
-template <typename T, bool QUANT>
+template <typename T, int BITS>
 __global__ void __launch_bounds__(kWarps * 32) chunk_simt_kernel(ChunkArgs a) {
   __shared__ float sh_m[kWarps], sh_l[kWarps], sh_o[kWarps][256];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -75,8 +77,8 @@ __global__ void __launch_bounds__(kWarps * 32) chunk_simt_kernel(ChunkArgs a) {
     }
     const int64_t off = int64_t(phys) * a.kv_stride_b + int64_t(p - lb * a.BS) * a.kv_stride_s;
     float k[kMaxPer], v[kMaxPer];
-    load_row<T, QUANT>(a, a.kv, off, h, lane, k);
-    load_row<T, QUANT>(a, a.kv, off + a.kv_stride_kv, h, lane, v);
+    load_row<T, BITS>(a, a.kv, off, h, lane, k);
+    load_row<T, BITS>(a, a.kv, off + a.kv_stride_kv, h, lane, v);
     float x = 0.0f;
 #pragma unroll
     for (int i = 0; i < kMaxPer; ++i) x = fmaf(q[i], k[i], x);
@@ -119,18 +121,23 @@ __global__ void __launch_bounds__(kWarps * 32) chunk_simt_kernel(ChunkArgs a) {
 
 }  // namespace
 
+namespace {
+
+template <typename T>
+void launch_simt(const ChunkArgs& a, dim3 grid, dim3 block, cudaStream_t st) {
+  if (a.quant == 8) chunk_simt_kernel<T, 8><<<grid, block, 0, st>>>(a);
+  else if (a.quant == 4) chunk_simt_kernel<T, 4><<<grid, block, 0, st>>>(a);
+  else chunk_simt_kernel<T, 0><<<grid, block, 0, st>>>(a);
+}
+
+}  // namespace
+
 cudaError_t launch_chunk_simt(const ChunkArgs& a, int dtype, cudaStream_t st) {
   const int64_t ctas = int64_t(a.T) * a.Hq;
   const dim3 grid = dim3(unsigned(ctas)), block = dim3(kWarps * 32);
-  if (a.quant) {
-    if (dtype == ACTKV_BF16) chunk_simt_kernel<__nv_bfloat16, true><<<grid, block, 0, st>>>(a);
-    else if (dtype == ACTKV_F16) chunk_simt_kernel<__half, true><<<grid, block, 0, st>>>(a);
-    else chunk_simt_kernel<float, true><<<grid, block, 0, st>>>(a);
-  } else {
-    if (dtype == ACTKV_BF16) chunk_simt_kernel<__nv_bfloat16, false><<<grid, block, 0, st>>>(a);
-    else if (dtype == ACTKV_F16) chunk_simt_kernel<__half, false><<<grid, block, 0, st>>>(a);
-    else chunk_simt_kernel<float, false><<<grid, block, 0, st>>>(a);
-  }
+  if (dtype == ACTKV_BF16) launch_simt<__nv_bfloat16>(a, grid, block, st);
+  else if (dtype == ACTKV_F16) launch_simt<__half>(a, grid, block, st);
+  else launch_simt<float>(a, grid, block, st);
   return cudaGetLastError();
 }
 

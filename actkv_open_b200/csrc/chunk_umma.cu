@@ -1391,6 +1391,7 @@ bool chunk_umma_supported(const ChunkArgs& a, int dtype, const char** why) {
     *why = w;
     return false;
   };
+  if (a.quant == 4) return no("not over the 4-bit cache");
   if (dtype != ACTKV_BF16 && dtype != ACTKV_F16) return no("needs bf16 or fp16");
   if (a.D != 64 && a.D != 128) return no("needs head_dim 64 or 128");
   if (a.G > chunk::kRows) return no("needs a GQA group of at most 128");

@@ -308,8 +308,8 @@ struct ChunkArgs {
   const void* q;             // [T][Hq][D], D contiguous
   int64_t q_stride_t, q_stride_h;
   const int32_t* q_off;      // [R + 1] packed offsets of the sessions' queries
-  const void* kv;            // one layer: [2][NB][BS][Hkv][D], or the 8-bit rows [2][NB][BS][row]
-  int64_t kv_stride_kv, kv_stride_b, kv_stride_s, kv_stride_h;   // 8-bit rows: in bytes, no stride_h
+  const void* kv;            // one layer: [2][NB][BS][Hkv][D], or the 8- or 4-bit rows [2][NB][BS][row]
+  int64_t kv_stride_kv, kv_stride_b, kv_stride_s, kv_stride_h;   // rows: in bytes, no stride_h
   const int32_t* block_table;
   int64_t bt_stride_r;
   const int32_t* seq_used;
@@ -318,7 +318,7 @@ struct ChunkArgs {
   float* lse;                // [T][Hq]
   int64_t lse_stride_t;
   int T, R, MB, NB, BS, Hq, Hkv, G, D;
-  bool quant;
+  int quant;                 // 0, or the bits of the rows' values: 8, 4
   float scale;
   void* workspace;           // chunk_workspace_bytes()
   int32_t* status;
@@ -367,6 +367,33 @@ struct QuantMoveArgs {
 
 cudaError_t launch_quant_write(const QuantMoveArgs& a, int dtype, cudaStream_t st);
 cudaError_t launch_quant_read(const QuantMoveArgs& a, int dtype, cudaStream_t st);
+
+// 4-bit rows into k / v (rotary.cu has the writer)
+cudaError_t launch_quant4_read(const QuantMoveArgs& a, int dtype, cudaStream_t st);
+
+// ---------------------------------------------------------------- rows with their rotation (rotary.cu)
+struct RotateArgs {
+  const void* in[3];         // q (or null), k, v: [L][T][H][D], D contiguous
+  int64_t in_l[3], in_t[3], in_h[3];
+  void* q_out;               // [L][T][Hq][D]; may be q
+  int64_t out_l, out_t, out_h;
+  const int32_t* positions;  // [T]; null with rot 0
+  const float* angles;       // [P][rot]: rot / 2 cosines, then as many sines
+  int64_t angles_stride;
+  int P, rot, pairs;         // pairs: dims (2 i, 2 i + 1) turn together, else (i, i + rot / 2)
+  const int32_t* tok_off;    // [R + 1]; session r's last tok_off[r + 1] - tok_off[r] tokens
+  void* cache;               // [L][2][NB][BS][Hkv][D] of the inputs' type, or rows [L][2][NB][BS][row]
+  int64_t c_l, c_kv, c_b, c_s, c_h;      // in elements; rows: in bytes, no c_h
+  const int32_t* block_table;
+  int64_t bt_stride_r;
+  const int32_t* seq_used;
+  const int32_t* ok;         // nullable: sessions with ok[r] == 0 are left alone
+  int T, R, L, MB, NB, BS, Hq, Hkv, D;
+  int bits;                  // 0: a cache of the inputs' type; 8, 4: rows
+  bool vec_in, vec_out;      // 16-byte accesses allowed on q, q_out, k, v and angles / on the cache
+  int32_t* status;
+};
+cudaError_t launch_rotate_write(const RotateArgs& a, int dtype, cudaStream_t st);
 
 // Which sessions the last launch_append over this workspace appended ([R] flags).
 const int32_t* append_ok_flags(void* workspace, int R);

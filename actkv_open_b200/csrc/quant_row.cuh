@@ -1,4 +1,5 @@
-// The 8-bit cache row, shared by the kernels that write it, read it back and attend over it.
+// The rows of the 8-bit and the 4-bit cache, shared by the kernels that write them, read them back and
+// attend over them.
 //
 // A token's row of one plane: Hkv * D e4m3 values, then Hkv * D / 32 scale bytes, one per group of
 // 32 values along D, then padding.  Value i of a group with scale byte b stands for
@@ -7,8 +8,18 @@
 // zeros has b = 0; a group with a non-finite value has b = 255.  A power of two as scale keeps the
 // products x * 2^(127 - b) and e4m3 * 2^(b - 127) exact, so the only rounding is the one to e4m3
 // (nearest, ties to even; half a unit in the fourth significant bit).
+//
+// The 4-bit row: Hkv * D / 2 bytes of e2m1 values (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), then
+// the scale bytes as above.  b is the smallest exponent with max|x| <= 7 * 2^(b - 127), clamped to 0 .. 252:
+// up to 7 the largest value errs by at most 1 (it becomes 6), half of what the level 8 above would be away, and
+// normal groups come out 0.3 dB nearer than with the limit at 6 (19.0 against 18.7).  Up to 252 every value is
+// finite in bf16; 253 to 255 stand for NaN (the writer uses 255, with values of 0).
+// Order within a head: value 32 g + 4 p + j (p < 8, j < 4) is in byte p * D / 16 + 2 g + j / 2, the low half for even
+// j.  So the four values of every group that a lane of the attention's products takes come in one load, and the 16
+// dims of a product are of one group: the scales multiply 32-bit sums and the probabilities, not every value.
 #pragma once
 
+#include <cuda_fp4.h>
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -41,6 +52,51 @@ __device__ __forceinline__ float2 e4m3x2_f32(uint32_t two) {
 
 __device__ __forceinline__ uint32_t f32_e4m3x2(float lo, float hi) {
   return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+
+constexpr uint32_t kNan4 = 253;             // from here on a scale byte of the 4-bit row stands for NaN
+
+// Scale byte of a 4-bit group whose largest magnitude has the bits `top`: 7 = 1.75 * 2^2.
+__device__ __forceinline__ uint32_t scale_byte4(uint32_t top) {
+  if (top >= 0x7f800000u) return 255u;
+  const int e = int(top >> 23) - 2 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return uint32_t(min(max(e, 0), 252));
+}
+__device__ __forceinline__ float scale_of4(uint32_t b) { return scale_of(b >= kNan4 ? 255u : b); }
+
+// Four values (the first in the lowest half byte) and back: one conversion per pair.
+__device__ __forceinline__ uint32_t f32_e2m1x4(float x0, float x1, float x2, float x3) {
+  const uint32_t lo = __nv_cvt_float2_to_fp4x2(make_float2(x0, x1), __NV_E2M1, cudaRoundNearest);
+  const uint32_t hi = __nv_cvt_float2_to_fp4x2(make_float2(x2, x3), __NV_E2M1, cudaRoundNearest);
+  return lo | hi << 8;
+}
+__device__ __forceinline__ uint32_t e2m1x2_f16(uint32_t two) {
+  const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2(__nv_fp4x2_storage_t(two), __NV_E2M1);
+  return uint32_t(h.x) | uint32_t(h.y) << 16;
+}
+// The eight values of a word, byte i's in r[i], as fp16 (exact).  (For words as they were loaded: on a word put together
+// from two single bytes, upper half zero, this gave zeros with nvcc 12.9.)
+__device__ __forceinline__ void e2m1x8_f16(uint32_t w, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+      : "r"(w));
+}
+__device__ __forceinline__ float2 f16x2_f32(uint32_t h) { return __half22float2(reinterpret_cast<const __half2&>(h)); }
+
+// Bytes of values of a row, and the row's least length.
+__host__ __device__ inline int64_t payload_bytes(int bits, int Hkv, int D) { return int64_t(Hkv) * D * bits / 8; }
+__host__ __device__ inline int64_t least_row_bytes(int bits, int Hkv, int D) {
+  return payload_bytes(bits, Hkv, D) + int64_t(Hkv) * (D / kQuantGroup);
+}
+// Value d of head h of a 4-bit row, in 32 bits.
+__device__ __forceinline__ float value4(const uint8_t* row, int Hkv, int D, int h, int d) {
+  const uint32_t g = uint32_t(d) / 32u, p = uint32_t(d) % 32u / 4u, j = uint32_t(d) & 3u;
+  const uint32_t code = row[h * (D / 2) + int(p * (uint32_t(D) / 16u) + 2u * g + j / 2u)] >> (4u * (j & 1u)) & 15u;
+  const uint32_t e = code >> 1 & 3u, m = code & 1u;        // 0.5 m, or (1 + 0.5 m) 2^(e - 1)
+  const float size = e == 0u ? 0.5f * float(m) : __uint_as_float((126u + e) << 23 | m << 22);
+  return (code & 8u ? -size : size) * scale_of4(row[Hkv * (D / 2) + h * (D / kQuantGroup) + int(g)]);
 }
 
 // A value of the cache in the type it is read in.

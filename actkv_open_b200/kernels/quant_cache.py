@@ -1,4 +1,4 @@
-"""A paged KV cache in 8 bits: quantising rows as they are written, reading them back, and attention
+"""A paged KV cache in 8 or 4 bits: quantising rows as they are written, reading them back, and attention
 over it.  (The reference has no counterpart; its cache is 16-bit, actkv/paged.py:54.)
 
 ``rows`` [L, 2, NB, BS, row_bytes] uint8 (one layer for attention: [2, NB, BS, row_bytes]).  A token's
@@ -7,6 +7,13 @@ row of one plane is Hkv * D e4m3 values, then Hkv * D / 32 scale bytes, one per 
 two with max|x| <= 448 * scale, so values are exact in bf16 and err by at most 1/16 of themselves
 (or 2^-10 of the scale's unit, for values that small).  Rows move as bytes: append, release and
 compaction treat such a cache like any other (``engine.QuantPagedCache``).
+
+With ``bits`` 4 a row is Hkv * D / 2 bytes of e2m1 values (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their
+negatives), then the scale bytes (from 253 on: NaN), then padding.  The scale is the smallest power of
+two, up to 2^125, with max|x| <= 7 * scale (between 6 and 7 the largest value becomes 6): values err by
+at most 1 / 7 of the largest of their 32, about 0.11 of themselves in the mean square.  Value
+32 g + 4 p + j of a head (p < 8, j < 4) is in the head's byte p * D / 16 + 2 g + j // 2, the low half for
+even j.
 """
 from __future__ import annotations
 
@@ -18,22 +25,30 @@ from .chunk_attn import _PATHS, _check
 QUANT_GROUP = 32
 
 
-def quant_row_bytes(n_kv_heads: int, head_dim: int) -> int:
+def _bits(bits) -> bool:
+    """Whether it is the 4-bit cache."""
+    if bits != 8 and bits != 4:
+        raise ValueError(f"bits {bits}: the cache holds its rows in 8 or 4")
+    return bits == 4
+
+
+def quant_row_bytes(n_kv_heads: int, head_dim: int, bits: int = 8) -> int:
     """Bytes of a token's row of one plane: values and scales, padded to whole 64-byte pieces (so
-    that every head's values start on one)."""
+    that every head's values start on one); in 4 bits, where a head of 64 has half of that, to 32-byte ones."""
     assert head_dim % QUANT_GROUP == 0, f"head_dim must be a multiple of {QUANT_GROUP}"
-    return -(-n_kv_heads * (head_dim + head_dim // QUANT_GROUP) // 64) * 64
+    pad = 32 if _bits(bits) else 64
+    return -(-n_kv_heads * (head_dim * bits // 8 + head_dim // QUANT_GROUP) // pad) * pad
 
 
 _I32, _U8 = torch.int32, torch.uint8
 
 
-def _tables(dev, L, t_n, hkv, d, rows, tok_off, block_table, seq_used):
+def _tables(dev, L, t_n, hkv, d, rows, tok_off, block_table, seq_used, bits):
     """The checks and the arguments that writing and reading share."""
     assert rows.dim() == 5 and rows.dtype is _U8, "rows is [L, 2, NB, BS, row_bytes] uint8"
     rl, _2, nb, bs, row = rows.shape
     assert _2 == 2 and rl == L, "rows and the tokens must have the same layers"
-    assert row >= hkv * (d + d // QUANT_GROUP), "rows are too short for these heads"
+    assert row >= hkv * (d * bits // 8 + d // QUANT_GROUP), "rows are too short for these heads"
     s_l, s_kv, s_b, s_s, s_1 = rows.stride()
     assert s_1 == 1 and block_table.stride(1) == 1
     assert tok_off.dtype is _I32 and seq_used.dtype is _I32 and block_table.dtype is _I32
@@ -45,8 +60,9 @@ def _tables(dev, L, t_n, hkv, d, rows, tok_off, block_table, seq_used):
             N.status_word(dev).data_ptr(), N.stream_ptr(dev))
 
 
-def quantize_write(k_new, v_new, tok_off, rows, block_table, seq_used):
+def quantize_write(k_new, v_new, tok_off, rows, block_table, seq_used, bits: int = 8):
     """Quantise new K / V rows into the cache, every layer in one launch.  In place; returns ``rows``.
+    (``rotary.rotate_write`` does the same with the keys' position rotation on the way.)
 
     k_new / v_new [L, T, Hkv, D] (bf16, fp16 or fp32) hold the sessions' new tokens packed, session r
     owning tok_off[r]:tok_off[r+1] (int32 [R+1], T = tok_off[R]); they become the newest
@@ -62,16 +78,17 @@ def quantize_write(k_new, v_new, tok_off, rows, block_table, seq_used):
     k_l, k_t, k_h, k_1 = k_new.stride()
     v_l, v_t, v_h, v_1 = v_new.stride()
     assert k_1 == 1 and v_1 == 1
-    code = N.load().actkv_quantize_write(
+    lib = N.load()
+    code = (lib.actkv_quantize_write4 if _bits(bits) else lib.actkv_quantize_write)(
         k_new.data_ptr(), v_new.data_ptr(), N.dtype_code(k_new), k_l, k_t, k_h, v_l, v_t, v_h,
-        *_tables(dev, *shape, rows, tok_off, block_table, seq_used))
+        *_tables(dev, *shape, rows, tok_off, block_table, seq_used, bits))
     if code:
         N.check(code, "quantize_write")
     return rows
 
 
 def dequantize_read(rows, n_kv_heads, head_dim, tok_off, block_table, seq_used, n_tokens, dtype=torch.bfloat16,
-                    k_out=None, v_out=None, planes: str = "kv"):
+                    k_out=None, v_out=None, planes: str = "kv", bits: int = 8):
     """Read each session's newest tok_off[r+1] - tok_off[r] tokens back: (k, v) [L, n_tokens, Hkv, D],
     packed as ``quantize_write`` takes them (n_tokens = tok_off[R]), rounded to ``dtype`` (fp16:
     values past its range become its largest).
@@ -102,29 +119,32 @@ def dequantize_read(rows, n_kv_heads, head_dim, tok_off, block_table, seq_used, 
         *three, one = x.stride()
         assert x.shape == shape and x.dtype is some.dtype and one == 1
         strides += three
-    code = N.load().actkv_dequantize_read(
+    lib = N.load()
+    code = (lib.actkv_dequantize_read4 if _bits(bits) else lib.actkv_dequantize_read)(
         N.ptr(k_out), N.ptr(v_out), N.dtype_code(some), *strides,
-        *_tables(dev, *shape, rows, tok_off, block_table, seq_used))
+        *_tables(dev, *shape, rows, tok_off, block_table, seq_used, bits))
     if code:
         N.check(code, "dequantize_read")
     return k_out, v_out
 
 
 def paged_chunk_attention_quant(q, q_off, rows, n_kv_heads, block_table, seq_used, scale=None, out=None, lse=None,
-                                workspace=None, path: str = "auto"):
-    """``paged_chunk_attention`` over one layer of the 8-bit cache, rows [2, NB, BS, row_bytes]: the
-    keys and values are what ``dequantize_read`` gives in q's dtype."""
+                                workspace=None, path: str = "auto", bits: int = 8):
+    """``paged_chunk_attention`` over one layer of the 8- or 4-bit cache, rows [2, NB, BS, row_bytes]:
+    the keys and values are what ``dequantize_read`` gives in q's dtype."""
+    four = _bits(bits)
     dev, r_n, out, lse, workspace = _check(q, q_off, rows, block_table, seq_used, out, lse, workspace)
     t_n, hq, d = q.shape
     _2, nb, bs, row = rows.shape
     assert _2 == 2 and rows.dtype is _U8, "rows is [2, NB, BS, row_bytes] uint8"
     assert hq % n_kv_heads == 0
-    assert row >= n_kv_heads * (d + d // QUANT_GROUP), "rows are too short for these heads"
+    assert row >= n_kv_heads * (d * bits // 8 + d // QUANT_GROUP), "rows are too short for these heads"
     s_kv, s_b, s_s, s_1 = rows.stride()
     assert s_1 == 1
     q_t, q_h, _1 = q.stride()
     o_t, o_h, _1 = out.stride()
-    code = N.load().actkv_chunk_attention_quant(
+    lib = N.load()
+    code = (lib.actkv_chunk_attention_quant4 if four else lib.actkv_chunk_attention_quant)(
         q.data_ptr(), N.dtype_code(q), q_t, q_h, q_off.data_ptr(), t_n, rows.data_ptr(), s_kv, s_b, s_s,
         block_table.data_ptr(), block_table.stride(0), seq_used.data_ptr(), out.data_ptr(), o_t, o_h, lse.data_ptr(),
         lse.stride(0), r_n, block_table.size(1), nb, bs, hq, n_kv_heads, d,

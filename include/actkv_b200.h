@@ -470,8 +470,9 @@ ACTKV_API int actkv_decode_attention(const void* q, int dtype, int64_t q_stride_
  * workspace: actkv_chunk_workspace_bytes() bytes, 16-byte aligned, of any contents; calls that may
  * overlap on the GPU need one each.
  *
- * actkv_chunk_attention_quant: the same over the 8-bit cache rows [2][NB][BS][row_bytes] (strides in
- * bytes), see actkv_quantize_write; the values are those the bytes stand for, rounded to q's dtype.
+ * actkv_chunk_attention_quant, actkv_chunk_attention_quant4: the same over the 8- or 4-bit cache rows
+ * [2][NB][BS][row_bytes] (strides in bytes), see actkv_quantize_write; the values are those the bytes stand for, rounded to
+ * q's dtype.
  */
 ACTKV_API size_t actkv_chunk_workspace_bytes(void);
 ACTKV_API int actkv_chunk_attention(const void* q, int dtype, int64_t q_stride_t, int64_t q_stride_h,
@@ -491,6 +492,15 @@ ACTKV_API int actkv_chunk_attention_quant(const void* q, int dtype, int64_t q_st
                                           int64_t lse_stride_t, int R, int MB, int NB, int BS, int Hq, int Hkv,
                                           int D, float scale, int path, void* workspace, size_t workspace_bytes,
                                           int32_t* status, void* stream);
+ACTKV_API int actkv_chunk_attention_quant4(const void* q, int dtype, int64_t q_stride_t, int64_t q_stride_h,
+                                           const int32_t* q_off, int T, const uint8_t* rows,
+                                           int64_t rows_stride_kv_bytes, int64_t rows_stride_b_bytes,
+                                           int64_t rows_stride_s_bytes, const int32_t* block_table,
+                                           int64_t bt_stride_r, const int32_t* seq_used, void* out,
+                                           int64_t out_stride_t, int64_t out_stride_h, float* lse,
+                                           int64_t lse_stride_t, int R, int MB, int NB, int BS, int Hq, int Hkv,
+                                           int D, float scale, int path, void* workspace, size_t workspace_bytes,
+                                           int32_t* status, void* stream);
 
 /*
  * The 8-bit paged cache (no counterpart in the reference).  rows [L][2][NB][BS][row_bytes]: a
@@ -533,6 +543,64 @@ ACTKV_API int actkv_quant_append(const void* k_new, const void* v_new, int dtype
                                  int32_t* free_top, int64_t free_capacity, int R, int L, int MB, int NB, int BS,
                                  int Hkv, int D, void* workspace, size_t workspace_bytes, int32_t* status,
                                  void* stream);
+
+/*
+ * The 4-bit paged cache (no counterpart in the reference), used like the 8-bit one.  A token's row of one plane is
+ * Hkv * D / 2 bytes of e2m1 values (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives, the sign in the fourth bit), then
+ * Hkv * D / 32 scale bytes (value = e2m1 * 2^(byte - 127); from 253 on: NaN), then padding; row_bytes >=
+ * Hkv * (D / 2 + D / 32).  Value 32 g + 4 p + j of a head (p < 8, j < 4) is in the head's byte p * D / 16 + 2 g + j / 2, the
+ * low half for even j.  actkv_quantize_write4 takes per group of 32 the smallest scale, up to byte 252, with
+ * max|x| <= 7 * scale (the largest value becomes at most 6 * scale), values rounded to the nearest, ties to the even
+ * code; a group with a non-finite value becomes NaN (byte 255, values 0).
+ */
+ACTKV_API int actkv_quantize_write4(const void* k_new, const void* v_new, int dtype, int64_t k_stride_l,
+                                    int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_l, int64_t v_stride_t,
+                                    int64_t v_stride_h, const int32_t* tok_off, int T, uint8_t* rows,
+                                    int64_t rows_stride_l_bytes, int64_t rows_stride_kv_bytes,
+                                    int64_t rows_stride_b_bytes, int64_t rows_stride_s_bytes,
+                                    const int32_t* block_table, int64_t bt_stride_r, const int32_t* seq_used, int R,
+                                    int L, int MB, int NB, int BS, int Hkv, int D, int32_t* status, void* stream);
+ACTKV_API int actkv_dequantize_read4(void* k_out, void* v_out, int dtype, int64_t k_stride_l, int64_t k_stride_t,
+                                     int64_t k_stride_h, int64_t v_stride_l, int64_t v_stride_t, int64_t v_stride_h,
+                                     const int32_t* tok_off, int T, const uint8_t* rows, int64_t rows_stride_l_bytes,
+                                     int64_t rows_stride_kv_bytes, int64_t rows_stride_b_bytes,
+                                     int64_t rows_stride_s_bytes, const int32_t* block_table, int64_t bt_stride_r,
+                                     const int32_t* seq_used, int R, int L, int MB, int NB, int BS, int Hkv, int D,
+                                     int32_t* status, void* stream);
+ACTKV_API int actkv_quant4_append(const void* k_new, const void* v_new, int dtype, int64_t k_stride_l,
+                                  int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_l, int64_t v_stride_t,
+                                  int64_t v_stride_h, const int32_t* new_off, int T, uint8_t* rows,
+                                  int64_t rows_stride_l_bytes, int64_t rows_stride_kv_bytes,
+                                  int64_t rows_stride_b_bytes, int64_t rows_stride_s_bytes, int32_t* block_table,
+                                  int64_t bt_stride_r, int32_t* seq_used, const int32_t* free_list,
+                                  int32_t* free_top, int64_t free_capacity, int R, int L, int MB, int NB, int BS,
+                                  int Hkv, int D, void* workspace, size_t workspace_bytes, int32_t* status,
+                                  void* stream);
+
+/*
+ * New tokens into a paged cache with their position rotation (no counterpart in the reference, whose caller rotates before
+ * append), every layer in one launch.  q [L][T][Hq][D] (NULL with Hq 0), k_new and v_new [L][T][Hkv][D] of one dtype
+ * (element strides, D contiguous) hold the sessions' new tokens packed, session r owning tok_off[r]..tok_off[r+1]; they
+ * become the newest tokens of its seq_used[r], whose blocks the tables already hold.  positions [T]; angles fp32
+ * [P][angles_stride]: row p holds rot / 2 cosines, then rot / 2 sines, of position p.  q and k turn: pair i, dims (i, i + rot / 2)
+ * or, with pairs, (2 i, 2 i + 1), becomes (x c - y s, y c + x s), computed in 32 bits and rounded once; dims from rot on stay.
+ * Turned q goes to q_out (which may be q; other overlaps are not allowed), turned k and v into the cache:
+ *   bits 0     cache [L][2][NB][BS][Hkv][D] of that dtype, strides in elements
+ *   bits 8, 4  rows [L][2][NB][BS][row_bytes], strides in bytes (cache_stride_h unused): quantised as
+ *              actkv_quantize_write / actkv_quantize_write4 do, from the 32-bit values; D a multiple of 32, rot of 8
+ * A token of no session is left alone; so is one whose position the angles do not have, and the cache for one that the
+ * tables do not hold (ACTKV_DEV_BAD_INDEX, both).
+ */
+ACTKV_API int actkv_rotate_write(const void* q, int64_t q_stride_l, int64_t q_stride_t, int64_t q_stride_h, void* q_out,
+                                 int64_t out_stride_l, int64_t out_stride_t, int64_t out_stride_h, const void* k_new,
+                                 int64_t k_stride_l, int64_t k_stride_t, int64_t k_stride_h, const void* v_new,
+                                 int64_t v_stride_l, int64_t v_stride_t, int64_t v_stride_h, int dtype,
+                                 const int32_t* positions, const float* angles, int64_t angles_stride, int P, int rot,
+                                 int pairs, const int32_t* tok_off, int T, void* cache, int bits, int64_t cache_stride_l,
+                                 int64_t cache_stride_kv, int64_t cache_stride_b, int64_t cache_stride_s,
+                                 int64_t cache_stride_h, const int32_t* block_table, int64_t bt_stride_r,
+                                 const int32_t* seq_used, int R, int L, int MB, int NB, int BS, int Hq, int Hkv, int D,
+                                 int32_t* status, void* stream);
 
 /*
  * Self-test of the kernels' failure path (no counterpart in the reference): one block waits, with
