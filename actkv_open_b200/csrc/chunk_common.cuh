@@ -15,7 +15,7 @@ using namespace umma;
 constexpr int kRows = 128;                  // query rows per row tile (MMA M)
 constexpr int kTile = 128;                  // tokens per key tile, the grain of the schedule
 constexpr int kFewRows = 16;                // query rows of a session and KV head that chunk_few_kernel takes
-constexpr int few_limit(bool quant) { return quant ? 8 : kFewRows; }      // ... of which over the 8-bit cache
+constexpr int few_limit(int quant) { return quant ? 8 : kFewRows; }       // ... of which over the 8- and 4-bit caches
 constexpr int kFewParts = 8 * kFewRows;     // rows of its units: up to 8 heads
 // (6 sessions of 2000 to 10000 tokens with 1088 new: 749 us with a cost of 2, 713 with 4, 708 with 6; prompts and
 // single tokens of head size 64: 157, 153, 157)
@@ -82,8 +82,8 @@ __device__ __forceinline__ int few_rows_now(const ChunkArgs& a, int64_t (&sums)[
     atomicAdd(reinterpret_cast<unsigned long long*>(&sums[1]), static_cast<unsigned long long>(all));
   }
   __syncthreads();
-  const int64_t bytes = sums[0] * a.Hkv * a.D * 2 * (a.quant ? 1 : 2);
-  return sums[0] == sums[1] || bytes >= (int64_t(a.quant ? 64 : 512) << 20) ? a.few_rows : 0;
+  const int64_t bytes = sums[0] * a.Hkv * a.D * 2 * (a.quant ? a.quant : 16) / 8;
+  return sums[0] == sums[1] || bytes >= (int64_t(a.quant ? 8 * a.quant : 512) << 20) ? a.few_rows : 0;
 }
 
 // CTAs that get work when a share is at least `least`.
@@ -276,6 +276,56 @@ __device__ __forceinline__ uint32_t mul_rest(uint32_t x, uint32_t f1, uint32_t f
     asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(x) : "r"(0xfbfffbffu));
   }
   return x;
+}
+// The 4-bit cache.  Eight values as 16-bit ones, times the power of two of their scale byte: fp16 by one conversion per
+// pair; for bf16 its exponent and first mantissa bit moved under bf16's exponent, where it reads as the value times
+// 2^-112.  Where no scale byte of a word is out of the ordinary one multiplication does:
+template <bool BF16>
+__device__ __forceinline__ bool plain_scales4(uint32_t w) {
+  return __vcmpgtu4(w, BF16 ? 0x8e8e8e8eu : 0x8c8c8c8cu) == 0 && (BF16 || __vcmpgtu4(0x71717171u, w) == 0);   // <= 142 (fp16: 113 .. 140)
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t plain_factor4(uint32_t b) {
+  return BF16 ? b * 0x00800080u + 0x38003800u : (b - 112u) * 0x04000400u;
+}
+template <bool BF16>
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t f, uint32_t (&r)[4]) {
+  e2m1x8_f16(w, r[0], r[1], r[2], r[3]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (BF16) {
+      const uint32_t m = r[i] & 0x7fff7fffu;
+      r[i] = (r[i] ^ m) | (m >> 3);
+    }
+    r[i] = mul16x2<BF16>(r[i], f);
+  }
+}
+// ... for any scale byte: two multiplications, of which only the last rounds; fp16 past its range: its largest.
+template <bool BF16>
+__device__ __forceinline__ void widen4_any(uint32_t w, uint32_t b, uint32_t (&r)[4]) {
+  uint32_t f0, f1;
+  if constexpr (BF16) {
+    const uint32_t e = min(b, 142u);
+    f0 = e * 0x00800080u + 0x38003800u;
+    f1 = (b - e + 127u) * 0x00800080u;
+  } else if (b < 113u) {                       // 2^-14, exact for what comes first, and the rest down to its subnormals
+    f0 = 0x04000400u;
+    f1 = (b >= 99u ? b - 98u << 10 : (b >= 89u ? 1u << b - 89u : 0u)) * 0x00010001u;
+  } else {
+    const uint32_t e = min(b, 140u);
+    f0 = (e - 112u) * 0x04000400u;
+    f1 = (min(b - e, 15u) + 15u) * 0x04000400u;
+  }
+  if (b >= kNan4) f1 = 0x7fff7fffu;            // NaN
+  widen4<BF16>(w, f0, r);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    r[i] = mul16x2<BF16>(r[i], f1);
+    if constexpr (!BF16) {
+      asm("min.NaN.f16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(0x7bff7bffu));
+      asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(0xfbfffbffu));
+    }
+  }
 }
 // What is not finite among two 16-bit values, in the halves `hide` (0xffff per half), becomes 0.
 template <bool BF16>

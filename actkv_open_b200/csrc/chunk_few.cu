@@ -36,7 +36,7 @@
 // instruction per pair instead, with the ranges kept by powers of two, measured no faster).
 #include <type_traits>
 
-#include "chunk_common.cuh"
+#include "few_common.cuh"
 
 namespace actkv {
 namespace chunk {
@@ -70,47 +70,6 @@ __device__ __forceinline__ int value_piece(int r, int c) {
   return CH == 16 ? c ^ (((r >> 1) & 1) | (r & 4)) : (CH == 8 ? c ^ (r & 6) : c ^ ((r >> 1) & 2));
 }
 
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copy4(uint32_t dst, const void* src, bool on) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
-}
-__device__ __forceinline__ uint4 lds16(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint2 lds8(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint32_t lds4(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
-  return v;
-}
-
-template <bool BF16>
-__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (BF16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// Lane (r, c) has elements (r, 2 c) and (r, 2 c + 1) of an 8 x 8 matrix; of its transpose after.
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
-  uint32_t y;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-  return y;
-}
-
 // Two e4m3 bytes, at the bottom of x's halves, times f.  (Two of four operations on the logic pipe: 260 us for 32
 // single tokens of 18432; with the bytes' order and mask of widen16 269, with a shift, two masks and an or 278, all
 // before NaN bytes were looked for.)
@@ -127,13 +86,6 @@ __device__ __forceinline__ uint32_t widen2_any(uint32_t x, uint32_t b_lo, uint32
   return put_nan(mul_rest<BF16>(widen2<BF16>(x, __byte_perm(lo[0], hi[0], 0x5410)), __byte_perm(lo[1], hi[1], 0x5410),
                                 __byte_perm(lo[2], hi[2], 0x5410)), x & 0x007f007fu);
 }
-struct Sched {
-  Share share;
-  int64_t scan[32], sums[2];
-  int bad_v;                 // values that are not finite went in as 0: 1 among those some row does not see, 2 anywhere
-};
-static_assert(sizeof(Sched) <= 512, "the schedule's place in shared memory");
-
 template <int D, bool BF16, bool QUANT>
 __global__ void __launch_bounds__(Ring<D, QUANT>::kThreads, 1) chunk_few_kernel(const __grid_constant__ ChunkArgs a, bool vec_out) {
   using Rg = Ring<D, QUANT>;

@@ -1,0 +1,731 @@
+// Chunk attention of sessions with few new tokens over the 4-bit cache (quant_row.cuh): the formulas of
+// chunk_umma.cu, the plan of chunk_few.cu (a warp per KV head and run of tokens, a private ring of cp.async
+// copies, running sums in registers, no hand-overs), with products laid out so that no value is scaled by itself.
+//
+// e2m1 values are exact in fp16 and one instruction widens two of them, so both products take them as they are, in fp16
+// whatever the queries' type, and the scales enter elsewhere:
+//   S^T = K Q^T    the 16 dims of a product are of one group of 32, so a group's two products give a 32-bit partial sum
+//                  per (token, row), which is multiplied by the token's scale as it is added: 4 multiply-adds per
+//                  512 values.
+//   O^T = V^T p^T  the 16 dims that a product gives are of one group, so p is multiplied by the token's scale of
+//                  that group, in fp16, once per group: 2 multiplications per 512 values.  So that a scale of any size
+//                  fits, it is taken relative to the largest that the warp has met in the group, 2^(b - E) <= 1; E is
+//                  raised, and O rescaled exactly, when a larger one comes, like the running maximum.
+// Queries of 16-bit types go in as fp16: bf16 rows times the power of two that brings their largest value to 2^14 .. 2^15, so
+// that what is 2^-28 of it is still exact.  p is rounded to fp16's 11 bits (times 2^7 and the scale: what comes out
+// below fp16's normal range loses the digits below 2^-32 of the largest).
+//
+// Tokens that some of the rows do not see are the newest ones, 7 at most: their values are added in 32 bits one
+// token at a time, each row with an E of its own from there on, so that a hidden value of any size changes nothing in the
+// rows that do not see it.
+#include <type_traits>
+
+#include "few_common.cuh"
+
+namespace actkv {
+namespace chunk {
+namespace few {
+namespace four {
+
+constexpr int kStep = 32;                   // tokens per step of a warp
+constexpr int kWarps = 16, kThreads = kWarps * 32;
+constexpr int kRoundCost = 3;               // a unit's fixed cost in rounds of its warps
+constexpr int kMinRounds = 3;               // a CTA's share is at least so many: fewer partial results to join
+constexpr int kRowsMax = 8;                 // query rows
+
+template <int D>
+struct Ring4 {
+  static constexpr int G = D / 32;
+  static constexpr int kChunks = D / 32;                    // 16-byte pieces of a row
+  static constexpr uint32_t kPlane = kStep * D / 2;         // keys, then values
+  static constexpr uint32_t kStage = 2 * kPlane + 2 * kStep * 4;        // and their scale words
+  static constexpr int kStages = D == 128 ? 3 : 6;
+  // a step's scales as its products take them: of keys in 32 bits, of values in fp16 relative to E
+  static constexpr uint32_t kKeyScale = kStep * G * 4, kTable = kKeyScale + kStep * G * 2;
+  static constexpr uint32_t kWarpBytes = kStages * kStage + kTable;
+  static constexpr int kJoin = (D / 16 * 4 + 4) * 32;       // a warp's O, m, l as floats
+  static constexpr uint32_t kBytes = kWarps * kWarpBytes, kJoinBytes = kWarps * kJoin * 4;
+  static constexpr uint32_t kSmemBytes = (kBytes > kJoinBytes ? kBytes : kJoinBytes) + 512;
+  static_assert(kSmemBytes <= 232448, "exceeds the 227 KB of shared memory a CTA can have");
+};
+
+// Token of the 16 (of the 8) that row i of a product is: pairs (2 c, 2 c + 1) of rows are the pairs of tokens that a lane takes
+// of the values, and with these the eight lanes that read together find their pieces in different banks.
+__device__ __forceinline__ int token_of(int i) { return i ^ (i >> 1 & 1); }
+// Where piece c of 16 bytes of token row r is kept.
+template <int D>
+__device__ __forceinline__ int piece(int r, int c) { return D == 128 ? c ^ ((r >> 2 & 1) << 1) : c; }
+
+// 2^(b - 127), and 2^d (0 from -127 down).
+__device__ __forceinline__ float pow2_of(uint32_t b) { return __uint_as_float(b == 0u ? 0x00400000u : b << 23); }
+__device__ __forceinline__ float pow2(int d) { return __uint_as_float(uint32_t(min(max(127 + d, 0), 254)) << 23); }
+
+// fp16 reads: what the value pair h of scale byte b stands for as fp16 has it (subnormals rounded, past the range the
+// largest), divided by the scale of byte `held(b)`.
+__device__ __forceinline__ uint32_t held(uint32_t b) { return min(max(b, 104u), 140u); }
+__device__ __forceinline__ uint32_t as_fp16(uint32_t h, uint32_t b_lo, uint32_t b_hi) {
+  auto one = [](__half x, uint32_t b) {
+    const int by = int(b) - int(held(b));
+    if (by > 0) return __hmin(__hmax(__hmul(x, __float2half_rn(pow2(min(by, 15)))),
+                                     __ushort_as_half(0xc7ffu)), __ushort_as_half(0x47ffu));        // 65504 / 2^13
+    if (by < 0) {                             // to multiples of a half: fp16's smallest number over 2^-23
+      const __half y = __hmul(x, __float2half_rn(pow2(max(by, -24))));
+      return __hsub(__hadd(y, __ushort_as_half(0x6200u)), __ushort_as_half(0x6200u));
+    }
+    return x;
+  };
+  const __half2 x = reinterpret_cast<const __half2&>(h);
+  const __half2 y = __halves2half2(one(__low2half(x), b_lo), one(__high2half(x), b_hi));
+  return reinterpret_cast<const uint32_t&>(y);
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_constant__ ChunkArgs a, bool vec_out) {
+  using Rg = Ring4<D>;
+  constexpr int G = Rg::G, CH = Rg::kChunks, kRowsPerCopy = 32 / CH, kCopies = kStep / kRowsPerCopy;
+  constexpr int kOut = D / 16;                // products of O: two per group
+  constexpr int kTiles = kStep / 16;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r8 = lane >> 2, c4 = lane & 3;
+  Sched& sched = *reinterpret_cast<Sched*>(smem + Rg::kSmemBytes - 512);
+  const int cta = blockIdx.x, n_cta = gridDim.x;
+  const uint32_t ring = smem_u32(smem) + warp * Rg::kWarpBytes, table_at = ring + Rg::kStages * Rg::kStage;
+  const unsigned full = 0xffffffffu;
+  const float ninf = -__int_as_float(0x7f800000);
+  const Parts ps = few_parts(a.workspace, n_cta);
+  pdl_trigger();
+  if (threadIdx.x == 0) {
+    sched.share = Share{0, 0, a.R};
+    sched.bad_v = 0;
+    ps.desc[cta].valid = 0;
+  }
+  __syncthreads();
+  const int HG = a.Hkv % 8 == 0 ? 8 : (a.Hkv % 4 == 0 ? 4 : (a.Hkv % 2 == 0 ? 2 : 1));   // heads per unit
+  const int wph = kWarps / HG, round = kStep * wph;         // warps per head, tokens of a round of theirs
+  const int my_head = warp % HG, my_part = warp / HG;
+  const int few_rows = few_rows_now<kThreads>(a, sched.sums);
+  if (few_rows == 0) return;
+  share_out<kThreads>(a.R, [&](int r) -> int64_t {
+    const int A = new_tokens(a, r), S = a.seq_used[r];
+    if (A == 0 || A * a.G > few_rows) return 0;
+    flag_long(a, S);
+    return int64_t(a.Hkv / HG) * (kRoundCost + (held_tokens(a, S) + round - 1) / round);
+  }, sched.share, sched.scan, cta, n_cta, kMinRounds);
+  const int64_t total = sched.share.total;
+  const int n_used = used_ctas(total, n_cta, kMinRounds);
+  const int64_t lo = total * cta / n_used, hi = total * (cta + 1) / n_used;
+  if (cta >= n_used || lo >= hi) return;
+  int r = sched.share.r0;
+  int64_t at = sched.share.pre;              // start of (session r, head group hg) in the schedule
+  int hg = 0;
+  bool seek = true;
+  const float c2 = a.scale * kLog2e;
+  const char* kv = static_cast<const char*>(a.kv);
+  const int64_t stride_s = a.kv_stride_s, stride_b = a.kv_stride_b, to_values = a.kv_stride_kv;
+  const int shift = (a.BS & (a.BS - 1)) == 0 ? __ffs(a.BS) - 1 : -1;
+  auto block_of = [&](int tok) { return shift >= 0 ? tok >> shift : tok / a.BS; };
+
+  for (; r < a.R && at < hi; ++r, hg = 0) {
+    const int a0 = a.q_off[r], A = new_tokens(a, r), S = a.seq_used[r];
+    if (A == 0 || A * a.G > few_rows) continue;
+    const int rows = A * a.G;
+    const int nt = (held_tokens(a, S) + round - 1) / round;
+    const int64_t weight = kRoundCost + nt;
+    if (seek) {                               // the group that holds lo
+      hg = int((lo - at) / weight);
+      at += hg * weight;
+      seek = false;
+    }
+    const int32_t* table = a.block_table + r * a.bt_stride_r;
+    for (; hg < a.Hkv / HG && at < hi; ++hg, at += weight) {
+      const int64_t first = at + kRoundCost;
+      const int t0 = int(lo > first ? lo - first : 0), t1 = nt == 0 ? 0 : int(min(int64_t(nt), hi - first));
+      if (nt == 0 ? at < lo : t0 >= t1) continue;
+      const int h = hg * HG + my_head;
+      const int begin = t0 * round, end = min(t1 * round, held_tokens(a, S));
+      const int start = begin + my_part * kStep;              // this warp's steps: start, start + round, ...
+      const int mine = start < end ? (end - start + round - 1) / round : 0;
+      // the lane's two query rows, and the last tokens they see
+      const int row0 = 2 * c4, row1 = row0 + 1;
+      const int lim0 = S - A + row0 / a.G, lim1 = S - A + row1 / a.G;
+      // ---- queries as the second operand, row r8: of k-step (group g, i) dims 32 g + 8 c4 + 4 i .. + 3
+      uint32_t q[2 * G][2];
+      {
+        const int jq = r8 / a.G;
+        const uint16_t* p = static_cast<const uint16_t*>(a.q) + (int64_t(a0) + jq) * a.q_stride_t +
+                            int64_t(h * a.G + r8 - jq * a.G) * a.q_stride_h;
+#pragma unroll
+        for (int k = 0; k < 2 * G; ++k) {
+          const uint2 u = r8 < rows ? *reinterpret_cast<const uint2*>(p + 32 * (k >> 1) + 8 * c4 + 4 * (k & 1)) : make_uint2(0u, 0u);
+          q[k][0] = u.x;
+          q[k][1] = u.y;
+        }
+      }
+      // what undoes the queries' power of two, for rows row0 and row1
+      float qs0 = 1.0f, qs1 = 1.0f;
+      if constexpr (BF16) {
+        uint32_t top = 0;                     // the row's largest finite value, by its bits
+#pragma unroll
+        for (int k = 0; k < 2 * G; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t x = q[k][e] & 0x7fffu, y = q[k][e] >> 16 & 0x7fffu;
+            top = max(top, max(x < 0x7f80u ? x : 0u, y < 0x7f80u ? y : 0u));
+          }
+        top = max(top, __shfl_xor_sync(full, top, 1));
+        top = max(top, __shfl_xor_sync(full, top, 2));
+        const int by = min(141 - int(top >> 7), 126);
+        const float f = pow2(by), back = pow2(-by);
+#pragma unroll
+        for (int k = 0; k < 2 * G; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            q[k][e] = pack2<false>(__uint_as_float(q[k][e] << 16) * f, __uint_as_float(q[k][e] & 0xffff0000u) * f);
+        qs0 = __shfl_sync(full, back, 4 * row0);
+        qs1 = __shfl_sync(full, back, 4 * row1);
+      }
+      const float cq0 = c2 * qs0, cq1 = c2 * qs1;
+      float o[kOut][4];
+#pragma unroll
+      for (int j = 0; j < kOut; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
+      float m0 = ninf, m1 = ninf, l0 = 0.0f, l1 = 0.0f;
+      // by group (a byte each), what O is relative to, 2^(E - 127), for the two rows; equal until tokens are added one by one
+      uint32_t E0 = 0, E1 = 0;
+      auto byte_of = [](uint32_t w, int g) { return int(w >> (8 * g) & 255u); };
+
+      // ---- copies of step i of this warp: a lane looks up its token's block a step ahead
+      auto look_up = [&](int i) -> int {
+        const int tok = start + i * round + lane;
+        if (i >= mine || tok >= end) return -1;
+        const int lb = block_of(tok);
+        return lb < a.MB ? table[lb] : -1;
+      };
+      int phys = look_up(0);
+      const char* head = kv + int64_t(h) * (D / 2);
+      const int at_word = a.Hkv * (D / 2) + (D == 128 ? h * 4 : (h * 2) & ~3);
+      const int sh = D == 64 && (h & 1) ? 16 : 0;             // the head's bytes within the word
+      bool gaps = false;                      // this lane met a block outside the cache: from there on every step looks
+      auto issue = [&](int i, int slot) {
+        if (i < mine) {
+          const int tok = start + i * round + lane;
+          const bool none = uint32_t(phys) >= uint32_t(a.NB); // past the end, or an id outside the cache: zeros
+          if (none && tok < end) {
+            flag(a.status, ACTKV_DEV_BAD_INDEX);
+            gaps = true;
+          }
+          const int in_block = shift >= 0 ? tok & (a.BS - 1) : tok % a.BS;
+          const int64_t off = none ? -1 : int64_t(phys) * stride_b + int64_t(in_block) * stride_s;
+          const uint32_t dst = ring + slot * Rg::kStage;
+#pragma unroll
+          for (int e = 0; e < kCopies; ++e) {
+            const int row = e * kRowsPerCopy + lane / CH, c = lane % CH;
+            const int64_t from = __shfl_sync(full, off, row);
+            const char* p = (from < 0 ? kv : head + from) + c * 16;
+            const uint32_t to = dst + row * (CH * 16) + piece<D>(row, c) * 16;
+            copy16(to, p, from >= 0);
+            copy16(to + Rg::kPlane, p + to_values, from >= 0);
+          }
+          const char* w = kv + (off < 0 ? 0 : off + at_word);
+          copy4(dst + 2 * Rg::kPlane + lane * 4, w, off >= 0);
+          copy4(dst + 2 * Rg::kPlane + kStep * 4 + lane * 4, w + to_values, off >= 0);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        phys = look_up(i + 1);
+      };
+
+      // the references of rows that have outgrown theirs go up to the maxima given (the same in all lanes of a row; each
+      // row by its own tokens alone, so that what others see does not show in its digits)
+      auto raise = [&](float top0, float top1) {
+        const float n0 = top0 > m0 + kSlack ? top0 : m0, n1 = top1 > m1 + kSlack ? top1 : m1;
+        const float e0 = m0 == n0 ? 1.0f : ex2(m0 - n0), e1 = m1 == n1 ? 1.0f : ex2(m1 - n1);
+        m0 = n0;
+        m1 = n1;
+        l0 *= e0;
+        l1 *= e1;
+#pragma unroll
+        for (int j = 0; j < kOut; ++j) {
+          o[j][0] *= e0;
+          o[j][1] *= e1;
+          o[j][2] *= e0;
+          o[j][3] *= e1;
+        }
+      };
+      // ... and the scales' references
+      auto raise_scale = [&](uint32_t n0, uint32_t n1) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const float e0 = pow2(byte_of(E0, g) - byte_of(n0, g)), e1 = pow2(byte_of(E1, g) - byte_of(n1, g));
+#pragma unroll
+          for (int j = 2 * g; j < 2 * g + 2; ++j) {
+            o[j][0] *= e0;
+            o[j][1] *= e1;
+            o[j][2] *= e0;
+            o[j][3] *= e1;
+          }
+        }
+        E0 = n0;
+        E1 = n1;
+      };
+      auto step = [&](int i, int slot, uint32_t wk, uint32_t wv, auto edge_) {
+        constexpr bool EDGE = decltype(edge_)::value;        // hidden tokens, or scale bytes out of the ordinary
+        const int t = start + i * round;
+        const uint32_t kb = ring + slot * Rg::kStage, vb = kb + Rg::kPlane, sb = kb + 2 * Rg::kPlane;
+        // the step's tokens that are there (neither past the end nor in a block outside the cache), and those of them
+        // that every row sees
+        [[maybe_unused]] uint32_t there = full, common = full;
+        if constexpr (EDGE) {
+          bool here = t + lane < end;
+          if (__any_sync(full, gaps) && here) {
+            const int lb = block_of(t + lane);
+            here = lb < a.MB && uint32_t(table[lb]) < uint32_t(a.NB);
+          }
+          there = __ballot_sync(full, here);
+          common = there & __ballot_sync(full, t + lane <= S - A);
+        }
+        // ---- the lane's token: its scales into the tables
+        {
+          float ks[G];
+          uint32_t vs = wv;                   // of the values, the bytes that count: 0 for what is not of all rows, and for NaN
+          if constexpr (EDGE) {
+            vs = 0;
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+              uint32_t b = byte_of(wv, g);
+              if (b >= kNan4 && (there >> lane & 1u)) atomicOr(&sched.bad_v, 2);   // it comes back when the unit ends
+              if (b < kNan4 && (common >> lane & 1u)) vs |= (BF16 ? b : held(b)) << (8 * g);
+            }
+          }
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            uint32_t b = byte_of(wk, g);
+            if constexpr (EDGE && !BF16)
+              if (b < kNan4) b = held(b);
+            ks[g] = EDGE && b >= kNan4 ? __int_as_float(0x7fffffff) : pow2_of(b);
+          }
+          if (__any_sync(full, __vcmpgtu4(vs, E0) != 0)) {    // (E0 and E1 are equal where some token is common)
+            uint32_t n = __vmaxu4(vs, E0);
+#pragma unroll
+            for (int x = 1; x < 32; x *= 2) n = __vmaxu4(n, __shfl_xor_sync(full, n, x));
+            raise_scale(n, n);
+          }
+          if constexpr (G == 4)
+            *reinterpret_cast<float4*>(smem + (table_at - smem_u32(smem)) + lane * 16) = make_float4(ks[0], ks[1], ks[2], ks[3]);
+          else
+            *reinterpret_cast<float2*>(smem + (table_at - smem_u32(smem)) + lane * 8) = make_float2(ks[0], ks[1]);
+          uint32_t f[G / 2];
+#pragma unroll
+          for (int g = 0; g < G; g += 2) {
+            float x[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              x[e] = pow2(byte_of(vs, g + e) - byte_of(E0, g + e));
+              if (EDGE && ((common >> lane & 1u) == 0 || byte_of(wv, g + e) >= int(kNan4))) x[e] = 0.0f;
+            }
+            f[g / 2] = pack2<false>(x[0], x[1]);
+          }
+          uint8_t* ft = smem + (table_at - smem_u32(smem)) + Rg::kKeyScale;
+          if constexpr (G == 4) *reinterpret_cast<uint2*>(ft + lane * 8) = make_uint2(f[0], f[G / 2 - 1]);
+          else *reinterpret_cast<uint32_t*>(ft + lane * 4) = f[0];
+        }
+        __syncwarp();
+        // ---- S^T = K Q^T: s[n][0..1] token 16 n + token_of(r8), s[n][2..3] the one 8 on, query rows 2 c4 and 2 c4 + 1
+        float s[kTiles][4];
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+          const int tk0 = 16 * n + token_of(r8), tk1 = tk0 + 8;
+          uint32_t w[2][4];                   // by token: words of pieces 2 c4 and 2 c4 + 1
+          float ks[2][G];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int tk = e ? tk1 : tk0;
+            if constexpr (D == 128) {
+              const uint4 u = lds16(kb + tk * 64 + piece<D>(tk, c4) * 16);
+              w[e][0] = u.x;
+              w[e][1] = u.y;
+              w[e][2] = u.z;
+              w[e][3] = u.w;
+              const uint4 f = lds16(table_at + tk * 16);
+              ks[e][0] = __uint_as_float(f.x);
+              ks[e][1] = __uint_as_float(f.y);
+              ks[e][G - 2] = __uint_as_float(f.z);
+              ks[e][G - 1] = __uint_as_float(f.w);
+            } else {
+              const uint2 u = lds8(kb + tk * 32 + c4 * 8);
+              w[e][0] = u.x;
+              w[e][1] = u.y;
+              const uint2 f = lds8(table_at + tk * 8);
+              ks[e][0] = __uint_as_float(f.x);
+              ks[e][1] = __uint_as_float(f.y);
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
+#pragma unroll
+          for (int g2 = 0; g2 < G / 2; ++g2) {
+            // of two groups: x[token][piece][byte]
+            uint32_t x[2][2][4];
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+              for (int pc = 0; pc < 2; ++pc)
+                e2m1x8_f16(w[e][pc * (G / 2) + g2], x[e][pc][0], x[e][pc][1], x[e][pc][2], x[e][pc][3]);
+#pragma unroll
+            for (int gg = 0; gg < 2; ++gg) {
+              const int g = 2 * g2 + gg;
+              if constexpr (EDGE && !BF16) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const uint32_t b = lds4(sb + (e ? tk1 : tk0) * 4) >> (sh + 8 * g) & 255u;
+#pragma unroll
+                  for (int pc = 0; pc < 2; ++pc)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) x[e][pc][2 * gg + k] = as_fp16(x[e][pc][2 * gg + k], b, b);
+                }
+              }
+              float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+              for (int pc = 0; pc < 2; ++pc) {
+                const uint32_t m[4] = {x[0][pc][2 * gg], x[1][pc][2 * gg], x[0][pc][2 * gg + 1], x[1][pc][2 * gg + 1]};
+                mma16816<false>(c, m, q[2 * g + pc][0], q[2 * g + pc][1]);
+              }
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float k = ks[e >> 1][g];
+                // (powers of two: the same digits either way, but a scale of any size stays in range)
+                s[n][e] = EDGE ? fmaf(c[e], k * (e & 1 ? qs1 : qs0), s[n][e]) : fmaf(c[e], k, s[n][e]);
+              }
+            }
+          }
+          if constexpr (EDGE) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int tk = e >> 1 ? tk1 : tk0;
+              s[n][e] = t + tk <= (e & 1 ? lim1 : lim0) && (there >> tk & 1u) ? s[n][e] : ninf;
+            }
+          }
+        }
+        // (the product rounded before the difference, not in one step with it: the largest logit's is then 0 whatever its size)
+        const float f0 = EDGE ? c2 : cq0, f1 = EDGE ? c2 : cq1;
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][e] = __fmul_rn(s[n][e], e & 1 ? f1 : f0);
+        float top0 = fmaxf(s[0][0], s[0][2]), top1 = fmaxf(s[0][1], s[0][3]);
+#pragma unroll
+        for (int n = 1; n < kTiles; ++n) {
+          top0 = fmaxf(top0, fmaxf(s[n][0], s[n][2]));
+          top1 = fmaxf(top1, fmaxf(s[n][1], s[n][3]));
+        }
+        if (__any_sync(full, top0 > m0 + kSlack || top1 > m1 + kSlack)) {
+#pragma unroll
+          for (int x = 4; x < 32; x *= 2) {
+            top0 = fmaxf(top0, __shfl_xor_sync(full, top0, x));
+            top1 = fmaxf(top1, __shfl_xor_sync(full, top1, x));
+          }
+          raise(top0, top1);
+        }
+        const float b0 = m0 == ninf ? 0.0f : m0, b1 = m1 == ninf ? 0.0f : m1;
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][e] = ex2(__fsub_rn(s[n][e], e & 1 ? b1 : b0));
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+          l0 += s[n][0] + s[n][2];
+          l1 += s[n][1] + s[n][3];
+        }
+        // ---- O^T += V^T p^T: the lane's tokens are those of rows 2 c4, 2 c4 + 1 and 8 on, its dims 4 r8 .. + 3 of each group
+        if (!EDGE || common) {
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n) {
+            const uint32_t p0 = transpose8x8(pack_p<false>(s[n][0], s[n][1])), p1 = transpose8x8(pack_p<false>(s[n][2], s[n][3]));
+            const int tok[4] = {16 * n + token_of(2 * c4), 16 * n + token_of(2 * c4 + 1), 16 * n + 8 + token_of(2 * c4),
+                                16 * n + 8 + token_of(2 * c4 + 1)};
+            uint32_t vw[4][G / 2], ft[4][G / 2];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if constexpr (D == 128) {
+                const uint2 u = lds8(vb + tok[e] * 64 + piece<D>(tok[e], r8 >> 1) * 16 + (r8 & 1) * 8);
+                vw[e][0] = u.x;
+                vw[e][G / 2 - 1] = u.y;
+                const uint2 f = lds8(table_at + Rg::kKeyScale + tok[e] * 8);
+                ft[e][0] = f.x;
+                ft[e][G / 2 - 1] = f.y;
+              } else {
+                vw[e][0] = lds4(vb + tok[e] * 32 + r8 * 4);
+                ft[e][0] = lds4(table_at + Rg::kKeyScale + tok[e] * 4);
+              }
+            }
+#pragma unroll
+            for (int g2 = 0; g2 < G / 2; ++g2) {
+              // two tokens' half bytes of a dim next to one another: even dims, odd dims; x[pair][odd][byte]
+              uint32_t x[2][2][4];
+#pragma unroll
+              for (int pr = 0; pr < 2; ++pr) {
+                const uint32_t u = vw[2 * pr][g2], v = vw[2 * pr + 1][g2];
+                const uint32_t even = (u & 0x0f0f0f0fu) | ((v << 4) & 0xf0f0f0f0u);
+                const uint32_t odd = ((u >> 4) & 0x0f0f0f0fu) | (v & 0xf0f0f0f0u);
+                e2m1x8_f16(even, x[pr][0][0], x[pr][0][1], x[pr][0][2], x[pr][0][3]);
+                e2m1x8_f16(odd, x[pr][1][0], x[pr][1][1], x[pr][1][2], x[pr][1][3]);
+              }
+#pragma unroll
+              for (int gg = 0; gg < 2; ++gg) {
+                const int g = 2 * g2 + gg;
+                if constexpr (EDGE && !BF16) {
+#pragma unroll
+                  for (int pr = 0; pr < 2; ++pr) {
+                    const uint32_t b_lo = lds4(sb + (kStep + tok[2 * pr]) * 4) >> (sh + 8 * g) & 255u;
+                    const uint32_t b_hi = lds4(sb + (kStep + tok[2 * pr + 1]) * 4) >> (sh + 8 * g) & 255u;
+#pragma unroll
+                    for (int od = 0; od < 2; ++od)
+#pragma unroll
+                      for (int k = 0; k < 2; ++k) x[pr][od][2 * gg + k] = as_fp16(x[pr][od][2 * gg + k], b_lo, b_hi);
+                  }
+                }
+                const uint32_t sel = gg ? 0x7632 : 0x5410;
+                const uint32_t pg0 = mul16x2<false>(p0, __byte_perm(ft[0][g2], ft[1][g2], sel));
+                const uint32_t pg1 = mul16x2<false>(p1, __byte_perm(ft[2][g2], ft[3][g2], sel));
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                  const uint32_t m[4] = {x[0][0][2 * gg + k], x[0][1][2 * gg + k], x[1][0][2 * gg + k], x[1][1][2 * gg + k]};
+                  mma16816<false>(o[2 * g + k], m, pg0, pg1);
+                }
+              }
+            }
+          }
+        }
+        // ---- tokens that some row does not see, one by one
+        if constexpr (EDGE) {
+#pragma unroll 1
+          for (uint32_t some = there & ~common; some; some &= some - 1) {
+            const int tk = __ffs(some) - 1, of = tk & 7;
+            // p of the lane's two rows: from the lanes of the product's row that the token is
+            float x0 = 0.0f, x1 = 0.0f;
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if ((tk >> 3) == 2 * n + e) {
+                  x0 = s[n][2 * e];
+                  x1 = s[n][2 * e + 1];
+                }
+            x0 = __shfl_sync(full, x0, token_of(of) * 4 + c4) * kPScale<false>;
+            x1 = __shfl_sync(full, x1, token_of(of) * 4 + c4) * kPScale<false>;
+            const bool see0 = t + tk <= lim0, see1 = t + tk <= lim1;
+            const uint32_t word = lds4(sb + (kStep + tk) * 4) >> sh;
+            uint32_t seen = 0;                // its scale bytes, NaN without
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+              const uint32_t b = byte_of(word, g);
+              if (b < kNan4) seen |= (BF16 ? b : held(b)) << (8 * g);
+            }
+            raise_scale(see0 ? __vmaxu4(E0, seen) : E0, see1 ? __vmaxu4(E1, seen) : E1);
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+              const uint32_t b = byte_of(word, g);
+              if (b >= kNan4) continue;
+              const int by0 = byte_of(seen, g) - byte_of(E0, g), by1 = byte_of(seen, g) - byte_of(E1, g);
+              const float g0 = see0 ? x0 * pow2(by0) : 0.0f, g1 = see1 ? x1 * pow2(by1) : 0.0f;
+              // the lane's four dims of the group: two bytes of piece r8
+              const uint32_t byte_at = D == 128 ? tk * 64 + piece<D>(tk, r8 >> 1) * 16 + (r8 & 1) * 8 : tk * 32 + r8 * 4;
+              const uint32_t two = lds4(vb + byte_at + (g >> 1) * 4) >> (16 * (g & 1));
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                uint32_t v = e2m1x2_f16(two >> (8 * k) & 255u);
+                if constexpr (!BF16) v = as_fp16(v, b, b);
+                const float2 y = f16x2_f32(v);
+                o[2 * g + k][0] = fmaf(g0, y.x, o[2 * g + k][0]);
+                o[2 * g + k][1] = fmaf(g1, y.x, o[2 * g + k][1]);
+                o[2 * g + k][2] = fmaf(g0, y.y, o[2 * g + k][2]);
+                o[2 * g + k][3] = fmaf(g1, y.y, o[2 * g + k][3]);
+              }
+            }
+          }
+        }
+      };
+
+      // ---- the steps
+      constexpr int kAhead = Rg::kStages - 1;
+#pragma unroll 1
+      for (int i = 0; i < kAhead; ++i) issue(i, i);
+      int slot = 0, fill = kAhead;
+#pragma unroll 1
+      for (int i = 0; i < mine; ++i) {
+        issue(i + kAhead, fill);
+        asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+        __syncwarp();
+        const int t = start + i * round;
+        const uint32_t sb = ring + slot * Rg::kStage + 2 * Rg::kPlane;
+        uint32_t wk = lds4(sb + lane * 4) >> sh, wv = lds4(sb + (kStep + lane) * 4) >> sh;
+        if constexpr (D == 64) {
+          wk &= 0xffffu;
+          wv &= 0xffffu;
+        }
+        bool odd;
+        if constexpr (BF16) odd = ((wk & (wk << 1)) | (wv & (wv << 1))) & 0x80808080u;
+        else odd = __vcmpgtu4(wk, 0x8c8c8c8cu) | __vcmpgtu4(wv, 0x8c8c8c8cu) |
+                   ((__vcmpgtu4(0x68686868u, wk) | __vcmpgtu4(0x68686868u, wv)) & (D == 64 ? 0xffffu : 0xffffffffu));
+        if (t + kStep - 1 > S - A || t + kStep > end || __any_sync(full, odd || gaps)) step(i, slot, wk, wv, std::true_type());
+        else step(i, slot, wk, wv, std::false_type());
+        __syncwarp();                         // every lane has read the slot that the next copies fill, and the tables
+        slot = slot + 1 == Rg::kStages ? 0 : slot + 1;
+        fill = fill + 1 == Rg::kStages ? 0 : fill + 1;
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      // ---- results: l of a row over the lanes that share it; O as the sums of p v (of 2^7 p v in fp16) that the join takes
+#pragma unroll
+      for (int x = 4; x < 32; x *= 2) {
+        l0 += __shfl_xor_sync(full, l0, x);
+        l1 += __shfl_xor_sync(full, l1, x);
+      }
+      {
+        constexpr float kBack = BF16 ? 1.0f / kPScale<false> : 1.0f;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const float y0 = pow2_of(byte_of(E0, g)), y1 = pow2_of(byte_of(E1, g));
+#pragma unroll
+          for (int j = 2 * g; j < 2 * g + 2; ++j) {
+            o[j][0] = o[j][0] * kBack * y0;
+            o[j][1] = o[j][1] * kBack * y1;
+            o[j][2] = o[j][2] * kBack * y0;
+            o[j][3] = o[j][3] * kBack * y1;
+          }
+        }
+      }
+      const bool whole = t0 == 0 && t1 == nt;
+      const int ps_slot = t0 > 0 ? 0 : 1;
+      __syncthreads();                        // the rings are free, and every warp's NaN groups are known
+      if (wph > 1) {                          // the warps of a head meet through shared memory, the first goes on
+        float* jo = reinterpret_cast<float*>(smem) + warp * Rg::kJoin;
+        if (my_part > 0) {
+#pragma unroll
+          for (int j = 0; j < kOut; ++j)
+            *reinterpret_cast<float4*>(jo + (j * 32 + lane) * 4) = make_float4(o[j][0], o[j][1], o[j][2], o[j][3]);
+          *reinterpret_cast<float4*>(jo + (kOut * 32 + lane) * 4) = make_float4(m0, l0, m1, l1);
+        }
+        __syncthreads();
+        if (my_part == 0)
+#pragma unroll 1
+          for (int w = warp + HG; w < kWarps; w += HG) {
+            const float4* po = reinterpret_cast<const float4*>(smem) + w * (Rg::kJoin / 4);
+            const float4 y = po[kOut * 32 + lane];
+            const float M0 = fmaxf(m0, y.x), M1 = fmaxf(m1, y.z);
+            // an empty side (sum 0) counts for nothing; a NaN sum stays
+            const float p0 = l0 == 0.0f ? 0.0f : (m0 == M0 ? 1.0f : ex2(m0 - M0)), q0 = y.y == 0.0f ? 0.0f : (y.x == M0 ? 1.0f : ex2(y.x - M0));
+            const float p1 = l1 == 0.0f ? 0.0f : (m1 == M1 ? 1.0f : ex2(m1 - M1)), q1 = y.w == 0.0f ? 0.0f : (y.z == M1 ? 1.0f : ex2(y.z - M1));
+            m0 = M0;
+            m1 = M1;
+            l0 = fmaf(l0, p0, y.y * q0);
+            l1 = fmaf(l1, p1, y.w * q1);
+#pragma unroll
+            for (int j = 0; j < kOut; ++j) {
+              const float4 x = po[j * 32 + lane];
+              o[j][0] = fmaf(o[j][0], p0, x.x * q0);
+              o[j][1] = fmaf(o[j][1], p1, x.y * q1);
+              o[j][2] = fmaf(o[j][2], p0, x.z * q0);
+              o[j][3] = fmaf(o[j][3], p1, x.w * q1);
+            }
+          }
+      }
+      if (my_part == 0) {
+        const int fix = *reinterpret_cast<volatile int*>(&sched.bad_v);
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const int row = hf ? row1 : row0;
+          if (row >= rows) continue;
+          const float L = hf ? l1 : l0, M = hf ? m1 : m0, inv = over<BF16>(L);
+          const int jq = row / a.G, hq = h * a.G + row - jq * a.G, hr = my_head * rows + row;
+          const int64_t qt = int64_t(a0) + jq;
+          uint16_t* dst = static_cast<uint16_t*>(a.out) + qt * a.out_stride_t + int64_t(hq) * a.out_stride_h;
+          float* part = ps.out(cta, ps_slot) + int64_t(hr) * D;
+          // NaN groups among the values of tokens that this row does see
+          uint32_t nan = 0;
+          if (fix) {
+            const int last = min(S - A + jq, end - 1);
+#pragma unroll 1
+            for (int t = begin; t <= last; ++t) {
+              const int lb = block_of(t), ph = lb < a.MB ? table[lb] : -1;
+              if (ph < 0 || ph >= a.NB) continue;
+              const uint8_t* p = reinterpret_cast<const uint8_t*>(kv) + to_values + int64_t(ph) * stride_b +
+                                 int64_t(t - lb * a.BS) * stride_s + a.Hkv * (D / 2) + h * G;
+#pragma unroll
+              for (int g = 0; g < G; ++g) nan |= p[g] >= kNan4 ? 1u << g : 0u;
+            }
+          }
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            const int d0 = 32 * g + 4 * r8;
+            float y[4] = {o[2 * g][hf], o[2 * g][2 + hf], o[2 * g + 1][hf], o[2 * g + 1][2 + hf]};
+            if (nan >> g & 1u) y[0] = y[1] = y[2] = y[3] = __int_as_float(0x7fffffff);
+            if (whole) {
+              const uint32_t u0 = pack2<BF16>(y[0] * inv, y[1] * inv), u1 = pack2<BF16>(y[2] * inv, y[3] * inv);
+              if (vec_out) {
+                *reinterpret_cast<uint2*>(dst + d0) = make_uint2(u0, u1);
+              } else {
+                dst[d0] = uint16_t(u0);
+                dst[d0 + 1] = uint16_t(u0 >> 16);
+                dst[d0 + 2] = uint16_t(u1);
+                dst[d0 + 3] = uint16_t(u1 >> 16);
+              }
+            } else {
+              *reinterpret_cast<float4*>(part + d0) = make_float4(y[0], y[1], y[2], y[3]);
+            }
+          }
+          if (r8 == 0) {
+            if (whole)
+              a.lse[qt * a.lse_stride_t + hq] = L == 0.0f ? ninf : (M == ninf ? L : (M + log2f(L)) * 0.69314718055994531f);
+            else
+              *reinterpret_cast<float2*>(ps.ml(cta, ps_slot, D) + 2 * hr) = make_float2(M, L);
+          }
+        }
+      }
+      if (!whole && t0 == 0 && threadIdx.x == 0) {
+        Desc ds = {};
+        ds.valid = 1;
+        ds.r = r;
+        ds.h = hg * HG;
+        ds.heads = HG;
+        ds.n_used = n_used;
+        ds.ntok = A;
+        ds.S = S;
+        ds.A = A;
+        ds.a0 = a0;
+        ds.end = first + nt;
+        ds.total = total;
+        ps.desc[cta] = ds;
+      }
+      __syncthreads();                        // the rings are written again
+    }
+  }
+}
+
+}  // namespace four
+}  // namespace few
+}  // namespace chunk
+
+namespace {
+
+template <int D, bool BF16>
+cudaError_t launch_few4_t(const ChunkArgs& a, int grid, cudaStream_t st) {
+  auto k = chunk::few::four::chunk_few4_kernel<D, BF16>;
+  constexpr int bytes = int(chunk::few::four::Ring4<D>::kSmemBytes);
+  static SmemLimit limit;
+  const cudaError_t e = limit.set(reinterpret_cast<const void*>(k), bytes);
+  if (e != cudaSuccess) return e;
+  const bool vec_out = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_stride_t % 8 == 0 && a.out_stride_h % 8 == 0;
+  k<<<grid, chunk::few::four::kThreads, bytes, st>>>(a, vec_out);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_chunk_few4(const ChunkArgs& a, int dtype, int grid, cudaStream_t st) {
+  const bool bf = dtype == ACTKV_BF16;
+  if (a.D == 128) return bf ? launch_few4_t<128, true>(a, grid, st) : launch_few4_t<128, false>(a, grid, st);
+  return bf ? launch_few4_t<64, true>(a, grid, st) : launch_few4_t<64, false>(a, grid, st);
+}
+
+}  // namespace actkv

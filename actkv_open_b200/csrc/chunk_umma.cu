@@ -64,16 +64,18 @@ constexpr int kUnitSlots = 4;               // units announced ahead of their re
 
 constexpr uint32_t kSchedBytes = 512;
 
-template <int D, bool QUANT>
+// BITS: of the cache's values: 16, 8 or 4
+template <int D, int BITS>
 struct Layout {
+  static constexpr bool QUANT = BITS != 16;
   static constexpr int kHalves = D / 64;
   static constexpr uint32_t kTileBytes = kTile * D * 2;      // a K, V or Q tile
-  static constexpr int kSlots = QUANT ? (D == 128 ? 3 : 6) : (D == 128 ? 5 : 10);
+  static constexpr int kSlots = (BITS == 8 ? 3 : (BITS == 4 ? 4 : 5)) * (128 / D);
   static constexpr uint32_t kGroupBytes = kHalves * 1024;    // 8 tokens of a K / V tile
   static constexpr uint32_t kKvOff = 2 * kTileBytes;
-  // the 8-bit cache's tiles before they are widened, and their scale words per token
+  // the 8- or 4-bit cache's tiles before they are widened, and their scale words per token
   static constexpr int kRaw = QUANT ? (D == 128 ? 3 : 6) : 0;
-  static constexpr uint32_t kRawBytes = kTile * D;
+  static constexpr uint32_t kRawBytes = kTile * D * BITS / 8;
   static constexpr uint32_t kRawOff = kKvOff + kSlots * kTileBytes;
   static constexpr uint32_t kScaleOff = kRawOff + kRaw * kRawBytes;
   static constexpr uint32_t kMlOff = kScaleOff + kRaw * kTile * 4;       // stream 1's (m, l) per row
@@ -429,11 +431,12 @@ __device__ __forceinline__ void clean_values(uint8_t* tile, bool past, bool hidd
 }
 
 // ------------------------------------------------------------------------------------ the kernel
-template <int D, bool BF16, bool QUANT>
-__global__ void __launch_bounds__(threads(QUANT), 1)
+template <int D, bool BF16, int BITS>
+__global__ void __launch_bounds__(threads(BITS != 16), 1)
     chunk_umma_kernel(const __grid_constant__ CUtensorMap tmap_kv, const __grid_constant__ CUtensorMap tmap_q,
                       const __grid_constant__ ChunkArgs a, bool vec_out) {
-  using Ly = Layout<D, QUANT>;
+  using Ly = Layout<D, BITS>;
+  constexpr bool QUANT = BITS != 16;
   extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = smem_u32(smem);
@@ -524,7 +527,7 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
     const int bs_box = min(a.BS, kTile);         // token rows of a box
     const int bpt = kTile / bs_box;              // boxes per tile (<= 16: one per lane)
     const int mpb = a.BS / bs_box;               // tiles per block, of blocks longer than a tile
-    const uint32_t box_bytes = uint32_t(bs_box) * D * (QUANT ? 1 : 2);
+    const uint32_t box_bytes = uint32_t(bs_box) * D * BITS / 8;
     // where the copies go: the ring itself, or the tiles to be widened into it
     constexpr int kIn = QUANT ? Ly::kRaw : kSlots, B_FULL = QUANT ? B_RF : B_KVF, B_EMPTY = QUANT ? B_RE : B_KVE;
     Walker wk(&a, sched, cta, n_cta);
@@ -577,8 +580,8 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
         __syncwarp();
         if (id >= 0) {
           if constexpr (QUANT)
-            tma_load_3d(base + Ly::kRawOff + slot * Ly::kRawBytes + lane * box_bytes, &tmap_kv, bar(B_FULL + slot), x.h * D,
-                        id, plane);
+            tma_load_3d(base + Ly::kRawOff + slot * Ly::kRawBytes + lane * box_bytes, &tmap_kv, bar(B_FULL + slot),
+                        x.h * (D * BITS / 8), id, plane);
           else
             tma_load_5d(base + Ly::kKvOff + slot * Ly::kTileBytes + lane * box_bytes, &tmap_kv, bar(B_FULL + slot), 0, 0,
                         x.h * Ly::kHalves, id, plane);
@@ -777,7 +780,7 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
     }
     if (*abort_flag && last_bar >= 0 && lane == 0) mbar_drain(bar(last_bar), last_par);
   } else if (QUANT && warp == 2) {
-    // ------------------------------------------------------------------ scale words of the 8-bit rows
+    // ------------------------------------------------------------------ scale words of the 8- or 4-bit rows
     // Four tokens per lane, from the cache through registers (one tile ahead) into the tile's words.
     const int bpt = a.BS < kTile ? kTile / a.BS : 1, mpb = a.BS < kTile ? 1 : a.BS / kTile;
     int sub[4], in_block[4];
@@ -823,7 +826,7 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
         u.next(t, plane);
         const int block0 = mpb == 1 ? t * bpt : t / mpb, off = mpb == 1 ? 0 : (t - block0 * mpb) * kTile;
         const int32_t* table = a.block_table + u.r * a.bt_stride_r;
-        const uint8_t* p0 = static_cast<const uint8_t*>(a.kv) + plane * a.kv_stride_kv + a.Hkv * D + u.h * (D / 32);
+        const uint8_t* p0 = static_cast<const uint8_t*>(a.kv) + plane * a.kv_stride_kv + a.Hkv * (D * BITS / 8) + u.h * (D / 32);
         int phys[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -1105,7 +1108,8 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
             for (int d = 0; d < D; ++d) {
               float f;
               if constexpr (QUANT) {
-                f = quant_value<BF16>(static_cast<const uint8_t*>(a.kv) + at, a.Hkv, D, x.h * D + d);
+                if constexpr (BITS == 4) f = value4(static_cast<const uint8_t*>(a.kv) + at, a.Hkv, D, x.h, d);
+                else f = quant_value<BF16>(static_cast<const uint8_t*>(a.kv) + at, a.Hkv, D, x.h * D + d);
               } else {
                 const uint16_t u = static_cast<const uint16_t*>(a.kv)[at + int64_t(x.h) * a.kv_stride_h + d];
                 f = BF16 ? __uint_as_float(uint32_t(u) << 16) : __half2float(__ushort_as_half(u));
@@ -1157,24 +1161,25 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
     }
     fence_before();
   } else if constexpr (QUANT) {
-    // ------------------------------------------------------------------ e4m3 -> 16 bits (eight warps)
-    // A warp takes 16 of a tile's tokens, D / 16 lanes per token, and leaves them in the ring in the layout
-    // the TMA leaves 16-bit rows in.
+    // ------------------------------------------------------------------ 8 or 4 -> 16 bits (eight warps)
+    // A warp takes 16 of a tile's tokens, 16 bytes of one per lane, and leaves them in the ring in the layout the TMA
+    // leaves 16-bit rows in.
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    constexpr int kLpr = D / 16, kRpi = 32 / kLpr;
+    constexpr int kLpr = D * BITS / 128, kRpi = 32 / kLpr;   // lanes per token, tokens at a time
     const int row0 = (warp - 12) * 16, lr = lane / kLpr, lc = lane % kLpr;
     // Where a lane's piece comes from and its two 16-byte pieces go within 8 tokens.  The lanes of a token's two
     // halves write even and odd chunks first: eight banks' worth each time.
     const bool sw = D == 128 && lc >= 4;
-    uint32_t get[8 / kRpi], put0[8 / kRpi], put1[8 / kRpi];
+    constexpr int kPer8 = BITS == 8 ? 8 / kRpi : 1;
+    [[maybe_unused]] uint32_t get[kPer8], put0[kPer8], put1[kPer8];
 #pragma unroll
-    for (int i = 0; i < 8 / kRpi; ++i) {
+    for (int i = 0; i < kPer8; ++i) {
       const int r8 = i * kRpi + lr, c0 = (lc & 3) * 2;
       get[i] = r8 * D + ((lc ^ (D == 128 ? r8 : (r8 >> 1) & 3)) << 4);
       put0[i] = (lc >> 2) * 1024 + r8 * 128 + (((c0 + sw) ^ r8) << 4);
       put1[i] = (lc >> 2) * 1024 + r8 * 128 + (((c0 + 1 - sw) ^ r8) << 4);
     }
-    auto put = [&](uint8_t* p0, uint8_t* p1, const uint32_t (&r)[8]) {
+    [[maybe_unused]] auto put = [&](uint8_t* p0, uint8_t* p1, const uint32_t (&r)[8]) {
       *reinterpret_cast<uint4*>(p0) = sw ? make_uint4(r[4], r[5], r[6], r[7]) : make_uint4(r[0], r[1], r[2], r[3]);
       *reinterpret_cast<uint4*>(p1) = sw ? make_uint4(r[0], r[1], r[2], r[3]) : make_uint4(r[4], r[5], r[6], r[7]);
     };
@@ -1204,7 +1209,7 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
       uint32_t sc = reinterpret_cast<const uint32_t*>(smem + Ly::kScaleOff)[in.slot * kTile + row0 + (lane & 15)];
       const int first = t * kTile + row0;                     // the warp's first token
       const bool gap = *gaps, edge = first + 16 > min(u.S, plane ? u.hidden : u.S);
-      const bool plain = __all_sync(full, plain_scales<BF16>(sc) && !gap);
+      const bool plain = __all_sync(full, (BITS == 4 ? plain_scales4<BF16>(sc) : plain_scales<BF16>(sc)) && !gap);
       uint32_t gone = 0;                                      // the warp's tokens that are not there: zeros
       if (edge || !plain) {
         const int tok = first + (lane & 15);
@@ -1212,8 +1217,47 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
         gone = __ballot_sync(full, out);
         if (out) sc = 0x7f7f7f7fu;
       }
-      const uint8_t* src = smem + Ly::kRawOff + in.slot * Ly::kRawBytes + row0 * D;
+      const uint8_t* src = smem + Ly::kRawOff + in.slot * Ly::kRawBytes + row0 * (D * BITS / 8);
       uint8_t* dst = smem + Ly::kKvOff + ring.slot * Ly::kTileBytes + (row0 >> 3) * Ly::kGroupBytes;
+      if constexpr (BITS == 4) {
+        // A lane's 16 bytes are four chunks of 8 dims: of each of four groups (head size 128), of two halves of two (64).
+        // Lanes whose tokens share banks take the groups in another order.
+        bool found = false;
+        const bool swap = (D == 128 ? lr : lr >> 1) & 1;
+#pragma unroll 1
+        for (int i = 0; i < 16 / kRpi; ++i) {
+          const int row = i * kRpi + lr, r8 = row & 7;        // of the warp's 16
+          uint4 x = *reinterpret_cast<const uint4*>(src + row * (D / 2) + lc * 16);
+          const uint32_t word = __shfl_sync(full, sc, row);
+          if (gone >> row & 1u) x = make_uint4(0u, 0u, 0u, 0u);
+          const bool hide = plane && first + row >= u.hidden; // some row does not see it: NaN goes in as 0
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t eight;                   // the chunk's values
+            int g, chunk;
+            if constexpr (D == 128) {
+              g = swap ? c ^ 1 : c;
+              chunk = (g & 1) * 4 + lc;
+              eight = __byte_perm(c < 2 ? x.x : x.y, c < 2 ? x.z : x.w, g & 1 ? 0x7632 : 0x5410);
+            } else {
+              g = swap ? (c >> 1) ^ 1 : c >> 1;
+              chunk = g * 4 + lc * 2 + (c & 1);
+              eight = __byte_perm(c & 1 ? x.z : x.x, c & 1 ? x.w : x.y, g & 1 ? 0x7632 : 0x5410);
+            }
+            const uint32_t b = word >> (8 * g) & 255u;
+            uint32_t y[4];
+            if (plain) widen4<BF16>(eight, plain_factor4<BF16>(b), y);
+            else widen4_any<BF16>(eight, b, y);
+            if (hide) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) y[k] = drop_bad<BF16>(y[k], 0xffffffffu, found);
+            }
+            *reinterpret_cast<uint4*>(dst + (row >> 3) * Ly::kGroupBytes + (g >> 1) * (D == 128 ? 1024 : 0) + r8 * 128 +
+                                      ((chunk ^ r8) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
+          }
+        }
+        if (found) *bad_v = 1;
+      } else {
       // Rolled, 8 tokens at a time: the warps of a scheduler are at five places of the kernel, and straight code
       // for all 16 tokens starved it of instructions.
       bool slow = edge || !plain;
@@ -1258,6 +1302,7 @@ __global__ void __launch_bounds__(threads(QUANT), 1)
           uint8_t* d8 = dst + g8 * Ly::kGroupBytes;
           put(d8 + (odd ? put0[8 / kRpi - 1] : put0[0]), d8 + (odd ? put1[8 / kRpi - 1] : put1[0]), r);
         }
+      }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
@@ -1391,7 +1436,6 @@ bool chunk_umma_supported(const ChunkArgs& a, int dtype, const char** why) {
     *why = w;
     return false;
   };
-  if (a.quant == 4) return no("not over the 4-bit cache");
   if (dtype != ACTKV_BF16 && dtype != ACTKV_F16) return no("needs bf16 or fp16");
   if (a.D != 64 && a.D != 128) return no("needs head_dim 64 or 128");
   if (a.G > chunk::kRows) return no("needs a GQA group of at most 128");
@@ -1410,9 +1454,9 @@ bool chunk_umma_supported(const ChunkArgs& a, int dtype, const char** why) {
 
 namespace {
 
-template <int D, bool BF16, bool QUANT>
+template <int D, bool BF16, int BITS>
 cudaError_t launch_chunk_t(const CUtensorMap& mkv, const CUtensorMap& mq, const ChunkArgs& a, int grid, cudaStream_t st) {
-  auto k = chunk::chunk_umma_kernel<D, BF16, QUANT>;
+  auto k = chunk::chunk_umma_kernel<D, BF16, BITS>;
   cudaError_t e = cudaSuccess;
   const bool vec_out = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.out_stride_t % 8 == 0 && a.out_stride_h % 8 == 0;
   cudaLaunchConfig_t cfg = {};
@@ -1424,8 +1468,8 @@ cudaError_t launch_chunk_t(const CUtensorMap& mkv, const CUtensorMap& mq, const 
   const bool wide = a.T * int64_t(a.G) > a.few_rows;         // else every session is chunk_few_kernel's
   if (wide) {
     cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(chunk::threads(QUANT));
-    cfg.dynamicSmemBytes = chunk::Layout<D, QUANT>::kSmemBytes;
+    cfg.blockDim = dim3(chunk::threads(BITS != 16));
+    cfg.dynamicSmemBytes = chunk::Layout<D, BITS>::kSmemBytes;
     static SmemLimit limit;
     if ((e = limit.set(reinterpret_cast<const void*>(k), int(cfg.dynamicSmemBytes))) != cudaSuccess) return e;
     cfg.numAttrs = a.few_rows > 0 ? 1 : 0;   // beside chunk_few_kernel's last CTAs
@@ -1438,6 +1482,13 @@ cudaError_t launch_chunk_t(const CUtensorMap& mkv, const CUtensorMap& mq, const 
   return cudaLaunchKernelEx(&cfg, chunk::chunk_combine_kernel<D, BF16>, a, grid, wide ? 0 : chunk::kJoinSlices);
 }
 
+template <int BITS>
+cudaError_t launch_chunk_bits(const CUtensorMap& mkv, const CUtensorMap& mq, const ChunkArgs& a, int dtype, int grid, cudaStream_t st) {
+  const bool bf = dtype == ACTKV_BF16;
+  if (a.D == 128) return bf ? launch_chunk_t<128, true, BITS>(mkv, mq, a, grid, st) : launch_chunk_t<128, false, BITS>(mkv, mq, a, grid, st);
+  return bf ? launch_chunk_t<64, true, BITS>(mkv, mq, a, grid, st) : launch_chunk_t<64, false, BITS>(mkv, mq, a, grid, st);
+}
+
 }  // namespace
 
 cudaError_t launch_chunk_umma(const ChunkArgs& args, int dtype, cudaStream_t st, const char** why) {
@@ -1447,7 +1498,7 @@ cudaError_t launch_chunk_umma(const ChunkArgs& args, int dtype, cudaStream_t st,
   // sessions of few query rows go to a kernel of their own, where a GQA group fits it
   a.few_rows = a.G <= chunk::few_limit(a.quant) ? chunk::few_limit(a.quant) : 0;
   if (a.few_rows > 0) {
-    const cudaError_t e = launch_chunk_few(a, dtype, grid, st);
+    const cudaError_t e = a.quant == 4 ? launch_chunk_few4(a, dtype, grid, st) : launch_chunk_few(a, dtype, grid, st);
     if (e != cudaSuccess) return e;
   }
   CUtensorMap mkv, mq;
@@ -1462,13 +1513,15 @@ cudaError_t launch_chunk_umma(const ChunkArgs& args, int dtype, cudaStream_t st,
     if (a.quant) {
       // (the heads' values of a row, slot, plane): one head's values of a paged block per box
       const cuuint32_t rows = cuuint32_t(a.BS < chunk::kTile ? a.BS : chunk::kTile);
-      const cuuint64_t dims[3] = {cuuint64_t(a.Hkv) * a.D, cuuint64_t(a.NB) * a.BS, 2};
+      const cuuint32_t bytes = cuuint32_t(a.D * a.quant / 8);
+      const cuuint64_t dims[3] = {cuuint64_t(a.Hkv) * bytes, cuuint64_t(a.NB) * a.BS, 2};
       const cuuint64_t strides[2] = {cuuint64_t(a.kv_stride_s), cuuint64_t(a.kv_stride_kv)};
-      const cuuint32_t box[3] = {cuuint32_t(a.D), rows, 1};
+      const cuuint32_t box[3] = {bytes, rows, 1};
       if (enc(&mkv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(a.kv), dims, strides, box, es,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, a.D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+              CU_TENSOR_MAP_INTERLEAVE_NONE,
+              a.quant == 4 ? CU_TENSOR_MAP_SWIZZLE_NONE : (a.D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B),
               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
-        *why = "cuTensorMapEncodeTiled rejected the layout of the 8-bit rows";
+        *why = "cuTensorMapEncodeTiled rejected the layout of the rows";
         return cudaErrorInvalidValue;
       }
     } else {
@@ -1497,13 +1550,9 @@ cudaError_t launch_chunk_umma(const ChunkArgs& args, int dtype, cudaStream_t st,
     }
   }
   *why = "chunk attention";
-  const bool bf = dtype == ACTKV_BF16;
-  if (a.quant) {
-    if (a.D == 128) return bf ? launch_chunk_t<128, true, true>(mkv, mq, a, grid, st) : launch_chunk_t<128, false, true>(mkv, mq, a, grid, st);
-    return bf ? launch_chunk_t<64, true, true>(mkv, mq, a, grid, st) : launch_chunk_t<64, false, true>(mkv, mq, a, grid, st);
-  }
-  if (a.D == 128) return bf ? launch_chunk_t<128, true, false>(mkv, mq, a, grid, st) : launch_chunk_t<128, false, false>(mkv, mq, a, grid, st);
-  return bf ? launch_chunk_t<64, true, false>(mkv, mq, a, grid, st) : launch_chunk_t<64, false, false>(mkv, mq, a, grid, st);
+  if (a.quant == 8) return launch_chunk_bits<8>(mkv, mq, a, dtype, grid, st);
+  if (a.quant == 4) return launch_chunk_bits<4>(mkv, mq, a, dtype, grid, st);
+  return launch_chunk_bits<16>(mkv, mq, a, dtype, grid, st);
 }
 
 }  // namespace actkv

@@ -343,8 +343,9 @@ struct SmemLimit {
 size_t chunk_workspace_bytes(int n_sm);
 bool chunk_umma_supported(const ChunkArgs& a, int dtype, const char** why);
 cudaError_t launch_chunk_umma(const ChunkArgs& a, int dtype, cudaStream_t st, const char** why);
-// the sessions of at most a.few_rows query rows per KV head
+// the sessions of at most a.few_rows query rows per KV head (over the 4-bit cache: launch_chunk_few4)
 cudaError_t launch_chunk_few(const ChunkArgs& a, int dtype, int grid, cudaStream_t st);
+cudaError_t launch_chunk_few4(const ChunkArgs& a, int dtype, int grid, cudaStream_t st);
 cudaError_t launch_chunk_simt(const ChunkArgs& a, int dtype, cudaStream_t st);
 
 // ---------------------------------------------------------------- 8-bit cache rows (quant_cache.cu)
