@@ -4,6 +4,8 @@
 // plane, head): lane p takes the run of bytes that holds values 4 p .. 4 p + 3 of every group of 32 (one load for
 // head sizes 64 and 128) and writes four values per group, 64 bytes of 16-bit values from the eight lanes
 // together.  A warp takes four such rows at a time, kPasses times, of one token, whose session and slot it finds once.
+#include <type_traits>
+
 #include "kernels.cuh"
 #include "quant_row.cuh"
 
@@ -33,6 +35,17 @@ template <typename T, int G>
 __global__ void __launch_bounds__(kThreads) quant4_read_kernel(const __grid_constant__ QuantMoveArgs a) {
   struct alignas(4 * sizeof(T)) Four {
     T v[4];
+  };
+  auto narrow2 = [](float x, float y, T* p) {
+    if constexpr (sizeof(T) == 4) {
+      p[0] = x;
+      p[1] = y;
+    } else if constexpr (std::is_same<T, __half>::value) {   // past the range: the largest (NaN stays)
+      *reinterpret_cast<__half2*>(p) = __hmin2_nan(__hmax2_nan(__floats2half2_rn(x, y), __float2half2_rn(-65504.0f)),
+                                                   __float2half2_rn(65504.0f));
+    } else {
+      *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(x, y);
+    }
   };
   constexpr int kAt = G ? G : 1;
   const int lane = threadIdx.x & 31, p = lane & 7;
@@ -98,10 +111,8 @@ __global__ void __launch_bounds__(kThreads) quant4_read_kernel(const __grid_cons
             const float s = scale_of4(sc[i] >> (8 * (g + e)) & 255u);
             const float2 lo = f16x2_f32(h[2 * e]), hi = f16x2_f32(h[2 * e + 1]);
             Four y;
-            y.v[0] = from_f32<T>(lo.x * s);
-            y.v[1] = from_f32<T>(lo.y * s);
-            y.v[2] = from_f32<T>(hi.x * s);
-            y.v[3] = from_f32<T>(hi.y * s);
+            narrow2(lo.x * s, lo.y * s, y.v);
+            narrow2(hi.x * s, hi.y * s, y.v + 2);
             T* dst = ext[i] + 32 * (g + e);
             if (a.vec) {
               *reinterpret_cast<Four*>(dst) = y;

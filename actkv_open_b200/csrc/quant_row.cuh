@@ -66,9 +66,13 @@ __device__ __forceinline__ float scale_of4(uint32_t b) { return scale_of(b >= kN
 
 // Four values (the first in the lowest half byte) and back: one conversion per pair.
 __device__ __forceinline__ uint32_t f32_e2m1x4(float x0, float x1, float x2, float x3) {
-  const uint32_t lo = __nv_cvt_float2_to_fp4x2(make_float2(x0, x1), __NV_E2M1, cudaRoundNearest);
-  const uint32_t hi = __nv_cvt_float2_to_fp4x2(make_float2(x2, x3), __NV_E2M1, cudaRoundNearest);
-  return lo | hi << 8;
+  uint32_t r;                                // (a NaN: any code)
+  asm("{\n\t.reg .b8 a, b, z;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "mov.b32 %0, {a, b, a, b};\n\t}"
+      : "=r"(r)
+      : "f"(x0), "f"(x1), "f"(x2), "f"(x3));
+  return r & 0xffffu;
 }
 __device__ __forceinline__ uint32_t e2m1x2_f16(uint32_t two) {
   const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2(__nv_fp4x2_storage_t(two), __NV_E2M1);

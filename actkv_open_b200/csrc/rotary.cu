@@ -8,10 +8,12 @@
 // which of the two products it takes, so that rows quantised here are those of the plain formula bit for bit.
 //
 // Memory bounds it: every value is read and written once, and the table's row of a token (8 bytes per pair) once per
-// warp that works on the token, from L2.  A warp takes a run of one token: where the type stays, items of 16
-// values (two pieces of 8 that turn together: 16-byte loads), the same dims for every item of a lane, so that sines
-// and cosines stay in registers; for rows, eight lanes per (layer, plane, head), lane p holding values 4 p .. 4 p + 3 of
-// every group of 32, which is what the 4-bit row keeps together, and a group's maximum is three shuffles.
+// warp that works on the token, from L2.  A warp takes a run of one token's passes:
+//   where the type stays, a pass is 16 values per lane (two pieces of 8 that turn together: 16-byte accesses) of as
+//     many heads as 32 lanes hold; a lane's dims are the same in every pass, so its sines and cosines stay in registers;
+//   into rows, a pass is four heads, eight lanes each, lane p holding values 4 p .. 4 p + 3 of every group of 32, which
+//     is what the 4-bit row keeps together, and a group's maximum is three shuffles (of two groups at once where the
+//     values are 16-bit and do not turn).
 #include "kernels.cuh"
 #include "quant_row.cuh"
 
@@ -98,15 +100,23 @@ struct Divisor {
   __device__ __forceinline__ int operator()(int a) const { return shift >= 0 ? a >> shift : a / b; }
 };
 
-// Which array, layer and head a row of a token is; heads: q's, then k's, then v's.
-struct Row {
-  int which, l, h;
-};
+__device__ __forceinline__ void narrow2(float2 x, float* p) {
+  p[0] = x.x;
+  p[1] = x.y;
+}
+__device__ __forceinline__ void narrow2(float2 x, __half* p) { *reinterpret_cast<__half2*>(p) = __float22half2_rn(x); }
+__device__ __forceinline__ void narrow2(float2 x, __nv_bfloat16* p) { *reinterpret_cast<__nv_bfloat162*>(p) = __float22bfloat162_rn(x); }
+
+// Two pairs.  (Packed 32-bit products and sums give other digits: they are fused on the way to machine code.)
+__device__ __forceinline__ void turn2(float2& x, float2& y, float2 c, float2 s) {
+  turn(x.x, y.x, c.x, s.x);
+  turn(x.y, y.y, c.y, s.y);
+}
 
 // ------------------------------------------------------------------------------ the type stays
-// An item is 16 values: pieces at dims d0 and d1 that turn together.
+// A lane's 16 values of a head: pieces at dims d0 and d1 that turn together; i: the pair of the first value, -1: they stay.
 struct Item {
-  int d0, d1, i;             // i: the pair of the first value, -1: they stay
+  int d0, d1, i;
 };
 __device__ __forceinline__ Item item_of(const RotateArgs& a, int j) {
   const int turned = a.rot / 16;
@@ -115,86 +125,102 @@ __device__ __forceinline__ Item item_of(const RotateArgs& a, int j) {
   return {8 * j, 8 * j + a.rot / 2, 8 * j};
 }
 
-// Items [first, first + 32 N) of token t.  SAME: the items of a head (`per`) divide 32, so a lane's dims are the
-// same in all of its items.
-template <typename T, int N, bool SAME>
-__device__ __forceinline__ void same_type(const RotateArgs& a, int t, int first, int items, int heads, int per,
-                                          const Token& tok, const float* angles, int lane) {
+// Four neighbouring pairs.
+template <typename T>
+__device__ __forceinline__ void turn_pairs(Piece<T, 8>& p, float2 c0, float2 s0, float2 c1, float2 s1) {
+#pragma unroll
+  for (int k = 0; k < 8; k += 4) {
+    float2 u = make_float2(to_f32(p.v[k]), to_f32(p.v[k + 2])), v = make_float2(to_f32(p.v[k + 1]), to_f32(p.v[k + 3]));
+    turn2(u, v, k ? c1 : c0, k ? s1 : s0);
+    p.v[k] = narrow<T>(u.x);
+    p.v[k + 1] = narrow<T>(v.x);
+    p.v[k + 2] = narrow<T>(u.y);
+    p.v[k + 3] = narrow<T>(v.y);
+  }
+}
+
+// Passes [first, first + n) of token t: heads in blocks of as many as 32 lanes hold, of q, then k, then v, layer by layer.
+template <typename T, bool KV>
+__device__ __forceinline__ void same_type(const RotateArgs& a, int t, int first, int n, const Token& tok,
+                                          const float* angles, int lane) {
   using P8 = Piece<T, 8>;
-  const Divisor by_per(per), by_heads(heads);
-  float c[8], s[8];
-  auto take = [&](int i) {
+  const int per = a.D / 16, block = 32 / per;               // lanes per head, heads per pass
+  const int hl = lane / per, j = lane - hl * per;
+  const Item it = item_of(a, j);
+  float2 c[4], s[4];
+  if (it.i >= 0) {
 #pragma unroll
-    for (int k = 0; k < 8; k += 4) {
-      *reinterpret_cast<float4*>(c + k) = __ldg(reinterpret_cast<const float4*>(angles + i + k));
-      *reinterpret_cast<float4*>(s + k) = __ldg(reinterpret_cast<const float4*>(angles + a.rot / 2 + i + k));
+    for (int k = 0; k < 2; ++k) {
+      reinterpret_cast<float4*>(c)[k] = __ldg(reinterpret_cast<const float4*>(angles + it.i + 4 * k));
+      reinterpret_cast<float4*>(s)[k] = __ldg(reinterpret_cast<const float4*>(angles + a.rot / 2 + it.i + 4 * k));
     }
-  };
-  if constexpr (SAME) {
-    const int f = first + lane, i = item_of(a, f - by_per(f) * per).i;
-    if (i >= 0) take(i);
   }
-  P8 x[N], y[N];
-  Row row[N];
-  Item it[N];
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    const int f = first + n * 32 + lane;
-    row[n].which = -1;
-    if (f >= items) continue;
-    const int hr = by_per(f);
-    it[n] = item_of(a, f - hr * per);
-    const int l = by_heads(hr), h = hr - l * heads;
-    row[n] = h < a.Hq ? Row{0, l, h} : (h < a.Hq + a.Hkv ? Row{1, l, h - a.Hq} : Row{2, l, h - a.Hq - a.Hkv});
-    const int w = row[n].which;
-    const T* p = static_cast<const T*>(a.in[w]) + (int64_t(l) * a.in_l[w] + int64_t(t) * a.in_t[w] + int64_t(row[n].h) * a.in_h[w]);
-    x[n] = load<T, 8>(p + it[n].d0, true);
-    y[n] = load<T, 8>(p + it[n].d1, true);
+  const int nq = (a.Hq + block - 1) / block, nk = KV ? (a.Hkv + block - 1) / block : 0;
+  int l = first / (nq + 2 * nk), hb = first - l * (nq + 2 * nk), w = 0;
+  if (KV && hb >= nq) {
+    hb -= nq;
+    w = 1;
+    if (hb >= nk) {
+      hb -= nk;
+      w = 2;
+    }
   }
+  constexpr int kAhead = 2;                   // passes in flight
+  while (n > 0) {                             // the passes of one array and layer
+    const int heads = w == 0 ? a.Hq : a.Hkv, m = min(n, (w == 0 ? nq : nk) - hb), h0 = hb * block + hl;
+    const T* src = static_cast<const T*>(a.in[w]) + (int64_t(l) * a.in_l[w] + int64_t(t) * a.in_t[w] + int64_t(h0) * a.in_h[w]);
+    const int64_t out_h = w == 0 ? a.out_h : a.c_h;
+    T* dst = w == 0 ? static_cast<T*>(a.q_out) + (int64_t(l) * a.out_l + int64_t(t) * a.out_t + int64_t(h0) * out_h)
+                    : static_cast<T*>(a.cache) + (int64_t(l) * a.c_l + int64_t(w - 1) * a.c_kv + tok.at + int64_t(h0) * out_h);
+    const int64_t src_step = block * a.in_h[w], dst_step = block * out_h;
+    const bool turns = w < 2 && it.i >= 0;
+    const int live = hl < block && (w == 0 || tok.at >= 0) ? heads - h0 : 0;      // heads from this lane's on
+#pragma unroll 1
+    for (int i = 0; i < m; i += kAhead, src += kAhead * src_step, dst += kAhead * dst_step) {
+      P8 x[kAhead], y[kAhead];
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
-    if (row[n].which < 0) continue;
-    const int w = row[n].which;
-    if (w < 2 && it[n].i >= 0) {
-      if constexpr (!SAME) take(it[n].i);
-      if (a.pairs) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float u = to_f32(x[n].v[2 * i]), v = to_f32(x[n].v[2 * i + 1]), e = to_f32(y[n].v[2 * i]), f = to_f32(y[n].v[2 * i + 1]);
-          turn(u, v, c[i], s[i]);
-          turn(e, f, c[4 + i], s[4 + i]);
-          x[n].v[2 * i] = narrow<T>(u);
-          x[n].v[2 * i + 1] = narrow<T>(v);
-          y[n].v[2 * i] = narrow<T>(e);
-          y[n].v[2 * i + 1] = narrow<T>(f);
+      for (int e = 0; e < kAhead; ++e)
+        if (i + e < m && (i + e) * block < live) {
+          x[e] = load<T, 8>(src + e * src_step + it.d0, true);
+          y[e] = load<T, 8>(src + e * src_step + it.d1, true);
         }
-      } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float u = to_f32(x[n].v[i]), v = to_f32(y[n].v[i]);
-          turn(u, v, c[i], s[i]);
-          x[n].v[i] = narrow<T>(u);
-          y[n].v[i] = narrow<T>(v);
+      for (int e = 0; e < kAhead; ++e) {
+        if (i + e >= m || (i + e) * block >= live) continue;
+        if (turns) {
+          if (a.pairs) {
+            turn_pairs(x[e], c[0], s[0], c[1], s[1]);
+            turn_pairs(y[e], c[2], s[2], c[3], s[3]);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              float2 u = make_float2(to_f32(x[e].v[2 * k]), to_f32(x[e].v[2 * k + 1]));
+              float2 v = make_float2(to_f32(y[e].v[2 * k]), to_f32(y[e].v[2 * k + 1]));
+              turn2(u, v, c[k], s[k]);
+              narrow2(u, x[e].v + 2 * k);
+              narrow2(v, y[e].v + 2 * k);
+            }
+          }
         }
+        store<T, 8>(dst + e * dst_step + it.d0, x[e], true);
+        store<T, 8>(dst + e * dst_step + it.d1, y[e], true);
       }
     }
-    T* p;
-    if (w == 0) {
-      p = static_cast<T*>(a.q_out) + (int64_t(row[n].l) * a.out_l + int64_t(t) * a.out_t + int64_t(row[n].h) * a.out_h);
-    } else {
-      if (tok.at < 0) continue;
-      p = static_cast<T*>(a.cache) + (int64_t(row[n].l) * a.c_l + int64_t(w - 1) * a.c_kv + tok.at + int64_t(row[n].h) * a.c_h);
+    n -= m;
+    hb = 0;
+    if (!KV || ++w == 3) {
+      w = nq > 0 ? 0 : 1;
+      ++l;
     }
-    store<T, 8>(p + it[n].d0, x[n], true);
-    store<T, 8>(p + it[n].d1, y[n], true);
   }
 }
 
 // Any sizes, strides and alignment: a lane takes a pair, or a value that stays.
 template <typename T>
-__device__ __forceinline__ void any_layout(const RotateArgs& a, int t, int first, int n, int units, int heads,
-                                           const Token& tok, const float* angles, int lane) {
+__device__ __forceinline__ void any_layout(const RotateArgs& a, int t, int first, int n, const Token& tok,
+                                           const float* angles, int lane) {
   const int half = a.rot / 2, per = half + a.D - a.rot;
+  const int heads = a.Hq + (a.bits == 0 ? 2 * a.Hkv : 0), units = a.L * heads * per;
   for (int f = first + lane; f < min(first + n, units); f += 32) {
     const int hr = f / per, i = f - hr * per, l = hr / heads, hh = hr - l * heads;
     const int w = hh < a.Hq ? 0 : (hh < a.Hq + a.Hkv ? 1 : 2), h = hh - (w == 0 ? 0 : (w == 1 ? a.Hq : a.Hq + a.Hkv));
@@ -220,187 +246,247 @@ __device__ __forceinline__ void any_layout(const RotateArgs& a, int t, int first
 }
 
 // ------------------------------------------------------------------------------ into 8- or 4-bit rows
-// Rows [first, first + 4 n) of token t's 2 L Hkv (layer, head, plane) rows, eight lanes each.
+__device__ __forceinline__ uint32_t max16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// The bits of the largest magnitudes of N groups, four values of each per lane, over eight lanes.  Without the sign, floats
+// order as their bits do, NaN above all.  Of 16-bit values two groups at a time.
+template <typename T, int N>
+__device__ __forceinline__ void tops(const Piece<T, 4> (&raw)[N], uint32_t (&top)[N]) {
+  static_assert(sizeof(T) == 2);
+#pragma unroll
+  for (int g = 0; g < N; g += 2) {
+    uint32_t m[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint2 w = reinterpret_cast<const uint2&>(raw[g + e < N ? g + e : g]);
+      m[e] = max16x2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu);
+    }
+    uint32_t both = max16x2(__byte_perm(m[0], m[1], 0x5410), __byte_perm(m[0], m[1], 0x7632));
+#pragma unroll
+    for (int o = 1; o < 8; o *= 2) both = max16x2(both, __shfl_xor_sync(0xffffffffu, both, o));
+    const uint16_t lo = uint16_t(both), hi = uint16_t(both >> 16);
+    top[g] = __float_as_uint(to_f32(reinterpret_cast<const T&>(lo)));
+    if (g + 1 < N) top[g + 1 < N ? g + 1 : g] = __float_as_uint(to_f32(reinterpret_cast<const T&>(hi)));
+  }
+}
+template <int N>
+__device__ __forceinline__ void tops(const float (&x)[N][4], uint32_t (&top)[N]) {
+#pragma unroll
+  for (int g = 0; g < N; ++g) {
+    top[g] = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) top[g] = max(top[g], __float_as_uint(x[g][k]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 1; o < 8; o *= 2) top[g] = max(top[g], __shfl_xor_sync(0xffffffffu, top[g], o));
+  }
+}
+
+// How keys turn on their way into rows: not at all; all of a head's dims in halves, so that the values that turn together are
+// in one lane; or in any way, the other value of a pair fetched from memory.
+enum Turns { kStay, kInLane, kAny };
+
+// Passes [first, first + n) of token t's 2 L Hkv (layer, plane, head) rows: four rows each, eight lanes per row.
 // G: groups of a head (0: any number, a.D / 32, one at a time).
-template <typename T, int BITS, int G>
+template <typename T, int BITS, int G, Turns TURNS>
 __device__ __forceinline__ void quantise(const RotateArgs& a, int t, int first, int n, int rows, const Token& tok,
                                          const float* angles, int lane) {
-  const int p = lane & 7, groups = G ? G : a.D / 32, half = a.rot / 2;
+  const int p = lane & 7, groups = G ? G : a.D / 32;
+  [[maybe_unused]] const int half = a.rot / 2;
   const Divisor by_heads(a.Hkv);
   constexpr int kAt = G ? G : 1;              // groups at a time
+  [[maybe_unused]] float4 c[(kAt + 1) / 2], s[(kAt + 1) / 2];
+  if constexpr (TURNS == kInLane) {
+#pragma unroll
+    for (int g = 0; g < kAt / 2; ++g) {
+      c[g] = __ldg(reinterpret_cast<const float4*>(angles + 32 * g + 4 * p));
+      s[g] = __ldg(reinterpret_cast<const float4*>(angles + half + 32 * g + 4 * p));
+    }
+  }
+  // A lane's rows past the last are the last once more, not stored: the shuffles are the whole warp's.
+  auto source = [&](int f, int& w) -> const T* {
+    const int lp = by_heads(f), h = f - lp * a.Hkv, l = lp >> 1;
+    w = 1 + (lp & 1);
+    return static_cast<const T*>(a.in[w]) + (int64_t(l) * a.in_l[w] + int64_t(t) * a.in_t[w] + int64_t(h) * a.in_h[w]) + 4 * p;
+  };
+  const int steps = groups / kAt;             // of a pass
+  Piece<T, 4> ahead[kAt];                     // the next step's values
+  auto fetch = [&](int i) {
+    int w;
+    const int pass = G ? i : i / steps, g0 = G ? 0 : i - pass * steps;
+    const T* src = source(min(4 * (first + pass) + (lane >> 3), rows - 1), w);
+#pragma unroll
+    for (int g = 0; g < kAt; ++g) ahead[g] = load<T, 4>(src + 32 * (g0 + g), a.vec_in);
+  };
+  fetch(0);
 #pragma unroll 1
-  for (int i = 0; i < n; ++i) {
-    const int f = first + 4 * i + (lane >> 3);
-    const bool on = f < rows;                 // the shuffles below are the whole warp's
-    const int lp = on ? by_heads(f) : 0, h = on ? f - lp * a.Hkv : 0, l = lp >> 1, w = 1 + (lp & 1);
-    const T* src = static_cast<const T*>(a.in[w]) + (int64_t(l) * a.in_l[w] + int64_t(t) * a.in_t[w] + int64_t(h) * a.in_h[w]) + 4 * p;
-    uint8_t* row = static_cast<uint8_t*>(a.cache) + (int64_t(l) * a.c_l + int64_t(w - 1) * a.c_kv + tok.at);
-    uint8_t* vals = row + h * (a.D * BITS / 8);
-    uint8_t* scales = row + a.Hkv * (a.D * BITS / 8) + h * groups;
-    const bool turns = on && w == 1 && a.rot > 0;
-#pragma unroll 1
-    for (int g0 = 0; g0 < groups; g0 += kAt) {
-      Piece<T, 4> raw[kAt], other[kAt];
+  for (int i = 0; i < n * steps; ++i) {
+    const int pass = G ? i : i / steps, g0 = G ? 0 : i - pass * steps;
+    Piece<T, 4> raw[kAt];
 #pragma unroll
-      for (int g = 0; g < kAt; ++g)
-        if (on) raw[g] = load<T, 4>(src + 32 * (g0 + g), a.vec_in);
-      // the values that turn with them, when those are not in this lane (all of a head's dims in halves: they are)
-      const bool inside = G > 1 && a.rot == a.D && a.vec_in;
-      if (turns && !a.pairs && !inside) {
+    for (int g = 0; g < kAt; ++g) raw[g] = ahead[g];
+    if (i + 1 < n * steps) fetch(i + 1);
+    const int f0 = 4 * (first + pass) + (lane >> 3), f = min(f0, rows - 1);
+    const int lp = by_heads(f), h = f - lp * a.Hkv;
+    const bool turns = TURNS != kStay && (lp & 1) == 0;
+    float x[kAt][4];
 #pragma unroll
-        for (int g = 0; g < kAt; ++g) {
-          const int d = 32 * (g0 + g) + 4 * p;
-          if (d < a.rot) other[g] = load<T, 4>(src + 32 * (g0 + g) + (d < half ? half : -half), a.vec_in);
-        }
-      }
-      float x[kAt][4];
+    for (int g = 0; g < kAt; ++g)
 #pragma unroll
-      for (int g = 0; g < kAt; ++g)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[g][k] = on ? to_f32(raw[g].v[k]) : 0.0f;
-      if (turns && a.pairs) {
-#pragma unroll
-        for (int g = 0; g < kAt; ++g) {
-          const int d = 32 * (g0 + g) + 4 * p;
-          if (d >= a.rot) continue;
-          turn(x[g][0], x[g][1], __ldg(angles + d / 2), __ldg(angles + half + d / 2));
-          turn(x[g][2], x[g][3], __ldg(angles + d / 2 + 1), __ldg(angles + half + d / 2 + 1));
-        }
-      } else if (turns && inside) {
+      for (int k = 0; k < 4; ++k) x[g][k] = to_f32(raw[g].v[k]);
+    if constexpr (TURNS == kInLane) {
+      if (turns) {
 #pragma unroll
         for (int g = 0; g < kAt / 2; ++g) {
-          const float4 c = __ldg(reinterpret_cast<const float4*>(angles + 32 * g + 4 * p));
-          const float4 s = __ldg(reinterpret_cast<const float4*>(angles + half + 32 * g + 4 * p));
-          turn(x[g][0], x[g + kAt / 2][0], c.x, s.x);
-          turn(x[g][1], x[g + kAt / 2][1], c.y, s.y);
-          turn(x[g][2], x[g + kAt / 2][2], c.z, s.z);
-          turn(x[g][3], x[g + kAt / 2][3], c.w, s.w);
-        }
-      } else if (turns) {
+        turn(x[g][0], x[g + kAt / 2][0], c[g].x, s[g].x);
+        turn(x[g][1], x[g + kAt / 2][1], c[g].y, s[g].y);
+        turn(x[g][2], x[g + kAt / 2][2], c[g].z, s[g].z);
+        turn(x[g][3], x[g + kAt / 2][3], c[g].w, s[g].w);
+      }
+      }
+    } else if constexpr (TURNS == kAny) {
+      if (turns) {
 #pragma unroll
-        for (int g = 0; g < kAt; ++g) {
-          const int d = 32 * (g0 + g) + 4 * p;
-          if (d >= a.rot) continue;
+      for (int g = 0; g < kAt; ++g) {
+        const int d = 32 * (g0 + g) + 4 * p;
+        if (d >= a.rot) continue;
+        if (a.pairs) {
+          turn(x[g][0], x[g][1], __ldg(angles + d / 2), __ldg(angles + half + d / 2));
+          turn(x[g][2], x[g][3], __ldg(angles + d / 2 + 1), __ldg(angles + half + d / 2 + 1));
+        } else {                              // the other values of the pairs, from memory
           const bool low = d < half;
+          int w;
+          const Piece<T, 4> other = load<T, 4>(source(f, w) + 32 * (g0 + g) + (low ? half : -half), a.vec_in);
           const float* at = angles + (low ? d : d - half);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            float u = low ? x[g][k] : to_f32(other[g].v[k]), v = low ? to_f32(other[g].v[k]) : x[g][k];
+            float u = low ? x[g][k] : to_f32(other.v[k]), v = low ? to_f32(other.v[k]) : x[g][k];
             turn(u, v, __ldg(at + k), __ldg(at + half + k));
             x[g][k] = low ? u : v;
           }
         }
       }
-      uint32_t packed[kAt], bytes = 0;
+    }
+    }
+    uint32_t top[kAt];
+    if constexpr (sizeof(T) == 2) {
+      if (TURNS != kStay && __any_sync(0xffffffffu, turns)) tops<kAt>(x, top);
+      else tops<T, kAt>(raw, top);
+    } else {
+      tops<kAt>(x, top);
+    }
+    uint32_t packed[kAt], bytes = 0;
+#pragma unroll
+    for (int g = 0; g < kAt; ++g) {
+      const uint32_t b = BITS == 4 ? scale_byte4(top[g]) : scale_byte(top[g]);
+      const float inv = inverse_scale(b);     // (anything for 255)
+      uint32_t u;
+      if constexpr (BITS == 4)
+        u = f32_e2m1x4(x[g][0] * inv, x[g][1] * inv, x[g][2] * inv, x[g][3] * inv);
+      else
+        u = (f32_e4m3x2(x[g][0] * inv, x[g][1] * inv) & 0xffffu) | f32_e4m3x2(x[g][2] * inv, x[g][3] * inv) << 16;
+      packed[g] = b == 255u ? 0u : u;
+      bytes |= b << (8 * g);
+    }
+    if (f0 >= rows) continue;
+    uint8_t* row = static_cast<uint8_t*>(a.cache) + (int64_t(lp >> 1) * a.c_l + int64_t(lp & 1) * a.c_kv + tok.at);
+    uint8_t* vals = row + h * (a.D * BITS / 8);
+    uint8_t* scales = row + a.Hkv * (a.D * BITS / 8) + h * groups + g0;
+    if constexpr (BITS == 8) {
 #pragma unroll
       for (int g = 0; g < kAt; ++g) {
-        // without the sign, floats order as their bits do, NaN above all
-        uint32_t top = 0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) top = max(top, __float_as_uint(x[g][k]) & 0x7fffffffu);
-#pragma unroll
-        for (int o = 1; o < 8; o *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const uint32_t b = BITS == 4 ? scale_byte4(top) : scale_byte(top);
-        const float inv = inverse_scale(b == 255u ? 0u : b);
-        uint32_t u;
-        if constexpr (BITS == 4)
-          u = f32_e2m1x4(x[g][0] * inv, x[g][1] * inv, x[g][2] * inv, x[g][3] * inv);
+        uint8_t* dst = vals + 32 * (g0 + g) + 4 * p;
+        if (a.vec_out) *reinterpret_cast<uint32_t*>(dst) = packed[g];
         else
-          u = (f32_e4m3x2(x[g][0] * inv, x[g][1] * inv) & 0xffffu) | f32_e4m3x2(x[g][2] * inv, x[g][3] * inv) << 16;
-        packed[g] = b == 255u ? 0u : u;
-        bytes |= b << (8 * g);
+          for (int k = 0; k < 4; ++k) dst[k] = uint8_t(packed[g] >> (8 * k));
       }
-      if (!on) continue;
-      if constexpr (BITS == 8) {
+    } else {
+      uint8_t* dst = vals + 2 * groups * p + 2 * g0;
+      if (G == 4 && a.vec_out) {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(__byte_perm(packed[0], packed[kAt > 1 ? 1 : 0], 0x5410),
+                                                    __byte_perm(packed[kAt > 2 ? 2 : 0], packed[kAt > 3 ? 3 : 0], 0x5410));
+      } else if (G == 2 && a.vec_out) {
+        *reinterpret_cast<uint32_t*>(dst) = __byte_perm(packed[0], packed[kAt > 1 ? 1 : 0], 0x5410);
+      } else {
 #pragma unroll
         for (int g = 0; g < kAt; ++g) {
-          uint8_t* dst = vals + 32 * (g0 + g) + 4 * p;
-          if (a.vec_out) *reinterpret_cast<uint32_t*>(dst) = packed[g];
-          else
-            for (int k = 0; k < 4; ++k) dst[k] = uint8_t(packed[g] >> (8 * k));
-        }
-      } else {
-        uint8_t* dst = vals + 2 * groups * p + 2 * g0;
-        if (G == 4 && a.vec_out) {
-          *reinterpret_cast<uint2*>(dst) = make_uint2(packed[0] | packed[kAt > 1 ? 1 : 0] << 16,
-                                                      packed[kAt > 2 ? 2 : 0] | packed[kAt > 3 ? 3 : 0] << 16);
-        } else if (G == 2 && a.vec_out) {
-          *reinterpret_cast<uint32_t*>(dst) = packed[0] | packed[kAt > 1 ? 1 : 0] << 16;
-        } else {
-#pragma unroll
-          for (int g = 0; g < kAt; ++g) {
-            dst[2 * g] = uint8_t(packed[g]);
-            dst[2 * g + 1] = uint8_t(packed[g] >> 8);
-          }
+          dst[2 * g] = uint8_t(packed[g]);
+          dst[2 * g + 1] = uint8_t(packed[g] >> 8);
         }
       }
-      if (p == 0) {
-        if (G == 4 && a.vec_out) *reinterpret_cast<uint32_t*>(scales) = bytes;
-        else
+    }
+    if (p == 0) {
+      if (G == 4 && a.vec_out) *reinterpret_cast<uint32_t*>(scales) = bytes;
+      else
 #pragma unroll
-          for (int g = 0; g < kAt; ++g) scales[g0 + g] = uint8_t(bytes >> (8 * g));
-      }
+        for (int g = 0; g < kAt; ++g) scales[g] = uint8_t(bytes >> (8 * g));
     }
   }
 }
 
 // ------------------------------------------------------------------------------ the kernel
-// A token's work in runs of 32 N items (q's, and with BITS 0 also k's and v's), then runs of 4 N rows to
-// quantise, a run per warp.
-template <typename T, int BITS, int G, int N, bool VEC>
-__global__ void __launch_bounds__(kThreads) rotate_write_kernel(const __grid_constant__ RotateArgs a) {
+// A token's work: passes of q (and where the type stays of k and v), then passes of rows to quantise, in runs of `run`
+// passes of one kind, a run per warp.
+template <typename T, int BITS, int G, Turns TURNS, bool VEC>
+__global__ void __launch_bounds__(kThreads, BITS == 0 || TURNS == kStay ? 8 : 5)
+    rotate_write_kernel(const __grid_constant__ RotateArgs a, int run, int item_passes, int item_runs, int runs) {
   const int lane = threadIdx.x & 31;
-  const int heads = a.Hq + (BITS == 0 ? 2 * a.Hkv : 0);
-  const int per = VEC ? a.D / 16 : a.rot / 2 + a.D - a.rot;  // items of a head
-  const int items = a.L * heads * per, rows = BITS == 0 ? 0 : 2 * a.L * a.Hkv;
-  const int item_runs = (items + 32 * N - 1) / (32 * N), runs = item_runs + (rows + 4 * N - 1) / (4 * N);
   const int64_t warp = (int64_t(blockIdx.x) * kThreads + threadIdx.x) >> 5;
   const int64_t nwarps = (int64_t(gridDim.x) * kThreads) >> 5;
-  const bool same = VEC && 32 % per == 0;
+  const int rows = BITS == 0 ? 0 : 2 * a.L * a.Hkv;
   for (int64_t w = warp; w < int64_t(a.T) * runs; w += nwarps) {
-    const int t = int(w / runs), run = int(w - int64_t(t) * runs);
+    const int t = int(w / runs), which = int(w - int64_t(t) * runs);
     const float* angles = nullptr;
     const Token tok = find(a, t, lane, angles);
     if (!tok.live) continue;
-    if (run < item_runs) {
-      if constexpr (VEC) {
-        if (same) same_type<T, N, true>(a, t, run * 32 * N, items, heads, per, tok, angles, lane);
-        else same_type<T, N, false>(a, t, run * 32 * N, items, heads, per, tok, angles, lane);
-      } else {
-        any_layout<T>(a, t, run * 32 * N, 32 * N, items, heads, tok, angles, lane);
-      }
+    if (TURNS != kStay && which < item_runs) {
+      const int first = which * run, n = min(run, item_passes - first);
+      if constexpr (VEC) same_type<T, BITS == 0>(a, t, first, n, tok, angles, lane);
+      else any_layout<T>(a, t, first * 32, n * 32, tok, angles, lane);
     } else if constexpr (BITS != 0) {
-      if (tok.at >= 0) quantise<T, BITS, G>(a, t, (run - item_runs) * 4 * N, N, rows, tok, angles, lane);
+      const int first = (which - item_runs) * run;
+      if (tok.at >= 0) quantise<T, BITS, G, TURNS>(a, t, first, min(run, (rows + 3) / 4 - first), rows, tok, angles, lane);
     }
   }
 }
 
-template <typename T, int BITS, int G, int N, bool VEC>
-cudaError_t launch(const RotateArgs& a, int64_t warps, cudaStream_t st) {
-  const int64_t ctas = (warps + kThreads / 32 - 1) / (kThreads / 32);
-  rotate_write_kernel<T, BITS, G, N, VEC><<<unsigned(ctas < (1 << 20) ? ctas : (1 << 20)), kThreads, 0, st>>>(a);
+template <typename T, int BITS, int G, Turns TURNS, bool VEC>
+cudaError_t launch(const RotateArgs& a, cudaStream_t st) {
+  const int block = VEC ? 32 / (a.D / 16) : 1;
+  const int64_t items = TURNS == kStay ? 0 : VEC
+      ? int64_t(a.L) * ((a.Hq + block - 1) / block + (BITS == 0 ? 2 * ((a.Hkv + block - 1) / block) : 0))
+      : (int64_t(a.L) * (a.Hq + (BITS == 0 ? 2 * a.Hkv : 0)) * (a.rot / 2 + a.D - a.rot) + 31) / 32;
+  const int64_t rows = BITS == 0 ? 0 : (int64_t(2) * a.L * a.Hkv + 3) / 4;
+  auto runs = [&](int run) { return (items + run - 1) / run + (rows + run - 1) / run; };
+  // long runs find a token once for more work, short ones give a small call more warps
+  int run = 8;
+  while (run > 1 && a.T * runs(run) < int64_t(device_sm_count()) * 16) run /= 2;
+  const int64_t warps = a.T * runs(run), ctas = (warps + kThreads / 32 - 1) / (kThreads / 32);
+  if (ctas == 0) return cudaSuccess;
+  rotate_write_kernel<T, BITS, G, TURNS, VEC><<<unsigned(ctas < (1 << 20) ? ctas : (1 << 20)), kThreads, 0, st>>>(
+      a, run, int(items), int((items + run - 1) / run), int(runs(run)));
   return cudaGetLastError();
 }
 
-template <typename T, int BITS, int G>
+template <typename T, int BITS>
 cudaError_t launch_bits(const RotateArgs& a, cudaStream_t st) {
   // whole pieces of 8 values, with the rotation's ends on them, in q (and in the cache where its type stays)
-  const bool vec = a.vec_in && (BITS != 0 || a.vec_out) && a.D % 16 == 0 && a.rot % 16 == 0;
-  const int heads = a.Hq + (BITS == 0 ? 2 * a.Hkv : 0), per = vec ? a.D / 16 : a.rot / 2 + a.D - a.rot;
-  const int64_t items = int64_t(a.L) * heads * per, rows = BITS == 0 ? 0 : int64_t(2) * a.L * a.Hkv;
-  auto warps = [&](int n) { return int64_t(a.T) * ((items + 32 * n - 1) / (32 * n) + (rows + 4 * n - 1) / (4 * n)); };
-  if (warps(1) == 0) return cudaSuccess;
-  // several items per lane hide a call's latency, fewer give a small call more warps
-  const bool few = warps(4) < int64_t(device_sm_count()) * 8;
-  if (!vec) return few ? launch<T, BITS, G, 1, false>(a, warps(1), st) : launch<T, BITS, G, 4, false>(a, warps(4), st);
-  return few ? launch<T, BITS, G, 1, true>(a, warps(1), st) : launch<T, BITS, G, 4, true>(a, warps(4), st);
+  const bool vec = a.vec_in && (BITS != 0 || a.vec_out) && a.D % 16 == 0 && a.D <= 512 && a.rot % 16 == 0;
+  if constexpr (BITS == 4) {
+    if (a.rot == 0)
+      return a.D == 128 ? launch<T, 4, 4, kStay, true>(a, st) : (a.D == 64 ? launch<T, 4, 2, kStay, true>(a, st) : launch<T, 4, 0, kStay, true>(a, st));
+    if (vec && a.rot == a.D && !a.pairs && a.D == 64) return launch<T, 4, 2, kInLane, true>(a, st);
+  }
+  if constexpr (BITS != 0)
+    if (vec && a.rot == a.D && !a.pairs && a.D == 128) return launch<T, BITS, 4, kInLane, true>(a, st);
+  return vec ? launch<T, BITS, 0, kAny, true>(a, st) : launch<T, BITS, 0, kAny, false>(a, st);
 }
 
 template <typename T>
 cudaError_t launch_type(const RotateArgs& a, cudaStream_t st) {
-  if (a.bits == 0) return launch_bits<T, 0, 0>(a, st);
-  if (a.bits == 8) return a.D == 128 ? launch_bits<T, 8, 4>(a, st) : launch_bits<T, 8, 0>(a, st);
-  return a.D == 128 ? launch_bits<T, 4, 4>(a, st) : (a.D == 64 ? launch_bits<T, 4, 2>(a, st) : launch_bits<T, 4, 0>(a, st));
+  return a.bits == 0 ? launch_bits<T, 0>(a, st) : (a.bits == 8 ? launch_bits<T, 8>(a, st) : launch_bits<T, 4>(a, st));
 }
 
 }  // namespace
