@@ -196,13 +196,6 @@ __device__ __forceinline__ float over(float l) { return l == 0.0f ? 0.0f : 1.0f 
 // subnormals included, so one multiplication by a power of two, 2^(b - 127) with that put right, gives
 // the value exactly; a power of two outside the type takes a second one.  fp16 values past its range
 // become its largest.
-template <bool BF16>
-__device__ __forceinline__ uint32_t mul16x2(uint32_t x, uint32_t f) {
-  uint32_t r;
-  if constexpr (BF16) asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(f));
-  else asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(f));
-  return r;
-}
 // Whether one multiplication does for every byte of a word of scale bytes.
 template <bool BF16>
 __device__ __forceinline__ bool plain_scales(uint32_t w) {
@@ -276,56 +269,6 @@ __device__ __forceinline__ uint32_t mul_rest(uint32_t x, uint32_t f1, uint32_t f
     asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(x) : "r"(0xfbfffbffu));
   }
   return x;
-}
-// The 4-bit cache.  Eight values as 16-bit ones, times the power of two of their scale byte: fp16 by one conversion per
-// pair; for bf16 its exponent and first mantissa bit moved under bf16's exponent, where it reads as the value times
-// 2^-112.  Where no scale byte of a word is out of the ordinary one multiplication does:
-template <bool BF16>
-__device__ __forceinline__ bool plain_scales4(uint32_t w) {
-  return __vcmpgtu4(w, BF16 ? 0x8e8e8e8eu : 0x8c8c8c8cu) == 0 && (BF16 || __vcmpgtu4(0x71717171u, w) == 0);   // <= 142 (fp16: 113 .. 140)
-}
-template <bool BF16>
-__device__ __forceinline__ uint32_t plain_factor4(uint32_t b) {
-  return BF16 ? b * 0x00800080u + 0x38003800u : (b - 112u) * 0x04000400u;
-}
-template <bool BF16>
-__device__ __forceinline__ void widen4(uint32_t w, uint32_t f, uint32_t (&r)[4]) {
-  e2m1x8_f16(w, r[0], r[1], r[2], r[3]);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (BF16) {
-      const uint32_t m = r[i] & 0x7fff7fffu;
-      r[i] = (r[i] ^ m) | (m >> 3);
-    }
-    r[i] = mul16x2<BF16>(r[i], f);
-  }
-}
-// ... for any scale byte: two multiplications, of which only the last rounds; fp16 past its range: its largest.
-template <bool BF16>
-__device__ __forceinline__ void widen4_any(uint32_t w, uint32_t b, uint32_t (&r)[4]) {
-  uint32_t f0, f1;
-  if constexpr (BF16) {
-    const uint32_t e = min(b, 142u);
-    f0 = e * 0x00800080u + 0x38003800u;
-    f1 = (b - e + 127u) * 0x00800080u;
-  } else if (b < 113u) {                       // 2^-14, exact for what comes first, and the rest down to its subnormals
-    f0 = 0x04000400u;
-    f1 = (b >= 99u ? b - 98u << 10 : (b >= 89u ? 1u << b - 89u : 0u)) * 0x00010001u;
-  } else {
-    const uint32_t e = min(b, 140u);
-    f0 = (e - 112u) * 0x04000400u;
-    f1 = (min(b - e, 15u) + 15u) * 0x04000400u;
-  }
-  if (b >= kNan4) f1 = 0x7fff7fffu;            // NaN
-  widen4<BF16>(w, f0, r);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    r[i] = mul16x2<BF16>(r[i], f1);
-    if constexpr (!BF16) {
-      asm("min.NaN.f16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(0x7bff7bffu));
-      asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(0xfbfffbffu));
-    }
-  }
 }
 // What is not finite among two 16-bit values, in the halves `hide` (0xffff per half), becomes 0.
 template <bool BF16>

@@ -3,7 +3,7 @@
 // Bound by memory: per value 17 / 32 bytes of the cache and 2 of 16-bit rows.  Eight lanes per (token, layer,
 // plane, head): lane p takes the run of bytes that holds values 4 p .. 4 p + 3 of every group of 32 (one load for
 // head sizes 64 and 128) and writes four values per group, 64 bytes of 16-bit values from the eight lanes
-// together.  A warp takes four such rows at a time, kPasses times, of one token, whose session and slot it finds once.
+// together.  A warp takes kRun passes of four heads of one token, whose session and slot it finds once, plane by plane.
 #include <type_traits>
 
 #include "kernels.cuh"
@@ -14,7 +14,7 @@ namespace actkv {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kPasses = 4;
+constexpr int kRun = 8;
 
 // The slot of packed token t (one per warp), as an offset within a plane; -1 when no session's or (flagged) not held.
 __device__ __forceinline__ int64_t slot_of(const QuantMoveArgs& a, int t, int lane) {
@@ -30,113 +30,143 @@ __device__ __forceinline__ int64_t slot_of(const QuantMoveArgs& a, int t, int la
   return int64_t(phys) * a.rows_stride_b + int64_t(pos - lb * a.BS) * a.rows_stride_s;
 }
 
-// G: groups of a head (0: any number, one at a time).
-template <typename T, int G>
-__global__ void __launch_bounds__(kThreads) quant4_read_kernel(const __grid_constant__ QuantMoveArgs a) {
-  struct alignas(4 * sizeof(T)) Four {
-    T v[4];
-  };
-  auto narrow2 = [](float x, float y, T* p) {
-    if constexpr (sizeof(T) == 4) {
-      p[0] = x;
-      p[1] = y;
-    } else if constexpr (std::is_same<T, __half>::value) {   // past the range: the largest (NaN stays)
-      *reinterpret_cast<__half2*>(p) = __hmin2_nan(__hmax2_nan(__floats2half2_rn(x, y), __float2half2_rn(-65504.0f)),
-                                                   __float2half2_rn(65504.0f));
+template <typename T>
+struct alignas(4 * sizeof(T)) Four {
+  T v[4];
+};
+template <typename T>
+__device__ __forceinline__ void store4(T* p, const Four<T>& y, bool vec) {
+  if (vec) {
+    *reinterpret_cast<Four<T>*>(p) = y;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) p[k] = y.v[k];
+  }
+}
+
+// G: groups of a head, 2 or 4 (0: any number, one at a time).  What a lane reads of a row:
+template <int G>
+struct Raw {
+  uint32_t w[G / 2], scales;
+};
+template <int G>
+__device__ __forceinline__ Raw<G> load_raw(const uint8_t* at, const uint8_t* scale, bool vec) {
+  Raw<G> r;
+  if (vec) {
+    if constexpr (G == 4) {
+      const uint2 x = __ldcs(reinterpret_cast<const uint2*>(at));
+      r.w[0] = x.x;
+      r.w[G / 2 - 1] = x.y;
+      r.scales = *reinterpret_cast<const uint32_t*>(scale);
     } else {
-      *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(x, y);
+      r.w[0] = __ldcs(reinterpret_cast<const uint32_t*>(at));
+      r.scales = *reinterpret_cast<const uint16_t*>(scale) | 0x7f7f0000u;
     }
-  };
-  constexpr int kAt = G ? G : 1;
+  } else {
+    r.scales = G == 4 ? 0u : 0x7f7f0000u;
+#pragma unroll
+    for (int k = 0; k < G / 2; ++k) r.w[k] = 0;
+#pragma unroll
+    for (int k = 0; k < 2 * G; ++k) r.w[k / 4] |= uint32_t(at[k]) << (8 * (k % 4));
+#pragma unroll
+    for (int g = 0; g < G; ++g) r.scales |= uint32_t(scale[g]) << (8 * g);
+#pragma unroll
+    for (int k = 0; k < G / 2; ++k) asm("" : "+r"(r.w[k]));  // (see e2m1x8_f16)
+  }
+  return r;
+}
+template <typename T, int G>
+__device__ __forceinline__ void write(T* dst, const Raw<G>& r, bool vec) {
+  if constexpr (sizeof(T) == 2) {
+    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+    const bool plain = plain_scales4<BF16>(r.scales);
+#pragma unroll
+    for (int k = 0; k < G / 2; ++k) {
+      const uint32_t b0 = r.scales >> (16 * k) & 255u, b1 = r.scales >> (16 * k + 8) & 255u;
+      uint32_t y[4];
+      if (plain) {
+        widen4<BF16>(r.w[k], plain_factor4<BF16>(b0), plain_factor4<BF16>(b1), y);
+      } else {
+        uint32_t z[4];
+        widen4_any<BF16>(r.w[k], b0, y);
+        widen4_any<BF16>(r.w[k], b1, z);
+        y[2] = z[2];
+        y[3] = z[3];
+      }
+      store4<T>(dst + 64 * k, reinterpret_cast<const Four<T>&>(y[0]), vec);
+      store4<T>(dst + 64 * k + 32, reinterpret_cast<const Four<T>&>(y[2]), vec);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < G / 2; ++k) {
+      uint32_t h[4];
+      e2m1x8_f16(r.w[k], h[0], h[1], h[2], h[3]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float s = scale_of4(r.scales >> (16 * k + 8 * e) & 255u);
+        const float2 lo = f16x2_f32(h[2 * e]), hi = f16x2_f32(h[2 * e + 1]);
+        store4<T>(dst + 64 * k + 32 * e, Four<T>{lo.x * s, lo.y * s, hi.x * s, hi.y * s}, vec);
+      }
+    }
+  }
+}
+
+template <typename T, int G>
+__global__ void __launch_bounds__(kThreads) quant4_read_kernel(const __grid_constant__ QuantMoveArgs a, int runs) {
   const int lane = threadIdx.x & 31, p = lane & 7;
-  const int groups = G ? G : a.D / 32, rows = a.planes * a.Hkv;
-  const int runs = (rows + 4 * kPasses - 1) / (4 * kPasses);
-  const int shift = (a.Hkv & (a.Hkv - 1)) == 0 ? __ffs(a.Hkv) - 1 : -1;
+  const int groups = G ? G : a.D / 32, nb = (a.Hkv + 3) / 4, passes = a.planes * nb;
   const int64_t warp = (int64_t(blockIdx.x) * kThreads + threadIdx.x) >> 5;
   const int64_t nwarps = (int64_t(gridDim.x) * kThreads) >> 5;
-  int last = -1;
-  int64_t slot = -1;
-  for (int64_t w = warp; w < int64_t(a.T) * runs; w += nwarps) {
-    const int t = int(w / runs), run = int(w - int64_t(t) * runs);
-    if (t != last) slot = slot_of(a, t, lane);
-    last = t;
+  for (int64_t x = warp; x < int64_t(a.T) * runs; x += nwarps) {
+    const int t = int(x / runs), first = int(x - int64_t(t) * runs) * kRun;
+    const int64_t slot = slot_of(a, t, lane);
     if (slot < 0) continue;
-    for (int g0 = 0; g0 < groups; g0 += kAt) {
-      T* ext[kPasses];
-      uint32_t u[kPasses][(kAt + 1) / 2], sc[kPasses];
+    int n = min(kRun, passes - first), lp = first / nb, hb = first - lp * nb;
+    while (n > 0) {                           // the passes of one plane
+      const int m = min(n, nb - hb), h = 4 * hb + (lane >> 3), pl = a.both ? lp & 1 : a.only, l = a.both ? lp >> 1 : lp;
+      const int64_t step = 4 * a.ext_stride_h[pl];
+      T* dst = static_cast<T*>(pl ? a.v : a.k) + (int64_t(l) * a.ext_stride_l[pl] + int64_t(t) * a.ext_stride_t[pl] +
+                                                  int64_t(h) * a.ext_stride_h[pl] + 4 * p);
+      const uint8_t* row = a.rows + int64_t(l) * a.rows_stride_l + int64_t(pl) * a.rows_stride_kv + slot;
+      const uint8_t* at = row + h * (a.D / 2) + 2 * groups * p;
+      const uint8_t* scale = row + a.Hkv * (a.D / 2) + h * groups;
+      const int live = a.Hkv - h;             // heads from this lane's on
+      if constexpr (G > 0) {
+        constexpr int kAhead = 4;
+#pragma unroll 1
+        for (int i = 0; i < m; i += kAhead, dst += kAhead * step, at += kAhead * 4 * (G * 16), scale += kAhead * 4 * G) {
+          Raw<G> raw[kAhead];
 #pragma unroll
-      for (int i = 0; i < kPasses; ++i) {
-        const int f = (run * kPasses + i) * 4 + (lane >> 3);
-        ext[i] = nullptr;
-        if (f >= rows) continue;
-        const int lp = shift >= 0 ? f >> shift : f / a.Hkv, h = f - lp * a.Hkv;
-        const int l = a.both ? lp >> 1 : lp, pl = a.both ? lp & 1 : a.only;
-        ext[i] = static_cast<T*>(pl ? a.v : a.k) +
-                 (int64_t(l) * a.ext_stride_l[pl] + int64_t(t) * a.ext_stride_t[pl] + int64_t(h) * a.ext_stride_h[pl] + 4 * p + 32 * g0);
-        const uint8_t* row = a.rows + int64_t(l) * a.rows_stride_l + int64_t(pl) * a.rows_stride_kv + slot;
-        const uint8_t* at = row + h * (a.D / 2) + 2 * groups * p + 2 * g0;
-        const uint8_t* scale = row + a.Hkv * (a.D / 2) + h * groups + g0;
-        if (G == 4 && a.vec_rows) {
-          const uint2 x = __ldcs(reinterpret_cast<const uint2*>(at));
-          u[i][0] = x.x;
-          u[i][(kAt + 1) / 2 - 1] = x.y;
-          sc[i] = *reinterpret_cast<const uint32_t*>(scale);
-        } else if (G == 2 && a.vec_rows) {
-          u[i][0] = __ldcs(reinterpret_cast<const uint32_t*>(at));
-          sc[i] = *reinterpret_cast<const uint16_t*>(scale);
-        } else {
-          sc[i] = 0;
+          for (int e = 0; e < kAhead; ++e)
+            if (i + e < m && 4 * (i + e) < live) raw[e] = load_raw<G>(at + e * 4 * (G * 16), scale + e * 4 * G, a.vec_rows);
 #pragma unroll
-          for (int g = 0; g < kAt; ++g) {
-            const uint32_t two = uint32_t(at[2 * g]) | uint32_t(at[2 * g + 1]) << 8;
-            u[i][g / 2] = g & 1 ? u[i][g / 2] | two << 16 : two;
-            sc[i] |= uint32_t(scale[g]) << (8 * g);
-          }
+          for (int e = 0; e < kAhead; ++e)
+            if (i + e < m && 4 * (i + e) < live) write<T, G>(dst + e * step, raw[e], a.vec);
         }
-      }
-#pragma unroll
-      for (int i = 0; i < kPasses; ++i) {
-        if (!ext[i]) continue;
-#pragma unroll
-        for (int g = 0; g < kAt; g += 2) {
-          uint32_t h[4];
-          if constexpr (G > 0) {
-            e2m1x8_f16(u[i][g / 2], h[0], h[1], h[2], h[3]);
-          } else {
-            h[0] = e2m1x2_f16(u[i][0] & 255u);
-            h[1] = e2m1x2_f16(u[i][0] >> 8);
+      } else {
+        for (int i = 0; i < m && 4 * i < live; ++i, dst += step, at += 2 * a.D, scale += 4 * groups)
+          for (int g = 0; g < groups; ++g) {
+            const float2 lo = f16x2_f32(e2m1x2_f16(at[2 * g])), hi = f16x2_f32(e2m1x2_f16(at[2 * g + 1]));
+            const float s = scale_of4(scale[g]);
+            store4<T>(dst + 32 * g, Four<T>{from_f32<T>(lo.x * s), from_f32<T>(lo.y * s), from_f32<T>(hi.x * s), from_f32<T>(hi.y * s)}, a.vec);
           }
-#pragma unroll
-          for (int e = 0; e < 2 && g + e < kAt; ++e) {
-            const float s = scale_of4(sc[i] >> (8 * (g + e)) & 255u);
-            const float2 lo = f16x2_f32(h[2 * e]), hi = f16x2_f32(h[2 * e + 1]);
-            Four y;
-            narrow2(lo.x * s, lo.y * s, y.v);
-            narrow2(hi.x * s, hi.y * s, y.v + 2);
-            T* dst = ext[i] + 32 * (g + e);
-            if (a.vec) {
-              *reinterpret_cast<Four*>(dst) = y;
-            } else {
-#pragma unroll
-              for (int k = 0; k < 4; ++k) dst[k] = y.v[k];
-            }
-          }
-        }
       }
+      n -= m;
+      hb = 0;
+      ++lp;
     }
   }
 }
 
 template <typename T>
 cudaError_t launch(const QuantMoveArgs& a, cudaStream_t st) {
-  const int rows = a.planes * a.Hkv;
-  const int64_t warps = int64_t(a.T) * ((rows + 4 * kPasses - 1) / (4 * kPasses));
-  const int64_t ctas = (warps + kThreads / 32 - 1) / (kThreads / 32);
+  const int runs = (a.planes * ((a.Hkv + 3) / 4) + kRun - 1) / kRun;
+  const int64_t ctas = (int64_t(a.T) * runs + kThreads / 32 - 1) / (kThreads / 32);
   const int grid = int(ctas < (1 << 20) ? ctas : (1 << 20));
   if (grid <= 0) return cudaSuccess;
-  if (a.D == 128) quant4_read_kernel<T, 4><<<grid, kThreads, 0, st>>>(a);
-  else if (a.D == 64) quant4_read_kernel<T, 2><<<grid, kThreads, 0, st>>>(a);
-  else quant4_read_kernel<T, 0><<<grid, kThreads, 0, st>>>(a);
+  if (a.D == 128) quant4_read_kernel<T, 4><<<grid, kThreads, 0, st>>>(a, runs);
+  else if (a.D == 64) quant4_read_kernel<T, 2><<<grid, kThreads, 0, st>>>(a, runs);
+  else quant4_read_kernel<T, 0><<<grid, kThreads, 0, st>>>(a, runs);
   return cudaGetLastError();
 }
 

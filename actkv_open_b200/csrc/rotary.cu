@@ -11,7 +11,7 @@
 // warp that works on the token, from L2.  A warp takes a run of one token's passes:
 //   where the type stays, a pass is 16 values per lane (two pieces of 8 that turn together: 16-byte accesses) of as
 //     many heads as 32 lanes hold; a lane's dims are the same in every pass, so its sines and cosines stay in registers;
-//   into rows, a pass is four heads, eight lanes each, lane p holding values 4 p .. 4 p + 3 of every group of 32, which
+//   into rows, a pass is four heads of a plane, eight lanes each, lane p holding values 4 p .. 4 p + 3 of every group of 32, which
 //     is what the 4-bit row keeps together, and a group's maximum is three shuffles (of two groups at once where the
 //     values are 16-bit and do not turn).
 #include "kernels.cuh"
@@ -89,16 +89,6 @@ template <typename T> __device__ __forceinline__ T narrow(float x);
 template <> __device__ __forceinline__ float narrow<float>(float x) { return x; }
 template <> __device__ __forceinline__ __half narrow<__half>(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-
-// a / b for a small unsigned a: a shift where b is a power of two.
-struct Divisor {
-  int b, shift;
-  __device__ __forceinline__ explicit Divisor(int n) {
-    b = n;
-    shift = (n & (n - 1)) == 0 ? __ffs(n) - 1 : -1;
-  }
-  __device__ __forceinline__ int operator()(int a) const { return shift >= 0 ? a >> shift : a / b; }
-};
 
 __device__ __forceinline__ void narrow2(float2 x, float* p) {
   p[0] = x.x;
@@ -288,14 +278,13 @@ __device__ __forceinline__ void tops(const float (&x)[N][4], uint32_t (&top)[N])
 // in one lane; or in any way, the other value of a pair fetched from memory.
 enum Turns { kStay, kInLane, kAny };
 
-// Passes [first, first + n) of token t's 2 L Hkv (layer, plane, head) rows: four rows each, eight lanes per row.
+// Passes [first, first + n) of token t, plane by plane (k's, then v's, of each layer): four heads each, eight lanes per head.
 // G: groups of a head (0: any number, a.D / 32, one at a time).
 template <typename T, int BITS, int G, Turns TURNS>
-__device__ __forceinline__ void quantise(const RotateArgs& a, int t, int first, int n, int rows, const Token& tok,
+__device__ __forceinline__ void quantise(const RotateArgs& a, int t, int first, int n, const Token& tok,
                                          const float* angles, int lane) {
-  const int p = lane & 7, groups = G ? G : a.D / 32;
+  const int p = lane & 7, groups = G ? G : a.D / 32, nb = (a.Hkv + 3) / 4;
   [[maybe_unused]] const int half = a.rot / 2;
-  const Divisor by_heads(a.Hkv);
   constexpr int kAt = G ? G : 1;              // groups at a time
   [[maybe_unused]] float4 c[(kAt + 1) / 2], s[(kAt + 1) / 2];
   if constexpr (TURNS == kInLane) {
@@ -305,32 +294,48 @@ __device__ __forceinline__ void quantise(const RotateArgs& a, int t, int first, 
       s[g] = __ldg(reinterpret_cast<const float4*>(angles + half + 32 * g + 4 * p));
     }
   }
-  // A lane's rows past the last are the last once more, not stored: the shuffles are the whole warp's.
-  auto source = [&](int f, int& w) -> const T* {
-    const int lp = by_heads(f), h = f - lp * a.Hkv, l = lp >> 1;
-    w = 1 + (lp & 1);
-    return static_cast<const T*>(a.in[w]) + (int64_t(l) * a.in_l[w] + int64_t(t) * a.in_t[w] + int64_t(h) * a.in_h[w]) + 4 * p;
+  // A lane's heads past the last are the last once more, not stored: the shuffles are the whole warp's.
+  auto source = [&](int lp, int hb) -> const T* {
+    const bool k = (lp & 1) == 0;
+    return static_cast<const T*>(k ? a.in[1] : a.in[2]) +
+           (int64_t(lp >> 1) * (k ? a.in_l[1] : a.in_l[2]) + int64_t(t) * (k ? a.in_t[1] : a.in_t[2]) +
+            int64_t(min(4 * hb + (lane >> 3), a.Hkv - 1)) * (k ? a.in_h[1] : a.in_h[2])) + 4 * p;
   };
-  const int steps = groups / kAt;             // of a pass
+  int lp = first / nb, hb = first - lp * nb;  // the pass
+  const T* src = source(lp, hb);
   Piece<T, 4> ahead[kAt];                     // the next step's values
-  auto fetch = [&](int i) {
-    int w;
-    const int pass = G ? i : i / steps, g0 = G ? 0 : i - pass * steps;
-    const T* src = source(min(4 * (first + pass) + (lane >> 3), rows - 1), w);
 #pragma unroll
-    for (int g = 0; g < kAt; ++g) ahead[g] = load<T, 4>(src + 32 * (g0 + g), a.vec_in);
-  };
-  fetch(0);
+  for (int g = 0; g < kAt; ++g) ahead[g] = load<T, 4>(src + 32 * g, a.vec_in);
+  uint8_t* plane = static_cast<uint8_t*>(a.cache) + (int64_t(lp >> 1) * a.c_l + int64_t(lp & 1) * a.c_kv + tok.at);
 #pragma unroll 1
-  for (int i = 0; i < n * steps; ++i) {
-    const int pass = G ? i : i / steps, g0 = G ? 0 : i - pass * steps;
+  for (int i = 0, g0 = 0; i < n;) {
     Piece<T, 4> raw[kAt];
 #pragma unroll
     for (int g = 0; g < kAt; ++g) raw[g] = ahead[g];
-    if (i + 1 < n * steps) fetch(i + 1);
-    const int f0 = 4 * (first + pass) + (lane >> 3), f = min(f0, rows - 1);
-    const int lp = by_heads(f), h = f - lp * a.Hkv;
-    const bool turns = TURNS != kStay && (lp & 1) == 0;
+    // the step after this one
+    const int this_lp = lp, this_hb = hb, this_g = g0;
+    uint8_t* const this_plane = plane;
+    [[maybe_unused]] const T* const this_src = src;
+    g0 += kAt;
+    if (g0 >= groups) {
+      g0 = 0;
+      ++i;
+      if (++hb == nb) {
+        hb = 0;
+        ++lp;
+        plane = static_cast<uint8_t*>(a.cache) + (int64_t(lp >> 1) * a.c_l + int64_t(lp & 1) * a.c_kv + tok.at);
+        src = source(min(lp, 2 * a.L - 1), hb);
+      } else if (4 * hb + 4 <= a.Hkv) {
+        src += 4 * (lp & 1 ? a.in_h[2] : a.in_h[1]);
+      } else {
+        src = source(lp, hb);
+      }
+    }
+    if (i < n) {
+#pragma unroll
+      for (int g = 0; g < kAt; ++g) ahead[g] = load<T, 4>(src + 32 * (g0 + g), a.vec_in);
+    }
+    const bool turns = TURNS != kStay && (this_lp & 1) == 0;
     float x[kAt][4];
 #pragma unroll
     for (int g = 0; g < kAt; ++g)
@@ -340,39 +345,34 @@ __device__ __forceinline__ void quantise(const RotateArgs& a, int t, int first, 
       if (turns) {
 #pragma unroll
         for (int g = 0; g < kAt / 2; ++g) {
-        turn(x[g][0], x[g + kAt / 2][0], c[g].x, s[g].x);
-        turn(x[g][1], x[g + kAt / 2][1], c[g].y, s[g].y);
-        turn(x[g][2], x[g + kAt / 2][2], c[g].z, s[g].z);
-        turn(x[g][3], x[g + kAt / 2][3], c[g].w, s[g].w);
-      }
+          turn(x[g][0], x[g + kAt / 2][0], c[g].x, s[g].x);
+          turn(x[g][1], x[g + kAt / 2][1], c[g].y, s[g].y);
+          turn(x[g][2], x[g + kAt / 2][2], c[g].z, s[g].z);
+          turn(x[g][3], x[g + kAt / 2][3], c[g].w, s[g].w);
+        }
       }
     } else if constexpr (TURNS == kAny) {
-      if (turns) {
-#pragma unroll
-      for (int g = 0; g < kAt; ++g) {
-        const int d = 32 * (g0 + g) + 4 * p;
-        if (d >= a.rot) continue;
+      const int d = 32 * this_g + 4 * p;
+      if (turns && d < a.rot) {
         if (a.pairs) {
-          turn(x[g][0], x[g][1], __ldg(angles + d / 2), __ldg(angles + half + d / 2));
-          turn(x[g][2], x[g][3], __ldg(angles + d / 2 + 1), __ldg(angles + half + d / 2 + 1));
+          turn(x[0][0], x[0][1], __ldg(angles + d / 2), __ldg(angles + half + d / 2));
+          turn(x[0][2], x[0][3], __ldg(angles + d / 2 + 1), __ldg(angles + half + d / 2 + 1));
         } else {                              // the other values of the pairs, from memory
           const bool low = d < half;
-          int w;
-          const Piece<T, 4> other = load<T, 4>(source(f, w) + 32 * (g0 + g) + (low ? half : -half), a.vec_in);
+          const Piece<T, 4> other = load<T, 4>(this_src + 32 * this_g + (low ? half : -half), a.vec_in);
           const float* at = angles + (low ? d : d - half);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            float u = low ? x[g][k] : to_f32(other.v[k]), v = low ? to_f32(other.v[k]) : x[g][k];
+            float u = low ? x[0][k] : to_f32(other.v[k]), v = low ? to_f32(other.v[k]) : x[0][k];
             turn(u, v, __ldg(at + k), __ldg(at + half + k));
-            x[g][k] = low ? u : v;
+            x[0][k] = low ? u : v;
           }
         }
       }
     }
-    }
     uint32_t top[kAt];
     if constexpr (sizeof(T) == 2) {
-      if (TURNS != kStay && __any_sync(0xffffffffu, turns)) tops<kAt>(x, top);
+      if (turns) tops<kAt>(x, top);           // (the same for the whole warp)
       else tops<T, kAt>(raw, top);
     } else {
       tops<kAt>(x, top);
@@ -390,20 +390,20 @@ __device__ __forceinline__ void quantise(const RotateArgs& a, int t, int first, 
       packed[g] = b == 255u ? 0u : u;
       bytes |= b << (8 * g);
     }
-    if (f0 >= rows) continue;
-    uint8_t* row = static_cast<uint8_t*>(a.cache) + (int64_t(lp >> 1) * a.c_l + int64_t(lp & 1) * a.c_kv + tok.at);
-    uint8_t* vals = row + h * (a.D * BITS / 8);
-    uint8_t* scales = row + a.Hkv * (a.D * BITS / 8) + h * groups + g0;
+    const int h = 4 * this_hb + (lane >> 3);
+    if (h >= a.Hkv) continue;
+    uint8_t* vals = this_plane + h * (a.D * BITS / 8);
+    uint8_t* scales = this_plane + a.Hkv * (a.D * BITS / 8) + h * groups + this_g;
     if constexpr (BITS == 8) {
 #pragma unroll
       for (int g = 0; g < kAt; ++g) {
-        uint8_t* dst = vals + 32 * (g0 + g) + 4 * p;
+        uint8_t* dst = vals + 32 * (this_g + g) + 4 * p;
         if (a.vec_out) *reinterpret_cast<uint32_t*>(dst) = packed[g];
         else
           for (int k = 0; k < 4; ++k) dst[k] = uint8_t(packed[g] >> (8 * k));
       }
     } else {
-      uint8_t* dst = vals + 2 * groups * p + 2 * g0;
+      uint8_t* dst = vals + 2 * groups * p + 2 * this_g;
       if (G == 4 && a.vec_out) {
         *reinterpret_cast<uint2*>(dst) = make_uint2(__byte_perm(packed[0], packed[kAt > 1 ? 1 : 0], 0x5410),
                                                     __byte_perm(packed[kAt > 2 ? 2 : 0], packed[kAt > 3 ? 3 : 0], 0x5410));
@@ -435,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, BITS == 0 || TURNS == kStay ? 8 : 5)
   const int lane = threadIdx.x & 31;
   const int64_t warp = (int64_t(blockIdx.x) * kThreads + threadIdx.x) >> 5;
   const int64_t nwarps = (int64_t(gridDim.x) * kThreads) >> 5;
-  const int rows = BITS == 0 ? 0 : 2 * a.L * a.Hkv;
+  const int row_passes = BITS == 0 ? 0 : 2 * a.L * ((a.Hkv + 3) / 4);
   for (int64_t w = warp; w < int64_t(a.T) * runs; w += nwarps) {
     const int t = int(w / runs), which = int(w - int64_t(t) * runs);
     const float* angles = nullptr;
@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, BITS == 0 || TURNS == kStay ? 8 : 5)
       else any_layout<T>(a, t, first * 32, n * 32, tok, angles, lane);
     } else if constexpr (BITS != 0) {
       const int first = (which - item_runs) * run;
-      if (tok.at >= 0) quantise<T, BITS, G, TURNS>(a, t, first, min(run, (rows + 3) / 4 - first), rows, tok, angles, lane);
+      if (tok.at >= 0) quantise<T, BITS, G, TURNS>(a, t, first, min(run, row_passes - first), tok, angles, lane);
     }
   }
 }
@@ -458,7 +458,7 @@ cudaError_t launch(const RotateArgs& a, cudaStream_t st) {
   const int64_t items = TURNS == kStay ? 0 : VEC
       ? int64_t(a.L) * ((a.Hq + block - 1) / block + (BITS == 0 ? 2 * ((a.Hkv + block - 1) / block) : 0))
       : (int64_t(a.L) * (a.Hq + (BITS == 0 ? 2 * a.Hkv : 0)) * (a.rot / 2 + a.D - a.rot) + 31) / 32;
-  const int64_t rows = BITS == 0 ? 0 : (int64_t(2) * a.L * a.Hkv + 3) / 4;
+  const int64_t rows = BITS == 0 ? 0 : int64_t(2) * a.L * ((a.Hkv + 3) / 4);
   auto runs = [&](int run) { return (items + run - 1) / run + (rows + run - 1) / run; };
   // long runs find a token once for more work, short ones give a small call more warps
   int run = 8;
