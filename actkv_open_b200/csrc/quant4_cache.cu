@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kThreads) quant4_read_kernel(const __grid_cons
   const int64_t warp = (int64_t(blockIdx.x) * kThreads + threadIdx.x) >> 5;
   const int64_t nwarps = (int64_t(gridDim.x) * kThreads) >> 5;
   for (int64_t x = warp; x < int64_t(a.T) * runs; x += nwarps) {
-    const int t = int(x / runs), first = int(x - int64_t(t) * runs) * kRun;
+    const int t = x >> 31 ? int(x / runs) : int(uint32_t(x) / uint32_t(runs)), first = int(x - int64_t(t) * runs) * kRun;
     const int64_t slot = slot_of(a, t, lane);
     if (slot < 0) continue;
     int n = min(kRun, passes - first), lp = first / nb, hb = first - lp * nb;

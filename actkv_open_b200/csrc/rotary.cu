@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, BITS == 0 || TURNS == kStay ? 8 : 5)
   const int64_t nwarps = (int64_t(gridDim.x) * kThreads) >> 5;
   const int row_passes = BITS == 0 ? 0 : 2 * a.L * ((a.Hkv + 3) / 4);
   for (int64_t w = warp; w < int64_t(a.T) * runs; w += nwarps) {
-    const int t = int(w / runs), which = int(w - int64_t(t) * runs);
+    const int t = w >> 31 ? int(w / runs) : int(uint32_t(w) / uint32_t(runs)), which = int(w - int64_t(t) * runs);
     const float* angles = nullptr;
     const Token tok = find(a, t, lane, angles);
     if (!tok.live) continue;
@@ -461,7 +461,7 @@ cudaError_t launch(const RotateArgs& a, cudaStream_t st) {
   const int64_t rows = BITS == 0 ? 0 : int64_t(2) * a.L * ((a.Hkv + 3) / 4);
   auto runs = [&](int run) { return (items + run - 1) / run + (rows + run - 1) / run; };
   // long runs find a token once for more work, short ones give a small call more warps
-  int run = 8;
+  int run = 16;
   while (run > 1 && a.T * runs(run) < int64_t(device_sm_count()) * 16) run /= 2;
   const int64_t warps = a.T * runs(run), ctas = (warps + kThreads / 32 - 1) / (kThreads / 32);
   if (ctas == 0) return cudaSuccess;
