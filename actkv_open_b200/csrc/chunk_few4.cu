@@ -31,7 +31,7 @@ constexpr int kStep = 32;                   // tokens per step of a warp
 constexpr int kWarps = 16, kThreads = kWarps * 32;
 constexpr int kRoundCost = 3;               // a unit's fixed cost in rounds of its warps
 constexpr int kMinRounds = 3;               // a CTA's share is at least so many: fewer partial results to join
-constexpr int kRowsMax = 8;                 // query rows
+constexpr float kPBits = 7.0f;              // p, and l with it, is held times 2^7 (kPScale, here by way of the exponent)
 
 template <int D>
 struct Ring4 {
@@ -79,6 +79,18 @@ __device__ __forceinline__ uint32_t as_fp16(uint32_t h, uint32_t b_lo, uint32_t 
   return reinterpret_cast<const uint32_t&>(y);
 }
 
+// The low half bytes of u with the high ones of v.
+__device__ __forceinline__ uint32_t low_halves(uint32_t u, uint32_t v) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, 0x0f0f0f0f, 0xe4;" : "=r"(r) : "r"(u), "r"(v));
+  return r;
+}
+// The first product of a sum.
+__device__ __forceinline__ void mma16816_new(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_constant__ ChunkArgs a, bool vec_out) {
   using Rg = Ring4<D>;
@@ -88,11 +100,20 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
   extern __shared__ __align__(1024) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r8 = lane >> 2, c4 = lane & 3;
+  auto value_piece = [&](int t) -> uint32_t { return t * (D / 2) + (D == 128 ? piece<D>(t, r8 >> 1) * 16 + (r8 & 1) * 8 : r8 * 4); };
   Sched& sched = *reinterpret_cast<Sched*>(smem + Rg::kSmemBytes - 512);
   const int cta = blockIdx.x, n_cta = gridDim.x;
   const uint32_t ring = smem_u32(smem) + warp * Rg::kWarpBytes, table_at = ring + Rg::kStages * Rg::kStage;
   const unsigned full = 0xffffffffu;
   const float ninf = -__int_as_float(0x7f800000);
+  // where the lane reads within a stage and the tables; tiles of 16 tokens, and 8 tokens within one, are constant steps on
+  const int row_tok = token_of(r8);
+  const uint32_t key_at = row_tok * (D / 2) + (D == 128 ? piece<D>(row_tok, c4) * 16 : c4 * 8);
+  const uint32_t value_at = value_piece(token_of(2 * c4));  // ... and the other token's of the pair: the bit of token 1 turned
+  const uint32_t key_scale = table_at + row_tok * (G * 4), value_scale = table_at + Rg::kKeyScale + c4 * (G * 4);
+  // ... and where it puts its token's: the second of a pair of tokens takes the second half of the groups
+  const int odd = token_of(lane & 7) & 1;
+  const uint32_t pair_at = table_at + Rg::kKeyScale + ((lane >> 3) * 4 + (token_of(lane & 7) >> 1)) * (G * 4) + odd * (G * 2);
   const Parts ps = few_parts(a.workspace, n_cta);
   pdl_trigger();
   if (threadIdx.x == 0) {
@@ -112,36 +133,36 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
     flag_long(a, S);
     return int64_t(a.Hkv / HG) * (kRoundCost + (held_tokens(a, S) + round - 1) / round);
   }, sched.share, sched.scan, cta, n_cta, kMinRounds);
-  const int64_t total = sched.share.total;
-  const int n_used = used_ctas(total, n_cta, kMinRounds);
-  const int64_t lo = total * cta / n_used, hi = total * (cta + 1) / n_used;
-  if (cta >= n_used || lo >= hi) return;
+  // The share is [lo, lo + span) of the schedule; places in it are kept relative to lo, in 32 bits (registers are short).
+  auto n_used = [&] { return used_ctas(sched.share.total, n_cta, kMinRounds); };
+  auto low = [&] { return sched.share.total * cta / n_used(); };
+  if (cta >= n_used()) return;
+  const int span = int(sched.share.total * (cta + 1) / n_used() - low());
+  if (span <= 0) return;
   int r = sched.share.r0;
-  int64_t at = sched.share.pre;              // start of (session r, head group hg) in the schedule
+  int at = int(sched.share.pre - low());     // start of (session r, head group hg) in the schedule
   int hg = 0;
   bool seek = true;
   const float c2 = a.scale * kLog2e;
-  const char* kv = static_cast<const char*>(a.kv);
-  const int64_t stride_s = a.kv_stride_s, stride_b = a.kv_stride_b, to_values = a.kv_stride_kv;
   const int shift = (a.BS & (a.BS - 1)) == 0 ? __ffs(a.BS) - 1 : -1;
   auto block_of = [&](int tok) { return shift >= 0 ? tok >> shift : tok / a.BS; };
+  auto bytes_at = [&](int64_t off) { return static_cast<const char*>(a.kv) + off; };
 
-  for (; r < a.R && at < hi; ++r, hg = 0) {
-    const int a0 = a.q_off[r], A = new_tokens(a, r), S = a.seq_used[r];
+  for (; r < a.R && at < span; ++r, hg = 0) {
+    const int A = new_tokens(a, r), S = a.seq_used[r];
     if (A == 0 || A * a.G > few_rows) continue;
     const int rows = A * a.G;
-    const int nt = (held_tokens(a, S) + round - 1) / round;
-    const int64_t weight = kRoundCost + nt;
+    const int nt = (held_tokens(a, S) + round - 1) / round, weight = kRoundCost + nt;
     if (seek) {                               // the group that holds lo
-      hg = int((lo - at) / weight);
+      hg = -at / weight;
       at += hg * weight;
       seek = false;
     }
     const int32_t* table = a.block_table + r * a.bt_stride_r;
-    for (; hg < a.Hkv / HG && at < hi; ++hg, at += weight) {
-      const int64_t first = at + kRoundCost;
-      const int t0 = int(lo > first ? lo - first : 0), t1 = nt == 0 ? 0 : int(min(int64_t(nt), hi - first));
-      if (nt == 0 ? at < lo : t0 >= t1) continue;
+    for (; hg < a.Hkv / HG && at < span; ++hg, at += weight) {
+      const int first = at + kRoundCost;
+      const int t0 = max(-first, 0), t1 = nt == 0 ? 0 : min(nt, span - first);
+      if (nt == 0 ? at < 0 : t0 >= t1) continue;
       const int h = hg * HG + my_head;
       const int begin = t0 * round, end = min(t1 * round, held_tokens(a, S));
       const int start = begin + my_part * kStep;              // this warp's steps: start, start + round, ...
@@ -153,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
       uint32_t q[2 * G][2];
       {
         const int jq = r8 / a.G;
-        const uint16_t* p = static_cast<const uint16_t*>(a.q) + (int64_t(a0) + jq) * a.q_stride_t +
+        const uint16_t* p = static_cast<const uint16_t*>(a.q) + (int64_t(a.q_off[r]) + jq) * a.q_stride_t +
                             int64_t(h * a.G + r8 - jq * a.G) * a.q_stride_h;
 #pragma unroll
         for (int k = 0; k < 2 * G; ++k) {
@@ -204,33 +225,33 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
         return lb < a.MB ? table[lb] : -1;
       };
       int phys = look_up(0);
-      const char* head = kv + int64_t(h) * (D / 2);
+      const char* const head = static_cast<const char*>(a.kv) + (h * (D / 2) + lane % CH * 16);
       const int at_word = a.Hkv * (D / 2) + (D == 128 ? h * 4 : (h * 2) & ~3);
       const int sh = D == 64 && (h & 1) ? 16 : 0;             // the head's bytes within the word
       bool gaps = false;                      // this lane met a block outside the cache: from there on every step looks
       auto issue = [&](int i, int slot) {
         if (i < mine) {
           const int tok = start + i * round + lane;
-          const bool none = uint32_t(phys) >= uint32_t(a.NB); // past the end, or an id outside the cache: zeros
+          const bool none = uint32_t(phys) >= uint32_t(a.NB); // past the end, or an id outside the cache
           if (none && tok < end) {
             flag(a.status, ACTKV_DEV_BAD_INDEX);
             gaps = true;
           }
-          const int in_block = shift >= 0 ? tok & (a.BS - 1) : tok % a.BS;
-          const int64_t off = none ? -1 : int64_t(phys) * stride_b + int64_t(in_block) * stride_s;
-          const uint32_t dst = ring + slot * Rg::kStage;
+          // The token's place, in tokens (blocks are whole and in order, and all of them fewer than 2^31, a token's bytes too).
+          // One that is not there takes the cache's first: it is hidden, and nothing of a hidden token counts.
+          const uint32_t place = none ? 0u : uint32_t(phys * a.BS + (shift >= 0 ? tok & (a.BS - 1) : tok % a.BS));
+          const uint32_t stride = uint32_t(a.kv_stride_s), dst = ring + slot * Rg::kStage;
 #pragma unroll
           for (int e = 0; e < kCopies; ++e) {
-            const int row = e * kRowsPerCopy + lane / CH, c = lane % CH;
-            const int64_t from = __shfl_sync(full, off, row);
-            const char* p = (from < 0 ? kv : head + from) + c * 16;
-            const uint32_t to = dst + row * (CH * 16) + piece<D>(row, c) * 16;
-            copy16(to, p, from >= 0);
-            copy16(to + Rg::kPlane, p + to_values, from >= 0);
+            const int row = e * kRowsPerCopy + lane / CH;
+            const char* p = head + uint64_t(__shfl_sync(full, place, row)) * stride;
+            const uint32_t to = dst + row * (CH * 16) + piece<D>(row, lane % CH) * 16;
+            copy16(to, p, true);
+            copy16(to + Rg::kPlane, p + a.kv_stride_kv, true);
           }
-          const char* w = kv + (off < 0 ? 0 : off + at_word);
-          copy4(dst + 2 * Rg::kPlane + lane * 4, w, off >= 0);
-          copy4(dst + 2 * Rg::kPlane + kStep * 4 + lane * 4, w + to_values, off >= 0);
+          const char* w = static_cast<const char*>(a.kv) + at_word + uint64_t(place) * stride;
+          copy4(dst + 2 * Rg::kPlane + lane * 4, w, true);
+          copy4(dst + 2 * Rg::kPlane + kStep * 4 + lane * 4, w + a.kv_stride_kv, true);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
         phys = look_up(i + 1);
@@ -303,7 +324,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
             uint32_t b = byte_of(wk, g);
             if constexpr (EDGE && !BF16)
               if (b < kNan4) b = held(b);
-            ks[g] = EDGE && b >= kNan4 ? __int_as_float(0x7fffffff) : pow2_of(b);
+            // (of a step with nothing out of the ordinary, byte 0 as 0: such keys are below 2^-124)
+            ks[g] = EDGE ? (b >= kNan4 ? __int_as_float(0x7fffffff) : pow2_of(b)) : __uint_as_float(b << 23);
           }
           if (__any_sync(full, __vcmpgtu4(vs, E0) != 0)) {    // (E0 and E1 are equal where some token is common)
             uint32_t n = __vmaxu4(vs, E0);
@@ -311,58 +333,66 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
             for (int x = 1; x < 32; x *= 2) n = __vmaxu4(n, __shfl_xor_sync(full, n, x));
             raise_scale(n, n);
           }
-          if constexpr (G == 4)
-            *reinterpret_cast<float4*>(smem + (table_at - smem_u32(smem)) + lane * 16) = make_float4(ks[0], ks[1], ks[2], ks[3]);
-          else
-            *reinterpret_cast<float2*>(smem + (table_at - smem_u32(smem)) + lane * 8) = make_float2(ks[0], ks[1]);
+          uint8_t* const tables = smem + (table_at - smem_u32(smem));
+          if constexpr (G == 4) *reinterpret_cast<float4*>(tables + lane * 16) = make_float4(ks[0], ks[1], ks[G - 2], ks[G - 1]);
+          else *reinterpret_cast<float2*>(tables + lane * 8) = make_float2(ks[0], ks[1]);
           uint32_t f[G / 2];
+          const uint32_t down = E0 - vs;      // by byte: no byte of vs is above E0's
 #pragma unroll
           for (int g = 0; g < G; g += 2) {
             float x[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              x[e] = pow2(byte_of(vs, g + e) - byte_of(E0, g + e));
+              x[e] = __uint_as_float(uint32_t(max(127 - byte_of(down, g + e), 0)) << 23);
               if (EDGE && ((common >> lane & 1u) == 0 || byte_of(wv, g + e) >= int(kNan4))) x[e] = 0.0f;
             }
             f[g / 2] = pack2<false>(x[0], x[1]);
           }
-          uint8_t* ft = smem + (table_at - smem_u32(smem)) + Rg::kKeyScale;
-          if constexpr (G == 4) *reinterpret_cast<uint2*>(ft + lane * 8) = make_uint2(f[0], f[G / 2 - 1]);
-          else *reinterpret_cast<uint32_t*>(ft + lane * 4) = f[0];
+          // by pair of tokens and group, the pair's factors: each of the two lanes puts half of the groups
+          if constexpr (G == 4) {
+            const uint32_t got = __shfl_xor_sync(full, odd ? f[0] : f[G / 2 - 1], 1);
+            const uint32_t lo = odd ? got : f[0], hi = odd ? f[G / 2 - 1] : got;
+            *reinterpret_cast<uint2*>(smem + (pair_at - smem_u32(smem))) =
+                make_uint2(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
+          } else {
+            const uint32_t got = __shfl_xor_sync(full, f[0], 1);
+            *reinterpret_cast<uint32_t*>(smem + (pair_at - smem_u32(smem))) =
+                odd ? __byte_perm(got, f[0], 0x7632) : __byte_perm(f[0], got, 0x5410);
+          }
         }
         __syncwarp();
-        // ---- S^T = K Q^T: s[n][0..1] token 16 n + token_of(r8), s[n][2..3] the one 8 on, query rows 2 c4 and 2 c4 + 1
-        float s[kTiles][4];
-#pragma unroll
+        // Tile by tile of 16 tokens, in a loop: both at once take more registers than there are.
+#pragma unroll 1
         for (int n = 0; n < kTiles; ++n) {
-          const int tk0 = 16 * n + token_of(r8), tk1 = tk0 + 8;
+          // ---- S^T = K Q^T: s[0..1] token 16 n + token_of(r8), s[2..3] the one 8 on, query rows 2 c4 and 2 c4 + 1
+          float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          const uint32_t tile_k = kb + key_at + n * (16 * D / 2), tile_ks = key_scale + n * (16 * G * 4);
+          [[maybe_unused]] const int tk0 = 16 * n + row_tok, tk1 = tk0 + 8;
           uint32_t w[2][4];                   // by token: words of pieces 2 c4 and 2 c4 + 1
           float ks[2][G];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const int tk = e ? tk1 : tk0;
+            const int on = 8 * e;
             if constexpr (D == 128) {
-              const uint4 u = lds16(kb + tk * 64 + piece<D>(tk, c4) * 16);
+              const uint4 u = lds16(tile_k + on * 64);
               w[e][0] = u.x;
               w[e][1] = u.y;
               w[e][2] = u.z;
               w[e][3] = u.w;
-              const uint4 f = lds16(table_at + tk * 16);
+              const uint4 f = lds16(tile_ks + on * 16);
               ks[e][0] = __uint_as_float(f.x);
               ks[e][1] = __uint_as_float(f.y);
               ks[e][G - 2] = __uint_as_float(f.z);
               ks[e][G - 1] = __uint_as_float(f.w);
             } else {
-              const uint2 u = lds8(kb + tk * 32 + c4 * 8);
+              const uint2 u = lds8(tile_k + on * 32);
               w[e][0] = u.x;
               w[e][1] = u.y;
-              const uint2 f = lds8(table_at + tk * 8);
+              const uint2 f = lds8(tile_ks + on * 8);
               ks[e][0] = __uint_as_float(f.x);
               ks[e][1] = __uint_as_float(f.y);
             }
           }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
 #pragma unroll
           for (int g2 = 0; g2 < G / 2; ++g2) {
             // of two groups: x[token][piece][byte]
@@ -385,78 +415,73 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
                     for (int k = 0; k < 2; ++k) x[e][pc][2 * gg + k] = as_fp16(x[e][pc][2 * gg + k], b, b);
                 }
               }
-              float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+              float c[4];
 #pragma unroll
               for (int pc = 0; pc < 2; ++pc) {
                 const uint32_t m[4] = {x[0][pc][2 * gg], x[1][pc][2 * gg], x[0][pc][2 * gg + 1], x[1][pc][2 * gg + 1]};
-                mma16816<false>(c, m, q[2 * g + pc][0], q[2 * g + pc][1]);
+                if (pc == 0) mma16816_new(c, m, q[2 * g + pc][0], q[2 * g + pc][1]);
+                else mma16816<false>(c, m, q[2 * g + pc][0], q[2 * g + pc][1]);
               }
+              // (powers of two: the same digits with the queries' or without, but so a scale of any size stays in range)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float k = ks[e >> 1][g];
-                // (powers of two: the same digits either way, but a scale of any size stays in range)
-                s[n][e] = EDGE ? fmaf(c[e], k * (e & 1 ? qs1 : qs0), s[n][e]) : fmaf(c[e], k, s[n][e]);
-              }
+              for (int e = 0; e < 4; ++e)
+                s[e] = fmaf(c[e], EDGE ? ks[e >> 1][g] * (e & 1 ? qs1 : qs0) : ks[e >> 1][g], s[e]);
             }
           }
           if constexpr (EDGE) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int tk = e >> 1 ? tk1 : tk0;
-              s[n][e] = t + tk <= (e & 1 ? lim1 : lim0) && (there >> tk & 1u) ? s[n][e] : ninf;
+              s[e] = t + tk <= (e & 1 ? lim1 : lim0) && (there >> tk & 1u) ? s[e] : ninf;
             }
           }
-        }
-        // (the product rounded before the difference, not in one step with it: the largest logit's is then 0 whatever its size)
-        const float f0 = EDGE ? c2 : cq0, f1 = EDGE ? c2 : cq1;
+          // (the product rounded before the difference, not in one step with it: the largest logit's is then 0 whatever its size)
+          const float f0 = EDGE ? c2 : cq0, f1 = EDGE ? c2 : cq1;
 #pragma unroll
-        for (int n = 0; n < kTiles; ++n)
+          for (int e = 0; e < 4; ++e) s[e] = __fmul_rn(s[e], e & 1 ? f1 : f0);
+          float top0 = fmaxf(s[0], s[2]), top1 = fmaxf(s[1], s[3]);
+          if (__any_sync(full, top0 > m0 + kSlack || top1 > m1 + kSlack)) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][e] = __fmul_rn(s[n][e], e & 1 ? f1 : f0);
-        float top0 = fmaxf(s[0][0], s[0][2]), top1 = fmaxf(s[0][1], s[0][3]);
-#pragma unroll
-        for (int n = 1; n < kTiles; ++n) {
-          top0 = fmaxf(top0, fmaxf(s[n][0], s[n][2]));
-          top1 = fmaxf(top1, fmaxf(s[n][1], s[n][3]));
-        }
-        if (__any_sync(full, top0 > m0 + kSlack || top1 > m1 + kSlack)) {
-#pragma unroll
-          for (int x = 4; x < 32; x *= 2) {
-            top0 = fmaxf(top0, __shfl_xor_sync(full, top0, x));
-            top1 = fmaxf(top1, __shfl_xor_sync(full, top1, x));
+            for (int x = 4; x < 32; x *= 2) {
+              top0 = fmaxf(top0, __shfl_xor_sync(full, top0, x));
+              top1 = fmaxf(top1, __shfl_xor_sync(full, top1, x));
+            }
+            raise(top0, top1);
           }
-          raise(top0, top1);
-        }
-        const float b0 = m0 == ninf ? 0.0f : m0, b1 = m1 == ninf ? 0.0f : m1;
+          const float b0 = (m0 == ninf ? 0.0f : m0) - kPBits, b1 = (m1 == ninf ? 0.0f : m1) - kPBits;
 #pragma unroll
-        for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][e] = ex2(__fsub_rn(s[n][e], e & 1 ? b1 : b0));
-#pragma unroll
-        for (int n = 0; n < kTiles; ++n) {
-          l0 += s[n][0] + s[n][2];
-          l1 += s[n][1] + s[n][3];
-        }
-        // ---- O^T += V^T p^T: the lane's tokens are those of rows 2 c4, 2 c4 + 1 and 8 on, its dims 4 r8 .. + 3 of each group
-        if (!EDGE || common) {
-#pragma unroll
-          for (int n = 0; n < kTiles; ++n) {
-            const uint32_t p0 = transpose8x8(pack_p<false>(s[n][0], s[n][1])), p1 = transpose8x8(pack_p<false>(s[n][2], s[n][3]));
-            const int tok[4] = {16 * n + token_of(2 * c4), 16 * n + token_of(2 * c4 + 1), 16 * n + 8 + token_of(2 * c4),
-                                16 * n + 8 + token_of(2 * c4 + 1)};
-            uint32_t vw[4][G / 2], ft[4][G / 2];
+          for (int e = 0; e < 4; ++e) s[e] = ex2(__fsub_rn(s[e], e & 1 ? b1 : b0));
+          l0 += s[0] + s[2];
+          l1 += s[1] + s[3];
+          // ---- O^T += V^T p^T: the lane's tokens are those of rows 2 c4, 2 c4 + 1 and 8 on, its dims 4 r8 .. + 3 of each group
+          if (!EDGE || common) {
+            const uint32_t tile_v0 = vb + value_at + n * (16 * D / 2), tile_v1 = vb + (value_at ^ uint32_t(D / 2)) + n * (16 * D / 2);
+            const uint32_t tile_vs = value_scale + n * (8 * G * 4);
+            const uint32_t p0 = transpose8x8(pack2<false>(s[0], s[1])), p1 = transpose8x8(pack2<false>(s[2], s[3]));
+            uint32_t vw[4][G / 2], ft[2][G];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
+              const int on = 8 * (e >> 1);
               if constexpr (D == 128) {
-                const uint2 u = lds8(vb + tok[e] * 64 + piece<D>(tok[e], r8 >> 1) * 16 + (r8 & 1) * 8);
+                const uint2 u = lds8((e & 1 ? tile_v1 : tile_v0) + on * 64);
                 vw[e][0] = u.x;
                 vw[e][G / 2 - 1] = u.y;
-                const uint2 f = lds8(table_at + Rg::kKeyScale + tok[e] * 8);
-                ft[e][0] = f.x;
-                ft[e][G / 2 - 1] = f.y;
               } else {
-                vw[e][0] = lds4(vb + tok[e] * 32 + r8 * 4);
-                ft[e][0] = lds4(table_at + Rg::kKeyScale + tok[e] * 4);
+                vw[e][0] = lds4((e & 1 ? tile_v1 : tile_v0) + on * 32);
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              if constexpr (G == 4) {
+                const uint4 f = lds16(tile_vs + e * 4 * (G * 4));
+                ft[e][0] = f.x;
+                ft[e][1] = f.y;
+                ft[e][G - 2] = f.z;
+                ft[e][G - 1] = f.w;
+              } else {
+                const uint2 f = lds8(tile_vs + e * 4 * (G * 4));
+                ft[e][0] = f.x;
+                ft[e][1] = f.y;
               }
             }
 #pragma unroll
@@ -466,8 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
 #pragma unroll
               for (int pr = 0; pr < 2; ++pr) {
                 const uint32_t u = vw[2 * pr][g2], v = vw[2 * pr + 1][g2];
-                const uint32_t even = (u & 0x0f0f0f0fu) | ((v << 4) & 0xf0f0f0f0u);
-                const uint32_t odd = ((u >> 4) & 0x0f0f0f0fu) | (v & 0xf0f0f0f0u);
+                const uint32_t even = low_halves(u, v * 16u), odd = low_halves(u >> 4, v);
                 e2m1x8_f16(even, x[pr][0][0], x[pr][0][1], x[pr][0][2], x[pr][0][3]);
                 e2m1x8_f16(odd, x[pr][1][0], x[pr][1][1], x[pr][1][2], x[pr][1][3]);
               }
@@ -477,17 +501,16 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
                 if constexpr (EDGE && !BF16) {
 #pragma unroll
                   for (int pr = 0; pr < 2; ++pr) {
-                    const uint32_t b_lo = lds4(sb + (kStep + tok[2 * pr]) * 4) >> (sh + 8 * g) & 255u;
-                    const uint32_t b_hi = lds4(sb + (kStep + tok[2 * pr + 1]) * 4) >> (sh + 8 * g) & 255u;
+                    const uint32_t at = sb + (kStep + 16 * n + 8 * pr) * 4;
+                    const uint32_t b_lo = lds4(at + token_of(2 * c4) * 4) >> (sh + 8 * g) & 255u;
+                    const uint32_t b_hi = lds4(at + token_of(2 * c4 + 1) * 4) >> (sh + 8 * g) & 255u;
 #pragma unroll
                     for (int od = 0; od < 2; ++od)
 #pragma unroll
                       for (int k = 0; k < 2; ++k) x[pr][od][2 * gg + k] = as_fp16(x[pr][od][2 * gg + k], b_lo, b_hi);
                   }
                 }
-                const uint32_t sel = gg ? 0x7632 : 0x5410;
-                const uint32_t pg0 = mul16x2<false>(p0, __byte_perm(ft[0][g2], ft[1][g2], sel));
-                const uint32_t pg1 = mul16x2<false>(p1, __byte_perm(ft[2][g2], ft[3][g2], sel));
+                const uint32_t pg0 = mul16x2<false>(p0, ft[0][g]), pg1 = mul16x2<false>(p1, ft[1][g]);
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                   const uint32_t m[4] = {x[0][0][2 * gg + k], x[0][1][2 * gg + k], x[1][0][2 * gg + k], x[1][1][2 * gg + k]};
@@ -496,24 +519,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
               }
             }
           }
-        }
-        // ---- tokens that some row does not see, one by one
-        if constexpr (EDGE) {
+          // ---- tokens that some row does not see, one by one
+          if constexpr (EDGE) {
 #pragma unroll 1
-          for (uint32_t some = there & ~common; some; some &= some - 1) {
+          for (uint32_t some = there & ~common & 0xffffu << (16 * n); some; some &= some - 1) {
             const int tk = __ffs(some) - 1, of = tk & 7;
             // p of the lane's two rows: from the lanes of the product's row that the token is
-            float x0 = 0.0f, x1 = 0.0f;
-#pragma unroll
-            for (int n = 0; n < kTiles; ++n)
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-                if ((tk >> 3) == 2 * n + e) {
-                  x0 = s[n][2 * e];
-                  x1 = s[n][2 * e + 1];
-                }
-            x0 = __shfl_sync(full, x0, token_of(of) * 4 + c4) * kPScale<false>;
-            x1 = __shfl_sync(full, x1, token_of(of) * 4 + c4) * kPScale<false>;
+            const float x0 = __shfl_sync(full, tk & 8 ? s[2] : s[0], token_of(of) * 4 + c4);
+            const float x1 = __shfl_sync(full, tk & 8 ? s[3] : s[1], token_of(of) * 4 + c4);
             const bool see0 = t + tk <= lim0, see1 = t + tk <= lim1;
             const uint32_t word = lds4(sb + (kStep + tk) * 4) >> sh;
             uint32_t seen = 0;                // its scale bytes, NaN without
@@ -543,6 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
                 o[2 * g + k][3] = fmaf(g1, y.y, o[2 * g + k][3]);
               }
             }
+          }
           }
         }
       };
@@ -581,6 +595,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
         l0 += __shfl_xor_sync(full, l0, x);
         l1 += __shfl_xor_sync(full, l1, x);
       }
+      l0 *= 1.0f / kPScale<false>;
+      l1 *= 1.0f / kPScale<false>;
       {
         constexpr float kBack = BF16 ? 1.0f / kPScale<false> : 1.0f;
 #pragma unroll
@@ -638,7 +654,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
           if (row >= rows) continue;
           const float L = hf ? l1 : l0, M = hf ? m1 : m0, inv = over<BF16>(L);
           const int jq = row / a.G, hq = h * a.G + row - jq * a.G, hr = my_head * rows + row;
-          const int64_t qt = int64_t(a0) + jq;
+          const int64_t qt = int64_t(a.q_off[r]) + jq;
           uint16_t* dst = static_cast<uint16_t*>(a.out) + qt * a.out_stride_t + int64_t(hq) * a.out_stride_h;
           float* part = ps.out(cta, ps_slot) + int64_t(hr) * D;
           // NaN groups among the values of tokens that this row does see
@@ -649,8 +665,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
             for (int t = begin; t <= last; ++t) {
               const int lb = block_of(t), ph = lb < a.MB ? table[lb] : -1;
               if (ph < 0 || ph >= a.NB) continue;
-              const uint8_t* p = reinterpret_cast<const uint8_t*>(kv) + to_values + int64_t(ph) * stride_b +
-                                 int64_t(t - lb * a.BS) * stride_s + a.Hkv * (D / 2) + h * G;
+              const uint8_t* p = reinterpret_cast<const uint8_t*>(
+                  bytes_at(a.kv_stride_kv + (int64_t(ph) * a.BS + (t - lb * a.BS)) * a.kv_stride_s)) + a.Hkv * (D / 2) + h * G;
 #pragma unroll
               for (int g = 0; g < G; ++g) nan |= p[g] >= kNan4 ? 1u << g : 0u;
             }
@@ -688,13 +704,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
         ds.r = r;
         ds.h = hg * HG;
         ds.heads = HG;
-        ds.n_used = n_used;
+        ds.n_used = n_used();
         ds.ntok = A;
         ds.S = S;
         ds.A = A;
-        ds.a0 = a0;
-        ds.end = first + nt;
-        ds.total = total;
+        ds.a0 = a.q_off[r];
+        ds.end = low() + first + nt;
+        ds.total = sched.share.total;
         ps.desc[cta] = ds;
       }
       __syncthreads();                        // the rings are written again
