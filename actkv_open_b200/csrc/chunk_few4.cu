@@ -39,13 +39,14 @@ struct Ring4 {
   static constexpr int kChunks = D / 32;                    // 16-byte pieces of a row
   static constexpr uint32_t kPlane = kStep * D / 2;         // keys, then values
   static constexpr uint32_t kStage = 2 * kPlane + 2 * kStep * 4;        // and their scale words
-  static constexpr int kStages = D == 128 ? 3 : 6;
+  static constexpr int kStages = D == 128 ? 2 : 4;          // (a step takes a warp 3 us: one ahead is enough)
   // a step's scales as its products take them: of keys in 32 bits, of values in fp16 relative to E
   static constexpr uint32_t kKeyScale = kStep * G * 4, kTable = kKeyScale + kStep * G * 2;
   static constexpr uint32_t kWarpBytes = kStages * kStage + kTable;
   static constexpr int kJoin = (D / 16 * 4 + 4) * 32;       // a warp's O, m, l as floats
   static constexpr uint32_t kBytes = kWarps * kWarpBytes, kJoinBytes = kWarps * kJoin * 4;
-  static constexpr uint32_t kSmemBytes = (kBytes > kJoinBytes ? kBytes : kJoinBytes) + 512;
+  static constexpr uint32_t kQ = kBytes > kJoinBytes ? kBytes : kJoinBytes, kQBytes = 8 * G * 512;   // 8 heads' queries
+  static constexpr uint32_t kSmemBytes = kQ + kQBytes + 512;
   static_assert(kSmemBytes <= 232448, "exceeds the 227 KB of shared memory a CTA can have");
 };
 
@@ -206,13 +207,24 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
         qs0 = __shfl_sync(full, back, 4 * row0);
         qs1 = __shfl_sync(full, back, 4 * row1);
       }
+      // ... in shared memory, the head's first warp putting them there: they are read again for every tile
+      if (my_part == 0) {
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+          *reinterpret_cast<uint4*>(smem + Rg::kQ + (my_head * G + g) * 512 + lane * 16) =
+              make_uint4(q[2 * g][0], q[2 * g][1], q[2 * g + 1][0], q[2 * g + 1][1]);
+      }
+      __syncthreads();
       const float cq0 = c2 * qs0, cq1 = c2 * qs1;
+      const uint32_t q_at = smem_u32(smem) + Rg::kQ + my_head * (G * 512) + lane * 16;
       float o[kOut][4];
 #pragma unroll
       for (int j = 0; j < kOut; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
       float m0 = ninf, m1 = ninf, l0 = 0.0f, l1 = 0.0f;
+      float up0 = ninf, up1 = ninf;           // what a row's maximum may be before its m is raised
+      float base0 = -kPBits, base1 = -kPBits; // m less the power of two that p is held times; 0 less it before any token
       // by group (a byte each), what O is relative to, 2^(E - 127), for the two rows; equal until tokens are added one by one
       uint32_t E0 = 0, E1 = 0;
       auto byte_of = [](uint32_t w, int g) { return int(w >> (8 * g) & 255u); };
@@ -260,10 +272,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
       // the references of rows that have outgrown theirs go up to the maxima given (the same in all lanes of a row; each
       // row by its own tokens alone, so that what others see does not show in its digits)
       auto raise = [&](float top0, float top1) {
-        const float n0 = top0 > m0 + kSlack ? top0 : m0, n1 = top1 > m1 + kSlack ? top1 : m1;
+        const float n0 = top0 > up0 ? top0 : m0, n1 = top1 > up1 ? top1 : m1;
         const float e0 = m0 == n0 ? 1.0f : ex2(m0 - n0), e1 = m1 == n1 ? 1.0f : ex2(m1 - n1);
         m0 = n0;
         m1 = n1;
+        up0 = m0 + kSlack;
+        up1 = m1 + kSlack;
+        base0 = (m0 == ninf ? 0.0f : m0) - kPBits;
+        base1 = (m1 == ninf ? 0.0f : m1) - kPBits;
         l0 *= e0;
         l1 *= e1;
 #pragma unroll
@@ -361,54 +377,51 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
           }
         }
         __syncwarp();
-        // Tile by tile of 16 tokens, in a loop: both at once take more registers than there are.
-#pragma unroll 1
-        for (int n = 0; n < kTiles; ++n) {
-          // ---- S^T = K Q^T: s[0..1] token 16 n + token_of(r8), s[2..3] the one 8 on, query rows 2 c4 and 2 c4 + 1
-          float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          const uint32_t tile_k = kb + key_at + n * (16 * D / 2), tile_ks = key_scale + n * (16 * G * 4);
-          [[maybe_unused]] const int tk0 = 16 * n + row_tok, tk1 = tk0 + 8;
-          uint32_t w[2][4];                   // by token: words of pieces 2 c4 and 2 c4 + 1
-          float ks[2][G];
+        // ---- S^T = K Q^T: s[n][0..1] token 16 n + token_of(r8), s[n][2..3] the one 8 on, query rows 2 c4 and 2 c4 + 1
+        float s[kTiles][4];
+        uint32_t w[kTiles][2][2 * (G / 2)];   // by tile and token: words of pieces 2 c4 and 2 c4 + 1
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const int on = 8 * e;
+            const int on = 16 * n + 8 * e;
             if constexpr (D == 128) {
-              const uint4 u = lds16(tile_k + on * 64);
-              w[e][0] = u.x;
-              w[e][1] = u.y;
-              w[e][2] = u.z;
-              w[e][3] = u.w;
-              const uint4 f = lds16(tile_ks + on * 16);
-              ks[e][0] = __uint_as_float(f.x);
-              ks[e][1] = __uint_as_float(f.y);
-              ks[e][G - 2] = __uint_as_float(f.z);
-              ks[e][G - 1] = __uint_as_float(f.w);
+              const uint4 u = lds16(kb + key_at + on * 64);
+              w[n][e][0] = u.x;
+              w[n][e][1] = u.y;
+              w[n][e][G - 2] = u.z;
+              w[n][e][G - 1] = u.w;
             } else {
-              const uint2 u = lds8(tile_k + on * 32);
-              w[e][0] = u.x;
-              w[e][1] = u.y;
-              const uint2 f = lds8(tile_ks + on * 8);
-              ks[e][0] = __uint_as_float(f.x);
-              ks[e][1] = __uint_as_float(f.y);
+              const uint2 u = lds8(kb + key_at + on * 32);
+              w[n][e][0] = u.x;
+              w[n][e][1] = u.y;
             }
           }
 #pragma unroll
-          for (int g2 = 0; g2 < G / 2; ++g2) {
+        for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
+#pragma unroll
+        for (int g2 = 0; g2 < G / 2; ++g2) {
+          const uint4 q0 = lds16(q_at + 2 * g2 * 512), q1 = lds16(q_at + (2 * g2 + 1) * 512);
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n) {
             // of two groups: x[token][piece][byte]
             uint32_t x[2][2][4];
+            uint2 ks[2];
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int e = 0; e < 2; ++e) {
+              ks[e] = lds8(key_scale + (16 * n + 8 * e) * (G * 4) + g2 * 8);
 #pragma unroll
               for (int pc = 0; pc < 2; ++pc)
-                e2m1x8_f16(w[e][pc * (G / 2) + g2], x[e][pc][0], x[e][pc][1], x[e][pc][2], x[e][pc][3]);
+                e2m1x8_f16(w[n][e][pc * (G / 2) + g2], x[e][pc][0], x[e][pc][1], x[e][pc][2], x[e][pc][3]);
+            }
 #pragma unroll
             for (int gg = 0; gg < 2; ++gg) {
-              const int g = 2 * g2 + gg;
               if constexpr (EDGE && !BF16) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                  const uint32_t b = lds4(sb + (e ? tk1 : tk0) * 4) >> (sh + 8 * g) & 255u;
+                  const uint32_t b = lds4(sb + (16 * n + 8 * e + row_tok) * 4) >> (sh + 8 * (2 * g2 + gg)) & 255u;
 #pragma unroll
                   for (int pc = 0; pc < 2; ++pc)
 #pragma unroll
@@ -416,70 +429,87 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
                 }
               }
               float c[4];
+              const uint4 qg = gg ? q1 : q0;
 #pragma unroll
               for (int pc = 0; pc < 2; ++pc) {
                 const uint32_t m[4] = {x[0][pc][2 * gg], x[1][pc][2 * gg], x[0][pc][2 * gg + 1], x[1][pc][2 * gg + 1]};
-                if (pc == 0) mma16816_new(c, m, q[2 * g + pc][0], q[2 * g + pc][1]);
-                else mma16816<false>(c, m, q[2 * g + pc][0], q[2 * g + pc][1]);
+                if (pc == 0) mma16816_new(c, m, qg.x, qg.y);
+                else mma16816<false>(c, m, qg.z, qg.w);
               }
               // (powers of two: the same digits with the queries' or without, but so a scale of any size stays in range)
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                s[e] = fmaf(c[e], EDGE ? ks[e >> 1][g] * (e & 1 ? qs1 : qs0) : ks[e >> 1][g], s[e]);
+              for (int e = 0; e < 4; ++e) {
+                const float k = __uint_as_float(gg ? ks[e >> 1].y : ks[e >> 1].x);
+                s[n][e] = fmaf(c[e], EDGE ? k * (e & 1 ? qs1 : qs0) : k, s[n][e]);
+              }
             }
           }
-          if constexpr (EDGE) {
+        }
+        if constexpr (EDGE) {
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int tk = e >> 1 ? tk1 : tk0;
-              s[e] = t + tk <= (e & 1 ? lim1 : lim0) && (there >> tk & 1u) ? s[e] : ninf;
+              const int tk = 16 * n + 8 * (e >> 1) + row_tok;
+              s[n][e] = t + tk <= (e & 1 ? lim1 : lim0) && (there >> tk & 1u) ? s[n][e] : ninf;
             }
+        }
+        // (the product rounded before the difference, not in one step with it: the largest logit's is then 0 whatever its size)
+        const float f0 = EDGE ? c2 : cq0, f1 = EDGE ? c2 : cq1;
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][e] = __fmul_rn(s[n][e], e & 1 ? f1 : f0);
+        float top0 = fmaxf(s[0][0], s[0][2]), top1 = fmaxf(s[0][1], s[0][3]);
+#pragma unroll
+        for (int n = 1; n < kTiles; ++n) {
+          top0 = fmaxf(top0, fmaxf(s[n][0], s[n][2]));
+          top1 = fmaxf(top1, fmaxf(s[n][1], s[n][3]));
+        }
+        if (__any_sync(full, top0 > up0 || top1 > up1)) {
+#pragma unroll
+          for (int x = 4; x < 32; x *= 2) {
+            top0 = fmaxf(top0, __shfl_xor_sync(full, top0, x));
+            top1 = fmaxf(top1, __shfl_xor_sync(full, top1, x));
           }
-          // (the product rounded before the difference, not in one step with it: the largest logit's is then 0 whatever its size)
-          const float f0 = EDGE ? c2 : cq0, f1 = EDGE ? c2 : cq1;
+          raise(top0, top1);
+        }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[e] = __fmul_rn(s[e], e & 1 ? f1 : f0);
-          float top0 = fmaxf(s[0], s[2]), top1 = fmaxf(s[1], s[3]);
-          if (__any_sync(full, top0 > m0 + kSlack || top1 > m1 + kSlack)) {
+        for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-            for (int x = 4; x < 32; x *= 2) {
-              top0 = fmaxf(top0, __shfl_xor_sync(full, top0, x));
-              top1 = fmaxf(top1, __shfl_xor_sync(full, top1, x));
-            }
-            raise(top0, top1);
-          }
-          const float b0 = (m0 == ninf ? 0.0f : m0) - kPBits, b1 = (m1 == ninf ? 0.0f : m1) - kPBits;
+          for (int e = 0; e < 4; ++e) s[n][e] = ex2(__fsub_rn(s[n][e], e & 1 ? base1 : base0));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[e] = ex2(__fsub_rn(s[e], e & 1 ? b1 : b0));
-          l0 += s[0] + s[2];
-          l1 += s[1] + s[3];
-          // ---- O^T += V^T p^T: the lane's tokens are those of rows 2 c4, 2 c4 + 1 and 8 on, its dims 4 r8 .. + 3 of each group
-          if (!EDGE || common) {
-            const uint32_t tile_v0 = vb + value_at + n * (16 * D / 2), tile_v1 = vb + (value_at ^ uint32_t(D / 2)) + n * (16 * D / 2);
-            const uint32_t tile_vs = value_scale + n * (8 * G * 4);
-            const uint32_t p0 = transpose8x8(pack2<false>(s[0], s[1])), p1 = transpose8x8(pack2<false>(s[2], s[3]));
+        for (int n = 0; n < kTiles; ++n) {
+          l0 += s[n][0] + s[n][2];
+          l1 += s[n][1] + s[n][3];
+        }
+        // ---- O^T += V^T p^T: the lane's tokens are those of rows 2 c4, 2 c4 + 1 and 8 on, its dims 4 r8 .. + 3 of each group
+        if (!EDGE || common) {
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n) {
+            const uint32_t p0 = transpose8x8(pack2<false>(s[n][0], s[n][1])), p1 = transpose8x8(pack2<false>(s[n][2], s[n][3]));
             uint32_t vw[4][G / 2], ft[2][G];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int on = 8 * (e >> 1);
+              const int on = 16 * n + 8 * (e >> 1);
               if constexpr (D == 128) {
-                const uint2 u = lds8((e & 1 ? tile_v1 : tile_v0) + on * 64);
+                const uint2 u = lds8(vb + (e & 1 ? value_at ^ 64u : value_at) + on * 64);
                 vw[e][0] = u.x;
                 vw[e][G / 2 - 1] = u.y;
               } else {
-                vw[e][0] = lds4((e & 1 ? tile_v1 : tile_v0) + on * 32);
+                vw[e][0] = lds4(vb + (e & 1 ? value_at ^ 32u : value_at) + on * 32);
               }
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               if constexpr (G == 4) {
-                const uint4 f = lds16(tile_vs + e * 4 * (G * 4));
+                const uint4 f = lds16(value_scale + (2 * n + e) * 4 * (G * 4));
                 ft[e][0] = f.x;
                 ft[e][1] = f.y;
                 ft[e][G - 2] = f.z;
                 ft[e][G - 1] = f.w;
               } else {
-                const uint2 f = lds8(tile_vs + e * 4 * (G * 4));
+                const uint2 f = lds8(value_scale + (2 * n + e) * 4 * (G * 4));
                 ft[e][0] = f.x;
                 ft[e][1] = f.y;
               }
@@ -519,14 +549,24 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
               }
             }
           }
-          // ---- tokens that some row does not see, one by one
-          if constexpr (EDGE) {
+        }
+        // ---- tokens that some row does not see, one by one
+        if constexpr (EDGE) {
 #pragma unroll 1
-          for (uint32_t some = there & ~common & 0xffffu << (16 * n); some; some &= some - 1) {
+          for (uint32_t some = there & ~common; some; some &= some - 1) {
             const int tk = __ffs(some) - 1, of = tk & 7;
             // p of the lane's two rows: from the lanes of the product's row that the token is
-            const float x0 = __shfl_sync(full, tk & 8 ? s[2] : s[0], token_of(of) * 4 + c4);
-            const float x1 = __shfl_sync(full, tk & 8 ? s[3] : s[1], token_of(of) * 4 + c4);
+            float x0 = 0.0f, x1 = 0.0f;
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if ((tk >> 3) == 2 * n + e) {
+                  x0 = s[n][2 * e];
+                  x1 = s[n][2 * e + 1];
+                }
+            x0 = __shfl_sync(full, x0, token_of(of) * 4 + c4);
+            x1 = __shfl_sync(full, x1, token_of(of) * 4 + c4);
             const bool see0 = t + tk <= lim0, see1 = t + tk <= lim1;
             const uint32_t word = lds4(sb + (kStep + tk) * 4) >> sh;
             uint32_t seen = 0;                // its scale bytes, NaN without
@@ -556,7 +596,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
                 o[2 * g + k][3] = fmaf(g1, y.y, o[2 * g + k][3]);
               }
             }
-          }
           }
         }
       };
