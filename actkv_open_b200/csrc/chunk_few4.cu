@@ -31,6 +31,7 @@ constexpr int kStep = 32;                   // tokens per step of a warp
 constexpr int kWarps = 16, kThreads = kWarps * 32;
 constexpr int kRoundCost = 3;               // a unit's fixed cost in rounds of its warps
 constexpr int kMinRounds = 3;               // a CTA's share is at least so many: fewer partial results to join
+constexpr float kLowest = -3.0e38f;         // m of a row before its first token: below any logit, and finite
 constexpr float kPBits = 7.0f;              // p, and l with it, is held times 2^7 (kPScale, here by way of the exponent)
 
 template <int D>
@@ -46,7 +47,7 @@ struct Ring4 {
   static constexpr int kJoin = (D / 16 * 4 + 4) * 32;       // a warp's O, m, l as floats
   static constexpr uint32_t kBytes = kWarps * kWarpBytes, kJoinBytes = kWarps * kJoin * 4;
   static constexpr uint32_t kQ = kBytes > kJoinBytes ? kBytes : kJoinBytes, kQBytes = 8 * G * 512;   // 8 heads' queries
-  static constexpr uint32_t kSmemBytes = kQ + kQBytes + 512;
+  static constexpr uint32_t kBack = kQ + kQBytes, kSmemBytes = kBack + 8 * 32 + 512;    // ... what undoes their power of two
   static_assert(kSmemBytes <= 232448, "exceeds the 227 KB of shared memory a CTA can have");
 };
 
@@ -80,6 +81,10 @@ __device__ __forceinline__ uint32_t as_fp16(uint32_t h, uint32_t b_lo, uint32_t 
   return reinterpret_cast<const uint32_t&>(y);
 }
 
+// Keeps a value in a register that the compiler would work out again at every use (of the 630 instructions of a step 70
+// were such).
+template <typename T>
+__device__ __forceinline__ void keep(T& x) { asm volatile("" : "+r"(x)); }
 // The low half bytes of u with the high ones of v.
 __device__ __forceinline__ uint32_t low_halves(uint32_t u, uint32_t v) {
   uint32_t r;
@@ -99,7 +104,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
   constexpr int kOut = D / 16;                // products of O: two per group
   constexpr int kTiles = kStep / 16;
   extern __shared__ __align__(1024) uint8_t smem[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
+  int lane = threadIdx.x & 31;
+  keep(lane);
   const int r8 = lane >> 2, c4 = lane & 3;
   auto value_piece = [&](int t) -> uint32_t { return t * (D / 2) + (D == 128 ? piece<D>(t, r8 >> 1) * 16 + (r8 & 1) * 8 : r8 * 4); };
   Sched& sched = *reinterpret_cast<Sched*>(smem + Rg::kSmemBytes - 512);
@@ -109,12 +116,19 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
   const float ninf = -__int_as_float(0x7f800000);
   // where the lane reads within a stage and the tables; tiles of 16 tokens, and 8 tokens within one, are constant steps on
   const int row_tok = token_of(r8);
-  const uint32_t key_at = row_tok * (D / 2) + (D == 128 ? piece<D>(row_tok, c4) * 16 : c4 * 8);
-  const uint32_t value_at = value_piece(token_of(2 * c4));  // ... and the other token's of the pair: the bit of token 1 turned
-  const uint32_t key_scale = table_at + row_tok * (G * 4), value_scale = table_at + Rg::kKeyScale + c4 * (G * 4);
+  uint32_t key_at = row_tok * (D / 2) + (D == 128 ? piece<D>(row_tok, c4) * 16 : c4 * 8);
+  uint32_t value_at = value_piece(token_of(2 * c4));  // ... and the other token's of the pair: the bit of token 1 turned
+  uint32_t key_scale = table_at + row_tok * (G * 4), value_scale = table_at + Rg::kKeyScale + c4 * (G * 4);
   // ... and where it puts its token's: the second of a pair of tokens takes the second half of the groups
   const int odd = token_of(lane & 7) & 1;
-  const uint32_t pair_at = table_at + Rg::kKeyScale + ((lane >> 3) * 4 + (token_of(lane & 7) >> 1)) * (G * 4) + odd * (G * 2);
+  uint32_t pair_at = table_at + Rg::kKeyScale + ((lane >> 3) * 4 + (token_of(lane & 7) >> 1)) * (G * 4) + odd * (G * 2);
+  uint32_t copy_at = lane / CH * (CH * 16) + piece<D>(lane / CH, lane % CH) * 16;
+  keep(key_at);
+  keep(value_at);
+  keep(key_scale);
+  keep(value_scale);
+  keep(pair_at);
+  keep(copy_at);
   const Parts ps = few_parts(a.workspace, n_cta);
   pdl_trigger();
   if (threadIdx.x == 0) {
@@ -168,9 +182,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
       const int begin = t0 * round, end = min(t1 * round, held_tokens(a, S));
       const int start = begin + my_part * kStep;              // this warp's steps: start, start + round, ...
       const int mine = start < end ? (end - start + round - 1) / round : 0;
-      // the lane's two query rows, and the last tokens they see
-      const int row0 = 2 * c4, row1 = row0 + 1;
-      const int lim0 = S - A + row0 / a.G, lim1 = S - A + row1 / a.G;
+      // the lane's two query rows; the first sees the tokens up to all + row0 / G, the second up to all + row1 / G
+      const int row0 = 2 * c4, row1 = row0 + 1, all = S - A;
       // ---- queries as the second operand, row r8: of k-step (group g, i) dims 32 g + 8 c4 + 4 i .. + 3
       uint32_t q[2 * G][2];
       {
@@ -184,8 +197,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
           q[k][1] = u.y;
         }
       }
-      // what undoes the queries' power of two, for rows row0 and row1
-      float qs0 = 1.0f, qs1 = 1.0f;
+      // scale * log2 e, and what undoes the queries' power of two, for rows row0 and row1
+      float cq0 = c2, cq1 = c2;
       if constexpr (BF16) {
         uint32_t top = 0;                     // the row's largest finite value, by its bits
 #pragma unroll
@@ -204,8 +217,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
 #pragma unroll
           for (int e = 0; e < 2; ++e)
             q[k][e] = pack2<false>(__uint_as_float(q[k][e] << 16) * f, __uint_as_float(q[k][e] & 0xffff0000u) * f);
-        qs0 = __shfl_sync(full, back, 4 * row0);
-        qs1 = __shfl_sync(full, back, 4 * row1);
+        cq0 *= __shfl_sync(full, back, 4 * row0);
+        cq1 *= __shfl_sync(full, back, 4 * row1);
+        if (my_part == 0 && c4 == 0) reinterpret_cast<float*>(smem + Rg::kBack)[my_head * 8 + r8] = back;
       }
       // ... in shared memory, the head's first warp putting them there: they are read again for every tile
       if (my_part == 0) {
@@ -215,16 +229,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
               make_uint4(q[2 * g][0], q[2 * g][1], q[2 * g + 1][0], q[2 * g + 1][1]);
       }
       __syncthreads();
-      const float cq0 = c2 * qs0, cq1 = c2 * qs1;
       const uint32_t q_at = smem_u32(smem) + Rg::kQ + my_head * (G * 512) + lane * 16;
       float o[kOut][4];
 #pragma unroll
       for (int j = 0; j < kOut; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
-      float m0 = ninf, m1 = ninf, l0 = 0.0f, l1 = 0.0f;
-      float up0 = ninf, up1 = ninf;           // what a row's maximum may be before its m is raised
-      float base0 = -kPBits, base1 = -kPBits; // m less the power of two that p is held times; 0 less it before any token
+      float m0 = kLowest, m1 = kLowest, l0 = 0.0f, l1 = 0.0f;
       // by group (a byte each), what O is relative to, 2^(E - 127), for the two rows; equal until tokens are added one by one
       uint32_t E0 = 0, E1 = 0;
       auto byte_of = [](uint32_t w, int g) { return int(w >> (8 * g) & 255u); };
@@ -257,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
           for (int e = 0; e < kCopies; ++e) {
             const int row = e * kRowsPerCopy + lane / CH;
             const char* p = head + uint64_t(__shfl_sync(full, place, row)) * stride;
-            const uint32_t to = dst + row * (CH * 16) + piece<D>(row, lane % CH) * 16;
+            const uint32_t to = dst + copy_at + e * 512;
             copy16(to, p, true);
             copy16(to + Rg::kPlane, p + a.kv_stride_kv, true);
           }
@@ -272,14 +283,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
       // the references of rows that have outgrown theirs go up to the maxima given (the same in all lanes of a row; each
       // row by its own tokens alone, so that what others see does not show in its digits)
       auto raise = [&](float top0, float top1) {
-        const float n0 = top0 > up0 ? top0 : m0, n1 = top1 > up1 ? top1 : m1;
+        const float n0 = top0 > m0 + kSlack ? top0 : m0, n1 = top1 > m1 + kSlack ? top1 : m1;
         const float e0 = m0 == n0 ? 1.0f : ex2(m0 - n0), e1 = m1 == n1 ? 1.0f : ex2(m1 - n1);
         m0 = n0;
         m1 = n1;
-        up0 = m0 + kSlack;
-        up1 = m1 + kSlack;
-        base0 = (m0 == ninf ? 0.0f : m0) - kPBits;
-        base1 = (m1 == ninf ? 0.0f : m1) - kPBits;
         l0 *= e0;
         l1 *= e1;
 #pragma unroll
@@ -313,14 +320,23 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
         // the step's tokens that are there (neither past the end nor in a block outside the cache), and those of them
         // that every row sees
         [[maybe_unused]] uint32_t there = full, common = full;
+        [[maybe_unused]] int lim0 = 0, lim1 = 0;             // the last tokens that the lane's rows see
+        [[maybe_unused]] float qs0 = 1.0f, qs1 = 1.0f;       // what undoes the queries' power of two
         if constexpr (EDGE) {
+          lim0 = all + row0 / a.G;
+          lim1 = all + row1 / a.G;
+          if constexpr (BF16) {
+            const float* back = reinterpret_cast<const float*>(smem + Rg::kBack) + my_head * 8;
+            qs0 = back[row0];
+            qs1 = back[row1];
+          }
           bool here = t + lane < end;
           if (__any_sync(full, gaps) && here) {
             const int lb = block_of(t + lane);
             here = lb < a.MB && uint32_t(table[lb]) < uint32_t(a.NB);
           }
           there = __ballot_sync(full, here);
-          common = there & __ballot_sync(full, t + lane <= S - A);
+          common = there & __ballot_sync(full, t + lane <= all);
         }
         // ---- the lane's token: its scales into the tables
         {
@@ -455,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
             }
         }
         // (the product rounded before the difference, not in one step with it: the largest logit's is then 0 whatever its size)
-        const float f0 = EDGE ? c2 : cq0, f1 = EDGE ? c2 : cq1;
+        const float f0 = EDGE ? a.scale * kLog2e : cq0, f1 = EDGE ? a.scale * kLog2e : cq1;
 #pragma unroll
         for (int n = 0; n < kTiles; ++n)
 #pragma unroll
@@ -466,7 +482,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
           top0 = fmaxf(top0, fmaxf(s[n][0], s[n][2]));
           top1 = fmaxf(top1, fmaxf(s[n][1], s[n][3]));
         }
-        if (__any_sync(full, top0 > up0 || top1 > up1)) {
+        if (__any_sync(full, top0 > m0 + kSlack || top1 > m1 + kSlack)) {
 #pragma unroll
           for (int x = 4; x < 32; x *= 2) {
             top0 = fmaxf(top0, __shfl_xor_sync(full, top0, x));
@@ -474,6 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
           }
           raise(top0, top1);
         }
+        const float base0 = m0 - kPBits, base1 = m1 - kPBits;
 #pragma unroll
         for (int n = 0; n < kTiles; ++n)
 #pragma unroll
@@ -604,10 +621,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
       constexpr int kAhead = Rg::kStages - 1;
 #pragma unroll 1
       for (int i = 0; i < kAhead; ++i) issue(i, i);
-      int slot = 0, fill = kAhead;
 #pragma unroll 1
       for (int i = 0; i < mine; ++i) {
-        issue(i + kAhead, fill);
+        const int slot = i % Rg::kStages;
+        issue(i + kAhead, (i + kAhead) % Rg::kStages);
         asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
         __syncwarp();
         const int t = start + i * round;
@@ -621,11 +638,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
         if constexpr (BF16) odd = ((wk & (wk << 1)) | (wv & (wv << 1))) & 0x80808080u;
         else odd = __vcmpgtu4(wk, 0x8c8c8c8cu) | __vcmpgtu4(wv, 0x8c8c8c8cu) |
                    ((__vcmpgtu4(0x68686868u, wk) | __vcmpgtu4(0x68686868u, wv)) & (D == 64 ? 0xffffu : 0xffffffffu));
-        if (t + kStep - 1 > S - A || t + kStep > end || __any_sync(full, odd || gaps)) step(i, slot, wk, wv, std::true_type());
+        if (t + kStep - 1 > all || t + kStep > end || __any_sync(full, odd || gaps)) step(i, slot, wk, wv, std::true_type());
         else step(i, slot, wk, wv, std::false_type());
         __syncwarp();                         // every lane has read the slot that the next copies fill, and the tables
-        slot = slot + 1 == Rg::kStages ? 0 : slot + 1;
-        fill = fill + 1 == Rg::kStages ? 0 : fill + 1;
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
       // ---- results: l of a row over the lanes that share it; O as the sums of p v (of 2^7 p v in fp16) that the join takes
@@ -699,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
           // NaN groups among the values of tokens that this row does see
           uint32_t nan = 0;
           if (fix) {
-            const int last = min(S - A + jq, end - 1);
+            const int last = min(all + jq, end - 1);
 #pragma unroll 1
             for (int t = begin; t <= last; ++t) {
               const int lb = block_of(t), ph = lb < a.MB ? table[lb] : -1;
@@ -744,9 +759,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
         ds.h = hg * HG;
         ds.heads = HG;
         ds.n_used = n_used();
-        ds.ntok = A;
-        ds.S = S;
-        ds.A = A;
+        ds.ntok = ds.A = a.q_off[r + 1] - a.q_off[r];
+        ds.S = a.seq_used[r];
         ds.a0 = a.q_off[r];
         ds.end = low() + first + nt;
         ds.total = sched.share.total;
