@@ -1246,7 +1246,7 @@ __global__ void __launch_bounds__(threads(BITS != 16), 1)
             }
             const uint32_t b = word >> (8 * g) & 255u;
             uint32_t y[4];
-            if (plain) widen4<BF16>(eight, plain_factor4<BF16>(b), y);
+            if (plain) widen4<BF16>(eight, plain_factor4(b), y);
             else widen4_any<BF16>(eight, b, y);
             if (hide) {
 #pragma unroll

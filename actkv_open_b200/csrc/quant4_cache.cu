@@ -85,7 +85,7 @@ __device__ __forceinline__ void write(T* dst, const Raw<G>& r, bool vec) {
       const uint32_t b0 = r.scales >> (16 * k) & 255u, b1 = r.scales >> (16 * k + 8) & 255u;
       uint32_t y[4];
       if (plain) {
-        widen4<BF16>(r.w[k], plain_factor4<BF16>(b0), plain_factor4<BF16>(b1), y);
+        widen4<BF16>(r.w[k], plain_factor4(b0), plain_factor4(b1), y);
       } else {
         uint32_t z[4];
         widen4_any<BF16>(r.w[k], b0, y);

@@ -95,32 +95,32 @@ __device__ __forceinline__ uint32_t mul16x2(uint32_t x, uint32_t f) {
   else asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(f));
   return r;
 }
-// The 4-bit cache.  Eight values as 16-bit ones, times the power of two of their scale byte: fp16 by one conversion per
-// pair; for bf16 its exponent and first mantissa bit moved under bf16's exponent, where it reads as the value times
-// 2^-112.  Where no scale byte of a word is out of the ordinary one multiplication does:
+// The 4-bit cache.  Eight values as 16-bit ones, times the power of two of their scale byte.  fp16 by one conversion
+// and one multiplication per pair; bf16 by way of that: the product is exact in fp16 where the scale byte is an ordinary
+// one, and goes through 32 bits (half of these five operations off the pipe that converts, which is the busiest here:
+// moving fp16's exponent under bf16's by masks and shifts takes four of five on it).
+// Whether the scale bytes of a word are ordinary:
 template <bool BF16>
 __device__ __forceinline__ bool plain_scales4(uint32_t w) {
-  return __vcmpgtu4(w, BF16 ? 0x8e8e8e8eu : 0x8c8c8c8cu) == 0 && (BF16 || __vcmpgtu4(0x71717171u, w) == 0);   // <= 142 (fp16: 113 .. 140)
+  return __vcmpgtu4(w, 0x8c8c8c8cu) == 0 && __vcmpgtu4(0x71717171u, w) == 0;    // 113 .. 140
 }
-template <bool BF16>
-__device__ __forceinline__ uint32_t plain_factor4(uint32_t b) {
-  return BF16 ? b * 0x00800080u + 0x38003800u : (b - 112u) * 0x04000400u;
-}
+__device__ __forceinline__ uint32_t plain_factor4(uint32_t b) { return (b - 112u) * 0x04000400u; }
 template <bool BF16>
 __device__ __forceinline__ void widen4(uint32_t w, uint32_t f_lo, uint32_t f_hi, uint32_t (&r)[4]) {   // a factor per four values
   e2m1x8_f16(w, r[0], r[1], r[2], r[3]);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
+    r[i] = mul16x2<false>(r[i], i < 2 ? f_lo : f_hi);
     if constexpr (BF16) {
-      const uint32_t m = r[i] & 0x7fff7fffu;
-      r[i] = (r[i] ^ m) | (m >> 3);
+      const float2 x = f16x2_f32(r[i]);
+      asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r[i]) : "f"(x.y), "f"(x.x));
     }
-    r[i] = mul16x2<BF16>(r[i], i < 2 ? f_lo : f_hi);
   }
 }
 template <bool BF16>
 __device__ __forceinline__ void widen4(uint32_t w, uint32_t f, uint32_t (&r)[4]) { widen4<BF16>(w, f, f, r); }
-// ... for any scale byte: two multiplications, of which only the last rounds; fp16 past its range: its largest.
+// ... for any scale byte: two multiplications, of which only the last rounds; fp16 past its range: its largest.  (bf16: the
+// exponent and first mantissa bit moved under bf16's exponent read as the value times 2^-112.)
 template <bool BF16>
 __device__ __forceinline__ void widen4_any(uint32_t w, uint32_t b, uint32_t (&r)[4]) {
   uint32_t f0, f1;
@@ -137,10 +137,14 @@ __device__ __forceinline__ void widen4_any(uint32_t w, uint32_t b, uint32_t (&r)
     f1 = (min(b - e, 15u) + 15u) * 0x04000400u;
   }
   if (b >= kNan4) f1 = 0x7fff7fffu;            // NaN
-  widen4<BF16>(w, f0, r);
+  e2m1x8_f16(w, r[0], r[1], r[2], r[3]);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    r[i] = mul16x2<BF16>(r[i], f1);
+    if constexpr (BF16) {
+      const uint32_t m = r[i] & 0x7fff7fffu;
+      r[i] = (r[i] ^ m) | (m >> 3);
+    }
+    r[i] = mul16x2<BF16>(mul16x2<BF16>(r[i], f0), f1);
     if constexpr (!BF16) {
       asm("min.NaN.f16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(0x7bff7bffu));
       asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(0xfbfffbffu));
