@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -91,11 +92,22 @@ SIGNATURES = {
                                  I32, I32, I32, P, I32, P, I32, I64, I64, I64, I64, I64, P, I64, P, I32, I32, I32, I32,
                                  I32, I32, I32, I32, P, P]),
 }
+# calls of many arguments as an array of 64-bit words: what ``words`` packs
+SIGNATURES["actkv_rotate_write_words"] = (I32, [ctypes.c_char_p])
+for _name in ("actkv_quantize_write", "actkv_dequantize_read", "actkv_chunk_attention_quant"):
+    SIGNATURES[_name + "_words"] = (I32, [I32, ctypes.c_char_p])
 # the 4-bit cache's entries take what the 8-bit cache's do
 for _eight, _four in (("actkv_chunk_attention_quant", "actkv_chunk_attention_quant4"),
                       ("actkv_quantize_write", "actkv_quantize_write4"),
                       ("actkv_dequantize_read", "actkv_dequantize_read4"), ("actkv_quant_append", "actkv_quant4_append")):
     SIGNATURES[_four] = SIGNATURES[_eight]
+
+
+
+def words(entry: str):
+    """The packer of a call's arguments for its ``_words`` form (None is not an argument: pass 0)."""
+    return struct.Struct("=" + "".join("f4x" if a is F else "q" for a in SIGNATURES[entry][1])).pack
+
 
 _lib = None
 _lock = threading.Lock()

@@ -3,6 +3,10 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <string.h>
+#include <type_traits>
+#include <utility>
+
 #include "kernels.cuh"
 #include "quant_row.cuh"
 
@@ -183,6 +187,29 @@ int quant_append(int bits, const void* k_new, const void* v_new, int dtype, int6
   return done(write_rows(a, dtype, L, bits, st), "quant_append");
 }
 
+// An entry called with its arguments as 64-bit words.
+template <typename A>
+A from_word(const int64_t& w) {
+  if constexpr (std::is_pointer<A>::value) {
+    return reinterpret_cast<A>(static_cast<intptr_t>(w));
+  } else if constexpr (std::is_same<A, float>::value) {
+    float f;
+    memcpy(&f, &w, sizeof(f));
+    return f;
+  } else {
+    return static_cast<A>(w);
+  }
+}
+template <typename... A, size_t... I>
+int call_words(int (*entry)(A...), const int64_t* w, std::index_sequence<I...>) {
+  return entry(from_word<A>(w[I])...);
+}
+template <typename... A>
+int call_words(int (*entry)(A...), const int64_t* w) {
+  if (!w) return fail(ACTKV_ERR_INVALID, "the words are required");
+  return call_words(entry, w, std::index_sequence_for<A...>());
+}
+
 }  // namespace
 
 extern "C" {
@@ -340,6 +367,17 @@ int actkv_rotate_write(const void* q, int64_t q_stride_l, int64_t q_stride_t, in
   a.vec_out = (uint64_t(reinterpret_cast<uintptr_t>(cache)) | (uint64_t(cache_stride_l) | uint64_t(cache_stride_kv) |
                uint64_t(cache_stride_b) | uint64_t(cache_stride_s) | uint64_t(cache_stride_h)) * cs) % 16 == 0;
   return done(launch_rotate_write(a, dtype, static_cast<cudaStream_t>(stream)), "rotate_write");
+}
+
+int actkv_rotate_write_words(const int64_t* words) { return call_words(actkv_rotate_write, words); }
+int actkv_quantize_write_words(int bits, const int64_t* words) {
+  return call_words(bits == 4 ? actkv_quantize_write4 : actkv_quantize_write, words);
+}
+int actkv_dequantize_read_words(int bits, const int64_t* words) {
+  return call_words(bits == 4 ? actkv_dequantize_read4 : actkv_dequantize_read, words);
+}
+int actkv_chunk_attention_quant_words(int bits, const int64_t* words) {
+  return call_words(bits == 4 ? actkv_chunk_attention_quant4 : actkv_chunk_attention_quant, words);
 }
 
 }  // extern "C"

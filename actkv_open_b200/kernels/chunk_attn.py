@@ -39,8 +39,8 @@ def _check(q, q_off, cache, block_table, seq_used, out, lse, workspace):
     assert q.dim() == 3 and q.stride(2) == 1, "q is [T, Hq, D] with contiguous rows"
     assert q_off.dtype is _I32 and seq_used.dtype is _I32 and block_table.dtype is _I32
     assert block_table.stride(1) == 1 and q_off.is_contiguous() and seq_used.is_contiguous()
-    r_n = len(seq_used)
-    assert len(q_off) == r_n + 1 and len(block_table) == r_n, "q_off [R + 1], block_table [R, MB], seq_used [R]"
+    r_n = block_table.shape[0]
+    assert q_off.shape == (r_n + 1,) and seq_used.shape == (r_n,), "q_off [R + 1], block_table [R, MB], seq_used [R]"
     if out is None:
         out = q.new_empty(q.shape)
     else:

@@ -41,6 +41,7 @@ def quant_row_bytes(n_kv_heads: int, head_dim: int, bits: int = 8) -> int:
 
 
 _I32, _U8 = torch.int32, torch.uint8
+_pack_write, _pack_read, _pack_attend = (N.words("actkv_" + x) for x in ("quantize_write", "dequantize_read", "chunk_attention_quant"))
 
 
 def _tables(dev, L, t_n, hkv, d, rows, tok_off, block_table, seq_used, bits):
@@ -53,10 +54,10 @@ def _tables(dev, L, t_n, hkv, d, rows, tok_off, block_table, seq_used, bits):
     assert s_1 == 1 and block_table.stride(1) == 1
     assert tok_off.dtype is _I32 and seq_used.dtype is _I32 and block_table.dtype is _I32
     assert tok_off.is_contiguous() and seq_used.is_contiguous()
-    r_n = len(seq_used)
-    assert len(tok_off) == r_n + 1 and len(block_table) == r_n, "tok_off [R + 1], block_table [R, MB], seq_used [R]"
+    r_n, mb = block_table.shape
+    assert tok_off.shape == (r_n + 1,) and seq_used.shape == (r_n,), "tok_off [R + 1], block_table [R, MB], seq_used [R]"
     return (tok_off.data_ptr(), t_n, rows.data_ptr(), s_l, s_kv, s_b, s_s, block_table.data_ptr(),
-            block_table.stride(0), seq_used.data_ptr(), r_n, L, block_table.size(1), nb, bs, hkv, d,
+            block_table.stride(0), seq_used.data_ptr(), r_n, L, mb, nb, bs, hkv, d,
             N.status_word(dev).data_ptr(), N.stream_ptr(dev))
 
 
@@ -78,10 +79,10 @@ def quantize_write(k_new, v_new, tok_off, rows, block_table, seq_used, bits: int
     k_l, k_t, k_h, k_1 = k_new.stride()
     v_l, v_t, v_h, v_1 = v_new.stride()
     assert k_1 == 1 and v_1 == 1
-    lib = N.load()
-    code = (lib.actkv_quantize_write4 if _bits(bits) else lib.actkv_quantize_write)(
+    _bits(bits)
+    code = N.load().actkv_quantize_write_words(bits, _pack_write(
         k_new.data_ptr(), v_new.data_ptr(), N.dtype_code(k_new), k_l, k_t, k_h, v_l, v_t, v_h,
-        *_tables(dev, *shape, rows, tok_off, block_table, seq_used, bits))
+        *_tables(dev, *shape, rows, tok_off, block_table, seq_used, bits)))
     if code:
         N.check(code, "quantize_write")
     return rows
@@ -119,10 +120,10 @@ def dequantize_read(rows, n_kv_heads, head_dim, tok_off, block_table, seq_used, 
         *three, one = x.stride()
         assert x.shape == shape and x.dtype is some.dtype and one == 1
         strides += three
-    lib = N.load()
-    code = (lib.actkv_dequantize_read4 if _bits(bits) else lib.actkv_dequantize_read)(
-        N.ptr(k_out), N.ptr(v_out), N.dtype_code(some), *strides,
-        *_tables(dev, *shape, rows, tok_off, block_table, seq_used, bits))
+    _bits(bits)
+    code = N.load().actkv_dequantize_read_words(bits, _pack_read(
+        N.ptr(k_out) or 0, N.ptr(v_out) or 0, N.dtype_code(some), *strides,
+        *_tables(dev, *shape, rows, tok_off, block_table, seq_used, bits)))
     if code:
         N.check(code, "dequantize_read")
     return k_out, v_out
@@ -132,7 +133,7 @@ def paged_chunk_attention_quant(q, q_off, rows, n_kv_heads, block_table, seq_use
                                 workspace=None, path: str = "auto", bits: int = 8):
     """``paged_chunk_attention`` over one layer of the 8- or 4-bit cache, rows [2, NB, BS, row_bytes]:
     the keys and values are what ``dequantize_read`` gives in q's dtype."""
-    four = _bits(bits)
+    _bits(bits)
     dev, r_n, out, lse, workspace = _check(q, q_off, rows, block_table, seq_used, out, lse, workspace)
     t_n, hq, d = q.shape
     _2, nb, bs, row = rows.shape
@@ -143,13 +144,12 @@ def paged_chunk_attention_quant(q, q_off, rows, n_kv_heads, block_table, seq_use
     assert s_1 == 1
     q_t, q_h, _1 = q.stride()
     o_t, o_h, _1 = out.stride()
-    lib = N.load()
-    code = (lib.actkv_chunk_attention_quant4 if four else lib.actkv_chunk_attention_quant)(
+    code = N.load().actkv_chunk_attention_quant_words(bits, _pack_attend(
         q.data_ptr(), N.dtype_code(q), q_t, q_h, q_off.data_ptr(), t_n, rows.data_ptr(), s_kv, s_b, s_s,
         block_table.data_ptr(), block_table.stride(0), seq_used.data_ptr(), out.data_ptr(), o_t, o_h, lse.data_ptr(),
         lse.stride(0), r_n, block_table.size(1), nb, bs, hq, n_kv_heads, d,
         d ** -0.5 if scale is None else float(scale), _PATHS[path], workspace.data_ptr(), workspace.nbytes,
-        N.status_word(dev).data_ptr(), N.stream_ptr(dev))
+        N.status_word(dev).data_ptr(), N.stream_ptr(dev)))
     if code:
         N.check(code, "paged_chunk_attention_quant")
     return out, lse

@@ -14,6 +14,7 @@ from .. import _native as N
 from .quant_cache import QUANT_GROUP
 
 _I32, _F32, _U8 = torch.int32, torch.float32, torch.uint8
+_pack = N.words("actkv_rotate_write")
 
 
 def rotary_table(rot: int, max_positions: int, base: float = 10000.0, frequencies=None, device="cuda") -> torch.Tensor:
@@ -43,58 +44,67 @@ def rotate_write(q, k_new, v_new, positions, angles, tok_off, cache, block_table
     A token whose position the angles do not have is left alone, one that the tables do not hold is not
     written into the cache (device status BAD_INDEX, both); so is a token of no session, unflagged.
     """
+    # (each look at a tensor costs a fraction of a microsecond, and a call of one token's rows little more than they do)
     dev = k_new.device
-    N.require_cuda(k_new, v_new, q, positions, angles, tok_off, cache, block_table, seq_used, q_out)
-    shape = k_new.shape
-    assert len(shape) == 4 and shape == v_new.shape and k_new.dtype is v_new.dtype, \
-        "k_new / v_new are [L, T, Hkv, D] of one dtype"
+    if not k_new.is_cuda or v_new.device != dev or positions.device != dev or angles.device != dev or \
+            tok_off.device != dev or cache.device != dev or block_table.device != dev or seq_used.device != dev or \
+            q is not None and q.device != dev or q_out is not None and q_out.device != dev:
+        N.require_cuda(k_new, v_new, q, positions, angles, tok_off, cache, block_table, seq_used, q_out)
+    shape, dtype = k_new.shape, k_new.dtype
+    assert len(shape) == 4 and shape == v_new.shape and dtype is v_new.dtype, "k_new / v_new are [L, T, Hkv, D] of one dtype"
     L, t_n, hkv, d = shape
     k_l, k_t, k_h, k_1 = k_new.stride()
     v_l, v_t, v_h, v_1 = v_new.stride()
     assert k_1 == 1 and v_1 == 1
-    hq = 0
-    qs = os = (0, 0, 0)
-    if q is not None:
-        assert q.dim() == 4 and q.shape[0] == L and q.shape[1] == t_n and q.shape[3] == d and \
-            q.dtype is k_new.dtype, "q is [L, T, Hq, D] of k_new's dtype"
-        hq = q.shape[2]
-        if q_out is None:
-            q_out = q.new_empty(q.shape)
-        assert q_out.shape == q.shape and q_out.dtype is q.dtype
-        *qs, q_1 = q.stride()
-        *os, o_1 = q_out.stride()
-        assert q_1 == 1 and o_1 == 1
-    else:
+    if q is None:
         assert q_out is None, "q_out without q"
+        hq = q_p = o_p = 0
+        q_l = q_t = q_h = o_l = o_t = o_h = 0
+    else:
+        q_shape = q.shape
+        assert len(q_shape) == 4 and q.dtype is dtype, "q is [L, T, Hq, D] of k_new's dtype"
+        q_n, q_tn, hq, q_d = q_shape
+        assert q_n == L and q_tn == t_n and q_d == d, "q is [L, T, Hq, D] of k_new's dtype"
+        q_l, q_t, q_h, q_1 = q.stride()
+        if q_out is None:
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        else:
+            assert q_out.shape == q_shape and q_out.dtype is dtype
+        o_l, o_t, o_h, o_1 = q_out.stride()
+        assert q_1 == 1 and o_1 == 1
+        q_p, o_p = q.data_ptr(), q_out.data_ptr()
     assert positions.dtype is _I32 and positions.shape == (t_n,) and positions.is_contiguous(), "positions int32 [T]"
-    assert angles.dim() == 2 and angles.dtype is _F32 and angles.stride(1) == 1, "angles fp32 [P, rot]"
+    a_s, a_1 = angles.stride()
+    assert angles.dtype is _F32 and a_1 == 1, "angles fp32 [P, rot]"
     places, rot = angles.shape
     assert 0 < rot <= d and rot % 2 == 0, "rot is even and at most D"
     if bits is None:
-        assert cache.dim() == 6 and cache.dtype is k_new.dtype and cache.shape[0] == L and cache.shape[1] == 2 and \
-            cache.shape[4] == hkv and cache.shape[5] == d and cache.stride(5) == 1, \
+        c_shape = cache.shape
+        assert len(c_shape) == 6 and cache.dtype is dtype, "the cache is [L, 2, NB, BS, Hkv, D] of k_new's dtype"
+        c_n, c_2, nb, bs, c_hn, c_d = c_shape
+        c_l, c_kv, c_b, c_s, c_h, c_1 = cache.stride()
+        assert c_n == L and c_2 == 2 and c_hn == hkv and c_d == d and c_1 == 1, \
             "the cache is [L, 2, NB, BS, Hkv, D] of k_new's dtype"
-        c_l, c_kv, c_b, c_s, c_h = cache.stride()[:5]
     else:
         if bits not in (8, 4):
             raise ValueError(f"bits {bits}: the cache holds its rows in 8 or 4")
-        assert cache.dim() == 5 and cache.dtype is _U8 and cache.shape[0] == L and cache.shape[1] == 2 and \
-            cache.stride(4) == 1, "rows is [L, 2, NB, BS, row_bytes] uint8"
-        assert d % QUANT_GROUP == 0 and cache.shape[4] >= hkv * (d * bits // 8 + d // QUANT_GROUP), \
-            "rows are too short for these heads"
-        c_l, c_kv, c_b, c_s = cache.stride()[:4]
+        c_shape = cache.shape
+        assert len(c_shape) == 5 and cache.dtype is _U8, "rows is [L, 2, NB, BS, row_bytes] uint8"
+        c_n, c_2, nb, bs, row = c_shape
+        c_l, c_kv, c_b, c_s, c_1 = cache.stride()
         c_h = 0
-    nb, bs = cache.shape[2], cache.shape[3]
+        assert c_n == L and c_2 == 2 and c_1 == 1, "rows is [L, 2, NB, BS, row_bytes] uint8"
+        assert d % QUANT_GROUP == 0 and row >= hkv * (d * bits // 8 + d // QUANT_GROUP), "rows are too short for these heads"
     assert tok_off.dtype is _I32 and seq_used.dtype is _I32 and block_table.dtype is _I32
-    assert tok_off.is_contiguous() and seq_used.is_contiguous() and block_table.stride(1) == 1
-    r_n = len(seq_used)
-    assert len(tok_off) == r_n + 1 and len(block_table) == r_n, "tok_off [R + 1], block_table [R, MB], seq_used [R]"
-    code = N.load().actkv_rotate_write(
-        N.ptr(q), *qs, N.ptr(q_out), *os, k_new.data_ptr(), k_l, k_t, k_h, v_new.data_ptr(), v_l, v_t, v_h,
-        N.dtype_code(k_new), positions.data_ptr(), angles.data_ptr(), angles.stride(0), places, rot, interleaved,
-        tok_off.data_ptr(), t_n, cache.data_ptr(), bits or 0, c_l, c_kv, c_b, c_s, c_h, block_table.data_ptr(),
-        block_table.stride(0), seq_used.data_ptr(), r_n, L, block_table.size(1), nb, bs, hq, hkv, d,
-        N.status_word(dev).data_ptr(), N.stream_ptr(dev))
+    b_r, b_1 = block_table.stride()
+    assert b_1 == 1 and tok_off.is_contiguous() and seq_used.is_contiguous()
+    r_n, mb = block_table.shape
+    assert tok_off.shape == (r_n + 1,) and seq_used.shape == (r_n,), "tok_off [R + 1], block_table [R, MB], seq_used [R]"
+    code = N.load().actkv_rotate_write_words(_pack(
+        q_p, q_l, q_t, q_h, o_p, o_l, o_t, o_h, k_new.data_ptr(), k_l, k_t, k_h, v_new.data_ptr(), v_l, v_t, v_h,
+        N.dtype_code(k_new), positions.data_ptr(), angles.data_ptr(), a_s, places, rot, interleaved, tok_off.data_ptr(),
+        t_n, cache.data_ptr(), bits or 0, c_l, c_kv, c_b, c_s, c_h, block_table.data_ptr(), b_r, seq_used.data_ptr(),
+        r_n, L, mb, nb, bs, hq, hkv, d, N.status_word(dev).data_ptr(), N.stream_ptr(dev)))
     if code:
         N.check(code, "rotate_write")
     return q_out

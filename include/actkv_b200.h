@@ -603,6 +603,16 @@ ACTKV_API int actkv_rotate_write(const void* q, int64_t q_stride_l, int64_t q_st
                                  int32_t* status, void* stream);
 
 /*
+ * The same calls with their arguments as an array of 64-bit words, one per argument in order: pointers and integers as they
+ * are, a float's bits in the low half.  For bindings in which every argument of a call costs time (45 of them 4 us through
+ * ctypes, their array 1).  bits 4: the 4-bit cache's entries, else the 8-bit one's.
+ */
+ACTKV_API int actkv_rotate_write_words(const int64_t* words);
+ACTKV_API int actkv_quantize_write_words(int bits, const int64_t* words);
+ACTKV_API int actkv_dequantize_read_words(int bits, const int64_t* words);
+ACTKV_API int actkv_chunk_attention_quant_words(int bits, const int64_t* words);
+
+/*
  * Self-test of the kernels' failure path (no counterpart in the reference): one block waits, with
  * the bounded mbarrier wait that every pipelined kernel here uses, on a barrier that nothing
  * completes.  The wait gives up after ~2^31 cycles (about a second), sets ACTKV_DEV_TIMEOUT in
