@@ -10,7 +10,8 @@ behind actkv-open's own module layout:
     actkv_open_b200.budget              ~ actkv.budget (Algorithm 2 on the device)
     actkv_open_b200.engine              batched, device-resident eviction of many sessions
     actkv_open_b200.kernels.chunk_attn  attention of new tokens over the paged cache
-    actkv_open_b200.kernels.quant_cache the 8-bit cache: write, read back, attention over it
+    actkv_open_b200.kernels.quant_cache the 8- and 4-bit caches: write, read back, attention over them
+    actkv_open_b200.kernels.rotary      new tokens' position rotation on the way into a cache
 
 The kernels are reached through the C ABI in include/actkv_b200.h (libactkv_b200.so).
 """

@@ -35,6 +35,7 @@ from .kernels.chunk_attn import chunk_workspace, paged_chunk_attention
 from .kernels.lse_attn import (action_region_lse, action_scores_region, region_lse_workspace_bytes,
                                 score_region_workspace_bytes, stream_signal)
 from .kernels.quant_cache import (dequantize_read, paged_chunk_attention_quant, quant_row_bytes)
+from .kernels.rotary import rotate_write
 
 
 class DevicePagedCache:
@@ -155,6 +156,57 @@ class DevicePagedCache:
             if bits:
                 raise RuntimeError(f"append: device status {bits:#x}")
 
+    def reserve(self, n_new, check: bool = True) -> torch.Tensor:
+        """Room for n_new[r] more tokens of session r, every layer: tables, lengths and the free stack as
+        ``append`` leaves them, without any rows; returns the offsets (device int32 [R+1]) that
+        ``write_rotated`` takes for the rows, layer by layer as a model makes them.  ``n_new`` as for
+        ``append``; with ``check`` false the caller reads the device status before writing any (a session that
+        did not fit has no room, and its rows would go where its last tokens are)."""
+        if isinstance(n_new, torch.Tensor):
+            off, R = n_new, n_new.numel() - 1
+        else:
+            offs = [0]
+            for x in n_new:
+                offs.append(offs[-1] + int(x))
+            R = len(offs) - 1
+            if R <= self.max_sessions:
+                off = self._upload(offs).clone()      # (the staging buffer is used again)
+        if R > self.max_sessions:
+            raise ValueError(f"{R} sessions, room for {self.max_sessions}")
+        dev, ws = self.device, self._blocks_workspace()
+        plane, slot, row, n_slots = self.flat_planes()
+        N.check(N.load().actkv_append(
+            self.kv.data_ptr(), self.n_layers, plane, slot, row, n_slots, None, None, 0, 0, off.data_ptr(), 0,
+            self.seq_used.data_ptr(), self.block_table.data_ptr(), self.block_table.stride(0), self.max_blocks,
+            self.block_size, self.free_list.data_ptr(), self.free_top.data_ptr(), self.num_blocks, R, ws.data_ptr(),
+            ws.numel(), N.status_word(dev).data_ptr(), N.stream_ptr(dev)), "reserve")
+        self.n_sessions = max(self.n_sessions, R)
+        if check:
+            bits = N.read_device_status(dev)
+            if bits & N.DEV_OUT_OF_BLOCKS:
+                raise OutOfBlocks("reserve: the free stack (or a table row) ran out of blocks")
+            if bits:
+                raise RuntimeError(f"reserve: device status {bits:#x}")
+        return off
+
+    def write_rotated(self, layer: int, q: torch.Tensor | None, k_new: torch.Tensor, v_new: torch.Tensor,
+                      positions: torch.Tensor, angles: torch.Tensor, off: torch.Tensor, interleaved: bool = False,
+                      q_out: torch.Tensor | None = None):
+        """One layer's new rows into the room that ``reserve`` made, the keys rotated on the way, and the
+        queries rotated (returned): q [T, Hq, D] (or None), k_new / v_new [T, Hkv, D] packed by off [R+1],
+        positions int32 [T], angles as ``kernels.rotary.rotary_table`` gives them.  A session's next position is
+        not its length once it has been evicted: the caller counts them."""
+        R = off.shape[0] - 1
+        cache, bits = self._layer_rows(layer)
+        out = rotate_write(None if q is None else q[None], k_new[None], v_new[None], positions, angles, off, cache,
+                           self.block_table[:R], self.seq_used[:R], q_out=None if q_out is None else q_out[None],
+                           interleaved=interleaved, bits=bits)
+        return None if out is None else out[0]
+
+    def _layer_rows(self, layer: int):
+        """(one layer as ``rotate_write`` takes it, its bits)."""
+        return self.kv[layer:layer + 1], None
+
     def _blocks_workspace(self) -> torch.Tensor:
         if self._blocks_ws is None:
             self._blocks_ws = N.workspace(N.load().actkv_blocks_workspace_bytes(self.max_sessions), self.device)
@@ -210,17 +262,18 @@ class DevicePagedCache:
 
 
 class QuantPagedCache(DevicePagedCache):
-    """A ``DevicePagedCache`` whose rows are held in 8 bits (``kernels.quant_cache``): half the memory
-    per token, and half the bytes per attention call.  append quantises; release, eviction and
-    compaction move rows as bytes; ``EvictionPipeline`` scores it from keys read back into 16 bits,
-    a few layers at a time.  ``dtype`` (bf16 or fp16) is the type of its queries and outputs.
-    ``rows`` is the cache as the functions of ``kernels.quant_cache`` take it."""
+    """A ``DevicePagedCache`` whose rows are held in 8 bits, or in 4 with ``bits`` 4 (``kernels.quant_cache``): half
+    or a quarter of the memory per token, and as much less to read per attention call.  append and
+    write_rotated quantise; release, eviction and compaction move rows as bytes; ``EvictionPipeline`` scores
+    it from keys read back into 16 bits, a few layers at a time.  ``dtype`` (bf16 or fp16) is the type of its
+    queries and outputs.  ``rows`` is the cache as the functions of ``kernels.quant_cache`` take it."""
 
     def __init__(self, num_blocks: int, block_size: int, n_kv_heads: int, head_dim: int, n_layers: int,
-                 max_sessions: int, max_tokens: int, dtype=torch.bfloat16, device="cuda"):
+                 max_sessions: int, max_tokens: int, dtype=torch.bfloat16, device="cuda", bits: int = 8):
         if dtype not in (torch.bfloat16, torch.float16):
-            raise ValueError(f"dtype {dtype}: the 8-bit cache works in bf16 or fp16")
-        row = quant_row_bytes(n_kv_heads, head_dim)
+            raise ValueError(f"dtype {dtype}: the {bits}-bit cache works in bf16 or fp16")
+        row = quant_row_bytes(n_kv_heads, head_dim, bits)
+        self.bits = bits
         super().__init__(num_blocks, block_size, 1, row, n_layers, max_sessions, max_tokens, dtype=torch.uint8,
                          device=device)
         self.n_kv_heads, self.head_dim, self.row_bytes, self.dtype = n_kv_heads, head_dim, row, dtype
@@ -248,7 +301,8 @@ class QuantPagedCache(DevicePagedCache):
         if R > self.max_sessions:
             raise ValueError(f"{R} sessions, room for {self.max_sessions}")
         dev, ws, rows = self.device, self._blocks_workspace(), self.rows
-        N.check(N.load().actkv_quant_append(
+        lib = N.load()
+        N.check((lib.actkv_quant4_append if self.bits == 4 else lib.actkv_quant_append)(
             k_new.data_ptr(), v_new.data_ptr(), N.dtype_code(k_new), *k_new.stride()[:3], *v_new.stride()[:3],
             off.data_ptr(), k_new.shape[1], rows.data_ptr(), *rows.stride()[:4], self.block_table.data_ptr(),
             self.block_table.stride(0), self.seq_used.data_ptr(), self.free_list.data_ptr(), self.free_top.data_ptr(),
@@ -264,12 +318,16 @@ class QuantPagedCache(DevicePagedCache):
 
     def chunk_attention(self, layer: int, q: torch.Tensor, q_off: torch.Tensor, scale: float | None = None,
                         out: torch.Tensor | None = None, lse: torch.Tensor | None = None):
-        """As ``DevicePagedCache.chunk_attention``, over the 8-bit rows."""
+        """As ``DevicePagedCache.chunk_attention``, over the rows as they are held."""
         R = q_off.shape[0] - 1
         if self._chunk_ws is None:
             self._chunk_ws = chunk_workspace(self.device)
         return paged_chunk_attention_quant(q, q_off, self.rows[layer], self.n_kv_heads, self.block_table[:R],
-                                           self.seq_used[:R], scale=scale, out=out, lse=lse, workspace=self._chunk_ws)
+                                           self.seq_used[:R], scale=scale, out=out, lse=lse, workspace=self._chunk_ws,
+                                           bits=self.bits)
+
+    def _layer_rows(self, layer: int):
+        return self.rows[layer:layer + 1], self.bits
 
     # The keys read back for scoring: every block of the pool in its place, so that the tables serve
     # unchanged (one "session" with the identity table), in layer groups of about a gigabyte.  ``keys16`` gives views of
@@ -289,7 +347,7 @@ class QuantPagedCache(DevicePagedCache):
         assert n <= self._keys.shape[0]
         keys = self._keys[:n]
         dequantize_read(self.rows[l0:l1], self.n_kv_heads, self.head_dim, self._all_slots, self._all_blocks,
-                        self._all_slots[1:], slots, k_out=keys, planes="k")
+                        self._all_slots[1:], slots, k_out=keys, planes="k", bits=self.bits)
         keys = keys.view(n, 1, self.num_blocks, self.block_size, self.n_kv_heads, self.head_dim)
         return keys.expand(-1, 2, -1, -1, -1, -1)          # scoring reads the key plane only
 
@@ -366,7 +424,7 @@ class EvictionPipeline:
         self.host_inputs_read = None              # event: step_host's last copy out of host memory done
         self._ready = None                        # step_host's streamed mode: copied-groups counter
         self._ready_base = 0
-        # None: not tried yet; False: the grouped launches (an 8-bit cache is scored in layer groups)
+        # None: not tried yet; False: the grouped launches (a cache in 8 or 4 bits is scored in layer groups)
         self._streamed = False if isinstance(cache, QuantPagedCache) else None
         self._lse_own = None                      # lse computed here when a step gets none
         self._lse_ws = None

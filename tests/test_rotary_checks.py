@@ -64,3 +64,11 @@ def test_python_refusals():
             rotary_table(rot, positions, device="cpu")
     with pytest.raises(AssertionError, match="frequencies"):
         rotary_table(8, 4, frequencies=[1.0, 0.5], device="cpu")
+
+
+def test_caches_hold_8_or_4_bits():
+    from actkv_open_b200.engine import QuantPagedCache
+    with pytest.raises(ValueError, match="bits 2"):
+        QuantPagedCache(4, 16, 2, 128, 1, 1, 64, device="cpu", bits=2)
+    with pytest.raises(ValueError, match="dtype"):
+        QuantPagedCache(4, 16, 2, 128, 1, 1, 64, device="cpu", dtype=torch.float32, bits=4)
