@@ -44,34 +44,34 @@ __device__ __forceinline__ void store4(T* p, const Four<T>& y, bool vec) {
   }
 }
 
-// G: groups of a head, 2 or 4 (0: any number, one at a time).  What a lane reads of a row:
+// G: groups of a head, 2 to 4 (0: any number, one at a time).  What a lane reads of a row:
 template <int G>
 struct Raw {
-  uint32_t w[G / 2], scales;
+  uint32_t w[(G + 1) / 2], scales;       // (places of groups that there are not: an ordinary scale)
 };
 template <int G>
 __device__ __forceinline__ Raw<G> load_raw(const uint8_t* at, const uint8_t* scale, bool vec) {
   Raw<G> r;
-  if (vec) {
-    if constexpr (G == 4) {
-      const uint2 x = __ldcs(reinterpret_cast<const uint2*>(at));
-      r.w[0] = x.x;
-      r.w[G / 2 - 1] = x.y;
-      r.scales = *reinterpret_cast<const uint32_t*>(scale);
-    } else {
-      r.w[0] = __ldcs(reinterpret_cast<const uint32_t*>(at));
-      r.scales = *reinterpret_cast<const uint16_t*>(scale) | 0x7f7f0000u;
-    }
+  if (vec && G == 4) {
+    const uint2 x = __ldcs(reinterpret_cast<const uint2*>(at));
+    r.w[0] = x.x;
+    r.w[(G + 1) / 2 - 1] = x.y;
+    r.scales = *reinterpret_cast<const uint32_t*>(scale);
+  } else if (vec && G == 2) {
+    r.w[0] = __ldcs(reinterpret_cast<const uint32_t*>(at));
+    r.scales = *reinterpret_cast<const uint16_t*>(scale) | 0x7f7f0000u;
   } else {
-    r.scales = G == 4 ? 0u : 0x7f7f0000u;
+    r.scales = G == 4 ? 0u : (G == 3 ? 0x7f000000u : 0x7f7f0000u);
 #pragma unroll
-    for (int k = 0; k < G / 2; ++k) r.w[k] = 0;
+    for (int k = 0; k < (G + 1) / 2; ++k) r.w[k] = 0;
 #pragma unroll
-    for (int k = 0; k < 2 * G; ++k) r.w[k / 4] |= uint32_t(at[k]) << (8 * (k % 4));
+    for (int g = 0; g < G; ++g) {
+      const uint32_t two = vec ? uint32_t(reinterpret_cast<const uint16_t*>(at)[g]) : uint32_t(at[2 * g]) | uint32_t(at[2 * g + 1]) << 8;
+      r.w[g / 2] |= two << (16 * (g & 1));
+      r.scales |= uint32_t(scale[g]) << (8 * g);
+    }
 #pragma unroll
-    for (int g = 0; g < G; ++g) r.scales |= uint32_t(scale[g]) << (8 * g);
-#pragma unroll
-    for (int k = 0; k < G / 2; ++k) asm("" : "+r"(r.w[k]));  // (see e2m1x8_f16)
+    for (int k = 0; k < (G + 1) / 2; ++k) asm("" : "+r"(r.w[k]));      // (see e2m1x8_f16)
   }
   return r;
 }
@@ -81,7 +81,7 @@ __device__ __forceinline__ void write(T* dst, const Raw<G>& r, bool vec) {
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
     const bool plain = plain_scales4<BF16>(r.scales);
 #pragma unroll
-    for (int k = 0; k < G / 2; ++k) {
+    for (int k = 0; k < (G + 1) / 2; ++k) {
       const uint32_t b0 = r.scales >> (16 * k) & 255u, b1 = r.scales >> (16 * k + 8) & 255u;
       uint32_t y[4];
       if (plain) {
@@ -94,15 +94,15 @@ __device__ __forceinline__ void write(T* dst, const Raw<G>& r, bool vec) {
         y[3] = z[3];
       }
       store4<T>(dst + 64 * k, reinterpret_cast<const Four<T>&>(y[0]), vec);
-      store4<T>(dst + 64 * k + 32, reinterpret_cast<const Four<T>&>(y[2]), vec);
+      if (2 * k + 1 < G) store4<T>(dst + 64 * k + 32, reinterpret_cast<const Four<T>&>(y[2]), vec);
     }
   } else {
 #pragma unroll
-    for (int k = 0; k < G / 2; ++k) {
+    for (int k = 0; k < (G + 1) / 2; ++k) {
       uint32_t h[4];
       e2m1x8_f16(r.w[k], h[0], h[1], h[2], h[3]);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
+      for (int e = 0; e < 2 && 2 * k + e < G; ++e) {
         const float s = scale_of4(r.scales >> (16 * k + 8 * e) & 255u);
         const float2 lo = f16x2_f32(h[2 * e]), hi = f16x2_f32(h[2 * e + 1]);
         store4<T>(dst + 64 * k + 32 * e, Four<T>{lo.x * s, lo.y * s, hi.x * s, hi.y * s}, vec);
@@ -165,6 +165,7 @@ cudaError_t launch(const QuantMoveArgs& a, cudaStream_t st) {
   const int grid = int(ctas < (1 << 20) ? ctas : (1 << 20));
   if (grid <= 0) return cudaSuccess;
   if (a.D == 128) quant4_read_kernel<T, 4><<<grid, kThreads, 0, st>>>(a, runs);
+  else if (a.D == 96) quant4_read_kernel<T, 3><<<grid, kThreads, 0, st>>>(a, runs);
   else if (a.D == 64) quant4_read_kernel<T, 2><<<grid, kThreads, 0, st>>>(a, runs);
   else quant4_read_kernel<T, 0><<<grid, kThreads, 0, st>>>(a, runs);
   return cudaGetLastError();

@@ -9,8 +9,9 @@
 //
 // Memory bounds it: every value is read and written once, and the table's row of a token (8 bytes per pair) once per
 // warp that works on the token, from L2.  A warp takes a run of one token's passes:
-//   where the type stays, a pass is 16 values per lane (two pieces of 8 that turn together: 16-byte accesses) of as
-//     many heads as 32 lanes hold; a lane's dims are the same in every pass, so its sines and cosines stay in registers;
+//   where the type stays, a pass is 16 values per lane (two pieces of 8 that turn together: 16-byte accesses; pieces of 4
+//     where the rotation ends on no multiple of 16) of as many heads as 32 lanes hold; a lane's dims are the same in every
+//     pass, so its sines and cosines stay in registers;
 //   into rows, a pass is four heads of a plane, eight lanes each, lane p holding values 4 p .. 4 p + 3 of every group of 32, which
 //     is what the 4-bit row keeps together, and a group's maximum is three shuffles (of two groups at once where the
 //     values are 16-bit and do not turn).
@@ -54,6 +55,7 @@ __device__ __forceinline__ Token find(const RotateArgs& a, int t, int lane, cons
   return k;
 }
 
+// (Scalar operations: packed 32-bit products and sums give other digits, they are fused on the way to machine code.)
 __device__ __forceinline__ void turn(float& x, float& y, float c, float s) {
   const float u = __fsub_rn(__fmul_rn(x, c), __fmul_rn(y, s));
   y = __fadd_rn(__fmul_rn(y, c), __fmul_rn(x, s));
@@ -97,52 +99,44 @@ __device__ __forceinline__ void narrow2(float2 x, float* p) {
 __device__ __forceinline__ void narrow2(float2 x, __half* p) { *reinterpret_cast<__half2*>(p) = __float22half2_rn(x); }
 __device__ __forceinline__ void narrow2(float2 x, __nv_bfloat16* p) { *reinterpret_cast<__nv_bfloat162*>(p) = __float22bfloat162_rn(x); }
 
-// Two pairs.  (Packed 32-bit products and sums give other digits: they are fused on the way to machine code.)
-__device__ __forceinline__ void turn2(float2& x, float2& y, float2 c, float2 s) {
-  turn(x.x, y.x, c.x, s.x);
-  turn(x.y, y.y, c.y, s.y);
-}
-
 // ------------------------------------------------------------------------------ the type stays
-// A lane's 16 values of a head: pieces at dims d0 and d1 that turn together; i: the pair of the first value, -1: they stay.
+// A lane's 2 N values of a head: pieces at dims d0 and d1 that turn together; i: the pair of the first value, -1: they stay.
 struct Item {
   int d0, d1, i;
 };
+template <int N>
 __device__ __forceinline__ Item item_of(const RotateArgs& a, int j) {
-  const int turned = a.rot / 16;
-  if (j >= turned) return {16 * j, 16 * j + 8, -1};
-  if (a.pairs) return {16 * j, 16 * j + 8, 8 * j};
-  return {8 * j, 8 * j + a.rot / 2, 8 * j};
+  if (2 * N * j >= a.rot) return {2 * N * j, 2 * N * j + N, -1};
+  if (a.pairs) return {2 * N * j, 2 * N * j + N, N * j};
+  return {N * j, N * j + a.rot / 2, N * j};
 }
 
-// Four neighbouring pairs.
-template <typename T>
-__device__ __forceinline__ void turn_pairs(Piece<T, 8>& p, float2 c0, float2 s0, float2 c1, float2 s1) {
+// Neighbouring pairs of a piece, from pair k of the lane's on.
+template <typename T, int N>
+__device__ __forceinline__ void turn_pairs(Piece<T, N>& p, const float* c, const float* s) {
 #pragma unroll
-  for (int k = 0; k < 8; k += 4) {
-    float2 u = make_float2(to_f32(p.v[k]), to_f32(p.v[k + 2])), v = make_float2(to_f32(p.v[k + 1]), to_f32(p.v[k + 3]));
-    turn2(u, v, k ? c1 : c0, k ? s1 : s0);
-    p.v[k] = narrow<T>(u.x);
-    p.v[k + 1] = narrow<T>(v.x);
-    p.v[k + 2] = narrow<T>(u.y);
-    p.v[k + 3] = narrow<T>(v.y);
+  for (int k = 0; k < N; k += 2) {
+    float u = to_f32(p.v[k]), v = to_f32(p.v[k + 1]);
+    turn(u, v, c[k / 2], s[k / 2]);
+    p.v[k] = narrow<T>(u);
+    p.v[k + 1] = narrow<T>(v);
   }
 }
 
 // Passes [first, first + n) of token t: heads in blocks of as many as 32 lanes hold, of q, then k, then v, layer by layer.
-template <typename T, bool KV>
+template <typename T, int N, bool KV>
 __device__ __forceinline__ void same_type(const RotateArgs& a, int t, int first, int n, const Token& tok,
                                           const float* angles, int lane) {
-  using P8 = Piece<T, 8>;
-  const int per = a.D / 16, block = 32 / per;               // lanes per head, heads per pass
+  using P = Piece<T, N>;
+  const int per = a.D / (2 * N), block = 32 / per;          // lanes per head, heads per pass
   const int hl = lane / per, j = lane - hl * per;
-  const Item it = item_of(a, j);
-  float2 c[4], s[4];
+  const Item it = item_of<N>(a, j);
+  float c[N], s[N];
   if (it.i >= 0) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      reinterpret_cast<float4*>(c)[k] = __ldg(reinterpret_cast<const float4*>(angles + it.i + 4 * k));
-      reinterpret_cast<float4*>(s)[k] = __ldg(reinterpret_cast<const float4*>(angles + a.rot / 2 + it.i + 4 * k));
+    for (int k = 0; k < N; k += 4) {
+      *reinterpret_cast<float4*>(c + k) = __ldg(reinterpret_cast<const float4*>(angles + it.i + k));
+      *reinterpret_cast<float4*>(s + k) = __ldg(reinterpret_cast<const float4*>(angles + a.rot / 2 + it.i + k));
     }
   }
   const int nq = (a.Hq + block - 1) / block, nk = KV ? (a.Hkv + block - 1) / block : 0;
@@ -167,33 +161,34 @@ __device__ __forceinline__ void same_type(const RotateArgs& a, int t, int first,
     const int live = hl < block && (w == 0 || tok.at >= 0) ? heads - h0 : 0;      // heads from this lane's on
 #pragma unroll 1
     for (int i = 0; i < m; i += kAhead, src += kAhead * src_step, dst += kAhead * dst_step) {
-      P8 x[kAhead], y[kAhead];
+      P x[kAhead], y[kAhead];
 #pragma unroll
       for (int e = 0; e < kAhead; ++e)
         if (i + e < m && (i + e) * block < live) {
-          x[e] = load<T, 8>(src + e * src_step + it.d0, true);
-          y[e] = load<T, 8>(src + e * src_step + it.d1, true);
+          x[e] = load<T, N>(src + e * src_step + it.d0, true);
+          y[e] = load<T, N>(src + e * src_step + it.d1, true);
         }
 #pragma unroll
       for (int e = 0; e < kAhead; ++e) {
         if (i + e >= m || (i + e) * block >= live) continue;
         if (turns) {
           if (a.pairs) {
-            turn_pairs(x[e], c[0], s[0], c[1], s[1]);
-            turn_pairs(y[e], c[2], s[2], c[3], s[3]);
+            turn_pairs<T, N>(x[e], c, s);
+            turn_pairs<T, N>(y[e], c + N / 2, s + N / 2);
           } else {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              float2 u = make_float2(to_f32(x[e].v[2 * k]), to_f32(x[e].v[2 * k + 1]));
-              float2 v = make_float2(to_f32(y[e].v[2 * k]), to_f32(y[e].v[2 * k + 1]));
-              turn2(u, v, c[k], s[k]);
-              narrow2(u, x[e].v + 2 * k);
-              narrow2(v, y[e].v + 2 * k);
+            for (int k = 0; k < N; k += 2) {
+              float2 u = make_float2(to_f32(x[e].v[k]), to_f32(x[e].v[k + 1]));
+              float2 v = make_float2(to_f32(y[e].v[k]), to_f32(y[e].v[k + 1]));
+              turn(u.x, v.x, c[k], s[k]);
+              turn(u.y, v.y, c[k + 1], s[k + 1]);
+              narrow2(u, x[e].v + k);
+              narrow2(v, y[e].v + k);
             }
           }
         }
-        store<T, 8>(dst + e * dst_step + it.d0, x[e], true);
-        store<T, 8>(dst + e * dst_step + it.d1, y[e], true);
+        store<T, N>(dst + e * dst_step + it.d0, x[e], true);
+        store<T, N>(dst + e * dst_step + it.d1, y[e], true);
       }
     }
     n -= m;
@@ -274,9 +269,10 @@ __device__ __forceinline__ void tops(const float (&x)[N][4], uint32_t (&top)[N])
   }
 }
 
-// How keys turn on their way into rows: not at all; all of a head's dims in halves, so that the values that turn together are
-// in one lane; or in any way, the other value of a pair fetched from memory.
-enum Turns { kStay, kInLane, kAny };
+// How keys turn on their way into rows: not at all; in halves a whole number of groups apart (1, or 2 of 4), so that the
+// values that turn together are in one lane; in neighbouring pairs, which always are; or in any way, the other value of a
+// pair fetched from memory.  In a lane, its angles stay in registers.
+enum Turns { kStay, kInLane, kPairs, kAny };
 
 // Passes [first, first + n) of token t, plane by plane (k's, then v's, of each layer): four heads each, eight lanes per head.
 // G: groups of a head (0: any number, a.D / 32, one at a time).
@@ -286,13 +282,26 @@ __device__ __forceinline__ void quantise(const RotateArgs& a, int t, int first, 
   const int p = lane & 7, groups = G ? G : a.D / 32, nb = (a.Hkv + 3) / 4;
   [[maybe_unused]] const int half = a.rot / 2;
   constexpr int kAt = G ? G : 1;              // groups at a time
-  [[maybe_unused]] float4 c[(kAt + 1) / 2], s[(kAt + 1) / 2];
+  [[maybe_unused]] float c[kAt][2], s[kAt][2];              // in halves: 4 of group pair i in c[2 i], c[2 i + 1]
+  [[maybe_unused]] const int apart = a.rot / 64;            // groups between the halves
   if constexpr (TURNS == kInLane) {
 #pragma unroll
-    for (int g = 0; g < kAt / 2; ++g) {
-      c[g] = __ldg(reinterpret_cast<const float4*>(angles + 32 * g + 4 * p));
-      s[g] = __ldg(reinterpret_cast<const float4*>(angles + half + 32 * g + 4 * p));
-    }
+    for (int g = 0; g < kAt / 2; ++g)
+      if (g < apart)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          c[2 * g + k / 2][k & 1] = __ldg(angles + 32 * g + 4 * p + k);
+          s[2 * g + k / 2][k & 1] = __ldg(angles + half + 32 * g + 4 * p + k);
+        }
+  } else if constexpr (TURNS == kPairs) {
+#pragma unroll
+    for (int g = 0; g < kAt; ++g)
+      if (32 * g + 4 * p < a.rot)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          c[g][k] = __ldg(angles + 16 * g + 2 * p + k);
+          s[g][k] = __ldg(angles + half + 16 * g + 2 * p + k);
+        }
   }
   // A lane's heads past the last are the last once more, not stored: the shuffles are the whole warp's.
   auto source = [&](int lp, int hb) -> const T* {
@@ -341,31 +350,43 @@ __device__ __forceinline__ void quantise(const RotateArgs& a, int t, int first, 
     for (int g = 0; g < kAt; ++g)
 #pragma unroll
       for (int k = 0; k < 4; ++k) x[g][k] = to_f32(raw[g].v[k]);
-    if constexpr (TURNS == kInLane) {
-      if (turns) {
+    if (turns) {
+      if constexpr (TURNS == kInLane) {
+        auto both = [&](int g, int other, int at) {
 #pragma unroll
-        for (int g = 0; g < kAt / 2; ++g) {
-          turn(x[g][0], x[g + kAt / 2][0], c[g].x, s[g].x);
-          turn(x[g][1], x[g + kAt / 2][1], c[g].y, s[g].y);
-          turn(x[g][2], x[g + kAt / 2][2], c[g].z, s[g].z);
-          turn(x[g][3], x[g + kAt / 2][3], c[g].w, s[g].w);
+          for (int k = 0; k < 4; ++k) turn(x[g][k], x[other][k], c[2 * at + k / 2][k & 1], s[2 * at + k / 2][k & 1]);
+        };
+        if (kAt == 2 || apart == 1) {
+          both(0, kAt > 1 ? 1 : 0, 0);
+        } else {
+          both(0, kAt / 2, 0);
+          both(kAt > 2 ? 1 : 0, kAt > 2 ? 3 : 0, kAt > 2 ? 1 : 0);
         }
-      }
-    } else if constexpr (TURNS == kAny) {
-      const int d = 32 * this_g + 4 * p;
-      if (turns && d < a.rot) {
-        if (a.pairs) {
-          turn(x[0][0], x[0][1], __ldg(angles + d / 2), __ldg(angles + half + d / 2));
-          turn(x[0][2], x[0][3], __ldg(angles + d / 2 + 1), __ldg(angles + half + d / 2 + 1));
-        } else {                              // the other values of the pairs, from memory
-          const bool low = d < half;
-          const Piece<T, 4> other = load<T, 4>(this_src + 32 * this_g + (low ? half : -half), a.vec_in);
-          const float* at = angles + (low ? d : d - half);
+      } else if constexpr (TURNS == kPairs) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            float u = low ? x[0][k] : to_f32(other.v[k]), v = low ? to_f32(other.v[k]) : x[0][k];
-            turn(u, v, __ldg(at + k), __ldg(at + half + k));
-            x[0][k] = low ? u : v;
+        for (int g = 0; g < kAt; ++g)
+          if (32 * g + 4 * p < a.rot) {
+            turn(x[g][0], x[g][1], c[g][0], s[g][0]);
+            turn(x[g][2], x[g][3], c[g][1], s[g][1]);
+          }
+      } else {
+#pragma unroll
+        for (int g = 0; g < kAt; ++g) {
+          const int d = 32 * (this_g + g) + 4 * p;
+          if (d >= a.rot) continue;
+          if (a.pairs) {
+            turn(x[g][0], x[g][1], __ldg(angles + d / 2), __ldg(angles + half + d / 2));
+            turn(x[g][2], x[g][3], __ldg(angles + d / 2 + 1), __ldg(angles + half + d / 2 + 1));
+          } else {
+            const bool low = d < half;
+            const Piece<T, 4> other = load<T, 4>(this_src + 32 * (this_g + g) + (low ? half : -half), a.vec_in);
+            const float* at = angles + (low ? d : d - half);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              float u = low ? x[g][k] : to_f32(other.v[k]), v = low ? to_f32(other.v[k]) : x[g][k];
+              turn(u, v, __ldg(at + k), __ldg(at + half + k));
+              x[g][k] = low ? u : v;
+            }
           }
         }
       }
@@ -412,8 +433,12 @@ __device__ __forceinline__ void quantise(const RotateArgs& a, int t, int first, 
       } else {
 #pragma unroll
         for (int g = 0; g < kAt; ++g) {
-          dst[2 * g] = uint8_t(packed[g]);
-          dst[2 * g + 1] = uint8_t(packed[g] >> 8);
+          if (a.vec_out) {
+            reinterpret_cast<uint16_t*>(dst)[g] = uint16_t(packed[g]);
+          } else {
+            dst[2 * g] = uint8_t(packed[g]);
+            dst[2 * g + 1] = uint8_t(packed[g] >> 8);
+          }
         }
       }
     }
@@ -429,7 +454,7 @@ __device__ __forceinline__ void quantise(const RotateArgs& a, int t, int first, 
 // ------------------------------------------------------------------------------ the kernel
 // A token's work: passes of q (and where the type stays of k and v), then passes of rows to quantise, in runs of `run`
 // passes of one kind, a run per warp.
-template <typename T, int BITS, int G, Turns TURNS, bool VEC>
+template <typename T, int BITS, int G, Turns TURNS, int PIECE>
 __global__ void __launch_bounds__(kThreads, BITS == 0 || TURNS == kStay ? 8 : 5)
     rotate_write_kernel(const __grid_constant__ RotateArgs a, int run, int item_passes, int item_runs, int runs) {
   const int lane = threadIdx.x & 31;
@@ -443,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, BITS == 0 || TURNS == kStay ? 8 : 5)
     if (!tok.live) continue;
     if (TURNS != kStay && which < item_runs) {
       const int first = which * run, n = min(run, item_passes - first);
-      if constexpr (VEC) same_type<T, BITS == 0>(a, t, first, n, tok, angles, lane);
+      if constexpr (PIECE > 0) same_type<T, PIECE, BITS == 0>(a, t, first, n, tok, angles, lane);
       else any_layout<T>(a, t, first * 32, n * 32, tok, angles, lane);
     } else if constexpr (BITS != 0) {
       const int first = (which - item_runs) * run;
@@ -452,10 +477,10 @@ __global__ void __launch_bounds__(kThreads, BITS == 0 || TURNS == kStay ? 8 : 5)
   }
 }
 
-template <typename T, int BITS, int G, Turns TURNS, bool VEC>
+template <typename T, int BITS, int G, Turns TURNS, int PIECE>
 cudaError_t launch(const RotateArgs& a, cudaStream_t st) {
-  const int block = VEC ? 32 / (a.D / 16) : 1;
-  const int64_t items = TURNS == kStay ? 0 : VEC
+  const int block = PIECE ? 32 / (a.D / (2 * PIECE)) : 1;
+  const int64_t items = TURNS == kStay ? 0 : PIECE
       ? int64_t(a.L) * ((a.Hq + block - 1) / block + (BITS == 0 ? 2 * ((a.Hkv + block - 1) / block) : 0))
       : (int64_t(a.L) * (a.Hq + (BITS == 0 ? 2 * a.Hkv : 0)) * (a.rot / 2 + a.D - a.rot) + 31) / 32;
   const int64_t rows = BITS == 0 ? 0 : int64_t(2) * a.L * ((a.Hkv + 3) / 4);
@@ -465,28 +490,43 @@ cudaError_t launch(const RotateArgs& a, cudaStream_t st) {
   while (run > 1 && a.T * runs(run) < int64_t(device_sm_count()) * 16) run /= 2;
   const int64_t warps = a.T * runs(run), ctas = (warps + kThreads / 32 - 1) / (kThreads / 32);
   if (ctas == 0) return cudaSuccess;
-  rotate_write_kernel<T, BITS, G, TURNS, VEC><<<unsigned(ctas < (1 << 20) ? ctas : (1 << 20)), kThreads, 0, st>>>(
+  rotate_write_kernel<T, BITS, G, TURNS, PIECE><<<unsigned(ctas < (1 << 20) ? ctas : (1 << 20)), kThreads, 0, st>>>(
       a, run, int(items), int((items + run - 1) / run), int(runs(run)));
   return cudaGetLastError();
 }
 
+template <typename T>
+cudaError_t launch_same(const RotateArgs& a, cudaStream_t st) {
+  const bool aligned = a.vec_in && a.vec_out;               // pieces with the rotation's ends on them, and a head in 32 lanes
+  if (aligned && a.D % 16 == 0 && a.rot % 16 == 0 && a.D <= 512) return launch<T, 0, 0, kAny, 8>(a, st);
+  if (aligned && a.D % 8 == 0 && a.rot % 8 == 0 && a.D <= 256) return launch<T, 0, 0, kAny, 4>(a, st);
+  return launch<T, 0, 0, kAny, 0>(a, st);
+}
+
 template <typename T, int BITS>
-cudaError_t launch_bits(const RotateArgs& a, cudaStream_t st) {
-  // whole pieces of 8 values, with the rotation's ends on them, in q (and in the cache where its type stays)
-  const bool vec = a.vec_in && (BITS != 0 || a.vec_out) && a.D % 16 == 0 && a.D <= 512 && a.rot % 16 == 0;
-  if constexpr (BITS == 4) {
-    if (a.rot == 0)
-      return a.D == 128 ? launch<T, 4, 4, kStay, true>(a, st) : (a.D == 64 ? launch<T, 4, 2, kStay, true>(a, st) : launch<T, 4, 0, kStay, true>(a, st));
-    if (vec && a.rot == a.D && !a.pairs && a.D == 64) return launch<T, 4, 2, kInLane, true>(a, st);
+cudaError_t launch_rows(const RotateArgs& a, cudaStream_t st) {
+  if constexpr (BITS == 4)
+    if (a.rot == 0) {
+      if (a.D == 128) return launch<T, 4, 4, kStay, 8>(a, st);
+      if (a.D == 96) return launch<T, 4, 3, kStay, 8>(a, st);
+      return a.D == 64 ? launch<T, 4, 2, kStay, 8>(a, st) : launch<T, 4, 0, kStay, 8>(a, st);
+    }
+  if (!a.vec_in || a.D % 16 || a.rot % 16 || a.D > 512) return launch<T, BITS, 0, kAny, 0>(a, st);
+  if (a.D == 128) {
+    if (a.pairs) return launch<T, BITS, 4, kPairs, 8>(a, st);
+    if (a.rot == 128 || a.rot == 64) return launch<T, BITS, 4, kInLane, 8>(a, st);
   }
-  if constexpr (BITS != 0)
-    if (vec && a.rot == a.D && !a.pairs && a.D == 128) return launch<T, BITS, 4, kInLane, true>(a, st);
-  return vec ? launch<T, BITS, 0, kAny, true>(a, st) : launch<T, BITS, 0, kAny, false>(a, st);
+  if constexpr (BITS == 4) {
+    if (a.D == 64 && a.pairs) return launch<T, 4, 2, kPairs, 8>(a, st);
+    if (a.D == 64 && a.rot == 64) return launch<T, 4, 2, kInLane, 8>(a, st);
+    if (a.D == 96) return launch<T, 4, 3, kAny, 8>(a, st);
+  }
+  return launch<T, BITS, 0, kAny, 8>(a, st);
 }
 
 template <typename T>
 cudaError_t launch_type(const RotateArgs& a, cudaStream_t st) {
-  return a.bits == 0 ? launch_bits<T, 0>(a, st) : (a.bits == 8 ? launch_bits<T, 8>(a, st) : launch_bits<T, 4>(a, st));
+  return a.bits == 0 ? launch_same<T>(a, st) : (a.bits == 8 ? launch_rows<T, 8>(a, st) : launch_rows<T, 4>(a, st));
 }
 
 }  // namespace

@@ -20,6 +20,8 @@ SHAPES = {
     "one narrow head": ([50], [50], 1, 32, 24, 2, BF),
     "wide head": ([50], [9], 2, 256, 16, 1, BF),
     "odd layers": ([70, 80], [9, 1], 4, 128, 16, 5, BF),
+    "96": ([33, 80], [33, 1], 5, 96, 16, 2, BF),
+    "96 fp16": ([33, 80], [33, 1], 8, 96, 16, 2, HF),
     "seven heads of 64": ([33, 80], [33, 1], 7, 64, 16, 1, FP),
 }
 
@@ -118,7 +120,12 @@ def test_odd_strides_and_alignment():
     """Rows longer than they need be and off 16 bytes, inputs and outputs of other strides and off alignment."""
     dev = need_gpu()
     from actkv_open_b200.kernels.quant_cache import dequantize_read, quantize_write
-    lens, new, hkv, d, bs = [40, 21], [33, 5], 3, 64, 16
+    for d in (64, 96, 128):
+        _odd(dev, d, dequantize_read, quantize_write)
+
+
+def _odd(dev, d, dequantize_read, quantize_write):
+    lens, new, hkv, bs = [40, 21], [33, 5], 3, 16
     table, nb, off, _, k, v, _ = Q.new_tokens(lens, new, 1, hkv, d, bs, 2, BF, seed=9)
     seq = torch.tensor(lens, dtype=torch.int32, device=dev)
     n = int(off[-1])

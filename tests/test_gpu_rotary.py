@@ -25,6 +25,14 @@ SHAPES = {
     "odd sizes": ([37, 5], [20, 5], 3, 1, 50, 5, 2, BF, 22, False),
     "odd sizes, pairs": ([37, 5], [20, 5], 3, 1, 50, 5, 2, FP, 22, True),
     "wide head": ([40], [30], 2, 2, 256, 16, 1, BF, 256, False),
+    "pairs of 128": ([100, 20], [50, 7], 4, 2, 128, 16, 2, BF, 128, True),
+    "part, pairs of 128": ([100, 20], [50, 7], 4, 5, 128, 16, 2, BF, 80, True),
+    "part of 80": ([100, 20], [50, 7], 7, 4, 80, 16, 3, BF, 40, False),
+    "part of 80, pairs": ([100, 20], [50, 7], 7, 4, 80, 16, 3, HF, 40, True),
+    "pieces of 4, fp32": ([70, 20], [50, 7], 3, 2, 72, 16, 2, FP, 24, False),
+    "96, three heads": ([100, 20], [50, 7], 5, 3, 96, 16, 2, BF, 96, False),
+    "96, pairs": ([100, 20], [50, 7], 5, 3, 96, 16, 2, HF, 48, True),
+    "64, one head": ([100, 20], [50, 7], 1, 1, 64, 16, 4, HF, 64, False),
     "many tokens": ([2000, 700, 3], [1500, 700, 3], 8, 2, 128, 16, 2, BF, 128, False),
 }
 
