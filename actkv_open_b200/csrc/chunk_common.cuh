@@ -15,7 +15,9 @@ using namespace umma;
 constexpr int kRows = 128;                  // query rows per row tile (MMA M)
 constexpr int kTile = 128;                  // tokens per key tile, the grain of the schedule
 constexpr int kFewRows = 16;                // query rows of a session and KV head that chunk_few_kernel takes
-constexpr int few_limit(int quant) { return quant ? 8 : kFewRows; }       // ... of which over the 8- and 4-bit caches
+constexpr int few_group(int quant) { return quant ? 8 : kFewRows; }       // ... at a time over the 8- and 4-bit caches
+constexpr int kFewRows4 = 32;               // chunk_few4_kernel takes several times as many
+constexpr int few_limit(int quant) { return quant == 4 ? kFewRows4 : few_group(quant); }
 constexpr int kFewParts = 8 * kFewRows;     // rows of its units: up to 8 heads
 // (6 sessions of 2000 to 10000 tokens with 1088 new: 749 us with a cost of 2, 713 with 4, 708 with 6; prompts and
 // single tokens of head size 64: 157, 153, 157)

@@ -15,7 +15,10 @@
 // that what is 2^-28 of it is still exact.  p is rounded to fp16's 11 bits (times 2^7 and the scale: what comes out
 // below fp16's normal range loses the digits below 2^-32 of the largest).
 //
-// Tokens that some of the rows do not see are the newest ones, 7 at most: their values are added in 32 bits one
+// A session of more than 8 rows per KV head goes in groups of 8, each reading the cache again (most of it from L2): up to
+// 32 rows that is faster than the wide kernel.
+//
+// Tokens that some of a group's rows do not see are the newest ones, 7 at most: their values are added in 32 bits one
 // token at a time, each row with an E of its own from there on, so that a hidden value of any size changes nothing in the
 // rows that do not see it.
 #include <type_traits>
@@ -31,6 +34,7 @@ constexpr int kStep = 32;                   // tokens per step of a warp
 constexpr int kWarps = 16, kThreads = kWarps * 32;
 constexpr int kRoundCost = 3;               // a unit's fixed cost in rounds of its warps
 constexpr int kMinRounds = 1;               // the least share of a CTA (one token over 2000: 27.6 us with 3, 25.3 with 2, 23.0 with 1)
+constexpr int kRowsMax = 8;                 // query rows of a group: the products' columns
 constexpr float kLowest = -3.0e38f;         // m of a row before its first token: below any logit, and finite
 constexpr float kPBits = 7.0f;              // p, and l with it, is held times 2^7 (kPScale, here by way of the exponent)
 
@@ -142,11 +146,19 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
   const int my_head = warp % HG, my_part = warp / HG;
   const int few_rows = few_rows_now<kThreads>(a, sched.sums);
   if (few_rows == 0) return;
+  // A session's rows go in groups of up to 8 (whole tokens), each reading the tokens that some row of it sees.
+  const int per_group = kRowsMax / a.G;
+  auto rounds = [&](int sees) { return (held_tokens(a, sees) + round - 1) / round; };
+  auto rounds_of = [&](int A, int S) {        // of one group of heads, with the groups' fixed costs
+    int n = 0;
+    for (int j = 0; j < A; j += per_group) n += kRoundCost + rounds(S - A + min(A, j + per_group));
+    return n;
+  };
   share_out<kThreads>(a.R, [&](int r) -> int64_t {
     const int A = new_tokens(a, r), S = a.seq_used[r];
     if (A == 0 || A * a.G > few_rows) return 0;
     flag_long(a, S);
-    return int64_t(a.Hkv / HG) * (kRoundCost + (held_tokens(a, S) + round - 1) / round);
+    return int64_t(a.Hkv / HG) * rounds_of(A, S);
   }, sched.share, sched.scan, cta, n_cta, kMinRounds);
   // The share is [lo, lo + span) of the schedule; places in it are kept relative to lo, in 32 bits (registers are short).
   auto n_used = [&] { return used_ctas(sched.share.total, n_cta, kMinRounds); };
@@ -164,31 +176,35 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
   auto bytes_at = [&](int64_t off) { return static_cast<const char*>(a.kv) + off; };
 
   for (; r < a.R && at < span; ++r, hg = 0) {
-    const int A = new_tokens(a, r), S = a.seq_used[r];
+    int A = new_tokens(a, r);
+    const int S = a.seq_used[r];
     if (A == 0 || A * a.G > few_rows) continue;
-    const int rows = A * a.G;
-    const int nt = (held_tokens(a, S) + round - 1) / round, weight = kRoundCost + nt;
-    if (seek) {                               // the group that holds lo
-      hg = -at / weight;
-      at += hg * weight;
+    if (seek) {                               // the group of heads that holds lo
+      const int each = rounds_of(A, S);
+      hg = -at / each;
+      at += hg * each;
       seek = false;
     }
-    const int32_t* table = a.block_table + r * a.bt_stride_r;
-    for (; hg < a.Hkv / HG && at < span; ++hg, at += weight) {
-      const int first = at + kRoundCost;
-      const int t0 = max(-first, 0), t1 = nt == 0 ? 0 : min(nt, span - first);
-      if (nt == 0 ? at < 0 : t0 >= t1) continue;
-      const int h = hg * HG + my_head;
-      const int begin = t0 * round, end = min(t1 * round, held_tokens(a, S));
+    for (int j0 = 0; hg < a.Hkv / HG && at < span; j0 = j0 + per_group < A ? j0 + per_group : 0, hg += j0 == 0) {
+      int ntok = min(per_group, A - j0), rows = ntok * a.G;
+      const int all = a.seq_used[r] - A + j0; // tokens that all rows see: up to this one
+      int nt = rounds(all + ntok), first = at + kRoundCost;
+      at += kRoundCost + nt;
+      int t0 = max(-first, 0), t1 = nt == 0 ? 0 : min(nt, span - first);
+      if (nt == 0 ? first < kRoundCost : t0 >= t1) continue;
+      int h = hg * HG + my_head;
+      const int32_t* table = a.block_table + r * a.bt_stride_r;
+      int begin = t0 * round;
+      const int end = min(t1 * round, held_tokens(a, all + ntok));
       const int start = begin + my_part * kStep;              // this warp's steps: start, start + round, ...
       const int mine = start < end ? (end - start + round - 1) / round : 0;
       // the lane's two query rows; the first sees the tokens up to all + row0 / G, the second up to all + row1 / G
-      const int row0 = 2 * c4, row1 = row0 + 1, all = S - A;
+      const int row0 = 2 * c4, row1 = row0 + 1;
       // ---- queries as the second operand, row r8: of k-step (group g, i) dims 32 g + 8 c4 + 4 i .. + 3
       uint32_t q[2 * G][2];
       {
         const int jq = r8 / a.G;
-        const uint16_t* p = static_cast<const uint16_t*>(a.q) + (int64_t(a.q_off[r]) + jq) * a.q_stride_t +
+        const uint16_t* p = static_cast<const uint16_t*>(a.q) + (int64_t(a.q_off[r]) + j0 + jq) * a.q_stride_t +
                             int64_t(h * a.G + r8 - jq * a.G) * a.q_stride_h;
 #pragma unroll
         for (int k = 0; k < 2 * G; ++k) {
@@ -227,6 +243,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
         for (int g = 0; g < G; ++g)
           *reinterpret_cast<uint4*>(smem + Rg::kQ + (my_head * G + g) * 512 + lane * 16) =
               make_uint4(q[2 * g][0], q[2 * g][1], q[2 * g + 1][0], q[2 * g + 1][1]);
+      }
+      // What the steps have no use for waits in shared memory (as spilled registers they came back in every step: 185 us for
+      // 32 single tokens of 4096 to 32768, 171 so).
+      if (threadIdx.x == 0) {
+        const int u[10] = {r, hg, j0, at, A, nt, first, t0, t1, ntok};
+#pragma unroll
+        for (int i = 0; i < 10; ++i) sched.unit[i] = u[i];
       }
       __syncthreads();
       const uint32_t q_at = smem_u32(smem) + Rg::kQ + my_head * (G * 512) + lane * 16;
@@ -643,6 +666,23 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
         __syncwarp();                         // every lane has read the slot that the next copies fill, and the tables
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
+      {
+        const volatile int* u = sched.unit;
+        r = u[0];
+        hg = u[1];
+        j0 = u[2];
+        at = u[3];
+        A = u[4];
+        nt = u[5];
+        first = u[6];
+        t0 = u[7];
+        t1 = u[8];
+        ntok = u[9];
+        rows = ntok * a.G;
+        h = hg * HG + my_head;
+        begin = t0 * round;
+        table = a.block_table + r * a.bt_stride_r;
+      }
       // ---- results: l of a row over the lanes that share it; O as the sums of p v (of 2^7 p v in fp16) that the join takes
 #pragma unroll
       for (int x = 4; x < 32; x *= 2) {
@@ -708,7 +748,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
           if (row >= rows) continue;
           const float L = hf ? l1 : l0, M = hf ? m1 : m0, inv = over<BF16>(L);
           const int jq = row / a.G, hq = h * a.G + row - jq * a.G, hr = my_head * rows + row;
-          const int64_t qt = int64_t(a.q_off[r]) + jq;
+          const int64_t qt = int64_t(a.q_off[r]) + j0 + jq;
           uint16_t* dst = static_cast<uint16_t*>(a.out) + qt * a.out_stride_t + int64_t(hq) * a.out_stride_h;
           float* part = ps.out(cta, ps_slot) + int64_t(hr) * D;
           // NaN groups among the values of tokens that this row does see
@@ -759,9 +799,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
         ds.h = hg * HG;
         ds.heads = HG;
         ds.n_used = n_used();
-        ds.ntok = ds.A = a.q_off[r + 1] - a.q_off[r];
-        ds.S = a.seq_used[r];
-        ds.a0 = a.q_off[r];
+        ds.ntok = ds.A = ntok;
+        ds.S = all + ntok;
+        ds.a0 = a.q_off[r] + j0;
         ds.end = low() + first + nt;
         ds.total = sched.share.total;
         ps.desc[cta] = ds;

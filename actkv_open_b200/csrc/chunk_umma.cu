@@ -1516,7 +1516,7 @@ cudaError_t launch_chunk_umma(const ChunkArgs& args, int dtype, cudaStream_t st,
   *why = "chunk attention";
   const int grid = device_sm_count();
   // sessions of few query rows go to a kernel of their own, where a GQA group fits it
-  a.few_rows = a.G <= chunk::few_limit(a.quant) ? chunk::few_limit(a.quant) : 0;
+  a.few_rows = a.G <= chunk::few_group(a.quant) ? chunk::few_limit(a.quant) : 0;
   if (a.few_rows > 0) {
     const cudaError_t e = a.quant == 4 ? launch_chunk_few4(a, dtype, grid, st) : launch_chunk_few(a, dtype, grid, st);
     if (e != cudaSuccess) return e;

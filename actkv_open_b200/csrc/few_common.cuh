@@ -53,6 +53,7 @@ struct Sched {
   Share share;
   int64_t scan[32], sums[2];
   int bad_v;                 // values that are not finite went in as 0: 1 among those some row does not see, 2 anywhere
+  int unit[10];              // chunk_few4_kernel: what the unit in hand is, out of the registers while its steps run
 };
 static_assert(sizeof(Sched) <= 512, "the schedule's place in shared memory");
 

@@ -60,6 +60,31 @@ def test_cuda_core_path(name):
     assert_device_clean(dev)
 
 
+GROUPS = {   # lens, new, hq, hkv, block size: 9 to 32 rows per KV head, in groups of up to 8
+    "four of four": ([700, 129, 128, 4, 3000, 2], [4, 3, 4, 4, 4, 4], 32, 8, 16),
+    "sixteen of one": ([500, 16, 3, 1200], [16, 9, 16, 13], 2, 2, 16),
+    "ten of three": ([333, 64, 1000], [10, 4, 3], 12, 4, 32),
+    "four of eight": ([900, 33, 2, 2500], [4, 3, 4, 2], 32, 4, 16),
+    "six of five, one KV head": ([900, 33], [6, 5], 5, 1, 8),
+    "thirty-two of one, and longer": ([2000, 31, 400, 64], [32, 32, 33, 1], 8, 8, 64),
+    "seven of four, many": ([40 + 13 * i for i in range(40)], [i % 8 for i in range(40)], 8, 2, 16),
+}
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("name", GROUPS)
+def test_sessions_of_several_groups_of_rows_match_64_bits(name, d, dtype):
+    dev = need_gpu()
+    lens, new, hq, hkv, bs = GROUPS[name]
+    case = Case4(lens, new, hq, hkv, d, bs, dtype, seed=50 + len(name))
+    x = case.device(dev)
+    first = case.run(dev, given=x)
+    case.check(first)
+    assert _equal(first, case.run(dev, given=x))
+    assert_device_clean(dev)
+
+
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("name", FEW)
@@ -68,6 +93,54 @@ def test_sessions_of_a_few_rows_match_64_bits(name, d, dtype):
     lens, new, hq, hkv, bs = FEW[name]
     case = Case4(lens, new, hq, hkv, d, bs, dtype, seed=30 + len(name))
     case.check(case.run(dev))
+    assert_device_clean(dev)
+
+
+@pytest.mark.parametrize("d, dtype", [(128, BF), (64, HF)])
+def test_both_kernels_in_one_call(d, dtype):
+    """Short sessions of 32 MB of rows and more, of one and of several groups of rows, beside longer ones."""
+    dev = need_gpu()
+    from actkv_open_b200.kernels.quant_cache import dequantize_read, paged_chunk_attention_quant, quant_row_bytes, quantize_write
+    hq, hkv, bs = 32, 8, 16
+    lens = [6400 * 128 // d + 7 * i for i in range(9)]
+    new = [(0, 1, 2, 5, 8)[i % 5] for i in range(9)]
+    for at, s, a in ((0, 1500, 300), (3, 6000, 70), (len(lens), 40, 40), (len(lens) - 1, 5, 130)):
+        lens.insert(at, s)
+        new.insert(at, a)
+    assert sum(s for s, a in zip(lens, new) if 0 < a <= 8) * hkv * d >= 32 << 20
+    gen = torch.Generator(device=dev).manual_seed(31)
+    table, nb = C.pages(lens, bs, torch.Generator().manual_seed(31))
+    off = C.offsets(new)
+    table, seq, q_off, tok = table.to(dev), torch.tensor(lens, dtype=torch.int32, device=dev), off.to(dev), C.offsets(lens).to(dev)
+    q = torch.randn(int(off[-1]), hq, d, generator=gen, device=dev).to(dtype)
+    n = sum(lens)
+    k, v = (torch.randn(1, n, hkv, d, generator=gen, device=dev).to(dtype) for _ in range(2))
+    rows = torch.full((1, 2, nb, bs, quant_row_bytes(hkv, d, 4)), 255, dtype=torch.uint8, device=dev)
+    quantize_write(k, v, tok, rows, table, seq, bits=4)
+    k, v = dequantize_read(rows, hkv, d, tok, table, seq, n, dtype=dtype, bits=4)
+    call = lambda: paged_chunk_attention_quant(q, q_off, rows[0], hkv, table, seq, bits=4)             # noqa: E731
+    out, lse = call()
+    g = hq // hkv
+    for r, (s, a) in enumerate(zip(lens, new)):
+        if a == 0:
+            continue
+        o0, o1, t0 = int(off[r]), int(off[r + 1]), int(tok[r])
+        kk, vv = (x[0, t0:t0 + s].double() for x in (k, v))
+        qq = q[o0:o1].double().view(a, hkv, g, d)
+        hide = torch.arange(s, device=dev)[None] > torch.arange(s - a, s, device=dev)[:, None]
+        x = (torch.einsum("ahgd,shd->ahgs", qq, kk) * d ** -0.5).masked_fill(hide[:, None, None], -torch.inf)
+        one = torch.logsumexp(x, -1)
+        p = torch.where(torch.isfinite(one)[..., None], torch.exp(x - one[..., None]), torch.zeros_like(x))
+        want, mag = (torch.einsum("ahgs,shd->ahgd", p, y).reshape(a, hq, d) for y in (vv, vv.abs()))
+        size = (torch.einsum("ahgd,shd->ahgs", qq.abs(), kk.abs()).amax(-1) * d ** -0.5).view(a, hq)
+        one = one.view(a, hq)
+        tol = (2 * U[dtype] + 1e-4) * mag + (s * 2.0 ** -25 * vv.abs().amax() if dtype == HF else 0.0)
+        assert ((out[o0:o1].double() - want).abs() <= tol).all(), r
+        none = one == -torch.inf
+        assert torch.equal(lse[o0:o1] == -torch.inf, none) and (out[o0:o1][none] == 0).all()
+        assert ((lse[o0:o1].double() - one).abs()[~none] <= (2e-5 + 8e-6 * size)[~none]).all(), r
+    for _ in range(3):
+        assert _equal((out, lse), call())
     assert_device_clean(dev)
 
 
@@ -95,7 +168,7 @@ def test_flat_and_peaked_logits(gain, new):
 
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("d", [64, 128])
-@pytest.mark.parametrize("new", [1, 3, 90])
+@pytest.mark.parametrize("new", [1, 3, 9, 90])
 def test_scales_far_apart(new, d, dtype):
     """Tokens, groups and heads whose scales differ by up to 2^16, the largest values on tokens of little weight and on
     the newest (which some rows do not see): every value counts by its weight, in every row."""
@@ -114,7 +187,7 @@ def test_scales_far_apart(new, d, dtype):
     assert_device_clean(dev)
 
 
-@pytest.mark.parametrize("new", [2, 4, 90])
+@pytest.mark.parametrize("new", [2, 4, 11, 90])
 @pytest.mark.parametrize("lens", [500, 6000])
 @pytest.mark.parametrize("byte", [150, 200, 252])
 def test_large_hidden_values_reach_only_the_rows_that_see_them(byte, lens, new):
@@ -135,7 +208,7 @@ def test_large_hidden_values_reach_only_the_rows_that_see_them(byte, lens, new):
     case.cache[0, at, case.scale_at(0, 0):case.scale_at(4, 0)] = min(byte, 186)
     got = case.run(dev)
     assert _equal([x[rows] for x in got], [x[rows] for x in clean])
-    if new < 90:
+    if new < 16:
         assert not torch.isnan(got[0]).any() and not torch.isnan(got[1]).any()
         one = got[0][new - 1].cpu().double()
         logits = case.q[new - 1].double().view(4, 2, 1, 128) * case.tokens(0, 0)[-1].view(4, 1, 1, 128)
@@ -146,7 +219,7 @@ def test_large_hidden_values_reach_only_the_rows_that_see_them(byte, lens, new):
 
 
 @pytest.mark.parametrize("path", ["auto", "simt"])
-@pytest.mark.parametrize("new", [1, 3, 90])
+@pytest.mark.parametrize("new", [1, 3, 9, 90])
 def test_hidden_tokens_do_not_reach_a_query(path, new):
     """NaN groups (scale bytes 253 to 255) among keys and values, at a session's start, in its middle and among its new
     tokens: a value makes its group's dims NaN in the rows that see it, a key the whole row of its head, and nothing
@@ -217,7 +290,7 @@ def test_every_scale_byte_is_attended_as_it_is_read_back(new, path, d, dtype):
     assert_device_clean(dev)
 
 
-@pytest.mark.parametrize("new", [1, 3, 90, 200])
+@pytest.mark.parametrize("new", [1, 3, 13, 90, 200])
 def test_fp16_keeps_what_a_dominant_token_leaves(new):
     """As over the other caches: one token 17.4 above all others, with a zero value; the 2000 others have p = 2^-25.1."""
     dev = need_gpu()
@@ -238,7 +311,8 @@ def test_fp16_keeps_what_a_dominant_token_leaves(new):
 
 
 @pytest.mark.parametrize("lens, new, bs, d", [([500], [1], 16, 128), ([500], [3], 16, 64), ([500, 300], [90, 2], 16, 128),
-                                              ([700, 129], [300, 33], 64, 64), ([9000], [2], 16, 128), ([900], [140], 256, 128)])
+                                              ([700, 129], [300, 33], 64, 64), ([9000], [2], 16, 128), ([900], [140], 256, 128),
+                                              ([500, 90], [15, 9], 16, 128)])
 def test_tokens_of_blocks_outside_the_cache_are_hidden(lens, new, bs, d):
     dev = need_gpu()
     from actkv_open_b200 import _native as N
@@ -300,7 +374,7 @@ def test_units_that_see_nothing_among_units_that_do(d):
     assert_device_clean(dev)
 
 
-@pytest.mark.parametrize("new", [1, 3, 90])
+@pytest.mark.parametrize("new", [1, 3, 12, 90])
 def test_negative_lengths_and_lengths_past_the_table(new):
     dev = need_gpu()
     from actkv_open_b200 import _native as N
