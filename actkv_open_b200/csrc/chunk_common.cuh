@@ -56,11 +56,14 @@ __device__ __forceinline__ void flag_long(const ChunkArgs& a, int S) {
 // Query rows per KV head up to which chunk_few_kernel takes a session in this call, 0 when chunk_umma_kernel takes
 // all.  The two kernels run one after the other, so short work is not split between them: where the other kernel
 // has sessions too, those of few rows go to their own only when they hold bytes enough to win back a
-// kernel's start and end (about 15 us) by its higher rate: 512 MB of 16-bit rows, 64 MB of 8-bit ones.  Single tokens
+// kernel's start and end (about 15 us) by its higher rate: 512 MB of 16-bit rows, 64 MB of 8-bit ones, 20 MB of 4-bit ones.  Single tokens
 // over 8192 (32 query heads over 8 of 128) beside one chunk, together and split, us:
 //                                   16-bit rows: 128 MB   256 MB    512 MB    1 GB      8-bit rows: 32 MB    64 MB     128 MB
 //   beside 512 new over 8192               139, 142  171, 160  226, 203  347, 283              142, 141  162, 149  198, 161
 //   beside 64 new over 2048                 79, 101  110, 122  158, 169  272, 246               61, 89    83, 94   123, 110
+//                                    4-bit rows: 8 MB     17 MB     34 MB     67 MB     134 MB
+//   beside 512 new over 8192               138, 144  149, 143  175, 147  220, 161  306, 179
+//   beside 64 new over 2048                 46, 70    57, 70    74, 75   121, 83   190, 107
 // The more the chunk has to do the sooner splitting pays; the limits lie between the two.  (16 sessions of 1000 to 9000
 // tokens with 3 to 7 new ones each, 4 query heads per KV head, 330 MB: 120 us split, 82 us together.)
 // Every thread of the block calls it; `sums` is shared.
@@ -85,7 +88,7 @@ __device__ __forceinline__ int few_rows_now(const ChunkArgs& a, int64_t (&sums)[
   }
   __syncthreads();
   const int64_t bytes = sums[0] * a.Hkv * a.D * 2 * (a.quant ? a.quant : 16) / 8;
-  return sums[0] == sums[1] || bytes >= (int64_t(a.quant ? 8 * a.quant : 512) << 20) ? a.few_rows : 0;
+  return sums[0] == sums[1] || bytes >= (int64_t(a.quant == 4 ? 20 : (a.quant ? 64 : 512)) << 20) ? a.few_rows : 0;
 }
 
 // CTAs that get work when a share is at least `least`.
