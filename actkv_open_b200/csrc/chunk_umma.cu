@@ -28,8 +28,8 @@
 // both D-halves, 4 KB for blocks of 16: the copy engine spends ~60 cycles per box whatever its size, and 2 KB
 // boxes, one per D-half, gave 7.1 TB/s from L2 against 10.6); warp 1 issues the MMAs (p from TMEM as
 // the A operand, V as an MN-major B operand straight from the tile); warps 4-7 and 8-11 are the
-// softmax warpgroups (a thread per row, p handed over in halves of 64 tokens).  Over the 8-bit cache the
-// TMA brings the e4m3 tiles, warp 2 their scale bytes, and warps 12-19 widen them into the ring.  Every
+// softmax warpgroups (a thread per row, p handed over in halves of 64 tokens).  Over the 8-bit and
+// 4-bit caches the TMA brings the tiles as they are, warp 2 their scale bytes, and warps 12-19 widen them into the ring.  Every
 // wait is bounded.
 //
 // What bounds it.  128 x 128 logits take the tensor core 1024 cycles (two products of head size 128) and the
@@ -48,7 +48,7 @@
 // elected lane of a converged warp, 880 to 963), p in halves, packed 32-bit math, and code that fits the
 // instruction cache (the 8-bit variant 650 to 480 us for 4 chunks of 512 over 4K to 16K tokens, and to 430 with the
 // softmax in a loop over halves of a row and a shorter widening, its cache's hit rate 0.88 to 0.96; 447 and 0.945 since
-// it looks for e4m3's NaN).
+// it looks for e4m3's NaN; the 4-bit variant, whose tiles are widened by way of 32 bits, 492).
 #include <cuda.h>
 
 #include "chunk_common.cuh"
@@ -201,9 +201,8 @@ struct Walker {
 
 // Total weight, and the session that holds this CTA's first unit of weight.
 template <int kThreads>
-__device__ void make_schedule(const ChunkArgs& a, Sched& s, int cta, int n) {
+__device__ void make_schedule(const ChunkArgs& a, Sched& s, int few_rows, int cta, int n) {
   const Geometry geo(a);
-  const int few_rows = few_rows_now<kThreads>(a, s.sums);
   if (threadIdx.x == 0) s.few_rows = few_rows;
   share_out<kThreads>(a.R, [&](int r) -> int64_t {
     const int A = new_tokens(a, r);
@@ -463,6 +462,13 @@ __global__ void __launch_bounds__(threads(BITS != 16), 1)
     if (threadIdx.x == 0) flag(a.status, ACTKV_DEV_MISALIGNED);
     return;
   }
+  const int few_rows = few_rows_now<threads(QUANT)>(a, sched.sums);
+  if (few_rows > 0 && sched.sums[0] == sched.sums[1]) {      // every session is of few rows: chunk_few_kernel's
+    if (threadIdx.x == 0) wide_parts(a.workspace, n_cta).desc[cta].valid = 0;
+    pdl_trigger();
+    pdl_wait();
+    return;
+  }
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSlots; ++i) {
       mbar_init(bar(B_KVF + i), QUANT ? 8 : 1);
@@ -497,8 +503,8 @@ __global__ void __launch_bounds__(threads(BITS != 16), 1)
   }
   pdl_trigger();
   __syncthreads();
-  make_schedule<threads(QUANT)>(a, sched, cta, n_cta);
-  if (sched.share.total == 0) {              // everything is chunk_few_kernel's
+  make_schedule<threads(QUANT)>(a, sched, few_rows, cta, n_cta);
+  if (sched.share.total == 0) {              // nothing to do
     pdl_wait();
     return;
   }
