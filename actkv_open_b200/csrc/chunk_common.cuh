@@ -1,5 +1,5 @@
 // What the two tensor-core kernels of chunk attention share (chunk_umma.cu, chunk_few.cu): the shares of
-// work, the partial results that a cut unit leaves, and 16-bit values from 8-bit rows.
+// work, the partial results that a cut unit leaves, and 16-bit values from 8- and 4-bit rows.
 #pragma once
 
 #include "common.cuh"

@@ -1,6 +1,6 @@
 // Chunk attention of sessions with few new tokens (a single token, a drafted run: at most 16 query rows,
 // token x head of the GQA group, per KV head; 8 over the 8-bit cache) over the paged cache: the formulas of
-// chunk_umma.cu.
+// chunk_umma.cu.  (Over the 4-bit cache: chunk_few4.cu.)
 //
 // Such a call reads each key and value once for a handful of products, so memory bounds it: 4 (2 over
 // the 8-bit cache) bytes per key-value pair of values against 4 operations per query row.  What matters is

@@ -21,6 +21,12 @@
 // Tokens that some of a group's rows do not see are the newest ones, 7 at most: their values are added in 32 bits one
 // token at a time, each row with an E of its own from there on, so that a hidden value of any size changes nothing in the
 // rows that do not see it.
+//
+// What bounds it: issue and latency, 573 instructions of a warp per 32 tokens and head, a quarter of them the conversions of e2m1 (one
+// per pair of values, at half rate), against 17 / 32 bytes per value.  Measured: 32 single tokens over 4096 to 32768 (32 query heads
+// over 8 of 128, 644 MB) 164 us, 3.9 TB/s, 0.60 of the measured copy rate (8-bit cache 280 us, 16-bit 384); one token over 2000 18.5,
+// over 32768 34; 16 sessions of 3 to 7 drafted tokens over 1000 to 9000 (4 query heads per KV head) 81 (the wide kernel: 131).
+// One tile of 16 tokens at a time instead of two: 193 us for the first; queries in registers spill (185).
 #include <type_traits>
 
 #include "few_common.cuh"
@@ -708,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
       const bool whole = t0 == 0 && t1 == nt;
       const int ps_slot = t0 > 0 ? 0 : 1;
       __syncthreads();                        // the rings are free, and every warp's NaN groups are known
-      if (wph > 1) {                          // the warps of a head meet through shared memory, the first goes on
+      {                                       // the warps of a head, two at least, meet through shared memory, the first goes on
         float* jo = reinterpret_cast<float*>(smem) + warp * Rg::kJoin;
         if (my_part > 0) {
 #pragma unroll

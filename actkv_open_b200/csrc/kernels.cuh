@@ -348,7 +348,7 @@ cudaError_t launch_chunk_few(const ChunkArgs& a, int dtype, int grid, cudaStream
 cudaError_t launch_chunk_few4(const ChunkArgs& a, int dtype, int grid, cudaStream_t st);
 cudaError_t launch_chunk_simt(const ChunkArgs& a, int dtype, cudaStream_t st);
 
-// ---------------------------------------------------------------- 8-bit cache rows (quant_cache.cu)
+// ---------------------------------------------------------------- 8- and 4-bit cache rows (quant_cache.cu, quant4_cache.cu)
 struct QuantMoveArgs {
   void *k, *v;               // the 16- / 32-bit rows [L][T][Hkv][D], D contiguous (read or written)
   int64_t ext_stride_l[2], ext_stride_t[2], ext_stride_h[2];     // of k and of v

@@ -551,7 +551,8 @@ ACTKV_API int actkv_quant_append(const void* k_new, const void* v_new, int dtype
  * Hkv * (D / 2 + D / 32).  Value 32 g + 4 p + j of a head (p < 8, j < 4) is in the head's byte p * D / 16 + 2 g + j / 2, the
  * low half for even j.  actkv_quantize_write4 takes per group of 32 the smallest scale, up to byte 252, with
  * max|x| <= 7 * scale (the largest value becomes at most 6 * scale), values rounded to the nearest, ties to the even
- * code; a group with a non-finite value becomes NaN (byte 255, values 0).
+ * code; a group with a non-finite value becomes NaN (byte 255, values 0).  actkv_chunk_attention_quant4 may read any slot of
+ * the cache (in place of a token that the tables do not hold it takes one that is there, and hides it).
  */
 ACTKV_API int actkv_quantize_write4(const void* k_new, const void* v_new, int dtype, int64_t k_stride_l,
                                     int64_t k_stride_t, int64_t k_stride_h, int64_t v_stride_l, int64_t v_stride_t,
