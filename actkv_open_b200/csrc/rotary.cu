@@ -250,7 +250,6 @@ __device__ __forceinline__ uint32_t max16x2(uint32_t a, uint32_t b) {
 // order as their bits do, NaN above all.  Of 16-bit values two groups at a time.
 template <typename T, int N>
 __device__ __forceinline__ void tops(const Piece<T, 4> (&raw)[N], uint32_t (&top)[N]) {
-  static_assert(sizeof(T) == 2);
 #pragma unroll
   for (int g = 0; g < N; g += 2) {
     uint32_t m[2];
@@ -277,6 +276,87 @@ __device__ __forceinline__ void tops(const float (&x)[N][4], uint32_t (&top)[N])
 #pragma unroll
     for (int o = 1; o < 8; o *= 2) top[g] = max(top[g], __shfl_xor_sync(0xffffffffu, top[g], o));
   }
+}
+
+template <int BITS>
+__device__ __forceinline__ uint32_t byte_of_top(uint32_t top) { return BITS == 4 ? scale_byte4(top) : scale_byte(top); }
+template <int BITS, int N>
+__device__ __forceinline__ uint32_t bytes_of_tops(const uint32_t (&top)[N]) {
+  uint32_t bytes = 0;
+#pragma unroll
+  for (int g = 0; g < N; ++g) bytes |= byte_of_top<BITS>(top[g]) << (8 * g);
+  return bytes;
+}
+// The scale bytes of N groups, byte g group g's, in all eight lanes (p: which of them).  Of 4 groups a lane goes on with
+// half of what it has at each exchange, so that it ends with one group's maximum and makes one byte (8 x 1088 tokens x 8 layers
+// into 4 bits and back 189 to 183 us; of 2 groups the choosing costs more than it saves, 12 prompts of head size 64 100 to 103).
+template <int BITS, int N>
+__device__ __forceinline__ uint32_t scale_bytes(const float (&x)[N][4], int p) {
+  if constexpr (N == 4) {
+    uint32_t m[N];
+#pragma unroll
+    for (int g = 0; g < N; ++g) {
+      m[g] = __float_as_uint(x[g][0]) & 0x7fffffffu;
+#pragma unroll
+      for (int k = 1; k < 4; ++k) m[g] = max(m[g], __float_as_uint(x[g][k]) & 0x7fffffffu);
+    }
+    const bool one = p & 1, two = p & 2;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {             // groups 2 g + (p & 1)
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, one ? m[2 * g] : m[2 * g + 1], 1);
+      m[g] = max(one ? m[2 * g + 1] : m[2 * g], other);
+    }
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, two ? m[0] : m[1], 2);
+    m[0] = max(two ? m[1] : m[0], other);     // group p & 3
+    m[0] = max(m[0], __shfl_xor_sync(0xffffffffu, m[0], 4));
+    uint32_t bytes = byte_of_top<BITS>(m[0]) << (8 * (p & 3));
+#pragma unroll
+    for (int o = 1; o < 4; o *= 2) bytes |= __shfl_xor_sync(0xffffffffu, bytes, o);
+    return bytes;
+  } else {
+    uint32_t top[N];
+    tops<N>(x, top);
+    return bytes_of_tops<BITS>(top);
+  }
+}
+// ... of 16-bit values as they are in memory
+template <int BITS, typename T, int N>
+__device__ __forceinline__ uint32_t scale_bytes(const Piece<T, 4> (&raw)[N], int p) {
+  static_assert(sizeof(T) == 2);
+  if constexpr (N == 4) {
+    uint32_t m[2];                            // of two groups, the first in the low half
+#pragma unroll
+    for (int g = 0; g < 4; g += 2) {
+      uint32_t w[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint2 u = reinterpret_cast<const uint2&>(raw[g + e]);
+        w[e] = max16x2(u.x & 0x7fff7fffu, u.y & 0x7fff7fffu);
+      }
+      m[g / 2] = max16x2(__byte_perm(w[0], w[1], 0x5410), __byte_perm(w[0], w[1], 0x7632));
+    }
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, p & 1 ? m[0] : m[1], 1);
+    uint32_t most = max16x2(p & 1 ? m[1] : m[0], other);    // groups 2 (p & 1) on
+    most = max16x2(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    most = max16x2(most, __shfl_xor_sync(0xffffffffu, most, 4));
+    const int high = p >> 1 & 1;              // the lane's of the two
+    const uint16_t top = uint16_t(most >> (16 * high));
+    uint32_t bytes = byte_of_top<BITS>(__float_as_uint(to_f32(reinterpret_cast<const T&>(top)))) << (8 * (2 * (p & 1) + high));
+#pragma unroll
+    for (int o = 1; o < 4; o *= 2) bytes |= __shfl_xor_sync(0xffffffffu, bytes, o);
+    return bytes;
+  } else {
+    uint32_t top[N];
+    tops<T, N>(raw, top);
+    return bytes_of_tops<BITS>(top);
+  }
+}
+// Four values times a power of two.
+__device__ __forceinline__ void scale4(float (&x)[4], float f) {
+  asm("{\n\t.reg .b64 a, b, s;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\tmov.b64 s, {%4, %4};\n\t"
+      "mul.rn.f32x2 a, a, s;\n\tmul.rn.f32x2 b, b, s;\n\tmov.b64 {%0, %1}, a;\n\tmov.b64 {%2, %3}, b;\n\t}"
+      : "+f"(x[0]), "+f"(x[1]), "+f"(x[2]), "+f"(x[3])
+      : "f"(f));
 }
 
 // How keys turn on their way into rows: not at all; in halves a whole number of groups apart (1, or 2 of 4), so that the
@@ -401,25 +481,23 @@ __device__ __forceinline__ void quantise(const RotateArgs& a, int t, int first, 
         }
       }
     }
-    uint32_t top[kAt];
+    uint32_t packed[kAt], bytes;
     if constexpr (sizeof(T) == 2) {
-      if (turns) tops<kAt>(x, top);           // (the same for the whole warp)
-      else tops<T, kAt>(raw, top);
+      if (turns) bytes = scale_bytes<BITS, kAt>(x, p);       // (the same for the whole warp)
+      else bytes = scale_bytes<BITS, T, kAt>(raw, p);
     } else {
-      tops<kAt>(x, top);
+      bytes = scale_bytes<BITS, kAt>(x, p);
     }
-    uint32_t packed[kAt], bytes = 0;
 #pragma unroll
     for (int g = 0; g < kAt; ++g) {
-      const uint32_t b = BITS == 4 ? scale_byte4(top[g]) : scale_byte(top[g]);
-      const float inv = inverse_scale(b);     // (anything for 255)
-      uint32_t u;
-      if constexpr (BITS == 4)
-        u = f32_e2m1x4(x[g][0] * inv, x[g][1] * inv, x[g][2] * inv, x[g][3] * inv);
-      else
-        u = (f32_e4m3x2(x[g][0] * inv, x[g][1] * inv) & 0xffffu) | f32_e4m3x2(x[g][2] * inv, x[g][3] * inv) << 16;
-      packed[g] = b == 255u ? 0u : u;
-      bytes |= b << (8 * g);
+      scale4(x[g], inverse_scale(bytes >> (8 * g) & 255u));  // (anything for 255)
+      if constexpr (BITS == 4) packed[g] = f32_e2m1x4(x[g][0], x[g][1], x[g][2], x[g][3]);
+      else packed[g] = (f32_e4m3x2(x[g][0], x[g][1]) & 0xffffu) | f32_e4m3x2(x[g][2], x[g][3]) << 16;
+    }
+    if (__vcmpeq4(bytes, 0xffffffffu)) {      // (of groups that are not there the byte is 0)
+#pragma unroll
+      for (int g = 0; g < kAt; ++g)
+        if ((bytes >> (8 * g) & 255u) == 255u) packed[g] = 0u;
     }
     const int h = 4 * this_hb + (lane >> 3);
     if (h >= a.Hkv) continue;
@@ -465,7 +543,7 @@ __device__ __forceinline__ void quantise(const RotateArgs& a, int t, int first, 
 // A token's work: passes of q (and where the type stays of k and v), then passes of rows to quantise, in runs of `run`
 // passes of one kind, a run per warp.
 template <typename T, int BITS, int G, Turns TURNS, int PIECE>
-__global__ void __launch_bounds__(kThreads, BITS == 0 || TURNS == kStay ? 8 : 5)
+__global__ void __launch_bounds__(kThreads, BITS == 0 || TURNS == kStay ? 8 : (G == 4 ? 4 : 5))
     rotate_write_kernel(const __grid_constant__ RotateArgs a, int run, int item_passes, int item_runs, int runs) {
   const int lane = threadIdx.x & 31;
   const int64_t warp = (int64_t(blockIdx.x) * kThreads + threadIdx.x) >> 5;
@@ -514,7 +592,20 @@ cudaError_t launch_same(const RotateArgs& a, cudaStream_t st) {
 }
 
 template <typename T, int BITS>
-cudaError_t launch_rows(const RotateArgs& a, cudaStream_t st) {
+cudaError_t launch_rows(const RotateArgs& all, cudaStream_t st) {
+  RotateArgs a = all;
+  // The rows' registers leave the queries, which only memory bounds, too few warps: large ones go first, in a launch of their
+  // own (4 x 8704 tokens of 32 heads of 128, 143 million values, and back: 276 us in one launch, 229 in two; 8 x 1088 tokens, 36
+  // million: 74 and 76; heads of 64, 71 million: 152 and 146; 18 million: 54 and 54).
+  constexpr int64_t kApart = 1 << 26;
+  if (a.rot > 0 && int64_t(a.T) * a.L * a.Hq * a.D >= kApart) {
+    RotateArgs b = a;
+    b.Hkv = b.bits = 0;
+    b.vec_out = true;                         // (nothing of it goes into the cache)
+    const cudaError_t e = launch_same<T>(b, st);
+    if (e != cudaSuccess) return e;
+    a.Hq = 0;
+  }
   if constexpr (BITS == 4)
     if (a.rot == 0) {
       if (a.D == 128) return launch<T, 4, 4, kStay, 8>(a, st);

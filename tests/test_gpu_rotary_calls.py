@@ -207,3 +207,36 @@ def test_two_attentions_over_4_bits_at_once():
         s.synchronize()
     assert all(_equal(want[i % 2], g) for i, g in enumerate(got))
     assert_device_clean(dev)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("d, dtype, pairs", [(128, BF, False), (64, HF, True)])
+def test_queries_so_large_that_they_go_apart(d, dtype, pairs, bits):
+    dev = need_gpu()
+    from actkv_open_b200.kernels.quant_cache import quant_row_bytes
+    from actkv_open_b200.kernels.rotary import rotary_table, rotate_write
+    n = (1 << 26) // (32 * d) + 77
+    gen = torch.Generator(device=dev).manual_seed(d)
+    q, k, v = (torch.randn(1, n, h, d, generator=gen, device=dev).to(dtype) for h in (32, 2, 2))
+    blocks = -(-n // 16)
+    table = torch.randperm(blocks, generator=gen, device=dev).int()[None]
+    pos = torch.randint(0, 900, (n + 3,), generator=gen, device=dev, dtype=torch.int32)[:n]
+    pos[5] = 900                                           # a position that the angles do not have
+    rest = (pos, rotary_table(d, 900), torch.tensor([0, n - 20], dtype=torch.int32, device=dev))
+    seq = torch.tensor([n - 20], dtype=torch.int32, device=dev)
+
+    def run(q, cache, bits, out=None):
+        return rotate_write(q, k, v, *rest, cache, table, seq, q_out=out, interleaved=pairs, bits=bits)
+
+    from actkv_open_b200 import _native as N
+    row = quant_row_bytes(2, d, bits)
+    rows, alone = (torch.zeros(1, 2, blocks, 16, row, dtype=torch.uint8, device=dev) for _ in range(2))
+    got, want = torch.full_like(q, 9.0), torch.full_like(q, 9.0)
+    N.read_device_status(dev)
+    run(q, rows, bits, got)
+    assert N.read_device_status(dev) == N.DEV_BAD_INDEX
+    run(None, alone, bits)
+    run(q, torch.zeros(1, 2, blocks, 16, 2, d, dtype=dtype, device=dev), None, want)
+    assert torch.equal(rows, alone) and bool(rows.any())
+    assert torch.equal(got, want) and bool((got[:, [5] + list(range(n - 20, n))] == 9.0).all())
+    N.read_device_status(dev)
