@@ -20,9 +20,10 @@
 // rate; 32 tokens of one layer 3.7 us on the device.  4 x 8704 tokens, where bytes alone would take the time in brackets, us:
 //   16-bit cache   all of 128 rotated 142 (131), half 145 (131), pairs 145 (131); 80 wide 110 (82), half of it 132 (82);
 //                  96 wide 122 (99); 64 wide 83 (66)
-//   4-bit rows, and read back   128 wide 283 (143), pairs 291 (143); 96 wide 274 (107); 64 wide 153 (71); unrotated, without
-//                  queries, 128 wide 104 (55)
-// Into rows it is issue that bounds: about 290 instructions of a warp per 512 values unrotated, rotation and the 32-bit maxima on top.
+//   4-bit rows, and read back   128 wide 229 (143), pairs 234 (143); 96 wide 215 (107); 64 wide 147 (71); unrotated, without
+//                  queries, 128 wide 100 (55)
+// Into rows it is issue that bounds: about 290 instructions of a warp per 512 values unrotated (65 % of the issue slots, 62 % of the
+// logic pipe), rotation and the 32-bit maxima on top.
 // Runs of 16 passes instead of 1: the token, its session and its angles are found once (8 x 1088 x 8 layers 998 to 285 us with
 // angles in registers).
 #include "kernels.cuh"
