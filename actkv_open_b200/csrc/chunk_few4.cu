@@ -8,12 +8,18 @@
 //                  per (token, row), which is multiplied by the token's scale as it is added: 4 multiply-adds per
 //                  512 values.
 //   O^T = V^T p^T  the 16 dims that a product gives are of one group, so p is multiplied by the token's scale of
-//                  that group, in fp16, once per group: 2 multiplications per 512 values.  So that a scale of any size
-//                  fits, it is taken relative to the largest that the warp has met in the group, 2^(b - E) <= 1; E is
-//                  raised, and O rescaled exactly, when a larger one comes, like the running maximum.
+//                  that group, in fp16, once per group: 2 multiplications per 512 values.  The scale is taken
+//                  relative to a reference of the warp and group, 2^(b - E), with b in E - 7 .. E.
 // Queries of 16-bit types go in as fp16: bf16 rows times the power of two that brings their largest value to 2^14 .. 2^15, so
-// that what is 2^-28 of it is still exact.  p is rounded to fp16's 11 bits (times 2^7 and the scale: what comes out
-// below fp16's normal range loses the digits below 2^-32 of the largest).
+// that what is 2^-28 of it is still exact.  p is rounded to fp16's 11 bits, times 2^7 and the scale.
+//
+// Scales of any size.  A value's size says nothing of its weight, and fp16 loses what is 2^-32 of the largest p.  So the
+// tokens of the products, those whose bytes are within the window of all groups' E, are a class of their own: m is the
+// maximum of THEIR logits, so one of them has p = 1 at 2^(E - 10) at least, and what another loses is below 2^-32 2^E.
+// The rest of a step's tokens are added in 32 bits one by one, p above 1 if need be.  Where a step does not fit E, E goes to
+// its largest byte, or to the largest of its lower ones if they are more, O is rescaled exactly, and, but for a rise of up
+// to 3, m goes, down or up, to the step's tokens.  (With E the largest byte met and m every token's maximum, a token of no weight
+// with values 2^25 times the others' took their share of the output away.)  Ordinary steps look at one difference of bytes for it.
 //
 // A session of more than 8 rows per KV head goes in groups of 8, each reading the cache again (most of it from L2): up to
 // 32 rows that is faster than the wide kernel.
@@ -43,6 +49,11 @@ constexpr int kMinRounds = 1;               // the least share of a CTA (one tok
 constexpr int kRowsMax = 8;                 // query rows of a group: the products' columns
 constexpr float kLowest = -3.0e38f;         // m of a row before its first token: below any logit, and finite
 constexpr float kPBits = 7.0f;              // p, and l with it, is held times 2^7 (kPScale, here by way of the exponent)
+constexpr int kWindow = 7;                  // a product's tokens have scale bytes E - kWindow .. E
+constexpr uint32_t kWindows = kWindow * 0x01010101u;
+constexpr int kRise = 3;                    // E may rise by this before m is set anew
+constexpr int kAbove = 90;                  // tokens added in 32 bits: at most this far above E,
+constexpr float kOver = 100.0f;             // ... and p times the scale over 2^E at most 2^kOver
 
 template <int D>
 struct Ring4 {
@@ -57,7 +68,7 @@ struct Ring4 {
   static constexpr int kJoin = (D / 16 * 4 + 4) * 32;       // a warp's O, m, l as floats
   static constexpr uint32_t kBytes = kWarps * kWarpBytes, kJoinBytes = kWarps * kJoin * 4;
   static constexpr uint32_t kQ = kBytes > kJoinBytes ? kBytes : kJoinBytes, kQBytes = 8 * G * 512;   // 8 heads' queries
-  static constexpr uint32_t kBack = kQ + kQBytes, kSmemBytes = kBack + 8 * 32 + 512;    // ... what undoes their power of two
+  static constexpr uint32_t kBack = kQ + kQBytes, kSmemBytes = kBack + 8 * 32 + kWarps * 4 + 512;    // ... what undoes their power of two, and a word per warp
   static_assert(kSmemBytes <= 232448, "exceeds the 227 KB of shared memory a CTA can have");
 };
 
@@ -280,14 +291,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
       const char* const head = static_cast<const char*>(a.kv) + (h * (D / 2) + lane % CH * 16);
       const int at_word = a.Hkv * (D / 2) + (D == 128 ? h * 4 : (h * 2) & ~3);
       const int sh = D == 64 && (h & 1) ? 16 : 0;             // the head's bytes within the word
-      bool gaps = false;                      // this lane met a block outside the cache: from there on every step looks
+      // What no ordinary step looks at: kGaps, this lane met a block outside the cache: from there on every step looks; kStale, m is not
+      // of the products' tokens: the next of them set it; kUneven, the rows' E differ (from there on no token is in all rows).
+      constexpr uint32_t kGaps = 1, kStale = 2, kUneven = 4;
+      uint32_t rare = 0;
       auto issue = [&](int i, int slot) {
         if (i < mine) {
           const int tok = start + i * round + lane;
           const bool none = uint32_t(phys) >= uint32_t(a.NB); // past the end, or an id outside the cache
           if (none && tok < end) {
             flag(a.status, ACTKV_DEV_BAD_INDEX);
-            gaps = true;
+            rare |= kGaps;
           }
           // The token's place, in tokens (blocks are whole and in order, and all of them fewer than 2^31, a token's bytes too).
           // One that is not there takes the cache's first: it is hidden, and nothing of a hidden token counts.
@@ -309,10 +323,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
         phys = look_up(i + 1);
       };
 
-      // the references of rows that have outgrown theirs go up to the maxima given (the same in all lanes of a row; each
-      // row by its own tokens alone, so that what others see does not show in its digits)
-      auto raise = [&](float top0, float top1) {
-        const float n0 = top0 > m0 + kSlack ? top0 : m0, n1 = top1 > m1 + kSlack ? top1 : m1;
+      // the rows' references go to those given (the same in all lanes of a row; each row by its own tokens alone, so
+      // that what others see does not show in its digits)
+      auto move = [&](float n0, float n1) {
         const float e0 = m0 == n0 ? 1.0f : ex2(m0 - n0), e1 = m1 == n1 ? 1.0f : ex2(m1 - n1);
         m0 = n0;
         m1 = n1;
@@ -327,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
         }
       };
       // ... and the scales' references
-      auto raise_scale = [&](uint32_t n0, uint32_t n1) {
+      auto move_scale = [&](uint32_t n0, uint32_t n1) {
 #pragma unroll
         for (int g = 0; g < G; ++g) {
           const float e0 = pow2(byte_of(E0, g) - byte_of(n0, g)), e1 = pow2(byte_of(E1, g) - byte_of(n1, g));
@@ -342,13 +355,57 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
         E0 = n0;
         E1 = n1;
       };
-      auto step = [&](int i, int slot, uint32_t wk, uint32_t wv, auto edge_) {
-        constexpr bool EDGE = decltype(edge_)::value;        // hidden tokens, or scale bytes out of the ordinary
+      // the value bytes of a scale word as they are held, 0 for NaN
+      auto counted = [&](uint32_t w) -> uint32_t {
+        uint32_t x = 0;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const uint32_t b = byte_of(w, g);
+          if (b < kNan4) x |= (BF16 ? b : held(b)) << (8 * g);
+        }
+        return x;
+      };
+      // The next E where a step's bytes (top: 0 for what does not count, low: 255) do not fit the present one.
+      auto fit = [&](uint32_t top, uint32_t low) -> uint32_t {
+        uint32_t next = 0;
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const uint32_t b = byte_of(top, g), now = byte_of(E0, g);
+          const bool in = byte_of(low, g) < 255;
+          const uint32_t hi = __reduce_max_sync(full, b), lo = __reduce_min_sync(full, in ? b : 255u);
+          uint32_t n = now;
+          if (lo <= hi && (hi > now || lo + kWindow < now)) {
+            n = hi;
+            if (hi - lo > kWindow) {
+              const int high = __popc(__ballot_sync(full, in && b + kWindow >= hi)), small = __popc(__ballot_sync(full, in && b <= lo + kWindow));
+              const uint32_t most = __reduce_max_sync(full, in && b <= lo + kWindow ? b : 0u);
+              if (small > high) n = max(most, hi > kAbove ? hi - kAbove : 0u);
+            }
+            if (n < now) {                    // O stays finite
+              uint32_t o_top = 0;
+#pragma unroll
+              for (int j = 2 * g; j < 2 * g + 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const uint32_t y = __float_as_uint(o[j][e]) & 0x7fffffffu;
+                  o_top = max(o_top, y < 0x7f800000u ? y : 0u);
+                }
+              const int room = max(247 - int(__reduce_max_sync(full, o_top) >> 23), 0);
+              n = uint32_t(max(int(n), int(now) - room));
+            }
+          }
+          next |= n << (8 * g);
+        }
+        return next;
+      };
+      // how far E may rise before m is set anew
+      volatile uint32_t* const E_set = reinterpret_cast<uint32_t*>(smem + Rg::kBack + 8 * 32) + warp;
+      // there: the step's tokens that are there (neither past the end nor in a block outside the cache); fast: those of them
+      // that every row sees and whose bytes vs fit E; restart: they set m
+      auto step = [&](int i, int slot, uint32_t wk, uint32_t wv, uint32_t there, uint32_t fast, uint32_t vs, bool restart, auto edge_) {
+        constexpr bool EDGE = decltype(edge_)::value;        // other tokens too, or scale bytes out of the ordinary
         const int t = start + i * round;
         const uint32_t kb = ring + slot * Rg::kStage, vb = kb + Rg::kPlane, sb = kb + 2 * Rg::kPlane;
-        // the step's tokens that are there (neither past the end nor in a block outside the cache), and those of them
-        // that every row sees
-        [[maybe_unused]] uint32_t there = full, common = full;
         [[maybe_unused]] int lim0 = 0, lim1 = 0;             // the last tokens that the lane's rows see
         [[maybe_unused]] float qs0 = 1.0f, qs1 = 1.0f;       // what undoes the queries' power of two
         if constexpr (EDGE) {
@@ -359,26 +416,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
             qs0 = back[row0];
             qs1 = back[row1];
           }
-          bool here = t + lane < end;
-          if (__any_sync(full, gaps) && here) {
-            const int lb = block_of(t + lane);
-            here = lb < a.MB && uint32_t(table[lb]) < uint32_t(a.NB);
-          }
-          there = __ballot_sync(full, here);
-          common = there & __ballot_sync(full, t + lane <= all);
         }
         // ---- the lane's token: its scales into the tables
         {
           float ks[G];
-          uint32_t vs = wv;                   // of the values, the bytes that count: 0 for what is not of all rows, and for NaN
           if constexpr (EDGE) {
-            vs = 0;
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-              uint32_t b = byte_of(wv, g);
-              if (b >= kNan4 && (there >> lane & 1u)) atomicOr(&sched.bad_v, 2);   // it comes back when the unit ends
-              if (b < kNan4 && (common >> lane & 1u)) vs |= (BF16 ? b : held(b)) << (8 * g);
-            }
+            for (int g = 0; g < G; ++g)
+              if (byte_of(wv, g) >= int(kNan4) && (there >> lane & 1u)) atomicOr(&sched.bad_v, 2);   // it comes back when the unit ends
           }
 #pragma unroll
           for (int g = 0; g < G; ++g) {
@@ -388,26 +433,21 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
             // (of a step with nothing out of the ordinary, byte 0 as 0: such keys are below 2^-124)
             ks[g] = EDGE ? (b >= kNan4 ? __int_as_float(0x7fffffff) : pow2_of(b)) : __uint_as_float(b << 23);
           }
-          if (__any_sync(full, __vcmpgtu4(vs, E0) != 0)) {    // (E0 and E1 are equal where some token is common)
-            uint32_t n = __vmaxu4(vs, E0);
-#pragma unroll
-            for (int x = 1; x < 32; x *= 2) n = __vmaxu4(n, __shfl_xor_sync(full, n, x));
-            raise_scale(n, n);
-          }
           uint8_t* const tables = smem + (table_at - smem_u32(smem));
           if constexpr (G == 4) *reinterpret_cast<float4*>(tables + lane * 16) = make_float4(ks[0], ks[1], ks[G - 2], ks[G - 1]);
           else *reinterpret_cast<float2*>(tables + lane * 8) = make_float2(ks[0], ks[1]);
+          // 2^(b - E) in fp16 (of equal E0 and E1), two groups' next to one another; 0 for other tokens' and NaN
           uint32_t f[G / 2];
-          const uint32_t down = E0 - vs;      // by byte: no byte of vs is above E0's
+          // (by byte: none of vs is above E0's or more than kWindow below, but for those that do not count)
+          const uint32_t up = 0x0f0f0f0fu - (EDGE ? (E0 - vs) & kWindows : E0 - vs);
 #pragma unroll
           for (int g = 0; g < G; g += 2) {
-            float x[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              x[e] = __uint_as_float(uint32_t(max(127 - byte_of(down, g + e), 0)) << 23);
-              if (EDGE && ((common >> lane & 1u) == 0 || byte_of(wv, g + e) >= int(kNan4))) x[e] = 0.0f;
+            f[g / 2] = (up >> (8 * g) & 0xffu) << 10 | (up >> (8 * g) & 0xff00u) << 18;
+            if constexpr (EDGE) {
+              const bool in = fast >> lane & 1u;
+              if (!in || byte_of(wv, g) >= int(kNan4)) f[g / 2] &= 0xffff0000u;
+              if (!in || byte_of(wv, g + 1) >= int(kNan4)) f[g / 2] &= 0x0000ffffu;
             }
-            f[g / 2] = pack2<false>(x[0], x[1]);
           }
           // by pair of tokens and group, the pair's factors: each of the two lanes puts half of the groups
           if constexpr (G == 4) {
@@ -505,19 +545,94 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
         for (int n = 0; n < kTiles; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[n][e] = __fmul_rn(s[n][e], e & 1 ? f1 : f0);
-        float top0 = fmaxf(s[0][0], s[0][2]), top1 = fmaxf(s[0][1], s[0][3]);
+        // the largest of the products' tokens
+        auto of_products = [&](int n, int e) { return !EDGE || (fast >> row_tok >> (16 * n + 8 * (e >> 1)) & 1u) ? s[n][e] : ninf; };
+        float top0 = fmaxf(of_products(0, 0), of_products(0, 2)), top1 = fmaxf(of_products(0, 1), of_products(0, 3));
 #pragma unroll
         for (int n = 1; n < kTiles; ++n) {
-          top0 = fmaxf(top0, fmaxf(s[n][0], s[n][2]));
-          top1 = fmaxf(top1, fmaxf(s[n][1], s[n][3]));
+          top0 = fmaxf(top0, fmaxf(of_products(n, 0), of_products(n, 2)));
+          top1 = fmaxf(top1, fmaxf(of_products(n, 1), of_products(n, 3)));
         }
-        if (__any_sync(full, top0 > m0 + kSlack || top1 > m1 + kSlack)) {
+        bool moves = top0 > m0 + kSlack || top1 > m1 + kSlack;
+        // ... and of the others: logits with the scales, which p times the scale must not outgrow; those that some row does not see
+        [[maybe_unused]] float far0 = ninf, far1 = ninf, last0 = ninf, last1 = ninf;
+        if constexpr (EDGE) {
+          const uint32_t others = there & ~fast;
+          if (others) {
+            // (in ordinary steps none is near: the largest logit, the largest scale above E)
+            auto above = [&](uint32_t bytes, uint32_t E) {
+              const uint32_t y = __vsubus4(bytes, E);
+              return min(max(max(byte_of(y, 0), byte_of(y, 1)), max(byte_of(y, 2), byte_of(y, 3))), kAbove);
+            };
+            const uint32_t bytes = counted(wv);
+            const float most = float(__reduce_max_sync(full, others >> lane & 1u ? above(bytes, E0) : 0)) - kOver;
+            float all0 = fmaxf(s[0][0], s[0][2]), all1 = fmaxf(s[0][1], s[0][3]);
+#pragma unroll
+            for (int n = 1; n < kTiles; ++n) {
+              all0 = fmaxf(all0, fmaxf(s[n][0], s[n][2]));
+              all1 = fmaxf(all1, fmaxf(s[n][1], s[n][3]));
+            }
+            if (__any_sync(full, (rare & kUneven) || moves || restart || all0 + most > m0 || all1 + most > m1)) {
+#pragma unroll
+              for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const int tk = 16 * n + 8 * (e >> 1) + row_tok;
+                  const int lift = above(__shfl_sync(full, bytes, tk), e & 1 ? E1 : E0);
+                  if (fast >> tk & 1u) continue;
+                  (e & 1 ? far1 : far0) = fmaxf(e & 1 ? far1 : far0, s[n][e] + float(lift));
+                  if (t + tk > all) (e & 1 ? last1 : last0) = fmaxf(e & 1 ? last1 : last0, s[n][e]);
+                }
+              moves = true;
+            }
+          }
+          moves |= restart;
+        }
+        if (__any_sync(full, moves)) {
 #pragma unroll
           for (int x = 4; x < 32; x *= 2) {
             top0 = fmaxf(top0, __shfl_xor_sync(full, top0, x));
             top1 = fmaxf(top1, __shfl_xor_sync(full, top1, x));
           }
-          raise(top0, top1);
+          if constexpr (EDGE) {
+#pragma unroll
+            for (int x = 4; x < 32; x *= 2) {
+              far0 = fmaxf(far0, __shfl_xor_sync(full, far0, x));
+              far1 = fmaxf(far1, __shfl_xor_sync(full, far1, x));
+              last0 = fmaxf(last0, __shfl_xor_sync(full, last0, x));
+              last1 = fmaxf(last1, __shfl_xor_sync(full, last1, x));
+            }
+            float room0 = 0.0f, room1 = 0.0f;                // what m may go down by: as long as O and l stay finite
+            if (restart) {
+              uint32_t y0 = __float_as_uint(l0), y1 = __float_as_uint(l1);
+              y0 = y0 < 0x7f800000u ? y0 : 0u;
+              y1 = y1 < 0x7f800000u ? y1 : 0u;
+#pragma unroll
+              for (int j = 0; j < kOut; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const uint32_t y = __float_as_uint(o[j][e]) & 0x7fffffffu;
+                  (e & 1 ? y1 : y0) = max(e & 1 ? y1 : y0, y < 0x7f800000u ? y : 0u);
+                }
+#pragma unroll
+              for (int x = 4; x < 32; x *= 2) {
+                y0 = max(y0, __shfl_xor_sync(full, y0, x));
+                y1 = max(y1, __shfl_xor_sync(full, y1, x));
+              }
+              room0 = float(min(max(237 - int(y0 >> 23), 0), 120));
+              room1 = float(min(max(237 - int(y1 >> 23), 0), 120));
+            }
+            auto next = [&](float m, float top, float far, float last, float room) {
+              float n = m;
+              if (top > m + kSlack || (restart && top > kLowest)) n = fmaxf(top, m - room);
+              // nothing before: p of at most 1, where that costs the products' tokens little
+              if (m == kLowest) n = fmaxf(n, n == kLowest ? last : fminf(last, n + 4.0f));
+              return fmaxf(n, far - kOver);
+            };
+            move(next(m0, top0, far0, last0, room0), next(m1, top1, far1, last1, room1));
+          } else {
+            move(top0 > m0 + kSlack ? top0 : m0, top1 > m1 + kSlack ? top1 : m1);
+          }
         }
         const float base0 = m0 - kPBits, base1 = m1 - kPBits;
 #pragma unroll
@@ -530,10 +645,16 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
           l1 += s[n][1] + s[n][3];
         }
         // ---- O^T += V^T p^T: the lane's tokens are those of rows 2 c4, 2 c4 + 1 and 8 on, its dims 4 r8 .. + 3 of each group
-        if (!EDGE || common) {
+        if (!EDGE || fast) {
 #pragma unroll
           for (int n = 0; n < kTiles; ++n) {
-            const uint32_t p0 = transpose8x8(pack2<false>(s[n][0], s[n][1])), p1 = transpose8x8(pack2<false>(s[n][2], s[n][3]));
+            uint32_t p0 = pack2<false>(s[n][0], s[n][1]), p1 = pack2<false>(s[n][2], s[n][3]);
+            if constexpr (EDGE) {             // (the others' may be infinite in fp16)
+              if (!(fast >> row_tok >> (16 * n) & 1u)) p0 = 0;
+              if (!(fast >> row_tok >> (16 * n + 8) & 1u)) p1 = 0;
+            }
+            p0 = transpose8x8(p0);
+            p1 = transpose8x8(p1);
             uint32_t vw[4][G / 2], ft[2][G];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -596,10 +717,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
             }
           }
         }
-        // ---- tokens that some row does not see, one by one
+        // ---- the other tokens, one by one: first those outside the window, then those that some row does not see
         if constexpr (EDGE) {
 #pragma unroll 1
-          for (uint32_t some = there & ~common; some; some &= some - 1) {
+          for (uint32_t some = there & ~fast; some; some &= some - 1) {
             const int tk = __ffs(some) - 1, of = tk & 7;
             // p of the lane's two rows: from the lanes of the product's row that the token is
             float x0 = 0.0f, x1 = 0.0f;
@@ -615,13 +736,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
             x1 = __shfl_sync(full, x1, token_of(of) * 4 + c4);
             const bool see0 = t + tk <= lim0, see1 = t + tk <= lim1;
             const uint32_t word = lds4(sb + (kStep + tk) * 4) >> sh;
-            uint32_t seen = 0;                // its scale bytes, NaN without
-#pragma unroll
-            for (int g = 0; g < G; ++g) {
-              const uint32_t b = byte_of(word, g);
-              if (b < kNan4) seen |= (BF16 ? b : held(b)) << (8 * g);
+            const uint32_t seen = counted(word), least = __vsubus4(seen, kAbove * 0x01010101u);
+            const uint32_t n0 = see0 ? __vmaxu4(E0, least) : E0, n1 = see1 ? __vmaxu4(E1, least) : E1;
+            if (__any_sync(full, n0 != E0 || n1 != E1)) {
+              move_scale(n0, n1);
+              rare |= kUneven;
             }
-            raise_scale(see0 ? __vmaxu4(E0, seen) : E0, see1 ? __vmaxu4(E1, seen) : E1);
 #pragma unroll
             for (int g = 0; g < G; ++g) {
               const uint32_t b = byte_of(word, g);
@@ -643,6 +763,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
               }
             }
           }
+          rare = fast == 0 ? rare | kStale : rare & ~kStale;
         }
       };
 
@@ -663,12 +784,50 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
           wk &= 0xffffu;
           wv &= 0xffffu;
         }
-        bool odd;
-        if constexpr (BF16) odd = ((wk & (wk << 1)) | (wv & (wv << 1))) & 0x80808080u;
-        else odd = __vcmpgtu4(wk, 0x8c8c8c8cu) | __vcmpgtu4(wv, 0x8c8c8c8cu) |
-                   ((__vcmpgtu4(0x68686868u, wk) | __vcmpgtu4(0x68686868u, wv)) & (D == 64 ? 0xffffu : 0xffffffffu));
-        if (t + kStep - 1 > all || t + kStep > end || __any_sync(full, odd || gaps)) step(i, slot, wk, wv, std::true_type());
-        else step(i, slot, wk, wv, std::false_type());
+        // bits of what is out of the ordinary: scale bytes, values' outside the window, and what the steps so far left behind
+        uint32_t odd = rare;
+        if constexpr (BF16) odd |= ((wk & (wk << 1)) | (wv & (wv << 1))) & 0x80808080u;
+        else odd |= __vcmpgtu4(wk, 0x8c8c8c8cu) | __vcmpgtu4(wv, 0x8c8c8c8cu) |
+                    ((__vcmpgtu4(0x68686868u, wk) | __vcmpgtu4(0x68686868u, wv)) & (D == 64 ? 0xffffu : 0xffffffffu));
+        const uint32_t off = (E0 - wv) & ~kWindows;
+        const bool ends = t + kStep - 1 > all || t + kStep > end;
+        uint32_t there = 0, fast = 0, vs = 0;
+        bool edge = false, restart = false;
+        if (ends || __any_sync(full, (odd | off) != 0)) {
+          edge = ends || __any_sync(full, odd != 0);
+          restart = rare & kStale;
+          bool here = t + lane < end;
+          if (__any_sync(full, rare & kGaps) && here) {
+            const int lb = block_of(t + lane);
+            here = lb < a.MB && uint32_t(table[lb]) < uint32_t(a.NB);
+          }
+          there = __ballot_sync(full, here);
+          fast = there & __ballot_sync(full, t + lane <= all);
+          // the lane's bytes that count, and with 255 in place of the others
+          vs = fast >> lane & 1u ? counted(wv) : 0u;
+          uint32_t low = vs;
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            if (!(fast >> lane & 1u) || g >= G || byte_of(wv, g) >= int(kNan4)) low |= 255u << (8 * g);
+          auto outside = [&] { return (__vcmpgtu4(vs, E0) | __vcmpgtu4(__vsubus4(E0, kWindows), low)) != 0; };
+          if (__any_sync(full, outside())) {
+            uint32_t n = __vmaxu4(vs, E0);    // the larger E, where that will do
+#pragma unroll
+            for (int x = 1; x < 32; x *= 2) n = __vmaxu4(n, __shfl_xor_sync(full, n, x));
+            if (__any_sync(full, __vcmpgtu4(__vsubus4(n, kWindows), low) != 0)) n = fit(vs, low);
+            const bool begun = __any_sync(full, m0 > kLowest || m1 > kLowest);
+            restart |= begun && (__vcmpgtu4(E0, n) | __vcmpgtu4(n, *E_set)) != 0;
+            __syncwarp();
+            if (restart || !begun) *E_set = n + kRise * 0x01010101u;
+            if (n != E0) move_scale(n, n);
+            const bool out = outside();
+            fast &= ~__ballot_sync(full, out);
+            if (out) vs = 0;
+            edge |= restart || __any_sync(full, out);
+          }
+        }
+        if (edge) step(i, slot, wk, wv, there, fast, vs, restart, std::true_type());
+        else step(i, slot, wk, wv, full, full, wv, false, std::false_type());
         __syncwarp();                         // every lane has read the slot that the next copies fill, and the tables
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -698,16 +857,28 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
       l0 *= 1.0f / kPScale<false>;
       l1 *= 1.0f / kPScale<false>;
       {
-        constexpr float kBack = BF16 ? 1.0f / kPScale<false> : 1.0f;
+        // A row whose m is far from the maximum of its logits goes on with m + k and 2^-k of O and l, so that l is of the order of 1:
+        // what the warps and CTAs have is added up in 32 bits.
+        auto shift_of = [](float l) -> int {
+          const int e = int(__float_as_uint(l) >> 23) - 127;
+          return e > -127 && e < 128 && (e < -8 || e > 40) ? e : 0;
+        };
+        const int k0 = shift_of(l0), k1 = shift_of(l1);
+        l0 = l0 * pow2(-k0 / 2) * pow2(-k0 - -k0 / 2);
+        l1 = l1 * pow2(-k1 / 2) * pow2(-k1 - -k1 / 2);
+        m0 += float(k0);
+        m1 += float(k1);
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          const float y0 = pow2_of(byte_of(E0, g)), y1 = pow2_of(byte_of(E1, g));
+          constexpr int kBack = BF16 ? int(kPBits) : 0;
+          const int e0 = byte_of(E0, g) - 127 - kBack - k0, e1 = byte_of(E1, g) - 127 - kBack - k1;
+          const float y0 = pow2(e0 / 2), z0 = pow2(e0 - e0 / 2), y1 = pow2(e1 / 2), z1 = pow2(e1 - e1 / 2);
 #pragma unroll
           for (int j = 2 * g; j < 2 * g + 2; ++j) {
-            o[j][0] = o[j][0] * kBack * y0;
-            o[j][1] = o[j][1] * kBack * y1;
-            o[j][2] = o[j][2] * kBack * y0;
-            o[j][3] = o[j][3] * kBack * y1;
+            o[j][0] = o[j][0] * y0 * z0;
+            o[j][1] = o[j][1] * y1 * z1;
+            o[j][2] = o[j][2] * y0 * z0;
+            o[j][3] = o[j][3] * y1 * z1;
           }
         }
       }

@@ -1,0 +1,144 @@
+"""Attention over the 4-bit cache where scales are far apart: values whose size has nothing to do with their weight.
+
+The bounds are those of test_gpu_chunk.py, with what the kernel for few rows adds.  It holds p times 2^7 in fp16, times 2^(b - E)
+for a token's scale byte b in E - 7 .. E, where fp16 numbers below 2^-14 err by 2^-25 at most; m is the maximum of the logits of the
+tokens that are added that way, and all others are added in 32 bits.  E rises by up to 3 before m is set anew.  A token so errs by
+6 2^-25 2^-7 2^(E - 127) at most, and the token with p = 1 has a value of 4 2^(E - 10 - 127) at least among the 32 of its
+group: S tokens err by S 2^-21 times what that one gives.  |out - ref| <= (2 u + 1e-4) A + S 2^-21 max of A over the group, A = sum p |v| / l; fp16: + 2^-25 for the result.  And a p of
+less than 2^-126 of the largest is below what 32 bits hold as normal numbers: it may be anything down to 0, + sum of those p |v| / l."""
+import math
+
+import pytest
+import torch
+
+import chunk_cases as C
+from gpu_util import assert_device_clean, need_gpu
+from test_gpu_chunk import BF, HF, U
+from test_gpu_chunk4 import Case4
+
+pytestmark = pytest.mark.gpu
+
+NEW = [1, 3, 9, 90]
+
+
+def _session(lens, new, d, dtype, low, seed, hkv=2, hq=4):
+    """A session whose logits (with scale 1) are 4 times dim 0 of its keys, exactly: up to 2.5 apart, those of the tokens
+    in ``low`` that much lower."""
+    case = Case4.__new__(Case4)
+    gen = torch.Generator().manual_seed(seed)
+    from actkv_open_b200.kernels.quant_cache import quant_row_bytes
+    case.lens, case.new, case.hq, case.hkv, case.d, case.bs, case.dtype, case.quant = [lens], [new], hq, hkv, d, 16, dtype, True
+    case.table, case.nb = C.pages([lens], 16, gen)
+    case.off, case.row = C.offsets([new]), quant_row_bytes(hkv, d, 4)
+    case.cache = torch.full((2, case.nb * 16, case.row), 255, dtype=torch.uint8)
+    case.q = torch.zeros(new, hq, d, dtype=dtype)
+    case.q[..., 0] = 4
+    k = torch.randn(lens, hkv, d, generator=gen)
+    k[..., 0] = torch.rand(lens, hkv, generator=gen) * 0.625
+    for t, drop in low.items():
+        k[t] = 0                             # (the other dims of its group would not fit beside it)
+        k[t, :, 0] = -drop / 4
+    case.put(0, 0, k.to(dtype))
+    case.v = [torch.randn(lens, hkv, d, generator=gen)]
+    return case
+
+
+def _reference(case, dev, scale=1.0):
+    s, a, g = case.lens[0], case.new[0], case.hq // case.hkv
+    k, v = (case.tokens(p, 0).double().to(dev).repeat_interleave(g, 1) for p in range(2))
+    q = case.q.double().to(dev)
+    x = torch.einsum("ahd,shd->ahs", q, k) * scale
+    x = x.masked_fill((torch.arange(s, device=dev) > torch.arange(s - a, s, device=dev)[:, None])[:, None], -math.inf)
+    lse = torch.logsumexp(x, -1)
+    p = torch.exp(x - lse[..., None])
+    size = torch.einsum("ahd,shd->ahs", q.abs(), k.abs()).amax(-1) * scale
+    tiny = torch.where(p < 2.0 ** -126 * p.amax(-1, keepdim=True), p, torch.zeros_like(p))
+    mag, lost = (torch.einsum("ahs,shd->ahd", y, v.abs()) for y in (p, tiny))
+    return torch.einsum("ahs,shd->ahd", p, v), lse, mag, size, lost
+
+
+def _check(case, dev, got, scale=1.0):
+    want, want_l, mag, size, lost = _reference(case, dev, scale)
+    out, lse = (x.double() for x in got)
+    group = mag.unflatten(-1, (-1, 32)).amax(-1, keepdim=True).expand(-1, -1, -1, 32).flatten(-2)
+    tol = (2 * U[case.dtype] + 1e-4) * mag + case.lens[0] * 2.0 ** -21 * group + lost + (2.0 ** -25 if case.dtype == HF else 0.0)
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+    off = (out - want).abs() - tol
+    worst = int(off.argmax())
+    assert (off <= 0).all(), f"{int((off > 0).sum())} of {off.numel()} outputs off, one {out.flatten()[worst]:.5g} for " \
+        f"{want.flatten()[worst]:.5g}, sum p |v| {mag.flatten()[worst]:.5g}"
+    assert ((lse - want_l).abs() <= 2e-5 + 8e-6 * size).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new", NEW)
+def test_a_large_value_of_no_weight_leaves_the_others_their_share(new, d, dtype):
+    """One token, 60 below all others in its logit, with values 2^spread times theirs: early in the session, in its middle,
+    at its end, and among the new tokens.  Its share is e^-60 2^spread at most."""
+    dev = need_gpu()
+    lens = 1000
+    base = 1.0 if dtype == BF else 2.0 ** -10                # (fp16 reads end at 65504)
+    for spread in (6, 10, 16, 20, 24, 26, 30, 50) if dtype == BF else (6, 10, 13, 22):
+        for at in ([0], [500], [lens - new], [lens - 1], [0, 33, 34, 700, 998]):
+            case = _session(lens, new, d, dtype, {t: 60 for t in at}, 60 + spread)
+            size = torch.full((lens, 1, 1), base)
+            size[at] *= 2.0 ** spread
+            case.put(1, 0, (case.v[0] * size).to(dtype))
+            if spread % 4 == 2:              # ... of one head and group only
+                for t in at:
+                    row = case.cache[1, int(C.slots(case.table, 0, t, t + 1, 16))]
+                    keep = int(row[case.scale_at(1, 1)])
+                    row[case.scale_at(0, 0):case.scale_at(2, 0)] -= spread
+                    row[case.scale_at(1, 1)] = keep
+            _check(case, dev, case.run(dev, scale=1.0))
+    assert_device_clean(dev)
+
+
+@pytest.mark.parametrize("new", NEW)
+def test_values_large_in_proportion_to_their_little_weight(new):
+    """Values 2^n times as large on tokens whose weight is about 2^-n: each has its share of the output."""
+    dev = need_gpu()
+    lens = 700
+    for seed, steps in enumerate(([0, 9, 18, 27], list(range(0, 64, 3)), [0] * 60 + [40], [0, 12, 0, 0, 0], [80, 0],
+                                  [0] * 100 + [20] * 150)):
+        shift = [steps[t % len(steps)] for t in range(lens)]
+        case = _session(lens, new, 128, BF, {t: n * math.log(2) for t, n in enumerate(shift) if n}, 70 + seed)
+        case.put(1, 0, (case.v[0] * torch.tensor([2.0 ** n for n in shift])[:, None, None]).to(BF))
+        _check(case, dev, case.run(dev, scale=1.0))
+    assert_device_clean(dev)
+
+
+@pytest.mark.parametrize("new", NEW)
+def test_runs_of_tokens_of_unlike_scales(new):
+    """Equal weights but for the largest values': stretches, single tokens and zeros between them, up to the ends of the range."""
+    dev = need_gpu()
+    lens = 900
+    gen = torch.Generator().manual_seed(3)
+    up = lambda *runs: [x for n, k in runs for x in [k] * n]                                             # noqa: E731
+    for seed, (shift, heavy) in enumerate((
+            (up((300, 0), (200, -40), (400, 0)), 1000), (up((64, 100), (836, 0)), 50), (up((1, 110), (899, -60)), 0),
+            (up((450, -100), (2, 100), (448, -100)), 0), ([0 if t % 2 else None for t in range(lens)], 1000),
+            (torch.randint(-8, 9, (lens,), generator=gen).tolist(), 1000),
+            (torch.randint(-30, 60, (lens,), generator=gen).tolist(), 5), ([None] * 100 + [-20] * 800, 1000))):
+        low = {t: 120 for t, n in enumerate(shift) if n is not None and n > heavy}
+        case = _session(lens, new, 128, BF, low, 80 + seed)
+        size = torch.tensor([0.0 if n is None else 2.0 ** n for n in shift])
+        case.put(1, 0, (case.v[0] * size[:, None, None]).to(BF))
+        _check(case, dev, case.run(dev, scale=1.0))
+    assert_device_clean(dev)
+
+
+@pytest.mark.parametrize("new", NEW)
+def test_a_dominant_token_of_small_values(new):
+    """A token with nearly all the weight and values 2^-n of the others', or none: theirs count by what is left to them."""
+    dev = need_gpu()
+    lens = 600
+    for seed, (n, at) in enumerate(((30, [0]), (30, [300]), (None, [5]), (None, [597 - new]), (60, [0, 1, 2]))):
+        drop = 25 if n is None else n * math.log(2)
+        case = _session(lens, new, 128, BF, {t: drop for t in range(lens) if t not in at}, 90 + seed)
+        size = torch.ones(lens, 1, 1)
+        size[at] = 0.0 if n is None else 2.0 ** -n
+        case.put(1, 0, (case.v[0] * size).to(BF))
+        _check(case, dev, case.run(dev, scale=1.0))
+    assert_device_clean(dev)
