@@ -80,7 +80,7 @@ template <int D>
 __device__ __forceinline__ int piece(int r, int c) { return D == 128 ? c ^ ((r >> 2 & 1) << 1) : c; }
 
 // 2^(b - 127), and 2^d (0 from -127 down).
-__device__ __forceinline__ float pow2_of(uint32_t b) { return __uint_as_float(b == 0u ? 0x00400000u : b << 23); }
+__device__ __forceinline__ float pow2_of(uint32_t b) { return __uint_as_float(max(b << 23, 0x00400000u)); }
 __device__ __forceinline__ float pow2(int d) { return __uint_as_float(uint32_t(min(max(127 + d, 0), 254)) << 23); }
 
 // fp16 reads: what the value pair h of scale byte b stands for as fp16 has it (subnormals rounded, past the range the
@@ -430,8 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
             uint32_t b = byte_of(wk, g);
             if constexpr (EDGE && !BF16)
               if (b < kNan4) b = held(b);
-            // (of a step with nothing out of the ordinary, byte 0 as 0: such keys are below 2^-124)
-            ks[g] = EDGE ? (b >= kNan4 ? __int_as_float(0x7fffffff) : pow2_of(b)) : __uint_as_float(b << 23);
+            ks[g] = EDGE && b >= kNan4 ? __int_as_float(0x7fffffff) : pow2_of(b);
           }
           uint8_t* const tables = smem + (table_at - smem_u32(smem));
           if constexpr (G == 4) *reinterpret_cast<float4*>(tables + lane * 16) = make_float4(ks[0], ks[1], ks[G - 2], ks[G - 1]);

@@ -142,3 +142,26 @@ def test_a_dominant_token_of_small_values(new):
         case.put(1, 0, (case.v[0] * size).to(BF))
         _check(case, dev, case.run(dev, scale=1.0))
     assert_device_clean(dev)
+
+
+def _keys(case, codes, scales):
+    """The session's keys from their bytes: codes [S, Hkv * D / 2], scales [S, Hkv * D / 32]."""
+    at, n = C.slots(case.table, 0, 0, case.lens[0], 16), case.hkv * case.d // 2
+    case.cache[0, at, :n] = codes.to(torch.uint8)
+    case.cache[0, at, n:n + case.hkv * case.d // 32] = scales.to(torch.uint8)
+
+
+@pytest.mark.parametrize("path", ["auto", "simt"])
+@pytest.mark.parametrize("new", NEW)
+def test_the_smallest_keys_count_beside_the_largest_queries(new, path):
+    """Keys of scale bytes 0 and 1 (up to 6 2^-126) and queries of 2^123: logits of the order of 1, wherever the token stands."""
+    dev = need_gpu()
+    lens = 300
+    for d in (64, 128):
+        case = _session(lens, new, d, BF, {}, 50)
+        case.put(1, 0, case.v[0].to(BF))
+        gen = torch.Generator().manual_seed(51)
+        _keys(case, torch.randint(0, 256, (lens, d), generator=gen), torch.randint(0, 2, (lens, d // 16), generator=gen))
+        case.q = ((torch.randint(0, 2, (new, 4, d), generator=gen) * 2 - 1) * 2.0 ** 123).to(BF)
+        _check(case, dev, case.run(dev, scale=1.0, path=path))
+    assert_device_clean(dev)
