@@ -520,11 +520,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
                 if (pc == 0) mma16816_new(c, m, qg.x, qg.y);
                 else mma16816<false>(c, m, qg.z, qg.w);
               }
-              // (powers of two: the same digits with the queries' or without, but so a scale of any size stays in range)
+              // (powers of two, the same digits with the queries' or without; the smaller one first, so that scales of any size
+              // stay in range, beside sums of 0 too)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const float k = __uint_as_float(gg ? ks[e >> 1].y : ks[e >> 1].x);
-                s[n][e] = fmaf(c[e], EDGE ? k * (e & 1 ? qs1 : qs0) : k, s[n][e]);
+                const float k = __uint_as_float(gg ? ks[e >> 1].y : ks[e >> 1].x), qs = e & 1 ? qs1 : qs0;
+                if constexpr (EDGE) s[n][e] = k < qs ? fmaf(c[e] * k, qs, s[n][e]) : fmaf(c[e] * qs, k, s[n][e]);
+                else s[n][e] = fmaf(c[e], k, s[n][e]);
               }
             }
           }

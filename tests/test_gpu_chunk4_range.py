@@ -165,3 +165,24 @@ def test_the_smallest_keys_count_beside_the_largest_queries(new, path):
         case.q = ((torch.randint(0, 2, (new, 4, d), generator=gen) * 2 - 1) * 2.0 ** 123).to(BF)
         _check(case, dev, case.run(dev, scale=1.0, path=path))
     assert_device_clean(dev)
+
+
+@pytest.mark.parametrize("path", ["auto", "simt"])
+@pytest.mark.parametrize("new", NEW)
+def test_large_keys_beside_queries_of_zero(new, path):
+    """Dims where the queries are 0 and some keys up to 6 2^123, beside dims of queries of 2^100 and keys of 2^-100: those
+    alone make the logits."""
+    dev = need_gpu()
+    lens = 300
+    for d in (64, 128):
+        case = _session(lens, new, d, BF, {}, 52)
+        case.put(1, 0, case.v[0].to(BF))
+        gen = torch.Generator().manual_seed(53)
+        scales = torch.full((lens, 2, d // 32), 27)
+        scales[::7, :, 1] = 250
+        _keys(case, torch.randint(0, 256, (lens, d), generator=gen), scales.flatten(1))
+        q = torch.randn(new, 4, d, generator=gen) * 2.0 ** 98
+        q[..., 32:64] = 0
+        case.q = q.to(BF)
+        _check(case, dev, case.run(dev, scale=0.25, path=path), 0.25)
+    assert_device_clean(dev)
