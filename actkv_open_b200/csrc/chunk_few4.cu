@@ -11,7 +11,8 @@
 //                  that group, in fp16, once per group: 2 multiplications per 512 values.  The scale is taken
 //                  relative to a reference of the warp and group, 2^(b - E), with b in E - 7 .. E.
 // Queries of 16-bit types go in as fp16: bf16 rows times the power of two that brings their largest value to 2^14 .. 2^15, so
-// that what is 2^-28 of it is still exact.  p is rounded to fp16's 11 bits, times 2^7 and the scale.
+// that what is 2^-28 of it is still exact; rows with a group whose largest value is 2^-12 of that (its keys may be as much larger)
+// have a power of two per group, which the steps of the uncommon kind undo.  p is rounded to fp16's 11 bits, times 2^7 and the scale.
 //
 // Scales of any size.  A value's size says nothing of its weight, and fp16 loses what is 2^-32 of the largest p.  So the
 // tokens of the products, those whose bytes are within the window of all groups' E, are a class of their own: m is the
@@ -49,6 +50,7 @@ constexpr int kMinRounds = 1;               // the least share of a CTA (one tok
 constexpr int kRowsMax = 8;                 // query rows of a group: the products' columns
 constexpr float kLowest = -3.0e38f;         // m of a row before its first token: below any logit, and finite
 constexpr float kPBits = 7.0f;              // p, and l with it, is held times 2^7 (kPScale, here by way of the exponent)
+constexpr int kQuerySpread = 12;            // groups of a query row whose largest values differ by more in their exponents are scaled apart
 constexpr int kWindow = 7;                  // a product's tokens have scale bytes E - kWindow .. E
 constexpr uint32_t kWindows = kWindow * 0x01010101u;
 constexpr int kRise = 3;                    // E may rise by this before m is set anew
@@ -68,7 +70,8 @@ struct Ring4 {
   static constexpr int kJoin = (D / 16 * 4 + 4) * 32;       // a warp's O, m, l as floats
   static constexpr uint32_t kBytes = kWarps * kWarpBytes, kJoinBytes = kWarps * kJoin * 4;
   static constexpr uint32_t kQ = kBytes > kJoinBytes ? kBytes : kJoinBytes, kQBytes = 8 * G * 512;   // 8 heads' queries
-  static constexpr uint32_t kBack = kQ + kQBytes, kSmemBytes = kBack + 8 * 32 + kWarps * 4 + 512;    // ... what undoes their power of two, and a word per warp
+  static constexpr uint32_t kBack = kQ + kQBytes, kWords = kBack + 8 * 8 * G * 4;     // ... what undoes their powers of two, a word per warp
+  static constexpr uint32_t kSmemBytes = kWords + kWarps * 4 + 512;
   static_assert(kSmemBytes <= 232448, "exceeds the 227 KB of shared memory a CTA can have");
 };
 
@@ -232,27 +235,43 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
       }
       // scale * log2 e, and what undoes the queries' power of two, for rows row0 and row1
       float cq0 = c2, cq1 = c2;
+      uint32_t rare = 0;                      // what no ordinary step looks at:
+      constexpr uint32_t kGaps = 1;           // this lane met a block outside the cache: from there on every step looks
+      constexpr uint32_t kStale = 2;          // m is not of the products' tokens: the next of them set it
+      constexpr uint32_t kUneven = 4;         // the rows' E differ (from there on no token is in all rows)
+      constexpr uint32_t kSpread = 8;         // the queries' groups have powers of two of their own
       if constexpr (BF16) {
-        uint32_t top = 0;                     // the row's largest finite value, by its bits
+        uint32_t tops[G], top = 0, least = 0x7f80u;           // the groups' largest finite values, by their bits
 #pragma unroll
-        for (int k = 0; k < 2 * G; ++k)
+        for (int g = 0; g < G; ++g) {
+          tops[g] = 0;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t x = q[k][e] & 0x7fffu, y = q[k][e] >> 16 & 0x7fffu;
-            top = max(top, max(x < 0x7f80u ? x : 0u, y < 0x7f80u ? y : 0u));
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t u = q[2 * g + (e >> 1)][e & 1], x = u & 0x7fffu, y = u >> 16 & 0x7fffu;
+            tops[g] = max(tops[g], max(x < 0x7f80u ? x : 0u, y < 0x7f80u ? y : 0u));
           }
-        top = max(top, __shfl_xor_sync(full, top, 1));
-        top = max(top, __shfl_xor_sync(full, top, 2));
-        const int by = min(141 - int(top >> 7), 126);
-        const float f = pow2(by), back = pow2(-by);
+          tops[g] = max(tops[g], __shfl_xor_sync(full, tops[g], 1));
+          tops[g] = max(tops[g], __shfl_xor_sync(full, tops[g], 2));
+          top = max(top, tops[g]);
+          if (tops[g] > 0) least = min(least, tops[g]);
+        }
+        const bool spread = __any_sync(full, top > 0 && (least >> 7) + kQuerySpread < (top >> 7));
+        if (spread) rare = kSpread;
+        float back = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 2 * G; ++k)
+        for (int g = 0; g < G; ++g) {
+          const int by = min(141 - int((spread && tops[g] > 0 ? tops[g] : top) >> 7), 126);
+          const float f = pow2(by);
+          back = pow2(-by);
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            q[k][e] = pack2<false>(__uint_as_float(q[k][e] << 16) * f, __uint_as_float(q[k][e] & 0xffff0000u) * f);
-        cq0 *= __shfl_sync(full, back, 4 * row0);
+          for (int e = 0; e < 4; ++e) {
+            uint32_t& u = q[2 * g + (e >> 1)][e & 1];
+            u = pack2<false>(__uint_as_float(u << 16) * f, __uint_as_float(u & 0xffff0000u) * f);
+          }
+          if (my_part == 0 && c4 == 0) reinterpret_cast<float*>(smem + Rg::kBack)[(my_head * 8 + r8) * G + g] = back;
+        }
+        cq0 *= __shfl_sync(full, back, 4 * row0);             // (of use where the groups share it)
         cq1 *= __shfl_sync(full, back, 4 * row1);
-        if (my_part == 0 && c4 == 0) reinterpret_cast<float*>(smem + Rg::kBack)[my_head * 8 + r8] = back;
       }
       // ... in shared memory, the head's first warp putting them there: they are read again for every tile
       if (my_part == 0) {
@@ -291,10 +310,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
       const char* const head = static_cast<const char*>(a.kv) + (h * (D / 2) + lane % CH * 16);
       const int at_word = a.Hkv * (D / 2) + (D == 128 ? h * 4 : (h * 2) & ~3);
       const int sh = D == 64 && (h & 1) ? 16 : 0;             // the head's bytes within the word
-      // What no ordinary step looks at: kGaps, this lane met a block outside the cache: from there on every step looks; kStale, m is not
-      // of the products' tokens: the next of them set it; kUneven, the rows' E differ (from there on no token is in all rows).
-      constexpr uint32_t kGaps = 1, kStale = 2, kUneven = 4;
-      uint32_t rare = 0;
       auto issue = [&](int i, int slot) {
         if (i < mine) {
           const int tok = start + i * round + lane;
@@ -399,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
         return next;
       };
       // how far E may rise before m is set anew
-      volatile uint32_t* const E_set = reinterpret_cast<uint32_t*>(smem + Rg::kBack + 8 * 32) + warp;
+      volatile uint32_t* const E_set = reinterpret_cast<uint32_t*>(smem + Rg::kWords) + warp;
       // there: the step's tokens that are there (neither past the end nor in a block outside the cache); fast: those of them
       // that every row sees and whose bytes vs fit E; restart: they set m
       auto step = [&](int i, int slot, uint32_t wk, uint32_t wv, uint32_t there, uint32_t fast, uint32_t vs, bool restart, auto edge_) {
@@ -407,16 +422,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
         const int t = start + i * round;
         const uint32_t kb = ring + slot * Rg::kStage, vb = kb + Rg::kPlane, sb = kb + 2 * Rg::kPlane;
         [[maybe_unused]] int lim0 = 0, lim1 = 0;             // the last tokens that the lane's rows see
-        [[maybe_unused]] float qs0 = 1.0f, qs1 = 1.0f;       // what undoes the queries' power of two
         if constexpr (EDGE) {
           lim0 = all + row0 / a.G;
           lim1 = all + row1 / a.G;
-          if constexpr (BF16) {
-            const float* back = reinterpret_cast<const float*>(smem + Rg::kBack) + my_head * 8;
-            qs0 = back[row0];
-            qs1 = back[row1];
-          }
         }
+        // (its address worked out here and read where it is used: kept over the loops below it spilled 128 bytes)
+        uint32_t back_at = 0;
+        if constexpr (EDGE && BF16) {
+          back_at = smem_u32(smem) + Rg::kBack + (my_head * 8 + row0) * (G * 4);
+          keep(back_at);
+        }
+        [[maybe_unused]] const volatile float* const backs = reinterpret_cast<const float*>(smem + (back_at - smem_u32(smem)));
         // ---- the lane's token: its scales into the tables
         {
           float ks[G];
@@ -512,7 +528,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
                     for (int k = 0; k < 2; ++k) x[e][pc][2 * gg + k] = as_fp16(x[e][pc][2 * gg + k], b, b);
                 }
               }
-              float c[4];
+              float c[4], qs0 = 1.0f, qs1 = 1.0f;             // (and what undoes the queries' power of two)
+              if constexpr (EDGE && BF16) {
+                qs0 = backs[2 * g2 + gg];
+                qs1 = backs[G + 2 * g2 + gg];
+              }
               const uint4 qg = gg ? q1 : q0;
 #pragma unroll
               for (int pc = 0; pc < 2; ++pc) {

@@ -186,3 +186,25 @@ def test_large_keys_beside_queries_of_zero(new, path):
         case.q = q.to(BF)
         _check(case, dev, case.run(dev, scale=0.25, path=path), 0.25)
     assert_device_clean(dev)
+
+
+@pytest.mark.parametrize("path", ["auto", "simt"])
+@pytest.mark.parametrize("new", NEW)
+def test_queries_and_keys_whose_groups_are_far_apart(new, path):
+    """Groups of 32 dims in which queries are 2^n times as large and keys 2^-n times: each has its share in the logits."""
+    dev = need_gpu()
+    lens = 300
+    for seed, shift in enumerate(([0, 40], [20, -20, 0, 10], [0, 13, 26, -14], [100, -100], [-60, 0, 60, None], [12, 0], [29, 0])):
+        d = 32 * len(shift)
+        case = _session(lens, new, d, BF, {}, 54 + seed)
+        case.put(1, 0, case.v[0].to(BF))
+        gen = torch.Generator().manual_seed(60 + seed)
+        scales = torch.tensor([125 - (n or 0) for n in shift]).expand(lens, 2, -1).clone()
+        scales += torch.randint(0, 2, scales.shape, generator=gen)
+        _keys(case, torch.randint(0, 256, (lens, d), generator=gen), scales.flatten(1))
+        size = torch.tensor([0.0 if n is None else 2.0 ** n for n in shift]).repeat_interleave(32)
+        case.q = (torch.randn(new, 4, d, generator=gen) * size).to(BF)
+        case.q[:, 1::2] *= 0.5
+        case.q[new // 2, 2] = 0
+        _check(case, dev, case.run(dev, scale=d ** -0.5, path=path), d ** -0.5)
+    assert_device_clean(dev)
