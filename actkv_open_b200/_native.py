@@ -94,6 +94,8 @@ SIGNATURES = {
 }
 # calls of many arguments as an array of 64-bit words: what ``words`` packs
 SIGNATURES["actkv_rotate_write_words"] = (I32, [ctypes.c_char_p])
+SIGNATURES["actkv_rotate_write_fits"] = (I32, [P, ctypes.c_char_p])
+SIGNATURES["actkv_append_fits"] = (P, [P, I32])
 for _name in ("actkv_quantize_write", "actkv_dequantize_read", "actkv_chunk_attention_quant"):
     SIGNATURES[_name + "_words"] = (I32, [I32, ctypes.c_char_p])
 # the 4-bit cache's entries take what the 8-bit cache's do
@@ -137,7 +139,10 @@ def load():
 
 
 class OutOfBlocks(RuntimeError):
-    """The allocator has fewer free blocks than a request needs (actkv/paged.py:19)."""
+    """The allocator has fewer free blocks than a request needs (actkv/paged.py:19).  Of a ``reserve``: ``off``, the
+    offsets it would have returned, and ``fits``, per session whether its room was made."""
+
+    off = fits = None
 
 
 def check(code: int, what: str = "") -> None:

@@ -544,6 +544,8 @@ int actkv_add_i32(int32_t* n, const int32_t* act_off, int R, void* stream) {
 
 size_t actkv_blocks_workspace_bytes(int R) { return blocks_workspace_bytes(R); }
 
+const int32_t* actkv_append_fits(void* workspace, int R) { return R > 0 ? append_ok_flags(workspace, R) : nullptr; }
+
 int actkv_append(void* kv, int L, int64_t plane_stride_bytes, int64_t slot_stride_bytes, int64_t row_bytes,
                  int64_t n_slots, const void* k_new, const void* v_new, int64_t new_layer_stride_bytes,
                  int64_t new_row_stride_bytes, const int32_t* new_off, int max_new, int32_t* seq_used,

@@ -187,6 +187,47 @@ int quant_append(int bits, const void* k_new, const void* v_new, int dtype, int6
   return done(write_rows(a, dtype, L, bits, st), "quant_append");
 }
 
+int rotate_write(const int32_t* ok, const void* q, int64_t q_stride_l, int64_t q_stride_t, int64_t q_stride_h, void* q_out,
+                 int64_t out_stride_l, int64_t out_stride_t, int64_t out_stride_h, const void* k_new,
+                 int64_t k_stride_l, int64_t k_stride_t, int64_t k_stride_h, const void* v_new, int64_t v_stride_l,
+                 int64_t v_stride_t, int64_t v_stride_h, int dtype, const int32_t* positions, const float* angles,
+                 int64_t angles_stride, int P, int rot, int pairs, const int32_t* tok_off, int T, void* cache,
+                 int bits, int64_t cache_stride_l, int64_t cache_stride_kv, int64_t cache_stride_b,
+                 int64_t cache_stride_s, int64_t cache_stride_h, const int32_t* block_table, int64_t bt_stride_r,
+                 const int32_t* seq_used, int R, int L, int MB, int NB, int BS, int Hq, int Hkv, int D,
+                 int32_t* status, void* stream) {
+  if (!dtype_ok(dtype)) return fail(ACTKV_ERR_INVALID, "unknown dtype code");
+  if (bits != 0 && bits != 8 && bits != 4) return fail(ACTKV_ERR_INVALID, "bits %d: 0 (the inputs' type), 8 or 4", bits);
+  if (L <= 0 || MB <= 0 || NB <= 0 || BS <= 0 || Hkv <= 0 || D <= 0 || R < 0 || T < 0 || Hq < 0)
+    return fail(ACTKV_ERR_INVALID, "bad sizes");
+  if (rot <= 0 || rot > D || rot % 2 != 0 || P <= 0)
+    return fail(ACTKV_ERR_INVALID, "a rotation of %d of %d dims over %d positions", rot, D, P);
+  if (bits && rot % 8 != 0) return fail(ACTKV_ERR_INVALID, "rows in %d bits need a rotated part in multiples of 8", bits);
+  if (bits)
+    if (int rc = check_row(bits, cache_stride_s, Hkv, D)) return rc;
+  if (angles_stride < rot) return fail(ACTKV_ERR_INVALID, "the angles' rows are shorter than the rotated part");
+  if (int64_t(L) * (int64_t(Hq) + 2 * int64_t(Hkv)) * D > 0x3fffffffll) return fail(ACTKV_ERR_INVALID, "too many values per token");
+  if (R == 0 || T == 0) return done(cudaSuccess, "");
+  if (!k_new || !v_new || !positions || !angles || !tok_off || !cache || !block_table || !seq_used || (Hq > 0 && (!q || !q_out)))
+    return fail(ACTKV_ERR_INVALID, "k_new, v_new, positions, angles, tok_off, the cache, block_table and seq_used are "
+                "required, and with Hq q and q_out");
+  RotateArgs a{{q, k_new, v_new}, {q_stride_l, k_stride_l, v_stride_l}, {q_stride_t, k_stride_t, v_stride_t},
+               {q_stride_h, k_stride_h, v_stride_h}, q_out, out_stride_l, out_stride_t, out_stride_h, positions, angles,
+               angles_stride, P, rot, pairs != 0, tok_off, cache, cache_stride_l, cache_stride_kv, cache_stride_b,
+               cache_stride_s, cache_stride_h, block_table, bt_stride_r, seq_used, ok, T, R, L, MB, NB, BS, Hq, Hkv,
+               D, bits, false, false, status};
+  const uint64_t es = dtype == ACTKV_F32 ? 4 : 2, cs = bits ? 1 : es;
+  uint64_t in = uint64_t(reinterpret_cast<uintptr_t>(angles)) | uint64_t(angles_stride) * 4;
+  for (int i = q ? 0 : 1; i < 3; ++i)
+    in |= uint64_t(reinterpret_cast<uintptr_t>(a.in[i])) | (uint64_t(a.in_l[i]) | uint64_t(a.in_t[i]) | uint64_t(a.in_h[i])) * es;
+  if (q)
+    in |= uint64_t(reinterpret_cast<uintptr_t>(q_out)) | (uint64_t(out_stride_l) | uint64_t(out_stride_t) | uint64_t(out_stride_h)) * es;
+  a.vec_in = in % 16 == 0;
+  a.vec_out = (uint64_t(reinterpret_cast<uintptr_t>(cache)) | (uint64_t(cache_stride_l) | uint64_t(cache_stride_kv) |
+               uint64_t(cache_stride_b) | uint64_t(cache_stride_s) | uint64_t(cache_stride_h)) * cs) % 16 == 0;
+  return done(launch_rotate_write(a, dtype, static_cast<cudaStream_t>(stream)), "rotate_write");
+}
+
 // An entry called with its arguments as 64-bit words.
 template <typename A>
 A from_word(const int64_t& w) {
@@ -208,6 +249,16 @@ template <typename... A>
 int call_words(int (*entry)(A...), const int64_t* w) {
   if (!w) return fail(ACTKV_ERR_INVALID, "the words are required");
   return call_words(entry, w, std::index_sequence_for<A...>());
+}
+
+// ... with an argument before them
+template <typename... A, size_t... I>
+int call_words(int (*entry)(const int32_t*, A...), const int32_t* first, const int64_t* w, std::index_sequence<I...>) {
+  return entry(first, from_word<A>(w[I])...);
+}
+template <typename... A>
+int call_rotate(int (*entry)(const int32_t*, A...), const int32_t* fits, const int64_t* w) {
+  return call_words(entry, fits, w, std::index_sequence_for<A...>());
 }
 
 }  // namespace
@@ -337,39 +388,18 @@ int actkv_rotate_write(const void* q, int64_t q_stride_l, int64_t q_stride_t, in
                        int64_t cache_stride_s, int64_t cache_stride_h, const int32_t* block_table, int64_t bt_stride_r,
                        const int32_t* seq_used, int R, int L, int MB, int NB, int BS, int Hq, int Hkv, int D,
                        int32_t* status, void* stream) {
-  if (!dtype_ok(dtype)) return fail(ACTKV_ERR_INVALID, "unknown dtype code");
-  if (bits != 0 && bits != 8 && bits != 4) return fail(ACTKV_ERR_INVALID, "bits %d: 0 (the inputs' type), 8 or 4", bits);
-  if (L <= 0 || MB <= 0 || NB <= 0 || BS <= 0 || Hkv <= 0 || D <= 0 || R < 0 || T < 0 || Hq < 0)
-    return fail(ACTKV_ERR_INVALID, "bad sizes");
-  if (rot <= 0 || rot > D || rot % 2 != 0 || P <= 0)
-    return fail(ACTKV_ERR_INVALID, "a rotation of %d of %d dims over %d positions", rot, D, P);
-  if (bits && rot % 8 != 0) return fail(ACTKV_ERR_INVALID, "rows in %d bits need a rotated part in multiples of 8", bits);
-  if (bits)
-    if (int rc = check_row(bits, cache_stride_s, Hkv, D)) return rc;
-  if (angles_stride < rot) return fail(ACTKV_ERR_INVALID, "the angles' rows are shorter than the rotated part");
-  if (int64_t(L) * (int64_t(Hq) + 2 * int64_t(Hkv)) * D > 0x3fffffffll) return fail(ACTKV_ERR_INVALID, "too many values per token");
-  if (R == 0 || T == 0) return done(cudaSuccess, "");
-  if (!k_new || !v_new || !positions || !angles || !tok_off || !cache || !block_table || !seq_used || (Hq > 0 && (!q || !q_out)))
-    return fail(ACTKV_ERR_INVALID, "k_new, v_new, positions, angles, tok_off, the cache, block_table and seq_used are "
-                "required, and with Hq q and q_out");
-  RotateArgs a{{q, k_new, v_new}, {q_stride_l, k_stride_l, v_stride_l}, {q_stride_t, k_stride_t, v_stride_t},
-               {q_stride_h, k_stride_h, v_stride_h}, q_out, out_stride_l, out_stride_t, out_stride_h, positions, angles,
-               angles_stride, P, rot, pairs != 0, tok_off, cache, cache_stride_l, cache_stride_kv, cache_stride_b,
-               cache_stride_s, cache_stride_h, block_table, bt_stride_r, seq_used, nullptr, T, R, L, MB, NB, BS, Hq, Hkv,
-               D, bits, false, false, status};
-  const uint64_t es = dtype == ACTKV_F32 ? 4 : 2, cs = bits ? 1 : es;
-  uint64_t in = uint64_t(reinterpret_cast<uintptr_t>(angles)) | uint64_t(angles_stride) * 4;
-  for (int i = q ? 0 : 1; i < 3; ++i)
-    in |= uint64_t(reinterpret_cast<uintptr_t>(a.in[i])) | (uint64_t(a.in_l[i]) | uint64_t(a.in_t[i]) | uint64_t(a.in_h[i])) * es;
-  if (q)
-    in |= uint64_t(reinterpret_cast<uintptr_t>(q_out)) | (uint64_t(out_stride_l) | uint64_t(out_stride_t) | uint64_t(out_stride_h)) * es;
-  a.vec_in = in % 16 == 0;
-  a.vec_out = (uint64_t(reinterpret_cast<uintptr_t>(cache)) | (uint64_t(cache_stride_l) | uint64_t(cache_stride_kv) |
-               uint64_t(cache_stride_b) | uint64_t(cache_stride_s) | uint64_t(cache_stride_h)) * cs) % 16 == 0;
-  return done(launch_rotate_write(a, dtype, static_cast<cudaStream_t>(stream)), "rotate_write");
+  return rotate_write(nullptr, q, q_stride_l, q_stride_t, q_stride_h, q_out, out_stride_l, out_stride_t,
+                      out_stride_h, k_new, k_stride_l, k_stride_t, k_stride_h, v_new, v_stride_l, v_stride_t,
+                      v_stride_h, dtype, positions, angles, angles_stride, P, rot, pairs, tok_off, T, cache, bits,
+                      cache_stride_l, cache_stride_kv, cache_stride_b, cache_stride_s, cache_stride_h, block_table,
+                      bt_stride_r, seq_used, R, L, MB, NB, BS, Hq, Hkv, D, status, stream);
 }
 
 int actkv_rotate_write_words(const int64_t* words) { return call_words(actkv_rotate_write, words); }
+int actkv_rotate_write_fits(const int32_t* fits, const int64_t* words) {
+  if (!words) return fail(ACTKV_ERR_INVALID, "the words are required");
+  return call_rotate(rotate_write, fits, words);
+}
 int actkv_quantize_write_words(int bits, const int64_t* words) {
   return call_words(bits == 4 ? actkv_quantize_write4 : actkv_quantize_write, words);
 }

@@ -388,7 +388,7 @@ struct RotateArgs {
   const int32_t* block_table;
   int64_t bt_stride_r;
   const int32_t* seq_used;
-  const int32_t* ok;         // nullable: sessions with ok[r] == 0 are left alone
+  const int32_t* ok;         // nullable: nothing of sessions with ok[r] == 0 goes into the cache
   int T, R, L, MB, NB, BS, Hq, Hkv, D;
   int bits;                  // 0: a cache of the inputs' type; 8, 4: rows
   bool vec_in, vec_out;      // 16-byte accesses allowed on q, q_out, k, v and angles / on the cache

@@ -45,7 +45,7 @@ struct Token {
 __device__ __forceinline__ Token find(const RotateArgs& a, int t, int lane, const float*& angles) {
   Token k{false, -1};
   const int r = session_of(a.tok_off, a.R, t, lane);
-  if (r >= a.R || (a.ok && !a.ok[r])) return k;
+  if (r >= a.R) return k;
   if (a.rot) {
     const int p = a.positions[t];
     if (p < 0 || p >= a.P) {
@@ -55,6 +55,7 @@ __device__ __forceinline__ Token find(const RotateArgs& a, int t, int lane, cons
     angles = a.angles + int64_t(p) * a.angles_stride;
   }
   k.live = true;
+  if (a.ok && !a.ok[r]) return k;             // no room: its queries turn, its rows go nowhere
   const int pos = a.seq_used[r] - (a.tok_off[r + 1] - t);
   const int lb = pos / a.BS;
   const int phys = pos >= 0 && lb < a.MB ? a.block_table[r * a.bt_stride_r + lb] : -1;

@@ -58,6 +58,8 @@ class DevicePagedCache:
         self.n_sessions = 0
         self._blocks_ws = None
         self._chunk_ws = None
+        self._room_ws = None
+        self._fits = None                         # per session of the last reserve, on the device: whether it fitted
         # pinned staging for the small per-call inputs of append / release (offsets, masks): reused,
         # guarded by the event of the last copy out of it
         self._stage = torch.empty(max_sessions + 1, dtype=torch.int32).pin_memory()
@@ -94,6 +96,7 @@ class DevicePagedCache:
         if protected:
             self.pinned[:R, :protected] = 1
         self.n_sessions = R
+        self._fits = None
 
     def state(self):
         """(tables, seq_lens, free) read back to the host (synchronises)."""
@@ -149,6 +152,7 @@ class DevicePagedCache:
             self.free_list.data_ptr(), self.free_top.data_ptr(), self.num_blocks, R, ws.data_ptr(), ws.numel(),
             N.status_word(dev).data_ptr(), N.stream_ptr(dev)), "append")
         self.n_sessions = max(self.n_sessions, R)
+        self._fits = None
         if check:
             bits = N.read_device_status(dev)
             if bits & N.DEV_OUT_OF_BLOCKS:
@@ -160,8 +164,9 @@ class DevicePagedCache:
         """Room for n_new[r] more tokens of session r, every layer: tables, lengths and the free stack as
         ``append`` leaves them, without any rows; returns the offsets (device int32 [R+1]) that
         ``write_rotated`` takes for the rows, layer by layer as a model makes them.  ``n_new`` as for
-        ``append``; with ``check`` false the caller reads the device status before writing any (a session that
-        did not fit has no room, and its rows would go where its last tokens are)."""
+        ``append``.  From the first session that does not fit on none has room, and ``write_rotated`` leaves their
+        rows out; with ``check`` OutOfBlocks is raised, which has the offsets (``off``: the rows of the sessions before
+        have yet to be written) and which sessions fitted (``fits``)."""
         if isinstance(n_new, torch.Tensor):
             off, R = n_new, n_new.numel() - 1
         else:
@@ -173,18 +178,25 @@ class DevicePagedCache:
                 off = self._upload(offs).clone()      # (the staging buffer is used again)
         if R > self.max_sessions:
             raise ValueError(f"{R} sessions, room for {self.max_sessions}")
-        dev, ws = self.device, self._blocks_workspace()
+        dev, lib = self.device, N.load()
+        if self._room_ws is None:                 # (its own: the flags in it stay until the next reserve)
+            self._room_ws = N.workspace(lib.actkv_blocks_workspace_bytes(self.max_sessions), dev)
+        ws = self._room_ws
         plane, slot, row, n_slots = self.flat_planes()
-        N.check(N.load().actkv_append(
+        N.check(lib.actkv_append(
             self.kv.data_ptr(), self.n_layers, plane, slot, row, n_slots, None, None, 0, 0, off.data_ptr(), 0,
             self.seq_used.data_ptr(), self.block_table.data_ptr(), self.block_table.stride(0), self.max_blocks,
             self.block_size, self.free_list.data_ptr(), self.free_top.data_ptr(), self.num_blocks, R, ws.data_ptr(),
             ws.numel(), N.status_word(dev).data_ptr(), N.stream_ptr(dev)), "reserve")
+        at = lib.actkv_append_fits(ws.data_ptr(), R) - ws.data_ptr() if R else 0
+        self._fits = ws[at:at + 4 * R].view(torch.int32)
         self.n_sessions = max(self.n_sessions, R)
         if check:
             bits = N.read_device_status(dev)
             if bits & N.DEV_OUT_OF_BLOCKS:
-                raise OutOfBlocks("reserve: the free stack (or a table row) ran out of blocks")
+                out = OutOfBlocks("reserve: the free stack (or a table row) ran out of blocks")
+                out.off, out.fits = off, [bool(x) for x in self._fits.tolist()]
+                raise out
             if bits:
                 raise RuntimeError(f"reserve: device status {bits:#x}")
         return off
@@ -195,12 +207,14 @@ class DevicePagedCache:
         """One layer's new rows into the room that ``reserve`` made, the keys rotated on the way, and the
         queries rotated (returned): q [T, Hq, D] (or None), k_new / v_new [T, Hkv, D] packed by off [R+1],
         positions int32 [T], angles as ``kernels.rotary.rotary_table`` gives them.  A session's next position is
-        not its length once it has been evicted: the caller counts them."""
+        not its length once it has been evicted: the caller counts them.  Nothing is written for sessions that the
+        last ``reserve`` of as many had no room for."""
         R = off.shape[0] - 1
+        fits = self._fits if self._fits is not None and self._fits.shape[0] == R else None
         cache, bits = self._layer_rows(layer)
         out = rotate_write(None if q is None else q[None], k_new[None], v_new[None], positions, angles, off, cache,
                            self.block_table[:R], self.seq_used[:R], q_out=None if q_out is None else q_out[None],
-                           interleaved=interleaved, bits=bits)
+                           interleaved=interleaved, bits=bits, fits=fits)
         return None if out is None else out[0]
 
     def _layer_rows(self, layer: int):
@@ -309,6 +323,7 @@ class QuantPagedCache(DevicePagedCache):
             self.num_blocks, R, L, self.max_blocks, self.num_blocks, self.block_size, H, D, ws.data_ptr(), ws.numel(),
             N.status_word(dev).data_ptr(), N.stream_ptr(dev)), "append")
         self.n_sessions = max(self.n_sessions, R)
+        self._fits = None
         if check:
             bits = N.read_device_status(dev)
             if bits & N.DEV_OUT_OF_BLOCKS:

@@ -30,7 +30,7 @@ def rotary_table(rot: int, max_positions: int, base: float = 10000.0, frequencie
 
 
 def rotate_write(q, k_new, v_new, positions, angles, tok_off, cache, block_table, seq_used, q_out=None,
-                 interleaved: bool = False, bits: int | None = None):
+                 interleaved: bool = False, bits: int | None = None, fits=None):
     """Rotate new queries and keys, and write the keys and the values into the cache, every layer in one
     launch; returns the rotated queries (None without ``q``).
 
@@ -39,7 +39,8 @@ def rotate_write(q, k_new, v_new, positions, angles, tok_off, cache, block_table
     they become the newest tok_off[r+1] - tok_off[r] of its seq_used[r] tokens, whose blocks block_table
     [R, MB] holds.  positions int32 [T]; ``angles`` fp32 [P, rot] as ``rotary_table`` gives them.  ``cache`` is
     [L, 2, NB, BS, Hkv, D] of that dtype, or with ``bits`` 8 or 4 the rows [L, 2, NB, BS, row_bytes] of such a
-    cache, quantised from the 32-bit results.  ``q_out`` may be q itself.
+    cache, quantised from the 32-bit results.  ``q_out`` may be q itself.  ``fits`` (int32 [R]): of sessions with 0
+    nothing is written into the cache (those that an allocation had no room for).
 
     A token whose position the angles do not have is left alone, one that the tables do not hold is not
     written into the cache (device status BAD_INDEX, both); so is a token of no session, unflagged.
@@ -48,8 +49,9 @@ def rotate_write(q, k_new, v_new, positions, angles, tok_off, cache, block_table
     dev = k_new.device
     if not k_new.is_cuda or v_new.device != dev or positions.device != dev or angles.device != dev or \
             tok_off.device != dev or cache.device != dev or block_table.device != dev or seq_used.device != dev or \
-            q is not None and q.device != dev or q_out is not None and q_out.device != dev:
-        N.require_cuda(k_new, v_new, q, positions, angles, tok_off, cache, block_table, seq_used, q_out)
+            q is not None and q.device != dev or q_out is not None and q_out.device != dev or \
+            fits is not None and fits.device != dev:
+        N.require_cuda(k_new, v_new, q, positions, angles, tok_off, cache, block_table, seq_used, q_out, fits)
     shape, dtype = k_new.shape, k_new.dtype
     assert len(shape) == 4 and shape == v_new.shape and dtype is v_new.dtype, "k_new / v_new are [L, T, Hkv, D] of one dtype"
     L, t_n, hkv, d = shape
@@ -100,7 +102,8 @@ def rotate_write(q, k_new, v_new, positions, angles, tok_off, cache, block_table
     assert b_1 == 1 and tok_off.is_contiguous() and seq_used.is_contiguous()
     r_n, mb = block_table.shape
     assert tok_off.shape == (r_n + 1,) and seq_used.shape == (r_n,), "tok_off [R + 1], block_table [R, MB], seq_used [R]"
-    code = N.load().actkv_rotate_write_words(_pack(
+    assert fits is None or fits.dtype is _I32 and fits.shape == (r_n,) and fits.is_contiguous(), "fits int32 [R]"
+    code = N.load().actkv_rotate_write_fits(N.ptr(fits), _pack(
         q_p, q_l, q_t, q_h, o_p, o_l, o_t, o_h, k_new.data_ptr(), k_l, k_t, k_h, v_new.data_ptr(), v_l, v_t, v_h,
         N.dtype_code(k_new), positions.data_ptr(), angles.data_ptr(), a_s, places, rot, interleaved, tok_off.data_ptr(),
         t_n, cache.data_ptr(), bits or 0, c_l, c_kv, c_b, c_s, c_h, block_table.data_ptr(), b_r, seq_used.data_ptr(),

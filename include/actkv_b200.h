@@ -324,6 +324,9 @@ ACTKV_API int actkv_add_i32(int32_t* n, const int32_t* act_off, int R, void* str
  *   max_new >= every session's new-token count (a launch-size bound, no host sync).
  */
 ACTKV_API size_t actkv_blocks_workspace_bytes(int R);
+/* Of the last actkv_append or actkv_quant_append of R sessions over this workspace: device int32 [R] in it, 1 for the sessions
+ * that fitted and 0 for the others, until the workspace is used again. */
+ACTKV_API const int32_t* actkv_append_fits(void* workspace, int R);
 ACTKV_API int actkv_append(void* kv, int L, int64_t plane_stride_bytes, int64_t slot_stride_bytes,
                            int64_t row_bytes, int64_t n_slots,
                            const void* k_new, const void* v_new, int64_t new_layer_stride_bytes,
@@ -609,6 +612,10 @@ ACTKV_API int actkv_rotate_write(const void* q, int64_t q_stride_l, int64_t q_st
  * ctypes, their array 1).  bits 4: the 4-bit cache's entries, else the 8-bit one's.
  */
 ACTKV_API int actkv_rotate_write_words(const int64_t* words);
+/* ... for rows whose room a call of actkv_append without rows (max_new 0) made: fits (device int32 [R], NULL: all did) is what
+ * actkv_append_fits gives.  The queries of a session that did not fit turn, and nothing of it goes into the cache, whose
+ * newest tokens of that session are older ones. */
+ACTKV_API int actkv_rotate_write_fits(const int32_t* fits, const int64_t* words);
 ACTKV_API int actkv_quantize_write_words(int bits, const int64_t* words);
 ACTKV_API int actkv_dequantize_read_words(int bits, const int64_t* words);
 ACTKV_API int actkv_chunk_attention_quant_words(int bits, const int64_t* words);
