@@ -286,6 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
         const int u[10] = {r, hg, j0, at, A, nt, first, t0, t1, ntok};
 #pragma unroll
         for (int i = 0; i < 10; ++i) sched.unit[i] = u[i];
+        sched.bad_v = 0;
       }
       __syncthreads();
       const uint32_t q_at = smem_u32(smem) + Rg::kQ + my_head * (G * 512) + lane * 16;
@@ -940,6 +941,24 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
       }
       if (my_part == 0) {
         const int fix = *reinterpret_cast<volatile int*>(&sched.bad_v);
+        // the head's NaN groups of token t; of the tokens that every row sees, each lane looking at every 32nd
+        auto nan_groups = [&](int t) -> uint32_t {
+          const int lb = block_of(t), ph = lb < a.MB ? table[lb] : -1;
+          uint32_t nan = 0;
+          if (ph >= 0 && ph < a.NB) {
+            const uint8_t* p = reinterpret_cast<const uint8_t*>(
+                bytes_at(a.kv_stride_kv + (int64_t(ph) * a.BS + (t - lb * a.BS)) * a.kv_stride_s)) + a.Hkv * (D / 2) + h * G;
+#pragma unroll
+            for (int g = 0; g < G; ++g) nan |= p[g] >= kNan4 ? 1u << g : 0u;
+          }
+          return nan;
+        };
+        uint32_t nan_all = 0;
+        if (fix) {
+#pragma unroll 1
+          for (int t = begin + lane; t < min(all + 1, end); t += 32) nan_all |= nan_groups(t);
+          nan_all = __reduce_or_sync(full, nan_all);
+        }
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           const int row = hf ? row1 : row0;
@@ -949,19 +968,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
           const int64_t qt = int64_t(a.q_off[r]) + j0 + jq;
           uint16_t* dst = static_cast<uint16_t*>(a.out) + qt * a.out_stride_t + int64_t(hq) * a.out_stride_h;
           float* part = ps.out(cta, ps_slot) + int64_t(hr) * D;
-          // NaN groups among the values of tokens that this row does see
-          uint32_t nan = 0;
+          uint32_t nan = nan_all;             // ... and of those that this row sees beside
           if (fix) {
-            const int last = min(all + jq, end - 1);
 #pragma unroll 1
-            for (int t = begin; t <= last; ++t) {
-              const int lb = block_of(t), ph = lb < a.MB ? table[lb] : -1;
-              if (ph < 0 || ph >= a.NB) continue;
-              const uint8_t* p = reinterpret_cast<const uint8_t*>(
-                  bytes_at(a.kv_stride_kv + (int64_t(ph) * a.BS + (t - lb * a.BS)) * a.kv_stride_s)) + a.Hkv * (D / 2) + h * G;
-#pragma unroll
-              for (int g = 0; g < G; ++g) nan |= p[g] >= kNan4 ? 1u << g : 0u;
-            }
+            for (int t = max(all + 1, begin); t <= min(all + jq, end - 1); ++t) nan |= nan_groups(t);
           }
 #pragma unroll
           for (int g = 0; g < G; ++g) {

@@ -208,3 +208,41 @@ def test_queries_and_keys_whose_groups_are_far_apart(new, path):
         case.q[new // 2, 2] = 0
         _check(case, dev, case.run(dev, scale=d ** -0.5, path=path), d ** -0.5)
     assert_device_clean(dev)
+
+
+def test_a_group_of_nan_holds_up_nobody():
+    """Two sessions of 60000 tokens in one call, a NaN group in the first: the other's results are as without it, and the call
+    takes about as long (its tokens are looked at once more at the end of the unit, 32 at a time; it took six times as long
+    where one lane looked at all, in every later unit too)."""
+    dev = need_gpu()
+    from actkv_open_b200.kernels.chunk_attn import chunk_workspace
+    from actkv_open_b200.kernels.quant_cache import paged_chunk_attention_quant, quant_row_bytes
+    hkv, d, s, r = 8, 128, 60000, 2
+    nb = r * s // 16
+    gen = torch.Generator(device=dev).manual_seed(1)
+    rows = torch.randint(0, 256, (2, nb, 16, quant_row_bytes(hkv, d, 4)), generator=gen, device=dev, dtype=torch.uint8)
+    rows[..., hkv * d // 2:] = torch.randint(124, 127, rows[..., hkv * d // 2:].shape, generator=gen, device=dev, dtype=torch.uint8)
+    table = torch.arange(nb, dtype=torch.int32, device=dev).view(r, -1)
+    seq, off = torch.full((r,), s, dtype=torch.int32, device=dev), torch.arange(r + 1, dtype=torch.int32, device=dev) * 2
+    q = torch.randn(2 * r, 32, d, generator=gen, device=dev).bfloat16()
+    ws = chunk_workspace(dev)
+
+    def timed():
+        best = math.inf
+        for _ in range(8):
+            a, b = torch.cuda.Event(True), torch.cuda.Event(True)
+            a.record()
+            got = paged_chunk_attention_quant(q, off, rows, hkv, table, seq, workspace=ws, bits=4)
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return got, best
+
+    clean, before = timed()
+    rows[1, 3, 5, hkv * d // 2 + 4 * 2 + 1] = 255          # head 2, group 1, token 53 of the first session
+    got, after = timed()
+    bad = torch.zeros(2 * r, 32, d, dtype=torch.bool, device=dev)
+    bad[:2, 8:12, 32:64] = True
+    assert torch.isnan(got[0][bad]).all() and torch.equal(got[0][~bad], clean[0][~bad]) and torch.equal(got[1], clean[1])
+    assert after < 3 * before, f"{before * 1e3:.0f} us without, {after * 1e3:.0f} us with one group of NaN"
+    assert_device_clean(dev)
