@@ -78,6 +78,13 @@ class DevicePagedCache:
         self._stage_ev.record()
         return out
 
+    def _offsets(self, off: torch.Tensor) -> torch.Tensor:
+        """Device offsets as append and reserve take them, checked: the kernels read them as they are."""
+        N.require_cuda(off, self.kv)
+        assert off.dtype is torch.int32 and off.dim() == 1 and off.numel() > 0 and off.is_contiguous(), \
+            "device offsets are int32 [R + 1]"
+        return off
+
     def set_state(self, tables: list[list[int]], seq_lens: list[int], free: list[int], protected: int = 0):
         """Load tables / lengths / free list (one host->device copy each); pins each session's
         first ``protected`` tokens."""
@@ -121,7 +128,7 @@ class DevicePagedCache:
         lib = N.load()
         dev = self.device
         if isinstance(n_new, torch.Tensor):
-            off = n_new
+            off = self._offsets(n_new)
             R = off.numel() - 1
             if max_new is None:
                 raise ValueError("max_new is required with device offsets")
@@ -168,7 +175,7 @@ class DevicePagedCache:
         rows out; with ``check`` OutOfBlocks is raised, which has the offsets (``off``: the rows of the sessions before
         have yet to be written) and which sessions fitted (``fits``)."""
         if isinstance(n_new, torch.Tensor):
-            off, R = n_new, n_new.numel() - 1
+            off, R = self._offsets(n_new), n_new.numel() - 1
         else:
             offs = [0]
             for x in n_new:
@@ -303,7 +310,7 @@ class QuantPagedCache(DevicePagedCache):
         assert k_new.dtype == v_new.dtype and k_new.stride(3) == 1 and v_new.stride(3) == 1
         N.require_cuda(k_new, v_new, self.kv)
         if isinstance(n_new, torch.Tensor):
-            off, R = n_new, n_new.numel() - 1
+            off, R = self._offsets(n_new), n_new.numel() - 1
         else:
             offs = [0]
             for x in n_new:
