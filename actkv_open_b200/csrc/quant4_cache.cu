@@ -73,8 +73,6 @@ __device__ __forceinline__ Raw<G> load_raw(const uint8_t* at, const uint8_t* sca
       r.w[g / 2] |= two << (16 * (g & 1));
       r.scales |= uint32_t(scale[g]) << (8 * g);
     }
-#pragma unroll
-    for (int k = 0; k < (G + 1) / 2; ++k) asm("" : "+r"(r.w[k]));      // (see e2m1x8_f16)
   }
   return r;
 }

@@ -77,9 +77,10 @@ __device__ __forceinline__ uint32_t e2m1x2_f16(uint32_t two) {
   const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2(__nv_fp4x2_storage_t(two), __NV_E2M1);
   return uint32_t(h.x) | uint32_t(h.y) << 16;
 }
-// The eight values of a word, byte i's in r[i], as fp16 (exact).  (For words as they were loaded: on a word put together
-// from two single bytes, upper half zero, this gave zeros with nvcc 12.9.)
+// The eight values of a word, byte i's in r[i], as fp16 (exact).  The compiler is not to look through how the word came about:
+// for one put together from two single bytes, upper half zero, nvcc 12.9 made zeros of this.
 __device__ __forceinline__ void e2m1x8_f16(uint32_t w, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+  asm("" : "+r"(w));
   asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
       "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
       "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
