@@ -416,6 +416,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_few4_kernel(const __grid_co
       };
       // how far E may rise before m is set anew
       volatile uint32_t* const E_set = reinterpret_cast<uint32_t*>(smem + Rg::kWords) + warp;
+      *E_set = kRise * 0x01010101u;           // (a unit may begin with bytes that fit E = 0)
+      __syncwarp();
       // there: the step's tokens that are there (neither past the end nor in a block outside the cache); fast: those of them
       // that every row sees and whose bytes vs fit E; restart: they set m
       auto step = [&](int i, int slot, uint32_t wk, uint32_t wv, uint32_t there, uint32_t fast, uint32_t vs, bool restart, auto edge_) {

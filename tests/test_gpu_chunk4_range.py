@@ -246,3 +246,31 @@ def test_a_group_of_nan_holds_up_nobody():
     assert torch.isnan(got[0][bad]).all() and torch.equal(got[0][~bad], clean[0][~bad]) and torch.equal(got[1], clean[1])
     assert after < 3 * before, f"{before * 1e3:.0f} us without, {after * 1e3:.0f} us with one group of NaN"
     assert_device_clean(dev)
+
+
+@pytest.mark.parametrize("new", NEW)
+def test_sessions_that_begin_with_zeros(new):
+    """The first tokens have nearly all the weight and zeros for values, after sessions of ordinary and of large ones in the
+    same call: what the others have is theirs."""
+    dev = need_gpu()
+    lens, first = 200, 64
+    for drop, shift in ((25, 0), (20, 60), (20, -60)):
+        case = _session(lens, new, 128, BF, {t: drop for t in range(first, lens)}, 95)
+        size = torch.full((lens, 1, 1), 2.0 ** shift)
+        size[:first] = 0
+        case.put(1, 0, (case.v[0] * size).to(BF))
+        alone = case.run(dev, scale=1.0)
+        _check(case, dev, alone)
+        # the same session forty times, every other one with ordinary values at its start
+        x = case.device(dev)
+        r = 40
+        rows = torch.cat([x["cache"]] * 2, 1)
+        at = C.slots(case.table, 0, 0, first, 16).to(dev)
+        rows[1].flatten(0, 1)[case.nb * 16 + at] = rows[1].flatten(0, 1)[C.slots(case.table, 0, lens - first, lens, 16).to(dev)]
+        table = torch.cat([x["table"] + case.nb, x["table"]]).repeat(r // 2, 1)
+        out, lse = case.run(dev, scale=1.0, given=dict(
+            q=case.q.to(dev).repeat(r, 1, 1), q_off=C.offsets([new] * r).to(dev), cache=rows, table=table.contiguous(),
+            seq=torch.full((r,), lens, dtype=torch.int32, device=dev)))
+        for i in range(1, r, 2):
+            _check(case, dev, (out[i * new:(i + 1) * new], lse[i * new:(i + 1) * new]))
+    assert_device_clean(dev)
