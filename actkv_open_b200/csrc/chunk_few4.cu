@@ -29,10 +29,11 @@
 // token at a time, each row with an E of its own from there on, so that a hidden value of any size changes nothing in the
 // rows that do not see it.
 //
-// What bounds it: issue and latency, 573 instructions of a warp per 32 tokens and head, a quarter of them the conversions of e2m1 (one
+// What bounds it: issue and latency, 581 instructions of a warp per 32 tokens and head, a quarter of them the conversions of e2m1 (one
 // per pair of values, at half rate), against 17 / 32 bytes per value.  Measured: 32 single tokens over 4096 to 32768 (32 query heads
-// over 8 of 128, 644 MB) 164 us, 3.9 TB/s, 0.60 of the measured copy rate (8-bit cache 280 us, 16-bit 384); one token over 2000 18.5,
-// over 32768 34; 16 sessions of 3 to 7 drafted tokens over 1000 to 9000 (4 query heads per KV head) 81 (the wide kernel: 131).
+// over 8 of 128, 644 MB) 173 us, 3.7 TB/s, 0.57 of the measured copy rate (8-bit cache 290 us, 16-bit 392); one token over 2000 20.5,
+// over 32768 36; 16 sessions of 3 to 7 drafted tokens over 1000 to 9000 (4 query heads per KV head) 85 (the wide kernel: 131).
+// (Before the window of scales 164, 18.5, 34 and 81, with other tokens' shares lost beside values 2^20 times theirs.)
 // One tile of 16 tokens at a time instead of two: 193 us for the first; queries in registers spill (185).
 #include <type_traits>
 

@@ -22,8 +22,11 @@
 //                  96 wide 122 (99); 64 wide 83 (66)
 //   4-bit rows, and read back   128 wide 229 (143), pairs 234 (143); 96 wide 215 (107); 64 wide 147 (71); unrotated, without
 //                  queries, 128 wide 100 (55)
-// Into rows it is issue that bounds: about 290 instructions of a warp per 512 values unrotated (65 % of the issue slots, 62 % of the
-// logic pipe), rotation and the 32-bit maxima on top.
+//   one KV head of 64 with 4 query heads   37 (8.5); into 4-bit rows unrotated, and back, 46 (3.4): a pass is one token's heads, so
+//                  most lanes have nothing to do
+// Into rows, unrotated: 299 instructions of a warp per 512 values, 63 % of the issue slots and of the logic pipe; the rest waits for
+// memory with 40 % of the warps.  Rotated (336 per 512, 124 registers, 22 % of the warps): 45 % of either, no resource near its end.
+// Head size 96 rotated spills 72 bytes (its partner from memory), the 16-bit rotation 32.
 // Runs of 16 passes instead of 1: the token, its session and its angles are found once (8 x 1088 x 8 layers 998 to 285 us with
 // angles in registers).
 #include "kernels.cuh"

@@ -132,7 +132,8 @@ def dequantize_read(rows, n_kv_heads, head_dim, tok_off, block_table, seq_used, 
 def paged_chunk_attention_quant(q, q_off, rows, n_kv_heads, block_table, seq_used, scale=None, out=None, lse=None,
                                 workspace=None, path: str = "auto", bits: int = 8):
     """``paged_chunk_attention`` over one layer of the 8- or 4-bit cache, rows [2, NB, BS, row_bytes]:
-    the keys and values are what ``dequantize_read`` gives in q's dtype."""
+    the keys and values are what ``dequantize_read`` gives in q's dtype, and each counts by its weight whatever its size
+    (over 4 bits, sessions of few rows take longer where value scales differ by more than 2^7 within 32 tokens)."""
     _bits(bits)
     dev, r_n, out, lse, workspace = _check(q, q_off, rows, block_table, seq_used, out, lse, workspace)
     t_n, hq, d = q.shape
